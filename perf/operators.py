@@ -266,12 +266,14 @@ def _own_append(c, s, a):
 
 def _own_attend(c, s, a):
     jv, ctx = _package()
+    ctx.ws.reset()
     jv.cachesdpa_(ctx, a["out"][0], a["q"], a["cache"], a["table"], a["lens"], a["news"], scale=s["scale"], causal=c["causal"])
     return s["out"]
 
 
 def _own_linear4(c, s, a):
     jv, ctx = _package()
+    ctx.ws.reset()
     jv.matmul4_(ctx, a["out"], a["w"], a["x"], a["bias"], epi={"none": "identity"}.get(c["epi"], c["epi"]))
     return s["out"]
 
