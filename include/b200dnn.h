@@ -42,6 +42,8 @@ enum {
 };
 
 enum { B200_F16 = 0, B200_F32 = 1 };
+/* Element types of an 8-bit cache: int8, and e4m3 (1 sign, 4 exponent, 3 mantissa bits, largest value 448). */
+enum { B200_I8 = 2, B200_E4M3 = 3 };
 /* actfn(name) (ops.jl:1684-1685): identity / relu_epi / geluexact, plus gelutanh. */
 enum { B200_EPI_NONE = 0, B200_EPI_RELU = 1, B200_EPI_GELU = 2, B200_EPI_GELU_TANH = 3 };
 
@@ -228,6 +230,76 @@ int b200_attention_f16_supported(int64_t E, int64_t Lq, int64_t Lk, int64_t H, i
  * multiples of 8, E contiguous), 2 the scalar kernel.  Every route takes the additive mask. */
 int b200_attention_f16_route(int64_t E, int64_t Lq, int64_t Lk, int64_t H, int64_t B, const int64_t* qstride,
                              const int64_t* kstride, const int64_t* vstride);
+
+/* -------------------------------------------------------------- rotary positions */
+/*
+ * (New surface, no reference counterpart: so are the 8-bit cache and the 4-bit products below.)
+ * Pair i of every head, elements (2i, 2i+1) when interleaved, else (i, i + rot/2), i < rot/2, is turned by the angle
+ * position * f_i and multiplied by gain: (u, w) -> gain * (u cos - w sin, w cos + u sin); elements rot.. of a head are
+ * passed on.  x and out are (E,L,H,B) fp16 with element strides {E,L,H,B}, E contiguous; out is x itself or apart from it.
+ * freq (device, rot/2 values): f_i in units of 2^-64 turns, modulo one turn, which makes position * f_i modulo one turn one
+ * 64-bit product, exact for every int32 position.  Token l of sequence b is at positions[l*pos_l + b*pos_b] or, with
+ * lens, at lens[b] - news[b] + l; rows l >= news[b] (L without news) are left as they were.  rot is even and at most E <= 4096.
+ */
+int b200_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t B, const b200_strided4* x,
+                    const b200_strided4* out, const uint64_t* freq, int64_t rot, int interleaved, float gain,
+                    const int32_t* positions, int64_t pos_l, int64_t pos_b, const int32_t* lens, const int32_t* news);
+
+/* ----------------------------------------------- keys and values held in 8 bits */
+/*
+ * A cache of P pages of T tokens (16, 32, 64 or 128) for H key heads of E elements (a multiple of 16 up to 128), k and v
+ * (E,T,H,P) with byte strides {1,T,H,P}, multiples of 16, on 16-byte boundaries; kmax and vmax (H,P) fp32: element q of a
+ * (page, head) stands for q * max / 127 (B200_I8) or q * max / 448 (B200_E4M3).  Token i of sequence b is row i % T of page
+ * table[i / T + b * table_ld]; a sequence has `width` entries, of which only those below its length are read.
+ * lens[b]: tokens of sequence b, the new ones included; news[b] (NULL: L): how many of the L rows of a call are new tokens,
+ * at positions lens[b] - news[b] + row.  Rows behind them are neither read nor written.  A page number outside [0, P) hides its
+ * tokens, a length outside [0, width * T] or a count outside [0, L] is cut; the next b200_sync reports either (B200_EKERNEL).
+ */
+typedef struct {
+    void *k, *v;
+    int64_t kstride[4], vstride[4];
+    float *kmax, *vmax;
+    int64_t E, T, H, P;
+    int32_t kind;
+    const int32_t* table;
+    int64_t table_ld, width;
+} b200_cache8;
+/* Writes the new tokens, k and v (E,L,H,B) fp16, E contiguous.  A page's max becomes the largest magnitude among the values
+ * written to it, or stays where it was larger and tokens before the new ones are in the page; those are rounded again when it
+ * grows.  Rounding is to nearest, ties to even, of the exact quotients.  A value that is not finite makes its page's max, for its head, a NaN.
+ * Pages that are written belong to one sequence of the call.  Rows at negative positions are skipped. */
+int b200_cache_append(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int64_t B, const b200_strided4* k,
+                      const b200_strided4* v, const int32_t* lens, const int32_t* news);
+/* Tokens starts[b] + row (starts NULL: row), row < L, of the keys (values = 0) or values (1) as numbers, rounded to out_dtype:
+ * out (E,L,H,B), E contiguous.  Rows at or past lens[b] are left as they were. */
+int b200_cache_read(b200_ctx* ctx, const b200_cache8* cache, int values, int64_t L, int64_t B, const int32_t* starts,
+                    const int32_t* lens, const b200_strided4* out, int out_dtype);
+/* out = softmax(scale * Q K') V over the cache: q and out (E,L,Hq,B), E contiguous, Hq a multiple of H; query head i reads key
+ * head i / (Hq / H).  Every query sees the keys below lens[b]; when causal, up to its own position.  A row that sees no key
+ * comes out as zeros; rows at or past news[b] are left as they were.  Scores, softmax and sums are fp32; the weights are rounded to
+ * fp16 for the second product.  Scratch comes from the context's workspace. */
+int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int64_t Hq, int64_t B, const b200_strided4* q,
+                         const b200_strided4* out, int out_dtype, float scale, int causal, const int32_t* lens,
+                         const int32_t* news);
+
+/* ------------------------------------------------------------------- 4-bit weights */
+/*
+ * A weight (M,K) of 4-bit values with a scale, and perhaps a zero point, for each `group` (32, 64 or 128) inputs of an
+ * output: w[m,k] = scales[m, k/group] * (q[m,k] - z[m, k/group]), z = 8 without zeros.  K is a multiple of group.
+ * data, scales and zeros are the library's own layout, of the sizes b200_q4_sizes gives, filled by b200_q4_pack from q
+ * (uint8, 0..15), scales (fp16) and zeros (uint8, 0..15, or NULL), each with its element strides along M and K (or groups).
+ */
+typedef struct {
+    void *data, *scales, *zeros;   /* zeros NULL: 8 everywhere */
+    int64_t M, K, group;
+} b200_q4;
+int b200_q4_sizes(int64_t M, int64_t K, int64_t group, int64_t* data_bytes, int64_t* scale_bytes, int64_t* zero_bytes);
+int b200_q4_pack(b200_ctx* ctx, const void* q, int64_t q_m, int64_t q_k, const void* scales, int64_t s_m, int64_t s_g,
+                 const void* zeros, int64_t z_m, int64_t z_g, const b200_q4* out);
+/* out(M,N) = epi(T(bias[m] + sum_k w[m,k] B(K,N)[k,n])): b200_gemm_f16 with such a weight, fp16 B and bias, fp32 accumulation,
+ * the weights taken exactly for few tokens; for many they are rounded to fp16 once into the context's workspace. */
+int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, int64_t ldb, const void* bias, void* out,
+                   int64_t ldo, int out_dtype, int epilogue);
 
 /* ------------------------------------------------------------------- layer norm */
 /*

@@ -7,6 +7,7 @@ is no fallback if the library is missing.
 """
 from ._lib import B200Error, SO_PATH, lib
 from .attention import sdpa, sdpa_, sdpaplan
+from .kvcache import Cache8, cache8, cacheappend_, cacheread_, cachesdpa_
 from .context import Ctx, DeviceArray, DeviceCaps, Workspace, caps
 from .conv import convolution_, convolutiontranspose_, convsize, convtransposesize, onebyone, shufflecase
 from .elementwise import act_, add_, clamp_, maxpool2d_, to_copy_
@@ -14,8 +15,10 @@ from .execute import Diagnostics, Model, execute_, foldgelu, foldincasts, foldou
 from .graph import Buffer, Graph, Op, evalshape, loadgraph
 from .kernelplans import AttnScalarPlan, Decline, FlashTCPlan, MMGemvPlan, MMScalarPlan, MMTilePlan, TwoGemmPlan
 from .layernorm import add_layernorm_, layernorm_, native_layer_norm
+from .linear4 import Weight4, matmul4_, pack4, quantise4
 from .matmul import batchedmatmul_, matmul_, mmplan
 from .rewrites import foldbatchnorm, foldrelu, hoistcasts, weightsource
+from .rotary import RotaryPlan, rotary_, rotaryfrequencies, rotaryplan
 from .safetensors import readsafetensors, safetensorsnames
 from .plan import Slab, alignup, checkslab, lifetimes, place, planslab
 from .shard import gather_shards, shard_range, shard_range_py
@@ -29,4 +32,6 @@ __all__ = [
     "Slab", "alignup", "checkslab", "lifetimes", "place", "planslab", "shard_range", "shard_range_py", "gather_shards",
     "maxpool2d_", "to_copy_", "MMGemvPlan", "foldoutcasts", "foldincasts", "foldbatchnorm", "foldrelu", "hoistcasts", "weightsource", "readsafetensors", "safetensorsnames",
     "Event", "StreamedPass", "Diagnostics", "TwoGemmPlan", "convolutiontranspose_", "convtransposesize", "shufflecase",
+    "Cache8", "cache8", "cacheappend_", "cacheread_", "cachesdpa_", "Weight4", "matmul4_", "pack4", "quantise4", "RotaryPlan", "rotary_",
+    "rotaryfrequencies", "rotaryplan",
 ]

@@ -17,6 +17,7 @@ HOST_PATH = os.path.join(HERE, "csrc", "hostcalls" + importlib.machinery.EXTENSI
 OK, EINVAL, ECUDA, ENOMEM, EKERNEL = 0, 1, 2, 3, 4
 DECLINE = {16: "operands", 17: "extent", 18: "wrapped", 19: "bias", 20: "eltype", 21: "tiling"}
 F16, F32 = 0, 1
+I8, E4M3 = 2, 3      # element types of an 8-bit cache
 EPI = {"identity": 0, "none": 0, None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3}
 
 
@@ -41,8 +42,20 @@ class Strided4(C.Structure):
     _fields_ = [("ptr", C.c_void_p), ("stride", C.c_int64 * 4)]
 
 
+class Cache8(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kstride", C.c_int64 * 4), ("vstride", C.c_int64 * 4), ("kmax", C.c_void_p),
+                ("vmax", C.c_void_p), ("E", C.c_int64), ("T", C.c_int64), ("H", C.c_int64), ("P", C.c_int64), ("kind", C.c_int32),
+                ("table", C.c_void_p), ("table_ld", C.c_int64), ("width", C.c_int64)]
+
+
+class Q4(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("M", C.c_int64), ("K", C.c_int64),
+                ("group", C.c_int64)]
+
+
 _i64, _i32, _vp, _f32, _sz = C.c_int64, C.c_int, C.c_void_p, C.c_float, C.c_size_t
 _pp = C.POINTER(C.c_void_p)
+_s4, _c8, _q4 = C.POINTER(Strided4), C.POINTER(Cache8), C.POINTER(Q4)
 
 # name -> (restype, argtypes); every symbol include/b200dnn.h declares.
 SIGNATURES = {
@@ -96,6 +109,13 @@ SIGNATURES = {
     "b200_attention_f16_supported": (_i32, [_i64, _i64, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64),
                                             C.POINTER(_i64), _i32]),
     "b200_attention_f16_route": (_i32, [_i64, _i64, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64)]),
+    "b200_rotary_f16": (_i32, [_vp, _i64, _i64, _i64, _i64, _s4, _s4, _vp, _i64, _i32, _f32, _vp, _i64, _i64, _vp, _vp]),
+    "b200_cache_append": (_i32, [_vp, _c8, _i64, _i64, _s4, _s4, _vp, _vp]),
+    "b200_cache_read": (_i32, [_vp, _c8, _i32, _i64, _i64, _vp, _vp, _s4, _i32]),
+    "b200_cache_attention": (_i32, [_vp, _c8, _i64, _i64, _i64, _s4, _s4, _i32, _f32, _i32, _vp, _vp]),
+    "b200_q4_sizes": (_i32, [_i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64)]),
+    "b200_q4_pack": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _q4]),
+    "b200_matmul_q4": (_i32, [_vp, _q4, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _i32]),
     "b200_layernorm": (_i32, [_vp, _i64, _i64, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _f32]),
     "b200_add_layernorm_f16": (_i32, [_vp, _i64, _i64, _vp, _vp, _i32, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _f32]),
     "b200_im2col_f16": (_i32, [_vp] + [_i64] * 14 + [_vp, _vp]),

@@ -289,6 +289,8 @@ int b200_sync(b200_ctx* c) {
         cudaMemsetAsync(c->d_status, 0, sizeof(int), c->stream);
         cudaMemsetAsync(c->sk_flags, 0, (SK_FLAG_COUNT + GEMV_COUNTER_COUNT) * sizeof(int), c->stream);
         cudaStreamSynchronize(c->stream);
+        if (st == KST_CACHE_PAGE) return fail(B200_EKERNEL, "a cache's table holds a page number outside the cache (device status %d)", st);
+        if (st == KST_CACHE_LENGTH) return fail(B200_EKERNEL, "a sequence's length or count of new tokens does not fit the call (device status %d)", st);
         return fail(B200_EKERNEL, "a kernel gave up a bounded wait (device status %d)", st);
     }
     return B200_OK;

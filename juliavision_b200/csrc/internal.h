@@ -76,6 +76,10 @@ struct b200_ctx {
     std::unordered_set<b200_graph*> graphs;                 // live graphs recorded on this context
 };
 
+// Device status of the paged cache, reported by the next synchronisation: a page number outside the cache, a length or a count of
+// new tokens that does not fit the call.  Nothing is read or written there.
+enum : int { KST_CACHE_PAGE = 120, KST_CACHE_LENGTH = 121 };
+
 constexpr int SK_FLAG_COUNT = 4096;
 constexpr int GEMV_COUNTER_COUNT = 1024;    // arrival counters of the split matrix-vector product, after the flags
 
