@@ -22,7 +22,7 @@ int cache_view(b200_ctx* ctx, const b200_cache8* c, const char* op, CacheView* o
                  "%s: %lld tokens a page (16, 32, 64 or 128)", op, (long long)c->T);
     B200_REQUIRE(c->H >= 1 && c->H < 65536 && c->P >= 1 && c->P < (1ll << 31), B200_DECLINE_EXTENT, "%s: %lld heads, %lld pages", op,
                  (long long)c->H, (long long)c->P);
-    B200_REQUIRE(c->width >= 1 && c->width * c->T < (1ll << 31) && c->table_ld >= c->width, B200_DECLINE_EXTENT,
+    B200_REQUIRE(c->width >= 1 && c->width * c->T <= (1ll << 30) && c->table_ld >= c->width, B200_DECLINE_EXTENT,
                  "%s: a table of %lld pages a sequence, leading dimension %lld", op, (long long)c->width, (long long)c->table_ld);
     B200_REQUIRE(c->k && c->v && c->kmax && c->vmax && c->table, B200_EINVAL, "%s: null array", op);
     uint64_t odd = (uintptr_t)c->k | (uintptr_t)c->v;

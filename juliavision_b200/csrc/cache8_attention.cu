@@ -8,6 +8,10 @@
 // onto P, relative to the largest one so far, whose change is one more factor of the running rescale.  P is rounded to fp16
 // times 2^12, so that weights down to 2^-26 of the row's largest keep all their bits.
 //
+// Each warp streams keys of its own, 32 at a time, through a ring that its first lane fills with TMA: nothing but the end of a
+// piece of work brings a block's warps together, and what a copy costs is one lane's few instructions (64-key tiles shared by
+// the block and copied 16 bytes a thread spent a third of the instructions on addresses: 32 x 8192 tokens 128 us).
+//
 // The work is one list of key tiles over all (sequence, key head, row tile), computed from the lengths on the device and dealt
 // out in equal shares, so ragged lengths and few sequences fill the GPU alike.  A share's first and last pieces may be parts
 // of a list entry; their rows meet in the workspace and the last block to arrive joins them, in block order.
@@ -19,10 +23,9 @@ namespace b200 {
 
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
-constexpr int CF_TILE = 64;               // keys of a tile, 16 a warp
-constexpr int CF_STAGES = 4;
-constexpr int CF_SHARE = 2;               // tiles of a share at least
-constexpr int CF_SCALES = 2 * CF_TILE / 16;   // scales of a tile: key and value scale of each 16 keys
+constexpr int CF_KEYS = 32;                      // keys of a warp's stage
+constexpr int CF_TILE = CF_WARPS * CF_KEYS;      // keys of a tile
+constexpr int CF_SHARE = 1;                      // tiles of a share at least
 
 struct CacheAttnParams {
     CacheView c;
@@ -38,29 +41,31 @@ struct CacheAttnParams {
 };
 
 template <int EP> struct CfCfg {
-    static constexpr int SIDE = CF_TILE * EP;                 // bytes of a tile's keys, or values
+    static constexpr int STAGES = EP == 128 ? 2 : 3;          // of each warp's own ring
+    static constexpr int SIDE = CF_KEYS * EP;                 // bytes of a stage's keys, or values
     static constexpr int STAGE = 2 * SIDE;
-    static constexpr int RING = CF_STAGES * STAGE;
+    static constexpr int RING = CF_WARPS * STAGES * STAGE;
     static constexpr int ROW = EP + 4;                        // floats: the row, its reference point, its sum
-    static constexpr int SMEM = RING + CF_STAGES * CF_SCALES * 4;
+    static constexpr int CTAS = EP == 128 ? 3 : 4;            // per SM
+    static constexpr int SMEM = RING + 1024;                  // the swizzle wants the ring on a 1024-byte boundary
     static_assert(CF_WARPS * 16 * ROW * 4 <= RING, "the warps' rows fit over the ring");
 };
 
-// Where 16-byte chunk c of row r of a tile lies, so that the eight lanes of a shared-memory phase meet all banks both when they
-// read rows (keys: two rows' four chunks) and when they read columns (values: rows 2 t + i).
+// Byte of 16-byte chunk c of row r of a stage's side, as the tensor map's swizzle lays it: 128-byte rows with the chunk turned
+// by r % 8, or two 64-byte rows a line with the chunk turned by r / 2 % 4.
 template <int EP> __device__ __forceinline__ int cf_place(int r, int c) {
-    if constexpr (EP == 128) return r * 128 + ((c ^ ((r & 1) << 2) ^ (((r >> 1) & 3) << 1)) << 4);
-    else return (r >> 1) * 128 + ((((r ^ r >> 2) & 1) << 2 | (c ^ (r & 2))) << 4);
+    if constexpr (EP == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+    else return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
-// The row of a 16-key group that a key tile's column g (tile 0 or 1) stands for.  At EP = 64 a lane's four values lie in rows t,
-// t + 4, t + 8, t + 12, at EP = 128 in rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9: both free of bank conflicts under cf_place.
+// The row of a 16-key group that column g of its key tile (0 or 1) stands for, and the chunk of a row that column g of the value
+// tiles stands for; both free, and chosen so that the eight (or sixteen) lanes of a shared-memory phase meet all banks: keys read
+// the same four chunks of two rows, values one or two chunks of four rows.
 template <int EP> __device__ __forceinline__ int cf_key(int tile, int g) {
-    return EP == 128 ? tile * 8 + g : tile * 8 + (g >> 1) + (g & 1) * 4;
+    if constexpr (EP == 128) return tile * 8 + (g >> 1) + (g & 1) * 4;   // two rows that differ in bit 2
+    else return tile * 8 + (g ^ ((g >> 1) & 1));                         // rows 0 1 3 2 4 5 7 6: an odd one to every even one
 }
+__device__ __forceinline__ int cf_chunk(int g) { return (g >> 1) | (g & 1) << 2; }   // EP = 128
 
-__device__ __forceinline__ void cf_copy16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cf_copy4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -83,18 +88,35 @@ template <bool FP8> __device__ __forceinline__ void cf_values(uint32_t a, uint32
     }
 }
 
+__device__ __forceinline__ float cf_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <int EP, bool FP8>
-__global__ void __launch_bounds__(CF_THREADS, EP == 64 ? 4 : 3)
-cache_attention_kernel(const CacheAttnParams p) {
+__global__ void __launch_bounds__(CF_THREADS, CfCfg<EP>::CTAS)
+cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_constant__ CUtensorMap tmapV, const CacheAttnParams p) {
     using Cfg = CfCfg<EP>;
-    constexpr int CH = EP / 16, W = EP / 8, ROW = Cfg::ROW, HH = EP / 64;
-    extern __shared__ __align__(128) uint8_t cf_smem[];
-    float* scales = reinterpret_cast<float*>(cf_smem + Cfg::RING);
-    __shared__ long long start_s;
-    __shared__ int where_s, last_s;
-    __shared__ long long sums_s[CF_WARPS];
+    constexpr int W = EP / 8, ROW = Cfg::ROW, HH = EP / 64, STAGES = Cfg::STAGES;
+    extern __shared__ uint8_t cf_raw[];
+    __shared__ __align__(8) uint64_t full_s[CF_WARPS][STAGES];
+    __shared__ __align__(16) float scales_s[CF_WARPS][STAGES][4];   // key and value scale of each 16 keys
+    __shared__ long long start_s, sums_s[CF_WARPS];
+    __shared__ int where_s, last_s, abort_s;
+    uint8_t* cf_smem = cf_raw + ((1024 - (smem_u32(cf_raw) & 1023)) & 1023);
     const CacheView& c = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(&full_s[warp][i], 1);
+        fence_barrier_init();
+    }
+    if (tid == 0) {
+        abort_s = 0;
+        prefetch_tmap(&tmapK);
+        prefetch_tmap(&tmapV);
+    }
+    __syncthreads();
     grid_dep_wait();
     grid_dep_launch();
 
@@ -154,6 +176,7 @@ cache_attention_kernel(const CacheAttnParams p) {
     long long bstart = start_s;
 
     // ---- its pieces
+    uint32_t fill = 0, use = 0;   // stages this warp has asked for, and has waited for
     for (long long at = from; at < to;) {
         int n, m, tiles;
         long long size = entry(b, n, m, tiles);
@@ -185,34 +208,56 @@ cache_attention_kernel(const CacheAttnParams p) {
                 last1 = p.causal ? n - m + l : n - 1;
             }
         }
-        auto fetch = [&](int j) {   // tile j0 + j into its stage; a commit group even when there is none
-            if (j0 + j < j1) {
-                const int st = j % CF_STAGES, key0 = (j0 + j) * CF_TILE;
-                const uint32_t ring = smem_u32(cf_smem) + st * Cfg::STAGE;
-#pragma unroll
-                for (int i = 0; i < CF_TILE * CH / CF_THREADS; ++i) {
-                    const int idx = tid + i * CF_THREADS, row = idx / CH, ch = idx % CH, key = key0 + row;
-                    const int64_t page = key < n ? c.page(b, key >> c.logT) : -1;
-                    const bool live = page >= 0 && ch * 16 < c.E;
+        // This warp's keys of tile j: 32 j' on, j' = 4 (j0 + j) + warp; its page or pages, looked up a tile ahead of the copies.
+        int64_t page0 = -1, page1 = -1;
+        auto look = [&](int j) {
+            const int key = (j0 + j) * CF_TILE + warp * CF_KEYS;
+            page0 = page1 = -1;
+            if (j0 + j < j1 && key < n) {
+                page0 = c.page(b, key >> c.logT);
+                page1 = key + 16 >= n ? -1 : c.T == 16 ? c.page(b, (key >> 4) + 1) : page0;
+            }
+        };
+        auto fetch = [&](int j) {   // a commit group even when there is none
+            const int key = (j0 + j) * CF_TILE + warp * CF_KEYS;
+            if (j0 + j < j1 && key < n) {
+                const int st = fill % STAGES;
+                if (lane < 4) {   // a group without a page gets a key scale below any magnitude
+                    const int64_t page = lane < 2 ? page0 : page1;
+                    float* dst = &scales_s[warp][st][lane];
+                    if (page >= 0) cf_copy4(smem_u32(dst), ((lane & 1) ? c.vmax : c.kmax) + page * c.H + h);
+                    else *dst = (lane & 1) ? 0.f : -1.f;
+                }
+                if (lane == 0) {
+                    uint8_t* dst = cf_smem + (warp * STAGES + st) * Cfg::STAGE;
                     const int in = key & (c.T - 1);
-                    const uint8_t* k = live ? c.k + page * c.kP + h * c.kH + in * c.kT + ch * 16 : c.k;
-                    const uint8_t* v = live ? c.v + page * c.vP + h * c.vH + in * c.vT + ch * 16 : c.v;
-                    const uint32_t dst = ring + cf_place<EP>(row, ch);
-                    cf_copy16(dst, k, live);
-                    cf_copy16(dst + Cfg::SIDE, v, live);
+                    if (c.T == 16) {
+                        mbar_arrive_expect_tx(&full_s[warp][st], (uint32_t)((page0 >= 0) + (page1 >= 0)) * Cfg::SIDE);
+                        if (page0 >= 0) {
+                            tma_load_4d(dst, &tmapK, &full_s[warp][st], 0, 0, h, (int)page0);
+                            tma_load_4d(dst + Cfg::SIDE, &tmapV, &full_s[warp][st], 0, 0, h, (int)page0);
+                        }
+                        if (page1 >= 0) {
+                            tma_load_4d(dst + Cfg::SIDE / 2, &tmapK, &full_s[warp][st], 0, 0, h, (int)page1);
+                            tma_load_4d(dst + Cfg::SIDE + Cfg::SIDE / 2, &tmapV, &full_s[warp][st], 0, 0, h, (int)page1);
+                        }
+                    } else {
+                        mbar_arrive_expect_tx(&full_s[warp][st], page0 >= 0 ? Cfg::STAGE : 0);
+                        if (page0 >= 0) {
+                            tma_load_4d(dst, &tmapK, &full_s[warp][st], 0, in, h, (int)page0);
+                            tma_load_4d(dst + Cfg::SIDE, &tmapV, &full_s[warp][st], 0, in, h, (int)page0);
+                        }
+                    }
                 }
-                if (tid < CF_SCALES) {   // a group without a page gets a key scale below any magnitude
-                    const int key = key0 + (tid >> 1) * 16, side = tid & 1;
-                    const int64_t page = key < n ? c.page(b, key >> c.logT) : -1;
-                    float* dst = scales + st * CF_SCALES + tid;
-                    if (page >= 0) cf_copy4(smem_u32(dst), (side ? c.vmax : c.kmax) + page * c.H + h);
-                    else *dst = side ? 0.f : -1.f;
-                }
+                ++fill;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int j = 0; j < CF_STAGES - 1; ++j) fetch(j);
+        for (int j = 0; j < STAGES; ++j) {
+            look(j);
+            fetch(j);
+        }
 
         // Q: lane (g, t) holds, for keys' elements 64 hh + 16 t + 4 s + (0 .. 3) of step (hh, s), rows g and g + 8
         uint32_t qa[HH * 4][4];
@@ -242,24 +287,29 @@ cache_attention_kernel(const CacheAttnParams p) {
         float o[W][4];
 #pragma unroll
         for (int i = 0; i < W; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, vref = 0.f;   // vref: the value scale P is relative to
+        float m0 = -INFINITY, m1 = -INFINITY, vref = 0.f;   // vref: the value scale P is relative to
+        uint64_t l0p = 0, l1p = 0;                          // sums of rows g and g + 8, in pairs
+        const int all_see = p.causal ? n - m + rt * 16 / p.G : n - 1;   // the last key that every row may see
 
         for (int j = 0; j0 + j < j1; ++j) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(CF_STAGES - 2) : "memory");
-            __syncthreads();   // tile j has landed for everyone, and tile j - 1 has been read by everyone
-            fetch(j + CF_STAGES - 1);
-            const int st = j % CF_STAGES, key0 = (j0 + j) * CF_TILE + warp * 16;
-            const uint8_t* K = cf_smem + st * Cfg::STAGE;
+            const int key0 = (j0 + j) * CF_TILE + warp * CF_KEYS;
+            if (key0 >= n) break;   // uniform over the warp, and so is every later tile
+            look(j + STAGES);
+            const int st = use % STAGES;
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            if (!mbar_wait(&full_s[warp][st], (use / STAGES) & 1, c.d_status, KST_WAIT_FULL, &abort_s)) break;
+            __syncwarp();
+            ++use;
+            const uint8_t* K = cf_smem + (warp * STAGES + st) * Cfg::STAGE;
             const uint8_t* V = K + Cfg::SIDE;
-            const float ks = scales[st * CF_SCALES + 2 * warp], vs = scales[st * CF_SCALES + 2 * warp + 1];
-            if (key0 >= n || ks < 0.f) continue;   // nothing of this warp's group (uniform over the warp)
-            float s[2][4];
+            const float4 sc = *reinterpret_cast<const float4*>(scales_s[warp][st]);   // key, value scale of group 0, of group 1
+            float s[4][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
                 for (int hh = 0; hh < HH; ++hh) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(K + cf_place<EP>(warp * 16 + cf_key<EP>(i, g), hh * 4 + t));
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(K + cf_place<EP>((i >> 1) * 16 + cf_key<EP>(i & 1, g), hh * 4 + t));
                     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -269,17 +319,30 @@ cache_attention_kernel(const CacheAttnParams p) {
                     }
                 }
             }
-            const float ksl = ks * p.scale_log2;
-            float x0 = -INFINITY, x1 = -INFINITY;
+            uint64_t s0[4], s1[4];   // scaled, in pairs, of rows g and g + 8
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 4; ++i) {
+                const float ksl = (i < 2 ? sc.x : sc.z) * p.scale_log2;
+                s0[i] = mul2(pack2(s[i][0], s[i][1]), pack2(ksl, ksl));
+                s1[i] = mul2(pack2(s[i][2], s[i][3]), pack2(ksl, ksl));
+                unpack2(s0[i], s[i][0], s[i][1]);
+                unpack2(s1[i], s[i][2], s[i][3]);
+            }
+            if (key0 + CF_KEYS - 1 > all_see || sc.x < 0.f || sc.z < 0.f) {   // someone does not see all of these
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int key = key0 + cf_key<EP>(i, 2 * t + (k & 1));
-                    s[i][k] = key <= (k < 2 ? last0 : last1) ? s[i][k] * ksl : -INFINITY;
-                    if (k < 2) x0 = fmaxf(x0, s[i][k]);
-                    else x1 = fmaxf(x1, s[i][k]);
+                for (int i = 0; i < 4; ++i) {
+                    const bool hidden = (i < 2 ? sc.x : sc.z) < 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int key = key0 + (i >> 1) * 16 + cf_key<EP>(i & 1, 2 * t + (k & 1));
+                        if (hidden || key > (k < 2 ? last0 : last1)) s[i][k] = -INFINITY;
+                    }
+                    s0[i] = pack2(s[i][0], s[i][1]);
+                    s1[i] = pack2(s[i][2], s[i][3]);
                 }
+            }
+            float x0 = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
+            float x1 = fmaxf(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])), fmaxf(fmaxf(s[2][2], s[2][3]), fmaxf(s[3][2], s[3][3])));
 #pragma unroll
             for (int d = 1; d < 4; d *= 2) {   // a quad of lanes shares a row
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
@@ -287,14 +350,15 @@ cache_attention_kernel(const CacheAttnParams p) {
             }
             x0 = fmaxf(m0, x0);
             x1 = fmaxf(m1, x1);
-            float vnew = vref;
-            if (vs < INFINITY && vs > vref) vnew = vs;            // one that is not finite is nobody's reference
+            float vnew = vref;                                     // a scale that is not finite is nobody's reference
+            if (sc.y < INFINITY && sc.y > vnew) vnew = sc.y;
+            if (sc.w < INFINITY && sc.w > vnew) vnew = sc.w;
             if (__any_sync(0xffffffffu, x0 != m0 || x1 != m1 || vnew != vref)) {
                 // a row that has seen nothing but hidden keys keeps the reference point -inf and contributes zeros
-                const float a0 = m0 == x0 ? 1.f : exp2f(m0 - x0), a1 = m1 == x1 ? 1.f : exp2f(m1 - x1);
+                const float a0 = m0 == x0 ? 1.f : cf_ex2(m0 - x0), a1 = m1 == x1 ? 1.f : cf_ex2(m1 - x1);
                 const float f = vnew == vref ? 1.f : vref / vnew;
-                l0 *= a0;
-                l1 *= a1;
+                l0p = mul2(l0p, pack2(a0, a0));
+                l1p = mul2(l1p, pack2(a1, a1));
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
                     o[i][0] *= a0 * f;
@@ -304,53 +368,67 @@ cache_attention_kernel(const CacheAttnParams p) {
                 }
                 m0 = x0, m1 = x1, vref = vnew;
             }
-            const float n0 = m0 == -INFINITY ? 0.f : m0, n1 = m1 == -INFINITY ? 0.f : m1;
-            const float f = (vs == vref ? 1.f : vs / vref) * 4096.f;   // both 0 while there are only pages of zeros
-            uint32_t pa[4];
-            float e[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    e[i][k] = exp2f(s[i][k] - (k < 2 ? n0 : n1));
-                    if (k < 2) l0 += e[i][k];
-                    else l1 += e[i][k];
-                    e[i][k] = s[i][k] == -INFINITY ? 0.f : e[i][k] * f;
-                }
-            pa[0] = cf_pack(e[0][0], e[0][1]);
-            pa[1] = cf_pack(e[0][2], e[0][3]);
-            pa[2] = cf_pack(e[1][0], e[1][1]);
-            pa[3] = cf_pack(e[1][2], e[1][3]);
-            // V: lane (g, t) holds four tokens' elements W g ... W g + W - 1, in the order of P's columns
-            const int row0 = warp * 16;
-            uint32_t w[4][W / 4];
+            const float n0 = m0 == -INFINITY ? 0.f : -m0, n1 = m1 == -INFINITY ? 0.f : -m1;
+            uint32_t pa[2][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint8_t* at = V + cf_place<EP>(row0 + cf_key<EP>(i >> 1, 2 * t + (i & 1)), g * W >> 4) + (g * W & 15);
-                if constexpr (W == 16) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(at);
-                    w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
-                } else {
-                    const uint2 v = *reinterpret_cast<const uint2*>(at);
-                    w[i][0] = v.x, w[i][1] = v.y;
+                const float vs = i < 2 ? sc.y : sc.w, f = (vs == vref ? 1.f : vs / vref) * 4096.f;   // both 0 while there are only pages of zeros
+                float e0, e1, e2, e3;
+                unpack2(add2(s0[i], pack2(n0, n0)), e0, e1);
+                unpack2(add2(s1[i], pack2(n1, n1)), e2, e3);
+                e0 = cf_ex2(e0), e1 = cf_ex2(e1), e2 = cf_ex2(e2), e3 = cf_ex2(e3);
+                l0p = add2(l0p, pack2(e0, e1));
+                l1p = add2(l1p, pack2(e2, e3));
+                unpack2(mul2(pack2(e0, e1), pack2(f, f)), e0, e1);
+                unpack2(mul2(pack2(e2, e3), pack2(f, f)), e2, e3);
+                if (!(vs < INFINITY)) {   // 0 times it is no number: a hidden key has no part
+                    if (s[i][0] == -INFINITY) e0 = 0.f;
+                    if (s[i][1] == -INFINITY) e1 = 0.f;
+                    if (s[i][2] == -INFINITY) e2 = 0.f;
+                    if (s[i][3] == -INFINITY) e3 = 0.f;
+                }
+                pa[i >> 1][(i & 1) * 2] = cf_pack(e0, e1);
+                pa[i >> 1][(i & 1) * 2 + 1] = cf_pack(e2, e3);
+            }
+            // V: lane (g, t) holds four tokens' W elements of column g, in the order of P's columns
+#pragma unroll
+            for (int grp = 0; grp < 2; ++grp) {
+                uint32_t w[4][W / 4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = grp * 16 + cf_key<EP>(i >> 1, 2 * t + (i & 1));
+                    if constexpr (W == 16) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(V + cf_place<EP>(row, cf_chunk(g)));
+                        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(V + cf_place<EP>(row, g >> 1) + (g & 1) * 8);
+                        w[i][0] = v.x, w[i][1] = v.y;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < W / 4; ++u) {
+                    uint32_t b0[4], b1[4];
+                    cf_values<FP8>(w[0][u], w[1][u], b0);
+                    cf_values<FP8>(w[2][u], w[3][u], b1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mma_16816(o[u * 4 + i], pa[grp], b0[i], b1[i]);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < W / 4; ++u) {
-                uint32_t b0[4], b1[4];
-                cf_values<FP8>(w[0][u], w[1][u], b0);
-                cf_values<FP8>(w[2][u], w[3][u], b1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mma_16816(o[u * 4 + i], pa, b0[i], b1[i]);
-            }
+            __syncwarp();   // the stage has been read
+            fetch(j + STAGES);
         }
+        float l0, l1, l0b, l1b;
+        unpack2(l0p, l0, l0b);
+        unpack2(l1p, l1, l1b);
+        l0 += l0b;
+        l1 += l1b;
 #pragma unroll
         for (int d = 1; d < 4; d *= 2) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, d);
             l1 += __shfl_xor_sync(0xffffffffu, l1, d);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();   // the ring is free
+        __syncthreads();   // the ring is free: every copy that was asked for has been waited for
         // this warp's rows: [row][EP values, reference point, sum]
         float* mine = reinterpret_cast<float*>(cf_smem) + warp * 16 * ROW;
         const float back = vref * (1.f / 4096.f) / cache_top<FP8>();
@@ -360,7 +438,7 @@ cache_attention_kernel(const CacheAttnParams p) {
             for (int col = 0; col < 2; ++col)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                    *reinterpret_cast<float4*>(mine + (g + 8 * r) * ROW + W * (2 * t + col) + i) =
+                    *reinterpret_cast<float4*>(mine + (g + 8 * r) * ROW + (EP == 128 ? 64 * col + 16 * t : 16 * t + 8 * col) + i) =
                         make_float4(o[i][2 * r + col] * back, o[i + 1][2 * r + col] * back, o[i + 2][2 * r + col] * back, o[i + 3][2 * r + col] * back);
         if (t == 0) {
             *reinterpret_cast<float2*>(mine + g * ROW + EP) = make_float2(m0, l0);
@@ -391,7 +469,7 @@ cache_attention_kernel(const CacheAttnParams p) {
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < CF_WARPS; ++w) {
-                const float mw = src[w * 16 * ROW + EP], f = mw == M ? 1.f : exp2f(mw - M);   // 1: both may be -inf, with zeros or a NaN
+                const float mw = src[w * 16 * ROW + EP], f = mw == M ? 1.f : cf_ex2(mw - M);   // 1: both may be -inf, with zeros or a NaN
                 const float4 x = *reinterpret_cast<const float4*>(src + w * 16 * ROW + e4);
                 v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
                 l = fmaf(src[w * 16 * ROW + EP + 1], f, l);
@@ -420,7 +498,7 @@ cache_attention_kernel(const CacheAttnParams p) {
                         const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + EP));
                         const float4 x = __ldcg(reinterpret_cast<const float4*>(src + e4));
                         const float top = fmaxf(M, ml.x);
-                        const float a = M == top ? 1.f : exp2f(M - top), f = ml.x == top ? 1.f : exp2f(ml.x - top);
+                        const float a = M == top ? 1.f : cf_ex2(M - top), f = ml.x == top ? 1.f : cf_ex2(ml.x - top);
                         v.x = v.x * a + x.x * f, v.y = v.y * a + x.y * f, v.z = v.z * a + x.z * f, v.w = v.w * a + x.w * f;
                         l = l * a + ml.y * f;
                         M = top;
@@ -431,28 +509,42 @@ cache_attention_kernel(const CacheAttnParams p) {
                 if (tid == 0) p.arrived[first] = 0;
             }
         }
+        fence_proxy_async_smem();
         __syncthreads();   // the ring may be filled again
         at = pstart + j1;
     }
+}
+
+// A tensor map over one side of the cache, boxes of `rows` tokens of a page and head.
+static int cf_map(b200_ctx* ctx, CUtensorMap* m, const void* base, const CacheView& c, int64_t sT, int64_t sH, int64_t sP, int EP, int rows) {
+    const uint64_t dims[4] = {(uint64_t)c.E, (uint64_t)c.T, (uint64_t)c.H, (uint64_t)c.P};
+    const uint64_t strides[3] = {(uint64_t)sT, (uint64_t)sH, (uint64_t)sP};
+    const uint32_t box[4] = {(uint32_t)EP, (uint32_t)rows, 1, 1};
+    return make_tmap(ctx, m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, EP == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 template <int EP, bool FP8>
 static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     using Cfg = CfCfg<EP>;
     auto kern = cache_attention_kernel<EP, FP8>;
+    CUtensorMap mk, mv;
+    const int rows = p.c.T < CF_KEYS ? p.c.T : CF_KEYS;
+    int rc = cf_map(ctx, &mk, p.c.k, p.c, p.c.kT, p.c.kH, p.c.kP, EP, rows);
+    if (!rc) rc = cf_map(ctx, &mv, p.c.v, p.c, p.c.vT, p.c.vH, p.c.vP, EP, rows);
+    if (rc) return rc;
     B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     // One resident wave at most, and no more blocks than there can be shares.
-    int64_t grid = (int64_t)ctx->prop.multiProcessorCount * (EP == 64 ? 4 : 3);
+    int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
     if (grid > GEMV_COUNTER_COUNT) grid = GEMV_COUNTER_COUNT;
     const int64_t tiles = cdiv((int64_t)p.c.width * p.c.T, CF_TILE), rts = cdiv((int64_t)p.L * p.G, 16);
     const double most = (double)tiles * rts * p.c.H * p.B / CF_SHARE;
     if (most + 1 < (double)grid) grid = (int64_t)most + 1;
     void* ws = nullptr;
-    int rc = ws_scratch(ctx, (size_t)grid * 2 * 16 * Cfg::ROW * sizeof(float), &ws);
+    rc = ws_scratch(ctx, (size_t)grid * 2 * 16 * Cfg::ROW * sizeof(float), &ws);
     if (rc) return rc;
     p.part = static_cast<float*>(ws);
     p.arrived = ctx->sk_flags + SK_FLAG_COUNT;
-    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(CF_THREADS), Cfg::SMEM, ctx->stream, 1, p));
+    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(CF_THREADS), Cfg::SMEM, ctx->stream, 1, mk, mv, p));
     ctx->launches++;
     return B200_OK;
 }
