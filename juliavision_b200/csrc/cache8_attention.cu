@@ -2,15 +2,19 @@
 //     out = softmax(scale Q K^T, keys below the sequence's length and, when causal, up to the query's own position) V
 //
 // Bandwidth-bound: the cache is read once, E + 4 / T bytes a key, head and side, against 4 E flops a query head and key.  The
-// query rows of a key head (the heads that share it, times the new tokens) are stacked, 16 to a tile, so the cache is read
-// once for all of them; the products are warp-level m16n8k16 tiles whose 8-bit operands become fp16 in registers, exactly.
-// A page's scales never touch the operands: the key scale multiplies the fp32 scores of its page, the value scale goes
-// onto P, relative to the largest one so far, whose change is one more factor of the running rescale.  P is rounded to fp16
-// times 2^12, so that weights down to 2^-26 of the row's largest keep all their bits.
+// query rows of a key head (the heads that share it, times the new tokens) are stacked, 8 or 16 to a tile, so the cache is read
+// once for all of them.  What the SMs are short of is instructions, most of them spent on making 8-bit operands into fp16
+// (exactly); so both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, as warp-level m16n8k16 tiles whose 16 rows
+// are keys, then elements, and whose 8 columns are query rows: every converted register pair serves a full tile, where tiles
+// of 16 query rows would be half empty for a group of four or eight heads.  P^T reaches its operand layout by movmatrix.
 //
-// Each warp streams keys of its own, 32 at a time, through a ring that its first lane fills with TMA: nothing but the end of a
-// piece of work brings a block's warps together, and what a copy costs is one lane's few instructions (64-key tiles shared by
-// the block and copied 16 bytes a thread spent a third of the instructions on addresses: 32 x 8192 tokens 128 us).
+// A page's scales never touch the operands: the key scale multiplies the fp32 scores of its page, the value scale goes onto P,
+// relative to the largest one so far, whose change is one more factor of the running rescale.  That rescale waits until a
+// score is 2^8 past its row's reference point; P is rounded to fp16 times 2^7, so that it stays in range and weights down to
+// 2^-21 of the reference keep all their bits.
+//
+// Each warp streams keys of its own, 64 at a time, which its first lanes fetch by TMA: nothing but the end of a piece of work
+// brings a block's warps together, and what a copy costs is a few instructions.
 //
 // The work is one list of key tiles over all (sequence, key head, row tile), computed from the lengths on the device and dealt
 // out in equal shares, so ragged lengths and few sequences fill the GPU alike.  A share's first and last pieces may be parts
@@ -23,7 +27,8 @@ namespace b200 {
 
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
-constexpr int CF_KEYS = 32;                      // keys of a warp's stage
+constexpr int CF_KEYS = 64;                      // keys a warp takes at a time
+constexpr int CF_GROUPS = CF_KEYS / 16;          // of one page each
 constexpr int CF_TILE = CF_WARPS * CF_KEYS;      // keys of a tile
 constexpr int CF_SHARE = 1;                      // tiles of a share at least
 
@@ -34,21 +39,21 @@ struct CacheAttnParams {
     int64_t qL, qH, qB, oL, oH, oB;
     const int32_t *lens, *news;
     int L, B, G;                          // rows at most, sequences, query heads a key head
-    int causal, out_f32, whole;           // whole: rows of q start on 16-byte boundaries
+    int causal, out_f32, whole, out_whole;   // rows of q start on 16-byte boundaries, fours of out on their own size
     float scale_log2;
-    float* part;                          // [block][first or last][16 rows][EP + 4]
+    float* part;                          // [block][first or last][row][EP + 4]
     int* arrived;
 };
 
-template <int EP> struct CfCfg {
-    static constexpr int STAGES = EP == 128 ? 2 : 3;          // of each warp's own ring
-    static constexpr int SIDE = CF_KEYS * EP;                 // bytes of a stage's keys, or values
+template <int EP, int NT> struct CfCfg {
+    static constexpr int SIDE = CF_KEYS * EP;                 // bytes of a warp's keys, or values
     static constexpr int STAGE = 2 * SIDE;
-    static constexpr int RING = CF_WARPS * STAGES * STAGE;
+    static constexpr int RING = CF_WARPS * STAGE;
+    static constexpr int RT = 8 * NT;                         // query rows of a tile
     static constexpr int ROW = EP + 4;                        // floats: the row, its reference point, its sum
-    static constexpr int CTAS = EP == 128 ? 3 : 4;            // per SM
+    static constexpr int CTAS = NT == 2 ? (EP == 128 ? 2 : 3) : (EP == 128 ? 3 : 4);   // per SM
     static constexpr int SMEM = RING + 1024;                  // the swizzle wants the ring on a 1024-byte boundary
-    static_assert(CF_WARPS * 16 * ROW * 4 <= RING, "the warps' rows fit over the ring");
+    static_assert(CF_WARPS * RT * ROW * 4 <= RING, "the warps' rows fit over the ring");
 };
 
 // Byte of 16-byte chunk c of row r of a stage's side, as the tensor map's swizzle lays it: 128-byte rows with the chunk turned
@@ -94,21 +99,34 @@ __device__ __forceinline__ float cf_ex2(float x) {
     return y;
 }
 
-template <int EP, bool FP8>
-__global__ void __launch_bounds__(CF_THREADS, CfCfg<EP>::CTAS)
+__device__ __forceinline__ float cf_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// the transpose of an 8 x 8 matrix of fp16, two neighbours of a row a lane
+__device__ __forceinline__ uint32_t cf_transpose(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <int EP, bool FP8, int NT>
+__global__ void __launch_bounds__(CF_THREADS, CfCfg<EP, NT>::CTAS)
 cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_constant__ CUtensorMap tmapV, const CacheAttnParams p) {
-    using Cfg = CfCfg<EP>;
-    constexpr int W = EP / 8, ROW = Cfg::ROW, HH = EP / 64, STAGES = Cfg::STAGES;
+    using Cfg = CfCfg<EP, NT>;
+    constexpr int W = EP / 8, ROW = Cfg::ROW, HH = EP / 64, NG = CF_GROUPS, RT = Cfg::RT;
     extern __shared__ uint8_t cf_raw[];
-    __shared__ __align__(8) uint64_t full_s[CF_WARPS][STAGES];
-    __shared__ __align__(16) float scales_s[CF_WARPS][STAGES][4];   // key and value scale of each 16 keys
+    __shared__ __align__(8) uint64_t full_s[CF_WARPS][2];              // keys have landed, values have landed
+    __shared__ __align__(16) float scales_s[CF_WARPS][2][2][NG];       // of the tile at hand and the next: key and value scales of each 16 keys
     __shared__ long long start_s, sums_s[CF_WARPS];
     __shared__ int where_s, last_s, abort_s;
     uint8_t* cf_smem = cf_raw + ((1024 - (smem_u32(cf_raw) & 1023)) & 1023);
     const CacheView& c = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (lane == 0) {
-        for (int i = 0; i < STAGES; ++i) mbar_init(&full_s[warp][i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&full_s[warp][i], 1);
         fence_barrier_init();
     }
     if (tid == 0) {
@@ -125,7 +143,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         n = c.tokens(b, p.lens);
         m = c.fresh(b, p.news, p.L);
         tiles = n > 0 ? (n + CF_TILE - 1) / CF_TILE : 1;
-        return (long long)tiles * c.H * ((m * p.G + 15) / 16);
+        return (long long)tiles * (c.H * ((m * p.G + RT - 1) / RT));
     };
     auto before = [&](long long v, long long& all) -> long long {        // sum over the threads before this one, and over all
         long long x = v;
@@ -146,11 +164,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         __syncthreads();
         return x - v + add;
     };
-    long long total = 0;
+    long long total = 0, mine = 0, mine_at = 0;
     for (int b0 = 0; b0 < p.B; b0 += CF_THREADS) {
         int n, m, tiles;
         long long all;
-        before(b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0, all);
+        mine = b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0;
+        mine_at = before(mine, all);
         total += all;
     }
     long long share = (total + gridDim.x - 1) / gridDim.x;
@@ -160,14 +179,17 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     {
         long long base = 0;
         for (int b0 = 0; b0 < p.B; b0 += CF_THREADS) {
-            int n, m, tiles;
-            long long all;
-            const long long mine = b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0, at = base + before(mine, all);
-            if (at <= from && from < at + mine) {
-                where_s = b0 + tid;
-                start_s = at;
+            if (p.B > CF_THREADS) {
+                int n, m, tiles;
+                long long all;
+                mine = b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0;
+                mine_at = base + before(mine, all);
+                base += all;
             }
-            base += all;
+            if (mine_at <= from && from < mine_at + mine) {
+                where_s = b0 + tid;
+                start_s = mine_at;
+            }
             if (base > from) break;
         }
         __syncthreads();
@@ -176,7 +198,10 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     long long bstart = start_s;
 
     // ---- its pieces
-    uint32_t fill = 0, use = 0;   // stages this warp has asked for, and has waited for
+    uint32_t phase = 0;           // of this warp's two barriers
+    const int rows_box = c.T < CF_KEYS ? c.T : CF_KEYS, boxes = CF_KEYS / rows_box;   // tokens that one copy brings, copies a side
+    uint8_t* const K = cf_smem + warp * Cfg::STAGE;
+    uint8_t* const V = K + Cfg::SIDE;
     for (long long at = from; at < to;) {
         int n, m, tiles;
         long long size = entry(b, n, m, tiles);
@@ -184,215 +209,216 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             bstart += size;
             size = entry(++b, n, m, tiles);
         }
-        const int rts = (m * p.G + 15) / 16;
-        const long long off = at - bstart;
-        const int piece = (int)(off / tiles), j0 = (int)(off - (long long)piece * tiles);
+        const int rts = (m * p.G + RT - 1) / RT;
+        const int piece = (int)((at - bstart) / tiles), j0 = (int)(at - bstart - (long long)piece * tiles);
         const int h = piece / rts, rt = piece - h * rts;
         const long long pstart = bstart + (long long)piece * tiles;
         const int j1 = to - pstart < tiles ? (int)(to - pstart) : tiles;
+        const int rows = m * p.G - rt * RT < RT ? m * p.G - rt * RT : RT;
 
-        // rows g and g + 8 of the tile: new token l, query head of the group
-        const int rows = m * p.G - rt * 16 < 16 ? m * p.G - rt * 16 : 16;
-        int last0 = -1, last1 = -1;           // the last key each may see
-        const __half *q0 = nullptr, *q1 = nullptr;
-        {
-            const int r0 = rt * 16 + g, r1 = r0 + 8;
-            if (g < rows) {
-                const int l = r0 / p.G;
-                q0 = p.q + l * p.qL + (h * p.G + r0 - l * p.G) * p.qH + b * p.qB;
-                last0 = p.causal ? n - m + l : n - 1;
-            }
-            if (g + 8 < rows) {
-                const int l = r1 / p.G;
-                q1 = p.q + l * p.qL + (h * p.G + r1 - l * p.G) * p.qH + b * p.qB;
-                last1 = p.causal ? n - m + l : n - 1;
-            }
-        }
-        // This warp's keys of tile j: 32 j' on, j' = 4 (j0 + j) + warp; its page or pages, looked up a tile ahead of the copies.
-        int64_t page0 = -1, page1 = -1;
+        // This warp's keys of tile j, 64 of them.  Lane i looks up box i (the tokens of one page) a tile ahead of its copies; keys and
+        // values have one stage each, refilled as soon as they are read: the other half of the work hides the way.
+        int page = -1;
+        auto first_key = [&](int j) { return (j0 + j) * CF_TILE + warp * CF_KEYS; };
         auto look = [&](int j) {
-            const int key = (j0 + j) * CF_TILE + warp * CF_KEYS;
-            page0 = page1 = -1;
-            if (j0 + j < j1 && key < n) {
-                page0 = c.page(b, key >> c.logT);
-                page1 = key + 16 >= n ? -1 : c.T == 16 ? c.page(b, (key >> 4) + 1) : page0;
-            }
+            const int key = first_key(j) + lane * rows_box;
+            page = j0 + j < j1 && lane < boxes && key < n ? (int)c.page(b, key >> c.logT) : -1;
         };
-        auto fetch = [&](int j) {   // a commit group even when there is none
-            const int key = (j0 + j) * CF_TILE + warp * CF_KEYS;
-            if (j0 + j < j1 && key < n) {
-                const int st = fill % STAGES;
-                if (lane < 4) {   // a group without a page gets a key scale below any magnitude
-                    const int64_t page = lane < 2 ? page0 : page1;
-                    float* dst = &scales_s[warp][st][lane];
-                    if (page >= 0) cf_copy4(smem_u32(dst), ((lane & 1) ? c.vmax : c.kmax) + page * c.H + h);
-                    else *dst = (lane & 1) ? 0.f : -1.f;
-                }
-                if (lane == 0) {
-                    uint8_t* dst = cf_smem + (warp * STAGES + st) * Cfg::STAGE;
-                    const int in = key & (c.T - 1);
-                    if (c.T == 16) {
-                        mbar_arrive_expect_tx(&full_s[warp][st], (uint32_t)((page0 >= 0) + (page1 >= 0)) * Cfg::SIDE);
-                        if (page0 >= 0) {
-                            tma_load_4d(dst, &tmapK, &full_s[warp][st], 0, 0, h, (int)page0);
-                            tma_load_4d(dst + Cfg::SIDE, &tmapV, &full_s[warp][st], 0, 0, h, (int)page0);
-                        }
-                        if (page1 >= 0) {
-                            tma_load_4d(dst + Cfg::SIDE / 2, &tmapK, &full_s[warp][st], 0, 0, h, (int)page1);
-                            tma_load_4d(dst + Cfg::SIDE + Cfg::SIDE / 2, &tmapV, &full_s[warp][st], 0, 0, h, (int)page1);
-                        }
-                    } else {
-                        mbar_arrive_expect_tx(&full_s[warp][st], page0 >= 0 ? Cfg::STAGE : 0);
-                        if (page0 >= 0) {
-                            tma_load_4d(dst, &tmapK, &full_s[warp][st], 0, in, h, (int)page0);
-                            tma_load_4d(dst + Cfg::SIDE, &tmapV, &full_s[warp][st], 0, in, h, (int)page0);
-                        }
-                    }
-                }
-                ++fill;
+        auto copy = [&](int j, int side) {
+            uint64_t* bar = &full_s[warp][side];
+            const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(live) * rows_box * EP);
+            __syncwarp();
+            if (page >= 0)
+                tma_load_4d((side ? V : K) + lane * rows_box * EP, side ? &tmapV : &tmapK, bar, 0, first_key(j) & (c.T - 1), h, page);
+        };
+        auto scales = [&](int j) {   // a group without a page gets a key scale below any magnitude
+            const int grp = lane & (NG - 1), side = lane / NG & 1;
+            const int pg = __shfl_sync(0xffffffffu, page, grp * 16 / rows_box);
+            float* dst = &scales_s[warp][j & 1][side][grp];
+            if (lane < 2 * NG) {
+                if (pg >= 0) cf_copy4(smem_u32(dst), (side ? c.vmax : c.kmax) + (int64_t)pg * c.H + h);
+                else *dst = side ? 0.f : -1.f;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-#pragma unroll
-        for (int j = 0; j < STAGES; ++j) {
-            look(j);
-            fetch(j);
+        if (first_key(0) < n) {
+            look(0);
+            copy(0, 0);
+            copy(0, 1);
+            scales(0);
         }
 
-        // Q: lane (g, t) holds, for keys' elements 64 hh + 16 t + 4 s + (0 .. 3) of step (hh, s), rows g and g + 8
-        uint32_t qa[HH * 4][4];
+        // Query row q of the tile: new token l, query head of the group.  As the products' second operand lane (g, t) holds row
+        // 8 i + g, elements 64 hh + 16 t + 4 s + (0 .. 3) in step (hh, s), the order in which it reads the keys.
+        uint32_t qb[NT][HH * 4][2];
 #pragma unroll
-        for (int hh = 0; hh < HH; ++hh)
+        for (int i = 0; i < NT; ++i) {
+            const int r = rt * RT + i * 8 + g, l = r / p.G;
+            const __half* q = p.q + l * p.qL + (h * p.G + r - l * p.G) * p.qH + b * p.qB;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const __half* q = r ? q1 : q0;
+            for (int hh = 0; hh < HH; ++hh) {
                 const int e = hh * 64 + t * 16;
                 uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (q != nullptr && e < c.E) {
+                if (i * 8 + g < rows && e < c.E) {
                     if (p.whole) {
                         const uint4 a = __ldg(reinterpret_cast<const uint4*>(q + e)), d = __ldg(reinterpret_cast<const uint4*>(q + e + 8));
                         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = d.x, w[5] = d.y, w[6] = d.z, w[7] = d.w;
                     } else {
                         const unsigned short* u = reinterpret_cast<const unsigned short*>(q + e);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+                        for (int k = 0; k < 8; ++k) w[k] = u[2 * k] | (uint32_t)u[2 * k + 1] << 16;
                     }
                 }
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    qa[hh * 4 + s][r] = w[2 * s];
-                    qa[hh * 4 + s][2 + r] = w[2 * s + 1];
+                    qb[i][hh * 4 + s][0] = w[2 * s];
+                    qb[i][hh * 4 + s][1] = w[2 * s + 1];
                 }
             }
-        float o[W][4];
+        }
+        // As results lane (g, t) holds rows 8 i + 2 t and 8 i + 2 t + 1.
+        int last[NT][2];                                     // the last key each may see
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, vref = 0.f;   // vref: the value scale P is relative to
-        uint64_t l0p = 0, l1p = 0;                          // sums of rows g and g + 8, in pairs
-        const int all_see = p.causal ? n - m + rt * 16 / p.G : n - 1;   // the last key that every row may see
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) last[i][k] = p.causal ? n - m + (rt * RT + i * 8 + 2 * t + k) / p.G : n - 1;
+        const int all_see = p.causal ? n - m + rt * RT / p.G : n - 1;   // that every row may see
+        float o[NT][W / 2][4], mref[NT][2], vref = 0.f, vinv = 0.f;     // mref: rows' reference points; vref: the value scale P is relative to
+        uint64_t lsum[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+#pragma unroll
+            for (int u = 0; u < W / 2; ++u) o[i][u][0] = o[i][u][1] = o[i][u][2] = o[i][u][3] = 0.f;
+            mref[i][0] = mref[i][1] = -INFINITY;
+            lsum[i] = 0;
+        }
 
         for (int j = 0; j0 + j < j1; ++j) {
-            const int key0 = (j0 + j) * CF_TILE + warp * CF_KEYS;
+            const int key0 = first_key(j);
             if (key0 >= n) break;   // uniform over the warp, and so is every later tile
-            look(j + STAGES);
-            const int st = use % STAGES;
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-            if (!mbar_wait(&full_s[warp][st], (use / STAGES) & 1, c.d_status, KST_WAIT_FULL, &abort_s)) break;
-            __syncwarp();
-            ++use;
-            const uint8_t* K = cf_smem + (warp * STAGES + st) * Cfg::STAGE;
-            const uint8_t* V = K + Cfg::SIDE;
-            const float4 sc = *reinterpret_cast<const float4*>(scales_s[warp][st]);   // key, value scale of group 0, of group 1
-            float s[4][4];
+            const bool more = j0 + j + 1 < j1 && first_key(j + 1) < n;
+            look(j + 1);
+            if (!mbar_wait(&full_s[warp][0], phase, c.d_status, KST_WAIT_FULL, &abort_s)) break;
+            float s[NT][NG][4];     // rows g and g + 8 of a group's keys, query rows 2 t and 2 t + 1
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+            for (int grp = 0; grp < NG; ++grp) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) s[i][grp][0] = s[i][grp][1] = s[i][grp][2] = s[i][grp][3] = 0.f;
 #pragma unroll
                 for (int hh = 0; hh < HH; ++hh) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(K + cf_place<EP>((i >> 1) * 16 + cf_key<EP>(i & 1, g), hh * 4 + t));
-                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                    const uint4 lo = *reinterpret_cast<const uint4*>(K + cf_place<EP>(grp * 16 + cf_key<EP>(0, g), hh * 4 + t));
+                    const uint4 hi = *reinterpret_cast<const uint4*>(K + cf_place<EP>(grp * 16 + cf_key<EP>(1, g), hh * 4 + t));
+                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        uint32_t b0, b1;
-                        cache_halves<FP8>(w[k], b0, b1);
-                        mma_16816(s[i], qa[hh * 4 + k], b0, b1);
+                        uint32_t a[4];
+                        cache_halves<FP8>(wl[k], a[0], a[2]);
+                        cache_halves<FP8>(wh[k], a[1], a[3]);
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) mma_16816(s[i][grp], a, qb[i][hh * 4 + k][0], qb[i][hh * 4 + k][1]);
                     }
                 }
             }
-            uint64_t s0[4], s1[4];   // scaled, in pairs, of rows g and g + 8
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float ksl = (i < 2 ? sc.x : sc.z) * p.scale_log2;
-                s0[i] = mul2(pack2(s[i][0], s[i][1]), pack2(ksl, ksl));
-                s1[i] = mul2(pack2(s[i][2], s[i][3]), pack2(ksl, ksl));
-                unpack2(s0[i], s[i][0], s[i][1]);
-                unpack2(s1[i], s[i][2], s[i][3]);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncwarp();            // the keys have been read, and this tile's scales are there for every lane
+            float ks[NG], vs[NG];
+            *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(scales_s[warp][j & 1][0]);
+            *reinterpret_cast<float4*>(vs) = *reinterpret_cast<const float4*>(scales_s[warp][j & 1][1]);
+            if (more) {
+                copy(j + 1, 0);
+                scales(j + 1);
             }
-            if (key0 + CF_KEYS - 1 > all_see || sc.x < 0.f || sc.z < 0.f) {   // someone does not see all of these
+            const float vmost = cf_max3(fmaxf(vs[0], vs[1]), vs[2], vs[3]);
+            const bool plain = key0 + CF_KEYS - 1 <= all_see && fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3])) >= 0.f;   // every row sees all of these
+            // a value scale that is not finite is nobody's reference; the sum finds it
+            const bool odd = !(vs[0] + vs[1] + vs[2] + vs[3] < INFINITY);
+            bool grown = false;
+            float top[NT][2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool hidden = (i < 2 ? sc.x : sc.z) < 0.f;
+            for (int i = 0; i < NT; ++i) {
+                top[i][0] = top[i][1] = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int key = key0 + (i >> 1) * 16 + cf_key<EP>(i & 1, 2 * t + (k & 1));
-                        if (hidden || key > (k < 2 ? last0 : last1)) s[i][k] = -INFINITY;
+                for (int grp = 0; grp < NG; ++grp) {
+                    const float ksl = ks[grp] * p.scale_log2;
+                    float* x = s[i][grp];
+                    unpack2(mul2(pack2(x[0], x[1]), pack2(ksl, ksl)), x[0], x[1]);
+                    unpack2(mul2(pack2(x[2], x[3]), pack2(ksl, ksl)), x[2], x[3]);
+                    if (!plain) {
+                        const int k0 = key0 + grp * 16 + cf_key<EP>(0, g), k1 = key0 + grp * 16 + cf_key<EP>(1, g);
+                        const bool hidden = ks[grp] < 0.f;
+                        if (hidden || k0 > last[i][0]) x[0] = -INFINITY;
+                        if (hidden || k0 > last[i][1]) x[1] = -INFINITY;
+                        if (hidden || k1 > last[i][0]) x[2] = -INFINITY;
+                        if (hidden || k1 > last[i][1]) x[3] = -INFINITY;
                     }
-                    s0[i] = pack2(s[i][0], s[i][1]);
-                    s1[i] = pack2(s[i][2], s[i][3]);
+                    top[i][0] = cf_max3(top[i][0], x[0], x[2]);
+                    top[i][1] = cf_max3(top[i][1], x[1], x[3]);
                 }
+                grown = grown || top[i][0] > mref[i][0] + 8.f || top[i][1] > mref[i][1] + 8.f;
             }
-            float x0 = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
-            float x1 = fmaxf(fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3])), fmaxf(fmaxf(s[2][2], s[2][3]), fmaxf(s[3][2], s[3][3])));
+            if (__any_sync(0xffffffffu, grown) || (odd ? true : vmost > vref)) {
+                float vnew = vref;
 #pragma unroll
-            for (int d = 1; d < 4; d *= 2) {   // a quad of lanes shares a row
-                x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-                x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-            }
-            x0 = fmaxf(m0, x0);
-            x1 = fmaxf(m1, x1);
-            float vnew = vref;                                     // a scale that is not finite is nobody's reference
-            if (sc.y < INFINITY && sc.y > vnew) vnew = sc.y;
-            if (sc.w < INFINITY && sc.w > vnew) vnew = sc.w;
-            if (__any_sync(0xffffffffu, x0 != m0 || x1 != m1 || vnew != vref)) {
-                // a row that has seen nothing but hidden keys keeps the reference point -inf and contributes zeros
-                const float a0 = m0 == x0 ? 1.f : cf_ex2(m0 - x0), a1 = m1 == x1 ? 1.f : cf_ex2(m1 - x1);
+                for (int grp = 0; grp < NG; ++grp)
+                    if (vs[grp] < INFINITY && vs[grp] > vnew) vnew = 1.5f * vs[grp];
                 const float f = vnew == vref ? 1.f : vref / vnew;
-                l0p = mul2(l0p, pack2(a0, a0));
-                l1p = mul2(l1p, pack2(a1, a1));
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    o[i][0] *= a0 * f;
-                    o[i][1] *= a0 * f;
-                    o[i][2] *= a1 * f;
-                    o[i][3] *= a1 * f;
-                }
-                m0 = x0, m1 = x1, vref = vnew;
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float x = top[i][k];
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));   // the lanes of a row
+                        x = fmaxf(x, mref[i][k]);
+                        // a row that has seen nothing but hidden keys keeps the reference point -inf and contributes zeros
+                        const float a = mref[i][k] == x ? 1.f : cf_ex2(mref[i][k] - x);
+                        mref[i][k] = x;
+                        float l0, l1;
+                        unpack2(lsum[i], l0, l1);
+                        if (k == 0) l0 *= a;
+                        else l1 *= a;
+                        lsum[i] = pack2(l0, l1);
+#pragma unroll
+                        for (int u = 0; u < W / 2; ++u) {
+                            o[i][u][k] *= a * f;
+                            o[i][u][2 + k] *= a * f;
+                        }
+                    }
+                vref = vnew;
+                vinv = vref > 0x1p-100f ? 128.f / vref : 0.f;   // 0 while there are only pages of zeros
             }
-            const float n0 = m0 == -INFINITY ? 0.f : -m0, n1 = m1 == -INFINITY ? 0.f : -m1;
-            uint32_t pa[2][4];
+            uint32_t pb[NT][NG][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float vs = i < 2 ? sc.y : sc.w, f = (vs == vref ? 1.f : vs / vref) * 4096.f;   // both 0 while there are only pages of zeros
-                float e0, e1, e2, e3;
-                unpack2(add2(s0[i], pack2(n0, n0)), e0, e1);
-                unpack2(add2(s1[i], pack2(n1, n1)), e2, e3);
-                e0 = cf_ex2(e0), e1 = cf_ex2(e1), e2 = cf_ex2(e2), e3 = cf_ex2(e3);
-                l0p = add2(l0p, pack2(e0, e1));
-                l1p = add2(l1p, pack2(e2, e3));
-                unpack2(mul2(pack2(e0, e1), pack2(f, f)), e0, e1);
-                unpack2(mul2(pack2(e2, e3), pack2(f, f)), e2, e3);
-                if (!(vs < INFINITY)) {   // 0 times it is no number: a hidden key has no part
-                    if (s[i][0] == -INFINITY) e0 = 0.f;
-                    if (s[i][1] == -INFINITY) e1 = 0.f;
-                    if (s[i][2] == -INFINITY) e2 = 0.f;
-                    if (s[i][3] == -INFINITY) e3 = 0.f;
+            for (int i = 0; i < NT; ++i) {
+                const uint64_t nm = pack2(mref[i][0] == -INFINITY ? 0.f : -mref[i][0], mref[i][1] == -INFINITY ? 0.f : -mref[i][1]);
+#pragma unroll
+                for (int grp = 0; grp < NG; ++grp) {
+                    const float f = vs[grp] * vinv;
+                    const float* x = s[i][grp];
+                    float e[4];
+                    unpack2(add2(pack2(x[0], x[1]), nm), e[0], e[1]);
+                    unpack2(add2(pack2(x[2], x[3]), nm), e[2], e[3]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) e[k] = cf_ex2(e[k]);
+                    lsum[i] = add2(lsum[i], add2(pack2(e[0], e[1]), pack2(e[2], e[3])));
+                    unpack2(mul2(pack2(e[0], e[1]), pack2(f, f)), e[0], e[1]);
+                    unpack2(mul2(pack2(e[2], e[3]), pack2(f, f)), e[2], e[3]);
+                    if (odd) {   // 0 times what is not finite is no number: a hidden key has no part
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (x[k] == -INFINITY) e[k] = 0.f;
+                    }
+                    pb[i][grp][0] = cf_transpose(cf_pack(e[0], e[1]));
+                    pb[i][grp][1] = cf_transpose(cf_pack(e[2], e[3]));
                 }
-                pa[i >> 1][(i & 1) * 2] = cf_pack(e0, e1);
-                pa[i >> 1][(i & 1) * 2 + 1] = cf_pack(e2, e3);
             }
-            // V: lane (g, t) holds four tokens' W elements of column g, in the order of P's columns
+            if (!mbar_wait(&full_s[warp][1], phase, c.d_status, KST_WAIT_FULL, &abort_s)) break;
+            phase ^= 1;
+            // V: lane (g, t) holds four tokens' W elements of its chunk, in the order of P's rows; elements 2 u and 2 u + 1 of the chunks are
+            // rows g and g + 8 of tile u
 #pragma unroll
-            for (int grp = 0; grp < 2; ++grp) {
+            for (int grp = 0; grp < NG; ++grp) {
                 uint32_t w[4][W / 4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -411,53 +437,56 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                     cf_values<FP8>(w[0][u], w[1][u], b0);
                     cf_values<FP8>(w[2][u], w[3][u], b1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mma_16816(o[u * 4 + i], pa[grp], b0[i], b1[i]);
+                    for (int i = 0; i < NT; ++i) {
+                        mma_16816(o[i][2 * u], b0[0], b0[1], b1[0], b1[1], pb[i][grp][0], pb[i][grp][1]);
+                        mma_16816(o[i][2 * u + 1], b0[2], b0[3], b1[2], b1[3], pb[i][grp][0], pb[i][grp][1]);
+                    }
                 }
             }
-            __syncwarp();   // the stage has been read
-            fetch(j + STAGES);
-        }
-        float l0, l1, l0b, l1b;
-        unpack2(l0p, l0, l0b);
-        unpack2(l1p, l1, l1b);
-        l0 += l0b;
-        l1 += l1b;
-#pragma unroll
-        for (int d = 1; d < 4; d *= 2) {
-            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+            __syncwarp();   // the values have been read
+            if (more) copy(j + 1, 1);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();   // the ring is free: every copy that was asked for has been waited for
         // this warp's rows: [row][EP values, reference point, sum]
-        float* mine = reinterpret_cast<float*>(cf_smem) + warp * 16 * ROW;
-        const float back = vref * (1.f / 4096.f) / cache_top<FP8>();
+        {
+            float* to_s = reinterpret_cast<float*>(cf_smem) + warp * RT * ROW;
+            const float back = vref * (1.f / 128.f) / cache_top<FP8>();
+            const int e0 = W * (EP == 128 ? cf_chunk(g) : g);
 #pragma unroll
-        for (int i = 0; i < W; i += 4)
+            for (int i = 0; i < NT; ++i) {
+                float l[2];
+                unpack2(lsum[i], l[0], l[1]);
 #pragma unroll
-            for (int col = 0; col < 2; ++col)
+                for (int k = 0; k < 2; ++k) {
+                    const int row = i * 8 + 2 * t + k;
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    *reinterpret_cast<float4*>(mine + (g + 8 * r) * ROW + (EP == 128 ? 64 * col + 16 * t : 16 * t + 8 * col) + i) =
-                        make_float4(o[i][2 * r + col] * back, o[i + 1][2 * r + col] * back, o[i + 2][2 * r + col] * back, o[i + 3][2 * r + col] * back);
-        if (t == 0) {
-            *reinterpret_cast<float2*>(mine + g * ROW + EP) = make_float2(m0, l0);
-            *reinterpret_cast<float2*>(mine + (g + 8) * ROW + EP) = make_float2(m1, l1);
+                    for (int d = 4; d < 32; d *= 2) l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
+                    if (row < rows) {
+#pragma unroll
+                        for (int u = 0; u < W / 2; u += 2)
+                            *reinterpret_cast<float4*>(to_s + row * ROW + e0 + 2 * u) =
+                                make_float4(o[i][u][k] * back, o[i][u][2 + k] * back, o[i][u + 1][k] * back, o[i][u + 1][2 + k] * back);
+                        if (g == 0) *reinterpret_cast<float2*>(to_s + row * ROW + EP) = make_float2(mref[i][k], l[k]);
+                    }
+                }
+            }
         }
         __syncthreads();
         const bool whole = j0 == 0 && j1 == tiles;
-        const long long first = pstart / share, final = (pstart + tiles - 1) / share;   // blocks that hold parts of this piece
-        float* part = p.part + ((int64_t)blockIdx.x * 2 + (j0 == 0)) * 16 * ROW;
+        float* part = p.part + ((int64_t)blockIdx.x * 2 + (j0 == 0)) * RT * ROW;
         auto store = [&](int row, int e4, float4 v) {
-            const int r = rt * 16 + row, l = r / p.G;
+            const int r = rt * RT + row, l = r / p.G;
             const int64_t at = l * p.oL + (h * p.G + r - l * p.G) * p.oH + b * p.oB + e4;
             if (e4 >= c.E) return;
             if (p.out_f32) {
                 float* d = (float*)p.out + at;
-                d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+                if (p.out_whole) *reinterpret_cast<float4*>(d) = v;
+                else d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
             } else {
                 __half* d = (__half*)p.out + at;
-                d[0] = __float2half_rn(v.x), d[1] = __float2half_rn(v.y), d[2] = __float2half_rn(v.z), d[3] = __float2half_rn(v.w);
+                if (p.out_whole) *reinterpret_cast<uint2*>(d) = make_uint2(cf_pack(v.x, v.y), cf_pack(v.z, v.w));
+                else d[0] = __float2half_rn(v.x), d[1] = __float2half_rn(v.y), d[2] = __float2half_rn(v.z), d[3] = __float2half_rn(v.w);
             }
         };
         for (int i = tid; i < rows * (EP / 4); i += CF_THREADS) {   // the warps of a row
@@ -465,14 +494,14 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             const float* src = reinterpret_cast<const float*>(cf_smem) + row * ROW;
             float M = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, src[w * 16 * ROW + EP]);
+            for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, src[w * RT * ROW + EP]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < CF_WARPS; ++w) {
-                const float mw = src[w * 16 * ROW + EP], f = mw == M ? 1.f : cf_ex2(mw - M);   // 1: both may be -inf, with zeros or a NaN
-                const float4 x = *reinterpret_cast<const float4*>(src + w * 16 * ROW + e4);
+                const float mw = src[w * RT * ROW + EP], f = mw == M ? 1.f : cf_ex2(mw - M);   // 1: both may be -inf, with zeros or a NaN
+                const float4 x = *reinterpret_cast<const float4*>(src + w * RT * ROW + e4);
                 v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
-                l = fmaf(src[w * 16 * ROW + EP + 1], f, l);
+                l = fmaf(src[w * RT * ROW + EP + 1], f, l);
             }
             if (whole) {
                 const float inv = l == 0.f ? 1.f : 1.f / l;
@@ -483,9 +512,10 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             }
         }
         if (!whole) {   // whoever is last joins the parts, in block order
+            const int first = (int)(pstart / share), final = (int)((pstart + tiles - 1) / share);   // blocks that hold parts of this piece
             __threadfence();
             __syncthreads();
-            if (tid == 0) last_s = atomicAdd(p.arrived + first, 1) == (int)(final - first);
+            if (tid == 0) last_s = atomicAdd(p.arrived + first, 1) == final - first;
             __syncthreads();
             if (last_s) {
                 __threadfence();
@@ -493,14 +523,29 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                     const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
                     float M = -INFINITY, l = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (long long k = first; k <= final; ++k) {
-                        const float* src = p.part + (k * 2 + (k == first)) * 16 * ROW + row * ROW;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + EP));
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(src + e4));
-                        const float top = fmaxf(M, ml.x);
-                        const float a = M == top ? 1.f : cf_ex2(M - top), f = ml.x == top ? 1.f : cf_ex2(ml.x - top);
-                        v.x = v.x * a + x.x * f, v.y = v.y * a + x.y * f, v.z = v.z * a + x.z * f, v.w = v.w * a + x.w * f;
-                        l = l * a + ml.y * f;
+                    constexpr int AT_ONCE = 8;   // parts in flight: each is a trip to L2
+                    for (int k0 = first; k0 <= final; k0 += AT_ONCE) {
+                        float2 ml[AT_ONCE];
+                        float4 x[AT_ONCE];
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k) {
+                            const int blk = k0 + k <= final ? k0 + k : final;
+                            const float* src = p.part + ((int64_t)blk * 2 + (blk == first)) * RT * ROW + row * ROW;
+                            ml[k] = __ldcg(reinterpret_cast<const float2*>(src + EP));
+                            x[k] = __ldcg(reinterpret_cast<const float4*>(src + e4));
+                        }
+                        float top = M;
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
+                        const float a = M == top ? 1.f : cf_ex2(M - top);
+                        v.x *= a, v.y *= a, v.z *= a, v.w *= a, l *= a;
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k)
+                            if (k0 + k <= final) {
+                                const float f = ml[k].x == top ? 1.f : cf_ex2(ml[k].x - top);
+                                v.x = fmaf(x[k].x, f, v.x), v.y = fmaf(x[k].y, f, v.y), v.z = fmaf(x[k].z, f, v.z), v.w = fmaf(x[k].w, f, v.w);
+                                l = fmaf(ml[k].y, f, l);
+                            }
                         M = top;
                     }
                     const float inv = l == 0.f ? 1.f : 1.f / l;
@@ -523,10 +568,10 @@ static int cf_map(b200_ctx* ctx, CUtensorMap* m, const void* base, const CacheVi
     return make_tmap(ctx, m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, EP == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-template <int EP, bool FP8>
+template <int EP, bool FP8, int NT>
 static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
-    using Cfg = CfCfg<EP>;
-    auto kern = cache_attention_kernel<EP, FP8>;
+    using Cfg = CfCfg<EP, NT>;
+    auto kern = cache_attention_kernel<EP, FP8, NT>;
     CUtensorMap mk, mv;
     const int rows = p.c.T < CF_KEYS ? p.c.T : CF_KEYS;
     int rc = cf_map(ctx, &mk, p.c.k, p.c, p.c.kT, p.c.kH, p.c.kP, EP, rows);
@@ -536,11 +581,11 @@ static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     // One resident wave at most, and no more blocks than there can be shares.
     int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
     if (grid > GEMV_COUNTER_COUNT) grid = GEMV_COUNTER_COUNT;
-    const int64_t tiles = cdiv((int64_t)p.c.width * p.c.T, CF_TILE), rts = cdiv((int64_t)p.L * p.G, 16);
+    const int64_t tiles = cdiv((int64_t)p.c.width * p.c.T, CF_TILE), rts = cdiv((int64_t)p.L * p.G, Cfg::RT);
     const double most = (double)tiles * rts * p.c.H * p.B / CF_SHARE;
     if (most + 1 < (double)grid) grid = (int64_t)most + 1;
     void* ws = nullptr;
-    rc = ws_scratch(ctx, (size_t)grid * 2 * 16 * Cfg::ROW * sizeof(float), &ws);
+    rc = ws_scratch(ctx, (size_t)grid * 2 * Cfg::RT * Cfg::ROW * sizeof(float), &ws);
     if (rc) return rc;
     p.part = static_cast<float*>(ws);
     p.arrived = ctx->sk_flags + SK_FLAG_COUNT;
@@ -577,11 +622,17 @@ int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int
     p.L = (int)L, p.B = (int)B, p.G = (int)(Hq / p.c.H);
     p.causal = causal, p.out_f32 = out_dtype == B200_F32;
     p.whole = ((uintptr_t)q->ptr % 16 | (uint64_t)q->stride[1] % 8 | (uint64_t)q->stride[2] % 8 | (uint64_t)q->stride[3] % 8) == 0;
+    const int64_t four = p.out_f32 ? 16 : 8, size = four / 4;
+    p.out_whole = ((uintptr_t)out->ptr | (uint64_t)(out->stride[1] * size) | (uint64_t)(out->stride[2] * size) | (uint64_t)(out->stride[3] * size)) % four == 0;
     const bool fp8 = cache->kind == B200_E4M3;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634 / (fp8 ? 448.0 : 127.0));
     B200_CUDA(cudaSetDevice(ctx->device));
-    if (p.c.E <= 64) return fp8 ? cf_launch<64, true>(ctx, p) : cf_launch<64, false>(ctx, p);
-    return fp8 ? cf_launch<128, true>(ctx, p) : cf_launch<128, false>(ctx, p);
+    if (p.L * p.G <= 8) {
+        if (p.c.E <= 64) return fp8 ? cf_launch<64, true, 1>(ctx, p) : cf_launch<64, false, 1>(ctx, p);
+        return fp8 ? cf_launch<128, true, 1>(ctx, p) : cf_launch<128, false, 1>(ctx, p);
+    }
+    if (p.c.E <= 64) return fp8 ? cf_launch<64, true, 2>(ctx, p) : cf_launch<64, false, 2>(ctx, p);
+    return fp8 ? cf_launch<128, true, 2>(ctx, p) : cf_launch<128, false, 2>(ctx, p);
 }
 
 } // extern "C"
