@@ -13,12 +13,14 @@
 // score is 2^8 past its row's reference point; P is rounded to fp16 times 2^7, so that it stays in range and weights down to
 // 2^-21 of the reference keep all their bits.
 //
-// Each warp streams keys of its own, 64 at a time, which its first lanes fetch by TMA: nothing but the end of a piece of work
-// brings a block's warps together, and what a copy costs is a few instructions.
-//
-// The work is one list of key tiles over all (sequence, key head, row tile), computed from the lengths on the device and dealt
-// out in equal shares, so ragged lengths and few sequences fill the GPU alike.  A share's first and last pieces may be parts
-// of a list entry; their rows meet in the workspace and the last block to arrive joins them, in block order.
+// The work is one list of 64-key tiles over all (sequence, key head, row tile): pieces.  It is computed from the lengths on the
+// device and dealt out to the warps in equal contiguous shares, so ragged lengths and few sequences fill the GPU alike.  A warp
+// streams its tiles by TMA and meets nobody before its block's end: it asks for the next piece's first tile before it writes the
+// results of the last.  (Blocks that walked the list together lost 8 us at every change of piece, the slowest warp's tile and
+// the trips to memory that nothing hid: 32 x 8192 tokens 62 us.)  A piece that one warp holds whole is stored at once.  Of the
+// others, what ends inside a warp's share waits in the workspace; the last pieces of a block's warps are joined in shared
+// memory at its end, and whichever block is last to bring a part of a piece joins them all, in the order of the list: the
+// result does not depend on timing.
 #include <cuda_fp16.h>
 
 #include "cache8.cuh"
@@ -27,10 +29,8 @@ namespace b200 {
 
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
-constexpr int CF_KEYS = 64;                      // keys a warp takes at a time
+constexpr int CF_KEYS = 64;                      // keys a warp takes at a time: a tile of the list
 constexpr int CF_GROUPS = CF_KEYS / 16;          // of one page each
-constexpr int CF_TILE = CF_WARPS * CF_KEYS;      // keys of a tile
-constexpr int CF_SHARE = 1;                      // tiles of a share at least
 
 struct CacheAttnParams {
     CacheView c;
@@ -41,8 +41,8 @@ struct CacheAttnParams {
     int L, B, G;                          // rows at most, sequences, query heads a key head
     int causal, out_f32, whole, out_whole;   // rows of q start on 16-byte boundaries, fours of out on their own size
     float scale_log2;
-    float* part;                          // [block][first or last][row][EP + 4]
-    int* arrived;
+    float* part;                          // [warp][ended inside its share, or its last][row][EP + 4]
+    int* arrived;                         // [warp], zero between launches
 };
 
 template <int EP, int NT> struct CfCfg {
@@ -51,9 +51,12 @@ template <int EP, int NT> struct CfCfg {
     static constexpr int RING = CF_WARPS * STAGE;
     static constexpr int RT = 8 * NT;                         // query rows of a tile
     static constexpr int ROW = EP + 4;                        // floats: the row, its reference point, its sum
-    static constexpr int CTAS = NT == 2 ? (EP == 128 ? 2 : 3) : (EP == 128 ? 3 : 4);   // per SM
+    // Per SM.  A third block of 128-wide rows adds parts to join and nothing to the rate (131071 tokens 57.7 -> 53.1 us with two).
+    static constexpr int CTAS = NT == 1 && EP == 64 ? 4 : 2;
     static constexpr int SMEM = RING + 1024;                  // the swizzle wants the ring on a 1024-byte boundary
     static_assert(CF_WARPS * RT * ROW * 4 <= RING, "the warps' rows fit over the ring");
+    static constexpr int BLOCKS = 148 * CTAS;                 // of a launch at most
+    static_assert(BLOCKS * CF_WARPS <= SK_FLAG_COUNT && RT * (BLOCKS + 3) * 4 <= RING, "a counter a warp; the parts' weights fit over the ring");
 };
 
 // Byte of 16-byte chunk c of row r of a stage's side, as the tensor map's swizzle lays it: 128-byte rows with the chunk turned
@@ -112,6 +115,25 @@ __device__ __forceinline__ uint32_t cf_transpose(uint32_t v) {
     return r;
 }
 
+// floor(a / b), 0 <= a < 2^52: an integer division of 64 bits takes ten times as long, and the ends of a share wait for several.
+__device__ __forceinline__ long long cf_div(long long a, long long b) {
+    long long q = (long long)((double)a / (double)b);
+    const long long r = a - q * b;
+    if (r < 0) --q;
+    else if (r >= b) ++q;
+    return q;
+}
+
+struct CfParts {              // where the parts of a piece are: its first and last warp, blocks with a part of it, parts
+    int w0, w1, blocks, count;
+};
+struct CfPiece {
+    long long start;          // its first tile in the list
+    int b, n, m, tiles;       // sequence, its length and new tokens; tiles of a piece of it
+    int h, rt, rows;          // key head, row tile, rows that count
+    int j0, j1;               // the tiles of it that this warp has
+};
+
 template <int EP, bool FP8, int NT>
 __global__ void __launch_bounds__(CF_THREADS, CfCfg<EP, NT>::CTAS)
 cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_constant__ CUtensorMap tmapV, const CacheAttnParams p) {
@@ -120,8 +142,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     extern __shared__ uint8_t cf_raw[];
     __shared__ __align__(8) uint64_t full_s[CF_WARPS][2];              // keys have landed, values have landed
     __shared__ __align__(16) float scales_s[CF_WARPS][2][2][NG];       // of the tile at hand and the next: key and value scales of each 16 keys
-    __shared__ long long start_s, sums_s[CF_WARPS];
-    __shared__ int where_s, last_s, abort_s;
+    __shared__ long long start_s[CF_WARPS], sums_s[CF_WARPS];
+    __shared__ int where_s[CF_WARPS], abort_s;
+    __shared__ CfPiece given_s[2 * CF_WARPS];                          // parts of pieces this block's warps have: ended, last
+    __shared__ CfParts parts_s[2 * CF_WARPS];
+    __shared__ int has_s[2 * CF_WARPS], join_s[2 * CF_WARPS];          // there is one; this block joins its piece
+    if (threadIdx.x < 2 * CF_WARPS) has_s[threadIdx.x] = 0;
     uint8_t* cf_smem = cf_raw + ((1024 - (smem_u32(cf_raw) & 1023)) & 1023);
     const CacheView& c = p.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -142,7 +168,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     auto entry = [&](int b, int& n, int& m, int& tiles) -> long long {   // tiles of sequence b, over its heads and row tiles
         n = c.tokens(b, p.lens);
         m = c.fresh(b, p.news, p.L);
-        tiles = n > 0 ? (n + CF_TILE - 1) / CF_TILE : 1;
+        tiles = n > 0 ? (n + CF_KEYS - 1) / CF_KEYS : 1;
         return (long long)tiles * (c.H * ((m * p.G + RT - 1) / RT));
     };
     auto before = [&](long long v, long long& all) -> long long {        // sum over the threads before this one, and over all
@@ -164,45 +190,66 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         __syncthreads();
         return x - v + add;
     };
-    long long total = 0, mine = 0, mine_at = 0;
-    for (int b0 = 0; b0 < p.B; b0 += CF_THREADS) {
+    long long total = 0, bstart = 0, from = 0, to = 0;
+    int b = 0, warps = 0;         // warps that have a share
+    const int me = blockIdx.x * CF_WARPS + warp;
+    auto deal = [&]() {
+        warps = gridDim.x * CF_WARPS;
+        if (total < warps) warps = (int)total;
+        if (me < warps) {
+            from = cf_div(me * total, warps);
+            to = cf_div((me + 1) * total, warps);
+        }
+    };
+    if (p.B <= 32) {              // every warp for itself
         int n, m, tiles;
-        long long all;
-        mine = b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0;
-        mine_at = before(mine, all);
-        total += all;
-    }
-    long long share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < CF_SHARE) share = CF_SHARE;
-    const long long from = blockIdx.x * share, to = from + share < total ? from + share : total;
-    if (from >= to) return;
-    {
+        const long long mine = lane < p.B ? entry(lane, n, m, tiles) : 0;
+        long long x = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        total = __shfl_sync(0xffffffffu, x, 31);
+        deal();
+        b = __ffs(__ballot_sync(0xffffffffu, from < x)) - 1;    // the first sequence that ends behind `from`
+        bstart = __shfl_sync(0xffffffffu, x - mine, b < 0 ? 0 : b);
+    } else {
+        for (int b0 = 0; b0 < p.B; b0 += CF_THREADS) {
+            int n, m, tiles;
+            long long all;
+            before(b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0, all);
+            total += all;
+        }
+        deal();
         long long base = 0;
         for (int b0 = 0; b0 < p.B; b0 += CF_THREADS) {
-            if (p.B > CF_THREADS) {
-                int n, m, tiles;
-                long long all;
-                mine = b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0;
-                mine_at = base + before(mine, all);
-                base += all;
+            int n, m, tiles;
+            long long all;
+            const long long mine = b0 + tid < p.B ? entry(b0 + tid, n, m, tiles) : 0, at = base + before(mine, all);
+#pragma unroll
+            for (int w = 0; w < CF_WARPS; ++w) {
+                const int who = blockIdx.x * CF_WARPS + w;
+                if (who >= warps) break;
+                const long long f = cf_div(who * total, warps);
+                if (at <= f && f < at + mine) {
+                    where_s[w] = b0 + tid;
+                    start_s[w] = at;
+                }
             }
-            if (mine_at <= from && from < mine_at + mine) {
-                where_s = b0 + tid;
-                start_s = mine_at;
-            }
-            if (base > from) break;
+            base += all;
         }
         __syncthreads();
+        b = where_s[warp];
+        bstart = start_s[warp];
     }
-    int b = where_s;
-    long long bstart = start_s;
 
     // ---- its pieces
     uint32_t phase = 0;           // of this warp's two barriers
     const int rows_box = c.T < CF_KEYS ? c.T : CF_KEYS, boxes = CF_KEYS / rows_box;   // tokens that one copy brings, copies a side
     uint8_t* const K = cf_smem + warp * Cfg::STAGE;
     uint8_t* const V = K + Cfg::SIDE;
-    for (long long at = from; at < to;) {
+    auto locate = [&](CfPiece& pc, long long at) {
         int n, m, tiles;
         long long size = entry(b, n, m, tiles);
         while (at >= bstart + size) {          // the next sequence with work
@@ -210,57 +257,56 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             size = entry(++b, n, m, tiles);
         }
         const int rts = (m * p.G + RT - 1) / RT;
-        const int piece = (int)((at - bstart) / tiles), j0 = (int)(at - bstart - (long long)piece * tiles);
-        const int h = piece / rts, rt = piece - h * rts;
-        const long long pstart = bstart + (long long)piece * tiles;
-        const int j1 = to - pstart < tiles ? (int)(to - pstart) : tiles;
-        const int rows = m * p.G - rt * RT < RT ? m * p.G - rt * RT : RT;
-
-        // This warp's keys of tile j, 64 of them.  Lane i looks up box i (the tokens of one page) a tile ahead of its copies; keys and
-        // values have one stage each, refilled as soon as they are read: the other half of the work hides the way.
-        int page = -1;
-        auto first_key = [&](int j) { return (j0 + j) * CF_TILE + warp * CF_KEYS; };
-        auto look = [&](int j) {
-            const int key = first_key(j) + lane * rows_box;
-            page = j0 + j < j1 && lane < boxes && key < n ? (int)c.page(b, key >> c.logT) : -1;
-        };
-        auto copy = [&](int j, int side) {
-            uint64_t* bar = &full_s[warp][side];
-            const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
-            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(live) * rows_box * EP);
-            __syncwarp();
-            if (page >= 0)
-                tma_load_4d((side ? V : K) + lane * rows_box * EP, side ? &tmapV : &tmapK, bar, 0, first_key(j) & (c.T - 1), h, page);
-        };
-        auto scales = [&](int j) {   // a group without a page gets a key scale below any magnitude
-            const int grp = lane & (NG - 1), side = lane / NG & 1;
-            const int pg = __shfl_sync(0xffffffffu, page, grp * 16 / rows_box);
-            float* dst = &scales_s[warp][j & 1][side][grp];
-            if (lane < 2 * NG) {
-                if (pg >= 0) cf_copy4(smem_u32(dst), (side ? c.vmax : c.kmax) + (int64_t)pg * c.H + h);
-                else *dst = side ? 0.f : -1.f;
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        if (first_key(0) < n) {
-            look(0);
-            copy(0, 0);
-            copy(0, 1);
-            scales(0);
+        const long long off = at - bstart;
+        const int piece = (int)cf_div(off, tiles);
+        pc.b = b, pc.n = n, pc.m = m, pc.tiles = tiles;
+        pc.h = piece / rts, pc.rt = piece - pc.h * rts;
+        pc.rows = m * p.G - pc.rt * RT < RT ? m * p.G - pc.rt * RT : RT;
+        pc.start = bstart + (long long)piece * tiles;
+        pc.j0 = (int)(at - pc.start);
+        pc.j1 = to - pc.start < tiles ? (int)(to - pc.start) : tiles;
+    };
+    // The tile to be asked for next, of this piece or the one behind it.  Lane i looks up box i of it (the tokens of one page) a tile
+    // ahead of its copies; keys and values have one stage each, refilled as soon as they are read: the other half of the work hides
+    // the way.
+    int tb = 0, tn = 0, th = 0, tj = -1, page = -1, slot = 1;
+    auto look = [&](const CfPiece& q, int j) {
+        tb = q.b, tn = q.n, th = q.h, tj = j;
+        const int key = j * CF_KEYS + lane * rows_box;
+        page = lane < boxes && key < tn ? (int)c.page(tb, key >> c.logT) : -1;
+    };
+    auto copy = [&](int side) {
+        uint64_t* bar = &full_s[warp][side];
+        const uint32_t live = __ballot_sync(0xffffffffu, page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(live) * rows_box * EP);
+        __syncwarp();
+        if (page >= 0)
+            tma_load_4d((side ? V : K) + lane * rows_box * EP, side ? &tmapV : &tmapK, bar, 0, tj * CF_KEYS & (c.T - 1), th, page);
+    };
+    auto scales = [&]() {   // into the other slot; a group without a page gets a key scale below any magnitude
+        slot ^= 1;
+        const int grp = lane & (NG - 1), side = lane / NG & 1;
+        const int pg = __shfl_sync(0xffffffffu, page, grp * 16 / rows_box);
+        float* dst = &scales_s[warp][slot][side][grp];
+        if (lane < 2 * NG) {
+            if (pg >= 0) cf_copy4(smem_u32(dst), (side ? c.vmax : c.kmax) + (int64_t)pg * c.H + th);
+            else *dst = side ? 0.f : -1.f;
         }
-
-        // Query row q of the tile: new token l, query head of the group.  As the products' second operand lane (g, t) holds row
-        // 8 i + g, elements 64 hh + 16 t + 4 s + (0 .. 3) in step (hh, s), the order in which it reads the keys.
-        uint32_t qb[NT][HH * 4][2];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // Query row r of a piece: new token l, query head of the group.  As the products' second operand lane (g, t) holds row
+    // 8 i + g, elements 64 hh + 16 t + 4 s + (0 .. 3) in step (hh, s), the order in which it reads the keys.
+    uint32_t qb[NT][HH * 4][2];
+    auto queries = [&](const CfPiece& x) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const int r = rt * RT + i * 8 + g, l = r / p.G;
-            const __half* q = p.q + l * p.qL + (h * p.G + r - l * p.G) * p.qH + b * p.qB;
+            const int r = x.rt * RT + i * 8 + g, l = r / p.G;
+            const __half* q = p.q + l * p.qL + (x.h * p.G + r - l * p.G) * p.qH + x.b * p.qB;
 #pragma unroll
             for (int hh = 0; hh < HH; ++hh) {
                 const int e = hh * 64 + t * 16;
                 uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (i * 8 + g < rows && e < c.E) {
+                if (i * 8 + g < x.rows && e < c.E) {
                     if (p.whole) {
                         const uint4 a = __ldg(reinterpret_cast<const uint4*>(q + e)), d = __ldg(reinterpret_cast<const uint4*>(q + e + 8));
                         w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = d.x, w[5] = d.y, w[6] = d.z, w[7] = d.w;
@@ -277,6 +323,65 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 }
             }
         }
+    };
+    // Four results of a row of a piece.
+    auto store = [&](const CfPiece& q, int row, int e4, float4 v) {
+        const int r = q.rt * RT + row, l = r / p.G;
+        const int64_t at = l * p.oL + (q.h * p.G + r - l * p.G) * p.oH + q.b * p.oB + e4;
+        if (e4 >= c.E) return;
+        if (p.out_f32) {
+            float* d = (float*)p.out + at;
+            if (p.out_whole) *reinterpret_cast<float4*>(d) = v;
+            else d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+        } else {
+            __half* d = (__half*)p.out + at;
+            if (p.out_whole) *reinterpret_cast<uint2*>(d) = make_uint2(cf_pack(v.x, v.y), cf_pack(v.z, v.w));
+            else d[0] = __float2half_rn(v.x), d[1] = __float2half_rn(v.y), d[2] = __float2half_rn(v.z), d[3] = __float2half_rn(v.w);
+        }
+    };
+    float o[NT][W / 2][4], mref[NT][2], vref = 0.f, vinv = 0.f;     // mref: rows' reference points; vref: the value scale P is relative to
+    uint64_t lsum[NT];
+    const int e0 = W * (EP == 128 ? cf_chunk(g) : g);               // this lane's W elements of its rows
+    // This warp's rows of piece q: `put` gets (row, element, four values times f(row's sum)) and `ends` (row, reference point, sum).
+    auto results = [&](const CfPiece& q, auto factor, auto put, auto ends) {
+        const float back = vref * (1.f / 128.f) / cache_top<FP8>();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            float l[2];
+            unpack2(lsum[i], l[0], l[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int row = i * 8 + 2 * t + k;
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
+                if (row < q.rows) {
+                    const float f = back * factor(l[k]);
+#pragma unroll
+                    for (int u = 0; u < W / 2; u += 2)
+                        put(row, e0 + 2 * u, make_float4(o[i][u][k] * f, o[i][u][2 + k] * f, o[i][u + 1][k] * f, o[i][u + 1][2 + k] * f));
+                    if (g == 0) ends(row, mref[i][k], l[k]);
+                }
+            }
+        }
+    };
+    const auto one = [](float) { return 1.f; };
+    auto keep = [&](float* to_p, const CfPiece& q) {   // as rows of [EP values, reference point, sum]
+        results(q, one, [&](int row, int e4, float4 v) { *reinterpret_cast<float4*>(to_p + row * ROW + e4) = v; },
+                [&](int row, float mr, float l) { *reinterpret_cast<float2*>(to_p + row * ROW + EP) = make_float2(mr, l); });
+    };
+
+    CfPiece pc, nx;
+    if (from < to) {
+        locate(pc, from);
+        look(pc, pc.j0);
+        copy(0);
+        copy(1);
+        scales();
+        queries(pc);
+    }
+    for (long long at = from; at < to;) {
+        const int n = pc.n, m = pc.m, rt = pc.rt;
+        at = pc.start + pc.j1;
         // As results lane (g, t) holds rows 8 i + 2 t and 8 i + 2 t + 1.
         int last[NT][2];                                     // the last key each may see
 #pragma unroll
@@ -284,8 +389,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
 #pragma unroll
             for (int k = 0; k < 2; ++k) last[i][k] = p.causal ? n - m + (rt * RT + i * 8 + 2 * t + k) / p.G : n - 1;
         const int all_see = p.causal ? n - m + rt * RT / p.G : n - 1;   // that every row may see
-        float o[NT][W / 2][4], mref[NT][2], vref = 0.f, vinv = 0.f;     // mref: rows' reference points; vref: the value scale P is relative to
-        uint64_t lsum[NT];
+        vref = vinv = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -294,11 +398,15 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             lsum[i] = 0;
         }
 
-        for (int j = 0; j0 + j < j1; ++j) {
-            const int key0 = first_key(j);
-            if (key0 >= n) break;   // uniform over the warp, and so is every later tile
-            const bool more = j0 + j + 1 < j1 && first_key(j + 1) < n;
-            look(j + 1);
+        for (int j = pc.j0; j < pc.j1; ++j) {
+            const int key0 = j * CF_KEYS;
+            const bool last_one = j + 1 == pc.j1, more = !last_one || at < to;
+            if (!last_one) {
+                look(pc, j + 1);
+            } else if (more) {   // the next piece's first tile
+                locate(nx, at);
+                look(nx, nx.j0);
+            }
             if (!mbar_wait(&full_s[warp][0], phase, c.d_status, KST_WAIT_FULL, &abort_s)) break;
             float s[NT][NG][4];     // rows g and g + 8 of a group's keys, query rows 2 t and 2 t + 1
 #pragma unroll
@@ -323,11 +431,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             asm volatile("cp.async.wait_all;" ::: "memory");
             __syncwarp();            // the keys have been read, and this tile's scales are there for every lane
             float ks[NG], vs[NG];
-            *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(scales_s[warp][j & 1][0]);
-            *reinterpret_cast<float4*>(vs) = *reinterpret_cast<const float4*>(scales_s[warp][j & 1][1]);
+            *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(scales_s[warp][slot][0]);
+            *reinterpret_cast<float4*>(vs) = *reinterpret_cast<const float4*>(scales_s[warp][slot][1]);
             if (more) {
-                copy(j + 1, 0);
-                scales(j + 1);
+                copy(0);
+                scales();
+                if (last_one) queries(nx);
             }
             const float vmost = cf_max3(fmaxf(vs[0], vs[1]), vs[2], vs[3]);
             const bool plain = key0 + CF_KEYS - 1 <= all_see && fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3])) >= 0.f;   // every row sees all of these
@@ -444,119 +553,172 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 }
             }
             __syncwarp();   // the values have been read
-            if (more) copy(j + 1, 1);
+            if (more) copy(1);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();   // the ring is free: every copy that was asked for has been waited for
-        // this warp's rows: [row][EP values, reference point, sum]
-        {
-            float* to_s = reinterpret_cast<float*>(cf_smem) + warp * RT * ROW;
-            const float back = vref * (1.f / 128.f) / cache_top<FP8>();
-            const int e0 = W * (EP == 128 ? cf_chunk(g) : g);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                float l[2];
-                unpack2(lsum[i], l[0], l[1]);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int row = i * 8 + 2 * t + k;
-#pragma unroll
-                    for (int d = 4; d < 32; d *= 2) l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
-                    if (row < rows) {
-#pragma unroll
-                        for (int u = 0; u < W / 2; u += 2)
-                            *reinterpret_cast<float4*>(to_s + row * ROW + e0 + 2 * u) =
-                                make_float4(o[i][u][k] * back, o[i][u][2 + k] * back, o[i][u + 1][k] * back, o[i][u + 1][2 + k] * back);
-                        if (g == 0) *reinterpret_cast<float2*>(to_s + row * ROW + EP) = make_float2(mref[i][k], l[k]);
-                    }
-                }
-            }
+        // the next piece's first tile is on its way while this one's results leave
+        const CfPiece done = pc;
+        const bool mine = done.j0 == 0 && done.j1 == done.tiles;
+        if (at < to) pc = nx;
+        if (mine)
+            results(done, [](float l) { return l == 0.f ? 1.f : 1.f / l; }, [&](int row, int e4, float4 v) { store(done, row, e4, v); },
+                    [](int, float, float) {});
+        else if (at < to) keep(p.part + (int64_t)(2 * me) * RT * ROW, done);
+        if (!mine && lane == 0) {
+            const int i = 2 * warp + (at == to);
+            given_s[i] = done;
+            has_s[i] = 1;
         }
-        __syncthreads();
-        const bool whole = j0 == 0 && j1 == tiles;
-        float* part = p.part + ((int64_t)blockIdx.x * 2 + (j0 == 0)) * RT * ROW;
-        auto store = [&](int row, int e4, float4 v) {
-            const int r = rt * RT + row, l = r / p.G;
-            const int64_t at = l * p.oL + (h * p.G + r - l * p.G) * p.oH + b * p.oB + e4;
-            if (e4 >= c.E) return;
-            if (p.out_f32) {
-                float* d = (float*)p.out + at;
-                if (p.out_whole) *reinterpret_cast<float4*>(d) = v;
-                else d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
-            } else {
-                __half* d = (__half*)p.out + at;
-                if (p.out_whole) *reinterpret_cast<uint2*>(d) = make_uint2(cf_pack(v.x, v.y), cf_pack(v.z, v.w));
-                else d[0] = __float2half_rn(v.x), d[1] = __float2half_rn(v.y), d[2] = __float2half_rn(v.z), d[3] = __float2half_rn(v.w);
-            }
-        };
-        for (int i = tid; i < rows * (EP / 4); i += CF_THREADS) {   // the warps of a row
+        __syncwarp();
+    }
+
+    // ---- the block's parts of pieces
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();   // the ring is free: every copy that was asked for has been waited for
+    float* rows_s = reinterpret_cast<float*>(cf_smem);
+    if (has_s[2 * warp + 1]) keep(rows_s + warp * RT * ROW, pc);
+    // A piece's last parts, one a block, from its first warp's block on; then perhaps the part that ended inside a warp's share.
+    if (tid < 2 * CF_WARPS && has_s[tid]) {
+        const CfPiece& q = given_s[tid];
+        const long long end = q.start + q.tiles;
+        auto holder = [&](long long u) { return (int)cf_div((u + 1) * warps - 1, total); };   // the warp that has tile u of the list
+        CfParts r;
+        r.w0 = holder(q.start);
+        r.w1 = holder(end - 1);
+        const bool inside = cf_div((r.w1 + 1) * total, warps) > end;
+        r.blocks = (r.w1 - (inside ? 1 : 0)) / CF_WARPS - r.w0 / CF_WARPS + 1;
+        r.count = r.blocks + (inside ? 1 : 0);
+        parts_s[tid] = r;
+    }
+    __syncthreads();
+    auto same = [&](int w) {   // warps w and w + 1 have the same last piece
+        return w + 1 < CF_WARPS && has_s[2 * w + 1] && has_s[2 * w + 3] && given_s[2 * w + 1].start == given_s[2 * w + 3].start;
+    };
+    for (int w = 0, end; w < CF_WARPS; w = end) {
+        end = w + 1;
+        while (same(end - 1)) ++end;
+        if (!has_s[2 * w + 1]) continue;
+        const CfPiece& q = given_s[2 * w + 1];
+        const bool all = parts_s[2 * w + 1].count == 1;
+        float* part = p.part + (int64_t)(2 * (blockIdx.x * CF_WARPS + w) + 1) * RT * ROW;
+        for (int i = tid; i < q.rows * (EP / 4); i += CF_THREADS) {
             const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
-            const float* src = reinterpret_cast<const float*>(cf_smem) + row * ROW;
+            const float* src = rows_s + row * ROW;
             float M = -INFINITY, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, src[w * RT * ROW + EP]);
+            for (int k = w; k < end; ++k) M = fmaxf(M, src[k * RT * ROW + EP]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < CF_WARPS; ++w) {
-                const float mw = src[w * RT * ROW + EP], f = mw == M ? 1.f : cf_ex2(mw - M);   // 1: both may be -inf, with zeros or a NaN
-                const float4 x = *reinterpret_cast<const float4*>(src + w * RT * ROW + e4);
+            for (int k = w; k < end; ++k) {
+                const float mw = src[k * RT * ROW + EP], f = mw == M ? 1.f : cf_ex2(mw - M);   // 1: both may be -inf, with zeros or a NaN
+                const float4 x = *reinterpret_cast<const float4*>(src + k * RT * ROW + e4);
                 v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
-                l = fmaf(src[w * RT * ROW + EP + 1], f, l);
+                l = fmaf(src[k * RT * ROW + EP + 1], f, l);
             }
-            if (whole) {
+            if (all) {
                 const float inv = l == 0.f ? 1.f : 1.f / l;
-                store(row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                store(q, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
             } else {
                 __stcg(reinterpret_cast<float4*>(part + row * ROW + e4), v);
                 if (e4 == 0) __stcg(reinterpret_cast<float2*>(part + row * ROW + EP), make_float2(M, l));
             }
         }
-        if (!whole) {   // whoever is last joins the parts, in block order
-            const int first = (int)(pstart / share), final = (int)((pstart + tiles - 1) / share);   // blocks that hold parts of this piece
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) last_s = atomicAdd(p.arrived + first, 1) == final - first;
-            __syncthreads();
-            if (last_s) {
-                __threadfence();
-                for (int i = tid; i < rows * (EP / 4); i += CF_THREADS) {
-                    const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
-                    float M = -INFINITY, l = 0.f;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    constexpr int AT_ONCE = 8;   // parts in flight: each is a trip to L2
-                    for (int k0 = first; k0 <= final; k0 += AT_ONCE) {
-                        float2 ml[AT_ONCE];
-                        float4 x[AT_ONCE];
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; ++k) {
-                            const int blk = k0 + k <= final ? k0 + k : final;
-                            const float* src = p.part + ((int64_t)blk * 2 + (blk == first)) * RT * ROW + row * ROW;
-                            ml[k] = __ldcg(reinterpret_cast<const float2*>(src + EP));
-                            x[k] = __ldcg(reinterpret_cast<const float4*>(src + e4));
-                        }
-                        float top = M;
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; ++k) top = fmaxf(top, ml[k].x);
-                        const float a = M == top ? 1.f : cf_ex2(M - top);
-                        v.x *= a, v.y *= a, v.z *= a, v.w *= a, l *= a;
-#pragma unroll
-                        for (int k = 0; k < AT_ONCE; ++k)
-                            if (k0 + k <= final) {
-                                const float f = ml[k].x == top ? 1.f : cf_ex2(ml[k].x - top);
-                                v.x = fmaf(x[k].x, f, v.x), v.y = fmaf(x[k].y, f, v.y), v.z = fmaf(x[k].z, f, v.z), v.w = fmaf(x[k].w, f, v.w);
-                                l = fmaf(ml[k].y, f, l);
-                            }
-                        M = top;
-                    }
-                    const float inv = l == 0.f ? 1.f : 1.f / l;
-                    store(row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-                }
-                if (tid == 0) p.arrived[first] = 0;
-            }
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid < 2 * CF_WARPS) {
+        join_s[tid] = 0;
+        if (has_s[tid] && (!(tid & 1) || tid == 1 || !same((tid >> 1) - 1))) {   // one of a group counts it
+            const CfParts r = parts_s[tid];
+            if (r.count > 1) join_s[tid] = atomicAdd(p.arrived + r.w0, 1) == r.count - 1;
         }
-        fence_proxy_async_smem();
-        __syncthreads();   // the ring may be filled again
-        at = pstart + j1;
+    }
+    __syncthreads();
+    for (int k = 0; k < 2 * CF_WARPS; ++k) {
+        if (!join_s[k]) continue;
+        __threadfence();
+        const CfPiece& q = given_s[k];
+        const CfParts r = parts_s[k];
+        auto part_of = [&](int i) {
+            const int w = r.w0 / CF_WARPS * CF_WARPS + i * CF_WARPS;
+            return p.part + (int64_t)(i == r.blocks ? 2 * r.w1 : 2 * (i == 0 ? r.w0 : w) + 1) * RT * ROW;
+        };
+        constexpr int AT_ONCE = 16;   // loads in flight: each is a trip to L2
+        if (r.count <= AT_ONCE) {
+            for (int i = tid; i < q.rows * (EP / 4); i += CF_THREADS) {
+                const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
+                float2 ml[AT_ONCE];
+                float4 x[AT_ONCE];
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    ml[u] = make_float2(-INFINITY, 0.f);
+                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (u < r.count) {
+                        const float* src = part_of(u) + row * ROW;
+                        ml[u] = __ldcg(reinterpret_cast<const float2*>(src + EP));
+                        x[u] = __ldcg(reinterpret_cast<const float4*>(src + e4));
+                    }
+                }
+                float M = -INFINITY, l = 0.f;
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) M = fmaxf(M, ml[u].x);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) {
+                    const float f = ml[u].x == M ? 1.f : cf_ex2(ml[u].x - M);
+                    v.x = fmaf(x[u].x, f, v.x), v.y = fmaf(x[u].y, f, v.y), v.z = fmaf(x[u].z, f, v.z), v.w = fmaf(x[u].w, f, v.w);
+                    l = fmaf(ml[u].y, f, l);
+                }
+                const float inv = l == 0.f ? 1.f : 1.f / l;
+                store(q, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+            }
+            if (tid == 0) p.arrived[r.w0] = 0;
+            continue;
+        }
+        // Rows' weights first, a part a lane: what is left is a sum whose loads wait for nothing.
+        float* weight = rows_s;       // [row][part]
+        for (int row = warp; row < q.rows; row += CF_WARPS) {
+            constexpr int KEPT = 4;   // a lane's first few are asked for once
+            float M = -INFINITY, l = 0.f;
+            float2 ml[KEPT];
+            auto load = [&](int i) { return __ldcg(reinterpret_cast<const float2*>(part_of(i) + row * ROW + EP)); };
+#pragma unroll
+            for (int u = 0; u < KEPT; ++u) ml[u] = lane + 32 * u < r.count ? load(lane + 32 * u) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int u = 0; u < KEPT; ++u) M = fmaxf(M, ml[u].x);
+            for (int i = lane + 32 * KEPT; i < r.count; i += 32) M = fmaxf(M, load(i).x);
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+            auto weigh = [&](int i, float2 v) {
+                const float f = v.x == M ? 1.f : cf_ex2(v.x - M);
+                weight[row * r.count + i] = f;
+                l = fmaf(v.y, f, l);
+            };
+#pragma unroll
+            for (int u = 0; u < KEPT; ++u)
+                if (lane + 32 * u < r.count) weigh(lane + 32 * u, ml[u]);
+            for (int i = lane + 32 * KEPT; i < r.count; i += 32) weigh(i, load(i));
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+            if (lane == 0) weight[q.rows * r.count + row] = l == 0.f ? 1.f : 1.f / l;
+        }
+        __syncthreads();
+        for (int i = tid; i < q.rows * (EP / 4); i += CF_THREADS) {
+            const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k0 = 0; k0 < r.count; k0 += AT_ONCE) {
+                float4 x[AT_ONCE];
+#pragma unroll
+                for (int i2 = 0; i2 < AT_ONCE; ++i2)
+                    x[i2] = k0 + i2 < r.count ? __ldcg(reinterpret_cast<const float4*>(part_of(k0 + i2) + row * ROW + e4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i2 = 0; i2 < AT_ONCE; ++i2) {
+                    const float f = k0 + i2 < r.count ? weight[row * r.count + k0 + i2] : 0.f;
+                    v.x = fmaf(x[i2].x, f, v.x), v.y = fmaf(x[i2].y, f, v.y), v.z = fmaf(x[i2].z, f, v.z), v.w = fmaf(x[i2].w, f, v.w);
+                }
+            }
+            const float inv = weight[q.rows * r.count + row];
+            store(q, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        }
+        if (tid == 0) p.arrived[r.w0] = 0;
+        __syncthreads();
     }
 }
 
@@ -580,15 +742,15 @@ static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
     // One resident wave at most, and no more blocks than there can be shares.
     int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
-    if (grid > GEMV_COUNTER_COUNT) grid = GEMV_COUNTER_COUNT;
-    const int64_t tiles = cdiv((int64_t)p.c.width * p.c.T, CF_TILE), rts = cdiv((int64_t)p.L * p.G, Cfg::RT);
-    const double most = (double)tiles * rts * p.c.H * p.B / CF_SHARE;
+    if (grid > Cfg::BLOCKS) grid = Cfg::BLOCKS;
+    const int64_t tiles = cdiv((int64_t)p.c.width * p.c.T, CF_KEYS), rts = cdiv((int64_t)p.L * p.G, Cfg::RT);
+    const double most = (double)tiles * rts * p.c.H * p.B / CF_WARPS;
     if (most + 1 < (double)grid) grid = (int64_t)most + 1;
     void* ws = nullptr;
-    rc = ws_scratch(ctx, (size_t)grid * 2 * Cfg::RT * Cfg::ROW * sizeof(float), &ws);
+    rc = ws_scratch(ctx, (size_t)grid * CF_WARPS * 2 * Cfg::RT * Cfg::ROW * sizeof(float), &ws);
     if (rc) return rc;
     p.part = static_cast<float*>(ws);
-    p.arrived = ctx->sk_flags + SK_FLAG_COUNT;
+    p.arrived = ctx->sk_flags;
     B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(CF_THREADS), Cfg::SMEM, ctx->stream, 1, mk, mv, p));
     ctx->launches++;
     return B200_OK;
