@@ -54,6 +54,10 @@ constexpr int CACHE_MOST_T = 128;
 // Checks what the host can see; fills `out`.
 int cache_view(b200_ctx* ctx, const b200_cache8* c, const char* op, CacheView* out);
 
+// Attention of many query rows a key head (cache8_prompt.cu); what cache_view checks has been checked, and the operands too.
+int cache_prompt_run(b200_ctx* ctx, const CacheView& c, int64_t L, int64_t B, int64_t G, const b200_strided4* q, const b200_strided4* out,
+                     int out_dtype, float scale, bool fp8, int causal, const int32_t* lens, const int32_t* news);
+
 template <bool FP8> __device__ __forceinline__ constexpr float cache_top() { return FP8 ? 448.f : 127.f; }
 
 // Four 8-bit values as fp16, exactly: (0, 1) and (2, 3).  A byte u under 0x64 is the fp16 number 1024 + u.

@@ -27,6 +27,9 @@
 
 namespace b200 {
 
+#ifndef CF_MOST_ROWS
+#define CF_MOST_ROWS 64
+#endif
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
 constexpr int CF_KEYS = 64;                      // keys a warp takes at a time: a tile of the list
@@ -789,6 +792,7 @@ int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int
     const bool fp8 = cache->kind == B200_E4M3;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634 / (fp8 ? 448.0 : 127.0));
     B200_CUDA(cudaSetDevice(ctx->device));
+    if ((int64_t)p.L * p.G > CF_MOST_ROWS) return cache_prompt_run(ctx, p.c, L, B, p.G, q, out, out_dtype, scale, fp8, causal, lens, news);
     if (p.L * p.G <= 8) {
         if (p.c.E <= 64) return fp8 ? cf_launch<64, true, 1>(ctx, p) : cf_launch<64, false, 1>(ctx, p);
         return fp8 ? cf_launch<128, true, 1>(ctx, p) : cf_launch<128, false, 1>(ctx, p);

@@ -1,0 +1,649 @@
+// Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
+// cache8_attention.cu.
+//
+// Tensor-bound: 4 E flops a row and visible key.  The query rows of a key head (the heads that share it, times the new tokens)
+// are stacked; a block owns two tiles of 128 of them and walks its keys in blocks of 128: S = Q K^T and O += P V on tcgen05 with
+// S, P and O in tensor memory.  The 8-bit operands become fp16 on the way to shared memory, exactly, once for 256 rows: four warps
+// read them from the pages into registers a side ahead and write them in the 128-byte swizzle.  No operand carries a scale: a
+// page's key scale (and the softmax's own) is the factor of its columns' exponents, its value scale, relative to the largest so
+// far, a summand of them; the row sum takes that back a group of 16 keys at a time.
+//
+//   warps 0-3  softmax of tile 0, warps 4-7 of tile 1: one thread a row, the row's 128 scores in registers
+//   warps 8-11 fetch and convert: K(j), V(j), K(j+1), ...
+//   warps 12, 13  issue one tile's products each:  Q K(j)',  P(j) V(j), Q K(j+1)', ...; P lies over the first half of S
+//   warp 14    looks up pages and scales and lays out each block's constants, two blocks ahead
+#include <cuda_fp16.h>
+
+#include "cache8.cuh"
+
+namespace b200 {
+
+constexpr int CP_THREADS = 512;
+constexpr int CP_ROWS = 128, CP_KEYS = 128;     // of a tile
+constexpr int CP_ATOM = 128 * 128;              // 128 rows x 64 fp16
+constexpr int CP_SCALES = 4;                    // blocks of constants in flight
+constexpr int CP_SOFTMAX_REGS = 184, CP_CONVERT_REGS = 96, CP_OTHER_REGS = 40;
+static_assert(2 * 128 * CP_SOFTMAX_REGS + 128 * CP_CONVERT_REGS + 128 * CP_OTHER_REGS <= CP_THREADS * 128, "what the launch holds");
+
+struct CpScales {              // of one block of keys, a group of 16 keys an entry
+    float key[8];              // score to exponent; 0 where the group has no page
+    float value[8];            // added to the exponent: log2 of 2^7 times the value scale over the reference
+    float back[8];             // an exponential of the group back to a weight
+    float change, reference;   // the reference before over the reference now; the reference
+    int hidden;                // bit g: the group has no page
+};
+
+template <int EP> struct CpCfg {
+    static constexpr int ATOMS = EP / 64;
+    static constexpr int SIDE = ATOMS * CP_ATOM;                 // an operand tile
+    static constexpr int STAGES = 2;
+    static constexpr int S_Q = 0, S_K = 2 * SIDE, S_V = S_K + STAGES * SIDE, S_C = S_V + STAGES * SIDE;
+    static constexpr int S_BARS = S_C + (CP_SCALES * (int)sizeof(CpScales) + 15) / 16 * 16;
+    static constexpr int BARRIERS = 2 + 4 * STAGES + 2 * 5 + 2 * CP_SCALES;
+    static constexpr int SMEM = S_BARS + (BARRIERS + 1) * 8;
+    static constexpr int O_COL = 2 * CP_KEYS;
+};
+
+struct CachePromptParams {
+    CacheView c;
+    const __half* q;
+    void* out;
+    int64_t qL, qH, qB, oL, oH, oB;
+    const int32_t *lens, *news;
+    int L, B, G;
+    int causal, out_f32, whole, out_whole;
+    float scale_log2;         // without its sign, which goes onto Q
+    int negate;
+    int items, nsplit;        // row pairs x heads x sequences; parts that an item's keys are cut into
+    float* part;              // [split][item][256 rows][EP], then [split][item][256][2]: reference point, sum
+    float* part_ml;
+};
+
+__device__ __forceinline__ float cp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float cp_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void cp_tmem_st16(uint32_t taddr, const uint32_t* r) {
+    uint32_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = r[i];
+    tmem_st16(taddr, v);
+}
+// four results of a row, 16 bytes of fp16 or two of fp32 at a time where rows allow it
+__device__ __forceinline__ void cp_store8(const CachePromptParams& p, int64_t at, const float (&v)[8]) {
+    if (p.out_f32) {
+        float* d = (float*)p.out + at;
+        if (p.out_whole) {
+            reinterpret_cast<float4*>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = v[i];
+        }
+    } else {
+        __half* d = (__half*)p.out + at;
+        if (p.out_whole) {
+            uint4 w;
+            __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            *reinterpret_cast<uint4*>(d) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = __float2half_rn(v[i]);
+        }
+    }
+}
+
+// What the rows of an item see: item -> (row pair, head, sequence), later rows, whose keys are more, first.
+struct CpItem {
+    int b, h, r0, rows, n, m, blocks;   // first row, rows of the sequence (all of its heads), length, new tokens, blocks of keys
+};
+__device__ __forceinline__ CpItem cp_item(const CachePromptParams& p, int item) {
+    CpItem it;
+    const int pairs = (p.L * p.G + 2 * CP_ROWS - 1) / (2 * CP_ROWS), hb = p.c.H * p.B;
+    const int rp = pairs - 1 - item / hb, rest = item % hb;
+    it.h = rest % p.c.H;
+    it.b = rest / p.c.H;
+    it.r0 = rp * 2 * CP_ROWS;
+    it.n = p.c.tokens(it.b, p.lens);
+    it.m = p.c.fresh(it.b, p.news, p.L);
+    it.rows = it.m * p.G;
+    const int top = it.r0 + 2 * CP_ROWS < it.rows ? it.r0 + 2 * CP_ROWS : it.rows;
+    int seen = p.causal && top > 0 ? it.n - it.m + (top - 1) / p.G + 1 : it.n;   // keys that some row sees
+    if (seen < 0) seen = 0;
+    it.blocks = (seen + CP_KEYS - 1) / CP_KEYS;
+    return it;
+}
+
+template <int EP, bool FP8>
+__global__ void __launch_bounds__(CP_THREADS, 1)
+cache_prompt_kernel(const CachePromptParams p) {
+    using Cfg = CpCfg<EP>;
+    constexpr int STAGES = Cfg::STAGES;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const CacheView& c = p.c;
+    if ((smem_u32(smem) & 1023u) != 0) {   // uniform across the grid
+        if (threadIdx.x == 0) atomicCAS(c.d_status, 0, KST_SMEM_LAYOUT);
+        return;
+    }
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::S_BARS);
+    uint64_t* q_full = bars;                       // [2] four softmax warps
+    uint64_t* k_full = q_full + 2;                 // [STAGES] four converting warps
+    uint64_t* k_empty = k_full + STAGES;           // one arrival a tile
+    uint64_t* v_full = k_empty + STAGES;
+    uint64_t* v_empty = v_full + STAGES;
+    uint64_t* s_full = v_empty + STAGES;           // [2] a tile's scores are there
+    uint64_t* p_half = s_full + 2;                 // [2] half of its P
+    uint64_t* p_full = p_half + 2;                 // [2] all of it
+    uint64_t* pv_done = p_full + 2;                // [2] its last product
+    uint64_t* exp_turn = pv_done + 2;              // [2] whose turn it is to run its exponentials
+    uint64_t* c_full = exp_turn + 2;                 // [CP_SCALES] a block's constants
+    uint64_t* c_empty = c_full + CP_SCALES;        // four softmax warps a tile
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_empty + CP_SCALES);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    CpScales* consts = reinterpret_cast<CpScales*>(smem + Cfg::S_C);
+    static_assert(Cfg::BARRIERS == 2 + 4 * STAGES + 10 + 2 * CP_SCALES, "barriers counted by the layout");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    grid_dep_wait();          // the lengths may come from the launch before
+    grid_dep_launch();
+    const int split = blockIdx.x % p.nsplit, item = blockIdx.x / p.nsplit;
+    const CpItem it = cp_item(p, item);
+    if (it.r0 >= it.rows) return;                  // uniform: before any barrier or tensor memory exists
+    const int j_begin = (int)((int64_t)split * it.blocks / p.nsplit), nblk = (int)((int64_t)(split + 1) * it.blocks / p.nsplit) - j_begin;
+    const int ntiles = it.r0 + CP_ROWS < it.rows ? 2 : 1;
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 4);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_half[t], 4);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&pv_done[t], 1);
+            mbar_init(&exp_turn[t], 4);
+        }
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&k_full[s], 4);
+            mbar_init(&k_empty[s], ntiles);
+            mbar_init(&v_full[s], 4);
+            mbar_init(&v_empty[s], ntiles);
+        }
+        for (int s = 0; s < CP_SCALES; ++s) {
+            mbar_init(&c_full[s], 1);
+            mbar_init(&c_empty[s], 4 * ntiles);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 15) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_OTHER_REGS));
+        if (warp == 14) {
+            // -------------------------------------------------- pages and scales of the blocks
+            float ref = 0.f;
+            auto page = [&](int j) {
+                const int key = (j_begin + j) * CP_KEYS + (lane & 7) * 16;
+                return j < nblk && key < it.n ? (int)c.page(it.b, key >> c.logT) : -1;
+            };
+            int pg = page(0), pg1 = page(1);
+            float k0 = 0.f, v0 = 0.f;
+            auto load = [&](int q, float& k, float& v) {
+                k = q >= 0 ? __ldg(c.kmax + (int64_t)q * c.H + it.h) : 0.f;
+                v = q >= 0 ? __ldg(c.vmax + (int64_t)q * c.H + it.h) : 0.f;
+            };
+            load(pg, k0, v0);
+            for (int j = 0; j < nblk; ++j) {
+                const int pg2 = page(j + 2);
+                float k1, v1;
+                load(pg1, k1, v1);
+                const int s = j % CP_SCALES;
+                if (!mbar_wait(&c_empty[s], (uint32_t)((j / CP_SCALES) & 1) ^ 1, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
+                float most = v0 < INFINITY ? v0 : 0.f;
+#pragma unroll
+                for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                const float was = ref;
+                if (most > ref) ref = 1.5f * most;
+                // a scale far below the reference, whose P is zero in fp16, keeps an exponent of its own so that the sum can take it back
+                float f = ref > 0x1p-100f ? v0 / ref : 1.f;
+                if (f < 0x1p-40f) f = 0x1p-40f;
+                const unsigned hidden = __ballot_sync(0xffffffffu, pg < 0) & 255u;
+                if (lane < 8) {
+                    consts[s].key[lane] = k0 * p.scale_log2;
+                    consts[s].value[lane] = log2f(f) + 7.f;
+                    consts[s].back[lane] = 0x1p-7f / f;
+                }
+                if (lane == 0) {
+                    consts[s].change = was == ref ? 1.f : was / ref;
+                    consts[s].reference = ref;
+                    consts[s].hidden = (int)hidden;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c_full[s]);
+                pg = pg1, pg1 = pg2, k0 = k1, v0 = v1;
+            }
+        } else if (warp < 14 && warp - 12 < ntiles) {
+            // -------------------------------------------------- issuers: the whole warp waits, one thread issues
+            const int t = warp - 12;
+            constexpr uint32_t idesc_s = make_idesc_f16(CP_ROWS, CP_KEYS, 0, 0);
+            constexpr uint32_t idesc_o = make_idesc_f16(CP_ROWS, EP, 0, 1);
+            constexpr uint64_t kdesc0 = make_smem_desc(16, 1024);
+            constexpr uint64_t vdesc0 = make_smem_desc(CP_ATOM, 1024);
+            const uint32_t q_addr = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE);
+            const uint32_t s_tmem = tmem_base + t * CP_KEYS, o_tmem = tmem_base + Cfg::O_COL + t * EP;
+            auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, c.d_status, code, abort_flag));
+            };
+            auto issue_qk = [&](int j) -> bool {
+                const int sk = j % STAGES;
+                if (!wait(&k_full[sk], (uint32_t)((j / STAGES) & 1), KST_WAIT_FULL)) return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t k_addr = smem_u32(smem + Cfg::S_K + sk * Cfg::SIDE);
+#pragma unroll
+                    for (int k = 0; k < EP / 16; ++k) {
+                        if (k * 16 >= c.E) break;
+                        const uint32_t in = (uint32_t)(k >> 2) * CP_ATOM + (uint32_t)(k & 3) * 32;
+                        umma_ss(s_tmem, smem_desc_at(kdesc0, q_addr + in), smem_desc_at(kdesc0, k_addr + in), idesc_s, k != 0);
+                    }
+                    umma_commit(&s_full[t]);
+                    umma_commit(&k_empty[sk]);
+                }
+                __syncwarp();
+                return true;
+            };
+            auto issue_pv = [&](int j, int sv, int k0, int k1) {
+                const uint32_t v_addr = smem_u32(smem + Cfg::S_V + sv * Cfg::SIDE);
+#pragma unroll
+                for (int k = k0; k < k1; ++k)
+                    umma_ts(o_tmem, s_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
+            };
+            bool ok = wait(&q_full[t], 0, KST_WAIT_FULL);
+            if (ok && nblk > 0) ok = issue_qk(0);
+            for (int j = 0; ok && j < nblk; ++j) {
+                const int sv = j % STAGES;
+                if (!wait(&v_full[sv], (uint32_t)((j / STAGES) & 1), KST_WAIT_FULL)) break;
+                if (!wait(&p_half[t], (uint32_t)(j & 1), KST_WAIT_SOFTMAX)) break;
+                tc_fence_after();
+                if (elect_one()) issue_pv(j, sv, 0, 4);
+                __syncwarp();
+                if (!wait(&p_full[t], (uint32_t)(j & 1), KST_WAIT_SOFTMAX)) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    issue_pv(j, sv, 4, 8);
+                    umma_commit(&pv_done[t]);
+                    umma_commit(&v_empty[sv]);
+                }
+                __syncwarp();
+                if (j + 1 < nblk && !issue_qk(j + 1)) break;   // over P(j): after the product that reads it, in issue order
+            }
+        }
+    } else if (warp >= 8) {
+        // ------------------------------------------------------ 8 bits to fp16, in the swizzle
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_CONVERT_REGS));
+        const int w = warp - 8, ch = lane & 7, sub = lane >> 3;   // keys 32 w + 4 i + sub of a block, elements 16 ch on
+        const bool mine = ch * 16 < c.E;
+        int page0 = -1, page1 = -1;
+        auto look = [&](int j) {
+            const int key = (j_begin + j) * CP_KEYS + w * 32;
+            page0 = page1 = -1;
+            if (j < nblk && key < it.n) {
+                page0 = (int)c.page(it.b, key >> c.logT);
+                page1 = c.T > 16 ? page0 : key + 16 < it.n ? (int)c.page(it.b, (key >> 4) + 1) : -1;
+            }
+        };
+        uint4 cur[8];
+        auto fetch = [&](int j, int side) {   // zeros where there is no key: what P = 0 multiplies is a number
+            const int key0 = (j_begin + j) * CP_KEYS + w * 32 + sub;
+            const uint8_t* base = (side ? c.v : c.k) + it.h * (side ? c.vH : c.kH) + ch * 16;
+            const int64_t sT = side ? c.vT : c.kT, sP = side ? c.vP : c.kP;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = key0 + 4 * i, page = i < 4 ? page0 : page1;
+                cur[i] = make_uint4(0, 0, 0, 0);
+                if (mine && page >= 0 && key < it.n && j < nblk) cur[i] = __ldg(reinterpret_cast<const uint4*>(base + page * sP + (key & (c.T - 1)) * sT));
+            }
+        };
+        auto write = [&](uint32_t tile, bool values) {
+            const uint32_t at = tile + (uint32_t)(ch >> 2) * CP_ATOM;
+            const int first = ch >> 2;       // lanes of the second atom write their second chunk first: a phase's eight lanes meet all banks
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = w * 32 + 4 * i + sub;
+                const uint32_t v[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    cache_halves<FP8>(v[k], h[2 * k], h[2 * k + 1]);
+                    if (FP8 && values) {     // the code of a NaN reads as 448: a row that may not see it must not meet it
+                        const __half2 most = __half2half2(__ushort_as_half(0x5f00));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const __half2 x = __hmin2(*reinterpret_cast<__half2*>(&h[2 * k + u]), most);
+                            h[2 * k + u] = *reinterpret_cast<const uint32_t*>(&x);
+                        }
+                    }
+                }
+                const uint32_t line = at + row * 128;
+                const int c0 = 2 * (ch & 3);
+                const uint32_t a0 = line + (((c0 + first) ^ (row & 7)) << 4), a1 = line + (((c0 + 1 - first) ^ (row & 7)) << 4);
+                uint32_t x[4], y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[k] = first ? h[4 + k] : h[k];
+                    y[k] = first ? h[k] : h[4 + k];
+                }
+                if (ch < EP / 16) {
+                    st_shared_v4(a0, x);
+                    st_shared_v4(a1, y);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+        };
+        look(0);
+        fetch(0, 0);
+        for (int j = 0; j < nblk; ++j) {
+            const int s = j % STAGES;
+            const uint32_t ph = (uint32_t)((j / STAGES) & 1) ^ 1;
+            if (!mbar_wait(&k_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
+            write(smem_u32(smem + Cfg::S_K + s * Cfg::SIDE), false);
+            if (lane == 0) mbar_arrive(&k_full[s]);
+            fetch(j, 1);
+            look(j + 1);
+            if (!mbar_wait(&v_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
+            write(smem_u32(smem + Cfg::S_V + s * Cfg::SIDE), true);
+            if (lane == 0) mbar_arrive(&v_full[s]);
+            fetch(j + 1, 0);
+        }
+    } else {
+        // ------------------------------------------------------ softmax and results
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CP_SOFTMAX_REGS));
+        const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        if (t < ntiles) {
+            const int r = it.r0 + t * CP_ROWS + row, l = r / p.G, hq = it.h * p.G + r - l * p.G;   // new token, query head
+            const bool live = r < it.rows;
+            {
+                const __half* q = p.q + l * p.qL + hq * p.qH + it.b * p.qB;
+                const uint32_t dst = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE) + row * 128, sign = p.negate ? 0x80008000u : 0u;
+#pragma unroll 4
+                for (int ch = 0; ch < EP / 8; ++ch) {
+                    uint32_t v[4] = {0, 0, 0, 0};
+                    if (live && ch * 8 < c.E) {
+                        if (p.whole) {
+                            const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + ch * 8));
+                            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+                        } else {
+                            const unsigned short* u = reinterpret_cast<const unsigned short*>(q + ch * 8);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] ^= sign;
+                    }
+                    st_shared_v4(dst + (uint32_t)(ch >> 3) * CP_ATOM + (((ch & 7) ^ (row & 7)) << 4), v);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[t]);
+            }
+            const uint32_t lane_base = uint32_t(quad * 32) << 16;
+            const uint32_t s_tmem = tmem_base + lane_base + t * CP_KEYS, o_tmem = tmem_base + lane_base + Cfg::O_COL + t * EP;
+            const int last = p.causal ? it.n - it.m + l : it.n - 1;                       // the last key this row sees
+            const int all_see = p.causal ? it.n - it.m + (it.r0 + t * CP_ROWS) / p.G : it.n - 1;   // that every row of the tile sees
+            float m_run = -INFINITY, l_run = 0.f, ref = 0.f;
+            bool ok = true;
+            const bool pingpong = ntiles == 2;
+            for (int j = 0; ok && j < nblk; ++j) {
+                const int cs = j % CP_SCALES, key0 = (j_begin + j) * CP_KEYS;
+                if (!mbar_wait(&c_full[cs], (uint32_t)((j / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag)) { ok = false; break; }
+                const CpScales& k = consts[cs];
+                if (!mbar_wait(&s_full[t], (uint32_t)(j & 1), c.d_status, KST_WAIT_TMEM_FULL, abort_flag)) { ok = false; break; }
+                __syncwarp();
+                tc_fence_after();
+                uint32_t x[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(s_tmem + i * 32, x[i]);
+                const int hidden = k.hidden;
+                const bool masked = key0 + CP_KEYS - 1 > all_see || hidden != 0;
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) asm volatile("" : "+r"(x[i][u]));   // in registers from here on
+                if (masked) {
+                    const int seen = last - key0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 32; ++u)
+                            if (i * 32 + u > seen || (hidden >> (i * 2 + u / 16) & 1)) x[i][u] = 0xff800000u;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int gq = 0; gq < 8; ++gq) {
+                    const uint32_t* y = &x[gq >> 1][(gq & 1) * 16];
+                    float a = __uint_as_float(y[0]), b2 = __uint_as_float(y[1]);
+#pragma unroll
+                    for (int u = 2; u < 16; u += 4) {
+                        a = cp_max3(a, __uint_as_float(y[u]), __uint_as_float(y[u + 1]));
+                        if (u + 2 < 16) b2 = cp_max3(b2, __uint_as_float(y[u + 2]), __uint_as_float(y[u + 3]));
+                    }
+                    top = fmaxf(top, fmaxf(a, b2) * k.key[gq]);   // -inf times 0 is no number, which a maximum passes over
+                }
+                // the reference point follows lazily: only when the maximum has grown by more than 2^8
+                const float m_new = top > m_run + 8.f ? top : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new;
+                const float change = k.change;
+                if (__any_sync(0xffffffffu, m_new != m_run) || change != 1.f) {
+                    const float alpha = m_run == m_new ? 1.f : cp_ex2(m_run - m_new);
+                    l_run *= alpha;
+                    if (j > 0) {          // these scores were issued after the last P V: it is done
+                        const float f = alpha * change;
+#pragma unroll 1
+                        for (int i = 0; i < EP / 16; ++i) {
+                            uint32_t o16[16];
+                            tmem_ld16(o_tmem + i * 16, o16);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) o16[u] = __float_as_uint(__uint_as_float(o16[u]) * f);
+                            tmem_st16(o_tmem + i * 16, o16);
+                        }
+                        tmem_wait_st();
+                    }
+                    m_run = m_new;
+                }
+                if (pingpong && (t == 1 || j > 0) &&
+                    !mbar_wait(&exp_turn[t], (uint32_t)((t == 1 ? j : j - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag)) { ok = false; break; }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int g2 = 0; g2 < 2; ++g2) {
+                        const float kf = k.key[2 * i + g2], add = k.value[2 * i + g2] - m_sub;
+                        const uint64_t k2 = pack2(kf, kf), a2 = pack2(add, add);
+                        uint64_t sum = pack2(0.f, 0.f);
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const uint32_t u0 = x[i][g2 * 16 + 2 * u], u1 = x[i][g2 * 16 + 2 * u + 1];
+                            float e0, e1;
+                            unpack2(fma2(pack2(__uint_as_float(u0), __uint_as_float(u1)), k2, a2), e0, e1);
+                            e0 = cp_ex2(e0), e1 = cp_ex2(e1);
+                            if (masked) {
+                                if (u0 == 0xff800000u) e0 = 0.f;
+                                if (u1 == 0xff800000u) e1 = 0.f;
+                            }
+                            sum = add2(sum, pack2(e0, e1));
+                            const __half2 h2 = __floats2half2_rn(e0, e1);
+                            pk[g2 * 8 + u] = *reinterpret_cast<const uint32_t*>(&h2);
+                        }
+                        float s0, s1;
+                        unpack2(sum, s0, s1);
+                        l_run = fmaf(s0 + s1, k.back[2 * i + g2], l_run);
+                    }
+                    cp_tmem_st16(s_tmem + i * 16, pk);
+                    if (i == 1) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_half[t]);
+                    }
+                }
+                if (pingpong) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&exp_turn[1 - t]);
+                }
+                ref = k.reference;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&p_full[t]);
+                    mbar_arrive(&c_empty[cs]);
+                }
+            }
+            if (ok && nblk > 0) ok = mbar_wait(&pv_done[t], (uint32_t)((nblk - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag);
+            __syncwarp();
+            if (ok) {
+                tc_fence_after();
+                const float back = ref * 0x1p-7f / cache_top<FP8>();
+                const float f = p.nsplit > 1 ? back : back / (l_run == 0.f ? 1.f : l_run);
+                const int64_t at = l * p.oL + hq * p.oH + it.b * p.oB;
+                const int64_t prow = ((int64_t)split * p.items + item) * 2 * CP_ROWS + t * CP_ROWS + row;
+#pragma unroll 1
+                for (int i = 0; i < EP / 16; ++i) {
+                    uint32_t o16[16];
+                    __syncwarp();
+                    if (nblk > 0) {
+                        tmem_ld16(o_tmem + i * 16, o16);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) o16[u] = 0;
+                    }
+                    if (!live || i * 16 >= c.E) continue;
+                    float v[2][8];
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) v[u >> 3][u & 7] = __uint_as_float(o16[u]) * f;
+                    if (p.nsplit > 1) {
+                        float4* d = reinterpret_cast<float4*>(p.part + prow * EP + i * 16);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) d[u] = make_float4(v[u >> 1][(u & 1) * 4], v[u >> 1][(u & 1) * 4 + 1], v[u >> 1][(u & 1) * 4 + 2], v[u >> 1][(u & 1) * 4 + 3]);
+                    } else {
+                        cp_store8(p, at + i * 16, v[0]);
+                        cp_store8(p, at + i * 16 + 8, v[1]);
+                    }
+                }
+                if (live && p.nsplit > 1) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
+            }
+        }
+    }
+    if (*abort_flag) {
+        for (int i = 0; i < 4; ++i) __nanosleep(1000000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 15) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// The parts of an item's keys, in order: eight elements a thread.
+template <int EP>
+__global__ void __launch_bounds__(256)
+cache_prompt_join_kernel(const CachePromptParams p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, prow = i / (EP / 8), rows = (int64_t)p.items * 2 * CP_ROWS;
+    const int e = (int)(i % (EP / 8)) * 8;
+    if (prow >= rows || e >= p.c.E) return;
+    const CpItem it = cp_item(p, (int)(prow / (2 * CP_ROWS)));
+    const int r = it.r0 + (int)(prow % (2 * CP_ROWS));
+    if (r >= it.rows) return;
+    const int l = r / p.G, hq = it.h * p.G + r - l * p.G;
+    float M = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, p.part_ml[(s * rows + prow) * 2]);
+    for (int s = 0; s < p.nsplit; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + prow) * 2);
+        const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
+        const float4* x = reinterpret_cast<const float4*>(p.part + (s * rows + prow) * EP + e);
+        const float4 a = x[0], b = x[1];
+        sum = fmaf(ml.y, f, sum);
+        v[0] = fmaf(a.x, f, v[0]), v[1] = fmaf(a.y, f, v[1]), v[2] = fmaf(a.z, f, v[2]), v[3] = fmaf(a.w, f, v[3]);
+        v[4] = fmaf(b.x, f, v[4]), v[5] = fmaf(b.y, f, v[5]), v[6] = fmaf(b.z, f, v[6]), v[7] = fmaf(b.w, f, v[7]);
+    }
+    const float inv = sum == 0.f ? 1.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= inv;
+    cp_store8(p, l * p.oL + hq * p.oH + it.b * p.oB + e, v);
+}
+
+template <int EP, bool FP8>
+static int cp_launch(b200_ctx* ctx, CachePromptParams& p) {
+    using Cfg = CpCfg<EP>;
+    auto kern = cache_prompt_kernel<EP, FP8>;
+    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    const int64_t sms = ctx->prop.multiProcessorCount;
+    const int64_t items = cdiv((int64_t)p.L * p.G, 2 * CP_ROWS) * p.c.H * p.B;
+    B200_REQUIRE(items < (1ll << 24), B200_DECLINE_EXTENT, "cache_attention: %lld row tiles", (long long)items);
+    // Fewer items than SMs: their keys are cut so that every SM has a part, four blocks of keys at least.
+    const int64_t blocks = cdiv((int64_t)p.c.width * p.c.T, CP_KEYS);
+    int64_t nsplit = sms / items;
+    if (nsplit > blocks / 4) nsplit = blocks / 4;
+    if (nsplit > 64) nsplit = 64;
+    if (nsplit < 1) nsplit = 1;
+    p.items = (int)items;
+    p.nsplit = (int)nsplit;
+    if (nsplit > 1) {
+        void* ws = nullptr;
+        const size_t rows = (size_t)nsplit * items * 2 * CP_ROWS;
+        int rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float), &ws);
+        if (rc) return rc;
+        p.part = static_cast<float*>(ws);
+        p.part_ml = p.part + rows * EP;
+    }
+    B200_CUDA(launch_dep(kern, dim3((unsigned)(items * nsplit)), dim3(CP_THREADS), Cfg::SMEM, ctx->stream, 1, p));
+    ctx->launches++;
+    if (nsplit > 1) {
+        B200_CUDA(launch_dep(cache_prompt_join_kernel<EP>, dim3((unsigned)cdiv(items * 2 * CP_ROWS * (EP / 8), 256)), dim3(256), 0, ctx->stream, 1, p));
+        ctx->launches++;
+    }
+    return B200_OK;
+}
+
+int cache_prompt_run(b200_ctx* ctx, const CacheView& c, int64_t L, int64_t B, int64_t G, const b200_strided4* q, const b200_strided4* out,
+                     int out_dtype, float scale, bool fp8, int causal, const int32_t* lens, const int32_t* news) {
+    CachePromptParams p = {};
+    p.c = c;
+    p.q = (const __half*)q->ptr;
+    p.qL = q->stride[1], p.qH = q->stride[2], p.qB = q->stride[3];
+    p.out = const_cast<void*>(out->ptr);
+    p.oL = out->stride[1], p.oH = out->stride[2], p.oB = out->stride[3];
+    p.lens = lens, p.news = news;
+    p.L = (int)L, p.B = (int)B, p.G = (int)G;
+    p.causal = causal, p.out_f32 = out_dtype == B200_F32;
+    p.whole = ((uintptr_t)q->ptr % 16 | (uint64_t)q->stride[1] % 8 | (uint64_t)q->stride[2] % 8 | (uint64_t)q->stride[3] % 8) == 0;
+    const int64_t size = p.out_f32 ? 4 : 2;
+    p.out_whole = ((uintptr_t)out->ptr | (uint64_t)(out->stride[1] * size) | (uint64_t)(out->stride[2] * size) | (uint64_t)(out->stride[3] * size)) % 16 == 0;
+    p.negate = scale < 0.f;
+    p.scale_log2 = (float)(fabs((double)scale) * 1.4426950408889634 / (fp8 ? 448.0 : 127.0));
+    if (c.E <= 64) return fp8 ? cp_launch<64, true>(ctx, p) : cp_launch<64, false>(ctx, p);
+    return fp8 ? cp_launch<128, true>(ctx, p) : cp_launch<128, false>(ctx, p);
+}
+
+} // namespace b200
