@@ -26,11 +26,11 @@ constexpr int CP_SOFTMAX_REGS = 184, CP_CONVERT_REGS = 96, CP_OTHER_REGS = 40;
 static_assert(2 * 128 * CP_SOFTMAX_REGS + 128 * CP_CONVERT_REGS + 128 * CP_OTHER_REGS <= CP_THREADS * 128, "what the launch holds");
 
 struct CpScales {              // of one block of keys, a group of 16 keys an entry
-    float key[8];              // score to exponent; 0 where the group has no page
+    float key[8];              // score to exponent: finite and above 0, so that a hidden score of -inf stays that
     float value[8];            // added to the exponent: log2 of 2^7 times the value scale over the reference
     float back[8];             // an exponential of the group back to a weight
     float change, reference;   // the reference before over the reference now; the reference
-    int hidden;                // bit g: the group has no page
+    int hidden, odd;           // bit g: the group has no page; one of its scales is not finite
 };
 
 template <int EP> struct CpCfg {
@@ -126,7 +126,7 @@ template <int EP, bool FP8>
 __global__ void __launch_bounds__(CP_THREADS, 1)
 cache_prompt_kernel(const CachePromptParams p) {
     using Cfg = CpCfg<EP>;
-    constexpr int STAGES = Cfg::STAGES;
+    constexpr int STAGES = Cfg::STAGES, ATOMS = Cfg::ATOMS;
     extern __shared__ __align__(1024) uint8_t smem[];
     const CacheView& c = p.c;
     if ((smem_u32(smem) & 1023u) != 0) {   // uniform across the grid
@@ -221,16 +221,19 @@ cache_prompt_kernel(const CachePromptParams p) {
                 // a scale far below the reference, whose P is zero in fp16, keeps an exponent of its own so that the sum can take it back
                 float f = ref > 0x1p-100f ? v0 / ref : 1.f;
                 if (f < 0x1p-40f) f = 0x1p-40f;
-                const unsigned hidden = __ballot_sync(0xffffffffu, pg < 0) & 255u;
+                const float kf = k0 * p.scale_log2;
+                const bool strange = !(kf < INFINITY) || !(v0 < INFINITY);
+                const unsigned hidden = __ballot_sync(0xffffffffu, pg < 0) & 255u, odd = __ballot_sync(0xffffffffu, strange) & 255u;
                 if (lane < 8) {
-                    consts[s].key[lane] = k0 * p.scale_log2;
-                    consts[s].value[lane] = log2f(f) + 7.f;
-                    consts[s].back[lane] = 0x1p-7f / f;
+                    consts[s].key[lane] = strange ? 1.f : fmaxf(kf, 0x1p-100f);   // a page of zeros: its scores are zeros whatever the factor
+                    consts[s].value[lane] = strange ? 7.f : log2f(f) + 7.f;
+                    consts[s].back[lane] = strange ? 0x1p-7f : 0x1p-7f / f;
                 }
                 if (lane == 0) {
                     consts[s].change = was == ref ? 1.f : was / ref;
                     consts[s].reference = ref;
                     consts[s].hidden = (int)hidden;
+                    consts[s].odd = (int)odd;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c_full[s]);
@@ -295,9 +298,11 @@ cache_prompt_kernel(const CachePromptParams p) {
     } else if (warp >= 8) {
         // ------------------------------------------------------ 8 bits to fp16, in the swizzle
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_CONVERT_REGS));
-        const int w = warp - 8, ch = lane & 7, sub = lane >> 3;   // keys 32 w + 4 i + sub of a block, elements 16 ch on
-        const bool mine = ch * 16 < c.E;
-        int page0 = -1, page1 = -1;
+        // Lane (sub, ch) of a warp has keys 32 w + 8 i + sub of a block and elements 64 a + 16 ch on: the eight lanes that a store to
+        // shared memory serves at a time hold four chunks of two neighbouring rows, which the swizzle puts into all banks.
+        const int w = warp - 8, ch = lane & 3, sub = lane >> 2;
+        constexpr int NV = 4 * ATOMS;           // vectors a lane holds of a side
+        int page0 = -1, page1 = -1;             // of the warp's first and second 16 keys
         auto look = [&](int j) {
             const int key = (j_begin + j) * CP_KEYS + w * 32;
             page0 = page1 = -1;
@@ -306,24 +311,25 @@ cache_prompt_kernel(const CachePromptParams p) {
                 page1 = c.T > 16 ? page0 : key + 16 < it.n ? (int)c.page(it.b, (key >> 4) + 1) : -1;
             }
         };
-        uint4 cur[8];
-        auto fetch = [&](int j, int side) {   // zeros where there is no key: what P = 0 multiplies is a number
-            const int key0 = (j_begin + j) * CP_KEYS + w * 32 + sub;
+        uint4 kq[NV], vq[NV];     // the next block's, on their way while this one's are written
+        auto fetch = [&](uint4 (&cur)[NV], int j, int side) {   // zeros where there is no key: what P = 0 multiplies is a number
+            const int key0 = (j_begin + j) * CP_KEYS + w * 32, in = (key0 & (c.T - 1)) + sub;
             const uint8_t* base = (side ? c.v : c.k) + it.h * (side ? c.vH : c.kH) + ch * 16;
             const int64_t sT = side ? c.vT : c.kT, sP = side ? c.vP : c.kP;
+            const uint8_t* at0 = base + page0 * sP + in * sT;
+            const uint8_t* at1 = base + page1 * sP + (c.T > 16 ? in + 16 : sub) * sT;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = key0 + 4 * i, page = i < 4 ? page0 : page1;
+            for (int i = 0; i < NV; ++i) {
+                const int a = i % ATOMS, r = i / ATOMS;
+                const bool on = (r < 2 ? page0 : page1) >= 0 && key0 + 8 * r + sub < it.n && a * 64 + ch * 16 < c.E;
                 cur[i] = make_uint4(0, 0, 0, 0);
-                if (mine && page >= 0 && key < it.n && j < nblk) cur[i] = __ldg(reinterpret_cast<const uint4*>(base + page * sP + (key & (c.T - 1)) * sT));
+                if (on) cur[i] = __ldg(reinterpret_cast<const uint4*>((r < 2 ? at0 : at1) + (r & 1) * 8 * sT + a * 64));
             }
         };
-        auto write = [&](uint32_t tile, bool values) {
-            const uint32_t at = tile + (uint32_t)(ch >> 2) * CP_ATOM;
-            const int first = ch >> 2;       // lanes of the second atom write their second chunk first: a phase's eight lanes meet all banks
+        auto write = [&](const uint4 (&cur)[NV], uint32_t tile, bool values) {
+            const uint32_t even = tile + (w * 32 + sub) * 128 + (((2 * ch) ^ sub) << 4);   // a row's place modulo 8 is sub
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = w * 32 + 4 * i + sub;
+            for (int i = 0; i < NV; ++i) {
                 const uint32_t v[4] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w};
                 uint32_t h[8];
 #pragma unroll
@@ -338,37 +344,29 @@ cache_prompt_kernel(const CachePromptParams p) {
                         }
                     }
                 }
-                const uint32_t line = at + row * 128;
-                const int c0 = 2 * (ch & 3);
-                const uint32_t a0 = line + (((c0 + first) ^ (row & 7)) << 4), a1 = line + (((c0 + 1 - first) ^ (row & 7)) << 4);
-                uint32_t x[4], y[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[k] = first ? h[4 + k] : h[k];
-                    y[k] = first ? h[k] : h[4 + k];
-                }
-                if (ch < EP / 16) {
-                    st_shared_v4(a0, x);
-                    st_shared_v4(a1, y);
-                }
+                const uint32_t at = even + (uint32_t)((i % ATOMS) * CP_ATOM + (i / ATOMS) * 1024);
+                st_shared_v4(at, h);
+                st_shared_v4(at ^ 16u, h + 4);   // the chunk's neighbour
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
         look(0);
-        fetch(0, 0);
+        fetch(kq, 0, 0);
+        fetch(vq, 0, 1);
+        look(1);
         for (int j = 0; j < nblk; ++j) {
             const int s = j % STAGES;
             const uint32_t ph = (uint32_t)((j / STAGES) & 1) ^ 1;
             if (!mbar_wait(&k_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
-            write(smem_u32(smem + Cfg::S_K + s * Cfg::SIDE), false);
+            write(kq, smem_u32(smem + Cfg::S_K + s * Cfg::SIDE), false);
             if (lane == 0) mbar_arrive(&k_full[s]);
-            fetch(j, 1);
-            look(j + 1);
+            fetch(kq, j + 1, 0);
             if (!mbar_wait(&v_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
-            write(smem_u32(smem + Cfg::S_V + s * Cfg::SIDE), true);
+            write(vq, smem_u32(smem + Cfg::S_V + s * Cfg::SIDE), true);
             if (lane == 0) mbar_arrive(&v_full[s]);
-            fetch(j + 1, 0);
+            fetch(vq, j + 1, 1);
+            look(j + 2);
         }
     } else {
         // ------------------------------------------------------ softmax and results
@@ -433,6 +431,13 @@ cache_prompt_kernel(const CachePromptParams p) {
                         for (int u = 0; u < 32; ++u)
                             if (i * 32 + u > seen || (hidden >> (i * 2 + u / 16) & 1)) x[i][u] = 0xff800000u;
                 }
+                if (k.odd != 0) {     // whoever sees one of the group's keys sees no number
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 32; ++u)
+                            if ((k.odd >> (i * 2 + u / 16) & 1) && x[i][u] != 0xff800000u) x[i][u] = 0x7fffffffu;
+                }
                 float top = -INFINITY;
 #pragma unroll
                 for (int gq = 0; gq < 8; ++gq) {
@@ -443,7 +448,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                         a = cp_max3(a, __uint_as_float(y[u]), __uint_as_float(y[u + 1]));
                         if (u + 2 < 16) b2 = cp_max3(b2, __uint_as_float(y[u + 2]), __uint_as_float(y[u + 3]));
                     }
-                    top = fmaxf(top, fmaxf(a, b2) * k.key[gq]);   // -inf times 0 is no number, which a maximum passes over
+                    top = fmaxf(top, fmaxf(a, b2) * k.key[gq]);
                 }
                 // the reference point follows lazily: only when the maximum has grown by more than 2^8
                 const float m_new = top > m_run + 8.f ? top : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new;
@@ -483,10 +488,6 @@ cache_prompt_kernel(const CachePromptParams p) {
                             float e0, e1;
                             unpack2(fma2(pack2(__uint_as_float(u0), __uint_as_float(u1)), k2, a2), e0, e1);
                             e0 = cp_ex2(e0), e1 = cp_ex2(e1);
-                            if (masked) {
-                                if (u0 == 0xff800000u) e0 = 0.f;
-                                if (u1 == 0xff800000u) e1 = 0.f;
-                            }
                             sum = add2(sum, pack2(e0, e1));
                             const __half2 h2 = __floats2half2_rn(e0, e1);
                             pk[g2 * 8 + u] = *reinterpret_cast<const uint32_t*>(&h2);
