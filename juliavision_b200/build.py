@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(CSRC, "libb200dnn.so")
 SOURCES = ["ctx.cu", "layernorm.cu", "gemm.cu", "attention.cu", "glue.cu", "conv.cu", "conv_implicit.cu", "gemv.cu", "gemm_rows.cu", "gemm_rows_tc.cu", "attention_window.cu", "attention_few.cu", "selftest.cu",
            "rotary.cu", "cache8.cu", "cache8_attention.cu", "cache8_prompt.cu", "linear4.cu"]
-HEADERS = ["internal.h", "ptx.cuh", "act.cuh", "gemm_rows.cuh", "cache8.cuh", os.path.join("..", "..", "include", "b200dnn.h")]
+HEADERS = ["internal.h", "ptx.cuh", "act.cuh", "gemm_rows.cuh", "cache8.cuh", "shares.cuh", os.path.join("..", "..", "include", "b200dnn.h")]
 HOST_SRC = os.path.join(CSRC, "hostcalls.c")   # the entry points' host side, a CPython extension
 HOST_SO = os.path.join(CSRC, "hostcalls" + EXTENSION_SUFFIXES[0])   # for this interpreter: another builds its own
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

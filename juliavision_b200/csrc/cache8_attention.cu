@@ -24,12 +24,10 @@
 #include <cuda_fp16.h>
 
 #include "cache8.cuh"
+#include "shares.cuh"
 
 namespace b200 {
 
-#ifndef CF_MOST_ROWS
-#define CF_MOST_ROWS 64
-#endif
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
 constexpr int CF_KEYS = 64;                      // keys a warp takes at a time: a tile of the list
@@ -118,18 +116,6 @@ __device__ __forceinline__ uint32_t cf_transpose(uint32_t v) {
     return r;
 }
 
-// floor(a / b), 0 <= a < 2^52: an integer division of 64 bits takes ten times as long, and the ends of a share wait for several.
-__device__ __forceinline__ long long cf_div(long long a, long long b) {
-    long long q = (long long)((double)a / (double)b);
-    const long long r = a - q * b;
-    if (r < 0) --q;
-    else if (r >= b) ++q;
-    return q;
-}
-
-struct CfParts {              // where the parts of a piece are: its first and last warp, blocks with a part of it, parts
-    int w0, w1, blocks, count;
-};
 struct CfPiece {
     long long start;          // its first tile in the list
     int b, n, m, tiles;       // sequence, its length and new tokens; tiles of a piece of it
@@ -148,7 +134,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     __shared__ long long start_s[CF_WARPS], sums_s[CF_WARPS];
     __shared__ int where_s[CF_WARPS], abort_s;
     __shared__ CfPiece given_s[2 * CF_WARPS];                          // parts of pieces this block's warps have: ended, last
-    __shared__ CfParts parts_s[2 * CF_WARPS];
+    __shared__ PieceParts parts_s[2 * CF_WARPS];
     __shared__ int has_s[2 * CF_WARPS], join_s[2 * CF_WARPS];          // there is one; this block joins its piece
     if (threadIdx.x < 2 * CF_WARPS) has_s[threadIdx.x] = 0;
     uint8_t* cf_smem = cf_raw + ((1024 - (smem_u32(cf_raw) & 1023)) & 1023);
@@ -194,14 +180,13 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         return x - v + add;
     };
     long long total = 0, bstart = 0, from = 0, to = 0;
-    int b = 0, warps = 0;         // warps that have a share
+    int b = 0;
     const int me = blockIdx.x * CF_WARPS + warp;
     auto deal = [&]() {
-        warps = gridDim.x * CF_WARPS;
-        if (total < warps) warps = (int)total;
-        if (me < warps) {
-            from = cf_div(me * total, warps);
-            to = cf_div((me + 1) * total, warps);
+        const Shares s(total, gridDim.x * CF_WARPS);
+        if (me < s.warps) {
+            from = s.begin(me);
+            to = s.begin(me + 1);
         }
     };
     if (p.B <= 32) {              // every warp for itself
@@ -233,8 +218,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
 #pragma unroll
             for (int w = 0; w < CF_WARPS; ++w) {
                 const int who = blockIdx.x * CF_WARPS + w;
-                if (who >= warps) break;
-                const long long f = cf_div(who * total, warps);
+                const Shares s(total, gridDim.x * CF_WARPS);
+                if (who >= s.warps) break;
+                const long long f = s.begin(who);
                 if (at <= f && f < at + mine) {
                     where_s[w] = b0 + tid;
                     start_s[w] = at;
@@ -261,7 +247,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         }
         const int rts = (m * p.G + RT - 1) / RT;
         const long long off = at - bstart;
-        const int piece = (int)cf_div(off, tiles);
+        const int piece = (int)floor_div(off, tiles);
         pc.b = b, pc.n = n, pc.m = m, pc.tiles = tiles;
         pc.h = piece / rts, pc.rt = piece - pc.h * rts;
         pc.rows = m * p.G - pc.rt * RT < RT ? m * p.G - pc.rt * RT : RT;
@@ -579,19 +565,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     __syncthreads();   // the ring is free: every copy that was asked for has been waited for
     float* rows_s = reinterpret_cast<float*>(cf_smem);
     if (has_s[2 * warp + 1]) keep(rows_s + warp * RT * ROW, pc);
-    // A piece's last parts, one a block, from its first warp's block on; then perhaps the part that ended inside a warp's share.
-    if (tid < 2 * CF_WARPS && has_s[tid]) {
-        const CfPiece& q = given_s[tid];
-        const long long end = q.start + q.tiles;
-        auto holder = [&](long long u) { return (int)cf_div((u + 1) * warps - 1, total); };   // the warp that has tile u of the list
-        CfParts r;
-        r.w0 = holder(q.start);
-        r.w1 = holder(end - 1);
-        const bool inside = cf_div((r.w1 + 1) * total, warps) > end;
-        r.blocks = (r.w1 - (inside ? 1 : 0)) / CF_WARPS - r.w0 / CF_WARPS + 1;
-        r.count = r.blocks + (inside ? 1 : 0);
-        parts_s[tid] = r;
-    }
+    if (tid < 2 * CF_WARPS && has_s[tid])
+        parts_s[tid] = PieceParts::of<CF_WARPS>(Shares(total, gridDim.x * CF_WARPS), given_s[tid].start, given_s[tid].start + given_s[tid].tiles);
     __syncthreads();
     auto same = [&](int w) {   // warps w and w + 1 have the same last piece
         return w + 1 < CF_WARPS && has_s[2 * w + 1] && has_s[2 * w + 3] && given_s[2 * w + 1].start == given_s[2 * w + 3].start;
@@ -629,7 +604,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     if (tid < 2 * CF_WARPS) {
         join_s[tid] = 0;
         if (has_s[tid] && (!(tid & 1) || tid == 1 || !same((tid >> 1) - 1))) {   // one of a group counts it
-            const CfParts r = parts_s[tid];
+            const PieceParts r = parts_s[tid];
             if (r.count > 1) join_s[tid] = atomicAdd(p.arrived + r.w0, 1) == r.count - 1;
         }
     }
@@ -638,11 +613,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         if (!join_s[k]) continue;
         __threadfence();
         const CfPiece& q = given_s[k];
-        const CfParts r = parts_s[k];
-        auto part_of = [&](int i) {
-            const int w = r.w0 / CF_WARPS * CF_WARPS + i * CF_WARPS;
-            return p.part + (int64_t)(i == r.blocks ? 2 * r.w1 : 2 * (i == 0 ? r.w0 : w) + 1) * RT * ROW;
-        };
+        const PieceParts r = parts_s[k];
+        auto part_of = [&](int i) { return p.part + r.place<CF_WARPS>(i) * RT * ROW; };
         constexpr int AT_ONCE = 16;   // loads in flight: each is a trip to L2
         if (r.count <= AT_ONCE) {
             for (int i = tid; i < q.rows * (EP / 4); i += CF_THREADS) {
@@ -792,7 +764,10 @@ int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int
     const bool fp8 = cache->kind == B200_E4M3;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634 / (fp8 ? 448.0 : 127.0));
     B200_CUDA(cudaSetDevice(ctx->device));
-    if ((int64_t)p.L * p.G > CF_MOST_ROWS) return cache_prompt_run(ctx, p.c, L, B, p.G, q, out, out_dtype, scale, fp8, causal, lens, news);
+    // Each tile of 16 rows converts the cache again; tiles of 128 rows convert it once.  4 x 4096 tokens, 32 heads on 8, E = 128, by few
+    // rows and by many: 16 rows 27.3 us and 30.5, 32 rows 33.4 and 30.9, 64 rows 45.8 and 31.4; 8 x 4096, 20 heads on 4, E = 64: 25 rows
+    // 23.3 and 24.7, 65 rows 35.9 and 25.2.
+    if ((int64_t)p.L * p.G > (p.c.E > 64 ? 24 : 32)) return cache_prompt_run(ctx, p.c, L, B, p.G, q, out, out_dtype, scale, fp8, causal, lens, news);
     if (p.L * p.G <= 8) {
         if (p.c.E <= 64) return fp8 ? cf_launch<64, true, 1>(ctx, p) : cf_launch<64, false, 1>(ctx, p);
         return fp8 ? cf_launch<128, true, 1>(ctx, p) : cf_launch<128, false, 1>(ctx, p);

@@ -8,30 +8,56 @@
 // and steps 2, 3 are 32 inputs each, so a group of 32 is two steps.  Nibbles (0,4) (1,5) (2,6) (3,7) are the four operand
 // registers: a nibble under 0x64 is the fp16 number 1024 + q (or, in the upper half of its byte, 1024 + 16 q), and q - z comes
 // out exactly of one subtraction (or one multiply-add by 1 / 16).  A group's sum is fp32, and so is its product by the scale.
+// Four row tiles lie side by side, unit by unit, so that 64 rows are one stream of 2 KB a k block.
+//
+// Two kernels for few tokens.  A small weight, whose rows do not fill the GPU for long, is a chain of round trips: a block takes 16
+// rows, its warps share K and have all their loads in flight at once (linear4_kernel).  A large one is bandwidth-bound: the list of
+// (64 rows, 8 or 16 tokens, k block) is dealt out to all warps in equal contiguous shares, each streamed by bulk copies through a ring
+// of its own; parts of rows meet at the ends of blocks (linear4_stream_kernel, shares.cuh).
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "act.cuh"
 #include "internal.h"
 #include "ptx.cuh"
+#include "shares.cuh"
 
 namespace b200 {
 
 constexpr int L4_WARPS = 8;      // of a block, which share K
-constexpr int L4_TOKENS = 64;    // tokens the kernel takes; more go through fp16 weights in the workspace
+#ifndef L4_STREAM_TILES
+#define L4_STREAM_TILES 8192
+#endif
+#ifndef L4_MOST
+#define L4_MOST 64
+#endif
+constexpr int L4_TOKENS = L4_MOST;    // tokens the kernel takes; more go through fp16 weights in the workspace
 
 struct Linear4Params {
-    const uint4* data;            // [row tile][k block][lane]
-    const uint32_t* scales;       // [row tile][group][8]: fp16 scales of rows g and g + 8
-    const uint8_t* zeros;         // [row tile][group][8]: zero points of rows g (low) and g + 8 (high), or null
+    const uint4* data;            // [four row tiles][k block][row tile][lane]
+    const uint32_t* scales;       // [four row tiles][group][row tile][8]: fp16 scales of rows g and g + 8
+    const uint8_t* zeros;         // the same: zero points of rows g (low) and g + 8 (high), or null
     const __half *x, *bias;
     void* out;
     int64_t ldx, ldo, M;
     int N, K, KB, NG, MT;         // k blocks of 64, groups a row, row tiles
     int logg;                     // log2 of the group size
     int out_f32, epi, whole;
+    float* part;                  // [place][row tile, token tile][lane][4] (linear4_stream_kernel)
+    int* arrived;
+    int* d_status;
+
+    __device__ __forceinline__ int64_t unit(int mt, int kb) const { return ((int64_t)(mt >> 2) * KB + kb) * 4 + (mt & 3); }
+    __device__ __forceinline__ int64_t group8(int mt, int grp) const { return (((int64_t)(mt >> 2) * NG + grp) * 4 + (mt & 3)) * 8; }
 };
 
-__device__ __forceinline__ uint32_t l4_and_or(uint32_t v, uint32_t m, uint32_t o) { return (v & m) | o; }
+// (v & M) | magic in one instruction: of two constants one has to be a register
+template <uint32_t M> __device__ __forceinline__ uint32_t l4_and_or(uint32_t v, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "n"(M), "r"(magic));
+    return r;
+}
 __device__ __forceinline__ uint32_t l4_sub(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -43,14 +69,14 @@ __device__ __forceinline__ uint32_t l4_fma16(uint32_t a, uint32_t b) {   // a / 
 }
 // The four operand registers of a word: q - z for rows g (z0 = 1024 + z, twice) and g + 8 (z1 = -(64 + z), twice).
 __device__ __forceinline__ void l4_weights(uint32_t v, uint32_t z0, uint32_t z1, uint32_t (&a)[4]) {
-    a[0] = l4_sub(l4_and_or(v, 0x000f000fu, 0x64006400u), z0);
-    a[1] = l4_fma16(l4_and_or(v, 0x00f000f0u, 0x64006400u), z1);
+    const uint32_t magic = 0x64006400u;
+    a[0] = l4_sub(l4_and_or<0x000f000fu>(v, magic), z0);
+    a[1] = l4_fma16(l4_and_or<0x00f000f0u>(v, magic), z1);
     v >>= 8;
-    a[2] = l4_sub(l4_and_or(v, 0x000f000fu, 0x64006400u), z0);
-    a[3] = l4_fma16(l4_and_or(v, 0x00f000f0u, 0x64006400u), z1);
+    a[2] = l4_sub(l4_and_or<0x000f000fu>(v, magic), z0);
+    a[3] = l4_fma16(l4_and_or<0x00f000f0u>(v, magic), z1);
 }
-__device__ __forceinline__ void l4_zero(const uint8_t* zeros, int64_t at, uint32_t& z0, uint32_t& z1) {
-    const uint32_t z = zeros != nullptr ? __ldg(zeros + at) : 0x88u;
+__device__ __forceinline__ void l4_zero(uint32_t z, uint32_t& z0, uint32_t& z1) {   // two zero points of a byte
     z0 = (0x6400u | (z & 15u)) * 0x10001u;
     z1 = (0xd400u | (z & 0xf0u)) * 0x10001u;
 }
@@ -74,86 +100,332 @@ __device__ __forceinline__ void l4_input(const Linear4Params& p, int n, int kb, 
     }
 }
 
-// MT row tiles and NT tiles of 8 tokens a block; the warps take every L4_WARPS-th k block.  SMALL: groups of 32.
-template <int MT, int NT, bool SMALL>
+// The first product of a sum.
+__device__ __forceinline__ void l4_mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// A k block of a row tile: acc += the products of its groups by their scales.
+template <int NT, bool SMALL>
+__device__ __forceinline__ void l4_block(float (&acc)[NT][4], const uint4& w, const uint32_t* sc, const uint32_t* zb, const uint32_t (&x)[NT][8]) {
+    constexpr int GROUPS = SMALL ? 2 : 1, STEPS = 4 / GROUPS;   // groups a k block, steps a group
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+        uint32_t z0, z1;
+        l4_zero(zb[j], z0, z1);
+        const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sc[j]));
+        float c[NT][4];
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            uint32_t a[4];
+            l4_weights(v[j * STEPS + k], z0, z1, a);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t b0 = x[n][2 * (j * STEPS + k)], b1 = x[n][2 * (j * STEPS + k) + 1];
+                if (k == 0) l4_mma0(c[n], a, b0, b1);
+                else mma_16816(c[n], a, b0, b1);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            acc[n][0] = fmaf(c[n][0], s.x, acc[n][0]);
+            acc[n][1] = fmaf(c[n][1], s.x, acc[n][1]);
+            acc[n][2] = fmaf(c[n][2], s.y, acc[n][2]);
+            acc[n][3] = fmaf(c[n][3], s.y, acc[n][3]);
+        }
+    }
+}
+__device__ __forceinline__ void l4_store(const Linear4Params& p, int64_t m, int n, float v) {
+    if (m >= p.M || n >= p.N) return;
+    if (p.bias != nullptr) v += __half2float(p.bias[m]);
+    // the activation sees the value rounded to the output type, as in the GEMM's store
+    if (p.out_f32) ((float*)p.out)[n * p.ldo + m] = apply_act(p.epi, v);
+    else ((__half*)p.out)[n * p.ldo + m] = __float2half_rn(apply_act(p.epi, __half2float(__float2half_rn(v))));
+}
+
+// One row tile and NT tiles of 8 tokens a block; the warps take every L4_WARPS-th k block, AT_ONCE of them at a time.  SMALL: groups of 32.
+template <int NT, bool SMALL>
 __global__ void __launch_bounds__(32 * L4_WARPS)
 linear4_kernel(const Linear4Params p) {
-    extern __shared__ __align__(16) float l4_red[];   // [warp][row][token]
-    constexpr int COLS = 8 * NT + 1, ROWS = 16 * MT, GROUPS = SMALL ? 2 : 1, STEPS = 4 / GROUPS;   // groups a k block, steps a group
+    constexpr int COLS = 8 * NT + 1, GROUPS = SMALL ? 2 : 1, AT_ONCE = NT == 1 ? 4 : 3;
+    __shared__ float red[L4_WARPS][16][COLS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int mt0 = blockIdx.x * MT, n0 = blockIdx.y * 8 * NT;
+    const int mt = blockIdx.x, n0 = blockIdx.y * 8 * NT;
     grid_dep_wait();
     grid_dep_launch();
-    float acc[MT][NT][4];
+    float acc[NT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    for (int kb0 = warp; kb0 < p.KB; kb0 += L4_WARPS * AT_ONCE) {
+        uint4 w[AT_ONCE];
+        uint32_t sc[AT_ONCE][GROUPS], zb[AT_ONCE][GROUPS], x[AT_ONCE][NT][8];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
-    for (int kb = warp; kb < p.KB; kb += L4_WARPS) {
-        uint4 w[MT];
-        uint32_t sc[MT][GROUPS];
-        uint32_t z0[MT][GROUPS], z1[MT][GROUPS];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const bool in = mt0 + i < p.MT;
-            w[i] = in ? __ldg(p.data + ((int64_t)(mt0 + i) * p.KB + kb) * 32 + lane) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int kb = kb0 + u * L4_WARPS;
+            const bool in = kb < p.KB;
+            w[u] = in ? __ldg(p.data + p.unit(mt, kb) * 32 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int j = 0; j < GROUPS; ++j) {
                 const int grp = (kb * 64 + j * 32) >> p.logg;
                 const bool live = in && grp < p.NG;    // the last k block may be half empty
-                const int64_t at = ((int64_t)(mt0 + i) * p.NG + grp) * 8 + g;
-                sc[i][j] = live ? __ldg(p.scales + at) : 0;
-                l4_zero(live ? p.zeros : nullptr, at, z0[i][j], z1[i][j]);
+                sc[u][j] = live ? __ldg(p.scales + p.group8(mt, grp) + g) : 0;
+                zb[u][j] = live && p.zeros != nullptr ? __ldg(p.zeros + p.group8(mt, grp) + g) : 0x88u;
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) l4_input(p, n0 + n * 8 + g, in ? kb : p.KB, t, x[u][n]);
         }
-        uint32_t x[NT][8];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) l4_input(p, n0 + n * 8 + g, kb, t, x[n]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-            for (int j = 0; j < GROUPS; ++j) {
-                const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sc[i][j]));
-                float c[NT][4];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    uint32_t a[4];
-                    l4_weights(v[j * STEPS + k], z0[i][j], z1[i][j], a);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(c[n], a, x[n][2 * (j * STEPS + k)], x[n][2 * (j * STEPS + k) + 1]);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    acc[i][n][0] = fmaf(c[n][0], s.x, acc[i][n][0]);
-                    acc[i][n][1] = fmaf(c[n][1], s.x, acc[i][n][1]);
-                    acc[i][n][2] = fmaf(c[n][2], s.y, acc[i][n][2]);
-                    acc[i][n][3] = fmaf(c[n][3], s.y, acc[i][n][3]);
-                }
-            }
-        }
+        for (int u = 0; u < AT_ONCE; ++u) l4_block<NT, SMALL>(acc, w[u], sc[u], zb[u], x[u]);
     }
-    float* mine = l4_red + warp * ROWS * COLS;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) red[warp][g + (k >> 1) * 8][n * 8 + 2 * t + (k & 1)] = acc[n][k];
+    __syncthreads();
+    for (int i = tid; i < 16 * 8 * NT; i += 32 * L4_WARPS) {
+        const int row = i % 16, col = i / 16;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < L4_WARPS; ++w) v += red[w][row][col];
+        l4_store(p, (int64_t)mt * 16 + row, n0 + col, v);
+    }
+}
+
+constexpr int L4_STAGES = 3;     // k blocks of 64 rows in flight, a warp
+__device__ __forceinline__ void l4_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar)) : "memory");
+}
+
+template <int NT, bool SMALL> struct L4Cfg {
+    static constexpr int GROUPS = SMALL ? 2 : 1;
+    static constexpr int SCALES = 2048, ZEROS = SCALES + GROUPS * 128, X = ZEROS + GROUPS * 32,
+                         STAGE = X + NT * 1024;   // 64 rows' weights, scales, zero points; the tokens' inputs
+    static_assert(X % 16 == 0 && STAGE % 16 == 0, "16-byte copies");
+    static constexpr int RING = L4_WARPS * L4_STAGES * STAGE;
+    static constexpr int FLOATS = 4 * NT * 128;      // a warp's results of 64 rows
+    static_assert(L4_WARPS * FLOATS * 4 <= RING, "the warps' results fit over the ring");
+    static constexpr int CTAS = 2;
+};
+
+// NT tiles of 8 tokens.  Tiles of the list: (64 rows, NT token tiles, k block), the k block fastest.  ZP: there are zero points.
+template <int NT, bool SMALL, bool ZP>
+__global__ void __launch_bounds__(32 * L4_WARPS, L4Cfg<NT, SMALL>::CTAS)
+linear4_stream_kernel(const Linear4Params p) {
+    using Cfg = L4Cfg<NT, SMALL>;
+    constexpr int GROUPS = Cfg::GROUPS;
+    extern __shared__ __align__(128) uint8_t l4_ring[];
+    __shared__ __align__(8) uint64_t full_s[L4_WARPS][L4_STAGES];
+    __shared__ PieceParts parts_s[2 * L4_WARPS];
+    __shared__ long long piece_s[2 * L4_WARPS];                    // the pieces this block's warps have parts of: ended, last; -1: none
+    __shared__ int join_s[2 * L4_WARPS], abort_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    if (lane == 0) {
+        for (int i = 0; i < L4_STAGES; ++i) mbar_init(&full_s[warp][i], 1);
+        fence_barrier_init();
+    }
+    if (tid == 0) abort_s = 0;
+    if (tid < 2 * L4_WARPS) piece_s[tid] = -1;
+    __syncthreads();
+    grid_dep_wait();
+    grid_dep_launch();
+    const int tgs = (p.N + 8 * NT - 1) / (8 * NT);
+    const Shares shares((long long)(p.MT + 3) / 4 * tgs * p.KB, gridDim.x * L4_WARPS);
+    const int me = blockIdx.x * L4_WARPS + warp;
+    const long long from = me < shares.warps ? shares.begin(me) : 0, to = me < shares.warps ? shares.begin(me + 1) : 0;
+    uint8_t* const ring = l4_ring + warp * L4_STAGES * Cfg::STAGE;
+
+    // The tile to be asked for next, everything about it carried along: a division for each would cost more than the tile's products.
+    // Inputs: token n's 64 in eight chunks of 16 bytes, an odd token's halves changed over, so that the eight lanes of a phase, four
+    // chunks of two tokens, meet all banks.  Lane (n, chunk) has tokens n, n + 4, ... of the 8 NT.
+    const int tiles = (int)(to - from), xn = lane >> 3, xk = (lane & 7) * 8;
+    const uint32_t x_at = Cfg::X + xn * 128 + (((lane & 7) ^ (xn & 1) << 2) << 4);
+    int asked = 0, ask_s = 0, ask_kb, ask_tg;
+    const uint8_t *ask_data, *ask_scales, *ask_zeros;
+    const __half* ask_x;
+    auto inputs = [&]() { ask_x = p.x + (int64_t)(ask_tg * NT * 8 + xn) * p.ldx + ask_kb * 64 + xk; };
+    {
+        const int piece = (int)floor_div(from, p.KB), rg = piece / tgs;
+        ask_kb = (int)(from - (long long)piece * p.KB);
+        ask_tg = piece - rg * tgs;
+        ask_data = reinterpret_cast<const uint8_t*>(p.data) + ((int64_t)rg * p.KB + ask_kb) * 2048;
+        ask_scales = reinterpret_cast<const uint8_t*>(p.scales) + (int64_t)rg * p.NG * 128;      // of the rows
+        ask_zeros = p.zeros + (int64_t)rg * p.NG * 32;
+        inputs();
+    }
+    auto fetch = [&]() {          // a commit group even when there is none
+        if (asked < tiles) {
+            const uint32_t dst = smem_u32(ring + ask_s * Cfg::STAGE);
+            if (lane == 0) {
+                const int g0 = (ask_kb * 64) >> p.logg, groups = SMALL && p.NG - g0 < GROUPS ? 1 : GROUPS;
+                uint64_t* bar = &full_s[warp][ask_s];
+                mbar_arrive_expect_tx(bar, 2048 + groups * (ZP ? 160 : 128));
+                l4_bulk(dst, ask_data, 2048, bar);
+                l4_bulk(dst + Cfg::SCALES, ask_scales + g0 * 128, groups * 128, bar);
+                if (ZP) l4_bulk(dst + Cfg::ZEROS, ask_zeros + g0 * 32, groups * 32, bar);
+            }
+            const int n = ask_tg * NT * 8 + xn;
+            const bool in = ask_kb * 64 + xk < p.K;        // K is a multiple of 32
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) {
+                const bool live = in && n + 4 * i < p.N;
+                const __half* src = live ? ask_x + i * 4 * p.ldx : p.x;
+                if (p.whole) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst + x_at + i * 512), "l"(src), "r"(live ? 16 : 0) : "memory");
+                } else {
+                    uint32_t v[4] = {0, 0, 0, 0};
+                    if (live) {
+                        const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) v[c] = u[2 * c] | (uint32_t)u[2 * c + 1] << 16;
+                    }
+                    st_shared_v4(dst + x_at + i * 512, v);
+                }
+            }
+            ++asked;
+            if (++ask_s == L4_STAGES) ask_s = 0;
+            ask_data += 2048;
+            ask_x += 64;
+            if (++ask_kb == p.KB) {      // the next piece: other tokens with the same rows, or the next rows
+                ask_kb = 0;
+                if (++ask_tg == tgs) {
+                    ask_tg = 0;
+                    ask_scales += (int64_t)p.NG * 128;
+                    ask_zeros += (int64_t)p.NG * 32;
+                } else {
+                    ask_data -= (int64_t)p.KB * 2048;
+                }
+                inputs();
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < L4_STAGES - 1; ++i) fetch();
+
+    int piece = (int)floor_div(from, p.KB), kb = (int)(from - (long long)piece * p.KB);
+    float acc[4][NT][4];
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
+    };
+    auto finish = [&](long long q, int i, int n, const float4& v, int ln) {   // results of row tile i, token tile n as lane ln has them
+        const int rg = (int)q / tgs, tg = (int)q % tgs;
+        const int64_t m = (int64_t)(rg * 4 + i) * 16 + (ln >> 2);
+        const int c = (tg * NT + n) * 8 + 2 * (ln & 3);
+        l4_store(p, m, c, v.x);
+        l4_store(p, m, c + 1, v.y);
+        l4_store(p, m + 8, c, v.z);
+        l4_store(p, m + 8, c + 1, v.w);
+    };
+    auto keep = [&](float* to_p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) *reinterpret_cast<float4*>(to_p + ((i * NT + n) * 32 + lane) * 4) = make_float4(acc[i][n][0], acc[i][n][1], acc[i][n][2], acc[i][n][3]);
+    };
+    clear();
+    int s = 0;
+    uint32_t phase = 0;
+    bool first = true;            // the piece at hand may have begun before this share
+    for (int at = 0; at < tiles; ++at) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(L4_STAGES - 2) : "memory");
+        if (!mbar_wait(&full_s[warp][s], phase, p.d_status, KST_WAIT_FULL, &abort_s)) break;
+        __syncwarp();             // this stage is there for every lane, and the one that is asked for now has been read
+        fetch();
+        const uint8_t* st = ring + s * Cfg::STAGE;
+        if (++s == L4_STAGES) s = 0, phase ^= 1;
+        uint32_t x[NT][8];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mine[(i * 16 + g + (k >> 1) * 8) * COLS + n * 8 + 2 * t + (k & 1)] = acc[i][n][k];
-    __syncthreads();
-    for (int i = tid; i < ROWS * 8 * NT; i += 32 * L4_WARPS) {
-        const int row = i % ROWS, col = i / ROWS, n = n0 + col;
-        const int64_t m = (int64_t)mt0 * 16 + row;
-        if (m >= p.M || n >= p.N) continue;
-        float v = 0.f;
+            for (int half = 0; half < 2; ++half) {
+                const uint4 v = *reinterpret_cast<const uint4*>(st + Cfg::X + (n * 8 + g) * 128 + (((half * 4 + t) ^ (g & 1) << 2) << 4));
+                x[n][4 * half] = v.x, x[n][4 * half + 1] = v.y, x[n][4 * half + 2] = v.z, x[n][4 * half + 3] = v.w;
+            }
 #pragma unroll
-        for (int w = 0; w < L4_WARPS; ++w) v += l4_red[(w * ROWS + row) * COLS + col];
-        if (p.bias != nullptr) v += __half2float(p.bias[m]);
-        // the activation sees the value rounded to the output type, as in the GEMM's store
-        if (p.out_f32) ((float*)p.out)[n * p.ldo + m] = apply_act(p.epi, v);
-        else ((__half*)p.out)[n * p.ldo + m] = __float2half_rn(apply_act(p.epi, __half2float(__float2half_rn(v))));
+        for (int i = 0; i < 4; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4*>(st + i * 512 + lane * 16);
+            uint32_t sc[GROUPS], zb[GROUPS];
+#pragma unroll
+            for (int j = 0; j < GROUPS; ++j) {
+                const bool live = j == 0 || kb * 2 + j < p.NG;
+                sc[j] = live ? *reinterpret_cast<const uint32_t*>(st + Cfg::SCALES + j * 128 + i * 32 + g * 4) : 0;
+                zb[j] = ZP && live ? st[Cfg::ZEROS + j * 32 + i * 8 + g] : 0x88u;
+            }
+            l4_block<NT, SMALL>(acc[i], w, sc, zb, x);
+        }
+        if (++kb == p.KB || at + 1 == tiles) {
+            const long long start = (long long)piece * p.KB;
+            const bool mine = kb == p.KB && (!first || from == start);
+            if (mine) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) finish(piece, i, n, make_float4(acc[i][n][0], acc[i][n][1], acc[i][n][2], acc[i][n][3]), lane);
+            } else {
+                if (at + 1 < tiles) keep(p.part + (int64_t)(2 * me) * Cfg::FLOATS);
+                if (lane == 0) piece_s[2 * warp + (at + 1 == tiles)] = piece;
+            }
+            if (at + 1 < tiles) {
+                clear();
+                first = false;
+                kb = 0, ++piece;
+            }
+        }
+    }
+
+    // ---- the block's parts of pieces
+    __syncthreads();              // the ring is free: every copy that was asked for has been waited for
+    float* rows_s = reinterpret_cast<float*>(l4_ring);
+    if (piece_s[2 * warp + 1] >= 0) keep(rows_s + warp * Cfg::FLOATS);
+    if (tid < 2 * L4_WARPS && piece_s[tid] >= 0) parts_s[tid] = PieceParts::of<L4_WARPS>(shares, piece_s[tid] * p.KB, (piece_s[tid] + 1) * p.KB);
+    __syncthreads();
+    auto same = [&](int w) { return w + 1 < L4_WARPS && piece_s[2 * w + 1] >= 0 && piece_s[2 * w + 1] == piece_s[2 * w + 3]; };
+    for (int w = 0, end; w < L4_WARPS; w = end) {
+        end = w + 1;
+        while (same(end - 1)) ++end;
+        const long long q = piece_s[2 * w + 1];
+        if (q < 0) continue;
+        const bool all = parts_s[2 * w + 1].count == 1;
+        float* part = p.part + (int64_t)(2 * (blockIdx.x * L4_WARPS + w) + 1) * Cfg::FLOATS;
+        for (int i = tid; i < Cfg::FLOATS / 4; i += 32 * L4_WARPS) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = w; k < end; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(rows_s + k * Cfg::FLOATS + i * 4);
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+            }
+            if (all) finish(q, i / 32 / NT, i / 32 % NT, v, i % 32);
+            else __stcg(reinterpret_cast<float4*>(part + i * 4), v);
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid < 2 * L4_WARPS) {
+        join_s[tid] = 0;
+        if (piece_s[tid] >= 0 && (!(tid & 1) || tid == 1 || !same((tid >> 1) - 1))) {   // one of a group counts it
+            const PieceParts r = parts_s[tid];
+            if (r.count > 1) join_s[tid] = atomicAdd(p.arrived + r.w0, 1) == r.count - 1;
+        }
+    }
+    __syncthreads();
+    for (int k = 0; k < 2 * L4_WARPS; ++k) {   // whoever is last adds the parts, in the order of the list
+        if (!join_s[k]) continue;
+        __threadfence();
+        const PieceParts r = parts_s[k];
+        for (int i = tid; i < Cfg::FLOATS / 4; i += 32 * L4_WARPS) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int u = 0; u < r.count; ++u) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part + r.place<L4_WARPS>(u) * Cfg::FLOATS + i * 4));
+                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+            }
+            finish(piece_s[k], i / 32 / NT, i / 32 % NT, v, i % 32);
+        }
+        if (tid == 0) p.arrived[r.w0] = 0;
     }
 }
 
@@ -167,16 +439,15 @@ linear4_unpack_kernel(const Linear4Params p, __half* out, int64_t ld) {
     grid_dep_wait();
     grid_dep_launch();
     if (mt < p.MT && kb < p.KB) {
-        const uint4 w = __ldg(p.data + ((int64_t)mt * p.KB + kb) * 32 + lane);
+        const uint4 w = __ldg(p.data + p.unit(mt, kb) * 32 + lane);
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int grp = (kb * 64 + (s >> 1) * 32) >> p.logg;
             const bool live = grp < p.NG;
-            const int64_t at = ((int64_t)mt * p.NG + grp) * 8 + g;
-            const uint32_t sc = live ? __ldg(p.scales + at) : 0;
+            const uint32_t sc = live ? __ldg(p.scales + p.group8(mt, grp) + g) : 0;
             uint32_t z0, z1, a[4];
-            l4_zero(live ? p.zeros : nullptr, at, z0, z1);
+            l4_zero(live && p.zeros != nullptr ? __ldg(p.zeros + p.group8(mt, grp) + g) : 0x88u, z0, z1);
             l4_weights(v[s], z0, z1, a);
             const __half2 s2 = *reinterpret_cast<const __half2*>(&sc);
 #pragma unroll
@@ -201,7 +472,7 @@ struct PackParams {
     const uint8_t *q, *zeros;
     const __half* scales;
     int64_t qM, qK, sM, sG, zM, zG, M;
-    int K, KB, NG, MT;
+    int K, KB, NG, M4;      // M4: fours of row tiles
     uint32_t *data, *oscales;
     uint8_t* ozeros;
 };
@@ -211,11 +482,11 @@ __global__ void __launch_bounds__(256)
 linear4_pack_kernel(const PackParams p) {
     grid_dep_wait();
     grid_dep_launch();
-    const int64_t words = (int64_t)p.MT * p.KB * 128, pairs = (int64_t)p.MT * p.NG * 8;
+    const int64_t words = (int64_t)p.M4 * p.KB * 512, pairs = (int64_t)p.M4 * p.NG * 32;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
         const int s = (int)(i & 3), lane = (int)(i >> 2 & 31), g = lane >> 2, t = lane & 3;
-        const int64_t unit = i >> 7, mt = unit / p.KB;
-        const int kb = (int)(unit - mt * p.KB);
+        const int64_t unit = i >> 9, m4 = unit / p.KB, mt = m4 * 4 + (i >> 7 & 3);
+        const int kb = (int)(unit - m4 * p.KB);
         uint32_t w = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {   // nibble j: register j % 4, half j / 4
@@ -228,7 +499,7 @@ linear4_pack_kernel(const PackParams p) {
     }
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pairs; i += (int64_t)gridDim.x * 256) {
         const int g = (int)(i & 7);
-        const int64_t unit = i >> 3, mt = unit / p.NG, grp = unit - mt * p.NG;
+        const int64_t unit = i >> 5, m4 = unit / p.NG, grp = unit - m4 * p.NG, mt = m4 * 4 + (i >> 3 & 3);
         uint32_t s = 0, z = 0;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -242,12 +513,26 @@ linear4_pack_kernel(const PackParams p) {
     }
 }
 
-template <int MT, int NT>
+template <int NT>
 static int l4_launch(b200_ctx* ctx, const Linear4Params& p) {
-    constexpr int SMEM = L4_WARPS * 16 * MT * (8 * NT + 1) * 4;
-    auto kern = p.logg == 5 ? linear4_kernel<MT, NT, true> : linear4_kernel<MT, NT, false>;
-    if (SMEM > 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-    B200_CUDA(launch_dep(kern, dim3((unsigned)cdiv(p.MT, MT), (unsigned)cdiv(p.N, 8 * NT)), dim3(32 * L4_WARPS), SMEM, ctx->stream, 1, p));
+    auto kern = p.logg == 5 ? linear4_kernel<NT, true> : linear4_kernel<NT, false>;
+    B200_CUDA(launch_dep(kern, dim3((unsigned)p.MT, (unsigned)cdiv(p.N, 8 * NT)), dim3(32 * L4_WARPS), 0, ctx->stream, 1, p));
+    ctx->launches++;
+    return B200_OK;
+}
+template <int NT, bool SMALL, bool ZP>
+static int l4_stream_launch(b200_ctx* ctx, Linear4Params& p) {
+    using Cfg = L4Cfg<NT, SMALL>;
+    auto kern = linear4_stream_kernel<NT, SMALL, ZP>;
+    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::RING));
+    int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
+    if (grid > SK_FLAG_COUNT / L4_WARPS) grid = SK_FLAG_COUNT / L4_WARPS;
+    void* ws = nullptr;
+    int rc = ws_scratch(ctx, (size_t)grid * L4_WARPS * 2 * Cfg::FLOATS * sizeof(float), &ws);
+    if (rc) return rc;
+    p.part = static_cast<float*>(ws);
+    p.arrived = ctx->sk_flags;
+    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(32 * L4_WARPS), Cfg::RING, ctx->stream, 1, p));
     ctx->launches++;
     return B200_OK;
 }
@@ -269,10 +554,10 @@ int b200_q4_sizes(int64_t M, int64_t K, int64_t group, int64_t* data_bytes, int6
     int rc = l4_shape("q4_sizes", M, K, group);
     if (rc) return rc;
     B200_REQUIRE(data_bytes && scale_bytes && zero_bytes, B200_EINVAL, "q4_sizes: null argument");
-    const int64_t tiles = cdiv(M, 16);
-    *data_bytes = tiles * cdiv(K, 64) * 512;
-    *scale_bytes = tiles * (K / group) * 32;
-    *zero_bytes = tiles * (K / group) * 8;
+    const int64_t fours = cdiv(M, 64);
+    *data_bytes = fours * cdiv(K, 64) * 2048;
+    *scale_bytes = fours * (K / group) * 128;
+    *zero_bytes = fours * (K / group) * 32;
     return B200_OK;
 }
 
@@ -282,14 +567,14 @@ int b200_q4_pack(b200_ctx* ctx, const void* q, int64_t q_m, int64_t q_k, const v
     int rc = l4_shape("q4_pack", out->M, out->K, out->group);
     if (rc) return rc;
     B200_REQUIRE(q && scales && out->data && out->scales && (!zeros == !out->zeros), B200_EINVAL, "q4_pack: null array");
-    B200_REQUIRE((uintptr_t)out->data % 16 == 0 && (uintptr_t)out->scales % 4 == 0, B200_DECLINE_ALIGN, "q4_pack: the packed arrays' alignment");
+    B200_REQUIRE((uintptr_t)out->data % 16 == 0 && (uintptr_t)out->scales % 16 == 0 && (uintptr_t)out->zeros % 16 == 0, B200_DECLINE_ALIGN, "q4_pack: the packed arrays' alignment");
     B200_CUDA(cudaSetDevice(ctx->device));
     PackParams p = {};
     p.q = (const uint8_t*)q, p.scales = (const __half*)scales, p.zeros = (const uint8_t*)zeros;
     p.qM = q_m, p.qK = q_k, p.sM = s_m, p.sG = s_g, p.zM = z_m, p.zG = z_g;
-    p.M = out->M, p.K = (int)out->K, p.KB = (int)cdiv(out->K, 64), p.NG = (int)(out->K / out->group), p.MT = (int)cdiv(out->M, 16);
+    p.M = out->M, p.K = (int)out->K, p.KB = (int)cdiv(out->K, 64), p.NG = (int)(out->K / out->group), p.M4 = (int)cdiv(out->M, 64);
     p.data = (uint32_t*)out->data, p.oscales = (uint32_t*)out->scales, p.ozeros = (uint8_t*)out->zeros;
-    const int64_t blocks = cdiv((int64_t)p.MT * p.KB * 128, 256), most = (int64_t)ctx->prop.multiProcessorCount * 16;
+    const int64_t blocks = cdiv((int64_t)p.M4 * p.KB * 512, 256), most = (int64_t)ctx->prop.multiProcessorCount * 16;
     B200_CUDA(launch_dep(linear4_pack_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, ctx->stream, 1, p));
     ctx->launches++;
     return B200_OK;
@@ -306,7 +591,7 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
     B200_REQUIRE(epilogue >= B200_EPI_NONE && epilogue <= B200_EPI_GELU_TANH, B200_EINVAL, "matmul_q4: epilogue %d", epilogue);
     if (N == 0) return B200_OK;
     B200_REQUIRE(A->data && A->scales && B && out, B200_EINVAL, "matmul_q4: null array");
-    B200_REQUIRE((uintptr_t)A->data % 16 == 0 && (uintptr_t)A->scales % 4 == 0, B200_DECLINE_ALIGN, "matmul_q4: the packed arrays' alignment");
+    B200_REQUIRE((uintptr_t)A->data % 16 == 0 && (uintptr_t)A->scales % 16 == 0 && (uintptr_t)A->zeros % 16 == 0, B200_DECLINE_ALIGN, "matmul_q4: the packed arrays' alignment");
     B200_CUDA(cudaSetDevice(ctx->device));
     Linear4Params p = {};
     p.data = (const uint4*)A->data, p.scales = (const uint32_t*)A->scales, p.zeros = (const uint8_t*)A->zeros;
@@ -327,11 +612,20 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
         ctx->launches++;
         return gemm_f16_run(ctx, A->M, N, A->K, w, ld, B, ldb, bias, 0, out, ldo, out_dtype, epilogue, 1, 0, 0, 0);
     }
-    const bool wide = p.MT >= 8 * ctx->prop.multiProcessorCount;   // enough row tiles to give a block four
-    if (N <= 8) return wide ? l4_launch<4, 1>(ctx, p) : l4_launch<1, 1>(ctx, p);
-    if (N <= 16) return wide ? l4_launch<4, 2>(ctx, p) : l4_launch<1, 2>(ctx, p);
-    if (N <= 32) return l4_launch<1, 4>(ctx, p);
-    return l4_launch<1, 8>(ctx, p);
+    p.d_status = ctx->d_status;
+    const int nt = N <= 8 ? 1 : 2;
+    const double tiles = (double)cdiv(p.MT, 4) * (double)cdiv(N, 8 * nt) * p.KB;
+    if (tiles >= L4_STREAM_TILES) {
+        const auto go = [&](auto small, auto zp) {
+            return nt == 1 ? l4_stream_launch<1, decltype(small)::value, decltype(zp)::value>(ctx, p)
+                           : l4_stream_launch<2, decltype(small)::value, decltype(zp)::value>(ctx, p);
+        };
+        using yes = std::true_type;
+        using no = std::false_type;
+        if (p.logg == 5) return p.zeros ? go(yes(), yes()) : go(yes(), no());
+        return p.zeros ? go(no(), yes()) : go(no(), no());
+    }
+    return nt == 1 ? l4_launch<1>(ctx, p) : l4_launch<2>(ctx, p);
 }
 
 } // extern "C"

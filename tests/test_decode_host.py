@@ -131,7 +131,7 @@ def test_linear4_refusals():
     refused(20, jv.matmul4_, arr(np.int8, (40, 3)), w, x)
     n = [C.c_int64() for _ in range(3)]
     at = lambda: [C.byref(v) for v in n]  # noqa: E731
-    assert _lib.lib().b200_q4_sizes(40, 160, 32, *at()) == 0 and [v.value for v in n] == [3 * 3 * 512, 3 * 5 * 32, 3 * 5 * 8]
+    assert _lib.lib().b200_q4_sizes(40, 160, 32, *at()) == 0 and [v.value for v in n] == [3 * 4 * 512, 5 * 4 * 32, 5 * 4 * 8]
     assert _lib.lib().b200_q4_sizes(40, 160, 64, *at()) == 17 and _lib.lib().b200_q4_sizes(0, 64, 64, *at()) == 17
 
 

@@ -426,7 +426,8 @@ LINEAR = [  # N, M, K, group, zeros, epi
     (1, 1280, 1280, 64, False, "identity"), (1, 1, 32, 32, True, "identity"), (2, 17, 96, 32, True, "relu"), (8, 200, 128, 128, False, "gelu"),
     (9, 333, 640, 64, True, "identity"), (16, 1000, 384, 128, True, "gelu_tanh"), (17, 64, 1024, 32, False, "identity"),
     (33, 47, 256, 64, True, "gelu"), (64, 130, 512, 128, False, "relu"), (65, 130, 512, 128, True, "identity"), (300, 1001, 224, 32, True, "gelu"),
-    (5, 20000, 256, 64, True, "identity"), (1, 40000, 192, 64, False, "identity"), (3, 24, 8192, 64, False, "identity")]
+    (5, 20000, 256, 64, True, "identity"), (1, 40000, 192, 64, False, "identity"), (3, 24, 8192, 64, False, "identity"),
+    (9, 9001, 4096, 128, False, "identity"), (2, 20011, 1696, 32, True, "relu"), (40, 2500, 8192, 64, True, "identity"), (1, 66000, 576, 64, False, "gelu")]
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
