@@ -413,7 +413,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                         cache_halves<FP8>(wl[k], a[0], a[2]);
                         cache_halves<FP8>(wh[k], a[1], a[3]);
 #pragma unroll
-                        for (int i = 0; i < NT; ++i) mma_16816(s[i][grp], a, qb[i][hh * 4 + k][0], qb[i][hh * 4 + k][1]);
+                        for (int i = 0; i < NT; ++i) mma_16816_free(s[i][grp], a[0], a[1], a[2], a[3], qb[i][hh * 4 + k][0], qb[i][hh * 4 + k][1]);
                     }
                 }
             }
@@ -536,8 +536,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                     cf_values<FP8>(w[2][u], w[3][u], b1);
 #pragma unroll
                     for (int i = 0; i < NT; ++i) {
-                        mma_16816(o[i][2 * u], b0[0], b0[1], b1[0], b1[1], pb[i][grp][0], pb[i][grp][1]);
-                        mma_16816(o[i][2 * u + 1], b0[2], b0[3], b1[2], b1[3], pb[i][grp][0], pb[i][grp][1]);
+                        mma_16816_free(o[i][2 * u], b0[0], b0[1], b1[0], b1[1], pb[i][grp][0], pb[i][grp][1]);
+                        mma_16816_free(o[i][2 * u + 1], b0[2], b0[3], b1[2], b1[3], pb[i][grp][0], pb[i][grp][1]);
                     }
                 }
             }

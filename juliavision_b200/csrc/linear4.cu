@@ -100,12 +100,6 @@ __device__ __forceinline__ void l4_input(const Linear4Params& p, int n, int kb, 
     }
 }
 
-// The first product of a sum.
-__device__ __forceinline__ void l4_mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
 // A k block of a row tile: acc += the products of its groups by their scales.
 template <int NT, bool SMALL>
 __device__ __forceinline__ void l4_block(float (&acc)[NT][4], const uint4& w, const uint32_t* sc, const uint32_t* zb, const uint32_t (&x)[NT][8]) {
@@ -124,8 +118,8 @@ __device__ __forceinline__ void l4_block(float (&acc)[NT][4], const uint4& w, co
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t b0 = x[n][2 * (j * STEPS + k)], b1 = x[n][2 * (j * STEPS + k) + 1];
-                if (k == 0) l4_mma0(c[n], a, b0, b1);
-                else mma_16816(c[n], a, b0, b1);
+                if (k == 0) mma_16816_first(c[n], a[0], a[1], a[2], a[3], b0, b1);
+                else mma_16816_free(c[n], a[0], a[1], a[2], a[3], b0, b1);
             }
         }
 #pragma unroll
@@ -201,10 +195,10 @@ __device__ __forceinline__ void l4_bulk(uint32_t dst, const void* src, uint32_t 
 
 template <int NT, bool SMALL> struct L4Cfg {
     static constexpr int GROUPS = SMALL ? 2 : 1;
-    static constexpr int SCALES = 2048, ZEROS = SCALES + GROUPS * 128, X = ZEROS + GROUPS * 32,
-                         STAGE = X + NT * 1024;   // 64 rows' weights, scales, zero points; the tokens' inputs
-    static_assert(X % 16 == 0 && STAGE % 16 == 0, "16-byte copies");
-    static constexpr int RING = L4_WARPS * L4_STAGES * STAGE;
+    static constexpr int SCALES = 2048, ZEROS = SCALES + GROUPS * 128, END = ZEROS + GROUPS * 32;   // 64 rows' weights, scales, zero points
+    static constexpr int STAGE = (END + 127) / 128 * 128, X_STAGE = NT * 1024;   // the tokens' inputs apart, where the swizzle wants them
+    static constexpr int X_RING = L4_WARPS * L4_STAGES * X_STAGE, RING = L4_WARPS * L4_STAGES * STAGE;
+    static constexpr int SMEM = X_RING + RING + 1024;
     static constexpr int FLOATS = 4 * NT * 128;      // a warp's results of 64 rows
     static_assert(L4_WARPS * FLOATS * 4 <= RING, "the warps' results fit over the ring");
     static constexpr int CTAS = 2;
@@ -213,20 +207,25 @@ template <int NT, bool SMALL> struct L4Cfg {
 // NT tiles of 8 tokens.  Tiles of the list: (64 rows, NT token tiles, k block), the k block fastest.  ZP: there are zero points.
 template <int NT, bool SMALL, bool ZP>
 __global__ void __launch_bounds__(32 * L4_WARPS, L4Cfg<NT, SMALL>::CTAS)
-linear4_stream_kernel(const Linear4Params p) {
+linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Params p) {
     using Cfg = L4Cfg<NT, SMALL>;
     constexpr int GROUPS = Cfg::GROUPS;
-    extern __shared__ __align__(128) uint8_t l4_ring[];
+    extern __shared__ uint8_t l4_raw[];
     __shared__ __align__(8) uint64_t full_s[L4_WARPS][L4_STAGES];
     __shared__ PieceParts parts_s[2 * L4_WARPS];
     __shared__ long long piece_s[2 * L4_WARPS];                    // the pieces this block's warps have parts of: ended, last; -1: none
     __shared__ int join_s[2 * L4_WARPS], abort_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    uint8_t* const l4_x = l4_raw + ((1024 - (smem_u32(l4_raw) & 1023)) & 1023);
+    uint8_t* const l4_ring = l4_x + Cfg::X_RING;
     if (lane == 0) {
         for (int i = 0; i < L4_STAGES; ++i) mbar_init(&full_s[warp][i], 1);
         fence_barrier_init();
     }
-    if (tid == 0) abort_s = 0;
+    if (tid == 0) {
+        abort_s = 0;
+        prefetch_tmap(&tmapX);
+    }
     if (tid < 2 * L4_WARPS) piece_s[tid] = -1;
     __syncthreads();
     grid_dep_wait();
@@ -236,16 +235,13 @@ linear4_stream_kernel(const Linear4Params p) {
     const int me = blockIdx.x * L4_WARPS + warp;
     const long long from = me < shares.warps ? shares.begin(me) : 0, to = me < shares.warps ? shares.begin(me + 1) : 0;
     uint8_t* const ring = l4_ring + warp * L4_STAGES * Cfg::STAGE;
+    uint8_t* const xring = l4_x + warp * L4_STAGES * Cfg::X_STAGE;
 
     // The tile to be asked for next, everything about it carried along: a division for each would cost more than the tile's products.
-    // Inputs: token n's 64 in eight chunks of 16 bytes, an odd token's halves changed over, so that the eight lanes of a phase, four
-    // chunks of two tokens, meet all banks.  Lane (n, chunk) has tokens n, n + 4, ... of the 8 NT.
-    const int tiles = (int)(to - from), xn = lane >> 3, xk = (lane & 7) * 8;
-    const uint32_t x_at = Cfg::X + xn * 128 + (((lane & 7) ^ (xn & 1) << 2) << 4);
+    // One lane asks for all of it, the inputs through a tensor map: copied 16 bytes a lane they cost a fifth of the loop's instructions.
+    const int tiles = (int)(to - from);
     int asked = 0, ask_s = 0, ask_kb, ask_tg;
     const uint8_t *ask_data, *ask_scales, *ask_zeros;
-    const __half* ask_x;
-    auto inputs = [&]() { ask_x = p.x + (int64_t)(ask_tg * NT * 8 + xn) * p.ldx + ask_kb * 64 + xk; };
     {
         const int piece = (int)floor_div(from, p.KB), rg = piece / tgs;
         ask_kb = (int)(from - (long long)piece * p.KB);
@@ -253,54 +249,32 @@ linear4_stream_kernel(const Linear4Params p) {
         ask_data = reinterpret_cast<const uint8_t*>(p.data) + ((int64_t)rg * p.KB + ask_kb) * 2048;
         ask_scales = reinterpret_cast<const uint8_t*>(p.scales) + (int64_t)rg * p.NG * 128;      // of the rows
         ask_zeros = p.zeros + (int64_t)rg * p.NG * 32;
-        inputs();
     }
-    auto fetch = [&]() {          // a commit group even when there is none
-        if (asked < tiles) {
+    auto fetch = [&]() {
+        if (asked >= tiles) return;
+        if (lane == 0) {
             const uint32_t dst = smem_u32(ring + ask_s * Cfg::STAGE);
-            if (lane == 0) {
-                const int g0 = (ask_kb * 64) >> p.logg, groups = SMALL && p.NG - g0 < GROUPS ? 1 : GROUPS;
-                uint64_t* bar = &full_s[warp][ask_s];
-                mbar_arrive_expect_tx(bar, 2048 + groups * (ZP ? 160 : 128));
-                l4_bulk(dst, ask_data, 2048, bar);
-                l4_bulk(dst + Cfg::SCALES, ask_scales + g0 * 128, groups * 128, bar);
-                if (ZP) l4_bulk(dst + Cfg::ZEROS, ask_zeros + g0 * 32, groups * 32, bar);
-            }
-            const int n = ask_tg * NT * 8 + xn;
-            const bool in = ask_kb * 64 + xk < p.K;        // K is a multiple of 32
-#pragma unroll
-            for (int i = 0; i < 2 * NT; ++i) {
-                const bool live = in && n + 4 * i < p.N;
-                const __half* src = live ? ask_x + i * 4 * p.ldx : p.x;
-                if (p.whole) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst + x_at + i * 512), "l"(src), "r"(live ? 16 : 0) : "memory");
-                } else {
-                    uint32_t v[4] = {0, 0, 0, 0};
-                    if (live) {
-                        const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) v[c] = u[2 * c] | (uint32_t)u[2 * c + 1] << 16;
-                    }
-                    st_shared_v4(dst + x_at + i * 512, v);
-                }
-            }
-            ++asked;
-            if (++ask_s == L4_STAGES) ask_s = 0;
-            ask_data += 2048;
-            ask_x += 64;
-            if (++ask_kb == p.KB) {      // the next piece: other tokens with the same rows, or the next rows
-                ask_kb = 0;
-                if (++ask_tg == tgs) {
-                    ask_tg = 0;
-                    ask_scales += (int64_t)p.NG * 128;
-                    ask_zeros += (int64_t)p.NG * 32;
-                } else {
-                    ask_data -= (int64_t)p.KB * 2048;
-                }
-                inputs();
+            const int g0 = (ask_kb * 64) >> p.logg, groups = SMALL && p.NG - g0 < GROUPS ? 1 : GROUPS;
+            uint64_t* bar = &full_s[warp][ask_s];
+            mbar_arrive_expect_tx(bar, 2048 + groups * (ZP ? 160 : 128) + Cfg::X_STAGE);
+            l4_bulk(dst, ask_data, 2048, bar);
+            l4_bulk(dst + Cfg::SCALES, ask_scales + g0 * 128, groups * 128, bar);
+            if (ZP) l4_bulk(dst + Cfg::ZEROS, ask_zeros + g0 * 32, groups * 32, bar);
+            tma_load_2d(xring + ask_s * Cfg::X_STAGE, &tmapX, bar, ask_kb * 64, ask_tg * NT * 8);
+        }
+        ++asked;
+        if (++ask_s == L4_STAGES) ask_s = 0;
+        ask_data += 2048;
+        if (++ask_kb == p.KB) {      // the next piece: other tokens with the same rows, or the next rows
+            ask_kb = 0;
+            if (++ask_tg == tgs) {
+                ask_tg = 0;
+                ask_scales += (int64_t)p.NG * 128;
+                ask_zeros += (int64_t)p.NG * 32;
+            } else {
+                ask_data -= (int64_t)p.KB * 2048;
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     for (int i = 0; i < L4_STAGES - 1; ++i) fetch();
 
@@ -332,18 +306,18 @@ linear4_stream_kernel(const Linear4Params p) {
     uint32_t phase = 0;
     bool first = true;            // the piece at hand may have begun before this share
     for (int at = 0; at < tiles; ++at) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(L4_STAGES - 2) : "memory");
         if (!mbar_wait(&full_s[warp][s], phase, p.d_status, KST_WAIT_FULL, &abort_s)) break;
         __syncwarp();             // this stage is there for every lane, and the one that is asked for now has been read
         fetch();
         const uint8_t* st = ring + s * Cfg::STAGE;
+        const uint8_t* xs = xring + s * Cfg::X_STAGE + g * 128;
         if (++s == L4_STAGES) s = 0, phase ^= 1;
         uint32_t x[NT][8];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const uint4 v = *reinterpret_cast<const uint4*>(st + Cfg::X + (n * 8 + g) * 128 + (((half * 4 + t) ^ (g & 1) << 2) << 4));
+                const uint4 v = *reinterpret_cast<const uint4*>(xs + n * 1024 + (((half * 4 + t) ^ g) << 4));
                 x[n][4 * half] = v.x, x[n][4 * half + 1] = v.y, x[n][4 * half + 2] = v.z, x[n][4 * half + 3] = v.w;
             }
 #pragma unroll
@@ -524,15 +498,20 @@ template <int NT, bool SMALL, bool ZP>
 static int l4_stream_launch(b200_ctx* ctx, Linear4Params& p) {
     using Cfg = L4Cfg<NT, SMALL>;
     auto kern = linear4_stream_kernel<NT, SMALL, ZP>;
-    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::RING));
+    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    CUtensorMap mx;               // rows of 64 inputs, zeros past the ends
+    const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)p.N}, strides[1] = {(uint64_t)p.ldx * 2};
+    const uint32_t box[2] = {64, 8 * NT};
+    int rc = make_tmap(ctx, &mx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
     int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
     if (grid > SK_FLAG_COUNT / L4_WARPS) grid = SK_FLAG_COUNT / L4_WARPS;
     void* ws = nullptr;
-    int rc = ws_scratch(ctx, (size_t)grid * L4_WARPS * 2 * Cfg::FLOATS * sizeof(float), &ws);
+    rc = ws_scratch(ctx, (size_t)grid * L4_WARPS * 2 * Cfg::FLOATS * sizeof(float), &ws);
     if (rc) return rc;
     p.part = static_cast<float*>(ws);
     p.arrived = ctx->sk_flags;
-    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(32 * L4_WARPS), Cfg::RING, ctx->stream, 1, p));
+    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(32 * L4_WARPS), Cfg::SMEM, ctx->stream, 1, mx, p));
     ctx->launches++;
     return B200_OK;
 }
@@ -615,7 +594,7 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
     p.d_status = ctx->d_status;
     const int nt = N <= 8 ? 1 : 2;
     const double tiles = (double)cdiv(p.MT, 4) * (double)cdiv(N, 8 * nt) * p.KB;
-    if (tiles >= L4_STREAM_TILES) {
+    if (tiles >= L4_STREAM_TILES && p.whole) {
         const auto go = [&](auto small, auto zp) {
             return nt == 1 ? l4_stream_launch<1, decltype(small)::value, decltype(zp)::value>(ctx, p)
                            : l4_stream_launch<2, decltype(small)::value, decltype(zp)::value>(ctx, p);
