@@ -19,8 +19,8 @@
 // results of the last.  (Blocks that walked the list together lost 8 us at every change of piece, the slowest warp's tile and
 // the trips to memory that nothing hid: 32 x 8192 tokens 62 us.)  A piece that one warp holds whole is stored at once.  Of the
 // others, what ends inside a warp's share waits in the workspace; the last pieces of a block's warps are joined in shared
-// memory at its end, and whichever block is last to bring a part of a piece joins them all, in the order of the list: the
-// result does not depend on timing.
+// memory at its end, and a second launch joins what then still lies in several places, in the order of the list: the result
+// does not depend on timing.
 #include <cuda_fp16.h>
 
 #include "cache8.cuh"
@@ -30,9 +30,14 @@ namespace b200 {
 
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
+constexpr int CF_JOIN_THREADS = 256;
 constexpr int CF_KEYS = 64;                      // keys a warp takes at a time: a tile of the list
 constexpr int CF_GROUPS = CF_KEYS / 16;          // of one page each
 
+struct CfJoin {               // a piece that lies in several places: sequence, key head, row tile, rows (0: there is none), where
+    int b, h, rt, rows;
+    PieceParts parts;
+};
 struct CacheAttnParams {
     CacheView c;
     const __half* q;
@@ -43,7 +48,7 @@ struct CacheAttnParams {
     int causal, out_f32, whole, out_whole;   // rows of q start on 16-byte boundaries, fours of out on their own size
     float scale_log2;
     float* part;                          // [warp][ended inside its share, or its last][row][EP + 4]
-    int* arrived;                         // [warp], zero between launches
+    CfJoin* joins;                        // [warp]
 };
 
 template <int EP, int NT> struct CfCfg {
@@ -57,7 +62,6 @@ template <int EP, int NT> struct CfCfg {
     static constexpr int SMEM = RING + 1024;                  // the swizzle wants the ring on a 1024-byte boundary
     static_assert(CF_WARPS * RT * ROW * 4 <= RING, "the warps' rows fit over the ring");
     static constexpr int BLOCKS = 148 * CTAS;                 // of a launch at most
-    static_assert(BLOCKS * CF_WARPS <= SK_FLAG_COUNT && RT * (BLOCKS + 3) * 4 <= RING, "a counter a warp; the parts' weights fit over the ring");
 };
 
 // Byte of 16-byte chunk c of row r of a stage's side, as the tensor map's swizzle lays it: 128-byte rows with the chunk turned
@@ -109,6 +113,21 @@ __device__ __forceinline__ float cf_max3(float a, float b, float c) {
     return d;
 }
 
+// Four results of a row of a piece.
+__device__ __forceinline__ void cf_store(const CacheAttnParams& p, int rows, int b, int h, int rt, int row, int e4, float4 v) {
+    const int r = rt * rows + row, l = r / p.G;
+    const int64_t at = l * p.oL + (h * p.G + r - l * p.G) * p.oH + b * p.oB + e4;
+    if (e4 >= p.c.E) return;
+    if (p.out_f32) {
+        float* d = (float*)p.out + at;
+        if (p.out_whole) *reinterpret_cast<float4*>(d) = v;
+        else d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+    } else {
+        __half* d = (__half*)p.out + at;
+        if (p.out_whole) *reinterpret_cast<uint2*>(d) = make_uint2(cf_pack(v.x, v.y), cf_pack(v.z, v.w));
+        else d[0] = __float2half_rn(v.x), d[1] = __float2half_rn(v.y), d[2] = __float2half_rn(v.z), d[3] = __float2half_rn(v.w);
+    }
+}
 // the transpose of an 8 x 8 matrix of fp16, two neighbours of a row a lane
 __device__ __forceinline__ uint32_t cf_transpose(uint32_t v) {
     uint32_t r;
@@ -135,7 +154,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     __shared__ int where_s[CF_WARPS], abort_s;
     __shared__ CfPiece given_s[2 * CF_WARPS];                          // parts of pieces this block's warps have: ended, last
     __shared__ PieceParts parts_s[2 * CF_WARPS];
-    __shared__ int has_s[2 * CF_WARPS], join_s[2 * CF_WARPS];          // there is one; this block joins its piece
+    __shared__ int has_s[2 * CF_WARPS];                                // there is one
     if (threadIdx.x < 2 * CF_WARPS) has_s[threadIdx.x] = 0;
     uint8_t* cf_smem = cf_raw + ((1024 - (smem_u32(cf_raw) & 1023)) & 1023);
     const CacheView& c = p.c;
@@ -313,21 +332,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             }
         }
     };
-    // Four results of a row of a piece.
-    auto store = [&](const CfPiece& q, int row, int e4, float4 v) {
-        const int r = q.rt * RT + row, l = r / p.G;
-        const int64_t at = l * p.oL + (q.h * p.G + r - l * p.G) * p.oH + q.b * p.oB + e4;
-        if (e4 >= c.E) return;
-        if (p.out_f32) {
-            float* d = (float*)p.out + at;
-            if (p.out_whole) *reinterpret_cast<float4*>(d) = v;
-            else d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
-        } else {
-            __half* d = (__half*)p.out + at;
-            if (p.out_whole) *reinterpret_cast<uint2*>(d) = make_uint2(cf_pack(v.x, v.y), cf_pack(v.z, v.w));
-            else d[0] = __float2half_rn(v.x), d[1] = __float2half_rn(v.y), d[2] = __float2half_rn(v.z), d[3] = __float2half_rn(v.w);
-        }
-    };
+    auto store = [&](const CfPiece& q, int row, int e4, float4 v) { cf_store(p, RT, q.b, q.h, q.rt, row, e4, v); };
     float o[NT][W / 2][4], mref[NT][2], vref = 0.f, vinv = 0.f;     // mref: rows' reference points; vref: the value scale P is relative to
     uint64_t lsum[NT];
     const int e0 = W * (EP == 128 ? cf_chunk(g) : g);               // this lane's W elements of its rows
@@ -594,106 +599,85 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 const float inv = l == 0.f ? 1.f : 1.f / l;
                 store(q, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
             } else {
-                __stcg(reinterpret_cast<float4*>(part + row * ROW + e4), v);
-                if (e4 == 0) __stcg(reinterpret_cast<float2*>(part + row * ROW + EP), make_float2(M, l));
+                *reinterpret_cast<float4*>(part + row * ROW + e4) = v;
+                if (e4 == 0) *reinterpret_cast<float2*>(part + row * ROW + EP) = make_float2(M, l);
             }
         }
     }
-    __threadfence();
-    __syncthreads();
-    if (tid < 2 * CF_WARPS) {
-        join_s[tid] = 0;
-        if (has_s[tid] && (!(tid & 1) || tid == 1 || !same((tid >> 1) - 1))) {   // one of a group counts it
-            const PieceParts r = parts_s[tid];
-            if (r.count > 1) join_s[tid] = atomicAdd(p.arrived + r.w0, 1) == r.count - 1;
-        }
+    if (lane == 0) {      // the warp in whose share a piece begins says where its parts are
+        const CfPiece& q = given_s[2 * warp + 1];
+        CfJoin d = {};
+        if (has_s[2 * warp + 1] && q.j0 == 0 && parts_s[2 * warp + 1].count > 1)
+            d = {q.b, q.h, q.rt, q.rows, parts_s[2 * warp + 1]};
+        p.joins[me] = d;
     }
-    __syncthreads();
-    for (int k = 0; k < 2 * CF_WARPS; ++k) {
-        if (!join_s[k]) continue;
-        __threadfence();
-        const CfPiece& q = given_s[k];
-        const PieceParts r = parts_s[k];
-        auto part_of = [&](int i) { return p.part + r.place<CF_WARPS>(i) * RT * ROW; };
-        constexpr int AT_ONCE = 16;   // loads in flight: each is a trip to L2
-        if (r.count <= AT_ONCE) {
-            for (int i = tid; i < q.rows * (EP / 4); i += CF_THREADS) {
-                const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
+}
+
+// One block a warp of the launch before: joins the parts of the piece that began in its share, in the order of the list, several parts
+// at a time where there are more threads than fours of results.
+template <int EP, int NT>
+__global__ void __launch_bounds__(CF_JOIN_THREADS)
+cache_attention_join_kernel(const CacheAttnParams p) {
+    constexpr int ROW = CfCfg<EP, NT>::ROW, RT = CfCfg<EP, NT>::RT, AT_ONCE = 8;   // parts in flight: each is a trip to L2
+    __shared__ float4 rows_s[CF_JOIN_THREADS];
+    __shared__ float2 ml_s[CF_JOIN_THREADS];
+    grid_dep_wait();
+    grid_dep_launch();
+    const CfJoin d = p.joins[blockIdx.x];
+    const int items = d.rows * (EP / 4), tid = threadIdx.x;
+    if (items == 0) return;
+    const int groups = items < CF_JOIN_THREADS ? CF_JOIN_THREADS / items : 1, grp = items < CF_JOIN_THREADS ? tid / items : 0;
+    for (int i0 = 0; i0 < items; i0 += CF_JOIN_THREADS) {      // once, but for more results than threads
+        const int i = items < CF_JOIN_THREADS ? tid - grp * items : i0 + tid;
+        const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
+        float M = -INFINITY, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (grp < groups && i < items)
+            for (int k0 = grp; k0 < d.parts.count; k0 += groups * AT_ONCE) {
                 float2 ml[AT_ONCE];
                 float4 x[AT_ONCE];
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u) {
+                    const int k = k0 + u * groups;
                     ml[u] = make_float2(-INFINITY, 0.f);
                     x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (u < r.count) {
-                        const float* src = part_of(u) + row * ROW;
-                        ml[u] = __ldcg(reinterpret_cast<const float2*>(src + EP));
-                        x[u] = __ldcg(reinterpret_cast<const float4*>(src + e4));
+                    if (k < d.parts.count) {
+                        const float* src = p.part + d.parts.place<CF_WARPS>(k) * RT * ROW + row * ROW;
+                        ml[u] = *reinterpret_cast<const float2*>(src + EP);
+                        x[u] = *reinterpret_cast<const float4*>(src + e4);
                     }
                 }
-                float M = -INFINITY, l = 0.f;
+                float top = M;
 #pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u) M = fmaxf(M, ml[u].x);
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int u = 0; u < AT_ONCE; ++u) top = fmaxf(top, ml[u].x);
+                const float a = M == top ? 1.f : cf_ex2(M - top);      // 1: both may be -inf, with zeros or a NaN
+                v.x *= a, v.y *= a, v.z *= a, v.w *= a, l *= a;
 #pragma unroll
                 for (int u = 0; u < AT_ONCE; ++u) {
-                    const float f = ml[u].x == M ? 1.f : cf_ex2(ml[u].x - M);
+                    const float f = ml[u].x == top ? 1.f : cf_ex2(ml[u].x - top);
                     v.x = fmaf(x[u].x, f, v.x), v.y = fmaf(x[u].y, f, v.y), v.z = fmaf(x[u].z, f, v.z), v.w = fmaf(x[u].w, f, v.w);
                     l = fmaf(ml[u].y, f, l);
                 }
-                const float inv = l == 0.f ? 1.f : 1.f / l;
-                store(q, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+                M = top;
             }
-            if (tid == 0) p.arrived[r.w0] = 0;
-            continue;
-        }
-        // Rows' weights first, a part a lane: what is left is a sum whose loads wait for nothing.
-        float* weight = rows_s;       // [row][part]
-        for (int row = warp; row < q.rows; row += CF_WARPS) {
-            constexpr int KEPT = 4;   // a lane's first few are asked for once
-            float M = -INFINITY, l = 0.f;
-            float2 ml[KEPT];
-            auto load = [&](int i) { return __ldcg(reinterpret_cast<const float2*>(part_of(i) + row * ROW + EP)); };
-#pragma unroll
-            for (int u = 0; u < KEPT; ++u) ml[u] = lane + 32 * u < r.count ? load(lane + 32 * u) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int u = 0; u < KEPT; ++u) M = fmaxf(M, ml[u].x);
-            for (int i = lane + 32 * KEPT; i < r.count; i += 32) M = fmaxf(M, load(i).x);
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-            auto weigh = [&](int i, float2 v) {
-                const float f = v.x == M ? 1.f : cf_ex2(v.x - M);
-                weight[row * r.count + i] = f;
-                l = fmaf(v.y, f, l);
-            };
-#pragma unroll
-            for (int u = 0; u < KEPT; ++u)
-                if (lane + 32 * u < r.count) weigh(lane + 32 * u, ml[u]);
-            for (int i = lane + 32 * KEPT; i < r.count; i += 32) weigh(i, load(i));
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
-            if (lane == 0) weight[q.rows * r.count + row] = l == 0.f ? 1.f : 1.f / l;
-        }
-        __syncthreads();
-        for (int i = tid; i < q.rows * (EP / 4); i += CF_THREADS) {
-            const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k0 = 0; k0 < r.count; k0 += AT_ONCE) {
-                float4 x[AT_ONCE];
-#pragma unroll
-                for (int i2 = 0; i2 < AT_ONCE; ++i2)
-                    x[i2] = k0 + i2 < r.count ? __ldcg(reinterpret_cast<const float4*>(part_of(k0 + i2) + row * ROW + e4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int i2 = 0; i2 < AT_ONCE; ++i2) {
-                    const float f = k0 + i2 < r.count ? weight[row * r.count + k0 + i2] : 0.f;
-                    v.x = fmaf(x[i2].x, f, v.x), v.y = fmaf(x[i2].y, f, v.y), v.z = fmaf(x[i2].z, f, v.z), v.w = fmaf(x[i2].w, f, v.w);
-                }
+        if (groups > 1) {
+            rows_s[tid] = v;
+            ml_s[tid] = make_float2(M, l);
+            __syncthreads();
+            if (grp > 0) return;
+            for (int k = 1; k < groups; ++k) M = fmaxf(M, ml_s[k * items + i].x);
+            float f = ml_s[i].x == M ? 1.f : cf_ex2(ml_s[i].x - M);
+            v.x *= f, v.y *= f, v.z *= f, v.w *= f, l *= f;
+            for (int k = 1; k < groups; ++k) {
+                const float2 ml = ml_s[k * items + i];
+                const float4 x = rows_s[k * items + i];
+                f = ml.x == M ? 1.f : cf_ex2(ml.x - M);
+                v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
+                l = fmaf(ml.y, f, l);
             }
-            const float inv = weight[q.rows * r.count + row];
-            store(q, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
-        if (tid == 0) p.arrived[r.w0] = 0;
-        __syncthreads();
+        const float inv = l == 0.f ? 1.f : 1.f / l;
+        if (i < items && grp == 0) cf_store(p, RT, d.b, d.h, d.rt, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     }
 }
 
@@ -722,12 +706,14 @@ static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     const double most = (double)tiles * rts * p.c.H * p.B / CF_WARPS;
     if (most + 1 < (double)grid) grid = (int64_t)most + 1;
     void* ws = nullptr;
-    rc = ws_scratch(ctx, (size_t)grid * CF_WARPS * 2 * Cfg::RT * Cfg::ROW * sizeof(float), &ws);
+    const size_t floats = (size_t)grid * CF_WARPS * 2 * Cfg::RT * Cfg::ROW;
+    rc = ws_scratch(ctx, floats * sizeof(float) + (size_t)grid * CF_WARPS * sizeof(CfJoin), &ws);
     if (rc) return rc;
     p.part = static_cast<float*>(ws);
-    p.arrived = ctx->sk_flags;
+    p.joins = reinterpret_cast<CfJoin*>(p.part + floats);
     B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(CF_THREADS), Cfg::SMEM, ctx->stream, 1, mk, mv, p));
-    ctx->launches++;
+    B200_CUDA(launch_dep(cache_attention_join_kernel<EP, NT>, dim3((unsigned)grid * CF_WARPS), dim3(CF_JOIN_THREADS), 0, ctx->stream, 1, p));
+    ctx->launches += 2;
     return B200_OK;
 }
 

@@ -13,7 +13,7 @@
 // Two kernels for few tokens.  A small weight, whose rows do not fill the GPU for long, is a chain of round trips: a block takes 16
 // rows, its warps share K and have all their loads in flight at once (linear4_kernel).  A large one is bandwidth-bound: the list of
 // (64 rows, 8 or 16 tokens, k block) is dealt out to all warps in equal contiguous shares, each streamed by bulk copies through a ring
-// of its own; parts of rows meet at the ends of blocks (linear4_stream_kernel, shares.cuh).
+// of its own; parts of rows meet at the ends of blocks and in a second launch (linear4_stream_kernel, shares.cuh).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -45,7 +45,6 @@ struct Linear4Params {
     int logg;                     // log2 of the group size
     int out_f32, epi, whole;
     float* part;                  // [place][row tile, token tile][lane][4] (linear4_stream_kernel)
-    int* arrived;
     int* d_status;
 
     __device__ __forceinline__ int64_t unit(int mt, int kb) const { return ((int64_t)(mt >> 2) * KB + kb) * 4 + (mt & 3); }
@@ -204,6 +203,17 @@ template <int NT, bool SMALL> struct L4Cfg {
     static constexpr int CTAS = 2;
 };
 
+// Results of row tile i, token tile n of piece q as lane ln of the warp has them.
+template <int NT> __device__ __forceinline__ void l4_finish(const Linear4Params& p, int tgs, long long q, int i, int n, const float4& v, int ln) {
+    const int rg = (int)q / tgs, tg = (int)q % tgs;
+    const int64_t m = (int64_t)(rg * 4 + i) * 16 + (ln >> 2);
+    const int c = (tg * NT + n) * 8 + 2 * (ln & 3);
+    l4_store(p, m, c, v.x);
+    l4_store(p, m, c + 1, v.y);
+    l4_store(p, m + 8, c, v.z);
+    l4_store(p, m + 8, c + 1, v.w);
+}
+
 // NT tiles of 8 tokens.  Tiles of the list: (64 rows, NT token tiles, k block), the k block fastest.  ZP: there are zero points.
 template <int NT, bool SMALL, bool ZP>
 __global__ void __launch_bounds__(32 * L4_WARPS, L4Cfg<NT, SMALL>::CTAS)
@@ -214,7 +224,7 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
     __shared__ __align__(8) uint64_t full_s[L4_WARPS][L4_STAGES];
     __shared__ PieceParts parts_s[2 * L4_WARPS];
     __shared__ long long piece_s[2 * L4_WARPS];                    // the pieces this block's warps have parts of: ended, last; -1: none
-    __shared__ int join_s[2 * L4_WARPS], abort_s;
+    __shared__ int abort_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* const l4_x = l4_raw + ((1024 - (smem_u32(l4_raw) & 1023)) & 1023);
     uint8_t* const l4_ring = l4_x + Cfg::X_RING;
@@ -286,15 +296,7 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.f;
     };
-    auto finish = [&](long long q, int i, int n, const float4& v, int ln) {   // results of row tile i, token tile n as lane ln has them
-        const int rg = (int)q / tgs, tg = (int)q % tgs;
-        const int64_t m = (int64_t)(rg * 4 + i) * 16 + (ln >> 2);
-        const int c = (tg * NT + n) * 8 + 2 * (ln & 3);
-        l4_store(p, m, c, v.x);
-        l4_store(p, m, c + 1, v.y);
-        l4_store(p, m + 8, c, v.z);
-        l4_store(p, m + 8, c + 1, v.w);
-    };
+    auto finish = [&](long long q, int i, int n, const float4& v, int ln) { l4_finish<NT>(p, tgs, q, i, n, v, ln); };
     auto keep = [&](float* to_p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -373,34 +375,32 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
                 v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
             }
             if (all) finish(q, i / 32 / NT, i / 32 % NT, v, i % 32);
-            else __stcg(reinterpret_cast<float4*>(part + i * 4), v);
+            else *reinterpret_cast<float4*>(part + i * 4) = v;
         }
     }
-    __threadfence();
+}
+
+// One block a piece: the sum of its parts, in the order of the list, where they lie in several places.
+template <int NT, bool SMALL>
+__global__ void __launch_bounds__(32 * NT * 4)
+linear4_join_kernel(const Linear4Params p, int64_t warps) {
+    using Cfg = L4Cfg<NT, SMALL>;
+    __shared__ PieceParts parts_s;
+    const long long q = blockIdx.x;
+    const int i = threadIdx.x, tgs = (p.N + 8 * NT - 1) / (8 * NT);
+    if (i == 0) parts_s = PieceParts::of<L4_WARPS>(Shares((long long)(p.MT + 3) / 4 * tgs * p.KB, (int)warps), q * p.KB, (q + 1) * p.KB);
     __syncthreads();
-    if (tid < 2 * L4_WARPS) {
-        join_s[tid] = 0;
-        if (piece_s[tid] >= 0 && (!(tid & 1) || tid == 1 || !same((tid >> 1) - 1))) {   // one of a group counts it
-            const PieceParts r = parts_s[tid];
-            if (r.count > 1) join_s[tid] = atomicAdd(p.arrived + r.w0, 1) == r.count - 1;
-        }
-    }
-    __syncthreads();
-    for (int k = 0; k < 2 * L4_WARPS; ++k) {   // whoever is last adds the parts, in the order of the list
-        if (!join_s[k]) continue;
-        __threadfence();
-        const PieceParts r = parts_s[k];
-        for (int i = tid; i < Cfg::FLOATS / 4; i += 32 * L4_WARPS) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    grid_dep_wait();
+    grid_dep_launch();
+    const PieceParts r = parts_s;
+    if (r.w0 == r.w1 || r.count == 1) return;     // a warp or a block had it whole
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-            for (int u = 0; u < r.count; ++u) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part + r.place<L4_WARPS>(u) * Cfg::FLOATS + i * 4));
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-            }
-            finish(piece_s[k], i / 32 / NT, i / 32 % NT, v, i % 32);
-        }
-        if (tid == 0) p.arrived[r.w0] = 0;
+    for (int u = 0; u < r.count; ++u) {
+        const float4 x = *reinterpret_cast<const float4*>(p.part + r.place<L4_WARPS>(u) * Cfg::FLOATS + i * 4);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
+    l4_finish<NT>(p, tgs, q, i / 32 / NT, i / 32 % NT, v, i % 32);
 }
 
 // The weight as dense fp16 (M, K), for many tokens: a block writes 64 rows of two k blocks through shared memory.
@@ -505,14 +505,14 @@ static int l4_stream_launch(b200_ctx* ctx, Linear4Params& p) {
     int rc = make_tmap(ctx, &mx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.x, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
-    if (grid > SK_FLAG_COUNT / L4_WARPS) grid = SK_FLAG_COUNT / L4_WARPS;
     void* ws = nullptr;
     rc = ws_scratch(ctx, (size_t)grid * L4_WARPS * 2 * Cfg::FLOATS * sizeof(float), &ws);
     if (rc) return rc;
     p.part = static_cast<float*>(ws);
-    p.arrived = ctx->sk_flags;
     B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(32 * L4_WARPS), Cfg::SMEM, ctx->stream, 1, mx, p));
-    ctx->launches++;
+    const int64_t pieces = cdiv(p.MT, 4) * cdiv(p.N, 8 * NT);
+    B200_CUDA(launch_dep(linear4_join_kernel<NT, SMALL>, dim3((unsigned)pieces), dim3(32 * NT * 4), 0, ctx->stream, 1, p, grid * L4_WARPS));
+    ctx->launches += 2;
     return B200_OK;
 }
 
