@@ -169,6 +169,7 @@ def host():
         at = lambda f: C.cast(f, C.c_void_p).value
         m.bind(at(L.b200_gemm_f16), at(L.b200_gemv), at(L.b200_attention_f16_bias), at(L.b200_layernorm),
                at(L.b200_conv2d_grouped_f16))
+        m.binddecode(at(L.b200_rotary_f16), at(L.b200_cache_append), at(L.b200_cache_read), at(L.b200_cache_attention), at(L.b200_matmul_q4))
         _host = m
     return _host
 

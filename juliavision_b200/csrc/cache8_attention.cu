@@ -491,7 +491,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 vref = vnew;
                 vinv = vref > 0x1p-100f ? 128.f / vref : 0.f;   // 0 while there are only pages of zeros
             }
-            uint32_t pb[NT][NG][2];
+            uint32_t pb[NT][NG][2], pl[NT][NG][2];   // the weights' upper and lower halves
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 const uint64_t nm = pack2(mref[i][0] == -INFINITY ? 0.f : -mref[i][0], mref[i][1] == -INFINITY ? 0.f : -mref[i][1]);
@@ -512,8 +512,15 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                         for (int k = 0; k < 4; ++k)
                             if (x[k] == -INFINITY) e[k] = 0.f;
                     }
-                    pb[i][grp][0] = cf_transpose(cf_pack(e[0], e[1]));
-                    pb[i][grp][1] = cf_transpose(cf_pack(e[2], e[3]));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t hi = cf_pack(e[2 * k], e[2 * k + 1]);
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                        float r0, r1;
+                        unpack2(add2(pack2(e[2 * k], e[2 * k + 1]), pack2(-back.x, -back.y)), r0, r1);
+                        pb[i][grp][k] = cf_transpose(hi);
+                        pl[i][grp][k] = cf_transpose(cf_pack(r0, r1));
+                    }
                 }
             }
             if (!mbar_wait(&full_s[warp][1], phase, c.d_status, KST_WAIT_FULL, &abort_s)) break;
@@ -543,6 +550,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                     for (int i = 0; i < NT; ++i) {
                         mma_16816_free(o[i][2 * u], b0[0], b0[1], b1[0], b1[1], pb[i][grp][0], pb[i][grp][1]);
                         mma_16816_free(o[i][2 * u + 1], b0[2], b0[3], b1[2], b1[3], pb[i][grp][0], pb[i][grp][1]);
+                        mma_16816_free(o[i][2 * u], b0[0], b0[1], b1[0], b1[1], pl[i][grp][0], pl[i][grp][1]);
+                        mma_16816_free(o[i][2 * u + 1], b0[2], b0[3], b1[2], b1[3], pl[i][grp][0], pl[i][grp][1]);
                     }
                 }
             }
@@ -698,7 +707,8 @@ static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     int rc = cf_map(ctx, &mk, p.c.k, p.c, p.c.kT, p.c.kH, p.c.kP, EP, rows);
     if (!rc) rc = cf_map(ctx, &mv, p.c.v, p.c, p.c.vT, p.c.vH, p.c.vP, EP, rows);
     if (rc) return rc;
-    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    static std::atomic<uint64_t> asked{0};
+    B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
     // One resident wave at most, and no more blocks than there can be shares.
     int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
     if (grid > Cfg::BLOCKS) grid = Cfg::BLOCKS;

@@ -598,7 +598,8 @@ template <int EP, bool FP8>
 static int cp_launch(b200_ctx* ctx, CachePromptParams& p) {
     using Cfg = CpCfg<EP>;
     auto kern = cache_prompt_kernel<EP, FP8>;
-    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    static std::atomic<uint64_t> asked{0};
+    B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
     const int64_t sms = ctx->prop.multiProcessorCount;
     const int64_t items = cdiv((int64_t)p.L * p.G, 2 * CP_ROWS) * p.c.H * p.B;
     B200_REQUIRE(items < (1ll << 24), B200_DECLINE_EXTENT, "cache_attention: %lld row tiles", (long long)items);

@@ -18,8 +18,8 @@ typedef struct {
     int nd, code;
 } Arr;
 
-static PyObject *s_ptr, *s_dtype, *s_shape, *s_strides;
-static PyObject *dt_f16, *dt_f32;   // numpy's own dtype objects; an equal one that is not the same goes the Python route
+static PyObject *s_ptr, *s_dtype, *s_shape, *s_strides, *s_addr, *s_rot, *s_interleaved, *s_gain, *s_freq;
+static PyObject *dt_f16, *dt_f32, *dt_i32;   // numpy's own dtype objects; an equal one that is not the same goes the Python route
 
 static int (*p_gemm)(b200_ctx*, int64_t, int64_t, int64_t, const void*, int64_t, const void*, int64_t, const void*, void*,
                      int64_t, int, int, int64_t, int64_t, int64_t, int64_t);
@@ -30,6 +30,14 @@ static int (*p_layernorm)(b200_ctx*, int64_t, int64_t, const void*, int, void*, 
                           float);
 static int (*p_conv)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                      int64_t, int64_t, int64_t, const void*, const void*, const void*, void*, int, int);
+
+static int (*p_rotary)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, const b200_strided4*, const b200_strided4*, const uint64_t*, int64_t, int,
+                       float, const int32_t*, int64_t, int64_t, const int32_t*, const int32_t*);
+static int (*p_append)(b200_ctx*, const b200_cache8*, int64_t, int64_t, const b200_strided4*, const b200_strided4*, const int32_t*, const int32_t*);
+static int (*p_read)(b200_ctx*, const b200_cache8*, int, int64_t, int64_t, const int32_t*, const int32_t*, const b200_strided4*, int);
+static int (*p_cachesdpa)(b200_ctx*, const b200_cache8*, int64_t, int64_t, int64_t, const b200_strided4*, const b200_strided4*, int, float, int,
+                          const int32_t*, const int32_t*);
+static int (*p_matmul4)(b200_ctx*, const b200_q4*, int64_t, const void*, int64_t, const void*, void*, int64_t, int, int);
 
 static int64_t attr_int(PyObject* o, PyObject* name, int* ok) {
     PyObject* v = PyObject_GetAttr(o, name);
@@ -50,12 +58,14 @@ static int ints(PyObject* t, int64_t* out, int n) {   // a tuple of n integers
     return !PyErr_Occurred();
 }
 
-// A DeviceArray of fp16 or fp32 with one to four axes and a size that is a number here; 0 for anything else.
-static int load(PyObject* o, Arr* a) {
+enum { CODE_I32 = 100 };   // of an array of counts or page numbers
+
+// A DeviceArray of fp16, fp32 or int32 with one to four axes and a size that is a number here; 0 for anything else.
+static int load_any(PyObject* o, Arr* a) {
     int ok;
     PyObject* dt = PyObject_GetAttr(o, s_dtype);
-    a->code = dt == dt_f16 ? B200_F16 : dt == dt_f32 ? B200_F32 : -1;
-    Py_XDECREF(dt);   // numpy holds the two that count
+    a->code = dt == dt_f16 ? B200_F16 : dt == dt_f32 ? B200_F32 : dt == dt_i32 ? CODE_I32 : -1;
+    Py_XDECREF(dt);   // numpy holds the ones that count
     ok = a->code >= 0;
     a->ptr = ok ? attr_int(o, s_ptr, &ok) : 0;
     if (ok) {
@@ -73,6 +83,8 @@ static int load(PyObject* o, Arr* a) {
     }
     return ok;
 }
+
+static int load(PyObject* o, Arr* a) { return load_any(o, a) && a->code != CODE_I32; }   // of fp16 or fp32
 
 static int dense(const Arr* a) {
     int64_t acc = 1;
@@ -224,6 +236,153 @@ static PyObject* h_convolution(PyObject* self, PyObject* const* v, Py_ssize_t n)
     return PyLong_FromLong(rc);
 }
 
+// A dense int32 number for each of B sequences, or None: 1 with *p set, else 0.
+static int counts(PyObject* o, int64_t B, const int32_t** p) {
+    Arr a;
+    *p = NULL;
+    if (o == Py_None) return 1;
+    if (!load_any(o, &a) || a.code != CODE_I32 || a.size != B || !dense(&a)) return 0;
+    *p = (const int32_t*)a.ptr;
+    return 1;
+}
+// The structure that a Python object keeps for the library.
+static const void* kept(PyObject* o) {
+    int ok = 1;
+    const int64_t p = attr_int(o, s_addr, &ok);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        ok = 0;
+    }
+    return ok ? (const void*)p : NULL;
+}
+// A cache with a table of page numbers, (pages a sequence, B).
+static int cached(PyObject* o, PyObject* table, int64_t B, b200_cache8* c) {
+    Arr t;
+    const b200_cache8* p = (const b200_cache8*)kept(o);
+    if (!p || !load_any(table, &t) || t.code != CODE_I32 || t.nd != 2 || t.shape[1] != B || (t.shape[0] != 1 && t.stride[0] != 1)) return 0;
+    *c = *p;
+    c->table = (const int32_t*)t.ptr;
+    c->width = t.shape[0];
+    c->table_ld = B > 1 ? t.stride[1] : (t.shape[0] > 1 ? t.shape[0] : 1);
+    return 1;
+}
+// An array of heads, (E, L, H, B) of fp16 or fp32.
+static int heads(PyObject* o, Arr* a, int64_t E, int64_t H, b200_strided4* s) {
+    if (!load(o, a) || a->nd != 4 || a->shape[0] != E || a->shape[2] != H) return 0;
+    strided(a, s);
+    return 1;
+}
+
+// rotary(handle, plan, out, x, lens, news)
+static PyObject* h_rotary(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+    Arr out, x;
+    const int32_t *lens, *news;
+    b200_ctx* c;
+    int rc, ok = 1;
+    if (n != 6 || !(c = handle(v[0])) || v[4] == Py_None || !load(v[2], &out) || !load(v[3], &x)) Py_RETURN_NONE;
+    if (out.nd != 4 || x.nd != 4 || out.code != B200_F16 || x.code != B200_F16) Py_RETURN_NONE;
+    for (int i = 0; i < 4; ++i)
+        if (out.shape[i] != x.shape[i]) Py_RETURN_NONE;
+    if (!counts(v[4], x.shape[3], &lens) || !counts(v[5], x.shape[3], &news)) Py_RETURN_NONE;
+    const int64_t rot = attr_int(v[1], s_rot, &ok), inter = attr_int(v[1], s_interleaved, &ok);
+    PyObject *gain = PyObject_GetAttr(v[1], s_gain), *freq = PyObject_GetAttr(v[1], s_freq);
+    const int64_t f = freq ? attr_int(freq, s_ptr, &ok) : 0;
+    float g = 0.f;
+    if (gain && PyFloat_Check(gain)) g = (float)PyFloat_AS_DOUBLE(gain);
+    else ok = 0;
+    Py_XDECREF(gain);
+    Py_XDECREF(freq);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        ok = 0;
+    }
+    if (!ok || !f) Py_RETURN_NONE;
+    b200_strided4 so, sx;
+    strided(&out, &so);
+    strided(&x, &sx);
+    ENTER(rc, p_rotary(c, x.shape[0], x.shape[1], x.shape[2], x.shape[3], &sx, &so, (const uint64_t*)f, rot, inter != 0, g, NULL, 0, 0, lens, news));
+    return PyLong_FromLong(rc);
+}
+
+// cacheappend(handle, cache, k, v, table, lens, news)
+static PyObject* h_cacheappend(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    Arr k, v;
+    b200_cache8 cache;
+    b200_strided4 sk, sv;
+    const int32_t *lens, *news;
+    b200_ctx* c;
+    int rc;
+    if (n != 7 || !(c = handle(a[0])) || !load(a[2], &k) || k.nd != 4 || k.code != B200_F16 || !cached(a[1], a[4], k.shape[3], &cache)) Py_RETURN_NONE;
+    if (k.shape[0] != cache.E || k.shape[2] != cache.H || !heads(a[3], &v, cache.E, cache.H, &sv) || v.code != B200_F16) Py_RETURN_NONE;
+    if (v.shape[1] != k.shape[1] || v.shape[3] != k.shape[3] || a[5] == Py_None || !counts(a[5], k.shape[3], &lens) || !counts(a[6], k.shape[3], &news))
+        Py_RETURN_NONE;
+    strided(&k, &sk);
+    ENTER(rc, p_append(c, &cache, k.shape[1], k.shape[3], &sk, &sv, lens, news));
+    return PyLong_FromLong(rc);
+}
+
+// cacheread(handle, out, cache, whether the values, table, lens, starts)
+static PyObject* h_cacheread(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    Arr out;
+    b200_cache8 cache;
+    b200_strided4 so;
+    const int32_t *lens, *starts;
+    b200_ctx* c;
+    int rc;
+    if (n != 7 || !(c = handle(a[0])) || !PyBool_Check(a[3]) || !load(a[1], &out) || out.nd != 4 || !cached(a[2], a[4], out.shape[3], &cache)) Py_RETURN_NONE;
+    if (out.shape[0] != cache.E || out.shape[2] != cache.H || a[5] == Py_None || !counts(a[5], out.shape[3], &lens) || !counts(a[6], out.shape[3], &starts))
+        Py_RETURN_NONE;
+    strided(&out, &so);
+    ENTER(rc, p_read(c, &cache, a[3] == Py_True, out.shape[1], out.shape[3], starts, lens, &so, out.code));
+    return PyLong_FromLong(rc);
+}
+
+// cachesdpa(handle, out, q, cache, table, lens, news, scale, causal)
+static PyObject* h_cachesdpa(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    Arr out, q;
+    b200_cache8 cache;
+    b200_strided4 sq, so;
+    const int32_t *lens, *news;
+    b200_ctx* c;
+    int rc;
+    if (n != 9 || !(c = handle(a[0])) || !PyFloat_Check(a[7]) || !PyBool_Check(a[8])) Py_RETURN_NONE;
+    if (!load(a[2], &q) || q.nd != 4 || q.code != B200_F16 || !cached(a[3], a[4], q.shape[3], &cache)) Py_RETURN_NONE;
+    if (q.shape[0] != cache.E || cache.H < 1 || q.shape[2] % cache.H || !heads(a[1], &out, cache.E, q.shape[2], &so)) Py_RETURN_NONE;
+    if (out.shape[1] != q.shape[1] || out.shape[3] != q.shape[3] || a[5] == Py_None || !counts(a[5], q.shape[3], &lens) || !counts(a[6], q.shape[3], &news))
+        Py_RETURN_NONE;
+    strided(&q, &sq);
+    const float scale = (float)PyFloat_AS_DOUBLE(a[7]);
+    ENTER(rc, p_cachesdpa(c, &cache, q.shape[1], q.shape[2], q.shape[3], &sq, &so, out.code, scale, a[8] == Py_True, lens, news));
+    return PyLong_FromLong(rc);
+}
+
+// matmul4(handle, out, W, B, bias, epilogue)
+static PyObject* h_matmul4(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+    Arr out, B;
+    const void* bias;
+    b200_ctx* c;
+    int epi, rc;
+    if (n != 6 || !(c = handle(v[0])) || (epi = epilogue(v[5])) < 0 || !load(v[1], &out) || !load(v[3], &B) || out.nd != 2 || B.nd != 2) Py_RETURN_NONE;
+    const b200_q4* W = (const b200_q4*)kept(v[2]);
+    if (!W || B.code != B200_F16 || B.shape[0] != W->K || out.shape[0] != W->M || out.shape[1] != B.shape[1]) Py_RETURN_NONE;
+    const int64_t ldb = colmajor(&B), ldo = colmajor(&out);
+    if (ldb < 0 || ldo < 0 || !vector(v[4], B200_F16, W->M, &bias)) Py_RETURN_NONE;
+    ENTER(rc, p_matmul4(c, W, B.shape[1], P(B), ldb, bias, P(out), ldo, out.code, epi));
+    return PyLong_FromLong(rc);
+}
+
+// binddecode(rotary, append, read, attention, product): a decoder's entry points, as addresses
+static PyObject* h_binddecode(PyObject* self, PyObject* args) {
+    unsigned long long a, b, c, d, e;
+    if (!PyArg_ParseTuple(args, "KKKKK", &a, &b, &c, &d, &e)) return NULL;
+    *(void**)&p_rotary = (void*)(uintptr_t)a;
+    *(void**)&p_append = (void*)(uintptr_t)b;
+    *(void**)&p_read = (void*)(uintptr_t)c;
+    *(void**)&p_cachesdpa = (void*)(uintptr_t)d;
+    *(void**)&p_matmul4 = (void*)(uintptr_t)e;
+    Py_RETURN_NONE;
+}
+
 // bind(gemm, gemv, attention, layernorm, convolution): the library's entry points, as addresses
 static PyObject* h_bind(PyObject* self, PyObject* args) {
     unsigned long long a, b, c, d, e;
@@ -241,6 +400,12 @@ static PyMethodDef methods[] = {{"bind", h_bind, METH_VARARGS, NULL},
                                 {"sdpa", (PyCFunction)(void (*)(void))h_sdpa, METH_FASTCALL, NULL},
                                 {"layernorm", (PyCFunction)(void (*)(void))h_layernorm, METH_FASTCALL, NULL},
                                 {"convolution", (PyCFunction)(void (*)(void))h_convolution, METH_FASTCALL, NULL},
+                                {"binddecode", h_binddecode, METH_VARARGS, NULL},
+                                {"rotary", (PyCFunction)(void (*)(void))h_rotary, METH_FASTCALL, NULL},
+                                {"cacheappend", (PyCFunction)(void (*)(void))h_cacheappend, METH_FASTCALL, NULL},
+                                {"cacheread", (PyCFunction)(void (*)(void))h_cacheread, METH_FASTCALL, NULL},
+                                {"cachesdpa", (PyCFunction)(void (*)(void))h_cachesdpa, METH_FASTCALL, NULL},
+                                {"matmul4", (PyCFunction)(void (*)(void))h_matmul4, METH_FASTCALL, NULL},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "hostcalls", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
@@ -249,12 +414,18 @@ PyMODINIT_FUNC PyInit_hostcalls(void) {
     s_dtype = PyUnicode_InternFromString("dtype");
     s_shape = PyUnicode_InternFromString("shape");
     s_strides = PyUnicode_InternFromString("strides");
-    if (!s_ptr || !s_dtype || !s_shape || !s_strides) return NULL;
+    s_addr = PyUnicode_InternFromString("_addr");
+    s_rot = PyUnicode_InternFromString("rot");
+    s_interleaved = PyUnicode_InternFromString("interleaved");
+    s_gain = PyUnicode_InternFromString("gain");
+    s_freq = PyUnicode_InternFromString("freq");
+    if (!s_ptr || !s_dtype || !s_shape || !s_strides || !s_addr || !s_rot || !s_interleaved || !s_gain || !s_freq) return NULL;
     PyObject* np = PyImport_ImportModule("numpy");
     if (!np) return NULL;
     dt_f16 = PyObject_CallMethod(np, "dtype", "s", "float16");
     dt_f32 = PyObject_CallMethod(np, "dtype", "s", "float32");
+    dt_i32 = PyObject_CallMethod(np, "dtype", "s", "int32");
     Py_DECREF(np);
-    if (!dt_f16 || !dt_f32) return NULL;
+    if (!dt_f16 || !dt_f32 || !dt_i32) return NULL;
     return PyModule_Create(&module);
 }

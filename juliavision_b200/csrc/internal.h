@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <unordered_map>
@@ -155,6 +156,16 @@ int gemm_rows_launch(b200_ctx* ctx, int64_t M, int64_t N, int64_t K, const void*
                      const void* bias, int bias_per_n, void* out, int64_t ldo, int out_dtype, int epilogue);
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Lets a kernel have `bytes` of dynamic shared memory, asked of each device once (`done`: a bit a device, the caller's own).
+template <typename... KArgs>
+inline cudaError_t allow_smem(const b200_ctx* ctx, void (*kern)(KArgs...), int bytes, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (ctx->device < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // Launch with the programmatic-serialization attribute (and a cluster width when > 1).  Only
 // kernels that call grid_dep_wait() before their first global access may be launched this way.

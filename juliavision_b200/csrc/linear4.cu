@@ -26,13 +26,8 @@
 namespace b200 {
 
 constexpr int L4_WARPS = 8;      // of a block, which share K
-#ifndef L4_STREAM_TILES
-#define L4_STREAM_TILES 8192
-#endif
-#ifndef L4_MOST
-#define L4_MOST 64
-#endif
-constexpr int L4_TOKENS = L4_MOST;    // tokens the kernel takes; more go through fp16 weights in the workspace
+constexpr int L4_TOKENS = 96;    // tokens the kernels take; more go through fp16 weights in the workspace (4096 x 4096: 64 tokens 17 us and 24, 128 28 and 24)
+constexpr double L4_STREAM_TILES = 4608;   // of 64 rows, 16 tokens and 64 inputs: from here on a list for all warps
 
 struct Linear4Params {
     const uint4* data;            // [four row tiles][k block][row tile][lane]
@@ -498,7 +493,8 @@ template <int NT, bool SMALL, bool ZP>
 static int l4_stream_launch(b200_ctx* ctx, Linear4Params& p) {
     using Cfg = L4Cfg<NT, SMALL>;
     auto kern = linear4_stream_kernel<NT, SMALL, ZP>;
-    B200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+    static std::atomic<uint64_t> asked{0};
+    B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
     CUtensorMap mx;               // rows of 64 inputs, zeros past the ends
     const uint64_t dims[2] = {(uint64_t)p.K, (uint64_t)p.N}, strides[1] = {(uint64_t)p.ldx * 2};
     const uint32_t box[2] = {64, 8 * NT};

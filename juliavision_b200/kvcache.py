@@ -51,6 +51,7 @@ class Cache8:
         s.E, s.T, s.H, s.P = E, T, H, P
         s.kind = KINDS[self.kind][0]
         object.__setattr__(self, "_c", s)
+        object.__setattr__(self, "_addr", C.addressof(s))
 
     def _with(self, table: DeviceArray, B: int):
         if table.dtype != np.int32 or table.ndim != 2 or table.shape[1] != B or (table.shape[0] != 1 and table.strides[0] != 1):
@@ -84,6 +85,10 @@ def cacheappend_(ctx: Ctx, cache: Cache8, k: DeviceArray, v: DeviceArray, table:
                  news: Optional[DeviceArray] = None) -> Cache8:
     """Write new tokens: k and v (E, L, H, B) fp16, E contiguous; row i of sequence b is its token lens[b] - news[b] + i (lens
     with the new tokens in it), rows from news[b] on (L without `news`) are not tokens.  The pages written belong to one sequence."""
+    rc = _lib.host().cacheappend(ctx.handle, cache, k, v, table, lens, news)
+    if rc is not None:
+        check(rc)
+        return cache
     E, T, H, P = cache.k.shape
     ks, vs = _rows("cacheappend!", k, E, H), _rows("cacheappend!", v, E, H)
     if k.shape != v.shape:
@@ -99,6 +104,10 @@ def cacheread_(ctx: Ctx, out: DeviceArray, cache: Cache8, which: str, table: Dev
     past lens[b] are left as they were."""
     if which not in ("k", "v"):
         raise B200Error(1, f"cacheread!: {which!r} is neither 'k' nor 'v'")
+    rc = _lib.host().cacheread(ctx.handle, out, cache, which == "v", table, lens, starts)
+    if rc is not None:
+        check(rc)
+        return out
     E, T, H, P = cache.k.shape
     os_ = _rows("cacheread!", out, E, H, (np.float16, np.float32))
     L, B = out.shape[1], out.shape[3]
@@ -113,6 +122,12 @@ def cachesdpa_(ctx: Ctx, out: DeviceArray, q: DeviceArray, cache: Cache8, table:
     multiple of the cache's heads, query head i reads key head i // (Hq // H).  Row i of sequence b is its token
     lens[b] - news[b] + i and sees, when causal, the tokens up to itself, else all lens[b]; a row that sees none comes out as
     zeros, rows from news[b] on (L without `news`) are left as they were."""
+    if scale is None and q.ndim == 4 and q.shape[0] > 0:
+        scale = 1.0 / sqrt(q.shape[0])
+    rc = _lib.host().cachesdpa(ctx.handle, out, q, cache, table, lens, news, scale, causal)
+    if rc is not None:
+        check(rc)
+        return out
     E, T, H, P = cache.k.shape
     if q.ndim != 4 or q.shape[2] % H:
         raise B200Error(17, f"cachesdpa!: q is {q.shape} over {H} key heads")

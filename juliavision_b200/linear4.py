@@ -33,6 +33,7 @@ class Weight4:
         s.data, s.scales, s.zeros = self.data.ptr, self.scales.ptr, self.zeros.ptr if self.zeros is not None else None
         s.M, s.K, s.group = self.M, self.K, self.group
         object.__setattr__(self, "_c", s)
+        object.__setattr__(self, "_addr", C.addressof(s))
 
 
 def quantise4(W: np.ndarray, group: int = 64, symmetric: bool = True) -> Tuple[np.ndarray, np.ndarray, Optional[np.ndarray]]:
@@ -80,6 +81,10 @@ def pack4(ctx: Ctx, q: DeviceArray, scales: DeviceArray, zeros: Optional[DeviceA
 def matmul4_(ctx: Ctx, out: DeviceArray, W: Weight4, B: DeviceArray, bias: Optional[DeviceArray] = None,
              epi: str = "identity") -> DeviceArray:
     """out (M, N) = epi(T(bias + W B)): matmul_ with a 4-bit weight, B (K, N) and bias (M) fp16, out fp16 or fp32."""
+    rc = _lib.host().matmul4(ctx.handle, out, W, B, bias, _lib.EPI.get(epi))
+    if rc is not None:
+        check(rc)
+        return out
     if B.dtype != np.float16 or B.ndim != 2 or out.ndim != 2:
         raise B200Error(16, "matmul4!: B must be an fp16 (K, N) array, out (M, N)")
     if B.shape[0] != W.K or out.shape != (W.M, B.shape[1]):

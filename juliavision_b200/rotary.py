@@ -89,6 +89,11 @@ def rotary_(ctx: Ctx, plan: RotaryPlan, out: DeviceArray, x: DeviceArray, positi
     """out = x turned by its positions; x and out (E, L, H, B) fp16, E contiguous, any other strides, out x itself or apart from it.
     Token l of sequence b is at positions[l, b] (int32, (L, B), either axis 1 to broadcast) or at lens[b] - news[b] + l, where
     rows from news[b] on (L without `news`) are left as they were.  Heads side by side in one projection take one call."""
+    if positions is None:
+        rc = _lib.host().rotary(ctx.handle, plan, out, x, lens, news)
+        if rc is not None:
+            check(rc)
+            return out
     if any(a.ndim != 4 or a.dtype != np.float16 for a in (x, out)):
         raise B200Error(16, "rotary!: x and out must be four-axis fp16 arrays")
     if x.shape != out.shape:

@@ -444,7 +444,7 @@ def test_matmul4(ctx, case, dtype):
     ctx.fill_bytes(out, 0xFF)
     jv.matmul4_(ctx, out, w, ctx.toback(x), ctx.toback(bias), epi=epi)
     ctx.synchronize()
-    check4(out.to_host(), x, ref.weight4(q, s, z, group), bias, epi, dtype, rounded=N > 64)
+    check4(out.to_host(), x, ref.weight4(q, s, z, group), bias, epi, dtype, rounded=N > 96)
 
 
 def check4(got, x, w, bias, epi, dtype, rounded):
@@ -541,9 +541,9 @@ def test_a_decoder_layer_step_by_step(ctx):
             y, reach = y.reshape(1, m, -1, E), reach.reshape(1, m, -1, E)
             at = np.arange(n - m, n)[None]
             turned = ref.rotary(y[:, :, :Hq + H], at, f, gain, False)
-            # The product, whose weights are rounded to fp16 once for more than 64 tokens: (q - z) s off by 2^-11 of itself, so the
+            # The product, whose weights are rounded to fp16 once for more than 96 tokens: (q - z) s off by 2^-11 of itself, so the
             # sum by 2^-11 of its terms' magnitudes.  Then a turn of two such elements.
-            many = 2.0 ** -11 if B * L > 64 else 0.0
+            many = 2.0 ** -11 if B * L > 96 else 0.0
             ytol = 2.0 ** -11 * np.abs(y) + (2.0 ** -17 + many) * reach + 2.0 ** -25
             pair = ytol[:, :, :Hq + H] + np.roll(ytol[:, :, :Hq + H], E // 2, -1)
             near(hq[b, :m, :Hq + H], turned[0], (pair + 2.0 ** -11 * np.abs(turned) + 2.0 ** -18)[0])
