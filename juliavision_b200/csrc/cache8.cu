@@ -51,12 +51,16 @@ struct AppendParams {
     int whole;       // rows of k and v start on 16-byte boundaries
 };
 
-// a / m rounded to nearest, a exact: the product by r = 1 / m corrected once by its residual (Markstein).  Where a / m is a
-// number of fp32 the residual is exact and so is the result.
-__device__ __forceinline__ float ca_quotient(float a, float m, float r) {
-    const float t = __fmul_rn(a, r);
-    return __fmaf_rn(__fmaf_rn(-t, m, a), r, t);
+// a / m of two numbers, rounded to nearest, a exact: the product by r = 1 / m corrected once by its residual (Markstein).  Where
+// a / m is a number of fp32 the residual is exact and so is the result.  Two at a time, since what an element costs here is
+// instructions (28 M elements of keys and values: one at a time 24 us).
+__device__ __forceinline__ float2 ca_quotients(float2 x, float f, float m, float r) {
+    const uint64_t a = mul2(pack2(x.x, x.y), pack2(f, f)), r2 = pack2(r, r), t = mul2(a, r2);
+    float2 q;
+    unpack2(fma2(fma2(t, pack2(-m, -m), a), r2, t), q.x, q.y);
+    return q;
 }
+__device__ __forceinline__ float2 ca_float2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 // four quotients as 8-bit values
 template <bool FP8> __device__ __forceinline__ uint32_t ca_pack(float a, float b, float c, float d) {
     if constexpr (FP8) {
@@ -65,9 +69,11 @@ template <bool FP8> __device__ __forceinline__ uint32_t ca_pack(float a, float b
             : "=r"(w) : "f"(a), "f"(b), "f"(c), "f"(d));
         return w;
     } else {   // 1.5 * 2^23 more: the sum's low byte is the nearest integer, ties to even
-        const float one = 12582912.f;
-        const uint32_t x = __float_as_uint(a + one), y = __float_as_uint(b + one), z = __float_as_uint(c + one), w = __float_as_uint(d + one);
-        return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+        const uint64_t one = pack2(12582912.f, 12582912.f);
+        float x, y, z, w;
+        unpack2(add2(pack2(a, b), one), x, y);
+        unpack2(add2(pack2(c, d), one), z, w);
+        return __byte_perm(__byte_perm(__float_as_uint(x), __float_as_uint(y), 0x0040), __byte_perm(__float_as_uint(z), __float_as_uint(w), 0x0040), 0x5410);
     }
 }
 
@@ -134,14 +140,10 @@ cache_append_kernel(const AppendParams p) {
         const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         uint2 q = make_uint2(0, 0);
         if (finite) {
-            float f[8];
+            float2 f[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-                f[2 * k] = ca_quotient(g.x * cache_top<FP8>(), most, r);
-                f[2 * k + 1] = ca_quotient(g.y * cache_top<FP8>(), most, r);
-            }
-            q = make_uint2(ca_pack<FP8>(f[0], f[1], f[2], f[3]), ca_pack<FP8>(f[4], f[5], f[6], f[7]));
+            for (int k = 0; k < 4; ++k) f[k] = ca_quotients(ca_float2(w[k]), cache_top<FP8>(), most, r);
+            q = make_uint2(ca_pack<FP8>(f[0].x, f[0].y, f[1].x, f[1].y), ca_pack<FP8>(f[2].x, f[2].y, f[3].x, f[3].y));
         }
         *reinterpret_cast<uint2*>(dst + row * dstT + e) = q;
     }
@@ -157,9 +159,8 @@ cache_append_kernel(const AppendParams p) {
                 for (int k = 0; k < 2; ++k) {
                     uint32_t lo2, hi2;
                     cache_halves<FP8>(w[k], lo2, hi2);
-                    const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&lo2)), l = __half22float2(*reinterpret_cast<const __half2*>(&hi2));
-                    o[k] = ca_pack<FP8>(ca_quotient(g.x * was, most, r), ca_quotient(g.y * was, most, r), ca_quotient(l.x * was, most, r),
-                                        ca_quotient(l.y * was, most, r));
+                    const float2 g = ca_quotients(ca_float2(lo2), was, most, r), l = ca_quotients(ca_float2(hi2), was, most, r);
+                    o[k] = ca_pack<FP8>(g.x, g.y, l.x, l.y);
                 }
                 q = make_uint2(o[0], o[1]);
             }
@@ -171,10 +172,10 @@ cache_append_kernel(const AppendParams p) {
 
 struct ReadParams {
     CacheView c;
-    int side, L;
+    int side, L, rows, blocks;   // rows of a block, blocks of a sequence
     const int32_t *starts, *lens;
     void* out;
-    int64_t oL, oH, oB, n;   // n: (rows, heads, sixteens) of elements in all
+    int64_t oL, oH, oB;
     int whole;
 };
 
@@ -184,55 +185,66 @@ cache_read_kernel(const ReadParams p) {
     const CacheView& c = p.c;
     grid_dep_wait();
     grid_dep_launch();
-    const int per = c.E / 16;
+    const int per = c.E / 16, b = blockIdx.x / p.blocks, row0 = (blockIdx.x - b * p.blocks) * p.rows;
+    const int rows = p.L - row0 < p.rows ? p.L - row0 : p.rows;
     const float inv = 1.f / cache_top<FP8>();
-    for (int64_t i = (int64_t)blockIdx.x * CA_THREADS + threadIdx.x; i < p.n; i += (int64_t)gridDim.x * CA_THREADS) {
-        const int64_t a = i / per;
-        const int e = (int)(i - a * per) * 16;
-        const int64_t rowb = a / c.H;
-        const int h = (int)(a - rowb * c.H), b = (int)(rowb / p.L), row = (int)(rowb - (int64_t)b * p.L);
-        const int n = c.tokens(b, p.lens), from = p.starts != nullptr ? p.starts[b] : 0;
-        const int64_t token = (int64_t)from + row;
-        if (token < 0 || token >= n) continue;
-        const int64_t page = c.page(b, (int)(token >> c.logT));
-        if (page < 0) continue;
-        const int in = (int)token & (c.T - 1);
-        const uint4 w4 = *reinterpret_cast<const uint4*>(p.side ? c.v + page * c.vP + h * c.vH + in * c.vT + e : c.k + page * c.kP + h * c.kH + in * c.kT + e);
-        const float most = (p.side ? c.vmax : c.kmax)[page * c.H + h];
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        OutT* o = (OutT*)p.out + b * p.oB + row * p.oL + h * p.oH + e;
-        float f[16];
+    const int n = c.tokens(b, p.lens), from = p.starts != nullptr ? p.starts[b] : 0;
+    const int64_t first = (int64_t)from + row0;
+    if (first >= n || first + rows <= 0) return;
+    constexpr int AT_ONCE = 2;        // sixteens of elements a thread has on their way: each is two trips, for the page's number and for it
+    const int all = rows * c.H * per;
+    for (int i0 = threadIdx.x; i0 < all; i0 += AT_ONCE * CA_THREADS) {
+        uint4 w4[AT_ONCE];
+        float most[AT_ONCE];
+        int64_t at[AT_ONCE];
+        bool live[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            uint32_t lo, hi;
-            cache_halves<FP8>(w[k], lo, hi);
-            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&lo)), l = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            f[4 * k] = ca_quotient(g.x * most, cache_top<FP8>(), inv);
-            f[4 * k + 1] = ca_quotient(g.y * most, cache_top<FP8>(), inv);
-            f[4 * k + 2] = ca_quotient(l.x * most, cache_top<FP8>(), inv);
-            f[4 * k + 3] = ca_quotient(l.y * most, cache_top<FP8>(), inv);
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + u * CA_THREADS, a = i / per, e = (i - a * per) * 16, r = a / c.H, h = a - r * c.H;
+            const int64_t token = first + r;
+            live[u] = i < all && token >= 0 && token < n;
+            const int64_t page = live[u] ? c.page(b, (int)(token >> c.logT)) : -1;
+            live[u] = page >= 0;
+            const int in = (int)token & (c.T - 1);
+            at[u] = (int64_t)b * p.oB + (row0 + r) * p.oL + h * p.oH + e;
+            w4[u] = make_uint4(0, 0, 0, 0);
+            most[u] = 0.f;
+            if (live[u]) {
+                w4[u] = *reinterpret_cast<const uint4*>(p.side ? c.v + page * c.vP + h * c.vH + in * c.vT + e : c.k + page * c.kP + h * c.kH + in * c.kT + e);
+                most[u] = (p.side ? c.vmax : c.kmax)[page * c.H + h];
+            }
         }
-        if constexpr (sizeof(OutT) == 2) {
-            if (p.whole) {
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (!live[u]) continue;
+            const uint32_t w[4] = {w4[u].x, w4[u].y, w4[u].z, w4[u].w};
+            OutT* o = (OutT*)p.out + at[u];
+            float2 f[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t lo, hi;
+                cache_halves<FP8>(w[k], lo, hi);
+                f[2 * k] = ca_quotients(ca_float2(lo), most[u], cache_top<FP8>(), inv);
+                f[2 * k + 1] = ca_quotients(ca_float2(hi), most[u], cache_top<FP8>(), inv);
+            }
+            if (sizeof(OutT) == 2 && p.whole) {
                 uint32_t r[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const __half2 v = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+                    const __half2 v = __floats2half2_rn(f[k].x, f[k].y);
                     r[k] = *reinterpret_cast<const uint32_t*>(&v);
                 }
                 reinterpret_cast<uint4*>(o)[0] = make_uint4(r[0], r[1], r[2], r[3]);
                 reinterpret_cast<uint4*>(o)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+            } else if (p.whole) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) reinterpret_cast<float4*>(o)[k] = make_float4(f[2 * k].x, f[2 * k].y, f[2 * k + 1].x, f[2 * k + 1].y);
             } else {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float2half_rn(f[k]);
-            }
-        } else {
-            if (p.whole) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) reinterpret_cast<float4*>(o)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = f[k];
+                for (int k = 0; k < 8; ++k) {
+                    o[2 * k] = (OutT)f[k].x;
+                    o[2 * k + 1] = (OutT)f[k].y;
+                }
             }
         }
     }
@@ -297,13 +309,18 @@ int b200_cache_read(b200_ctx* ctx, const b200_cache8* cache, int values, int64_t
     p.starts = starts, p.lens = lens;
     p.out = const_cast<void*>(out->ptr);
     p.oL = out->stride[1], p.oH = out->stride[2], p.oB = out->stride[3];
-    p.n = L * B * p.c.H * (p.c.E / 16);
     p.whole = ((uintptr_t)out->ptr | (uint64_t)(out->stride[1] * size) | (uint64_t)(out->stride[2] * size) | (uint64_t)(out->stride[3] * size)) % 16 == 0;
     B200_CUDA(cudaSetDevice(ctx->device));
-    const int64_t blocks = cdiv(p.n, CA_THREADS), most = (int64_t)ctx->prop.multiProcessorCount * 64;
+    // rows of a block: two steps a thread, as long as there are blocks for the GPU
+    const int64_t per_row = (int64_t)p.c.H * (p.c.E / 16);
+    int64_t rows = 1;
+    while (rows * per_row < 2 * CA_THREADS && cdiv(L, 2 * rows) * B >= 4 * ctx->prop.multiProcessorCount) rows *= 2;
+    p.rows = (int)rows;
+    p.blocks = (int)cdiv(L, rows);
+    B200_REQUIRE(p.blocks * B < (1ll << 31), B200_DECLINE_EXTENT, "cache_read: %lld rows of %lld sequences", (long long)L, (long long)B);
     auto kern = cache->kind == B200_E4M3 ? (size == 2 ? cache_read_kernel<true, __half> : cache_read_kernel<true, float>)
                                          : (size == 2 ? cache_read_kernel<false, __half> : cache_read_kernel<false, float>);
-    B200_CUDA(launch_dep(kern, dim3((unsigned)(blocks < most ? blocks : most)), dim3(CA_THREADS), 0, ctx->stream, 1, p));
+    B200_CUDA(launch_dep(kern, dim3((unsigned)(p.blocks * B)), dim3(CA_THREADS), 0, ctx->stream, 1, p));
     ctx->launches++;
     return B200_OK;
 }

@@ -30,7 +30,7 @@ namespace b200 {
 
 constexpr int CF_THREADS = 128;
 constexpr int CF_WARPS = 4;
-constexpr int CF_JOIN_THREADS = 256;
+constexpr int CF_JOIN_THREADS = 512;    // of a block that joins what began in a block's shares
 constexpr int CF_KEYS = 64;                      // keys a warp takes at a time: a tile of the list
 constexpr int CF_GROUPS = CF_KEYS / 16;          // of one page each
 
@@ -622,8 +622,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     }
 }
 
-// One block a warp of the launch before: joins the parts of the piece that began in its share, in the order of the list, several parts
-// at a time where there are more threads than fours of results.
+// One block for each of the launch before: joins the parts of the pieces that began in its warps' shares, in the order of the list,
+// several parts at a time where there are more threads than fours of results.
 template <int EP, int NT>
 __global__ void __launch_bounds__(CF_JOIN_THREADS)
 cache_attention_join_kernel(const CacheAttnParams p) {
@@ -632,16 +632,21 @@ cache_attention_join_kernel(const CacheAttnParams p) {
     __shared__ float2 ml_s[CF_JOIN_THREADS];
     grid_dep_wait();
     grid_dep_launch();
-    const CfJoin d = p.joins[blockIdx.x];
-    const int items = d.rows * (EP / 4), tid = threadIdx.x;
-    if (items == 0) return;
-    const int groups = items < CF_JOIN_THREADS ? CF_JOIN_THREADS / items : 1, grp = items < CF_JOIN_THREADS ? tid / items : 0;
-    for (int i0 = 0; i0 < items; i0 += CF_JOIN_THREADS) {      // once, but for more results than threads
-        const int i = items < CF_JOIN_THREADS ? tid - grp * items : i0 + tid;
+    __shared__ CfJoin joins_s[CF_WARPS];
+    if (threadIdx.x < CF_WARPS) joins_s[threadIdx.x] = p.joins[blockIdx.x * CF_WARPS + threadIdx.x];
+    __syncthreads();
+    const int tid = threadIdx.x;
+    for (int w = 0; w < CF_WARPS; ++w) {
+        const CfJoin& d = joins_s[w];
+        const int items = d.rows * (EP / 4);
+        if (items == 0) continue;
+        const int groups = items < CF_JOIN_THREADS ? CF_JOIN_THREADS / items : 1, grp = items < CF_JOIN_THREADS ? tid / items : 0;
+        const int i = tid - grp * items;      // 16 rows of 128 elements have as many fours as there are threads
+        static_assert(RT * EP / 4 <= CF_JOIN_THREADS, "a thread for each four of a piece's results");
         const int row = i / (EP / 4), e4 = i % (EP / 4) * 4;
         float M = -INFINITY, l = 0.f;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (grp < groups && i < items)
+        if (grp < groups)
             for (int k0 = grp; k0 < d.parts.count; k0 += groups * AT_ONCE) {
                 float2 ml[AT_ONCE];
                 float4 x[AT_ONCE];
@@ -669,11 +674,10 @@ cache_attention_join_kernel(const CacheAttnParams p) {
                 }
                 M = top;
             }
-        if (groups > 1) {
-            rows_s[tid] = v;
-            ml_s[tid] = make_float2(M, l);
-            __syncthreads();
-            if (grp > 0) return;
+        rows_s[tid] = v;
+        ml_s[tid] = make_float2(M, l);
+        __syncthreads();
+        if (grp == 0) {
             for (int k = 1; k < groups; ++k) M = fmaxf(M, ml_s[k * items + i].x);
             float f = ml_s[i].x == M ? 1.f : cf_ex2(ml_s[i].x - M);
             v.x *= f, v.y *= f, v.z *= f, v.w *= f, l *= f;
@@ -684,9 +688,10 @@ cache_attention_join_kernel(const CacheAttnParams p) {
                 v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
                 l = fmaf(ml.y, f, l);
             }
+            const float inv = l == 0.f ? 1.f : 1.f / l;
+            cf_store(p, RT, d.b, d.h, d.rt, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
-        const float inv = l == 0.f ? 1.f : 1.f / l;
-        if (i < items && grp == 0) cf_store(p, RT, d.b, d.h, d.rt, row, e4, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        __syncthreads();
     }
 }
 
@@ -722,7 +727,7 @@ static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     p.part = static_cast<float*>(ws);
     p.joins = reinterpret_cast<CfJoin*>(p.part + floats);
     B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(CF_THREADS), Cfg::SMEM, ctx->stream, 1, mk, mv, p));
-    B200_CUDA(launch_dep(cache_attention_join_kernel<EP, NT>, dim3((unsigned)grid * CF_WARPS), dim3(CF_JOIN_THREADS), 0, ctx->stream, 1, p));
+    B200_CUDA(launch_dep(cache_attention_join_kernel<EP, NT>, dim3((unsigned)grid), dim3(CF_JOIN_THREADS), 0, ctx->stream, 1, p));
     ctx->launches += 2;
     return B200_OK;
 }
