@@ -49,6 +49,7 @@ struct AppendParams {
     const int32_t *lens, *news;
     int L, blocks;   // pages a sequence's new tokens can touch
     int whole;       // rows of k and v start on 16-byte boundaries
+    Divisor per;     // eights of a row
 };
 
 // a / m of two numbers, rounded to nearest, a exact: the product by r = 1 / m corrected once by its residual (Markstein).  Where
@@ -105,7 +106,7 @@ cache_append_kernel(const AppendParams p) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = tid + i * CA_THREADS, row = lo + at / per, e = at % per * 8;
+        const int at = tid + i * CA_THREADS, r0 = p.per.div(at), row = lo + r0, e = (at - r0 * per) * 8;
         x[i] = make_uint4(0, 0, 0, 0);
         if (row < hi) {
             const __half* s = src + row * srcL + e;
@@ -135,7 +136,7 @@ cache_append_kernel(const AppendParams p) {
     if (!finite) most = __int_as_float(0x7fffffff);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = tid + i * CA_THREADS, row = lo + at / per, e = at % per * 8;
+        const int at = tid + i * CA_THREADS, r0 = p.per.div(at), row = lo + r0, e = (at - r0 * per) * 8;
         if (row >= hi) continue;
         const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         uint2 q = make_uint2(0, 0);
@@ -173,6 +174,7 @@ cache_append_kernel(const AppendParams p) {
 struct ReadParams {
     CacheView c;
     int side, L, rows, blocks;   // rows of a block, blocks of a sequence
+    Divisor per, heads;          // sixteens of a head, heads of a row
     const int32_t *starts, *lens;
     void* out;
     int64_t oL, oH, oB;
@@ -200,7 +202,7 @@ cache_read_kernel(const ReadParams p) {
         bool live[AT_ONCE];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
-            const int i = i0 + u * CA_THREADS, a = i / per, e = (i - a * per) * 16, r = a / c.H, h = a - r * c.H;
+            const int i = i0 + u * CA_THREADS, a = p.per.div(i), e = (i - a * per) * 16, r = p.heads.div(a), h = a - r * c.H;
             const int64_t token = first + r;
             live[u] = i < all && token >= 0 && token < n;
             const int64_t page = live[u] ? c.page(b, (int)(token >> c.logT)) : -1;
@@ -288,6 +290,7 @@ int b200_cache_append(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int64_
     uint64_t odd = ((uintptr_t)k->ptr | (uintptr_t)v->ptr) % 16;
     for (int i = 1; i < 4; ++i) odd |= ((uint64_t)k->stride[i] | (uint64_t)v->stride[i]) % 8;
     p.whole = odd == 0;
+    p.per = Divisor::of(p.c.E / 8);
     B200_CUDA(cudaSetDevice(ctx->device));
     return cache->kind == B200_E4M3 ? append_launch<true>(ctx, p, B) : append_launch<false>(ctx, p, B);
 }
@@ -316,6 +319,8 @@ int b200_cache_read(b200_ctx* ctx, const b200_cache8* cache, int values, int64_t
     int64_t rows = 1;
     while (rows * per_row < 2 * CA_THREADS && cdiv(L, 2 * rows) * B >= 4 * ctx->prop.multiProcessorCount) rows *= 2;
     p.rows = (int)rows;
+    p.per = Divisor::of(p.c.E / 16);
+    p.heads = Divisor::of(p.c.H);
     p.blocks = (int)cdiv(L, rows);
     B200_REQUIRE(p.blocks * B < (1ll << 31), B200_DECLINE_EXTENT, "cache_read: %lld rows of %lld sequences", (long long)L, (long long)B);
     auto kern = cache->kind == B200_E4M3 ? (size == 2 ? cache_read_kernel<true, __half> : cache_read_kernel<true, float>)

@@ -157,6 +157,16 @@ int gemm_rows_launch(b200_ctx* ctx, int64_t M, int64_t N, int64_t K, const void*
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Division by a number the host knows: a / d = (a * reciprocal) >> 32 for a < 2^32 / d, where an integer division costs some twenty
+// instructions.
+struct Divisor {
+    uint32_t d, reciprocal;
+    static Divisor of(int64_t d) { return {(uint32_t)d, d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u}; }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int div(int a) const { return d > 1 ? (int)__umulhi((uint32_t)a, reciprocal) : a; }
+#endif
+};
+
 // Lets a kernel have `bytes` of dynamic shared memory, asked of each device once (`done`: a bit a device, the caller's own).
 template <typename... KArgs>
 inline cudaError_t allow_smem(const b200_ctx* ctx, void (*kern)(KArgs...), int bytes, std::atomic<uint64_t>& done) {

@@ -30,6 +30,7 @@ struct RotaryParams {
     float gain;
     int E, rot, L, H, heads, rows;   // heads of a block, rows of a block
     int64_t total;                   // rows in all: L * B
+    Divisor per, per_heads;          // steps of a head, heads of a block
     int interleaved, moves;          // moves: out is not x, so the rest of a head is copied
 };
 
@@ -83,12 +84,13 @@ rotary_kernel(const RotaryParams p) {
     __syncthreads();
     if constexpr (VEC) {
         const int units = p.rot / 16, per = units + (p.moves ? (p.E - p.rot) / 16 : 0);
-        const int n = rows * heads * per;
+        const int n = rows * p.heads * per;
         for (int i = tid; i < n; i += ROT_THREADS) {
-            const int rh = i / per, u = i - rh * per, r = rh / heads, h = h0 + rh - r * heads;
+            const int rh = p.per.div(i), u = i - rh * per, r = p.per_heads.div(rh), h = rh - r * p.heads;
+            if (h >= heads) continue;        // the last block of a row may have fewer
             if (!on[r]) continue;
-            const __half* x = p.x + xat[r] + h * p.xH;
-            __half* o = p.out + oat[r] + h * p.oH;
+            const __half* x = p.x + xat[r] + (h0 + h) * p.xH;
+            __half* o = p.out + oat[r] + (h0 + h) * p.oH;
             if (u >= units) {   // past the turned part
                 const int e = p.rot + (u - units) * 16;
                 const uint4 a = *reinterpret_cast<const uint4*>(x + e), b = *reinterpret_cast<const uint4*>(x + e + 8);
@@ -189,10 +191,12 @@ int b200_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t B, c
     const int64_t per = vec ? E / 16 : (rot / 2 + E - rot), sms = ctx->prop.multiProcessorCount;
     int64_t rows = 1;
     while (rows < 32 && 2 * rows * (rot / 2) <= ROT_PAIRS && rows * H * per < 4 * ROT_THREADS && cdiv(p.total, 2 * rows) >= 8 * sms) rows *= 2;
-    int64_t heads = H;
+    int64_t heads = H < 2048 ? H : 2048;   // what the divisions take
     while (heads > 1 && cdiv(p.total, rows) * cdiv(H, heads) < 2 * sms && heads * per * rows > ROT_THREADS / 2) heads = cdiv(heads, 2);
     p.rows = (int)rows;
     p.heads = (int)heads;
+    p.per = Divisor::of(vec ? rot / 16 + (p.moves ? (E - rot) / 16 : 0) : 1);
+    p.per_heads = Divisor::of(heads);
     const int64_t gx = cdiv(p.total, rows), gy = cdiv(H, heads);
     B200_REQUIRE(gx < (1ll << 31) && gy < 65536, B200_DECLINE_EXTENT, "rotary: %lld rows of %lld heads", (long long)p.total, (long long)H);
     B200_CUDA(launch_dep(vec ? rotary_kernel<true> : rotary_kernel<false>, dim3((unsigned)gx, (unsigned)gy), dim3(ROT_THREADS), 0, ctx->stream, 1, p));
