@@ -12,17 +12,20 @@
 //   warps 8-11 fetch and convert: K(j), V(j), K(j+1), ...
 //   warps 12, 13  issue one tile's products each:  Q K(j)',  P(j) V(j), Q K(j+1)', ...; P lies over the first half of S
 //   warp 14    looks up pages and scales and lays out each block's constants, two blocks ahead
+//   warp 15    walks the block's share of the items' keys (CpWalk), an item's part at a time, and tells the others
 #include <cuda_fp16.h>
 
 #include "cache8.cuh"
+#include "shares.cuh"
 
 namespace b200 {
 
 constexpr int CP_THREADS = 512;
 constexpr int CP_ROWS = 128, CP_KEYS = 128;     // of a tile
 constexpr int CP_ATOM = 128 * 128;              // 128 rows x 64 fp16
+constexpr int CP_LEAST = 2;                     // blocks of keys of a share
 constexpr int CP_SCALES = 4;                    // blocks of constants in flight
-constexpr int CP_SOFTMAX_REGS = 184, CP_CONVERT_REGS = 96, CP_OTHER_REGS = 40;
+constexpr int CP_SOFTMAX_REGS = 176, CP_CONVERT_REGS = 104, CP_OTHER_REGS = 56;
 static_assert(2 * 128 * CP_SOFTMAX_REGS + 128 * CP_CONVERT_REGS + 128 * CP_OTHER_REGS <= CP_THREADS * 128, "what the launch holds");
 
 struct CpScales {              // of one block of keys, a group of 16 keys an entry
@@ -31,17 +34,6 @@ struct CpScales {              // of one block of keys, a group of 16 keys an en
     float back[8];             // an exponential of the group back to a weight
     float change, reference;   // the reference before over the reference now; the reference
     int hidden, odd;           // bit g: the group has no page; one of its scales is not finite
-};
-
-template <int EP> struct CpCfg {
-    static constexpr int ATOMS = EP / 64;
-    static constexpr int SIDE = ATOMS * CP_ATOM;                 // an operand tile
-    static constexpr int STAGES = 2;
-    static constexpr int S_Q = 0, S_K = 2 * SIDE, S_V = S_K + STAGES * SIDE, S_C = S_V + STAGES * SIDE;
-    static constexpr int S_BARS = S_C + (CP_SCALES * (int)sizeof(CpScales) + 15) / 16 * 16;
-    static constexpr int BARRIERS = 2 + 4 * STAGES + 2 * 5 + 2 * CP_SCALES;
-    static constexpr int SMEM = S_BARS + (BARRIERS + 1) * 8;
-    static constexpr int O_COL = 2 * CP_KEYS;
 };
 
 struct CachePromptParams {
@@ -54,9 +46,10 @@ struct CachePromptParams {
     int causal, out_f32, whole, out_whole;
     float scale_log2;         // without its sign, which goes onto Q
     int negate;
-    int items, nsplit;        // row pairs x heads x sequences; parts that an item's keys are cut into
-    float* part;              // [split][item][256 rows][EP], then [split][item][256][2]: reference point, sum
-    float* part_ml;
+    int items, shared;        // row pairs x heads x sequences; whether the blocks have equal shares of their keys, or an item each
+    float* part;              // [2 grid][EP / 4][256 rows][4]: a block's share that begins inside an item, and the one that ends inside one
+    float* part_ml;           // [2 grid][256][2]: reference point, sum
+    int4* joins;              // [grid]: the item of a block's first share and its first and last block, if it is the second of them
 };
 
 __device__ __forceinline__ float cp_ex2(float x) {
@@ -74,6 +67,21 @@ __device__ __forceinline__ void cp_tmem_st16(uint32_t taddr, const uint32_t* r) 
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = r[i];
     tmem_st16(taddr, v);
+}
+// 16 bytes to shared memory on their own, zeros where there are none to read
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void cp_load8(uint32_t (&v)[4], const __half* at, bool whole) {
+    if (whole) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(at));
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = u[2 * k] | (uint32_t)u[2 * k + 1] << 16;
+    }
 }
 // four results of a row, 16 bytes of fp16 or two of fp32 at a time where rows allow it
 __device__ __forceinline__ void cp_store8(const CachePromptParams& p, int64_t at, const float (&v)[8]) {
@@ -104,6 +112,8 @@ __device__ __forceinline__ void cp_store8(const CachePromptParams& p, int64_t at
 // What the rows of an item see: item -> (row pair, head, sequence), later rows, whose keys are more, first.
 struct CpItem {
     int b, h, r0, rows, n, m, blocks;   // first row, rows of the sequence (all of its heads), length, new tokens, blocks of keys
+    // its length in the list that is shared out: an item without keys has its rows of zeros to write
+    __device__ __forceinline__ int weight() const { return r0 >= rows ? 0 : blocks > 0 ? blocks : 1; }
 };
 __device__ __forceinline__ CpItem cp_item(const CachePromptParams& p, int item) {
     CpItem it;
@@ -121,6 +131,51 @@ __device__ __forceinline__ CpItem cp_item(const CachePromptParams& p, int item) 
     it.blocks = (seen + CP_KEYS - 1) / CP_KEYS;
     return it;
 }
+
+// A block's share of the list of all items' blocks of keys, an item's part at a time.
+struct CpWalk {
+    long long left;     // blocks of the share from here on
+    int item, j;        // where the next part begins
+
+    __device__ __forceinline__ bool next(const CachePromptParams& p, CpItem& it, int& at, int& j0, int& nblk) {
+        while (left > 0 && item < p.items) {
+            it = cp_item(p, item);
+            const int w = it.weight();
+            if (w == 0) {                     // nor has any other head of these rows
+                item += p.c.H - item % p.c.H;
+                j = 0;
+                continue;
+            }
+            at = item, j0 = j;
+            const int take = w - j < left ? w - j : (int)left;
+            nblk = it.blocks > 0 ? take : 0;
+            left -= take;
+            j += take;
+            if (j == w) ++item, j = 0;
+            return true;
+        }
+        return false;
+    }
+};
+
+constexpr int CP_PARTS = 2;    // on their way from the warp that walks to the others
+struct CpPart {
+    CpItem it;
+    int item, j0, nblk, more;
+};
+
+template <int EP> struct CpCfg {
+    static constexpr int ATOMS = EP / 64;
+    static constexpr int SIDE = ATOMS * CP_ATOM;                 // an operand tile
+    static constexpr int STAGES = 2;
+    static constexpr int S_Q = 0, S_K = 2 * SIDE, S_V = S_K + STAGES * SIDE, S_C = S_V + STAGES * SIDE;
+    static constexpr int S_BARS = S_C + (CP_SCALES * (int)sizeof(CpScales) + 15) / 16 * 16;
+    static constexpr int BARRIERS = 2 + 4 * STAGES + 2 * 5 + 2 * CP_SCALES + 2 * CP_PARTS;
+    static constexpr int S_WALK = S_BARS + (BARRIERS + 1) * 8;   // where the share begins; what finding it adds up
+    static constexpr int S_PART = S_WALK + 16 + 32 * 8;
+    static constexpr int SMEM = S_PART + CP_PARTS * (int)sizeof(CpPart);
+    static constexpr int O_COL = 2 * CP_KEYS;
+};
 
 template <int EP, bool FP8>
 __global__ void __launch_bounds__(CP_THREADS, 1)
@@ -146,20 +201,14 @@ cache_prompt_kernel(const CachePromptParams p) {
     uint64_t* exp_turn = pv_done + 2;              // [2] whose turn it is to run its exponentials
     uint64_t* c_full = exp_turn + 2;                 // [CP_SCALES] a block's constants
     uint64_t* c_empty = c_full + CP_SCALES;        // four softmax warps a tile
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_empty + CP_SCALES);
+    uint64_t* a_full = c_empty + CP_SCALES;        // [CP_PARTS] a part of an item
+    uint64_t* a_empty = a_full + CP_PARTS;         // every other warp
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(a_empty + CP_PARTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     CpScales* consts = reinterpret_cast<CpScales*>(smem + Cfg::S_C);
-    static_assert(Cfg::BARRIERS == 2 + 4 * STAGES + 10 + 2 * CP_SCALES, "barriers counted by the layout");
+    static_assert(Cfg::BARRIERS == 2 + 4 * STAGES + 10 + 2 * CP_SCALES + 2 * CP_PARTS, "barriers counted by the layout");
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    grid_dep_wait();          // the lengths may come from the launch before
-    grid_dep_launch();
-    const int split = blockIdx.x % p.nsplit, item = blockIdx.x / p.nsplit;
-    const CpItem it = cp_item(p, item);
-    if (it.r0 >= it.rows) return;                  // uniform: before any barrier or tensor memory exists
-    const int j_begin = (int)((int64_t)split * it.blocks / p.nsplit), nblk = (int)((int64_t)(split + 1) * it.blocks / p.nsplit) - j_begin;
-    const int ntiles = it.r0 + CP_ROWS < it.rows ? 2 : 1;
-
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 4);
@@ -171,17 +220,81 @@ cache_prompt_kernel(const CachePromptParams p) {
         }
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&k_full[s], 4);
-            mbar_init(&k_empty[s], ntiles);
+            mbar_init(&k_empty[s], 2);
             mbar_init(&v_full[s], 4);
-            mbar_init(&v_empty[s], ntiles);
+            mbar_init(&v_empty[s], 2);
         }
         for (int s = 0; s < CP_SCALES; ++s) {
             mbar_init(&c_full[s], 1);
-            mbar_init(&c_empty[s], 4 * ntiles);
+            mbar_init(&c_empty[s], 8);
+        }
+        for (int s = 0; s < CP_PARTS; ++s) {
+            mbar_init(&a_full[s], 1);
+            mbar_init(&a_empty[s], CP_THREADS / 32 - 1);
         }
         *abort_flag = 0;
         fence_barrier_init();
     }
+    grid_dep_wait();          // the lengths may come from the launch before
+    grid_dep_launch();
+    CpWalk* walk = reinterpret_cast<CpWalk*>(smem + Cfg::S_WALK);
+    if (!p.shared) {
+        const int w = cp_item(p, blockIdx.x).weight();
+        if (w == 0) return;                        // uniform: before any barrier or tensor memory exists
+        if (threadIdx.x == 0) *walk = {w, (int)blockIdx.x, 0};
+    } else {
+        // Weights are the same for all heads: an entry has the H items of a row pair of a sequence.  A thread sums a run of
+        // them; the sums before it tell which thread's run the share of this block begins in.
+        long long* sums = reinterpret_cast<long long*>(smem + Cfg::S_WALK + sizeof(CpWalk));
+        const int entries = p.items / c.H, run = (entries + CP_THREADS - 1) / CP_THREADS, e0 = threadIdx.x * run;
+        long long mine = 0;
+        int some = 0;
+        for (int e = e0; e < e0 + run && e < entries; ++e) {
+            const int w = cp_item(p, e * c.H).weight();
+            mine += (long long)w * c.H;
+            some += w > 0 ? c.H : 0;
+        }
+        long long upto = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += x;
+            some += __shfl_xor_sync(0xffffffffu, some, d);
+        }
+        if (lane == 31) sums[warp] = upto;
+        if (lane == 0) sums[16 + warp] = some;
+        __syncthreads();
+        long long total = 0, pieces = 0;
+        for (int i = 0; i < CP_THREADS / 32; ++i) {
+            if (i == warp) upto += total;
+            total += sums[i], pieces += sums[16 + i];
+        }
+        // as many shares as blocks, but of CP_LEAST blocks of keys at least where there are no more items than that makes
+        const long long want = pieces > total / CP_LEAST ? pieces : total / CP_LEAST;
+        const Shares shares(total, want < gridDim.x ? (int)want : gridDim.x);
+        if ((int)blockIdx.x >= shares.warps) {     // uniform
+            if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            return;
+        }
+        const long long begin = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1);
+        __syncthreads();        // the sums are read
+        if (begin >= upto - mine && begin < upto) {
+            long long at = upto - mine;
+            for (int e = e0; e < e0 + run && e < entries; ++e) {
+                const int w = cp_item(p, e * c.H).weight();
+                if (begin < at + (long long)w * c.H) {
+                    const int h = (int)floor_div(begin - at, w);
+                    at += (long long)h * w;
+                    *walk = {end - begin, e * c.H + h, (int)(begin - at)};
+                    sums[0] = at, sums[1] = at + w - 1, sums[2] = total;
+                    sums[3] = shares.warps;
+                    break;
+                }
+                at += (long long)w * c.H;
+            }
+        }
+    }
+
     if (warp == 15) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
@@ -190,56 +303,99 @@ cache_prompt_kernel(const CachePromptParams p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    CpPart* part = reinterpret_cast<CpPart*>(smem + Cfg::S_PART);
+    // The next part of the block's share; barriers go on over all of them.
+    CpItem it;
+    int item = 0, j_begin = 0, nblk = 0, parts_seen = 0;
+    auto next = [&]() -> bool {
+        const int s = parts_seen % CP_PARTS;
+        if (!__all_sync(0xffffffffu, mbar_wait(&a_full[s], (uint32_t)((parts_seen / CP_PARTS) & 1), c.d_status, KST_WAIT_FULL, abort_flag))) return false;
+        CpPart x = part[s];
+        // the same for all lanes, which the compiler sees: what depends on them stays in the warp's own registers
+        for (int* v : {&x.it.b, &x.it.h, &x.it.r0, &x.it.rows, &x.it.n, &x.it.m, &x.it.blocks, &x.item, &x.j0, &x.nblk, &x.more})
+            *v = __shfl_sync(0xffffffffu, *v, 0);
+        if (lane == 0) mbar_arrive(&a_empty[s]);
+        ++parts_seen;
+        it = x.it, item = x.item, j_begin = x.j0, nblk = x.nblk;
+        return x.more != 0;
+    };
 
     if (warp >= 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CP_OTHER_REGS));
         if (warp == 14) {
             // -------------------------------------------------- pages and scales of the blocks
-            float ref = 0.f;
-            auto page = [&](int j) {
-                const int key = (j_begin + j) * CP_KEYS + (lane & 7) * 16;
-                return j < nblk && key < it.n ? (int)c.page(it.b, key >> c.logT) : -1;
-            };
-            int pg = page(0), pg1 = page(1);
-            float k0 = 0.f, v0 = 0.f;
-            auto load = [&](int q, float& k, float& v) {
-                k = q >= 0 ? __ldg(c.kmax + (int64_t)q * c.H + it.h) : 0.f;
-                v = q >= 0 ? __ldg(c.vmax + (int64_t)q * c.H + it.h) : 0.f;
-            };
-            load(pg, k0, v0);
-            for (int j = 0; j < nblk; ++j) {
-                const int pg2 = page(j + 2);
-                float k1, v1;
-                load(pg1, k1, v1);
-                const int s = j % CP_SCALES;
-                if (!mbar_wait(&c_empty[s], (uint32_t)((j / CP_SCALES) & 1) ^ 1, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
-                float most = v0 < INFINITY ? v0 : 0.f;
+            int done = 0;
+            bool ok = true;
+            while (ok && next()) {
+                float ref = 0.f;
+                auto page = [&](int j) {
+                    const int key = (j_begin + j) * CP_KEYS + (lane & 7) * 16;
+                    return j < nblk && key < it.n ? (int)c.page(it.b, key >> c.logT) : -1;
+                };
+                int pg = page(0), pg1 = page(1);
+                float k0 = 0.f, v0 = 0.f;
+                auto load = [&](int q, float& k, float& v) {
+                    k = q >= 0 ? __ldg(c.kmax + (int64_t)q * c.H + it.h) : 0.f;
+                    v = q >= 0 ? __ldg(c.vmax + (int64_t)q * c.H + it.h) : 0.f;
+                };
+                load(pg, k0, v0);
+                for (int j = 0; j < nblk; ++j) {
+                    const int pg2 = page(j + 2);
+                    float k1, v1;
+                    load(pg1, k1, v1);
+                    const int s = done % CP_SCALES;
+                    if (!mbar_wait(&c_empty[s], (uint32_t)((done / CP_SCALES) & 1) ^ 1, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
+                    ++done;
+                    float most = v0 < INFINITY ? v0 : 0.f;
 #pragma unroll
-                for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                const float was = ref;
-                if (most > ref) ref = 1.5f * most;
-                // a scale far below the reference, whose P is zero in fp16, keeps an exponent of its own so that the sum can take it back
-                float f = ref > 0x1p-100f ? v0 / ref : 1.f;
-                if (f < 0x1p-40f) f = 0x1p-40f;
-                const float kf = k0 * p.scale_log2;
-                const bool strange = !(kf < INFINITY) || !(v0 < INFINITY);
-                const unsigned hidden = __ballot_sync(0xffffffffu, pg < 0) & 255u, odd = __ballot_sync(0xffffffffu, strange) & 255u;
-                if (lane < 8) {
-                    consts[s].key[lane] = strange ? 1.f : fmaxf(kf, 0x1p-100f);   // a page of zeros: its scores are zeros whatever the factor
-                    consts[s].value[lane] = strange ? 7.f : log2f(f) + 7.f;
-                    consts[s].back[lane] = strange ? 0x1p-7f : 0x1p-7f / f;
+                    for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+                    const float was = ref;
+                    if (most > ref) ref = 1.5f * most;
+                    // a scale far below the reference, whose P is zero in fp16, keeps an exponent of its own so that the sum can take it back
+                    float f = ref > 0x1p-100f ? v0 / ref : 1.f;
+                    if (f < 0x1p-40f) f = 0x1p-40f;
+                    const float kf = k0 * p.scale_log2;
+                    const bool strange = !(kf < INFINITY) || !(v0 < INFINITY);
+                    const unsigned hidden = __ballot_sync(0xffffffffu, pg < 0) & 255u, odd = __ballot_sync(0xffffffffu, strange) & 255u;
+                    if (lane < 8) {
+                        consts[s].key[lane] = strange ? 1.f : fmaxf(kf, 0x1p-100f);   // a page of zeros: its scores are zeros whatever the factor
+                        consts[s].value[lane] = strange ? 7.f : log2f(f) + 7.f;
+                        consts[s].back[lane] = strange ? 0x1p-7f : 0x1p-7f / f;
+                    }
+                    if (lane == 0) {
+                        consts[s].change = was == ref ? 1.f : was / ref;
+                        consts[s].reference = ref;
+                        consts[s].hidden = (int)hidden;
+                        consts[s].odd = (int)odd;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c_full[s]);
+                    pg = pg1, pg1 = pg2, k0 = k1, v0 = v1;
                 }
+            }
+        } else if (warp == 15) {
+            // -------------------------------------------------- parts of items
+            CpWalk mine = *walk;
+            const int first = mine.j > 0 ? mine.item : -1;
+            int s = 0;
+            CpPart x;
+            do {
+                x.more = mine.next(p, x.it, x.item, x.j0, x.nblk);
+                if (!mbar_wait(&a_empty[s % CP_PARTS], (uint32_t)((s / CP_PARTS) & 1) ^ 1, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
                 if (lane == 0) {
-                    consts[s].change = was == ref ? 1.f : was / ref;
-                    consts[s].reference = ref;
-                    consts[s].hidden = (int)hidden;
-                    consts[s].odd = (int)odd;
+                    part[s % CP_PARTS] = x;
+                    mbar_arrive(&a_full[s % CP_PARTS]);
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&c_full[s]);
-                pg = pg1, pg1 = pg2, k0 = k1, v0 = v1;
+                ++s;
+            } while (x.more);
+            if (p.shared && lane == 0) {     // who joins the item that the share begins inside
+                const long long* at = reinterpret_cast<const long long*>(smem + Cfg::S_WALK + sizeof(CpWalk));
+                const Shares shares(at[2], (int)at[3]);
+                const int w0 = shares.holder(at[0]), w1 = shares.holder(at[1]);
+                p.joins[blockIdx.x] = make_int4(w0 + 1 == (int)blockIdx.x ? first : -1, w0, w1, 0);
             }
-        } else if (warp < 14 && warp - 12 < ntiles) {
+        } else if (warp < 14) {
             // -------------------------------------------------- issuers: the whole warp waits, one thread issues
             const int t = warp - 12;
             constexpr uint32_t idesc_s = make_idesc_f16(CP_ROWS, CP_KEYS, 0, 0);
@@ -251,9 +407,10 @@ cache_prompt_kernel(const CachePromptParams p) {
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
                 return __all_sync(0xffffffffu, mbar_wait(bar, parity, c.d_status, code, abort_flag));
             };
+            int done = 0, busy = 0, parts = 0;      // blocks of the share, of this tile, parts of this tile, before this part
             auto issue_qk = [&](int j) -> bool {
-                const int sk = j % STAGES;
-                if (!wait(&k_full[sk], (uint32_t)((j / STAGES) & 1), KST_WAIT_FULL)) return false;
+                const int i = done + j, sk = i % STAGES;
+                if (!wait(&k_full[sk], (uint32_t)((i / STAGES) & 1), KST_WAIT_FULL)) return false;
                 tc_fence_after();
                 if (elect_one()) {
                     const uint32_t k_addr = smem_u32(smem + Cfg::S_K + sk * Cfg::SIDE);
@@ -275,24 +432,43 @@ cache_prompt_kernel(const CachePromptParams p) {
                 for (int k = k0; k < k1; ++k)
                     umma_ts(o_tmem, s_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
             };
-            bool ok = wait(&q_full[t], 0, KST_WAIT_FULL);
-            if (ok && nblk > 0) ok = issue_qk(0);
-            for (int j = 0; ok && j < nblk; ++j) {
-                const int sv = j % STAGES;
-                if (!wait(&v_full[sv], (uint32_t)((j / STAGES) & 1), KST_WAIT_FULL)) break;
-                if (!wait(&p_half[t], (uint32_t)(j & 1), KST_WAIT_SOFTMAX)) break;
-                tc_fence_after();
-                if (elect_one()) issue_pv(j, sv, 0, 4);
-                __syncwarp();
-                if (!wait(&p_full[t], (uint32_t)(j & 1), KST_WAIT_SOFTMAX)) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    issue_pv(j, sv, 4, 8);
-                    umma_commit(&pv_done[t]);
-                    umma_commit(&v_empty[sv]);
+            bool ok = true;
+            while (ok && next()) {
+                if (it.r0 + t * CP_ROWS >= it.rows) {      // no rows: what the other tile reads is released from here too
+                    for (int j = 0; ok && j < nblk; ++j) {
+                        const int i = done + j, s = i % STAGES;
+                        const uint32_t ph = (uint32_t)((i / STAGES) & 1);
+                        ok = wait(&k_full[s], ph, KST_WAIT_FULL);
+                        if (ok && elect_one()) mbar_arrive(&k_empty[s]);
+                        ok = ok && wait(&v_full[s], ph, KST_WAIT_FULL);
+                        if (ok && elect_one()) mbar_arrive(&v_empty[s]);
+                        __syncwarp();
+                    }
+                    done += nblk;
+                    continue;
                 }
-                __syncwarp();
-                if (j + 1 < nblk && !issue_qk(j + 1)) break;   // over P(j): after the product that reads it, in issue order
+                if (nblk == 0) continue;
+                ok = wait(&q_full[t], (uint32_t)(parts & 1), KST_WAIT_FULL) && issue_qk(0);
+                for (int j = 0; ok && j < nblk; ++j) {
+                    const int i = done + j, sv = i % STAGES;
+                    const uint32_t ph = (uint32_t)((busy + j) & 1);
+                    ok = wait(&v_full[sv], (uint32_t)((i / STAGES) & 1), KST_WAIT_FULL) && wait(&p_half[t], ph, KST_WAIT_SOFTMAX);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) issue_pv(j, sv, 0, 4);
+                    __syncwarp();
+                    ok = wait(&p_full[t], ph, KST_WAIT_SOFTMAX);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        issue_pv(j, sv, 4, 8);
+                        umma_commit(&pv_done[t]);
+                        umma_commit(&v_empty[sv]);
+                    }
+                    __syncwarp();
+                    if (j + 1 < nblk) ok = issue_qk(j + 1);   // over P(j): after the product that reads it, in issue order
+                }
+                done += nblk, busy += nblk, ++parts;
             }
         }
     } else if (warp >= 8) {
@@ -351,66 +527,84 @@ cache_prompt_kernel(const CachePromptParams p) {
             fence_proxy_async_smem();
             __syncwarp();
         };
-        look(0);
-        fetch(kq, 0, 0);
-        fetch(vq, 0, 1);
-        look(1);
-        for (int j = 0; j < nblk; ++j) {
-            const int s = j % STAGES;
-            const uint32_t ph = (uint32_t)((j / STAGES) & 1) ^ 1;
-            if (!mbar_wait(&k_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
-            write(kq, smem_u32(smem + Cfg::S_K + s * Cfg::SIDE), false);
-            if (lane == 0) mbar_arrive(&k_full[s]);
-            fetch(kq, j + 1, 0);
-            if (!mbar_wait(&v_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
-            write(vq, smem_u32(smem + Cfg::S_V + s * Cfg::SIDE), true);
-            if (lane == 0) mbar_arrive(&v_full[s]);
-            fetch(vq, j + 1, 1);
-            look(j + 2);
+        int done = 0;
+        bool ok = true;
+        while (ok && next()) {
+            look(0);
+            fetch(kq, 0, 0);
+            fetch(vq, 0, 1);
+            look(1);
+            for (int j = 0; j < nblk; ++j) {
+                const int s = done % STAGES;
+                const uint32_t ph = (uint32_t)((done / STAGES) & 1) ^ 1;
+                ++done;
+                if (!mbar_wait(&k_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
+                write(kq, smem_u32(smem + Cfg::S_K + s * Cfg::SIDE), false);
+                if (lane == 0) mbar_arrive(&k_full[s]);
+                fetch(kq, j + 1, 0);
+                if (!mbar_wait(&v_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
+                write(vq, smem_u32(smem + Cfg::S_V + s * Cfg::SIDE), true);
+                if (lane == 0) mbar_arrive(&v_full[s]);
+                fetch(vq, j + 1, 1);
+                look(j + 2);
+            }
         }
     } else {
         // ------------------------------------------------------ softmax and results
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CP_SOFTMAX_REGS));
         const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
-        if (t < ntiles) {
+        const uint32_t lane_base = uint32_t(quad * 32) << 16;
+        const uint32_t s_tmem = tmem_base + lane_base + t * CP_KEYS, o_tmem = tmem_base + lane_base + Cfg::O_COL + t * EP;
+        int done = 0, busy = 0, turns = 0;          // blocks of the share, of this tile, of both tiles, before this one
+        bool ok = true;
+        while (ok && next()) {
+            if (it.r0 + t * CP_ROWS >= it.rows) {
+                for (int j = 0; ok && j < nblk; ++j, ++done) {
+                    const int cs = done % CP_SCALES;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&c_full[cs], (uint32_t)((done / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag));
+                    if (ok && lane == 0) mbar_arrive(&c_empty[cs]);
+                }
+                continue;
+            }
             const int r = it.r0 + t * CP_ROWS + row, l = r / p.G, hq = it.h * p.G + r - l * p.G;   // new token, query head
             const bool live = r < it.rows;
-            {
-                const __half* q = p.q + l * p.qL + hq * p.qH + it.b * p.qB;
-                const uint32_t dst = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE) + row * 128, sign = p.negate ? 0x80008000u : 0u;
-#pragma unroll 4
-                for (int ch = 0; ch < EP / 8; ++ch) {
-                    uint32_t v[4] = {0, 0, 0, 0};
-                    if (live && ch * 8 < c.E) {
-                        if (p.whole) {
-                            const uint4 x = __ldg(reinterpret_cast<const uint4*>(q + ch * 8));
-                            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-                        } else {
-                            const unsigned short* u = reinterpret_cast<const unsigned short*>(q + ch * 8);
+            if (nblk > 0) {
+                // a row's chunks are read by neighbouring lanes, whole lines; all of them are on their way at once
+                constexpr int CH = EP / 8, STEP = 32 / CH;
+                const int ch = lane % CH;
+                const uint32_t dst = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE) + (uint32_t)(ch >> 3) * CP_ATOM;
+                int to = quad * 32 + lane / CH, lq = (it.r0 + t * CP_ROWS + to) / p.G, g = it.r0 + t * CP_ROWS + to - lq * p.G;
+                const __half* q = p.q + it.h * p.G * p.qH + it.b * p.qB + ch * 8;
+#pragma unroll 1
+                for (int i = 0; i < CH; ++i, to += STEP) {
+                    const bool on = it.r0 + t * CP_ROWS + to < it.rows && ch * 8 < c.E;
+                    const __half* at = on ? q + lq * p.qL + g * p.qH : p.q;
+                    const uint32_t to_smem = dst + to * 128 + (((ch & 7) ^ (to & 7)) << 4);
+                    if (p.whole && !p.negate) {
+                        cp_async16(to_smem, at, on);
+                    } else {
+                        uint32_t v[4] = {0, 0, 0, 0};
+                        if (on) cp_load8(v, at, p.whole);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i] ^= sign;
+                        for (int k = 0; k < 4; ++k) v[k] ^= p.negate ? 0x80008000u : 0u;
+                        st_shared_v4(to_smem, v);
                     }
-                    st_shared_v4(dst + (uint32_t)(ch >> 3) * CP_ATOM + (((ch & 7) ^ (row & 7)) << 4), v);
+                    for (g += STEP; g >= p.G; g -= p.G) ++lq;
                 }
+                cp_async_wait();
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[t]);
             }
-            const uint32_t lane_base = uint32_t(quad * 32) << 16;
-            const uint32_t s_tmem = tmem_base + lane_base + t * CP_KEYS, o_tmem = tmem_base + lane_base + Cfg::O_COL + t * EP;
             const int last = p.causal ? it.n - it.m + l : it.n - 1;                       // the last key this row sees
             const int all_see = p.causal ? it.n - it.m + (it.r0 + t * CP_ROWS) / p.G : it.n - 1;   // that every row of the tile sees
             float m_run = -INFINITY, l_run = 0.f, ref = 0.f;
-            bool ok = true;
-            const bool pingpong = ntiles == 2;
-            for (int j = 0; ok && j < nblk; ++j) {
-                const int cs = j % CP_SCALES, key0 = (j_begin + j) * CP_KEYS;
-                if (!mbar_wait(&c_full[cs], (uint32_t)((j / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag)) { ok = false; break; }
+            const bool pingpong = it.r0 + CP_ROWS < it.rows;
+            for (int j = 0; ok && j < nblk; ++j, ++done, ++busy) {
+                const int cs = done % CP_SCALES, key0 = (j_begin + j) * CP_KEYS;
+                if (!mbar_wait(&c_full[cs], (uint32_t)((done / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag)) { ok = false; break; }
                 const CpScales& k = consts[cs];
-                if (!mbar_wait(&s_full[t], (uint32_t)(j & 1), c.d_status, KST_WAIT_TMEM_FULL, abort_flag)) { ok = false; break; }
+                if (!mbar_wait(&s_full[t], (uint32_t)(busy & 1), c.d_status, KST_WAIT_TMEM_FULL, abort_flag)) { ok = false; break; }
                 __syncwarp();
                 tc_fence_after();
                 uint32_t x[4][32];
@@ -471,8 +665,8 @@ cache_prompt_kernel(const CachePromptParams p) {
                     }
                     m_run = m_new;
                 }
-                if (pingpong && (t == 1 || j > 0) &&
-                    !mbar_wait(&exp_turn[t], (uint32_t)((t == 1 ? j : j - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag)) { ok = false; break; }
+                if (pingpong && (t == 1 || turns > 0) &&
+                    !mbar_wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag)) { ok = false; break; }
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -507,6 +701,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                 if (pingpong) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&exp_turn[1 - t]);
+                    ++turns;
                 }
                 ref = k.reference;
                 tmem_wait_st();
@@ -517,14 +712,16 @@ cache_prompt_kernel(const CachePromptParams p) {
                     mbar_arrive(&c_empty[cs]);
                 }
             }
-            if (ok && nblk > 0) ok = mbar_wait(&pv_done[t], (uint32_t)((nblk - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag);
+            if (ok && nblk > 0) ok = mbar_wait(&pv_done[t], (uint32_t)((busy - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag);
             __syncwarp();
             if (ok) {
                 tc_fence_after();
                 const float back = ref * 0x1p-7f / cache_top<FP8>();
-                const float f = p.nsplit > 1 ? back : back / (l_run == 0.f ? 1.f : l_run);
+                const bool whole = j_begin == 0 && nblk == it.blocks;
+                const float f = !whole ? back : back / (l_run == 0.f ? 1.f : l_run);
                 const int64_t at = l * p.oL + hq * p.oH + it.b * p.oB;
-                const int64_t prow = ((int64_t)split * p.items + item) * 2 * CP_ROWS + t * CP_ROWS + row;
+                const int64_t place = (int64_t)blockIdx.x * 2 + (j_begin == 0 ? 1 : 0);
+                const int prow = t * CP_ROWS + row;
 #pragma unroll 1
                 for (int i = 0; i < EP / 16; ++i) {
                     uint32_t o16[16];
@@ -540,16 +737,16 @@ cache_prompt_kernel(const CachePromptParams p) {
                     float v[2][8];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) v[u >> 3][u & 7] = __uint_as_float(o16[u]) * f;
-                    if (p.nsplit > 1) {
-                        float4* d = reinterpret_cast<float4*>(p.part + prow * EP + i * 16);
+                    if (!whole) {
+                        float4* d = reinterpret_cast<float4*>(p.part + place * (2 * CP_ROWS * EP)) + i * 4 * (2 * CP_ROWS) + prow;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) d[u] = make_float4(v[u >> 1][(u & 1) * 4], v[u >> 1][(u & 1) * 4 + 1], v[u >> 1][(u & 1) * 4 + 2], v[u >> 1][(u & 1) * 4 + 3]);
+                        for (int u = 0; u < 4; ++u) d[u * 2 * CP_ROWS] = make_float4(v[u >> 1][(u & 1) * 4], v[u >> 1][(u & 1) * 4 + 1], v[u >> 1][(u & 1) * 4 + 2], v[u >> 1][(u & 1) * 4 + 3]);
                     } else {
                         cp_store8(p, at + i * 16, v[0]);
                         cp_store8(p, at + i * 16 + 8, v[1]);
                     }
                 }
-                if (live && p.nsplit > 1) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
+                if (live && !whole) *reinterpret_cast<float2*>(p.part_ml + (place * 2 * CP_ROWS + prow) * 2) = make_float2(m_run, l_run);
             }
         }
     }
@@ -564,34 +761,41 @@ cache_prompt_kernel(const CachePromptParams p) {
     }
 }
 
-// The parts of an item's keys, in order: eight elements a thread.
+// The items that several blocks have parts of, sixteen elements of a row a thread: the second block of an item stands for it.
 template <int EP>
 __global__ void __launch_bounds__(256)
 cache_prompt_join_kernel(const CachePromptParams p) {
     grid_dep_wait();
     grid_dep_launch();
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, prow = i / (EP / 8), rows = (int64_t)p.items * 2 * CP_ROWS;
-    const int e = (int)(i % (EP / 8)) * 8;
-    if (prow >= rows || e >= p.c.E) return;
-    const CpItem it = cp_item(p, (int)(prow / (2 * CP_ROWS)));
-    const int r = it.r0 + (int)(prow % (2 * CP_ROWS));
-    if (r >= it.rows) return;
+    const int4 at = p.joins[blockIdx.x / (EP / 16)];
+    if (at.x < 0) return;
+    const int row = threadIdx.x, e = (int)(blockIdx.x % (EP / 16)) * 16;
+    const CpItem it = cp_item(p, at.x);
+    const int r = it.r0 + row;
+    if (r >= it.rows || e >= p.c.E) return;
     const int l = r / p.G, hq = it.h * p.G + r - l * p.G;
-    float M = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, p.part_ml[(s * rows + prow) * 2]);
-    for (int s = 0; s < p.nsplit; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + prow) * 2);
+    auto place = [&](int w) { return (int64_t)w * 2 + (w == at.y ? 1 : 0); };
+    auto stat = [&](int w) { return *reinterpret_cast<const float2*>(p.part_ml + (place(w) * 2 * CP_ROWS + row) * 2); };
+    float M = -INFINITY, sum = 0.f, v[2][8] = {};
+    for (int w = at.y; w <= at.z; ++w) M = fmaxf(M, stat(w).x);
+    for (int w = at.y; w <= at.z; ++w) {
+        const float2 ml = stat(w);
         const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
-        const float4* x = reinterpret_cast<const float4*>(p.part + (s * rows + prow) * EP + e);
-        const float4 a = x[0], b = x[1];
+        const float4* x = reinterpret_cast<const float4*>(p.part + place(w) * (2 * CP_ROWS * EP)) + e / 4 * (2 * CP_ROWS) + row;
         sum = fmaf(ml.y, f, sum);
-        v[0] = fmaf(a.x, f, v[0]), v[1] = fmaf(a.y, f, v[1]), v[2] = fmaf(a.z, f, v[2]), v[3] = fmaf(a.w, f, v[3]);
-        v[4] = fmaf(b.x, f, v[4]), v[5] = fmaf(b.y, f, v[5]), v[6] = fmaf(b.z, f, v[6]), v[7] = fmaf(b.w, f, v[7]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float4 a = x[u * 2 * CP_ROWS];
+            float* d = &v[u >> 1][(u & 1) * 4];
+            d[0] = fmaf(a.x, f, d[0]), d[1] = fmaf(a.y, f, d[1]), d[2] = fmaf(a.z, f, d[2]), d[3] = fmaf(a.w, f, d[3]);
+        }
     }
     const float inv = sum == 0.f ? 1.f : 1.f / sum;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] *= inv;
-    cp_store8(p, l * p.oL + hq * p.oH + it.b * p.oB + e, v);
+    for (int k = 0; k < 16; ++k) v[k >> 3][k & 7] *= inv;
+    const int64_t to = l * p.oL + hq * p.oH + it.b * p.oB + e;
+    cp_store8(p, to, v[0]);
+    cp_store8(p, to + 8, v[1]);
 }
 
 template <int EP, bool FP8>
@@ -603,26 +807,27 @@ static int cp_launch(b200_ctx* ctx, CachePromptParams& p) {
     const int64_t sms = ctx->prop.multiProcessorCount;
     const int64_t items = cdiv((int64_t)p.L * p.G, 2 * CP_ROWS) * p.c.H * p.B;
     B200_REQUIRE(items < (1ll << 24), B200_DECLINE_EXTENT, "cache_attention: %lld row tiles", (long long)items);
-    // Fewer items than SMs: their keys are cut so that every SM has a part, four blocks of keys at least.
-    const int64_t blocks = cdiv((int64_t)p.c.width * p.c.T, CP_KEYS);
-    int64_t nsplit = sms / items;
-    if (nsplit > blocks / 4) nsplit = blocks / 4;
-    if (nsplit > 64) nsplit = 64;
-    if (nsplit < 1) nsplit = 1;
     p.items = (int)items;
-    p.nsplit = (int)nsplit;
-    if (nsplit > 1) {
+    // Equal shares keep every SM busy to the end; they cost a look for the share's place and a second launch that joins, together
+    // about what four blocks of keys do, and a further start and end for most items, about six (of 2 us at E = 128).  Items a launch
+    // block / shares, us: 128 items of 64 to 80 blocks 177 / 171 (E = 128), 167 / 147 (E = 64); 256 of 28 to 32 blocks 148 / 174;
+    // 8 of 782 blocks 1554 / 125; 32 of 2 to 8 blocks 27.5 / 23.5.
+    const int64_t blocks = cdiv((int64_t)p.c.width * p.c.T, CP_KEYS);
+    p.shared = items <= 8 * sms && items * (blocks + 6) + 4 * sms < cdiv(items, sms) * blocks * sms;
+    const int64_t grid = p.shared ? sms : items;
+    if (p.shared) {
         void* ws = nullptr;
-        const size_t rows = (size_t)nsplit * items * 2 * CP_ROWS;
-        int rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float), &ws);
+        const size_t rows = (size_t)grid * 4 * CP_ROWS;
+        int rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float) + grid * sizeof(int4), &ws);
         if (rc) return rc;
         p.part = static_cast<float*>(ws);
         p.part_ml = p.part + rows * EP;
+        p.joins = reinterpret_cast<int4*>(p.part_ml + rows * 2);
     }
-    B200_CUDA(launch_dep(kern, dim3((unsigned)(items * nsplit)), dim3(CP_THREADS), Cfg::SMEM, ctx->stream, 1, p));
+    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(CP_THREADS), Cfg::SMEM, ctx->stream, 1, p));
     ctx->launches++;
-    if (nsplit > 1) {
-        B200_CUDA(launch_dep(cache_prompt_join_kernel<EP>, dim3((unsigned)cdiv(items * 2 * CP_ROWS * (EP / 8), 256)), dim3(256), 0, ctx->stream, 1, p));
+    if (p.shared) {
+        B200_CUDA(launch_dep(cache_prompt_join_kernel<EP>, dim3((unsigned)(grid * (EP / 16))), dim3(256), 0, ctx->stream, 1, p));
         ctx->launches++;
     }
     return B200_OK;
