@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(32 * L4_WARPS)
 linear4_kernel(const Linear4Params p) {
     constexpr int COLS = 8 * NT + 1, GROUPS = SMALL ? 2 : 1, AT_ONCE = NT == 1 ? 4 : 3;
     __shared__ float red[L4_WARPS][16][COLS];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int mt = blockIdx.x, n0 = blockIdx.y * 8 * NT;
     grid_dep_wait();
     grid_dep_launch();
@@ -220,7 +220,7 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
     __shared__ PieceParts parts_s[2 * L4_WARPS];
     __shared__ long long piece_s[2 * L4_WARPS];                    // the pieces this block's warps have parts of: ended, last; -1: none
     __shared__ int abort_s;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* const l4_x = l4_raw + ((1024 - (smem_u32(l4_raw) & 1023)) & 1023);
     uint8_t* const l4_ring = l4_x + Cfg::X_RING;
     if (lane == 0) {
@@ -238,7 +238,9 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
     const int tgs = (p.N + 8 * NT - 1) / (8 * NT);
     const Shares shares((long long)(p.MT + 3) / 4 * tgs * p.KB, gridDim.x * L4_WARPS);
     const int me = blockIdx.x * L4_WARPS + warp;
-    const long long from = me < shares.warps ? shares.begin(me) : 0, to = me < shares.warps ? shares.begin(me + 1) : 0;
+    // the same for all lanes, which the compiler sees: the loop's addresses stay in the warp's own registers (42.4 to 38.9 us at 28672 x 8192 x 16)
+    const long long from = __shfl_sync(0xffffffffu, me < shares.warps ? shares.begin(me) : 0, 0);
+    const long long to = __shfl_sync(0xffffffffu, me < shares.warps ? shares.begin(me + 1) : 0, 0);
     uint8_t* const ring = l4_ring + warp * L4_STAGES * Cfg::STAGE;
     uint8_t* const xring = l4_x + warp * L4_STAGES * Cfg::X_STAGE;
 
@@ -257,7 +259,7 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
     }
     auto fetch = [&]() {
         if (asked >= tiles) return;
-        if (lane == 0) {
+        if (elect_one()) {
             const uint32_t dst = smem_u32(ring + ask_s * Cfg::STAGE);
             const int g0 = (ask_kb * 64) >> p.logg, groups = SMALL && p.NG - g0 < GROUPS ? 1 : GROUPS;
             uint64_t* bar = &full_s[warp][ask_s];
@@ -303,8 +305,8 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
     uint32_t phase = 0;
     bool first = true;            // the piece at hand may have begun before this share
     for (int at = 0; at < tiles; ++at) {
-        if (!mbar_wait(&full_s[warp][s], phase, p.d_status, KST_WAIT_FULL, &abort_s)) break;
-        __syncwarp();             // this stage is there for every lane, and the one that is asked for now has been read
+        if (!__all_sync(0xffffffffu, mbar_wait(&full_s[warp][s], phase, p.d_status, KST_WAIT_FULL, &abort_s))) break;
+                    // this stage is there for every lane, and the one that is asked for now has been read
         fetch();
         const uint8_t* st = ring + s * Cfg::STAGE;
         const uint8_t* xs = xring + s * Cfg::X_STAGE + g * 128;
