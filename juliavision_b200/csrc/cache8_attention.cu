@@ -158,7 +158,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     if (threadIdx.x < 2 * CF_WARPS) has_s[threadIdx.x] = 0;
     uint8_t* cf_smem = cf_raw + ((1024 - (smem_u32(cf_raw) & 1023)) & 1023);
     const CacheView& c = p.c;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     if (lane == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&full_s[warp][i], 1);
         fence_barrier_init();
@@ -207,6 +207,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             from = s.begin(me);
             to = s.begin(me + 1);
         }
+        from = __shfl_sync(0xffffffffu, from, 0), to = __shfl_sync(0xffffffffu, to, 0);   // the same for all lanes, which the compiler sees
     };
     if (p.B <= 32) {              // every warp for itself
         int n, m, tiles;
