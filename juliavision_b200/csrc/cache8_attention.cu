@@ -10,14 +10,15 @@
 //
 // A page's scales never touch the operands: the key scale multiplies the fp32 scores of its page, the value scale goes onto P,
 // relative to the largest one so far, whose change is one more factor of the running rescale.  That rescale waits until a
-// score is 2^8 past its row's reference point; P is rounded to fp16 times 2^7, so that it stays in range and weights down to
-// 2^-21 of the reference keep all their bits.
+// score is 2^8 past its row's reference point; P goes in times 2^7, so that it stays in range, as two fp16 halves (the rounded
+// weight and what that lost): 22 bits of weight for half as many more products, which hide behind the conversions (an error of
+// 2.1e-4 of the result's scale against 2.9e-4 with the upper half alone; 32 x 8192 tokens 65 us with both and 64 with one).
 //
 // The work is one list of 64-key tiles over all (sequence, key head, row tile): pieces.  It is computed from the lengths on the
 // device and dealt out to the warps in equal contiguous shares, so ragged lengths and few sequences fill the GPU alike.  A warp
 // streams its tiles by TMA and meets nobody before its block's end: it asks for the next piece's first tile before it writes the
 // results of the last.  (Blocks that walked the list together lost 8 us at every change of piece, the slowest warp's tile and
-// the trips to memory that nothing hid: 32 x 8192 tokens 62 us.)  A piece that one warp holds whole is stored at once.  Of the
+// the trips to memory that nothing hid.)  A piece that one warp holds whole is stored at once.  Of the
 // others, what ends inside a warp's share waits in the workspace; the last pieces of a block's warps are joined in shared
 // memory at its end, and a second launch joins what then still lies in several places, in the order of the list: the result
 // does not depend on timing.
@@ -61,7 +62,6 @@ template <int EP, int NT> struct CfCfg {
     static constexpr int CTAS = NT == 1 && EP == 64 ? 4 : 2;
     static constexpr int SMEM = RING + 1024;                  // the swizzle wants the ring on a 1024-byte boundary
     static_assert(CF_WARPS * RT * ROW * 4 <= RING, "the warps' rows fit over the ring");
-    static constexpr int BLOCKS = 148 * CTAS;                 // of a launch at most
 };
 
 // Byte of 16-byte chunk c of row r of a stage's side, as the tensor map's swizzle lays it: 128-byte rows with the chunk turned
@@ -366,6 +366,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     };
 
     CfPiece pc, nx;
+    bool ok = true;               // no wait has run out
     if (from < to) {
         locate(pc, from);
         look(pc, pc.j0);
@@ -374,7 +375,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         scales();
         queries(pc);
     }
-    for (long long at = from; at < to;) {
+    for (long long at = from; ok && at < to;) {
         const int n = pc.n, m = pc.m, rt = pc.rt;
         at = pc.start + pc.j1;
         // As results lane (g, t) holds rows 8 i + 2 t and 8 i + 2 t + 1.
@@ -402,7 +403,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 locate(nx, at);
                 look(nx, nx.j0);
             }
-            if (!mbar_wait(&full_s[warp][0], phase, c.d_status, KST_WAIT_FULL, &abort_s)) break;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full_s[warp][0], phase, c.d_status, KST_WAIT_FULL, &abort_s)))) break;
             float s[NT][NG][4];     // rows g and g + 8 of a group's keys, query rows 2 t and 2 t + 1
 #pragma unroll
             for (int grp = 0; grp < NG; ++grp) {
@@ -524,7 +525,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                     }
                 }
             }
-            if (!mbar_wait(&full_s[warp][1], phase, c.d_status, KST_WAIT_FULL, &abort_s)) break;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&full_s[warp][1], phase, c.d_status, KST_WAIT_FULL, &abort_s)))) break;
             phase ^= 1;
             // V: lane (g, t) holds four tokens' W elements of its chunk, in the order of P's rows; elements 2 u and 2 u + 1 of the chunks are
             // rows g and g + 8 of tile u
@@ -559,6 +560,7 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
             __syncwarp();   // the values have been read
             if (more) copy(1);
         }
+        if (!ok) break;
         // the next piece's first tile is on its way while this one's results leave
         const CfPiece done = pc;
         const bool mine = done.j0 == 0 && done.j1 == done.tiles;
@@ -576,6 +578,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
     }
 
     // ---- the block's parts of pieces
+    if (!ok)                      // copies may still land
+        for (int i = 0; i < 4; ++i) __nanosleep(1000000);
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();   // the ring is free: every copy that was asked for has been waited for
     float* rows_s = reinterpret_cast<float*>(cf_smem);
@@ -717,7 +721,6 @@ static int cf_launch(b200_ctx* ctx, CacheAttnParams& p) {
     B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
     // One resident wave at most, and no more blocks than there can be shares.
     int64_t grid = (int64_t)ctx->prop.multiProcessorCount * Cfg::CTAS;
-    if (grid > Cfg::BLOCKS) grid = Cfg::BLOCKS;
     const int64_t tiles = cdiv((int64_t)p.c.width * p.c.T, CF_KEYS), rts = cdiv((int64_t)p.L * p.G, Cfg::RT);
     const double most = (double)tiles * rts * p.c.H * p.B / CF_WARPS;
     if (most + 1 < (double)grid) grid = (int64_t)most + 1;

@@ -10,6 +10,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
+#include <string.h>
 
 #include "../../include/b200dnn.h"
 
@@ -18,7 +19,7 @@ typedef struct {
     int nd, code;
 } Arr;
 
-static PyObject *s_ptr, *s_dtype, *s_shape, *s_strides, *s_addr, *s_rot, *s_interleaved, *s_gain, *s_freq;
+static PyObject *s_ptr, *s_dtype, *s_shape, *s_strides, *s_c, *s_rot, *s_interleaved, *s_gain, *s_freq;
 static PyObject *dt_f16, *dt_f32, *dt_i32;   // numpy's own dtype objects; an equal one that is not the same goes the Python route
 
 static int (*p_gemm)(b200_ctx*, int64_t, int64_t, int64_t, const void*, int64_t, const void*, int64_t, const void*, void*,
@@ -245,22 +246,26 @@ static int counts(PyObject* o, int64_t B, const int32_t** p) {
     *p = (const int32_t*)a.ptr;
     return 1;
 }
-// The structure that a Python object keeps for the library.
-static const void* kept(PyObject* o) {
-    int ok = 1;
-    const int64_t p = attr_int(o, s_addr, &ok);
+// The structure that a Python object keeps for the library, copied.
+static int kept(PyObject* o, void* to, Py_ssize_t size) {
+    Py_buffer b;
+    PyObject* c = PyObject_GetAttr(o, s_c);
+    int ok = 0;
+    if (c && PyObject_GetBuffer(c, &b, PyBUF_SIMPLE) == 0) {
+        if ((ok = b.len == size)) memcpy(to, b.buf, (size_t)size);
+        PyBuffer_Release(&b);
+    }
+    Py_XDECREF(c);
     if (PyErr_Occurred()) {
         PyErr_Clear();
         ok = 0;
     }
-    return ok ? (const void*)p : NULL;
+    return ok;
 }
 // A cache with a table of page numbers, (pages a sequence, B).
 static int cached(PyObject* o, PyObject* table, int64_t B, b200_cache8* c) {
     Arr t;
-    const b200_cache8* p = (const b200_cache8*)kept(o);
-    if (!p || !load_any(table, &t) || t.code != CODE_I32 || t.nd != 2 || t.shape[1] != B || (t.shape[0] != 1 && t.stride[0] != 1)) return 0;
-    *c = *p;
+    if (!kept(o, c, sizeof *c) || !load_any(table, &t) || t.code != CODE_I32 || t.nd != 2 || t.shape[1] != B || (t.shape[0] != 1 && t.stride[0] != 1)) return 0;
     c->table = (const int32_t*)t.ptr;
     c->width = t.shape[0];
     c->table_ld = B > 1 ? t.stride[1] : (t.shape[0] > 1 ? t.shape[0] : 1);
@@ -363,11 +368,11 @@ static PyObject* h_matmul4(PyObject* self, PyObject* const* v, Py_ssize_t n) {
     b200_ctx* c;
     int epi, rc;
     if (n != 6 || !(c = handle(v[0])) || (epi = epilogue(v[5])) < 0 || !load(v[1], &out) || !load(v[3], &B) || out.nd != 2 || B.nd != 2) Py_RETURN_NONE;
-    const b200_q4* W = (const b200_q4*)kept(v[2]);
-    if (!W || B.code != B200_F16 || B.shape[0] != W->K || out.shape[0] != W->M || out.shape[1] != B.shape[1]) Py_RETURN_NONE;
+    b200_q4 W;
+    if (!kept(v[2], &W, sizeof W) || B.code != B200_F16 || B.shape[0] != W.K || out.shape[0] != W.M || out.shape[1] != B.shape[1]) Py_RETURN_NONE;
     const int64_t ldb = colmajor(&B), ldo = colmajor(&out);
-    if (ldb < 0 || ldo < 0 || !vector(v[4], B200_F16, W->M, &bias)) Py_RETURN_NONE;
-    ENTER(rc, p_matmul4(c, W, B.shape[1], P(B), ldb, bias, P(out), ldo, out.code, epi));
+    if (ldb < 0 || ldo < 0 || !vector(v[4], B200_F16, W.M, &bias)) Py_RETURN_NONE;
+    ENTER(rc, p_matmul4(c, &W, B.shape[1], P(B), ldb, bias, P(out), ldo, out.code, epi));
     return PyLong_FromLong(rc);
 }
 
@@ -414,12 +419,12 @@ PyMODINIT_FUNC PyInit_hostcalls(void) {
     s_dtype = PyUnicode_InternFromString("dtype");
     s_shape = PyUnicode_InternFromString("shape");
     s_strides = PyUnicode_InternFromString("strides");
-    s_addr = PyUnicode_InternFromString("_addr");
+    s_c = PyUnicode_InternFromString("_c");
     s_rot = PyUnicode_InternFromString("rot");
     s_interleaved = PyUnicode_InternFromString("interleaved");
     s_gain = PyUnicode_InternFromString("gain");
     s_freq = PyUnicode_InternFromString("freq");
-    if (!s_ptr || !s_dtype || !s_shape || !s_strides || !s_addr || !s_rot || !s_interleaved || !s_gain || !s_freq) return NULL;
+    if (!s_ptr || !s_dtype || !s_shape || !s_strides || !s_c || !s_rot || !s_interleaved || !s_gain || !s_freq) return NULL;
     PyObject* np = PyImport_ImportModule("numpy");
     if (!np) return NULL;
     dt_f16 = PyObject_CallMethod(np, "dtype", "s", "float16");

@@ -305,9 +305,11 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
     uint32_t phase = 0;
     bool first = true;            // the piece at hand may have begun before this share
     for (int at = 0; at < tiles; ++at) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&full_s[warp][s], phase, p.d_status, KST_WAIT_FULL, &abort_s))) break;
-                    // this stage is there for every lane, and the one that is asked for now has been read
-        fetch();
+        if (!__all_sync(0xffffffffu, mbar_wait(&full_s[warp][s], phase, p.d_status, KST_WAIT_FULL, &abort_s))) {
+            for (int i = 0; i < 4; ++i) __nanosleep(1000000);   // copies may still land
+            break;
+        }
+        fetch();                  // this stage is there for every lane, and the one that is asked for now has been read
         const uint8_t* st = ring + s * Cfg::STAGE;
         const uint8_t* xs = xring + s * Cfg::X_STAGE + g * 128;
         if (++s == L4_STAGES) s = 0, phase ^= 1;

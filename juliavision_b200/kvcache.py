@@ -7,7 +7,6 @@ between sequences that begin alike, and copied (`ctx.copy` of a page's slice) wi
 """
 from __future__ import annotations
 
-import ctypes as C
 from dataclasses import dataclass
 from math import sqrt
 from typing import Optional
@@ -51,7 +50,6 @@ class Cache8:
         s.E, s.T, s.H, s.P = E, T, H, P
         s.kind = KINDS[self.kind][0]
         object.__setattr__(self, "_c", s)
-        object.__setattr__(self, "_addr", C.addressof(s))
 
     def _with(self, table: DeviceArray, B: int):
         if table.dtype != np.int32 or table.ndim != 2 or table.shape[1] != B or (table.shape[0] != 1 and table.strides[0] != 1):

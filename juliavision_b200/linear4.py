@@ -33,7 +33,6 @@ class Weight4:
         s.data, s.scales, s.zeros = self.data.ptr, self.scales.ptr, self.zeros.ptr if self.zeros is not None else None
         s.M, s.K, s.group = self.M, self.K, self.group
         object.__setattr__(self, "_c", s)
-        object.__setattr__(self, "_addr", C.addressof(s))
 
 
 def quantise4(W: np.ndarray, group: int = 64, symmetric: bool = True) -> Tuple[np.ndarray, np.ndarray, Optional[np.ndarray]]:

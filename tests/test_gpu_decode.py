@@ -290,6 +290,22 @@ def test_attention_of_many_sequences(ctx, L):
     near(*attend(ctx, c, q, news, None, True))
 
 
+@pytest.mark.parametrize("case", [(170, 64, 1, 2, 40), (9, 128, 2, 4, 100), (40, 80, 1, 3, 90)], ids=str)
+def test_many_rows_of_sequences_of_unequal_lengths(ctx, case):
+    """A block's share of the keys spans several sequences, or a part of one: long ones among short ones, some empty, some without
+    new tokens, some with more new tokens than they have tokens (rows that see nothing)."""
+    B, E, H, G, L = case
+    rng = np.random.default_rng(19)
+    lens = rng.integers(0, 300, B)
+    lens[[1, B // 2, B - 1]] = 5000, 3001, 0
+    news = rng.integers(0, L + 1, B)
+    news[[1, B // 2]] = L, 1
+    news[B - 2:] = L
+    c = Cached(ctx, rng, E, 16, H, lens, "int8")
+    q = rng.standard_normal((B, L, H * G, E)).astype(F16)
+    near(*attend(ctx, c, q, news, None, True))
+
+
 @pytest.mark.parametrize("L", [2, 150])
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("pitch", [0, 1, 8])
