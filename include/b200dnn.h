@@ -276,8 +276,9 @@ int b200_cache_read(b200_ctx* ctx, const b200_cache8* cache, int values, int64_t
                     const int32_t* lens, const b200_strided4* out, int out_dtype);
 /* out = softmax(scale * Q K') V over the cache: q and out (E,L,Hq,B), E contiguous, Hq a multiple of H; query head i reads key
  * head i / (Hq / H).  Every query sees the keys below lens[b]; when causal, up to its own position.  A row that sees no key
- * comes out as zeros; rows at or past news[b] are left as they were.  Scores, softmax and sums are fp32; the weights are rounded to
- * fp16 for the second product.  Scratch comes from the context's workspace. */
+ * comes out as zeros; rows at or past news[b] are left as they were.  out does not overlap q.  Scores, softmax and sums are fp32;
+ * for the second product the weights are taken as two fp16 halves (22 bits), or rounded to fp16 where a key head has more than
+ * 24 query rows (E > 64; 32 otherwise).  Scratch comes from the context's workspace. */
 int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int64_t Hq, int64_t B, const b200_strided4* q,
                          const b200_strided4* out, int out_dtype, float scale, int causal, const int32_t* lens,
                          const int32_t* news);
@@ -297,7 +298,8 @@ int b200_q4_sizes(int64_t M, int64_t K, int64_t group, int64_t* data_bytes, int6
 int b200_q4_pack(b200_ctx* ctx, const void* q, int64_t q_m, int64_t q_k, const void* scales, int64_t s_m, int64_t s_g,
                  const void* zeros, int64_t z_m, int64_t z_g, const b200_q4* out);
 /* out(M,N) = epi(T(bias[m] + sum_k w[m,k] B(K,N)[k,n])): b200_gemm_f16 with such a weight, fp16 B and bias, fp32 accumulation,
- * the weights taken exactly for few tokens; for many they are rounded to fp16 once into the context's workspace. */
+ * the weights taken exactly for up to 96 tokens; for more they are rounded to fp16 once into the context's workspace.  out does
+ * not overlap B. */
 int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, int64_t ldb, const void* bias, void* out,
                    int64_t ldo, int out_dtype, int epilogue);
 

@@ -278,6 +278,108 @@ function matmul!(ctx::Ctx{B200Backend}, ::MMGemvPlan, out, A, B, bias, epi; gemm
     out
 end
 
+# ------------------------------------------------------------------ a decoder's step (new surface)
+# Counts (`lens`, `news`, `starts`) are Int32 device vectors of one number a sequence; rows are (E, L, H, B) views, E contiguous.
+nullable(a) = a === nothing ? C_NULL : pointer(a)
+
+# freq: `rot ÷ 2` UInt64 on the device, radians a position / 2π modulo one, in units of 2^-64.
+struct RotaryPlan
+    rot::Int64
+    interleaved::Bool
+    gain::Float32
+    freq::B200Array{UInt64,1}
+end
+function rotary!(ctx::Ctx{B200Backend}, plan::RotaryPlan, out, x; lens, news = nothing)
+    E, L, H, B = size(x)
+    check(ccall((:b200_rotary_f16, LIB), Cint,
+                (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Ptr{Cvoid}, Int64, Cint, Cfloat,
+                 Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, E, L, H, B, s4(x), s4(out), pointer(plan.freq), plan.rot, plan.interleaved, plan.gain,
+                C_NULL, 0, 0, pointer(lens), nullable(news)))
+    out
+end
+
+# kind 2: Int8, 3: e4m3 in UInt8 (b200dnn.h); k, v (E, T, H, P), kmax, vmax (H, P) Float32.
+struct Cache8{K}
+    k::K
+    v::K
+    kmax::B200Array{Float32,2}
+    vmax::B200Array{Float32,2}
+    kind::Int32
+end
+struct Cache8C                      # b200_cache8
+    k::Ptr{Cvoid}
+    v::Ptr{Cvoid}
+    kstride::NTuple{4,Int64}
+    vstride::NTuple{4,Int64}
+    kmax::Ptr{Cvoid}
+    vmax::Ptr{Cvoid}
+    E::Int64
+    T::Int64
+    H::Int64
+    P::Int64
+    kind::Int32
+    table::Ptr{Cvoid}
+    table_ld::Int64
+    width::Int64
+end
+cachec(c::Cache8, table) = Cache8C(s4(c.k).ptr, s4(c.v).ptr, s4(c.k).stride, s4(c.v).stride, pointer(c.kmax), pointer(c.vmax),
+                                   size(c.k)..., c.kind, pointer(table), stride(table, 2), size(table, 1))
+
+function cacheappend!(ctx::Ctx{B200Backend}, cache::Cache8, k, v, table, lens; news = nothing)
+    check(ccall((:b200_cache_append, LIB), Cint,
+                (Ptr{Cvoid}, Ref{Cache8C}, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, cachec(cache, table), size(k, 2), size(k, 4), s4(k), s4(v), pointer(lens), nullable(news)))
+    cache
+end
+function cacheread!(ctx::Ctx{B200Backend}, out, cache::Cache8, values::Bool, table, lens; starts = nothing)
+    check(ccall((:b200_cache_read, LIB), Cint,
+                (Ptr{Cvoid}, Ref{Cache8C}, Cint, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ref{Strided4}, Cint),
+                ctx.backend.handle, cachec(cache, table), values, size(out, 2), size(out, 4), nullable(starts), pointer(lens),
+                s4(out), dtcode(eltype(out))))
+    out
+end
+function cachesdpa!(ctx::Ctx{B200Backend}, out, q, cache::Cache8, table, lens; news = nothing, scale = 1 / sqrt(size(q, 1)), causal = true)
+    check(ccall((:b200_cache_attention, LIB), Cint,
+                (Ptr{Cvoid}, Ref{Cache8C}, Int64, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Cint, Cfloat, Cint, Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, cachec(cache, table), size(q, 2), size(q, 3), size(q, 4), s4(q), s4(out), dtcode(eltype(out)),
+                Float32(scale), causal, pointer(lens), nullable(news)))
+    out
+end
+
+struct Q4                           # b200_q4; the arrays it points to are Weight4's
+    data::Ptr{Cvoid}
+    scales::Ptr{Cvoid}
+    zeros::Ptr{Cvoid}
+    M::Int64
+    K::Int64
+    group::Int64
+end
+struct Weight4
+    arrays::Tuple
+    q4::Q4
+end
+# q (M, K) UInt8 of 0..15, scales (M, K ÷ group) Float16, zeros (M, K ÷ group) UInt8 or nothing
+function pack4(ctx::Ctx{B200Backend}, q, scales, zeros; group = 64)
+    M, K = size(q)
+    n = ntuple(_ -> Ref{Int64}(0), 3)
+    check(ccall((:b200_q4_sizes, LIB), Cint, (Int64, Int64, Int64, Ref{Int64}, Ref{Int64}, Ref{Int64}), M, K, group, n...))
+    arrays = ntuple(i -> i == 3 && zeros === nothing ? nothing : KernelAbstractions.allocate(ctx.backend, UInt8, n[i][]), 3)
+    w = Q4(nullable.(arrays)..., M, K, group)
+    zst = zeros === nothing ? (0, 0) : strides(zeros)
+    check(ccall((:b200_q4_pack, LIB), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Int64, Int64, Ref{Q4}),
+                ctx.backend.handle, pointer(q), strides(q)..., pointer(scales), strides(scales)..., nullable(zeros), zst..., w))
+    Weight4(arrays, w)
+end
+function matmul4!(ctx::Ctx{B200Backend}, out, W::Weight4, B, bias, epi)
+    check(ccall((:b200_matmul_q4, LIB), Cint,
+                (Ptr{Cvoid}, Ref{Q4}, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Cint, Cint),
+                ctx.backend.handle, W.q4, size(B, 2), pointer(B), stride(B, 2), nullable(bias), pointer(out), stride(out, 2),
+                dtcode(eltype(out)), epicode(epi)))
+    out
+end
+
 # ------------------------------------------------------------------ maxpool2d!, _to_copy (resample.jl:141, ops.jl:342-358)
 function maxpool2d!(ctx::Ctx{B200Backend}, out, x, k, s, p)
     xs, os = rootstrides(x), rootstrides(out)     # any (x, y, c, n) view: the NCHW permutes need no copy

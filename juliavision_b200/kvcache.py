@@ -119,7 +119,7 @@ def cachesdpa_(ctx: Ctx, out: DeviceArray, q: DeviceArray, cache: Cache8, table:
     """out = softmax(scale * Q K') V over the cache.  q and out (E, L, Hq, B), q fp16, out fp16 or fp32, E contiguous; Hq is a
     multiple of the cache's heads, query head i reads key head i // (Hq // H).  Row i of sequence b is its token
     lens[b] - news[b] + i and sees, when causal, the tokens up to itself, else all lens[b]; a row that sees none comes out as
-    zeros, rows from news[b] on (L without `news`) are left as they were."""
+    zeros, rows from news[b] on (L without `news`) are left as they were.  `out` does not overlap `q`."""
     if scale is None and q.ndim == 4 and q.shape[0] > 0:
         scale = 1.0 / sqrt(q.shape[0])
     rc = _lib.host().cachesdpa(ctx.handle, out, q, cache, table, lens, news, scale, causal)
