@@ -11,7 +11,8 @@
 // Four row tiles lie side by side, unit by unit, so that 64 rows are one stream of 2 KB a k block.
 //
 // Two kernels for few tokens.  A small weight, whose rows do not fill the GPU for long, is a chain of round trips: a block takes 16
-// rows, its warps share K and have all their loads in flight at once (linear4_kernel).  A large one is bandwidth-bound: the list of
+// rows, or 32 for up to 40 tokens at a time (each weight is made into fp16 once for all of them), its warps share K and have all
+// their loads in flight at once (linear4_kernel).  A large one is bandwidth-bound: the list of
 // (64 rows, 8 or 16 tokens, k block) is dealt out to all warps in equal contiguous shares, each streamed by bulk copies through a ring
 // of its own; parts of rows meet at the ends of blocks and in a second launch (linear4_stream_kernel, shares.cuh).
 #include <cuda_fp16.h>
@@ -28,6 +29,10 @@ namespace b200 {
 constexpr int L4_WARPS = 8;      // of a block, which share K
 constexpr int L4_TOKENS = 96;    // tokens the kernels take; more go through fp16 weights in the workspace (4096 x 4096: 64 tokens 17 us and 24, 128 28 and 24)
 constexpr double L4_STREAM_TILES = 4608;   // of 64 rows, 16 tokens and 64 inputs: from here on a list for all warps
+// More than 16 tokens: rounds of loads, times token tiles a block, up to which the blocks that have all of them at once are faster than
+// the list.  us, blocks / list: 24 x 5120 x 1280 6.7 / 10.6, 37 x 5120 x 1280 (15) 8.4 / 10.4, 22 x 3836 x 3456 (21) 9.9 / 11.3,
+// 32 x 4096 x 4096 (32) 12.4 / 12.2, 37 x 1280 x 5120 (50) 15.9 / 10.8.
+constexpr int64_t L4_ROUNDS = 21;
 
 struct Linear4Params {
     const uint4* data;            // [four row tiles][k block][row tile][lane]
@@ -133,51 +138,62 @@ __device__ __forceinline__ void l4_store(const Linear4Params& p, int64_t m, int 
     else ((__half*)p.out)[n * p.ldo + m] = __float2half_rn(apply_act(p.epi, __half2float(__float2half_rn(v))));
 }
 
-// One row tile and NT tiles of 8 tokens a block; the warps take every L4_WARPS-th k block, AT_ONCE of them at a time.  SMALL: groups of 32.
-template <int NT, bool SMALL>
-__global__ void __launch_bounds__(32 * L4_WARPS)
+// ROWS row tiles and NT tiles of 8 tokens a block; the warps take every L4_WARPS-th k block, AT_ONCE of them at a time.  SMALL: groups of 32.
+template <int ROWS, int NT, bool SMALL>
+__global__ void __launch_bounds__(32 * L4_WARPS, ROWS == 1 ? 1 : 2)
 linear4_kernel(const Linear4Params p) {
-    constexpr int COLS = 8 * NT + 1, GROUPS = SMALL ? 2 : 1, AT_ONCE = NT == 1 ? 4 : 3;
+    constexpr int COLS = 8 * NT + 1, GROUPS = SMALL ? 2 : 1, AT_ONCE = ROWS > 1 ? 1 : NT == 1 ? 4 : 3;
     __shared__ float red[L4_WARPS][16][COLS];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int mt = blockIdx.x, n0 = blockIdx.y * 8 * NT;
+    const int mt0 = blockIdx.x * ROWS, n0 = blockIdx.y * 8 * NT;
     grid_dep_wait();
     grid_dep_launch();
-    float acc[NT][4];
+    float acc[ROWS][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[r][n][0] = acc[r][n][1] = acc[r][n][2] = acc[r][n][3] = 0.f;
     for (int kb0 = warp; kb0 < p.KB; kb0 += L4_WARPS * AT_ONCE) {
-        uint4 w[AT_ONCE];
-        uint32_t sc[AT_ONCE][GROUPS], zb[AT_ONCE][GROUPS], x[AT_ONCE][NT][8];
+        uint4 w[AT_ONCE][ROWS];
+        uint32_t sc[AT_ONCE][ROWS][GROUPS], zb[AT_ONCE][ROWS][GROUPS], x[AT_ONCE][NT][8];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
             const int kb = kb0 + u * L4_WARPS;
             const bool in = kb < p.KB;
-            w[u] = in ? __ldg(p.data + p.unit(mt, kb) * 32 + lane) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < GROUPS; ++j) {
-                const int grp = (kb * 64 + j * 32) >> p.logg;
-                const bool live = in && grp < p.NG;    // the last k block may be half empty
-                sc[u][j] = live ? __ldg(p.scales + p.group8(mt, grp) + g) : 0;
-                zb[u][j] = live && p.zeros != nullptr ? __ldg(p.zeros + p.group8(mt, grp) + g) : 0x88u;
+            for (int r = 0; r < ROWS; ++r) {
+                w[u][r] = in ? __ldg(p.data + p.unit(mt0 + r, kb) * 32 + lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < GROUPS; ++j) {
+                    const int grp = (kb * 64 + j * 32) >> p.logg;
+                    const bool live = in && grp < p.NG;    // the last k block may be half empty
+                    sc[u][r][j] = live ? __ldg(p.scales + p.group8(mt0 + r, grp) + g) : 0;
+                    zb[u][r][j] = live && p.zeros != nullptr ? __ldg(p.zeros + p.group8(mt0 + r, grp) + g) : 0x88u;
+                }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) l4_input(p, n0 + n * 8 + g, in ? kb : p.KB, t, x[u][n]);
         }
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) l4_block<NT, SMALL>(acc, w[u], sc[u], zb[u], x[u]);
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) l4_block<NT, SMALL>(acc[r], w[u][r], sc[u][r], zb[u][r], x[u]);
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int r = 0; r < ROWS; ++r) {
+        if (r > 0) __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) red[warp][g + (k >> 1) * 8][n * 8 + 2 * t + (k & 1)] = acc[n][k];
-    __syncthreads();
-    for (int i = tid; i < 16 * 8 * NT; i += 32 * L4_WARPS) {
-        const int row = i % 16, col = i / 16;
-        float v = 0.f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int w = 0; w < L4_WARPS; ++w) v += red[w][row][col];
-        l4_store(p, (int64_t)mt * 16 + row, n0 + col, v);
+            for (int k = 0; k < 4; ++k) red[warp][g + (k >> 1) * 8][n * 8 + 2 * t + (k & 1)] = acc[r][n][k];
+        __syncthreads();
+        for (int i = tid; i < 16 * 8 * NT; i += 32 * L4_WARPS) {
+            const int row = i % 16, col = i / 16;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < L4_WARPS; ++w) v += red[w][row][col];
+            l4_store(p, (int64_t)(mt0 + r) * 16 + row, n0 + col, v);
+        }
     }
 }
 
@@ -486,10 +502,10 @@ linear4_pack_kernel(const PackParams p) {
     }
 }
 
-template <int NT>
+template <int ROWS, int NT>
 static int l4_launch(b200_ctx* ctx, const Linear4Params& p) {
-    auto kern = p.logg == 5 ? linear4_kernel<NT, true> : linear4_kernel<NT, false>;
-    B200_CUDA(launch_dep(kern, dim3((unsigned)p.MT, (unsigned)cdiv(p.N, 8 * NT)), dim3(32 * L4_WARPS), 0, ctx->stream, 1, p));
+    auto kern = p.logg == 5 ? linear4_kernel<ROWS, NT, true> : linear4_kernel<ROWS, NT, false>;
+    B200_CUDA(launch_dep(kern, dim3((unsigned)cdiv(p.MT, ROWS), (unsigned)cdiv(p.N, 8 * NT)), dim3(32 * L4_WARPS), 0, ctx->stream, 1, p));
     ctx->launches++;
     return B200_OK;
 }
@@ -593,8 +609,11 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
     }
     p.d_status = ctx->d_status;
     const int nt = N <= 8 ? 1 : 2;
+    // More than 16 tokens: up to 40 to a block of linear4_kernel, whose warps take a round trip of loads a k block.
+    const int64_t groups = N <= 16 ? 1 : cdiv(N, 40), many = N <= 16 ? nt : cdiv(cdiv(N, 8), groups);
+    const int64_t rounds = cdiv(p.KB, L4_WARPS) * cdiv(cdiv(p.MT, 2) * groups, 2 * (int64_t)ctx->prop.multiProcessorCount);
     const double tiles = (double)cdiv(p.MT, 4) * (double)cdiv(N, 8 * nt) * p.KB;
-    if (tiles >= L4_STREAM_TILES && p.whole) {
+    if (p.whole && (N <= 16 ? tiles >= L4_STREAM_TILES : rounds * many > L4_ROUNDS)) {
         const auto go = [&](auto small, auto zp) {
             return nt == 1 ? l4_stream_launch<1, decltype(small)::value, decltype(zp)::value>(ctx, p)
                            : l4_stream_launch<2, decltype(small)::value, decltype(zp)::value>(ctx, p);
@@ -604,7 +623,13 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
         if (p.logg == 5) return p.zeros ? go(yes(), yes()) : go(yes(), no());
         return p.zeros ? go(no(), yes()) : go(no(), no());
     }
-    return nt == 1 ? l4_launch<1>(ctx, p) : l4_launch<2>(ctx, p);
+    switch (many) {
+    case 1: return l4_launch<1, 1>(ctx, p);
+    case 2: return l4_launch<1, 2>(ctx, p);
+    case 3: return l4_launch<2, 3>(ctx, p);
+    case 4: return l4_launch<2, 4>(ctx, p);
+    default: return l4_launch<2, 5>(ctx, p);
+    }
 }
 
 } // extern "C"

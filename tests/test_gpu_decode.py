@@ -479,6 +479,28 @@ def check4(got, x, w, bias, epi, dtype, rounded):
     near(got, y, tol)
 
 
+@pytest.mark.parametrize("N", [17, 24, 25, 32, 40, 41, 64, 80, 81, 96, 97])
+@pytest.mark.parametrize("shape", [(33, 64, 32, True, 0), (175, 192, 64, False, 0), (16, 1344, 32, False, 0), (70, 4096, 128, True, 0), (49, 4096, 64, True, 1)], ids=str)
+def test_matmul4_between_few_and_many_tokens(ctx, N, shape):
+    """Token tiles of a block that are not full, an odd number of row tiles, a last k block that is half empty; by the list where K is
+    long, or not, where activations lie off 16-byte boundaries."""
+    M, K, group, zeros, pad = shape
+    rng = np.random.default_rng(20)
+    q = rng.integers(0, 16, (K, M)).astype(np.uint8)
+    s = (rng.random((K // group, M)) * 0.02 + 0.001).astype(F16)
+    z = rng.integers(0, 16, (K // group, M)).astype(np.uint8) if zeros else None
+    x, bias = rng.standard_normal((N, K + pad)).astype(F16), rng.standard_normal(M).astype(F16)
+    w = jv.pack4(ctx, ctx.toback(q), ctx.toback(s), None if z is None else ctx.toback(z), group)
+    d, buf = ctx.toback(x), ctx.allocate(F16, M + 3, N + 1)
+    ctx.fill_bytes(buf, 0xFF)
+    out = jv.DeviceArray(ctx, buf.ptr, F16, (M, N), (1, M + 3), owner=buf)
+    jv.matmul4_(ctx, out, w, jv.DeviceArray(ctx, d.ptr, F16, (K, N), (1, K + pad), owner=d), ctx.toback(bias))
+    ctx.synchronize()
+    got = buf.to_host()
+    check4(got[:N, :M], x[:, :K], ref.weight4(q, s, z, group), bias, "identity", F16, rounded=N > 96)
+    assert np.isnan(got[N:]).all() and np.isnan(got[:, M:]).all()
+
+
 def test_matmul4_strides(ctx):
     """Weights given (M, K) with K contiguous, activations and results in wider arrays, off 16-byte boundaries, no bias."""
     rng = np.random.default_rng(16)
