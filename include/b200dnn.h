@@ -267,7 +267,7 @@ typedef struct {
 /* Writes the new tokens, k and v (E,L,H,B) fp16, E contiguous.  A page's max becomes the largest magnitude among the values
  * written to it, or stays where it was larger and tokens before the new ones are in the page; those are rounded again when it
  * grows.  Rounding is to nearest, ties to even, of the exact quotients.  A value that is not finite makes its page's max, for its head, a NaN.
- * Pages that are written belong to one sequence of the call.  Rows at negative positions are skipped. */
+ * A page that is written belongs to one sequence of the call and to one place of its table.  Rows at negative positions are skipped. */
 int b200_cache_append(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int64_t B, const b200_strided4* k,
                       const b200_strided4* v, const int32_t* lens, const int32_t* news);
 /* Tokens starts[b] + row (starts NULL: row), row < L, of the keys (values = 0) or values (1) as numbers, rounded to out_dtype:

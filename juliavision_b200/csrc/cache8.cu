@@ -1,4 +1,6 @@
-// Writing tokens into the paged 8-bit cache and reading them back (cache8.cuh has the format).  Both are bandwidth-bound.
+// Writing tokens into the paged 8-bit cache and reading them back (cache8.cuh has the format).  Two bytes read and one written an
+// element, or the reverse, so HBM is the floor; what comes first is instructions, 19 an element written.  13600 tokens of four
+// sequences, 8 heads of 128: keys and values written in 21 us (3.9 TB/s), each read back as fp16 in 11.6 us (3.6 TB/s).
 //
 // Append: one block owns one (sequence, page, head) of the keys or of the values, so nothing is shared between blocks.  It holds
 // the page's new elements in registers (up to 64 a thread), takes their largest magnitude as an integer maximum over the fp16

@@ -82,7 +82,8 @@ def _rows(op: str, a: DeviceArray, E: int, H: int, dtypes=(np.float16,)):
 def cacheappend_(ctx: Ctx, cache: Cache8, k: DeviceArray, v: DeviceArray, table: DeviceArray, lens: DeviceArray,
                  news: Optional[DeviceArray] = None) -> Cache8:
     """Write new tokens: k and v (E, L, H, B) fp16, E contiguous; row i of sequence b is its token lens[b] - news[b] + i (lens
-    with the new tokens in it), rows from news[b] on (L without `news`) are not tokens.  The pages written belong to one sequence."""
+    with the new tokens in it), rows from news[b] on (L without `news`) are not tokens.  A page that is written belongs to one
+    sequence, and to one place of its table."""
     rc = _lib.host().cacheappend(ctx.handle, cache, k, v, table, lens, news)
     if rc is not None:
         check(rc)
