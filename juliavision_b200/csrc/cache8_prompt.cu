@@ -1,9 +1,9 @@
 // Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
 // cache8_attention.cu.
 //
-// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 170 us, 0.9 PFLOP/s.
-// What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', 3750 clocks a block of
-// 128 keys for two tiles whose products take 2048), which the other tile's covers in part.
+// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 163 us, 0.95 PFLOP/s.
+// What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 3600 clocks a block
+// of 128 keys for two tiles whose products take 2048), which the other tile's covers in part.
 //
 // The query rows of a key head (the heads that share it, times the new tokens) are stacked; a block takes two tiles of 128 of them
 // and walks their keys in blocks of 128: S = Q K^T and O += P V on tcgen05 with S, P (rounded to fp16, the products' operand type)
@@ -28,6 +28,7 @@ constexpr int CP_THREADS = 512;
 constexpr int CP_ROWS = 128, CP_KEYS = 128;     // of a tile
 constexpr int CP_ATOM = 128 * 128;              // 128 rows x 64 fp16
 constexpr int CP_LEAST = 2;                     // blocks of keys of a share
+constexpr int CP_START = 3;                     // blocks of keys that an item's start and end take as long as
 constexpr int CP_SCALES = 4;                    // blocks of constants in flight
 constexpr int CP_SOFTMAX_REGS = 176, CP_CONVERT_REGS = 104, CP_OTHER_REGS = 56;
 static_assert(2 * 128 * CP_SOFTMAX_REGS + 128 * CP_CONVERT_REGS + 128 * CP_OTHER_REGS <= CP_THREADS * 128, "what the launch holds");
@@ -116,8 +117,10 @@ __device__ __forceinline__ void cp_store8(const CachePromptParams& p, int64_t at
 // What the rows of an item see: item -> (row pair, head, sequence), later rows, whose keys are more, first.
 struct CpItem {
     int b, h, r0, rows, n, m, blocks;   // first row, rows of the sequence (all of its heads), length, new tokens, blocks of keys
-    // its length in the list that is shared out: an item without keys has its rows of zeros to write
-    __device__ __forceinline__ int weight() const { return r0 >= rows ? 0 : blocks > 0 ? blocks : 1; }
+    // Its length in the list that is shared out: `start` for its start and end, then its blocks.  An item without keys has rows of zeros
+    // to write.
+    __device__ __forceinline__ int weight(int start) const { return r0 >= rows ? 0 : start + (blocks > 0 ? blocks : 1); }
+    __device__ __forceinline__ int block(int j, int start) const { return j <= start ? 0 : j - start < blocks ? j - start : blocks; }
 };
 __device__ __forceinline__ CpItem cp_item(const CachePromptParams& p, int item) {
     CpItem it;
@@ -140,23 +143,23 @@ __device__ __forceinline__ CpItem cp_item(const CachePromptParams& p, int item) 
 struct CpWalk {
     long long left;     // blocks of the share from here on
     int item, j;        // where the next part begins
+    int start;          // CpItem::weight
 
     __device__ __forceinline__ bool next(const CachePromptParams& p, CpItem& it, int& at, int& j0, int& nblk) {
         while (left > 0 && item < p.items) {
             it = cp_item(p, item);
-            const int w = it.weight();
+            const int w = it.weight(start);
             if (w == 0) {                     // nor has any other head of these rows
                 item += p.c.H - item % p.c.H;
                 j = 0;
                 continue;
             }
-            at = item, j0 = j;
-            const int take = w - j < left ? w - j : (int)left;
-            nblk = it.blocks > 0 ? take : 0;
+            const int from = j, take = w - j < left ? w - j : (int)left;
+            at = item, j0 = it.block(j, start), nblk = it.block(j + take, start) - j0;
             left -= take;
             j += take;
             if (j == w) ++item, j = 0;
-            return true;
+            if (nblk > 0 || (it.blocks == 0 && from == 0)) return true;
         }
         return false;
     }
@@ -176,7 +179,7 @@ template <int EP> struct CpCfg {
     static constexpr int S_BARS = S_C + (CP_SCALES * (int)sizeof(CpScales) + 15) / 16 * 16;
     static constexpr int BARRIERS = 2 + 4 * STAGES + 2 * 5 + 2 * CP_SCALES + 2 * CP_PARTS;
     static constexpr int S_WALK = S_BARS + (BARRIERS + 1) * 8;   // where the share begins; what finding it adds up
-    static constexpr int S_PART = S_WALK + 16 + 48 * 8;
+    static constexpr int S_PART = S_WALK + (int)sizeof(CpWalk) + 48 * 8;
     static constexpr int SMEM = S_PART + CP_PARTS * (int)sizeof(CpPart);
     static constexpr int O_COL = 2 * CP_KEYS;
 };
@@ -243,43 +246,45 @@ cache_prompt_kernel(const CachePromptParams p) {
     grid_dep_launch();
     CpWalk* walk = reinterpret_cast<CpWalk*>(smem + Cfg::S_WALK);
     if (!p.shared) {
-        const int w = cp_item(p, blockIdx.x).weight();
+        const int w = cp_item(p, blockIdx.x).weight(0);
         if (w == 0) return;                        // uniform: before any barrier or tensor memory exists
-        if (threadIdx.x == 0) *walk = {w, (int)blockIdx.x, 0};
+        if (threadIdx.x == 0) *walk = {w, (int)blockIdx.x, 0, 0};
     } else {
         // Weights are the same for all heads: an entry has the H items of a row pair of a sequence.  A thread sums a run of
         // them; the sums before it tell which thread's run the share of this block begins in.
         long long* sums = reinterpret_cast<long long*>(smem + Cfg::S_WALK + sizeof(CpWalk));
         const int entries = p.items / c.H, run = (entries + CP_THREADS - 1) / CP_THREADS, e0 = threadIdx.x * run;
-        long long mine = 0;
-        int some = 0, longest = 0;
+        long long mine = 0, some = 0;              // blocks of keys, items
+        int longest = 0;
         for (int e = e0; e < e0 + run && e < entries; ++e) {
-            const int w = cp_item(p, e * c.H).weight();
+            const int w = cp_item(p, e * c.H).weight(0);
             mine += (long long)w * c.H;
             some += w > 0 ? c.H : 0;
             longest = w > longest ? w : longest;
         }
-        long long upto = mine;
+        long long upto = mine, items = some;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += x;
-            some += __shfl_xor_sync(0xffffffffu, some, d);
+            const long long x = __shfl_up_sync(0xffffffffu, upto, d), z = __shfl_up_sync(0xffffffffu, items, d);
+            if (lane >= d) upto += x, items += z;
             const int y = __shfl_xor_sync(0xffffffffu, longest, d);
             longest = y > longest ? y : longest;
         }
-        if (lane == 31) sums[warp] = upto;
-        if (lane == 0) sums[16 + warp] = some, sums[32 + warp] = longest;
+        if (lane == 31) sums[warp] = upto, sums[16 + warp] = items, sums[32 + warp] = longest;
         __syncthreads();
         long long total = 0, pieces = 0;
         for (int i = 0; i < CP_THREADS / 32; ++i) {
-            if (i == warp) upto += total;
+            if (i == warp) upto += total, items += pieces;
             total += sums[i], pieces += sums[16 + i];
             if (sums[32 + i] > longest) longest = (int)sums[32 + i];
         }
         // as many shares as blocks, but of CP_LEAST blocks of keys at least where there are no more items than that makes
         const long long want = pieces > total / CP_LEAST ? pieces : total / CP_LEAST;
         long long many = want < gridDim.x ? want : gridDim.x;
+        // Lengths far apart: what the start and end of an item take counts too, or a share of many short ones is the last to end (74
+        // items of 4 to 39 blocks 57 us without and 51 with; 128 of 64 to 80 170 and 174, 32 of 2 to 8 blocks 24 and 28).
+        const int start = 4 * total < 3 * pieces * longest && total >= 4 * many ? CP_START : 0;
+        total += start * pieces, upto += start * items, mine += start * some, longest += start;
         // Items of one length: whole shares an item, where the blocks that this leaves out would save the others less than the five
         // blocks of keys that a second part's start and end cost (32 items of 32 blocks: 37.5 us with 148 shares, 33.1 with 128).
         const long long even = pieces > 0 && pieces <= many ? many - many % pieces : many;
@@ -294,12 +299,12 @@ cache_prompt_kernel(const CachePromptParams p) {
         if (begin >= upto - mine && begin < upto) {
             long long at = upto - mine;
             for (int e = e0; e < e0 + run && e < entries; ++e) {
-                const int w = cp_item(p, e * c.H).weight();
+                const int w = cp_item(p, e * c.H).weight(start);
                 if (begin < at + (long long)w * c.H) {
                     const int h = (int)floor_div(begin - at, w);
                     at += (long long)h * w;
-                    *walk = {end - begin, e * c.H + h, (int)(begin - at)};
-                    sums[0] = at, sums[1] = at + w - 1, sums[2] = total;
+                    *walk = {end - begin, e * c.H + h, (int)(begin - at), start};
+                    sums[0] = at + start, sums[1] = at + w - 1, sums[2] = total;   // its first block, its last
                     sums[3] = shares.warps;
                     break;
                 }
@@ -389,7 +394,7 @@ cache_prompt_kernel(const CachePromptParams p) {
         } else if (warp == 15) {
             // -------------------------------------------------- parts of items
             CpWalk mine = *walk;
-            const int first = mine.j > 0 ? mine.item : -1;
+            const int first = mine.j > mine.start ? mine.item : -1;      // its share begins inside this item's blocks
             int s = 0;
             CpPart x;
             do {
@@ -500,8 +505,12 @@ cache_prompt_kernel(const CachePromptParams p) {
                 page1 = c.T > 16 ? page0 : key + 16 < it.n ? (int)c.page(it.b, (key >> 4) + 1) : -1;
             }
         };
-        uint4 kq[NV], vq[NV];     // the next block's, on their way while this one's are written
-        auto fetch = [&](uint4 (&cur)[NV], int j, int side) {   // zeros where there is no key: what P = 0 multiplies is a number
+        // Sides in turn: K(0), V(0), K(1), ...  One copy of the code serves both: the loops of all warps together do not fit the nearer
+        // instruction caches, and this one's length is everyone's wait (2048 tokens over 10240 177 us with a copy each, 163 with one).
+        // What it costs is a side less on its way from memory, which a cache that is read once misses: 64 tokens over 100000 122 us
+        // and 134.  Asking L2 for later rows gave half of that back, and its code took as much from the others.
+        uint4 cur[NV], nxt[NV];
+        auto fetch = [&](uint4 (&to)[NV], int j, int side) {   // zeros where there is no key: what P = 0 multiplies is a number
             const int key0 = (j_begin + j) * CP_KEYS + w * 32, in = (key0 & (c.T - 1)) + sub;
             const uint8_t* base = (side ? c.v : c.k) + it.h * (side ? c.vH : c.kH) + ch * 16;
             const int64_t sT = side ? c.vT : c.kT, sP = side ? c.vP : c.kP;
@@ -511,11 +520,13 @@ cache_prompt_kernel(const CachePromptParams p) {
             for (int i = 0; i < NV; ++i) {
                 const int a = i % ATOMS, r = i / ATOMS;
                 const bool on = (r < 2 ? page0 : page1) >= 0 && key0 + 8 * r + sub < it.n && a * 64 + ch * 16 < c.E;
-                cur[i] = make_uint4(0, 0, 0, 0);
-                if (on) cur[i] = __ldg(reinterpret_cast<const uint4*>((r < 2 ? at0 : at1) + (r & 1) * 8 * sT + a * 64));
+                to[i] = make_uint4(0, 0, 0, 0);
+                if (on) to[i] = __ldg(reinterpret_cast<const uint4*>((r < 2 ? at0 : at1) + (r & 1) * 8 * sT + a * 64));
             }
         };
-        auto write = [&](const uint4 (&cur)[NV], uint32_t tile, bool values) {
+        // A value that is the code of a NaN reads as 448: a row that may not see it must not meet it.  The lesser of a number and a NaN is
+        // the number, so for keys the bound is a NaN and all stays as it is.
+        auto write = [&](uint32_t tile, __half2 most) {
             const uint32_t even = tile + (w * 32 + sub) * 128 + (((2 * ch) ^ sub) << 4);   // a row's place modulo 8 is sub
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -524,8 +535,7 @@ cache_prompt_kernel(const CachePromptParams p) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     cache_halves<FP8>(v[k], h[2 * k], h[2 * k + 1]);
-                    if (FP8 && values) {     // the code of a NaN reads as 448: a row that may not see it must not meet it
-                        const __half2 most = __half2half2(__ushort_as_half(0x5f00));
+                    if (FP8) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             const __half2 x = __hmin2(*reinterpret_cast<__half2*>(&h[2 * k + u]), most);
@@ -544,23 +554,24 @@ cache_prompt_kernel(const CachePromptParams p) {
         bool ok = true;
         while (ok && next()) {
             look(0);
-            fetch(kq, 0, 0);
-            fetch(vq, 0, 1);
-            look(1);
-            for (int j = 0; j < nblk; ++j) {
-                const int s = done % STAGES;
-                const uint32_t ph = (uint32_t)((done / STAGES) & 1) ^ 1;
-                ++done;
-                if (!mbar_wait(&k_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
-                write(kq, smem_u32(smem + Cfg::S_K + s * Cfg::SIDE), false);
-                if (lane == 0) mbar_arrive(&k_full[s]);
-                fetch(kq, j + 1, 0);
-                if (!mbar_wait(&v_empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
-                write(vq, smem_u32(smem + Cfg::S_V + s * Cfg::SIDE), true);
-                if (lane == 0) mbar_arrive(&v_full[s]);
-                fetch(vq, j + 1, 1);
-                look(j + 2);
+            fetch(cur, 0, 0);
+#pragma unroll 1
+            for (int j = 0; ok && j < nblk; ++j) {
+                const int s = (done + j) % STAGES;
+                const uint32_t ph = (uint32_t)(((done + j) / STAGES) & 1) ^ 1;
+#pragma unroll 1
+                for (int side = 0; side < 2; ++side) {
+                    if (side) look(j + 1);           // what is fetched next is of the next block
+                    fetch(nxt, j + side, side ^ 1);
+                    uint64_t *empty = side ? v_empty : k_empty, *full = side ? v_full : k_full;
+                    if (!mbar_wait(&empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
+                    write(smem_u32(smem + Cfg::S_K + (side * STAGES + s) * Cfg::SIDE), __half2half2(__ushort_as_half(side ? 0x5f00 : 0x7fff)));
+                    if (lane == 0) mbar_arrive(&full[s]);
+#pragma unroll
+                    for (int u = 0; u < NV; ++u) cur[u] = nxt[u];
+                }
             }
+            done += nblk;
         }
     } else {
         // ------------------------------------------------------ softmax and results
@@ -821,10 +832,10 @@ static int cp_launch(b200_ctx* ctx, CachePromptParams& p) {
     const int64_t items = cdiv((int64_t)p.L * p.G, 2 * CP_ROWS) * p.c.H * p.B;
     B200_REQUIRE(items < (1ll << 24), B200_DECLINE_EXTENT, "cache_attention: %lld row tiles", (long long)items);
     p.items = (int)items;
-    // Equal shares keep every SM busy to the end; they cost a look for the share's place and a second launch that joins, together
-    // about what four blocks of keys do, and a further start and end for most items, about six (of 2 us at E = 128).  Items a launch
-    // block / shares, us: 128 items of 64 to 80 blocks 177 / 171 (E = 128), 167 / 147 (E = 64); 256 of 28 to 32 blocks 148 / 174;
-    // 8 of 782 blocks 1554 / 125; 32 of 2 to 8 blocks 27.5 / 23.5.
+    // Equal shares keep every SM busy to the end.  They cost a look for the share's place and a second launch that joins, together
+    // about what four blocks of keys do, and a further start and end for most items, about six (of 2 us at E = 128).  An item a launch
+    // block / shares, us: 128 items of 64 to 80 blocks 179 / 171 (E = 128), 166 / 147 (E = 64); 74 of 4 to 39 82 / 50; 8 of 782 1570 / 134;
+    // 32 of 2 to 8 27.7 / 23.9; 140 of 50 116 / 131; 256 of 28 to 32 148 / 167; 48 of 1 to 5 21 / 27; 1680 of 1 to 6 176 / 216.
     const int64_t blocks = cdiv((int64_t)p.c.width * p.c.T, CP_KEYS);
     p.shared = items <= 8 * sms && items * (blocks + 6) + 4 * sms < cdiv(items, sms) * blocks * sms;
     const int64_t grid = p.shared ? sms : items;
