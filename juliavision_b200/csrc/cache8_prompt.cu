@@ -508,7 +508,7 @@ cache_prompt_kernel(const CachePromptParams p) {
         // Sides in turn: K(0), V(0), K(1), ...  One copy of the code serves both: the loops of all warps together do not fit the nearer
         // instruction caches, and this one's length is everyone's wait (2048 tokens over 10240 177 us with a copy each, 163 with one).
         // What it costs is a side less on its way from memory, which a cache that is read once misses: 64 tokens over 100000 122 us
-        // and 134.  Asking L2 for later rows gave half of that back, and its code took as much from the others.
+        // and 127.  Asking L2 for later rows gave some of that back, and its code took as much from the others.
         uint4 cur[NV], nxt[NV];
         auto fetch = [&](uint4 (&to)[NV], int j, int side) {   // zeros where there is no key: what P = 0 multiplies is a number
             const int key0 = (j_begin + j) * CP_KEYS + w * 32, in = (key0 & (c.T - 1)) + sub;
@@ -561,8 +561,8 @@ cache_prompt_kernel(const CachePromptParams p) {
                 const uint32_t ph = (uint32_t)(((done + j) / STAGES) & 1) ^ 1;
 #pragma unroll 1
                 for (int side = 0; side < 2; ++side) {
-                    if (side) look(j + 1);           // what is fetched next is of the next block
                     fetch(nxt, j + side, side ^ 1);
+                    if (side == 0) look(j + 1);      // what is fetched next is of the next block
                     uint64_t *empty = side ? v_empty : k_empty, *full = side ? v_full : k_full;
                     if (!mbar_wait(&empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
                     write(smem_u32(smem + Cfg::S_K + (side * STAGES + s) * Cfg::SIDE), __half2half2(__ushort_as_half(side ? 0x5f00 : 0x7fff)));
@@ -834,7 +834,7 @@ static int cp_launch(b200_ctx* ctx, CachePromptParams& p) {
     p.items = (int)items;
     // Equal shares keep every SM busy to the end.  They cost a look for the share's place and a second launch that joins, together
     // about what four blocks of keys do, and a further start and end for most items, about six (of 2 us at E = 128).  An item a launch
-    // block / shares, us: 128 items of 64 to 80 blocks 179 / 171 (E = 128), 166 / 147 (E = 64); 74 of 4 to 39 82 / 50; 8 of 782 1570 / 134;
+    // block / shares, us: 128 items of 64 to 80 blocks 179 / 171 (E = 128), 166 / 147 (E = 64); 74 of 4 to 39 82 / 50; 8 of 782 1570 / 127;
     // 32 of 2 to 8 27.7 / 23.9; 140 of 50 116 / 131; 256 of 28 to 32 148 / 167; 48 of 1 to 5 21 / 27; 1680 of 1 to 6 176 / 216.
     const int64_t blocks = cdiv((int64_t)p.c.width * p.c.T, CP_KEYS);
     p.shared = items <= 8 * sms && items * (blocks + 6) + 4 * sms < cdiv(items, sms) * blocks * sms;
