@@ -1,20 +1,20 @@
 // Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
 // cache8_attention.cu.
 //
-// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 163 us, 0.95 PFLOP/s.
-// What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 3600 clocks a block
-// of 128 keys for two tiles whose products take 2048), which the other tile's covers in part.
+// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 207 us, 0.75 PFLOP/s.
+// What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 4600 clocks a block
+// of 128 keys for two tiles whose products take 3072), which the other tile's covers in part.
 //
 // The query rows of a key head (the heads that share it, times the new tokens) are stacked; a block takes two tiles of 128 of them
-// and walks their keys in blocks of 128: S = Q K^T and O += P V on tcgen05 with S, P (rounded to fp16, the products' operand type)
-// and O in tensor memory.  The 8-bit operands become fp16 on the way to shared memory, exactly, once for 256 rows: four warps
+// and walks their keys in blocks of 128: S = Q K^T and O += P V on tcgen05 with S, P (two fp16 halves, 21 bits and more of a
+// weight, as for few rows) and O in tensor memory.  The 8-bit operands become fp16 on the way to shared memory, exactly, once for 256 rows: four warps
 // read them from the pages into registers a side ahead and write them in the 128-byte swizzle.  No operand carries a scale: a
 // page's key scale (and the softmax's own) is the factor of its columns' exponents, its value scale, relative to the largest so
 // far, a summand of them; the row sum takes that back a group of 16 keys at a time.
 //
 //   warps 0-3  softmax of tile 0, warps 4-7 of tile 1: one thread a row, the row's 128 scores in registers
 //   warps 8-11 fetch and convert: K(j), V(j), K(j+1), ...
-//   warps 12, 13  issue one tile's products each:  Q K(j)',  P(j) V(j), Q K(j+1)', ...; P lies over the first half of S
+//   warps 12, 13  issue one tile's products each:  Q K(j)',  P(j) V(j), Q K(j+1)', ...; P's halves lie over the halves of S
 //   warp 14    looks up pages and scales and lays out each block's constants, two blocks ahead
 //   warp 15    walks the block's share of the items' keys (CpWalk), an item's part at a time, and tells the others
 #include <cuda_fp16.h>
@@ -72,6 +72,18 @@ __device__ __forceinline__ void cp_tmem_st16(uint32_t taddr, const uint32_t* r) 
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = r[i];
     tmem_st16(taddr, v);
+}
+// Two weights as two halves each: what fp16 holds of them, cut off, and what is left, rounded; off by 2^-21 of themselves, or, below
+// 2^-14, by a step of 2^-24.  (One half alone: 163 us for 207 at 2048 tokens over 10240, and 2.9e-4 of the result for 2.1e-4.  The upper
+// ones rounded to nearest and converted back 217; the lower ones made after the exponentials' turn has passed, beside the upper ones'
+// product, 216.)
+__device__ __forceinline__ void cp_halves(float a, float b, uint32_t& upper, uint32_t& lower) {
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(upper) : "f"(b), "f"(a));
+    const float ma = __uint_as_float((__float_as_uint(a) & 0xffffe000u) ^ 0x80000000u), mb = __uint_as_float((__float_as_uint(b) & 0xffffe000u) ^ 0x80000000u);
+    float ra, rb;
+    unpack2(add2(pack2(a, b), pack2(ma, mb)), ra, rb);
+    const __half2 l = __floats2half2_rn(ra, rb);
+    lower = *reinterpret_cast<const uint32_t*>(&l);
 }
 // 16 bytes to shared memory on their own, zeros where there are none to read
 __device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool on) {
@@ -447,8 +459,11 @@ cache_prompt_kernel(const CachePromptParams p) {
             auto issue_pv = [&](int j, int sv, int k0, int k1) {
                 const uint32_t v_addr = smem_u32(smem + Cfg::S_V + sv * Cfg::SIDE);
 #pragma unroll
-                for (int k = k0; k < k1; ++k)
-                    umma_ts(o_tmem, s_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
+                for (int k = k0; k < k1; ++k) {
+                    const uint64_t vdesc = smem_desc_at(vdesc0, v_addr + k * 2048);
+                    umma_ts(o_tmem, s_tmem + k * 8, vdesc, idesc_o, (j | k) != 0);
+                    umma_ts(o_tmem, s_tmem + CP_KEYS / 2 + k * 8, vdesc, idesc_o, 1);
+                }
             };
             bool ok = true;
             while (ok && next()) {
@@ -694,7 +709,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    uint32_t pk[16];
+                    uint32_t pk[16], pl[16];
 #pragma unroll
                     for (int g2 = 0; g2 < 2; ++g2) {
                         const float kf = k.key[2 * i + g2], add = k.value[2 * i + g2] - m_sub;
@@ -707,14 +722,14 @@ cache_prompt_kernel(const CachePromptParams p) {
                             unpack2(fma2(pack2(__uint_as_float(u0), __uint_as_float(u1)), k2, a2), e0, e1);
                             e0 = cp_ex2(e0), e1 = cp_ex2(e1);
                             sum = add2(sum, pack2(e0, e1));
-                            const __half2 h2 = __floats2half2_rn(e0, e1);
-                            pk[g2 * 8 + u] = *reinterpret_cast<const uint32_t*>(&h2);
+                            cp_halves(e0, e1, pk[g2 * 8 + u], pl[g2 * 8 + u]);
                         }
                         float s0, s1;
                         unpack2(sum, s0, s1);
                         l_run = fmaf(s0 + s1, k.back[2 * i + g2], l_run);
                     }
                     cp_tmem_st16(s_tmem + i * 16, pk);
+                    cp_tmem_st16(s_tmem + CP_KEYS / 2 + i * 16, pl);
                     if (i == 1) {
                         tmem_wait_st();
                         tc_fence_before();
