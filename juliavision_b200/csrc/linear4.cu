@@ -10,11 +10,12 @@
 // out exactly of one subtraction (or one multiply-add by 1 / 16).  A group's sum is fp32, and so is its product by the scale.
 // Four row tiles lie side by side, unit by unit, so that 64 rows are one stream of 2 KB a k block.
 //
-// Two kernels for few tokens.  A small weight, whose rows do not fill the GPU for long, is a chain of round trips: a block takes 16
+// Two kernels.  A small weight, whose rows do not fill the GPU for long, is a chain of round trips: a block takes 16
 // rows, or 32 for up to 40 tokens at a time (each weight is made into fp16 once for all of them), its warps share K and have all
 // their loads in flight at once (linear4_kernel).  A large one is bandwidth-bound: the list of
 // (64 rows, 8 or 16 tokens, k block) is dealt out to all warps in equal contiguous shares, each streamed by bulk copies through a ring
-// of its own; parts of rows meet at the ends of blocks and in a second launch (linear4_stream_kernel, shares.cuh).
+// of its own; parts of rows meet at the ends of blocks and in a second launch (linear4_stream_kernel, shares.cuh).  Past 512 tokens
+// the weight is laid out as fp16, exactly, for the GEMM (linear4_unpack_kernel).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -27,7 +28,13 @@
 namespace b200 {
 
 constexpr int L4_WARPS = 8;      // of a block, which share K
-constexpr int L4_TOKENS = 96;    // tokens the kernels take; more go through fp16 weights in the workspace (4096 x 4096: 64 tokens 17 us and 24, 128 28 and 24)
+// Tokens the two kernels take; more go through fp16 weights in the workspace, which are made once for all tokens and cost twice the
+// products, since an exact weight is two fp16 numbers.  us, kernels / fp16 weights: 384, 512 and 768 tokens of 4096 x 4096 62 / 78, 79 / 78,
+// 123 / 92; of 28672 x 8192 720 / 785, 951 / 818, 1415 / 1085; of 5120 x 1280 34 / 62, 50 / 51, 70 / 52; 1024 and 2048 of 1280 x 1280 25 / 32, 49 / 54.
+// (Weights rounded to one fp16 number: 512 tokens of 4096 x 4096 32 us, of 28672 x 8192 427; 2.8e-4 of the result off for 2.1e-4.)
+constexpr int L4_TOKENS = 512;
+// What fp16 weights take at a time: past it the next product's rows (28672 x 8192, 600 tokens: blocks of 64 MB 1130 us, of 128 MB 800).
+constexpr int64_t L4_DENSE_BYTES = 128ll << 20, L4_DENSE_TOKENS = 2048;
 constexpr double L4_STREAM_TILES = 4608;   // of 64 rows, 16 tokens and 64 inputs: from here on a list for all warps
 // More than 16 tokens: rounds of loads, times token tiles a block, up to which the blocks that have all of them at once are faster than
 // the list.  us, blocks / list: 24 x 5120 x 1280 6.7 / 10.6, 37 x 5120 x 1280 (15) 8.4 / 10.4, 22 x 3836 x 3456 (21) 9.9 / 11.3,
@@ -418,43 +425,94 @@ linear4_join_kernel(const Linear4Params p, int64_t warps) {
     l4_finish<NT>(p, tgs, q, i / 32 / NT, i / 32 % NT, v, i % 32);
 }
 
-// The weight as dense fp16 (M, K), for many tokens: a block writes 64 rows of two k blocks through shared memory.
+// For many tokens the weights of a block of rows become fp16 in the workspace, exactly: (q - z) s has 16 bits at most and is a whole
+// multiple of 2^-24, so what the nearest fp16 number leaves of it is one too.  Rows 0 .. R - 1 of the dense weight hold the upper parts,
+// rows R .. 2 R - 1 the lower ones, of 64-row units [four0, four0 + R / 64); one GEMM multiplies both and linear4_finish_kernel adds them.
+// (q - z) s may pass fp16's range: a row with a scale above 4096 is stored 2^4 smaller, whole multiples of 2^-20 of the weight, and
+// `shift` says so.
 constexpr int L4_UNPACK_PITCH = 64 + 8;
+constexpr int L4_UNPACK_STEPS = 4;       // of two k blocks, a block: the look at its rows' scales is paid once for them
 __global__ void __launch_bounds__(256)
-linear4_unpack_kernel(const Linear4Params p, __half* out, int64_t ld) {
-    __shared__ __align__(16) __half tile[2][64][L4_UNPACK_PITCH];   // [k block][input][row]
+linear4_unpack_kernel(const Linear4Params p, int64_t four0, __half* out, int64_t R, uint8_t* shift) {
+    __shared__ __align__(16) __half tile[2][2][64][L4_UNPACK_PITCH];   // [upper, lower][k block][input][row]
+    __shared__ uint32_t tops[8][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int mt = blockIdx.x * 4 + (warp & 3), kb = blockIdx.y * 2 + (warp >> 2);
+    const int mt0 = (int)(four0 + blockIdx.x) * 4, mt = mt0 + (warp & 3);
     grid_dep_wait();
     grid_dep_launch();
-    if (mt < p.MT && kb < p.KB) {
-        const uint4 w = __ldg(p.data + p.unit(mt, kb) * 32 + lane);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    uint32_t top = 0;                    // largest magnitudes of a row's and its neighbour's scales, as fp16 bits
+    for (int grp = warp; grp < p.NG; grp += 8) top = __vmaxu2(top, __ldg(p.scales + p.group8(mt0, grp) + lane) & 0x7fff7fffu);
+    tops[warp][lane] = top;
+    __syncthreads();
+    auto most = [&](int word) {          // bits 0 .. 15 of rows g, 16 .. 31 of rows g + 8
+        uint32_t m = 0;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int grp = (kb * 64 + (s >> 1) * 32) >> p.logg;
-            const bool live = grp < p.NG;
-            const uint32_t sc = live ? __ldg(p.scales + p.group8(mt, grp) + g) : 0;
-            uint32_t z0, z1, a[4];
-            l4_zero(live && p.zeros != nullptr ? __ldg(p.zeros + p.group8(mt, grp) + g) : 0x88u, z0, z1);
-            l4_weights(v[s], z0, z1, a);
-            const __half2 s2 = *reinterpret_cast<const __half2*>(&sc);
+        for (int i = 0; i < 8; ++i) m = __vmaxu2(m, tops[i][word]);
+        return m;
+    };
+    constexpr uint32_t LIMIT = 0x6c00;   // 4096: 15 of it are within the range
+    const uint32_t mine = most((warp & 3) * 8 + g);
+    const float f0 = (mine & 0xffffu) > LIMIT ? 0x1p-4f : 1.f, f1 = (mine >> 16) > LIMIT ? 0x1p-4f : 1.f;
+    if (blockIdx.y == 0 && tid < 64) shift[(int64_t)blockIdx.x * 64 + tid] = (most((tid >> 4) * 8 + (tid & 7)) >> (tid & 8 ? 16 : 0) & 0xffffu) > LIMIT ? 4 : 0;
+    for (int step = 0; step < L4_UNPACK_STEPS; ++step) {
+        const int kb0 = (blockIdx.y * L4_UNPACK_STEPS + step) * 2, kb = kb0 + (warp >> 2);
+        if (kb0 >= p.KB) break;
+        if (step > 0) __syncthreads();
+        if (kb < p.KB) {
+            const uint4 w = __ldg(p.data + p.unit(mt, kb) * 32 + lane);
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a[i]), i & 1 ? __high2half2(s2) : __low2half2(s2));
-                const int k = (s >> 1) * 32 + t * 8 + (s & 1) * 4 + (i >> 1) * 2, row = (warp & 3) * 16 + g + (i & 1) * 8;
-                tile[warp >> 2][k][row] = __low2half(r);
-                tile[warp >> 2][k + 1][row] = __high2half(r);
+            for (int s = 0; s < 4; ++s) {
+                const int grp = (kb * 64 + (s >> 1) * 32) >> p.logg;
+                const bool live = grp < p.NG;
+                const uint32_t sc = live ? __ldg(p.scales + p.group8(mt, grp) + g) : 0;
+                uint32_t z0, z1, a[4];
+                l4_zero(live && p.zeros != nullptr ? __ldg(p.zeros + p.group8(mt, grp) + g) : 0x88u, z0, z1);
+                l4_weights(v[s], z0, z1, a);
+                float2 s2 = __half22float2(*reinterpret_cast<const __half2*>(&sc));
+                s2.x *= f0, s2.y *= f1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+                    const float sv = i & 1 ? s2.y : s2.x, w0 = q.x * sv, w1 = q.y * sv;
+                    const __half2 hi = __floats2half2_rn(w0, w1);
+                    const float2 back = __half22float2(hi);
+                    const __half2 lo = __floats2half2_rn(w0 - back.x, w1 - back.y);
+                    const int k = (s >> 1) * 32 + t * 8 + (s & 1) * 4 + (i >> 1) * 2, row = (warp & 3) * 16 + g + (i & 1) * 8;
+                    tile[0][warp >> 2][k][row] = __low2half(hi);
+                    tile[0][warp >> 2][k + 1][row] = __high2half(hi);
+                    tile[1][warp >> 2][k][row] = __low2half(lo);
+                    tile[1][warp >> 2][k + 1][row] = __high2half(lo);
+                }
             }
         }
+        __syncthreads();
+        for (int i = tid; i < 2 * 2 * 64 * 8; i += 256) {
+            const int part = i >> 10, in = i >> 3 & 127, k = kb0 * 64 + in;
+            if (k < p.K)
+                *reinterpret_cast<uint4*>(out + (int64_t)k * 2 * R + part * R + blockIdx.x * 64 + (i & 7) * 8) =
+                    *reinterpret_cast<const uint4*>(&tile[part][in >> 6][in & 63][(i & 7) * 8]);
+        }
     }
-    __syncthreads();
-    const int64_t m0 = (int64_t)blockIdx.x * 64;
-    for (int i = tid; i < 2 * 64 * 8; i += 256) {
-        const int k = blockIdx.y * 128 + i / 8;
-        const int64_t m = m0 + i % 8 * 8;
-        if (k < p.K && m < ld) *reinterpret_cast<uint4*>(out + k * ld + m) = *reinterpret_cast<const uint4*>(&tile[i / 512][i / 8 % 64][i % 8 * 8]);
-    }
+}
+
+// Results of `rows` rows from m0 and `tokens` tokens from n0: both parts' sums, brought back to scale.
+constexpr int L4_FINISH_TOKENS = 8;      // a thread
+__global__ void __launch_bounds__(128)
+linear4_finish_kernel(const Linear4Params p, const float* __restrict__ y, int64_t R, const uint8_t* __restrict__ shift, int64_t m0, int rows, int n0, int tokens) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int r = blockIdx.x * 128 + threadIdx.x, at = blockIdx.y * L4_FINISH_TOKENS;
+    if (r >= rows) return;
+    const float f = shift[r] ? 16.f : 1.f;
+    float v[L4_FINISH_TOKENS][2];
+#pragma unroll
+    for (int i = 0; i < L4_FINISH_TOKENS; ++i)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) v[i][part] = at + i < tokens ? y[(at + i) * 2 * R + part * R + r] : 0.f;
+#pragma unroll
+    for (int i = 0; i < L4_FINISH_TOKENS; ++i)
+        if (at + i < tokens) l4_store(p, m0 + r, n0 + at + i, (v[i][0] + v[i][1]) * f);
 }
 
 struct PackParams {
@@ -532,6 +590,40 @@ static int l4_stream_launch(b200_ctx* ctx, Linear4Params& p) {
     return B200_OK;
 }
 
+// Many tokens: the weight as fp16, a block of rows at a time, and the GEMM.
+static int l4_dense(b200_ctx* ctx, const b200_q4* A, const Linear4Params& p, const void* B, int64_t ldb) {
+    const int64_t K = A->K, units = cdiv(A->M, 64), parts = cdiv(p.KB, 2 * L4_UNPACK_STEPS);
+    B200_REQUIRE(parts < 65536, B200_DECLINE_EXTENT, "matmul_q4: K=%lld", (long long)K);
+    int64_t block = L4_DENSE_BYTES / (4 * 64 * K);         // units of 64 rows, two parts of two bytes
+    if (block < 4) block = 4;
+    block = cdiv(units, cdiv(units, block));               // blocks of like sizes
+    const int64_t R = block * 64, most = p.N < L4_DENSE_TOKENS ? p.N : L4_DENSE_TOKENS;
+    void* ws = nullptr;
+    int rc = ws_scratch(ctx, (size_t)R * (4 * K + 8 * most + 1), &ws);
+    if (rc) return rc;
+    __half* w = static_cast<__half*>(ws);
+    float* y = reinterpret_cast<float*>(w + 2 * R * K);
+    uint8_t* shift = reinterpret_cast<uint8_t*>(y + 2 * R * most);
+    const size_t mark = ctx->ws_used;
+    for (int64_t n0 = 0; n0 < p.N; n0 += most) {
+        const int64_t tokens = p.N - n0 < most ? p.N - n0 : most;
+        for (int64_t u0 = 0; u0 < units; u0 += block) {
+            const int64_t have = units - u0 < block ? units - u0 : block, r = have * 64, rows = A->M - u0 * 64 < r ? A->M - u0 * 64 : r;
+            if (n0 == 0 || block < units) {
+                B200_CUDA(launch_dep(linear4_unpack_kernel, dim3((unsigned)have, (unsigned)parts), dim3(256), 0, ctx->stream, 1, p, u0, w, r, shift));
+                ctx->launches++;
+            }
+            rc = gemm_f16_run(ctx, 2 * r, tokens, K, w, 2 * r, (const __half*)B + n0 * ldb, ldb, nullptr, 0, y, 2 * r, B200_F32, B200_EPI_NONE, 1, 0, 0, 0);
+            if (rc) return rc;
+            ctx->ws_used = mark;                           // what the GEMM took; the next one runs behind it
+            B200_CUDA(launch_dep(linear4_finish_kernel, dim3((unsigned)cdiv(rows, 128), (unsigned)cdiv(tokens, L4_FINISH_TOKENS)), dim3(128), 0, ctx->stream, 1,
+                                 p, (const float*)y, r, (const uint8_t*)shift, u0 * 64, (int)rows, (int)n0, (int)tokens));
+            ctx->launches++;
+        }
+    }
+    return B200_OK;
+}
+
 static int l4_shape(const char* op, int64_t M, int64_t K, int64_t group) {
     B200_REQUIRE(M >= 1 && K >= 1 && M < (1ll << 31) - 64 && K < (1ll << 31) - 128, B200_DECLINE_EXTENT, "%s: M=%lld K=%lld", op, (long long)M, (long long)K);
     B200_REQUIRE(group == 32 || group == 64 || group == 128, B200_DECLINE_EXTENT, "%s: groups of %lld (32, 64 or 128)", op, (long long)group);
@@ -596,17 +688,7 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
     p.logg = A->group == 32 ? 5 : A->group == 64 ? 6 : 7;
     p.out_f32 = out_dtype == B200_F32, p.epi = epilogue;
     p.whole = (uintptr_t)B % 16 == 0 && ldb % 8 == 0;
-    if (N > L4_TOKENS) {
-        const int64_t ld = cdiv(A->M, 8) * 8;
-        void* w = nullptr;
-        rc = ws_scratch(ctx, (size_t)ld * A->K * 2, &w);
-        if (rc) return rc;
-        B200_REQUIRE(cdiv(p.KB, 2) < 65536, B200_DECLINE_EXTENT, "matmul_q4: K=%lld", (long long)A->K);
-        B200_CUDA(launch_dep(linear4_unpack_kernel, dim3((unsigned)cdiv(p.MT, 4), (unsigned)cdiv(p.KB, 2)), dim3(256), 0, ctx->stream, 1, p,
-                             (__half*)w, ld));
-        ctx->launches++;
-        return gemm_f16_run(ctx, A->M, N, A->K, w, ld, B, ldb, bias, 0, out, ldo, out_dtype, epilogue, 1, 0, 0, 0);
-    }
+    if (N > L4_TOKENS) return l4_dense(ctx, A, p, B, ldb);
     p.d_status = ctx->d_status;
     const int nt = N <= 8 ? 1 : 2;
     // More than 16 tokens: up to 40 to a block of linear4_kernel, whose warps take a round trip of loads a k block.

@@ -1,9 +1,8 @@
 """What a decoder's operators keep where fewer bits would go unnoticed beside a rounding to fp16: fp32 results, against fp64."""
-import math
-
 import numpy as np
 import pytest
 
+import juliavision_b200 as jv
 from tests import decode_ref as ref
 from tests.test_gpu_decode import F32, Cached, STEP, attend, near
 
@@ -36,3 +35,76 @@ def test_weights_keep_their_bits(ctx, E, G, L, kind):
     scale = 0.6 / E
     got, _, _ = attend(ctx, c, q, None, scale, True, F32)
     bound(c, q, scale, True, got)
+
+
+# ------------------------------------------------------------------------------------------------- 4-bit products
+def product(ctx, rng, N, M, K, group, zeros, scales, size, pad=0, epi="identity"):
+    """A product as fp32, the wanted one and the sum of magnitudes."""
+    q = rng.integers(0, 16, (K, M)).astype(np.uint8)
+    s = scales((K // group, M)).astype(np.float16)
+    z = rng.integers(0, 16, (K // group, M)).astype(np.uint8) if zeros else None
+    x = (rng.standard_normal((N, K + pad)) * size).astype(np.float16)
+    w = jv.pack4(ctx, ctx.toback(q), ctx.toback(s), None if z is None else ctx.toback(z), group)
+    d, buf = ctx.toback(x), ctx.allocate(F32, M + 1, N + 1)
+    ctx.fill_bytes(buf, 0xFF)
+    ctx.ws.reset()
+    jv.matmul4_(ctx, jv.DeviceArray(ctx, buf.ptr, F32, (M, N), (1, M + 1), owner=buf), w, jv.DeviceArray(ctx, d.ptr, np.float16, (K, N), (1, K + pad), owner=d),
+                epi=epi)
+    ctx.synchronize()
+    got = buf.to_host()
+    assert np.isnan(got[N:]).all() and np.isnan(got[:, M:]).all()
+    x, w = x[:, :K].astype(np.float64), ref.weight4(q, s, z, group)
+    return got[:N, :M], x @ w, np.abs(x) @ np.abs(w)
+
+
+def sums(K):
+    """fp32 sums of fp16 products, in steps of sixteen at least: each off by 2^-23 of what it adds up, which is the sum of magnitudes at most;
+    and a few more where parts meet."""
+    return 2.0 ** -23 * (K / 16 + 8)
+
+
+@pytest.mark.parametrize("N", [96, 97, 300, 513, 600])
+@pytest.mark.parametrize("M, K, group, zeros, pad", [(200, 512, 64, False, 0), (333, 480, 32, True, 0), (64, 256, 128, True, 1)])
+def test_weights_are_exact_for_any_number_of_tokens(ctx, M, K, group, zeros, pad, N):
+    rng = np.random.default_rng(22)
+    got, want, reach = product(ctx, rng, N, M, K, group, zeros, lambda n: rng.random(n) * 0.02 + 0.001, 1.0, pad)
+    near(got, want, reach * sums(K) + STEP[F32][0] * np.abs(want))
+
+
+@pytest.mark.parametrize("N", [1, 16, 40, 96, 97, 300, 513])
+def test_weights_past_the_range_of_fp16(ctx, N):
+    """Scales up to fp16's largest beside ones of 2^-24 and negative ones: (q - z) s is a number for any number of tokens.  In a row with a scale above 4096
+    it may be held to 2^-20, off by 2^-21, which is nothing beside what stands at that scale."""
+    rng = np.random.default_rng(23)
+    M, K, group = 130, 256, 32
+
+    def scales(n):
+        s = 2.0 ** rng.uniform(-24, 15.9, n) * rng.choice([-1, 1], n)
+        s[:, ::3] = np.minimum(np.abs(s[:, ::3]), 2.0)
+        return s
+
+    got, want, reach = product(ctx, rng, N, M, K, group, True, scales, 2.0 ** -6)
+    assert np.isfinite(got).all() and np.abs(want).max() > 2.0 ** 13
+    near(got, want, reach * sums(K) + STEP[F32][0] * np.abs(want) + 2.0 ** -21 * K * 2.0 ** -6 * 5 * (reach > 256))
+
+
+def test_many_tokens_through_blocks_of_rows(ctx):
+    """More rows than are laid out at a time, the last block of them a part, more tokens than a product takes at a time; every result against a column and
+    a row that are summed exactly."""
+    rng = np.random.default_rng(24)
+    N, M, K, group = 2100, 9000, 4096, 128
+    q, s = rng.integers(0, 16, (K, M)).astype(np.uint8), (rng.random((K // group, M)) * 0.02 + 0.001).astype(np.float16)
+    x, bias = rng.standard_normal((N, K)).astype(np.float16), rng.standard_normal(M).astype(np.float16)
+    w = jv.pack4(ctx, ctx.toback(q), ctx.toback(s), None, group)
+    out = ctx.allocate(np.float16, M, N)
+    ctx.fill_bytes(out, 0xFF)
+    ctx.ws.reset()
+    jv.matmul4_(ctx, out, w, ctx.toback(x), ctx.toback(bias), epi="relu")
+    got = out.to_host().astype(np.float64)
+    assert np.isfinite(got).all()
+    rows, tokens = np.r_[0:M:61, M - 1], np.r_[0:N:37, N - 1]
+    for m, n in ((rows, slice(None)), (slice(None), tokens)):
+        wm, xn = ref.weight4(q[:, m], s[:, m], None, group), x[n].astype(np.float64)
+        want, reach = xn @ wm + bias[m].astype(np.float64), np.abs(xn) @ np.abs(wm)
+        tol = reach * sums(K) + STEP[np.float16][0] * np.abs(want) + STEP[np.float16][1]
+        near(got[n][:, m] if isinstance(n, slice) else got[n], np.maximum(want, 0), tol)
