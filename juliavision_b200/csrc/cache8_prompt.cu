@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
 // cache8_attention.cu.
 //
-// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 207 us, 0.75 PFLOP/s.
+// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 208 us, 0.74 PFLOP/s.
 // What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 4600 clocks a block
 // of 128 keys for two tiles whose products take 3072), which the other tile's covers in part.
 //
@@ -74,7 +74,7 @@ __device__ __forceinline__ void cp_tmem_st16(uint32_t taddr, const uint32_t* r) 
     tmem_st16(taddr, v);
 }
 // Two weights as two halves each: what fp16 holds of them, cut off, and what is left, rounded; off by 2^-21 of themselves, or, below
-// 2^-14, by a step of 2^-24.  (One half alone: 163 us for 207 at 2048 tokens over 10240, and 2.9e-4 of the result for 2.1e-4.  The upper
+// 2^-14, by a step of 2^-24.  (One half alone: 163 us for 208 at 2048 tokens over 10240, and 2.9e-4 of the result for 2.1e-4.  The upper
 // ones rounded to nearest and converted back 217; the lower ones made after the exponentials' turn has passed, beside the upper ones'
 // product, 216.)
 __device__ __forceinline__ void cp_halves(float a, float b, uint32_t& upper, uint32_t& lower) {
@@ -334,12 +334,16 @@ cache_prompt_kernel(const CachePromptParams p) {
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     CpPart* part = reinterpret_cast<CpPart*>(smem + Cfg::S_PART);
+    // A warp leaves a wait that runs out as one: lanes that went on alone would wait for the others in the next vote, for good.
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, c.d_status, code, abort_flag));
+    };
     // The next part of the block's share; barriers go on over all of them.
     CpItem it;
     int item = 0, j_begin = 0, nblk = 0, parts_seen = 0;
     auto next = [&]() -> bool {
         const int s = parts_seen % CP_PARTS;
-        if (!__all_sync(0xffffffffu, mbar_wait(&a_full[s], (uint32_t)((parts_seen / CP_PARTS) & 1), c.d_status, KST_WAIT_FULL, abort_flag))) return false;
+        if (!wait(&a_full[s], (uint32_t)((parts_seen / CP_PARTS) & 1), KST_WAIT_FULL)) return false;
         CpPart x = part[s];
         // the same for all lanes, which the compiler sees: what depends on them stays in the warp's own registers
         for (int* v : {&x.it.b, &x.it.h, &x.it.r0, &x.it.rows, &x.it.n, &x.it.m, &x.it.blocks, &x.item, &x.j0, &x.nblk, &x.more})
@@ -374,7 +378,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                     float k1, v1;
                     load(pg1, k1, v1);
                     const int s = done % CP_SCALES;
-                    if (!mbar_wait(&c_empty[s], (uint32_t)((done / CP_SCALES) & 1) ^ 1, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
+                    if (!wait(&c_empty[s], (uint32_t)((done / CP_SCALES) & 1) ^ 1, KST_WAIT_EMPTY)) { ok = false; break; }
                     ++done;
                     float most = v0 < INFINITY ? v0 : 0.f;
 #pragma unroll
@@ -411,7 +415,7 @@ cache_prompt_kernel(const CachePromptParams p) {
             CpPart x;
             do {
                 x.more = mine.next(p, x.it, x.item, x.j0, x.nblk);
-                if (!mbar_wait(&a_empty[s % CP_PARTS], (uint32_t)((s / CP_PARTS) & 1) ^ 1, c.d_status, KST_WAIT_EMPTY, abort_flag)) break;
+                if (!wait(&a_empty[s % CP_PARTS], (uint32_t)((s / CP_PARTS) & 1) ^ 1, KST_WAIT_EMPTY)) break;
                 if (lane == 0) {
                     part[s % CP_PARTS] = x;
                     mbar_arrive(&a_full[s % CP_PARTS]);
@@ -434,9 +438,6 @@ cache_prompt_kernel(const CachePromptParams p) {
             constexpr uint64_t vdesc0 = make_smem_desc(CP_ATOM, 1024);
             const uint32_t q_addr = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE);
             const uint32_t s_tmem = tmem_base + t * CP_KEYS, o_tmem = tmem_base + Cfg::O_COL + t * EP;
-            auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-                return __all_sync(0xffffffffu, mbar_wait(bar, parity, c.d_status, code, abort_flag));
-            };
             int done = 0, busy = 0, parts = 0;      // blocks of the share, of this tile, parts of this tile, before this part
             auto issue_qk = [&](int j) -> bool {
                 const int i = done + j, sk = i % STAGES;
@@ -579,7 +580,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                     fetch(nxt, j + side, side ^ 1);
                     if (side == 0) look(j + 1);      // what is fetched next is of the next block
                     uint64_t *empty = side ? v_empty : k_empty, *full = side ? v_full : k_full;
-                    if (!mbar_wait(&empty[s], ph, c.d_status, KST_WAIT_EMPTY, abort_flag)) { ok = false; break; }
+                    if (!wait(&empty[s], ph, KST_WAIT_EMPTY)) { ok = false; break; }
                     write(smem_u32(smem + Cfg::S_K + (side * STAGES + s) * Cfg::SIDE), __half2half2(__ushort_as_half(side ? 0x5f00 : 0x7fff)));
                     if (lane == 0) mbar_arrive(&full[s]);
 #pragma unroll
@@ -600,7 +601,7 @@ cache_prompt_kernel(const CachePromptParams p) {
             if (it.r0 + t * CP_ROWS >= it.rows) {
                 for (int j = 0; ok && j < nblk; ++j, ++done) {
                     const int cs = done % CP_SCALES;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&c_full[cs], (uint32_t)((done / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag));
+                    ok = wait(&c_full[cs], (uint32_t)((done / CP_SCALES) & 1), KST_WAIT_FULL);
                     if (ok && lane == 0) mbar_arrive(&c_empty[cs]);
                 }
                 continue;
@@ -641,10 +642,10 @@ cache_prompt_kernel(const CachePromptParams p) {
             const bool pingpong = it.r0 + CP_ROWS < it.rows;
             for (int j = 0; ok && j < nblk; ++j, ++done, ++busy) {
                 const int cs = done % CP_SCALES, key0 = (j_begin + j) * CP_KEYS;
-                if (!mbar_wait(&c_full[cs], (uint32_t)((done / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag)) { ok = false; break; }
                 const CpScales& k = consts[cs];
-                if (!mbar_wait(&s_full[t], (uint32_t)(busy & 1), c.d_status, KST_WAIT_TMEM_FULL, abort_flag)) { ok = false; break; }
-                __syncwarp();
+                ok = __all_sync(0xffffffffu, mbar_wait(&c_full[cs], (uint32_t)((done / CP_SCALES) & 1), c.d_status, KST_WAIT_FULL, abort_flag) &&
+                                             mbar_wait(&s_full[t], (uint32_t)(busy & 1), c.d_status, KST_WAIT_TMEM_FULL, abort_flag));
+                if (!ok) break;
                 tc_fence_after();
                 uint32_t x[4][32];
 #pragma unroll
@@ -705,8 +706,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                     m_run = m_new;
                 }
                 if (pingpong && (t == 1 || turns > 0) &&
-                    !mbar_wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag)) { ok = false; break; }
-                __syncwarp();
+                    !wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), KST_WAIT_SOFTMAX)) { ok = false; break; }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t pk[16], pl[16];
@@ -751,7 +751,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                     mbar_arrive(&c_empty[cs]);
                 }
             }
-            if (ok && nblk > 0) ok = mbar_wait(&pv_done[t], (uint32_t)((busy - 1) & 1), c.d_status, KST_WAIT_SOFTMAX, abort_flag);
+            if (ok && nblk > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);
             __syncwarp();
             if (ok) {
                 tc_fence_after();
