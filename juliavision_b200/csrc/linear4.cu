@@ -332,7 +332,8 @@ linear4_stream_kernel(const __grid_constant__ CUtensorMap tmapX, const Linear4Pa
             for (int i = 0; i < 4; ++i) __nanosleep(1000000);   // copies may still land
             break;
         }
-        fetch();                  // this stage is there for every lane, and the one that is asked for now has been read
+        __syncwarp();             // every lane has read the stage that is asked for now; a vote alone orders no memory
+        fetch();
         const uint8_t* st = ring + s * Cfg::STAGE;
         const uint8_t* xs = xring + s * Cfg::X_STAGE + g * 128;
         if (++s == L4_STAGES) s = 0, phase ^= 1;

@@ -29,3 +29,12 @@ def test_a_warp_leaves_a_wait_as_one(name):
         found += len(re.findall(WAIT, text[at:end]))
         text = text[:at] + text[end:]
     assert found and not re.findall(WAIT, text)
+
+
+def test_a_stage_is_asked_for_behind_the_reads_of_it():
+    """The bulk copies into a stage that a warp has just read are asked for behind a barrier of the warp, which orders its lanes' reads;
+    the vote on a wait orders none."""
+    text = source("linear4.cu")
+    loop = text[text.index("for (int at = 0; at < tiles; ++at)"):]
+    loop = loop[:loop.index("fetch();")]
+    assert loop.rstrip().endswith("__syncwarp();")
