@@ -8,10 +8,11 @@
 // are keys, then elements, and whose 8 columns are query rows: every converted register pair serves a full tile, where tiles
 // of 16 query rows would be half empty for a group of four or eight heads.  P^T reaches its operand layout by movmatrix.
 //
-// A page's scales never touch the operands: the key scale multiplies the fp32 scores of its page, the value scale goes onto P,
-// relative to the largest one so far, whose change is one more factor of the running rescale.  That rescale waits until a
-// score is 2^8 past its row's reference point; P goes in times 2^7, so that it stays in range, as two fp16 halves (the rounded
-// weight and what that lost): 22 bits of weight for half as many more products, which hide behind the conversions (an error of
+// A page's scales never touch the operands: the key scale multiplies the fp32 scores of its page, the value scale goes onto P, its
+// power of two as a summand of the exponents, the rest as a factor.  A row's reference point is its largest exponent with that
+// summand: P has its bits where weight times scale is largest, whatever pages hold that the row does not see or gives no weight.  The
+// rescale waits until an exponent is 7 past the reference point; P goes in times 2^7, so that it stays below 2^15, as two fp16
+// halves (the rounded weight and what that lost): 22 bits of weight for half as many more products, which hide behind the conversions (an error of
 // 2.1e-4 of the result's scale against 2.9e-4 with the upper half alone; 32 x 8192 tokens 65 us with both and 64 with one).
 //
 // The work is one list of 64-key tiles over all (sequence, key head, row tile): pieces.  It is computed from the lengths on the
@@ -336,12 +337,12 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
         }
     };
     auto store = [&](const CfPiece& q, int row, int e4, float4 v) { cf_store(p, RT, q.b, q.h, q.rt, row, e4, v); };
-    float o[NT][W / 2][4], mref[NT][2], vref = 0.f, vinv = 0.f;     // mref: rows' reference points; vref: the value scale P is relative to
+    float o[NT][W / 2][4], mref[NT][2];                             // mref: rows' reference points
     uint64_t lsum[NT];
     const int e0 = W * (EP == 128 ? cf_chunk(g) : g);               // this lane's W elements of its rows
     // This warp's rows of piece q: `put` gets (row, element, four values times f(row's sum)) and `ends` (row, reference point, sum).
     auto results = [&](const CfPiece& q, auto factor, auto put, auto ends) {
-        const float back = vref * (1.f / 128.f) / cache_top<FP8>();
+        const float back = 1.f / cache_top<FP8>();
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             float l[2];
@@ -387,7 +388,6 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
 #pragma unroll
             for (int k = 0; k < 2; ++k) last[i][k] = p.causal ? n - m + (rt * RT + i * 8 + 2 * t + k) / p.G : n - 1;
         const int all_see = p.causal ? n - m + rt * RT / p.G : n - 1;   // that every row may see
-        vref = vinv = 0.f;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -436,9 +436,17 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 scales();
                 if (last_one) queries(nx);
             }
-            const float vmost = cf_max3(fmaxf(vs[0], vs[1]), vs[2], vs[3]);
+            // A value scale as 2^vk times vm, exactly, and 2^-vk, which takes a weight back for the row's sum.  2^-80 stands for less and for
+            // 0, whose weights count but whose vm is 0: fp32 holds them beside fp16's largest down to 2^-30 of the row's largest weight.
+            float vk[NG], vm[NG], vb[NG];
+#pragma unroll
+            for (int grp = 0; grp < NG; ++grp) {
+                const int e = min(max((__float_as_int(vs[grp]) >> 23) - 127, -80), 126);
+                vk[grp] = (float)e;
+                vb[grp] = __int_as_float((127 - e) << 23);
+                vm[grp] = vs[grp] * vb[grp];
+            }
             const bool plain = key0 + CF_KEYS - 1 <= all_see && fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3])) >= 0.f;   // every row sees all of these
-            // a value scale that is not finite is nobody's reference; the sum finds it
             const bool odd = !(vs[0] + vs[1] + vs[2] + vs[3] < INFINITY);
             bool grown = false;
             float top[NT][2];
@@ -449,8 +457,8 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                 for (int grp = 0; grp < NG; ++grp) {
                     const float ksl = ks[grp] * p.scale_log2;
                     float* x = s[i][grp];
-                    unpack2(mul2(pack2(x[0], x[1]), pack2(ksl, ksl)), x[0], x[1]);
-                    unpack2(mul2(pack2(x[2], x[3]), pack2(ksl, ksl)), x[2], x[3]);
+                    unpack2(fma2(pack2(x[0], x[1]), pack2(ksl, ksl), pack2(vk[grp], vk[grp])), x[0], x[1]);
+                    unpack2(fma2(pack2(x[2], x[3]), pack2(ksl, ksl), pack2(vk[grp], vk[grp])), x[2], x[3]);
                     if (!plain) {
                         const int k0 = key0 + grp * 16 + cf_key<EP>(0, g), k1 = key0 + grp * 16 + cf_key<EP>(1, g);
                         const bool hidden = ks[grp] < 0.f;
@@ -462,14 +470,9 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                     top[i][0] = cf_max3(top[i][0], x[0], x[2]);
                     top[i][1] = cf_max3(top[i][1], x[1], x[3]);
                 }
-                grown = grown || top[i][0] > mref[i][0] + 8.f || top[i][1] > mref[i][1] + 8.f;
+                grown = grown || top[i][0] > mref[i][0] + 7.f || top[i][1] > mref[i][1] + 7.f;
             }
-            if (__any_sync(0xffffffffu, grown) || (odd ? true : vmost > vref)) {
-                float vnew = vref;
-#pragma unroll
-                for (int grp = 0; grp < NG; ++grp)
-                    if (vs[grp] < INFINITY && vs[grp] > vnew) vnew = 1.5f * vs[grp];
-                const float f = vnew == vref ? 1.f : vref / vnew;
+            if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -488,29 +491,27 @@ cache_attention_kernel(const __grid_constant__ CUtensorMap tmapK, const __grid_c
                         lsum[i] = pack2(l0, l1);
 #pragma unroll
                         for (int u = 0; u < W / 2; ++u) {
-                            o[i][u][k] *= a * f;
-                            o[i][u][2 + k] *= a * f;
+                            o[i][u][k] *= a;
+                            o[i][u][2 + k] *= a;
                         }
                     }
-                vref = vnew;
-                vinv = vref > 0x1p-100f ? 128.f / vref : 0.f;   // 0 while there are only pages of zeros
             }
             uint32_t pb[NT][NG][2], pl[NT][NG][2];   // the weights' upper and lower halves
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const uint64_t nm = pack2(mref[i][0] == -INFINITY ? 0.f : -mref[i][0], mref[i][1] == -INFINITY ? 0.f : -mref[i][1]);
+                const uint64_t nm = pack2(mref[i][0] == -INFINITY ? 0.f : 7.f - mref[i][0], mref[i][1] == -INFINITY ? 0.f : 7.f - mref[i][1]);
 #pragma unroll
                 for (int grp = 0; grp < NG; ++grp) {
-                    const float f = vs[grp] * vinv;
+                    const uint64_t f = pack2(vm[grp], vm[grp]), b2 = pack2(vb[grp], vb[grp]);
                     const float* x = s[i][grp];
                     float e[4];
                     unpack2(add2(pack2(x[0], x[1]), nm), e[0], e[1]);
                     unpack2(add2(pack2(x[2], x[3]), nm), e[2], e[3]);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) e[k] = cf_ex2(e[k]);
-                    lsum[i] = add2(lsum[i], add2(pack2(e[0], e[1]), pack2(e[2], e[3])));
-                    unpack2(mul2(pack2(e[0], e[1]), pack2(f, f)), e[0], e[1]);
-                    unpack2(mul2(pack2(e[2], e[3]), pack2(f, f)), e[2], e[3]);
+                    lsum[i] = fma2(add2(pack2(e[0], e[1]), pack2(e[2], e[3])), b2, lsum[i]);
+                    unpack2(mul2(pack2(e[0], e[1]), f), e[0], e[1]);
+                    unpack2(mul2(pack2(e[2], e[3]), f), e[2], e[3]);
                     if (odd) {   // 0 times what is not finite is no number: a hidden key has no part
 #pragma unroll
                         for (int k = 0; k < 4; ++k)

@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
 // cache8_attention.cu.
 //
-// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 208 us, 0.74 PFLOP/s.
+// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 213 us, 0.73 PFLOP/s.
 // What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 4600 clocks a block
 // of 128 keys for two tiles whose products take 3072), which the other tile's covers in part.
 //
@@ -9,8 +9,8 @@
 // and walks their keys in blocks of 128: S = Q K^T and O += P V on tcgen05 with S, P (two fp16 halves, 21 bits and more of a
 // weight, as for few rows) and O in tensor memory.  The 8-bit operands become fp16 on the way to shared memory, exactly, once for 256 rows: four warps
 // read them from the pages into registers a side ahead and write them in the 128-byte swizzle.  No operand carries a scale: a
-// page's key scale (and the softmax's own) is the factor of its columns' exponents, its value scale, relative to the largest so
-// far, a summand of them; the row sum takes that back a group of 16 keys at a time.
+// page's key scale (and the softmax's own) is the factor of its columns' exponents, its value scale a summand of them; the row sum
+// takes that back a group of 16 keys at a time.  A row's reference point is its largest exponent with that summand (cache8_attention.cu).
 //
 //   warps 0-3  softmax of tile 0, warps 4-7 of tile 1: one thread a row, the row's 128 scores in registers
 //   warps 8-11 fetch and convert: K(j), V(j), K(j+1), ...
@@ -33,11 +33,9 @@ constexpr int CP_SCALES = 4;                    // blocks of constants in flight
 constexpr int CP_SOFTMAX_REGS = 176, CP_CONVERT_REGS = 104, CP_OTHER_REGS = 56;
 static_assert(2 * 128 * CP_SOFTMAX_REGS + 128 * CP_CONVERT_REGS + 128 * CP_OTHER_REGS <= CP_THREADS * 128, "what the launch holds");
 
-struct CpScales {              // of one block of keys, a group of 16 keys an entry
-    float key[8];              // score to exponent: finite and above 0, so that a hidden score of -inf stays that
-    float value[8];            // added to the exponent: log2 of 2^7 times the value scale over the reference
+struct __align__(16) CpScales {              // of one block of keys, a group of 16 keys an entry
+    float2 score[8];           // score to exponent: a factor, finite and above 0, so that a hidden score of -inf stays that; log2 of the value scale
     float back[8];             // an exponential of the group back to a weight
-    float change, reference;   // the reference before over the reference now; the reference
     int hidden, odd;           // bit g: the group has no page; one of its scales is not finite
 };
 
@@ -361,7 +359,6 @@ cache_prompt_kernel(const CachePromptParams p) {
             int done = 0;
             bool ok = true;
             while (ok && next()) {
-                float ref = 0.f;
                 auto page = [&](int j) {
                     const int key = (j_begin + j) * CP_KEYS + (lane & 7) * 16;
                     return j < nblk && key < it.n ? (int)c.page(it.b, key >> c.logT) : -1;
@@ -380,25 +377,16 @@ cache_prompt_kernel(const CachePromptParams p) {
                     const int s = done % CP_SCALES;
                     if (!wait(&c_empty[s], (uint32_t)((done / CP_SCALES) & 1) ^ 1, KST_WAIT_EMPTY)) { ok = false; break; }
                     ++done;
-                    float most = v0 < INFINITY ? v0 : 0.f;
-#pragma unroll
-                    for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                    const float was = ref;
-                    if (most > ref) ref = 1.5f * most;
-                    // a scale far below the reference, whose P is zero in fp16, keeps an exponent of its own so that the sum can take it back
-                    float f = ref > 0x1p-100f ? v0 / ref : 1.f;
-                    if (f < 0x1p-40f) f = 0x1p-40f;
+                    const float f = fmaxf(v0, 0x1p-80f);      // of a page of zeros, whose weights count: as for few rows
                     const float kf = k0 * p.scale_log2;
                     const bool strange = !(kf < INFINITY) || !(v0 < INFINITY);
                     const unsigned hidden = __ballot_sync(0xffffffffu, pg < 0) & 255u, odd = __ballot_sync(0xffffffffu, strange) & 255u;
                     if (lane < 8) {
-                        consts[s].key[lane] = strange ? 1.f : fmaxf(kf, 0x1p-100f);   // a page of zeros: its scores are zeros whatever the factor
-                        consts[s].value[lane] = strange ? 7.f : log2f(f) + 7.f;
-                        consts[s].back[lane] = strange ? 0x1p-7f : 0x1p-7f / f;
+                        // a page of zeros: its scores are zeros whatever the factor
+                        consts[s].score[lane] = make_float2(strange ? 1.f : fmaxf(kf, 0x1p-100f), strange ? 0.f : log2f(f));
+                        consts[s].back[lane] = strange ? 1.f : 1.f / f;
                     }
                     if (lane == 0) {
-                        consts[s].change = was == ref ? 1.f : was / ref;
-                        consts[s].reference = ref;
                         consts[s].hidden = (int)hidden;
                         consts[s].odd = (int)odd;
                     }
@@ -638,7 +626,7 @@ cache_prompt_kernel(const CachePromptParams p) {
             }
             const int last = p.causal ? it.n - it.m + l : it.n - 1;                       // the last key this row sees
             const int all_see = p.causal ? it.n - it.m + (it.r0 + t * CP_ROWS) / p.G : it.n - 1;   // that every row of the tile sees
-            float m_run = -INFINITY, l_run = 0.f, ref = 0.f;
+            float m_run = -INFINITY, l_run = 0.f;
             const bool pingpong = it.r0 + CP_ROWS < it.rows;
             for (int j = 0; ok && j < nblk; ++j, ++done, ++busy) {
                 const int cs = done % CP_SCALES, key0 = (j_begin + j) * CP_KEYS;
@@ -682,23 +670,21 @@ cache_prompt_kernel(const CachePromptParams p) {
                         a = cp_max3(a, __uint_as_float(y[u]), __uint_as_float(y[u + 1]));
                         if (u + 2 < 16) b2 = cp_max3(b2, __uint_as_float(y[u + 2]), __uint_as_float(y[u + 3]));
                     }
-                    top = fmaxf(top, fmaxf(a, b2) * k.key[gq]);
+                    top = fmaxf(top, fmaf(fmaxf(a, b2), k.score[gq].x, k.score[gq].y));
                 }
-                // the reference point follows lazily: only when the maximum has grown by more than 2^8
-                const float m_new = top > m_run + 8.f ? top : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new;
-                const float change = k.change;
-                if (__any_sync(0xffffffffu, m_new != m_run) || change != 1.f) {
+                // the reference point follows lazily: only when the maximum has grown by more than 2^8; P goes in times 2^7
+                const float m_new = top > m_run + 8.f ? top : m_run, m_sub = m_new == -INFINITY ? 0.f : m_new - 7.f;
+                if (__any_sync(0xffffffffu, m_new != m_run)) {
                     const float alpha = m_run == m_new ? 1.f : cp_ex2(m_run - m_new);
                     l_run *= alpha;
                     if (j > 0) {          // these scores were issued after the last P V: it is done
-                        const float f = alpha * change;
 #pragma unroll 1
                         for (int i = 0; i < EP / 16; ++i) {
                             uint32_t o16[16];
                             tmem_ld16(o_tmem + i * 16, o16);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int u = 0; u < 16; ++u) o16[u] = __float_as_uint(__uint_as_float(o16[u]) * f);
+                            for (int u = 0; u < 16; ++u) o16[u] = __float_as_uint(__uint_as_float(o16[u]) * alpha);
                             tmem_st16(o_tmem + i * 16, o16);
                         }
                         tmem_wait_st();
@@ -712,7 +698,7 @@ cache_prompt_kernel(const CachePromptParams p) {
                     uint32_t pk[16], pl[16];
 #pragma unroll
                     for (int g2 = 0; g2 < 2; ++g2) {
-                        const float kf = k.key[2 * i + g2], add = k.value[2 * i + g2] - m_sub;
+                        const float kf = k.score[2 * i + g2].x, add = k.score[2 * i + g2].y - m_sub;
                         const uint64_t k2 = pack2(kf, kf), a2 = pack2(add, add);
                         uint64_t sum = pack2(0.f, 0.f);
 #pragma unroll
@@ -742,7 +728,6 @@ cache_prompt_kernel(const CachePromptParams p) {
                     if (lane == 0) mbar_arrive(&exp_turn[1 - t]);
                     ++turns;
                 }
-                ref = k.reference;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -755,7 +740,7 @@ cache_prompt_kernel(const CachePromptParams p) {
             __syncwarp();
             if (ok) {
                 tc_fence_after();
-                const float back = ref * 0x1p-7f / cache_top<FP8>();
+                const float back = 1.f / cache_top<FP8>();
                 const bool whole = j_begin == 0 && nblk == it.blocks;
                 const float f = !whole ? back : back / (l_run == 0.f ? 1.f : l_run);
                 const int64_t at = l * p.oL + hq * p.oH + it.b * p.oB;

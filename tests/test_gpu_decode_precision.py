@@ -15,13 +15,18 @@ def bound(c, q, scale, causal, got):
     product of a weight and its page's scale is.  A score's fp32 sum, off by 2^-20 of the sum of magnitudes at most, moves a weight
     and the row's sum; exponential, sum and quotient 2^-19 together; the result's own rounding."""
     want, tol = np.full(q.shape, np.nan), np.zeros(q.shape)
-    L = q.shape[1]
+    L, G = q.shape[1], q.shape[2] // c.H
     for b, n in enumerate(c.lens):
         k, v = (ref.tokens(a, t, c.kind, c.table, b, n) for a, t in ((c.k, c.kmax), (c.v, c.vmax)))
         hidden = (np.arange(n) > np.arange(n - L, n)[:, None]) if causal else np.zeros((L, n), bool)
         o, a, reach = ref.attention(q[b].astype(np.float64), k, v, hidden, scale)
+        s = np.einsum("lhe,nhe->lhn", q[b].astype(np.float64), np.repeat(k, G, 1)) * scale
+        s[np.broadcast_to(hidden[:, None], s.shape)] = -np.inf
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        top = np.repeat(c.vmax[c.table[b, np.arange(n) // c.T]], G, 1).T                              # (Hq, n)
         want[b] = o
-        tol[b] = a * (2.0 ** -21 + 2 * 2.0 ** -20 * reach + 2.0 ** -19) + n * 2.0 ** -30 * np.abs(v).max(initial=0) + STEP[F32][0] * np.abs(o)
+        tol[b] = a * (2.0 ** -21 + 2 * 2.0 ** -20 * reach + 2.0 ** -19) + n * 2.0 ** -30 * (p * top).max(-1)[..., None] + STEP[F32][0] * np.abs(o)
     near(got, want, tol)
 
 
@@ -33,6 +38,33 @@ def test_weights_keep_their_bits(ctx, E, G, L, kind):
     c = Cached(ctx, rng, E, 32, 2, [500, 317], kind)
     q = rng.standard_normal((2, L, 2 * G, E)).astype(np.float16)
     scale = 0.6 / E
+    got, _, _ = attend(ctx, c, q, None, scale, True, F32)
+    bound(c, q, scale, True, got)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("ratio", [20, 28, 36])
+@pytest.mark.parametrize("where", ["unseen", "unweighed", "zeros"])
+@pytest.mark.parametrize("E, G, L", [(128, 1, 30), (128, 3, 60), (64, 1, 40), (64, 2, 250)])
+def test_large_values_reach_only_rows_that_weigh_them(ctx, E, G, L, where, ratio, kind):
+    """A page whose largest value is 2^ratio of the others', which a row does not see (the last page, but for the last rows) or gives no weight
+    (the first, whose scores are 50 and more below), and pages of zeros beside it: the others' values keep their bits."""
+    rng = np.random.default_rng(25)
+    n = 16 * 20 + L
+    c = Cached(ctx, rng, E, 16, 2, [n], kind)
+    q = np.abs(rng.standard_normal((1, L, 2 * G, E))).astype(np.float16)
+    scale = 0.5 / E
+    page = c.table[0, (n - 1) // 16 if where == "unseen" else 0]
+    c.vmax *= np.float32(2.0 ** -20)
+    c.vmax[page] *= np.float32(2.0 ** ratio)
+    if where == "unweighed":      # sums of E terms of some 0.8 times -kmax
+        c.k[page] = -127 if kind == "int8" else 0xfe
+        c.kmax[page] = 300.0
+    if where == "zeros":
+        c.vmax[c.table[0, 1:4]] = 0
+        c.k[page] = 0
+    for a, host in ((c.cache.k, c.k), (c.cache.kmax, c.kmax), (c.cache.vmax, c.vmax)):
+        ctx.upload(a, host)
     got, _, _ = attend(ctx, c, q, None, scale, True, F32)
     bound(c, q, scale, True, got)
 
