@@ -40,14 +40,16 @@ def quantise4(W: np.ndarray, group: int = 64, symmetric: bool = True) -> Tuple[n
     scales (K / group, M) fp16, zeros (K / group, M) uint8 or None.  Symmetric: codes -8 to 7 and no zero points, every
     value within half a step: the largest at 7, or half a step past the end, whichever leaves the group less error (a relative 2-norm of
     0.088, 0.097 and 0.105 of normal values in groups of 32, 64 and 128).  Otherwise 15 steps from the group's least to its greatest value,
-    zero among them."""
+    zero among them.  Weights whose scales fp16 does not hold are refused."""
     if W.ndim != 2 or group not in (32, 64, 128) or W.shape[0] % group:
         raise B200Error(17, f"quantise4: a (K, M) weight of whole groups of {group} (32, 64 or 128)")
     w = W.astype(np.float64).reshape(W.shape[0] // group, group, W.shape[1])
     if not np.all(np.isfinite(w)):
         raise B200Error(1, "quantise4: the weight is not finite")
+    lo, hi = np.maximum(-w.min(1), 0), np.maximum(w.max(1), 0)
+    if np.max(np.maximum(hi / 7, lo / 8) if symmetric else (hi + lo) / 15, initial=0) >= 65520:      # rounds to infinity
+        raise B200Error(1, "quantise4: weights whose scales fp16 does not hold")
     if symmetric:
-        lo, hi = np.maximum(-w.min(1), 0), np.maximum(w.max(1), 0)
         each = [np.maximum(hi / (7 + past), lo / (8 + past)).astype(np.float16) for past in (0.5, 0.0)]
         off = []
         for s in each:
@@ -56,9 +58,8 @@ def quantise4(W: np.ndarray, group: int = 64, symmetric: bool = True) -> Tuple[n
         s = np.where(off[0] <= off[1], *each)
         z = np.full(s.shape, 8.0)
     else:
-        lo, hi = np.minimum(w.min(1), 0), np.maximum(w.max(1), 0)
-        s = ((hi - lo) / 15).astype(np.float16)
-        z = np.clip(np.rint(-lo / np.where(s == 0, 1, s).astype(np.float64)), 0, 15)
+        s = ((hi + lo) / 15).astype(np.float16)
+        z = np.clip(np.rint(lo / np.where(s == 0, 1, s).astype(np.float64)), 0, 15)
     step = np.where(s == 0, 1, s).astype(np.float64)[:, None]
     q = np.clip(np.rint(w / step) + z[:, None], 0, 15)
     return q.astype(np.uint8).reshape(W.shape), s, None if symmetric else z.astype(np.uint8)

@@ -23,3 +23,16 @@ def test_the_largest_weights_are_within_half_a_step(group, most):
     step = np.abs(np.repeat(s.astype(np.float64), group, 0))
     assert np.all(off <= step * (0.5 + 8.5 * 2.0 ** -11))
     assert np.linalg.norm(off) <= most * np.linalg.norm(W.astype(np.float64))
+
+
+@pytest.mark.parametrize("symmetric, most", [(True, 7 * 65519.0), (False, 15 * 65519.0)])
+def test_weights_whose_scale_passes_fp16_are_refused(symmetric, most):
+    """65520 rounds to infinity in fp16, and 0 times infinity is no weight; below it every weight is a number."""
+    W = np.zeros((64, 3), np.float32)
+    W[5, 1] = most
+    q, s, z = jv.quantise4(W, 64, symmetric)
+    assert np.isfinite(s).all() and abs(ref.weight4(q, s, z, 64)[5, 1] / most - 1) < 2.0 ** -4
+    W[5, 1] = most * 1.001
+    with pytest.raises(jv.B200Error) as e:
+        jv.quantise4(W, 64, symmetric)
+    assert e.value.code == 1
