@@ -772,11 +772,12 @@ int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int
     const bool fp8 = cache->kind == B200_E4M3;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634 / (fp8 ? 448.0 : 127.0));
     B200_CUDA(cudaSetDevice(ctx->device));
-    // Each tile of 16 rows converts the cache again; tiles of 128 rows convert it once.  By few rows and by many, us: 4 x 4096 tokens,
-    // 32 heads on 8, E = 128: 32 rows 29.6 and 33.7, 40 rows 36.9 and 33.9, 64 rows 44.7 and 34.0; 60000 tokens: 32 rows 63.5 and 87.9, 48
-    // rows 87.8 both; 8 x 4096, 20 heads on 4, E = 64: 40 rows 27.1 and 29.3, 50 rows 32.5 and 29.4; 60000: 40 rows 42.3 and 57.3, 65 rows
-    // 55.4 and 59.2; 32 x 500: 30 rows 25.4 and 14.7.
-    if ((int64_t)p.L * p.G > (p.c.E > 64 ? 32 : 40)) return cache_prompt_run(ctx, p.c, L, B, p.G, q, out, out_dtype, scale, fp8, causal, lens, news);
+    // Each tile of 16 rows converts the cache again; tiles of 128 rows convert it once.  By few rows and by many, us, E = 128, 32 query heads on 8 but
+    // where noted: 32 rows (two tiles) 4 x 4096 tokens 29 and 36, 16 x 8192 120 and 152, 1 x 60000 63 and 87, 32 x 500 of 8 on 2 15.9 and 17.4; 48
+    // rows 36 and 36, 171 and 152, 87 and 87, 23 and 17.5.  E = 64: 48 rows 26 and 31, 121 and 133, 61 and 77, 19 and 14; 64 rows 32 and 31, 155
+    // and 133, 75 and 77, 20 and 14.  Short caches of few items gain from few rows for longer (1 x 1500 of 16 on 4, E = 128: 48 rows 14 and 21),
+    // but lengths are not known here.
+    if ((int64_t)p.L * p.G > (p.c.E > 64 ? 32 : 48)) return cache_prompt_run(ctx, p.c, L, B, p.G, q, out, out_dtype, scale, fp8, causal, lens, news);
     if (p.L * p.G <= 8) {
         if (p.c.E <= 64) return fp8 ? cf_launch<64, true, 1>(ctx, p) : cf_launch<64, false, 1>(ctx, p);
         return fp8 ? cf_launch<128, true, 1>(ctx, p) : cf_launch<128, false, 1>(ctx, p);

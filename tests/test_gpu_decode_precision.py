@@ -31,7 +31,7 @@ def bound(c, q, scale, causal, got):
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
-@pytest.mark.parametrize("E, G, L", [(128, 4, 1), (128, 4, 8), (128, 3, 11), (128, 4, 75), (64, 5, 1), (64, 5, 8), (64, 41, 1), (64, 1, 300)])
+@pytest.mark.parametrize("E, G, L", [(128, 4, 1), (128, 4, 8), (128, 3, 11), (128, 4, 75), (64, 5, 1), (64, 5, 8), (64, 41, 1), (64, 12, 4), (64, 49, 1), (64, 1, 300)])
 def test_weights_keep_their_bits(ctx, E, G, L, kind):
     """Few query rows a key head and many, on both sides of where one kernel takes over from the other: rows of nearly equal weights."""
     rng = np.random.default_rng(21)
