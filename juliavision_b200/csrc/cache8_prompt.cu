@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
 // cache8_attention.cu.
 //
-// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 213 us, 0.73 PFLOP/s.
+// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 208 us, 0.74 PFLOP/s.
 // What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 4600 clocks a block
 // of 128 keys for two tiles whose products take 3072), which the other tile's covers in part.
 //
@@ -98,7 +98,7 @@ __device__ __forceinline__ void cp_load8(uint32_t (&v)[4], const __half* at, boo
         for (int k = 0; k < 4; ++k) v[k] = u[2 * k] | (uint32_t)u[2 * k + 1] << 16;
     }
 }
-// four results of a row, 16 bytes of fp16 or two of fp32 at a time where rows allow it
+// eight results of a row, 16 bytes at a time where rows allow it
 __device__ __forceinline__ void cp_store8(const CachePromptParams& p, int64_t at, const float (&v)[8]) {
     if (p.out_f32) {
         float* d = (float*)p.out + at;
@@ -292,13 +292,13 @@ cache_prompt_kernel(const CachePromptParams p) {
         const long long want = pieces > total / CP_LEAST ? pieces : total / CP_LEAST;
         long long many = want < gridDim.x ? want : gridDim.x;
         // Lengths far apart: what the start and end of an item take counts too, or a share of many short ones is the last to end (74
-        // items of 4 to 39 blocks 57 us without and 51 with; 128 of 64 to 80 170 and 174, 32 of 2 to 8 blocks 24 and 28).
+        // items of 4 to 39 blocks 56 us without and 51 with; 128 of 64 to 80 213 and 212, 32 of 32 36.0 and 38.8).
         const int start = 4 * total < 3 * pieces * longest && total >= 4 * many ? CP_START : 0;
         total += start * pieces, upto += start * items, mine += start * some, longest += start;
-        // Items of one length: whole shares an item, where the blocks that this leaves out would save the others less than the five
-        // blocks of keys that a second part's start and end cost (32 items of 32 blocks: 37.5 us with 148 shares, 33.1 with 128).
+        // Items of one length: whole shares an item, where the blocks that this leaves out would save the others less than the four
+        // blocks of keys that a second part's start and end cost (32 items of 32 blocks: 39.5 us with 148 shares, 36.1 with 128; 64 of 64 86.8 and 90.4).
         const long long even = pieces > 0 && pieces <= many ? many - many % pieces : many;
-        if (pieces * longest == total && total * (many - even) <= 5 * many * even) many = even;
+        if (pieces * longest == total && total * (many - even) <= 4 * many * even) many = even;
         const Shares shares(total, (int)many);
         if ((int)blockIdx.x >= shares.warps) {     // uniform
             if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -834,8 +834,9 @@ static int cp_launch(b200_ctx* ctx, CachePromptParams& p) {
     p.items = (int)items;
     // Equal shares keep every SM busy to the end.  They cost a look for the share's place and a second launch that joins, together
     // about what four blocks of keys do, and a further start and end for most items, about six (of 2 us at E = 128).  An item a launch
-    // block / shares, us: 128 items of 64 to 80 blocks 179 / 171 (E = 128), 166 / 147 (E = 64); 74 of 4 to 39 82 / 50; 8 of 782 1570 / 127;
-    // 32 of 2 to 8 27.7 / 23.9; 140 of 50 116 / 131; 256 of 28 to 32 148 / 167; 48 of 1 to 5 21 / 27; 1680 of 1 to 6 176 / 216.
+    // block / shares, us: 128 items of 64 to 80 blocks 225 / 214 (E = 128), 191 / 163 (E = 64); 74 of 4 to 39 91 / 51; 8 of 782 1989 / 151;
+    // 32 of 2 to 8 31 / 25; 140 of 50 123 / 128; 256 of 28 to 32 182 / 203; 48 of 1 to 5 20 / 25; 1680 of 1 to 6 199 / 251.  Lengths are not
+    // known here: sequences much shorter than their table get shares as if they filled it, and lose what the last four do.
     const int64_t blocks = cdiv((int64_t)p.c.width * p.c.T, CP_KEYS);
     p.shared = items <= 8 * sms && items * (blocks + 6) + 4 * sms < cdiv(items, sms) * blocks * sms;
     const int64_t grid = p.shared ? sms : items;

@@ -140,3 +140,26 @@ def test_many_tokens_through_blocks_of_rows(ctx):
         want, reach = xn @ wm + bias[m].astype(np.float64), np.abs(xn) @ np.abs(wm)
         tol = reach * sums(K) + STEP[np.float16][0] * np.abs(want) + STEP[np.float16][1]
         near(got[n][:, m] if isinstance(n, slice) else got[n], np.maximum(want, 0), tol)
+
+
+# ---------------------------------------------------------------------------------------------------------- wide tables
+@pytest.mark.parametrize("E, G, L", [(128, 2, 1), (128, 4, 8), (64, 3, 100), (128, 1, 700)])
+def test_tables_for_longer_sequences(ctx, E, G, L):
+    """A table allotted for a hundred times the tokens there are, whose entries past a sequence's length name no page: they are not read."""
+    rng = np.random.default_rng(26)
+    c = Cached(ctx, rng, E, 16, 2, [900, 701, 0], "int8")
+    c.lens[2] = 0
+    table = rng.choice([-1, 1 << 30, -(1 << 31)], (3, 6000))
+    for b, n in enumerate(c.lens):
+        table[b, :-(-n // 16)] = c.table[b, :-(-n // 16)]
+    q = rng.standard_normal((3, L, 2 * G, E)).astype(np.float16)
+    news = np.array([L, L, 0])
+    wide = ctx.toback(table.astype(np.int32))
+    c.dtable = wide
+    got, want, tol = attend(ctx, c, q, news, 1 / E, True, F32)           # synchronises: an entry that was followed would be reported
+    near(got, want, tol)
+    new = ctx.toback(rng.standard_normal((3, L, 2, E)).astype(np.float16)).permute((0, 2, 1, 3))
+    lens, dnews = (ctx.toback(np.array(v, np.int32)) for v in (c.lens, news))
+    jv.cacheappend_(ctx, c.cache, new, new, wide, lens, dnews)
+    jv.cacheread_(ctx, ctx.allocate(F32, E, 1000, 2, 3), c.cache, "k", wide, lens)
+    ctx.synchronize()
