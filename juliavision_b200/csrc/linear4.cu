@@ -33,13 +33,17 @@ constexpr int L4_WARPS = 8;      // of a block, which share K
 // 123 / 92; of 28672 x 8192 720 / 785, 951 / 818, 1415 / 1085; of 5120 x 1280 34 / 62, 50 / 51, 70 / 52; 1024 and 2048 of 1280 x 1280 25 / 32, 49 / 54.
 // (Weights rounded to one fp16 number: 512 tokens of 4096 x 4096 32 us, of 28672 x 8192 427; 2.8e-4 of the result off for 2.1e-4.)
 constexpr int L4_TOKENS = 512;
-// What fp16 weights take at a time: past it the next product's rows (28672 x 8192, 600 tokens: blocks of 64 MB 1130 us, of 128 MB 800).
+// What fp16 weights take at a time: past it the next product's rows (28672 x 8192, 512 tokens: blocks of 64 MB 1130 us, of 128 MB 800).
 constexpr int64_t L4_DENSE_BYTES = 128ll << 20, L4_DENSE_TOKENS = 2048;
-constexpr double L4_STREAM_TILES = 4608;   // of 64 rows, 16 tokens and 64 inputs: from here on a list for all warps
+// Tiles of 64 rows, 16 tokens and 64 inputs from which on up to 16 tokens go by a list for all warps.  us, blocks / list, 16 tokens: 4096 x 2048
+// (2048 tiles) 6.4 / 7.9, 4096 x 4096 (4096) 9.3 / 9.9, 5120 x 5120 (6400) 17 / 11; one token: 4096 x 4096 5.9 / 8.5, 5120 x 5120 11.3 / 9.7,
+// 8192 x 4096 (8192) 10.4 / 10.2, 8192 x 8192 (16384) 19 / 14.
+constexpr double L4_STREAM_TILES = 4608;
 // More than 16 tokens: rounds of loads, times token tiles a block, up to which the blocks that have all of them at once are faster than
-// the list.  us, blocks / list: 24 x 5120 x 1280 6.7 / 10.6, 37 x 5120 x 1280 (15) 8.4 / 10.4, 22 x 3836 x 3456 (21) 9.9 / 11.3,
-// 32 x 4096 x 4096 (32) 12.4 / 12.2, 37 x 1280 x 5120 (50) 15.9 / 10.8.
-constexpr int64_t L4_ROUNDS = 21;
+// the list.  us, blocks / list: 37 x 5120 x 1280 (15) 8.4 / 10.4, 24 x 4096 x 4096 (24) 11.1 / 12.2, 24 x 8192 x 4096 (24) 14.3 / 16.1,
+// 64 x 5120 x 1280 (24) 12.5 / 11.8, 17 x 1280 x 5120 (30) 12.7 / 9.6, 17 x 5120 x 5120 (30) 16.7 / 14.4, 64 x 4096 x 4096 (32) 16.6 / 16.1,
+// 37 x 4096 x 4096 (40) 13.8 / 14.1, 37 x 5120 x 5120 (50) 22 / 18, 200 x 4096 x 4096 (120) 45 / 37.
+constexpr int64_t L4_ROUNDS = 24;
 
 struct Linear4Params {
     const uint4* data;            // [four row tiles][k block][row tile][lane]
