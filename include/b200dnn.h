@@ -239,7 +239,7 @@ int b200_attention_f16_route(int64_t E, int64_t Lq, int64_t Lk, int64_t H, int64
  * passed on.  x and out are (E,L,H,B) fp16 with element strides {E,L,H,B}, E contiguous; out is x itself or apart from it.
  * freq (device, rot/2 values): f_i in units of 2^-64 turns, modulo one turn, which makes position * f_i modulo one turn one
  * 64-bit product, exact for every int32 position.  Token l of sequence b is at positions[l*pos_l + b*pos_b] or, with
- * lens, at lens[b] - news[b] + l; rows l >= news[b] (L without news) are left as they were.  rot is even and at most E <= 4096.
+ * lens, at lens[b] - news[b] + l; rows l >= news[b] (L without news) are left as they were.  rot is even, at most E and at most 1024; E <= 4096.
  */
 int b200_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t B, const b200_strided4* x,
                     const b200_strided4* out, const uint64_t* freq, int64_t rot, int interleaved, float gain,

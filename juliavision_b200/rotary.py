@@ -60,9 +60,11 @@ def rotaryfrequencies(rot: int, base: float = 10000.0, scaling: Optional[Tuple] 
 
 def rotaryplan(ctx: Ctx, rot: int, base: float = 10000.0, interleaved: bool = False, scaling: Optional[Tuple] = None,
                gain: Optional[float] = None, frequencies: Optional[Sequence[float]] = None) -> RotaryPlan:
-    """The plan of the first `rot` elements of a head.  `frequencies` (rot / 2 radians a position) in the place of base and
+    """The plan of the first `rot` (at most 1024) elements of a head.  `frequencies` (rot / 2 radians a position) in the place of base and
     scaling; `gain` in the place of the scaling's own."""
     f, own = rotaryfrequencies(rot, base, scaling)
+    if rot > 1024:
+        raise B200Error(17, f"rotary: {rot} elements (at most 1024)")
     if frequencies is not None:
         f = np.asarray(frequencies, dtype=np.float64)
         if f.shape != (rot // 2,) or not np.all(np.isfinite(f)):

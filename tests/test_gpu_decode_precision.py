@@ -163,3 +163,17 @@ def test_tables_for_longer_sequences(ctx, E, G, L):
     jv.cacheappend_(ctx, c.cache, new, new, wide, lens, dnews)
     jv.cacheread_(ctx, ctx.allocate(F32, E, 1000, 2, 3), c.cache, "k", wide, lens)
     ctx.synchronize()
+
+
+@pytest.mark.parametrize("E, rot, inter", [(1024, 1024, False), (1100, 1024, True), (4096, 1000, False)])
+def test_rotary_of_the_widest_heads(ctx, E, rot, inter):
+    rng = np.random.default_rng(27)
+    x = rng.standard_normal((2, 5, 3, E)).astype(np.float16)
+    lens = np.array([100005, 7])
+    out = ctx.allocate(np.float16, E, 3, 5, 2).permute((0, 2, 1, 3))
+    jv.rotary_(ctx, jv.rotaryplan(ctx, rot, interleaved=inter), out, ctx.toback(x).permute((0, 2, 1, 3)), lens=ctx.toback(lens.astype(np.int32)))
+    ctx.synchronize()
+    want = ref.rotary(x, (lens - 5)[:, None] + np.arange(5), *jv.rotaryfrequencies(rot), inter)
+    # fp32: angles off by 2^-25 turns and the library's sine and cosine by 2^-23 or so, three roundings of at most 2^-24
+    slack = 2.0 ** -20 * 2 * np.abs(x.astype(np.float64)).max(-1, keepdims=True)
+    near(ctx.contiguous(out.permute((0, 2, 1, 3))).to_host(), want, STEP[np.float16][0] * np.abs(want) + STEP[np.float16][1] + slack)
