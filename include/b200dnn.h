@@ -276,9 +276,10 @@ int b200_cache_read(b200_ctx* ctx, const b200_cache8* cache, int values, int64_t
                     const int32_t* lens, const b200_strided4* out, int out_dtype);
 /* out = softmax(scale * Q K') V over the cache: q and out (E,L,Hq,B), E contiguous, Hq a multiple of H; query head i reads key
  * head i / (Hq / H).  Every query sees the keys below lens[b]; when causal, up to its own position.  A row that sees no key
- * comes out as zeros; rows at or past news[b] are left as they were.  out does not overlap q.  Scores, softmax and sums are fp32;
- * for the second product the weights are taken as two fp16 halves (21 bits), relative
- * to the row's largest product of a weight and its page's vmax (of 2^-80 at least).  Scratch comes from the context's workspace. */
+ * comes out as zeros; rows at or past news[b] are left as they were.  out does not overlap q.  e4m3's codes of a NaN, which append never
+ * writes, are NaN in a key and read as 448 in a value, since rows that do not see it share its tile (b200_cache_read says NaN).  Scores,
+ * softmax and sums are fp32; for the second product the weights are taken as two fp16 halves (21 bits), relative to the row's largest
+ * product of a weight and its page's vmax (of 2^-80 at least).  Scratch comes from the context's workspace. */
 int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int64_t Hq, int64_t B, const b200_strided4* q,
                          const b200_strided4* out, int out_dtype, float scale, int causal, const int32_t* lens,
                          const int32_t* news);

@@ -177,3 +177,20 @@ def test_rotary_of_the_widest_heads(ctx, E, rot, inter):
     # fp32: angles off by 2^-25 turns and the library's sine and cosine by 2^-23 or so, three roundings of at most 2^-24
     slack = 2.0 ** -20 * 2 * np.abs(x.astype(np.float64)).max(-1, keepdims=True)
     near(ctx.contiguous(out.permute((0, 2, 1, 3))).to_host(), want, STEP[np.float16][0] * np.abs(want) + STEP[np.float16][1] + slack)
+
+
+def test_the_code_of_a_nan_among_values(ctx):
+    """A cache that another program filled may hold e4m3's NaN: cacheread says so, attention's keys too; as a value attention takes it as 448, since rows
+    that do not see it share its tile."""
+    rng = np.random.default_rng(28)
+    for L in (2, 90):
+        c = Cached(ctx, rng, 64, 16, 1, [200], "e4m3")
+        c.v[c.table[0, 3], 0, 5, 7] = 0x7f
+        ctx.upload(c.cache.v, c.v)
+        out = ctx.allocate(F32, 64, 200, 1, 1)
+        jv.cacheread_(ctx, out, c.cache, "v", c.dtable, c.dlens)
+        ctx.synchronize()
+        assert np.argwhere(np.isnan(out.to_host()[0, 0])).tolist() == [[3 * 16 + 5, 7]]
+        c.v[c.table[0, 3], 0, 5, 7] = 0x7e                                       # 448
+        q = rng.standard_normal((1, L, 2, 64)).astype(np.float16)
+        near(*attend(ctx, c, q, None, 0.01, True))
