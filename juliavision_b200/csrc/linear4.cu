@@ -501,7 +501,8 @@ linear4_unpack_kernel(const Linear4Params p, int64_t four0, __half* out, int64_t
     }
 }
 
-// Results of `rows` rows from m0 and `tokens` tokens from n0: both parts' sums, brought back to scale.
+// Results of `rows` rows from m0 and `tokens` tokens from n0: both parts' sums, brought back to scale.  Where the upper parts' is not
+// finite it is the result: what is infinite times a lower part of 0 is no number.
 constexpr int L4_FINISH_TOKENS = 8;      // a thread
 __global__ void __launch_bounds__(128)
 linear4_finish_kernel(const Linear4Params p, const float* __restrict__ y, int64_t R, const uint8_t* __restrict__ shift, int64_t m0, int rows, int n0, int tokens) {
@@ -517,7 +518,7 @@ linear4_finish_kernel(const Linear4Params p, const float* __restrict__ y, int64_
         for (int part = 0; part < 2; ++part) v[i][part] = at + i < tokens ? y[(at + i) * 2 * R + part * R + r] : 0.f;
 #pragma unroll
     for (int i = 0; i < L4_FINISH_TOKENS; ++i)
-        if (at + i < tokens) l4_store(p, m0 + r, n0 + at + i, (v[i][0] + v[i][1]) * f);
+        if (at + i < tokens) l4_store(p, m0 + r, n0 + at + i, (v[i][0] + (isfinite(v[i][0]) ? v[i][1] : 0.f)) * f);
 }
 
 struct PackParams {

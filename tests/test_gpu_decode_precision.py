@@ -194,3 +194,25 @@ def test_the_code_of_a_nan_among_values(ctx):
         c.v[c.table[0, 3], 0, 5, 7] = 0x7e                                       # 448
         q = rng.standard_normal((1, L, 2, 64)).astype(np.float16)
         near(*attend(ctx, c, q, None, 0.01, True))
+
+
+@pytest.mark.parametrize("N", [1, 40, 300, 513, 600])
+def test_infinite_inputs_give_infinite_sums(ctx, N):
+    """An infinite input of some tokens against weights that are not zero: infinite of the weight's sign, other tokens as they were."""
+    rng = np.random.default_rng(29)
+    M, K = 70, 128
+    q = rng.integers(0, 7, (K, M)).astype(np.uint8) + rng.integers(0, 2, (K, M)).astype(np.uint8) * 9       # not 8
+    q[q == 8] = 9
+    s = (rng.random((2, M)) * 0.02 + 0.001).astype(np.float16)
+    s[:, ::2] = np.float16(0.0078125)                                  # products that one fp16 number holds
+    x = rng.standard_normal((N, K)).astype(np.float16)
+    x[N // 2, 5] = np.inf
+    w = jv.pack4(ctx, ctx.toback(q), ctx.toback(s), None, 64)
+    out = ctx.allocate(F32, M, N)
+    jv.matmul4_(ctx, out, w, ctx.toback(x))
+    ctx.synchronize()
+    got, wd = out.to_host(), ref.weight4(q, s, None, 64)
+    assert np.array_equal(got[N // 2], np.where(wd[5] > 0, np.inf, -np.inf))
+    rest = np.arange(N) != N // 2
+    xd = x[rest].astype(np.float64)
+    near(got[rest], xd @ wd, np.abs(xd) @ np.abs(wd) * sums(K) + STEP[F32][0] * np.abs(xd @ wd))
