@@ -568,6 +568,7 @@ linear4_pack_kernel(const PackParams p) {
 
 template <int ROWS, int NT>
 static int l4_launch(b200_ctx* ctx, const Linear4Params& p) {
+    B200_REQUIRE(cdiv(p.N, 8 * NT) < 65536, B200_DECLINE_EXTENT, "matmul_q4: %d tokens off 16-byte boundaries", p.N);
     auto kern = p.logg == 5 ? linear4_kernel<ROWS, NT, true> : linear4_kernel<ROWS, NT, false>;
     B200_CUDA(launch_dep(kern, dim3((unsigned)cdiv(p.MT, ROWS), (unsigned)cdiv(p.N, 8 * NT)), dim3(32 * L4_WARPS), 0, ctx->stream, 1, p));
     ctx->launches++;
@@ -694,7 +695,8 @@ int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, in
     p.logg = A->group == 32 ? 5 : A->group == 64 ? 6 : 7;
     p.out_f32 = out_dtype == B200_F32, p.epi = epilogue;
     p.whole = (uintptr_t)B % 16 == 0 && ldb % 8 == 0;
-    if (N > L4_TOKENS) return l4_dense(ctx, A, p, B, ldb);
+    // Inputs off 16-byte boundaries keep to the kernels, where the GEMM would read them one by one (1000 tokens of 4096 x 4096 403 us and 1153).
+    if (N > L4_TOKENS && p.whole) return l4_dense(ctx, A, p, B, ldb);
     p.d_status = ctx->d_status;
     const int nt = N <= 8 ? 1 : 2;
     // More than 16 tokens: up to 40 to a block of linear4_kernel, whose warps take a round trip of loads a k block.
