@@ -23,8 +23,8 @@
 // warp's share waits in the workspace; the last pieces of a block's warps are joined in shared memory at its end, and a second
 // launch joins what then still lies in several places, in the order of the list: the result does not depend on timing.
 //
-// 32 sequences of 1000 to 8192 tokens, 32 heads on 8, E = 128: 310 MB in 65 us (4.8 TB/s; some 5 us of it before the first tile and
-// in the join, the rest the uneven ends of the shares); 131071 tokens of one in 54 us (5.0 TB/s).
+// 32 sequences of 1000 to 8192 tokens, 32 heads on 8, E = 128: 310 MB in 68 us a call (4.6 TB/s; some 5 us of it before the first tile
+// and in the join, 2 at the uneven ends of the shares, the rest waits for stages that are asked for only once they are read); 131071 tokens of one in 54 us (5.0 TB/s).
 #include <cuda_fp16.h>
 
 #include "cache8.cuh"

@@ -1,7 +1,8 @@
 // Attention over the paged 8-bit cache (cache8.cuh) for many query rows a key head: a piece of a prompt, the formula of
 // cache8_attention.cu.
 //
-// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 208 us, 0.74 PFLOP/s.
+// Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 229 us a call
+// between others, 208 back to back (0.68 and 0.74 PFLOP/s).
 // What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 4600 clocks a block
 // of 128 keys for two tiles whose products take 3072), which the other tile's covers in part.
 //
@@ -510,7 +511,7 @@ cache_prompt_kernel(const CachePromptParams p) {
             }
         };
         // Sides in turn: K(0), V(0), K(1), ...  One copy of the code serves both: the loops of all warps together do not fit the nearer
-        // instruction caches, and this one's length is everyone's wait (2048 tokens over 10240 177 us with a copy each, 163 with one).
+        // instruction caches, and this one's length is everyone's wait (2048 tokens over 10240, with one half a weight, 177 us with a copy each, 163 with one).
         // What it costs is a side less on its way from memory, which a cache that is read once misses: 64 tokens over 100000 122 us
         // and 127.  Asking L2 for later rows gave some of that back, and its code took as much from the others.
         uint4 cur[NV], nxt[NV];

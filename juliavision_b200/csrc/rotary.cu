@@ -7,7 +7,7 @@
 // The fraction's top 32 bits become a float in [-1/2, 1/2), off by at most 2^-25 turns.  Sines and products are fp32; the
 // result is rounded once.
 //
-// Bandwidth-bound: two bytes read and two written an element (14336 tokens, 40 heads of 128: 52 us, 5.6 TB/s; a step of 8 x 40 heads
+// Bandwidth-bound: two bytes read and two written an element (14336 tokens, 40 heads of 128: 51 us a call, 5.8 TB/s; a step of 8 x 40 heads
 // of 64 3 us, the launch).  A block takes whole rows (a token of a sequence) over all or
 // some of the heads; a row's rot / 2 cosines and sines are computed once for them, into shared memory, since 40 instructions
 // a pair would cost more than the pair's eight bytes take.
