@@ -299,8 +299,9 @@ int b200_q4_sizes(int64_t M, int64_t K, int64_t group, int64_t* data_bytes, int6
 int b200_q4_pack(b200_ctx* ctx, const void* q, int64_t q_m, int64_t q_k, const void* scales, int64_t s_m, int64_t s_g,
                  const void* zeros, int64_t z_m, int64_t z_g, const b200_q4* out);
 /* out(M,N) = epi(T(bias[m] + sum_k w[m,k] B(K,N)[k,n])): b200_gemm_f16 with such a weight, fp16 B and bias, fp32 accumulation,
- * the weights taken exactly.  Past 512 tokens they are laid out in the context's workspace, up to 128 MB at a time, as pairs of
- * fp16 numbers; there a row with a scale above 4096 is held to whole multiples of 2^-20.  out does not overlap B. */
+ * the weights taken exactly.  Past 512 tokens they are laid out in the context's workspace, some rows at a time, as pairs of
+ * fp16 numbers (256 MB with their sums, or what 256 rows take); there a row with a scale above 4096 is held to whole multiples of
+ * 2^-20.  out does not overlap B. */
 int b200_matmul_q4(b200_ctx* ctx, const b200_q4* A, int64_t N, const void* B, int64_t ldb, const void* bias, void* out,
                    int64_t ldo, int out_dtype, int epilogue);
 

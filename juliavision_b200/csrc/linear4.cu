@@ -30,11 +30,11 @@ namespace b200 {
 constexpr int L4_WARPS = 8;      // of a block, which share K
 // Tokens the two kernels take; more go through fp16 weights in the workspace, which are made once for all tokens and cost twice the
 // products, since an exact weight is two fp16 numbers.  us, kernels / fp16 weights: 384, 512 and 768 tokens of 4096 x 4096 62 / 78, 79 / 78,
-// 123 / 92; of 28672 x 8192 720 / 785, 951 / 818, 1415 / 1085; of 5120 x 1280 34 / 62, 50 / 51, 70 / 52; 1024 and 2048 of 1280 x 1280 25 / 32, 49 / 54.
+// 123 / 92; of 28672 x 8192 720 / 785, 951 / 818, 1415 / 968; of 5120 x 1280 34 / 62, 50 / 51, 70 / 52; 1024 and 2048 of 1280 x 1280 25 / 32, 49 / 54.
 // (Weights rounded to one fp16 number: 512 tokens of 4096 x 4096 32 us, of 28672 x 8192 427; 2.8e-4 of the result off for 2.1e-4.)
 constexpr int L4_TOKENS = 512;
-// What fp16 weights take at a time: past it the next product's rows (28672 x 8192, 512 tokens: blocks of 64 MB 1130 us, of 128 MB 800).
-constexpr int64_t L4_DENSE_BYTES = 128ll << 20, L4_DENSE_TOKENS = 2048;
+// What fp16 weights and their fp32 sums take at a time: past it the next product's rows.
+constexpr int64_t L4_DENSE_BYTES = 256ll << 20, L4_DENSE_TOKENS = 2048;
 // Tiles of 64 rows, 16 tokens and 64 inputs from which on up to 16 tokens go by a list for all warps.  us, blocks / list, 16 tokens: 4096 x 2048
 // (2048 tiles) 6.4 / 7.9, 4096 x 4096 (4096) 9.3 / 9.9, 5120 x 5120 (6400) 17 / 11; one token: 4096 x 4096 5.9 / 8.5, 5120 x 5120 11.3 / 9.7,
 // 8192 x 4096 (8192) 10.4 / 10.2, 8192 x 8192 (16384) 19 / 14.
@@ -601,12 +601,13 @@ static int l4_stream_launch(b200_ctx* ctx, Linear4Params& p) {
 static int l4_dense(b200_ctx* ctx, const b200_q4* A, const Linear4Params& p, const void* B, int64_t ldb) {
     const int64_t K = A->K, units = cdiv(A->M, 64), parts = cdiv(p.KB, 2 * L4_UNPACK_STEPS);
     B200_REQUIRE(parts < 65536, B200_DECLINE_EXTENT, "matmul_q4: K=%lld", (long long)K);
-    int64_t block = L4_DENSE_BYTES / (4 * 64 * K);         // units of 64 rows, two parts of two bytes
+    const int64_t most = p.N < L4_DENSE_TOKENS ? p.N : L4_DENSE_TOKENS, row = 4 * K + 8 * most + 1;   // two parts of two bytes, their sums, a shift
+    int64_t block = L4_DENSE_BYTES / (64 * row);           // units of 64 rows
     if (block < 4) block = 4;
     block = cdiv(units, cdiv(units, block));               // blocks of like sizes
-    const int64_t R = block * 64, most = p.N < L4_DENSE_TOKENS ? p.N : L4_DENSE_TOKENS;
+    const int64_t R = block * 64;
     void* ws = nullptr;
-    int rc = ws_scratch(ctx, (size_t)R * (4 * K + 8 * most + 1), &ws);
+    int rc = ws_scratch(ctx, (size_t)(R * row), &ws);
     if (rc) return rc;
     __half* w = static_cast<__half*>(ws);
     float* y = reinterpret_cast<float*>(w + 2 * R * K);

@@ -216,3 +216,22 @@ def test_infinite_inputs_give_infinite_sums(ctx, N):
     rest = np.arange(N) != N // 2
     xd = x[rest].astype(np.float64)
     near(got[rest], xd @ wd, np.abs(xd) @ np.abs(wd) * sums(K) + STEP[F32][0] * np.abs(xd @ wd))
+
+
+def test_many_tokens_take_a_bounded_workspace(ctx):
+    """Rows are laid out some at a time, whatever the shape: 60000 rows' sums alone would be a gigabyte."""
+    rng = np.random.default_rng(30)
+    N, M, K = 2048, 60000, 64
+    q, s = rng.integers(0, 16, (K, M)).astype(np.uint8), (rng.random((1, M)) * 0.02).astype(np.float16)
+    x = rng.standard_normal((N, K)).astype(np.float16)
+    w = jv.pack4(ctx, ctx.toback(q), ctx.toback(s), None, 64)
+    out = ctx.allocate(np.float16, M, N)
+    ctx.ws.reset()
+    jv.matmul4_(ctx, out, w, ctx.toback(x))
+    ctx.synchronize()
+    used = ctx.ws.stats()[0]
+    ctx.ws.reset()
+    assert used <= 257 << 20, used
+    got = out.to_host()[::97]
+    xd, wd = x[::97].astype(np.float64), ref.weight4(q, s, None, 64)
+    near(got, xd @ wd, np.abs(xd) @ np.abs(wd) * sums(K) + STEP[np.float16][0] * np.abs(xd @ wd) + STEP[np.float16][1])
