@@ -4,7 +4,7 @@
 // Tensor-bound in the limit: 4 E flops a row and visible key; 2048 new tokens of 10240, 16 heads on 4, E = 128: 229 us a call
 // between others, 208 back to back (0.68 and 0.74 PFLOP/s).
 // What it waits for is the chain of one tile (scores into registers, maximum, exponentials, P V, the next Q K', some 4600 clocks a block
-// of 128 keys for two tiles whose products take 3072), which the other tile's covers in part.
+// of 128 keys for two tiles whose products take two thirds of that), which the other tile's covers in part.
 //
 // The query rows of a key head (the heads that share it, times the new tokens) are stacked; a block takes two tiles of 128 of them
 // and walks their keys in blocks of 128: S = Q K^T and O += P V on tcgen05 with S, P (two fp16 halves, 21 bits and more of a

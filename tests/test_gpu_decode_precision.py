@@ -235,3 +235,32 @@ def test_many_tokens_take_a_bounded_workspace(ctx):
     got = out.to_host()[::97]
     xd, wd = x[::97].astype(np.float64), ref.weight4(q, s, None, 64)
     near(got, xd @ wd, np.abs(xd) @ np.abs(wd) * sums(K) + STEP[np.float16][0] * np.abs(xd @ wd) + STEP[np.float16][1])
+
+
+@pytest.mark.parametrize("M, K, N", [(200, 512, 600), (9000, 4096, 520), (8192, 4096, 40), (1000, 512, 300)])
+def test_products_are_the_same_twice_and_replayed(ctx, M, K, N):
+    """The same bits by calls and by two graphs whose workspaces are one, replayed in turn with calls between them."""
+    rng = np.random.default_rng(31)
+    q, s = rng.integers(0, 16, (K, M)).astype(np.uint8), (rng.random((K // 64, M)) * 0.02).astype(np.float16)
+    w = jv.pack4(ctx, ctx.toback(q), ctx.toback(s), None, 64)
+    xs = [ctx.toback(rng.standard_normal((N, K)).astype(np.float16)) for _ in range(2)]
+    outs = [ctx.allocate(F32, M, N) for _ in range(2)]
+    first = []
+    for x, out in zip(xs, outs):
+        ctx.ws.reset()
+        jv.matmul4_(ctx, out, w, x)
+        first.append(out.to_host())
+    assert not np.array_equal(*first)
+    graphs = []
+    for x, out in zip(xs, outs):
+        ctx.ws.reset()
+        graphs.append(ctx.capture(lambda o=out, x=x: jv.matmul4_(ctx, o, w, x)))
+        ctx.fill_bytes(out, 0xFF)
+    spare = ctx.allocate(F32, M, N)
+    for _ in range(2):
+        for g in graphs:
+            g.replay()
+        ctx.ws.reset()
+        jv.matmul4_(ctx, spare, w, xs[0])
+    ctx.synchronize()
+    assert all(np.array_equal(a, o.to_host()) for a, o in zip(first + first[:1], outs + [spare]))
