@@ -245,6 +245,14 @@ int b200_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t B, c
                     const b200_strided4* out, const uint64_t* freq, int64_t rot, int interleaved, float gain,
                     const int32_t* positions, int64_t pos_l, int64_t pos_b, const int32_t* lens, const int32_t* news);
 
+/* Each head divided by sqrt(mean x^2 + eps) and multiplied by weight, then turned as above, rounded once.  weight (fp16 or fp32, NULL:
+ * ones) has E contiguous and columns weight_ld apart: head h takes column h (split -1; weight_ld 0: all heads the same), or column 0 below
+ * `split` and 1 from there on.  Squares, their sum and the root are fp32.  Everything else as for b200_rotary_f16; rot may be 0. */
+int b200_norm_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t B, const b200_strided4* x,
+                         const b200_strided4* out, const void* weight, int weight_dtype, int64_t weight_ld, int64_t split, float eps,
+                         const uint64_t* freq, int64_t rot, int interleaved, float gain, const int32_t* positions, int64_t pos_l,
+                         int64_t pos_b, const int32_t* lens, const int32_t* news);
+
 /* ----------------------------------------------- keys and values held in 8 bits */
 /*
  * A cache of P pages of T tokens (16, 32, 64 or 128) for H key heads of E elements (a multiple of 16 up to 128), k and v

@@ -18,7 +18,7 @@ from .layernorm import add_layernorm_, layernorm_, native_layer_norm
 from .linear4 import Weight4, matmul4_, pack4, quantise4
 from .matmul import batchedmatmul_, matmul_, mmplan
 from .rewrites import foldbatchnorm, foldrelu, hoistcasts, weightsource
-from .rotary import RotaryPlan, rotary_, rotaryfrequencies, rotaryplan
+from .rotary import RotaryPlan, normrotary_, rotary_, rotaryfrequencies, rotaryplan
 from .safetensors import readsafetensors, safetensorsnames
 from .plan import Slab, alignup, checkslab, lifetimes, place, planslab
 from .shard import gather_shards, shard_range, shard_range_py
@@ -33,5 +33,5 @@ __all__ = [
     "maxpool2d_", "to_copy_", "MMGemvPlan", "foldoutcasts", "foldincasts", "foldbatchnorm", "foldrelu", "hoistcasts", "weightsource", "readsafetensors", "safetensorsnames",
     "Event", "StreamedPass", "Diagnostics", "TwoGemmPlan", "convolutiontranspose_", "convtransposesize", "shufflecase",
     "Cache8", "cache8", "cacheappend_", "cacheread_", "cachesdpa_", "Weight4", "matmul4_", "pack4", "quantise4", "RotaryPlan", "rotary_",
-    "rotaryfrequencies", "rotaryplan",
+    "rotaryfrequencies", "rotaryplan", "normrotary_",
 ]

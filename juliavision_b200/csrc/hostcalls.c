@@ -40,6 +40,9 @@ static int (*p_cachesdpa)(b200_ctx*, const b200_cache8*, int64_t, int64_t, int64
                           const int32_t*, const int32_t*);
 static int (*p_matmul4)(b200_ctx*, const b200_q4*, int64_t, const void*, int64_t, const void*, void*, int64_t, int, int);
 
+static int (*p_normrotary)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, const b200_strided4*, const b200_strided4*, const void*, int, int64_t,
+                           int64_t, float, const uint64_t*, int64_t, int, float, const int32_t*, int64_t, int64_t, const int32_t*, const int32_t*);
+
 static int64_t attr_int(PyObject* o, PyObject* name, int* ok) {
     PyObject* v = PyObject_GetAttr(o, name);
     int64_t r = 0;
@@ -278,22 +281,20 @@ static int heads(PyObject* o, Arr* a, int64_t E, int64_t H, b200_strided4* s) {
     return 1;
 }
 
-// rotary(handle, plan, out, x, lens, news)
-static PyObject* h_rotary(PyObject* self, PyObject* const* v, Py_ssize_t n) {
-    Arr out, x;
-    const int32_t *lens, *news;
-    b200_ctx* c;
-    int rc, ok = 1;
-    if (n != 6 || !(c = handle(v[0])) || v[4] == Py_None || !load(v[2], &out) || !load(v[3], &x)) Py_RETURN_NONE;
-    if (out.nd != 4 || x.nd != 4 || out.code != B200_F16 || x.code != B200_F16) Py_RETURN_NONE;
-    for (int i = 0; i < 4; ++i)
-        if (out.shape[i] != x.shape[i]) Py_RETURN_NONE;
-    if (!counts(v[4], x.shape[3], &lens) || !counts(v[5], x.shape[3], &news)) Py_RETURN_NONE;
-    const int64_t rot = attr_int(v[1], s_rot, &ok), inter = attr_int(v[1], s_interleaved, &ok);
-    PyObject *gain = PyObject_GetAttr(v[1], s_gain), *freq = PyObject_GetAttr(v[1], s_freq);
-    const int64_t f = freq ? attr_int(freq, s_ptr, &ok) : 0;
-    float g = 0.f;
-    if (gain && PyFloat_Check(gain)) g = (float)PyFloat_AS_DOUBLE(gain);
+// A plan of positions: 1 with its numbers, else 0.
+typedef struct {
+    int64_t rot, freq;
+    int interleaved;
+    float gain;
+} Plan;
+static int rotation(PyObject* o, Plan* p) {
+    int ok = 1;
+    p->rot = attr_int(o, s_rot, &ok);
+    p->interleaved = attr_int(o, s_interleaved, &ok) != 0;
+    PyObject *gain = PyObject_GetAttr(o, s_gain), *freq = PyObject_GetAttr(o, s_freq);
+    p->freq = freq ? attr_int(freq, s_ptr, &ok) : 0;
+    p->gain = 0.f;
+    if (gain && PyFloat_Check(gain)) p->gain = (float)PyFloat_AS_DOUBLE(gain);
     else ok = 0;
     Py_XDECREF(gain);
     Py_XDECREF(freq);
@@ -301,11 +302,61 @@ static PyObject* h_rotary(PyObject* self, PyObject* const* v, Py_ssize_t n) {
         PyErr_Clear();
         ok = 0;
     }
-    if (!ok || !f) Py_RETURN_NONE;
+    return ok && p->freq;
+}
+// Heads to turn, x to out, by lengths: 1 where both are what the library takes.
+static int turned(PyObject* po, PyObject* px, PyObject* plens, PyObject* pnews, Arr* out, Arr* x, const int32_t** lens, const int32_t** news) {
+    if (plens == Py_None || !load(po, out) || !load(px, x)) return 0;
+    if (out->nd != 4 || x->nd != 4 || out->code != B200_F16 || x->code != B200_F16) return 0;
+    for (int i = 0; i < 4; ++i)
+        if (out->shape[i] != x->shape[i]) return 0;
+    return counts(plens, x->shape[3], lens) && counts(pnews, x->shape[3], news);
+}
+
+// rotary(handle, plan, out, x, lens, news)
+static PyObject* h_rotary(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+    Arr out, x;
+    Plan plan;
+    const int32_t *lens, *news;
+    b200_ctx* c;
+    int rc;
+    if (n != 6 || !(c = handle(v[0])) || !turned(v[2], v[3], v[4], v[5], &out, &x, &lens, &news) || !rotation(v[1], &plan)) Py_RETURN_NONE;
     b200_strided4 so, sx;
     strided(&out, &so);
     strided(&x, &sx);
-    ENTER(rc, p_rotary(c, x.shape[0], x.shape[1], x.shape[2], x.shape[3], &sx, &so, (const uint64_t*)f, rot, inter != 0, g, NULL, 0, 0, lens, news));
+    ENTER(rc, p_rotary(c, x.shape[0], x.shape[1], x.shape[2], x.shape[3], &sx, &so, (const uint64_t*)plan.freq, plan.rot, plan.interleaved, plan.gain,
+                       NULL, 0, 0, lens, news));
+    return PyLong_FromLong(rc);
+}
+
+// normrotary(handle, plan, out, x, weight, eps, split, lens, news)
+static PyObject* h_normrotary(PyObject* self, PyObject* const* v, Py_ssize_t n) {
+    Arr out, x, w;
+    Plan plan;
+    const int32_t *lens, *news;
+    b200_ctx* c;
+    int rc, over = 0;
+    if (n != 9 || !(c = handle(v[0])) || !PyFloat_Check(v[5]) || !turned(v[2], v[3], v[7], v[8], &out, &x, &lens, &news) || !rotation(v[1], &plan))
+        Py_RETURN_NONE;
+    const int64_t E = x.shape[0], H = x.shape[2];
+    int64_t split = -1, ld = 0;
+    memset(&w, 0, sizeof w);
+    if (v[6] != Py_None) {
+        if (!PyLong_Check(v[6]) || v[4] == Py_None) Py_RETURN_NONE;
+        split = PyLong_AsLongLongAndOverflow(v[6], &over);
+        if (over || split < 0 || split > H) Py_RETURN_NONE;
+    }
+    if (v[4] != Py_None) {
+        if (!load(v[4], &w) || w.nd > 2 || w.shape[0] != E || (E > 1 && w.stride[0] != 1)) Py_RETURN_NONE;
+        const int64_t columns = w.nd == 1 ? 1 : w.shape[1];
+        if (columns != (split >= 0 ? 2 : columns == 1 ? 1 : H)) Py_RETURN_NONE;
+        ld = columns == 1 ? 0 : w.stride[1];
+    }
+    b200_strided4 so, sx;
+    strided(&out, &so);
+    strided(&x, &sx);
+    ENTER(rc, p_normrotary(c, E, x.shape[1], H, x.shape[3], &sx, &so, P(w), w.code, ld, split, (float)PyFloat_AS_DOUBLE(v[5]),
+                           (const uint64_t*)plan.freq, plan.rot, plan.interleaved, plan.gain, NULL, 0, 0, lens, news));
     return PyLong_FromLong(rc);
 }
 
@@ -388,6 +439,14 @@ static PyObject* h_binddecode(PyObject* self, PyObject* args) {
     Py_RETURN_NONE;
 }
 
+// bindaround(norm and rotation): the entry points around a decoder's step, as addresses
+static PyObject* h_bindaround(PyObject* self, PyObject* args) {
+    unsigned long long a;
+    if (!PyArg_ParseTuple(args, "K", &a)) return NULL;
+    *(void**)&p_normrotary = (void*)(uintptr_t)a;
+    Py_RETURN_NONE;
+}
+
 // bind(gemm, gemv, attention, layernorm, convolution): the library's entry points, as addresses
 static PyObject* h_bind(PyObject* self, PyObject* args) {
     unsigned long long a, b, c, d, e;
@@ -407,6 +466,8 @@ static PyMethodDef methods[] = {{"bind", h_bind, METH_VARARGS, NULL},
                                 {"convolution", (PyCFunction)(void (*)(void))h_convolution, METH_FASTCALL, NULL},
                                 {"binddecode", h_binddecode, METH_VARARGS, NULL},
                                 {"rotary", (PyCFunction)(void (*)(void))h_rotary, METH_FASTCALL, NULL},
+                                {"bindaround", h_bindaround, METH_VARARGS, NULL},
+                                {"normrotary", (PyCFunction)(void (*)(void))h_normrotary, METH_FASTCALL, NULL},
                                 {"cacheappend", (PyCFunction)(void (*)(void))h_cacheappend, METH_FASTCALL, NULL},
                                 {"cacheread", (PyCFunction)(void (*)(void))h_cacheread, METH_FASTCALL, NULL},
                                 {"cachesdpa", (PyCFunction)(void (*)(void))h_cachesdpa, METH_FASTCALL, NULL},

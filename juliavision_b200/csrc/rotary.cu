@@ -15,31 +15,24 @@
 
 #include "internal.h"
 #include "ptx.cuh"
+#include "rotary.cuh"
 
 namespace b200 {
 
-constexpr int ROT_THREADS = 256;
-constexpr int ROT_PAIRS = 512;     // cosines and sines a block holds: rows * rot / 2 at most
+constexpr int ROT_THREADS = 256;   // a block holds ROT_PAIRS cosines and sines: rows * rot / 2 at most
 
 struct RotaryParams {
     const __half* x;
     __half* out;
     int64_t xL, xH, xB, oL, oH, oB;
     const unsigned long long* freq;
-    const int32_t *positions, *lens, *news;
-    int64_t posL, posB;
+    RotPositions at;
     float gain;
     int E, rot, L, H, heads, rows;   // heads of a block, rows of a block
     int64_t total;                   // rows in all: L * B
     Divisor per, per_heads;          // steps of a head, heads of a block
     int interleaved, moves;          // moves: out is not x, so the rest of a head is copied
 };
-
-__device__ __forceinline__ uint32_t rot_pack(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 rot_unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
 // VEC: 16 elements (8 pairs) a step as two aligned vectors; otherwise pair by pair, at any alignment.
 template <bool VEC>
@@ -54,19 +47,10 @@ rotary_kernel(const RotaryParams p) {
     const int h0 = blockIdx.y * p.heads, heads = p.H - h0 < p.heads ? p.H - h0 : p.heads;
     grid_dep_wait();
     grid_dep_launch();
-    auto position = [&](int64_t l, int64_t b, bool& live) {
-        if (p.positions != nullptr) {
-            live = true;
-            return p.positions[l * p.posL + b * p.posB];
-        }
-        const int m = p.news != nullptr ? p.news[b] : p.L;
-        live = l < m;
-        return (int)((unsigned)p.lens[b] - (unsigned)m + (unsigned)l);
-    };
     if (tid < rows) {
         const int64_t row = row0 + tid, b = row / p.L, l = row - b * p.L;
         bool live;
-        position(l, b, live);
+        p.at.at(l, b, live);
         on[tid] = live;
         xat[tid] = l * p.xL + b * p.xB;
         oat[tid] = l * p.oL + b * p.oB;
@@ -75,10 +59,8 @@ rotary_kernel(const RotaryParams p) {
         const int r = i / half, pair = i - r * half;
         const int64_t row = row0 + r, b = row / p.L, l = row - b * p.L;
         bool live;
-        const int at = position(l, b, live);
-        const unsigned long long turns = (unsigned long long)(long long)at * p.freq[pair];
         float s, c;
-        sincospif((float)(int)(turns >> 32) * 0x1p-31f, &s, &c);
+        rot_turn(p.at.at(l, b, live), p.freq[pair], s, c);
         cs[i] = c * p.gain;
         sn[i] = s * p.gain;
     }
@@ -176,8 +158,7 @@ int b200_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t B, c
     p.xL = x->stride[1], p.xH = x->stride[2], p.xB = x->stride[3];
     p.oL = out->stride[1], p.oH = out->stride[2], p.oB = out->stride[3];
     p.freq = (const unsigned long long*)freq;
-    p.positions = positions, p.lens = lens, p.news = news;
-    p.posL = pos_l, p.posB = pos_b;
+    p.at = {positions, lens, news, pos_l, pos_b, (int)L};
     p.gain = gain;
     p.E = (int)E, p.rot = (int)rot, p.L = (int)L, p.H = (int)H;
     p.total = L * B;

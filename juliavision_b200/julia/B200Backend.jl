@@ -299,6 +299,18 @@ function rotary!(ctx::Ctx{B200Backend}, plan::RotaryPlan, out, x; lens, news = n
     out
 end
 
+# weight (E,), (E, H), or with split (E, 2): heads up to `split` take its first column.
+function normrotary!(ctx::Ctx{B200Backend}, plan::RotaryPlan, out, x, weight = nothing; eps = 1f-6, split = nothing, lens, news = nothing)
+    E, L, H, B = size(x)
+    check(ccall((:b200_norm_rotary_f16, LIB), Cint,
+                (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Ptr{Cvoid}, Cint, Int64, Int64, Cfloat,
+                 Ptr{Cvoid}, Int64, Cint, Cfloat, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, E, L, H, B, s4(x), s4(out), nullable(weight), weight === nothing ? 0 : dtcode(eltype(weight)),
+                weight === nothing || ndims(weight) == 1 || size(weight, 2) == 1 ? 0 : stride(weight, 2), something(split, -1), eps,
+                pointer(plan.freq), plan.rot, plan.interleaved, plan.gain, C_NULL, 0, 0, pointer(lens), nullable(news)))
+    out
+end
+
 # kind 2: Int8, 3: e4m3 in UInt8 (b200dnn.h); k, v (E, T, H, P), kmax, vmax (H, P) Float32.
 struct Cache8{K}
     k::K

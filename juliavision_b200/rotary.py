@@ -1,7 +1,8 @@
 """Rotary positions for the B200 backend (new surface: the reference has no decoder).
 
 Pair i of a head is turned by position * f_i.  `rotaryplan` makes the frequencies once, in fp64, with the scalings that
-stretch a model over a longer context than it was made for; `rotary_` applies them to (E, L, H, B) views.
+stretch a model over a longer context than it was made for; `rotary_` applies them to (E, L, H, B) views, `normrotary_` behind
+each head's norm in the same pass.
 """
 from __future__ import annotations
 
@@ -14,7 +15,7 @@ import numpy as np
 from . import _lib
 from ._lib import B200Error, check
 from .attention import _s4
-from .context import Ctx, DeviceArray
+from .context import Ctx, DeviceArray, dtcode
 
 
 @dataclass(frozen=True)
@@ -86,6 +87,25 @@ def _counts(name: str, a: Optional[DeviceArray], B: int):
     return a.ptr
 
 
+def _positioned(op: str, out: DeviceArray, x: DeviceArray, positions, lens, news):
+    """The checks of the calls that turn heads: (E, L, H, B), and the strides of `positions`."""
+    if any(a.ndim != 4 or a.dtype != np.float16 for a in (x, out)):
+        raise B200Error(16, f"{op}: x and out must be four-axis fp16 arrays")
+    if x.shape != out.shape:
+        raise B200Error(17, f"{op}: out is {out.shape}, x {x.shape}")
+    E, L, H, B = x.shape
+    pl = pb = 0
+    if positions is not None:
+        if lens is not None or news is not None:
+            raise B200Error(1, f"{op}: positions as well as lens or news")
+        if positions.dtype != np.int32 or positions.ndim != 2 or any(have not in (1, want) for have, want in zip(positions.shape, (L, B))):
+            raise B200Error(16, f"{op}: positions must be an int32 (L, B) array")
+        pl, pb = (0 if n == 1 else s for n, s in zip(positions.shape, positions.strides))
+    elif lens is None:
+        raise B200Error(1, f"{op}: neither positions nor lens")
+    return (E, L, H, B), pl, pb
+
+
 def rotary_(ctx: Ctx, plan: RotaryPlan, out: DeviceArray, x: DeviceArray, positions: Optional[DeviceArray] = None,
             lens: Optional[DeviceArray] = None, news: Optional[DeviceArray] = None) -> DeviceArray:
     """out = x turned by its positions; x and out (E, L, H, B) fp16, E contiguous, any other strides, out x itself or apart from it.
@@ -96,22 +116,41 @@ def rotary_(ctx: Ctx, plan: RotaryPlan, out: DeviceArray, x: DeviceArray, positi
         if rc is not None:
             check(rc)
             return out
-    if any(a.ndim != 4 or a.dtype != np.float16 for a in (x, out)):
-        raise B200Error(16, "rotary!: x and out must be four-axis fp16 arrays")
-    if x.shape != out.shape:
-        raise B200Error(17, f"rotary!: out is {out.shape}, x {x.shape}")
-    E, L, H, B = x.shape
-    pl = pb = 0
-    if positions is not None:
-        if lens is not None or news is not None:
-            raise B200Error(1, "rotary!: positions as well as lens or news")
-        if positions.dtype != np.int32 or positions.ndim != 2 or any(have not in (1, want) for have, want in zip(positions.shape, (L, B))):
-            raise B200Error(16, "rotary!: positions must be an int32 (L, B) array")
-        pl, pb = (0 if n == 1 else s for n, s in zip(positions.shape, positions.strides))
-    elif lens is None:
-        raise B200Error(1, "rotary!: neither positions nor lens")
+    (E, L, H, B), pl, pb = _positioned("rotary!", out, x, positions, lens, news)
     xs, os_ = _s4(x), _s4(out)
     check(_lib.lib().b200_rotary_f16(ctx.handle, E, L, H, B, xs, os_, plan.freq.ptr, plan.rot, int(plan.interleaved), plan.gain,
                                      positions.ptr if positions is not None else None, pl, pb, _counts("lens", lens, B),
                                      _counts("news", news, B)))
+    return out
+
+
+def normrotary_(ctx: Ctx, plan: RotaryPlan, out: DeviceArray, x: DeviceArray, weight: Optional[DeviceArray] = None, eps: float = 1e-6,
+                split: Optional[int] = None, positions: Optional[DeviceArray] = None, lens: Optional[DeviceArray] = None,
+                news: Optional[DeviceArray] = None) -> DeviceArray:
+    """Each head divided by the root of its mean square (and of eps), times `weight`, then turned as `rotary_` turns it, in one pass with
+    one rounding.  `weight`, fp16 or fp32 with E contiguous: (E,) or (E, 1) for all heads, (E, H) a column a head, or with `split`
+    (E, 2): heads before `split` take the first column, the others the second, as queries and keys side by side in one projection do.
+    Everything else as for `rotary_`; a plan of 0 elements norms and turns nothing."""
+    if positions is None:
+        rc = _lib.host().normrotary(ctx.handle, plan, out, x, weight, eps, split, lens, news)
+        if rc is not None:
+            check(rc)
+            return out
+    (E, L, H, B), pl, pb = _positioned("normrotary!", out, x, positions, lens, news)
+    ptr, code, ld, at = None, 0, 0, -1
+    if split is not None and (weight is None or not 0 <= split <= H):
+        raise B200Error(1, f"normrotary!: split at {split} of {H} heads, weight {None if weight is None else weight.shape}")
+    if weight is not None:
+        if weight.dtype not in (np.float16, np.float32) or weight.ndim not in (1, 2):
+            raise B200Error(16, "normrotary!: weight must be an fp16 or fp32 (E,) or (E, heads) array")
+        columns = 1 if weight.ndim == 1 else weight.shape[1]
+        if weight.shape[0] != E or columns != (2 if split is not None else columns if columns == 1 else H):
+            raise B200Error(17, f"normrotary!: weight is {weight.shape} for {H} heads of {E}" + ("" if split is None else f" split at {split}"))
+        if E > 1 and weight.strides[0] != 1:
+            raise B200Error(18, "normrotary!: weight is not contiguous along E")
+        ptr, code, ld, at = weight.ptr, dtcode(weight.dtype), 0 if columns == 1 else weight.strides[1], -1 if split is None else int(split)
+    xs, os_ = _s4(x), _s4(out)
+    check(_lib.lib().b200_norm_rotary_f16(ctx.handle, E, L, H, B, xs, os_, ptr, code, ld, at, float(eps), plan.freq.ptr, plan.rot,
+                                          int(plan.interleaved), plan.gain, positions.ptr if positions is not None else None, pl, pb,
+                                          _counts("lens", lens, B), _counts("news", news, B)))
     return out
