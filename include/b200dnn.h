@@ -231,6 +231,22 @@ int b200_attention_f16_supported(int64_t E, int64_t Lq, int64_t Lk, int64_t H, i
 int b200_attention_f16_route(int64_t E, int64_t Lq, int64_t Lk, int64_t H, int64_t B, const int64_t* qstride,
                              const int64_t* kstride, const int64_t* vstride);
 
+/* ------------------------------------------------- attention of packed sequences */
+/*
+ * out = softmax(scale * Q K') V of B sequences that lie one behind the other: sequence b is rows starts[b] .. starts[b+1]-1 of q and out
+ * (E,N,Hq) and kstarts[b] .. kstarts[b+1]-1 of k and v (E,Nk,H); strides are {E,rows,heads,-}, E contiguous, E <= 128, Hq a multiple of H;
+ * query head i reads key head i / (Hq / H).  A sequence's last row stands at its last key: row i of n rows and m keys sees, when
+ * causal, the keys up to i + m - n, else all m.  A row that sees none comes out as zeros; rows that belong to no sequence are left as they
+ * were.  A key that a row does not see has no part in it, whatever it holds.  q, k and v fp16, out fp16 or fp32; scale is 0 or more.
+ * Scores, softmax and sums are fp32; the weights of the second product are rounded to fp16, up to 2^8 of the heaviest when it came and times 2^7.
+ * starts and kstarts are device arrays of B + 1 numbers; where they are not in order or past the arrays they are cut, and the next b200_sync
+ * reports it (B200_EKERNEL).  out overlaps no operand.  Scratch comes from the context's workspace (20 MB at most, and a copy of each
+ * operand whose pointer or strides are not multiples of 16 bytes).
+ */
+int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, int64_t Hq, int64_t H, int64_t B, const b200_strided4* q,
+                              const b200_strided4* k, const b200_strided4* v, const b200_strided4* out, int out_dtype, float scale,
+                              int causal, const int32_t* starts, const int32_t* kstarts);
+
 /* -------------------------------------------------------------- rotary positions */
 /*
  * (New surface, no reference counterpart: so are the 8-bit cache and the 4-bit products below.)

@@ -6,7 +6,7 @@ libb200dnn.so.  Importing the package does not need a GPU; creating a `Ctx` does
 is no fallback if the library is missing.
 """
 from ._lib import B200Error, SO_PATH, lib
-from .attention import sdpa, sdpa_, sdpaplan
+from .attention import packedsdpa_, sdpa, sdpa_, sdpaplan
 from .kvcache import Cache8, cache8, cacheappend_, cacheread_, cachesdpa_
 from .context import Ctx, DeviceArray, DeviceCaps, Workspace, caps
 from .conv import convolution_, convolutiontranspose_, convsize, convtransposesize, onebyone, shufflecase
@@ -33,5 +33,5 @@ __all__ = [
     "maxpool2d_", "to_copy_", "MMGemvPlan", "foldoutcasts", "foldincasts", "foldbatchnorm", "foldrelu", "hoistcasts", "weightsource", "readsafetensors", "safetensorsnames",
     "Event", "StreamedPass", "Diagnostics", "TwoGemmPlan", "convolutiontranspose_", "convtransposesize", "shufflecase",
     "Cache8", "cache8", "cacheappend_", "cacheread_", "cachesdpa_", "Weight4", "matmul4_", "pack4", "quantise4", "RotaryPlan", "rotary_",
-    "rotaryfrequencies", "rotaryplan", "normrotary_",
+    "rotaryfrequencies", "rotaryplan", "normrotary_", "packedsdpa_",
 ]

@@ -5,6 +5,8 @@ q, k, v are (E, L, H, B) views with any strides along L, H, B (E contiguous); ou
 (E, Lq, H, B).  Non-causal.  `bias` is the additive mask of the mem-efficient variant, fp16 in the
 graph's own (Lk, Lq, H, B) order with size-1 axes broadcasting (attention.jl:55-59); the reference
 declines it on its fused path and runs three passes, here it is added inside the fused kernel.
+
+`packedsdpa_` is the form of a decoder's prompts: sequences of different lengths side by side, causal, with grouped heads.
 """
 from __future__ import annotations
 
@@ -91,3 +93,48 @@ def sdpa(ctx: Ctx, q, k, v, bias=None, scale: Optional[float] = None, out: Optio
         check(rc)
         return out
     return sdpa_(ctx, sdpaplan(ctx, q, k, v, bias), out, q, k, v, bias, scale)
+
+
+def _starts(name: str, a: DeviceArray, B: int) -> int:
+    """First rows of B sequences and the end of the last."""
+    if a.dtype != np.int32 or a.size != B + 1 or not a.isdense():
+        raise B200Error(16, f"packedsdpa!: {name} must be a dense int32 array of {B + 1} rows")
+    return a.ptr
+
+
+def packedsdpa_(ctx: Ctx, out: DeviceArray, q: DeviceArray, k: DeviceArray, v: DeviceArray, starts: DeviceArray,
+                kstarts: Optional[DeviceArray] = None, scale: Optional[float] = None, causal: bool = True) -> DeviceArray:
+    """out = softmax(scale * Q K') V of sequences that lie one behind the other (new surface: the reference pads them).  q and out
+    (E, N, Hq), k and v (E, Nk, H), q, k and v fp16, out fp16 or fp32, E contiguous and at most 128, any other strides; Hq is a multiple of H,
+    query head i reads key head i // (Hq // H).  Sequence b is rows starts[b] .. starts[b + 1] - 1 of q and kstarts[b] .. kstarts[b + 1] - 1
+    (those of `starts` without it) of k and v; both are int32 on the device, one number more than sequences.  Its last row stands at its last
+    key: row i of n sees, when causal, the keys up to i + keys - n, else all of its sequence's.  A row that sees none comes out as zeros;
+    rows of `out` that belong to no sequence are left as they were.  `out` does not overlap q, k or v."""
+    if scale is None and q.ndim == 3 and q.shape[0] > 0:
+        scale = 1.0 / sqrt(q.shape[0])
+    rc = _lib.host().packedsdpa(ctx.handle, out, q, k, v, starts, kstarts, scale, causal)
+    if rc is not None:
+        check(rc)
+        return out
+    if any(a.ndim != 3 or a.dtype != np.float16 for a in (q, k, v)) or out.ndim != 3 or out.dtype not in (np.float16, np.float32):
+        raise B200Error(16, "packedsdpa!: q, k and v must be three-axis fp16 arrays, out one of fp16 or fp32")
+    (E, N, Hq), (_, Nk, H) = q.shape, k.shape
+    if k.shape != v.shape or k.shape[0] != E or out.shape != q.shape or (Hq % H if H else Hq):
+        raise B200Error(17, f"packedsdpa!: q is {q.shape}, k {k.shape}, v {v.shape}, out {out.shape}")
+    B = starts.size - 1
+    if B < 0:
+        raise B200Error(16, "packedsdpa!: starts is empty")
+    if kstarts is None and Nk < N:
+        raise B200Error(17, f"packedsdpa!: {N} rows and {Nk} keys at the same places")
+    at = _starts("starts", starts, B)
+    kat = at if kstarts is None else _starts("kstarts", kstarts, B)
+
+    def s3(a):
+        s = _lib.Strided4()
+        s.ptr = a.ptr
+        for i in range(3):
+            s.stride[i] = a.strides[i]
+        return s
+    check(_lib.lib().b200_attention_packed_f16(ctx.handle, E, N, Nk, Hq, H, B, s3(q), s3(k), s3(v), s3(out), dtcode(out.dtype),
+                                               1.0 if scale is None else float(scale), int(bool(causal)), at, kat))
+    return out

@@ -1,0 +1,943 @@
+// Attention of packed sequences: sequence b has the query rows starts[b] .. starts[b+1] - 1 of q and the keys kstarts[b] ..
+// kstarts[b+1] - 1, query head i reads key head i / (Hq / H), and the last query row stands at the last key:
+//     out = softmax(scale Q K' + mask) V, row i of n seeing, when causal, the keys up to i + keys - n, else all of its sequence's.
+//
+// Tensor-bound for long sequences: 4 E flops a row and visible key on tcgen05, and as many clocks for the exponentials as for the
+// products at E = 128, twice as many at 64.
+//
+// The query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads (G T <= 128), so that keys and
+// values are read once for all of them and a tile's rows lie close together under the causal mask.  A block takes two tiles and walks their keys
+// in blocks of 128: S = Q K' and O += P V with S, P (fp16) and O in tensor memory, Q, K and V by TMA through the caller's strides.
+//
+//   warps 0-3  softmax of tile 0, warps 4-7 of tile 1: one thread a row, its 128 scores in registers
+//   warp 8     finds the block's next part of the work (below), tells the others, and asks for Q, K and V
+//   warps 9, 10  issue one tile's products each:  Q K(0)', P(0) V(0), Q K(1)', ...
+//   warp 11    hands V on to them; where a row does not see a key of the block, it first takes out of the tile what is not finite
+//
+// Lengths are on the device, so the work is listed there: the row pairs of all sequences, longest first, those that are longer than an
+// SM's share cut along their keys (packed_plan_kernel).  Blocks take the list's units in order as they become free; a second launch joins what
+// was cut.  Calls whose pairs all run at once, over few keys, take them as they come and need neither.
+#include <cuda_fp16.h>
+
+#include "internal.h"
+#include "ptx.cuh"
+
+namespace b200 {
+
+constexpr int PK_THREADS = 384;
+constexpr int PK_ROWS = 128, PK_KEYS = 128;      // of a tile
+constexpr int PK_ATOM = 128 * 128;               // 128 rows x 64 fp16
+constexpr int PK_PARTS = 2;                      // parts of the work on their way from warp 8 to the others
+constexpr int PK_SOFTMAX_REGS = 232, PK_OTHER_REGS = 40;
+static_assert(256 * PK_SOFTMAX_REGS + 128 * PK_OTHER_REGS <= PK_THREADS * 168, "what the launch holds");
+constexpr int PK_BUCKETS = 1024;                 // lengths that the list tells apart
+
+struct PackedParams {
+    const __half* v;                   // for what is not finite
+    int64_t vN, vH;
+    void* out;
+    int64_t oN, oH;
+    const int32_t *starts, *kstarts;
+    int N, Nk, B, H, Hq, E;
+    int G, T, groups, share;           // heads and tokens of a tile; tiles' worth of heads of a key head; heads that share a key head
+    Divisor by_g;
+    int causal, out_f32, out_whole;
+    float scale_log2;
+    int heads;                         // H * groups: units of a row pair
+    int most;                          // row pairs that the list has room for: what sequences in order can have
+    int planned;
+    // the list (null without one): entries' first units, [entries + 1]; entries (sequence, pair, blocks of keys, parts); first slots; counters
+    int *unit, *slot, *counts;
+    int4* entry;
+    int* pairs;                        // [B + 1] first pair of a sequence
+    int4* loose;                       // entries in the order of the sequences
+    int4* cut;                         // (entry, head) of what was cut
+    float *part, *part_ml;             // [slots][E / 4][256 rows][4] and [slots][256][2]: reference point, sum
+    int sms;
+    int* d_status;
+};
+enum { PC_NEXT = 0, PC_UNITS = 1, PC_ENTRIES = 2, PC_CUT = 3 };
+
+__device__ __forceinline__ float pk_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pk_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void pk_tmem_st16(uint32_t taddr, const uint32_t* r) {
+    uint32_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = r[i];
+    tmem_st16(taddr, v);
+}
+
+// Where a sequence lies.  Whatever starts and kstarts hold, it is inside the arrays.
+struct PackedSeq {
+    int q0, n, k0, m;      // first row, rows, first key, keys
+    __device__ __forceinline__ void range(const PackedParams& p, const int32_t* s, int b, int most, int& at, int& count) const {
+        int lo = s[b], hi = s[b + 1];
+        if (lo < 0 || hi < lo || hi > most) {
+            atomicCAS(p.d_status, 0, KST_PACKED_STARTS);
+            lo = lo < 0 ? 0 : lo > most ? most : lo;
+            hi = hi < lo ? lo : hi > most ? most : hi;
+        }
+        at = lo, count = hi - lo;
+    }
+    __device__ __forceinline__ void of(const PackedParams& p, int b) {
+        range(p, p.starts, b, p.N, q0, n);
+        range(p, p.kstarts, b, p.Nk, k0, m);
+    }
+    __device__ __forceinline__ int pairs(const PackedParams& p) const { return (n + 2 * p.T - 1) / (2 * p.T); }
+    __device__ __forceinline__ int blocks(const PackedParams& p, int pair) const {   // of keys that some row of the pair sees
+        const int top = (pair + 1) * 2 * p.T < n ? (pair + 1) * 2 * p.T : n;
+        const int seen = p.causal ? m - n + top : m;
+        return seen <= 0 ? 0 : (seen + PK_KEYS - 1) / PK_KEYS;
+    }
+};
+
+// ------------------------------------------------------------------------------------------ the list of the work
+__device__ __forceinline__ int pk_block_scan(int x, int* sums, int& total) {   // exclusive, 1024 threads
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int upto = x;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < 32; ++i) {
+        if (i < warp) before += sums[i];
+        total += sums[i];
+    }
+    return before + upto - x;
+}
+
+__global__ void __launch_bounds__(1024)
+packed_plan_kernel(const PackedParams p) {
+    __shared__ int sums[32], bucket[PK_BUCKETS];
+    __shared__ unsigned long long blocks;
+    const int tid = threadIdx.x;
+    grid_dep_wait();
+    grid_dep_launch();
+    // pairs of each sequence
+    int entries = 0;
+    for (int base = 0; base < p.B; base += 1024) {
+        int n = 0, total;
+        if (base + tid < p.B) {
+            PackedSeq s;
+            s.of(p, base + tid);
+            n = s.pairs(p);
+        }
+        const int at = pk_block_scan(n, sums, total);
+        if (base + tid < p.B) p.pairs[base + tid] = entries + at;
+        entries = entries + total < p.most ? entries + total : p.most;      // sequences that overlap, which has been reported
+    }
+    if (tid == 0) {
+        p.pairs[p.B] = entries;
+        blocks = 0;
+    }
+    bucket[tid] = 0;
+    __syncthreads();
+    unsigned long long mine = 0;
+    for (int e = tid; e < entries; e += 1024) {
+        int lo = 0, hi = p.B;          // the last sequence whose first pair is at or before e
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (p.pairs[mid] <= e) lo = mid;
+            else hi = mid;
+        }
+        PackedSeq s;
+        s.of(p, lo);
+        const int pair = e - p.pairs[lo], n = s.blocks(p, pair);
+        p.loose[e] = make_int4(lo, pair, n, 1);
+        mine += n > 0 ? n : 1;
+    }
+    if (mine) atomicAdd(&blocks, mine);
+    __syncthreads();
+    const unsigned long long all = blocks * p.heads;
+    for (int e = tid; e < entries; e += 1024) {
+        int4 x = p.loose[e];
+        // as many parts as it has SMs' shares: the parts of all that is cut are no more than the SMs
+        const int s = all > 0 ? (int)((unsigned long long)x.z * p.sms / all) : 1;
+        x.w = s > 1 ? s < x.z ? s : x.z : 1;
+        p.loose[e] = x;
+        const int size = x.z / x.w;
+        atomicAdd(&bucket[size < PK_BUCKETS ? PK_BUCKETS - 1 - size : 0], 1);
+    }
+    __syncthreads();
+    {
+        int total;
+        const int n = bucket[tid], at = pk_block_scan(n, sums, total);
+        __syncthreads();
+        bucket[tid] = at;
+    }
+    __syncthreads();
+    for (int e = tid; e < entries; e += 1024) {
+        const int4 x = p.loose[e];
+        const int size = x.z / x.w;
+        p.entry[atomicAdd(&bucket[size < PK_BUCKETS ? PK_BUCKETS - 1 - size : 0], 1)] = x;
+    }
+    __syncthreads();
+    int units = 0, slots = 0, cuts = 0;
+    for (int base = 0; base < entries; base += 1024) {
+        const int e = base + tid, parts = e < entries ? p.entry[e].w : 0;
+        int total;
+        int at = pk_block_scan(parts * p.heads, sums, total);
+        if (e < entries) p.unit[e] = units + at;
+        units += total;
+        at = pk_block_scan(parts > 1 ? parts * p.heads : 0, sums, total);
+        if (e < entries) p.slot[e] = slots + at;
+        slots += total;
+        at = pk_block_scan(parts > 1 ? p.heads : 0, sums, total);
+        if (parts > 1)
+            for (int h = 0; h < p.heads; ++h) p.cut[cuts + at + h] = make_int4(e, h, 0, 0);
+        cuts += total;
+    }
+    if (tid == 0) {
+        p.unit[entries] = units;
+        p.counts[PC_NEXT] = 0;
+        p.counts[PC_UNITS] = units;
+        p.counts[PC_ENTRIES] = entries;
+        p.counts[PC_CUT] = cuts;
+    }
+}
+
+// A block's work: some of the key blocks of two tiles.
+struct PackedPart {
+    int q0, n, k0, m;            // the sequence
+    int h, g0, token;            // key head, first of its query heads, first token of tile 0
+    int j0, nblk, slot, more;    // key blocks; slot < 0: the whole of the item
+};
+
+__device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, int b, int pair, int head, int part, int parts, int slot) {
+    PackedSeq s;
+    s.of(p, b);
+    x.q0 = s.q0, x.n = s.n, x.k0 = s.k0, x.m = s.m;
+    x.h = head / p.groups, x.g0 = (head - x.h * p.groups) * p.G;
+    x.token = pair * 2 * p.T;
+    const int blocks = s.blocks(p, pair);
+    x.j0 = (int)((long long)part * blocks / parts);
+    x.nblk = (int)((long long)(part + 1) * blocks / parts) - x.j0;
+    x.slot = parts > 1 ? slot + head * parts + part : -1;
+    x.more = 1;
+}
+
+// Unit `unit` of the list, found by a whole warp.
+__device__ __forceinline__ bool pk_listed(const PackedParams& p, int unit, PackedPart& x) {
+    const int lane = threadIdx.x & 31;
+    if (unit >= p.counts[PC_UNITS]) return false;
+    int lo = 0, hi = p.counts[PC_ENTRIES];          // the last entry whose first unit is at or before this one
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const bool before = at < hi && p.unit[at] <= unit;
+        const int k = 31 - __clz(__ballot_sync(0xffffffffu, before));
+        lo += k * step;
+        hi = lo + step < hi ? lo + step : hi;
+    }
+    const int4 e = p.entry[lo];
+    const int rel = unit - p.unit[lo], part = rel / p.heads;
+    pk_part(p, x, e.x, e.y, rel - part * p.heads, part, e.w, p.slot[lo]);
+    return true;
+}
+// Pair `pair` of all sequences' in order, without a list.
+__device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, PackedPart& x) {
+    const int lane = threadIdx.x & 31, pair = unit / p.heads;
+    int before = 0;
+    for (int base = 0; base < p.B; base += 32) {
+        int n = 0;
+        if (base + lane < p.B) {
+            PackedSeq s;
+            s.of(p, base + lane);
+            n = s.pairs(p);
+        }
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + upto > pair);
+        if (past) {
+            const int k = __ffs(past) - 1;
+            pk_part(p, x, base + k, pair - before - __shfl_sync(0xffffffffu, upto - n, k), unit - pair * p.heads, 0, 1, 0);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+template <int EP> struct PkCfg {
+    static constexpr int ATOMS = EP / 64;
+    static constexpr int SIDE = ATOMS * PK_ATOM;                 // an operand tile
+    static constexpr bool OWN_P = EP == 64;                      // P beside S in tensor memory; else over S
+    static constexpr int STAGES = OWN_P ? 10 : 5;                // K(0), V(0), K(1), ...
+    static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_BARS = S_KV + STAGES * SIDE;
+    static constexpr int BARRIERS = 2 * 2 + 3 * STAGES + 2 * 6 + 2 * PK_PARTS;
+    static constexpr int S_PART = S_BARS + (BARRIERS + 1) * 8;
+    static constexpr int SMEM = S_PART + PK_PARTS * (int)sizeof(PackedPart) + 16;
+    static constexpr int O_COL = 2 * PK_KEYS, P_COL = O_COL + 2 * EP;
+    static_assert(SMEM <= 232448, "shared memory over budget");
+};
+
+__device__ __forceinline__ void pk_store8(const PackedParams& p, int64_t at, int count, const float (&v)[8]) {   // eight results of a row, or fewer
+    if (p.out_whole && count >= 8) {
+        if (p.out_f32) {
+            float4* d = reinterpret_cast<float4*>((float*)p.out + at);
+            d[0] = make_float4(v[0], v[1], v[2], v[3]);
+            d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint4 w;
+            __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            *reinterpret_cast<uint4*>((__half*)p.out + at) = w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < count) {
+            if (p.out_f32) ((float*)p.out)[at + i] = v[i];
+            else ((__half*)p.out)[at + i] = __float2half_rn(v[i]);
+        }
+}
+
+template <int EP>
+__global__ void __launch_bounds__(PK_THREADS, 1)
+attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_constant__ CUtensorMap tmapK,
+                        const __grid_constant__ CUtensorMap tmapV, const PackedParams p) {
+    using Cfg = PkCfg<EP>;
+    constexpr int STAGES = Cfg::STAGES, ATOMS = Cfg::ATOMS;
+    constexpr bool OWN_P = Cfg::OWN_P, HALVES = !OWN_P;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if ((smem_u32(smem) & 1023u) != 0) {   // uniform across the grid
+        if (threadIdx.x == 0) atomicCAS(p.d_status, 0, KST_SMEM_LAYOUT);
+        return;
+    }
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::S_BARS);
+    uint64_t* q_full = bars;                       // [2]
+    uint64_t* q_empty = q_full + 2;                // [2] a part's last Q K' is done
+    uint64_t* full = q_empty + 2;                  // [STAGES] K or V has landed
+    uint64_t* ready = full + STAGES;               // [STAGES, in the order of the blocks] V may be multiplied
+    uint64_t* empty = ready + STAGES;              // [STAGES] one arrival a tile
+    uint64_t* s_full = empty + STAGES;             // [2] a tile's scores are there
+    uint64_t* s_empty = s_full + 2;                // [2] and in registers
+    uint64_t* p_half = s_empty + 2;                // [2] half of its P
+    uint64_t* p_full = p_half + 2;                 // [2] all of it
+    uint64_t* pv_done = p_full + 2;                // [2] its last product
+    uint64_t* exp_turn = pv_done + 2;              // [2] whose turn it is to run its exponentials
+    uint64_t* a_full = exp_turn + 2;               // [PK_PARTS] a part of the work
+    uint64_t* a_empty = a_full + PK_PARTS;         // every other warp
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(a_empty + PK_PARTS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    PackedPart* part = reinterpret_cast<PackedPart*>(smem + Cfg::S_PART);
+    int* odd = reinterpret_cast<int*>(part + PK_PARTS);   // [PK_PARTS] the first key block of a part from which something was taken out
+    static_assert(Cfg::BARRIERS == 4 + 3 * STAGES + 12 + 2 * PK_PARTS, "barriers counted by the layout");
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 1);
+            mbar_init(&q_empty[t], 1);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&s_empty[t], 4);
+            mbar_init(&p_half[t], 4);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&pv_done[t], 1);
+            mbar_init(&exp_turn[t], 4);
+        }
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&ready[s], 1);
+            mbar_init(&empty[s], 2);
+        }
+        for (int s = 0; s < PK_PARTS; ++s) {
+            mbar_init(&a_full[s], 1);
+            mbar_init(&a_empty[s], PK_THREADS / 32 - 1);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tmap(&tmapQ);
+        prefetch_tmap(&tmapK);
+        prefetch_tmap(&tmapV);
+    }
+    if (warp == 8) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    grid_dep_wait();
+    grid_dep_launch();
+
+    // A warp leaves a wait that runs out as one: lanes that went on alone would wait for the others in the next vote, for good.
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.d_status, code, abort_flag));
+    };
+    PackedPart it;
+    int parts_seen = 0;
+    auto take = [&]() -> int {        // the next part: its place in the ring, or -1
+        const int s = parts_seen % PK_PARTS;
+        if (!wait(&a_full[s], (uint32_t)((parts_seen / PK_PARTS) & 1), KST_WAIT_FULL)) return -1;
+        it = part[s];
+        // the same for all lanes, which the compiler sees: what depends on them stays in the warp's own registers
+        for (int* v : {&it.q0, &it.n, &it.k0, &it.m, &it.h, &it.g0, &it.token, &it.j0, &it.nblk, &it.slot, &it.more})
+            *v = __shfl_sync(0xffffffffu, *v, 0);
+        return it.more ? s : -1;
+    };
+    auto done_with = [&](int s) {     // nobody of this warp reads the part's place any more
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_empty[s]);
+        ++parts_seen;
+    };
+    // The last key that every row of both tiles sees; blocks that end behind it are masked.
+    auto all_see = [&](int token) { return p.causal && it.m - it.n + token < it.m - 1 ? it.m - it.n + token : it.m - 1; };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OTHER_REGS));
+        if (warp == 8) {
+            // -------------------------------------------------- the work, and its operands
+            int unit = blockIdx.x, i = 0, tiles[2] = {0, 0};       // sides asked for so far; parts of a tile
+            bool ok = true;
+            for (int n = 0; ok; ++n) {
+                it.more = 0;
+                const bool some = p.planned ? pk_listed(p, unit, it) : n == 0 && pk_direct(p, unit, it);
+                if (!some) it.more = 0;
+                const int s = n % PK_PARTS;
+                if (!wait(&a_empty[s], (uint32_t)((n / PK_PARTS) & 1) ^ 1, KST_WAIT_EMPTY)) break;
+                if (lane == 0) {
+                    part[s] = it;
+                    odd[s] = 0x7fffffff;
+                    mbar_arrive(&a_full[s]);
+                }
+                __syncwarp();
+                if (!some) break;
+                if (p.planned) {          // on its way while this part's operands are asked for
+                    if (lane == 0) unit = gridDim.x + atomicAdd(&p.counts[PC_NEXT], 1);
+                    unit = __shfl_sync(0xffffffffu, unit, 0);
+                }
+                if (it.nblk == 0) continue;
+                for (int t = 0; ok && t < 2; ++t) {
+                    if (it.token + t * p.T >= it.n) continue;
+                    ok = wait(&q_empty[t], (uint32_t)(tiles[t] & 1) ^ 1, KST_WAIT_EMPTY);
+                    ++tiles[t];
+                    if (ok && elect_one()) {
+                        mbar_arrive_expect_tx(&q_full[t], ATOMS * 128 * p.G * p.T);
+#pragma unroll
+                        for (int a = 0; a < ATOMS; ++a)
+                            tma_load_3d(smem + Cfg::S_Q + t * Cfg::SIDE + a * PK_ATOM, &tmapQ, &q_full[t], a * 64, it.h * p.share + it.g0,
+                                        it.q0 + it.token + t * p.T);
+                    }
+                    __syncwarp();
+                }
+                for (int j = 0; ok && j < 2 * it.nblk; ++j, ++i) {
+                    const int st = i % STAGES;
+                    ok = wait(&empty[st], (uint32_t)((i / STAGES) & 1) ^ 1, KST_WAIT_EMPTY);
+                    if (ok && elect_one()) {
+                        mbar_arrive_expect_tx(&full[st], Cfg::SIDE);
+#pragma unroll
+                        for (int a = 0; a < ATOMS; ++a)
+                            tma_load_3d(smem + Cfg::S_KV + st * Cfg::SIDE + a * PK_ATOM, j & 1 ? &tmapV : &tmapK, &full[st], a * 64, it.h,
+                                        it.k0 + (it.j0 + (j >> 1)) * PK_KEYS);
+                    }
+                    __syncwarp();
+                }
+            }
+        } else if (warp == 11) {
+            // -------------------------------------------------- values that may be multiplied
+            int i = 0;
+            bool ok = true;
+            for (int s; ok && (s = take()) >= 0; done_with(s)) {
+                const int see = all_see(it.token);
+                int first = 0x7fffffff;
+                for (int j = 0; ok && j < it.nblk; ++j, i += 2) {
+                    const int st = (i + 1) % STAGES, key0 = (it.j0 + j) * PK_KEYS;
+                    ok = wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
+                    if (!ok) break;
+                    if (key0 + PK_KEYS - 1 > see) {       // some row does not see some key: 0 times what is not finite is no zero
+                        uint4* tile = reinterpret_cast<uint4*>(smem + Cfg::S_KV + st * Cfg::SIDE);
+                        bool mine = false;
+#pragma unroll 4
+                        for (int c = lane; c < Cfg::SIDE / 16; c += 32) {
+                            uint4 x = tile[c];
+                            const uint32_t hit = ((x.x & 0x7fff7fffu) + 0x04000400u) | ((x.y & 0x7fff7fffu) + 0x04000400u) |
+                                                 ((x.z & 0x7fff7fffu) + 0x04000400u) | ((x.w & 0x7fff7fffu) + 0x04000400u);
+                            if (hit & 0x80008000u) {
+                                uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint32_t bad = ((w[k] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                                    w[k] &= ~((bad >> 15) * 0xffffu);
+                                }
+                                tile[c] = x;
+                                mine |= key0 + (c % (PK_ATOM / 16)) / 8 < it.m;      // a key of this sequence
+                            }
+                        }
+                        if (__any_sync(0xffffffffu, mine) && key0 < first) {
+                            first = key0;
+                            if (lane == 0) odd[s] = it.j0 + j;
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(&ready[(i >> 1) % STAGES]);
+                }
+            }
+        } else {
+            // -------------------------------------------------- issuers: the whole warp waits, one thread issues
+            const int t = warp - 9;
+            constexpr uint32_t idesc_s = make_idesc_f16(PK_ROWS, PK_KEYS, 0, 0);
+            const int steps = (p.E + 15) / 16;                       // past the head dim both operands are zeros
+            const uint32_t idesc_o = make_idesc_f16(PK_ROWS, 16 * steps, 0, 1);
+            constexpr uint64_t kdesc0 = make_smem_desc(16, 1024);
+            constexpr uint64_t vdesc0 = make_smem_desc(PK_ATOM, 1024);
+            const uint32_t q_addr = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE), kv_addr = smem_u32(smem + Cfg::S_KV);
+            const uint32_t s_tmem = tmem_base + t * PK_KEYS, o_tmem = tmem_base + Cfg::O_COL + t * EP;
+            const uint32_t p_tmem = OWN_P ? tmem_base + Cfg::P_COL + t * 64 : s_tmem;
+            int i = 0, busy = 0, parts = 0;      // sides of the ring before this part; blocks of this tile; parts of this tile
+            auto issue_qk = [&](int j) -> bool {
+                const int st = (i + 2 * j) % STAGES;
+                if (!wait(&full[st], (uint32_t)(((i + 2 * j) / STAGES) & 1), KST_WAIT_FULL)) return false;
+                if (OWN_P && busy + j > 0 && !wait(&s_empty[t], (uint32_t)((busy + j - 1) & 1), KST_WAIT_SOFTMAX)) return false;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t k_addr = kv_addr + st * Cfg::SIDE;
+#pragma unroll
+                    for (int k = 0; k < EP / 16; ++k) {
+                        if (k >= steps) break;
+                        const uint32_t in = (uint32_t)(k >> 2) * PK_ATOM + (uint32_t)(k & 3) * 32;
+                        umma_ss(s_tmem, smem_desc_at(kdesc0, q_addr + in), smem_desc_at(kdesc0, k_addr + in), idesc_s, k != 0);
+                    }
+                    umma_commit(&s_full[t]);
+                    umma_commit(&empty[st]);
+                    if (j == it.nblk - 1) umma_commit(&q_empty[t]);
+                }
+                __syncwarp();
+                return true;
+            };
+            auto issue_pv = [&](int j, int st, int k0, int k1) {
+                const uint32_t v_addr = kv_addr + st * Cfg::SIDE;
+#pragma unroll
+                for (int k = k0; k < k1; ++k) umma_ts(o_tmem, p_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
+            };
+            bool ok = true;
+            for (int s; ok && (s = take()) >= 0; done_with(s)) {
+                if (it.token + t * p.T >= it.n) {      // no rows: what the other tile reads is released from here too
+                    for (int j = 0; ok && j < 2 * it.nblk; ++j) {
+                        const int st = (i + j) % STAGES;
+                        const int vb = (i + j) >> 1;
+                        ok = j & 1 ? wait(&ready[vb % STAGES], (uint32_t)((vb / STAGES) & 1), KST_WAIT_FULL)
+                                   : wait(&full[st], (uint32_t)(((i + j) / STAGES) & 1), KST_WAIT_FULL);
+                        if (ok && elect_one()) mbar_arrive(&empty[st]);
+                        __syncwarp();
+                    }
+                    i += 2 * it.nblk;
+                    continue;
+                }
+                if (it.nblk == 0) continue;
+                ok = wait(&q_full[t], (uint32_t)(parts & 1), KST_WAIT_FULL) && issue_qk(0);
+                for (int j = 0; ok && j < it.nblk; ++j) {
+                    if (OWN_P && j + 1 < it.nblk && !issue_qk(j + 1)) { ok = false; break; }
+                    const int st = (i + 2 * j + 1) % STAGES, vb = (i >> 1) + j;
+                    const uint32_t ph = (uint32_t)((busy + j) & 1);
+                    ok = wait(&ready[vb % STAGES], (uint32_t)((vb / STAGES) & 1), KST_WAIT_FULL);
+                    if (ok && HALVES) {
+                        ok = wait(&p_half[t], ph, KST_WAIT_SOFTMAX);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) issue_pv(j, st, 0, 4);
+                        __syncwarp();
+                    }
+                    ok = ok && wait(&p_full[t], ph, KST_WAIT_SOFTMAX);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        issue_pv(j, st, HALVES ? 4 : 0, 8);
+                        umma_commit(&pv_done[t]);
+                        umma_commit(&empty[st]);
+                    }
+                    __syncwarp();
+                    if (!OWN_P && j + 1 < it.nblk) ok = issue_qk(j + 1);   // over P(j): after the product that reads it, in issue order
+                }
+                i += 2 * it.nblk, busy += it.nblk, ++parts;
+            }
+        }
+    } else {
+        // ------------------------------------------------------ softmax and results
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PK_SOFTMAX_REGS));
+        const int t = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lane_base = uint32_t(quad * 32) << 16;
+        const uint32_t s_tmem = tmem_base + lane_base + t * PK_KEYS, o_tmem = tmem_base + lane_base + Cfg::O_COL + t * EP;
+        const uint32_t p_tmem = OWN_P ? tmem_base + lane_base + Cfg::P_COL + t * 64 : s_tmem;
+        const int l0 = p.by_g.div(row), g = row - l0 * p.G;       // the row's token and head in its tile
+        int busy = 0, turns = 0;          // blocks of this tile, of both tiles, before this one
+        bool ok = true;
+        for (int s; ok && (s = take()) >= 0; done_with(s)) {
+            if (it.token + t * p.T >= it.n) continue;
+            const int l = it.token + t * p.T + l0;                                   // its token in the sequence
+            const bool live = l0 < p.T && l < it.n && it.g0 + g < p.share;
+            const int last = p.causal && it.m - it.n + l < it.m - 1 ? it.m - it.n + l : it.m - 1;   // the last key this row sees
+            const int see = all_see(it.token + t * p.T);
+            float m_run = -INFINITY, l_run = 0.f;
+            const bool pingpong = it.token + p.T < it.n;
+            const uint64_t k2 = pack2(p.scale_log2, p.scale_log2);
+            for (int j = 0; ok && j < it.nblk; ++j, ++busy) {
+                const int key0 = (it.j0 + j) * PK_KEYS;
+                ok = wait(&s_full[t], (uint32_t)(busy & 1), KST_WAIT_TMEM_FULL);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t x[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld32(s_tmem + i * 32, x[i]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) asm volatile("" : "+r"(x[i][u]));   // in registers from here on
+                if (OWN_P) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_empty[t]);
+                }
+                if (key0 + PK_KEYS - 1 > see) {
+                    const int seen = last - key0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 32; ++u)
+                            if (i * 32 + u > seen) x[i][u] = 0xff800000u;
+                }
+                auto highest = [&]() -> float {
+                    float a = -INFINITY, b = -INFINITY, c = -INFINITY, d = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 32; u += 8) {
+                            a = pk_max3(a, __uint_as_float(x[i][u]), __uint_as_float(x[i][u + 1]));
+                            b = pk_max3(b, __uint_as_float(x[i][u + 2]), __uint_as_float(x[i][u + 3]));
+                            c = pk_max3(c, __uint_as_float(x[i][u + 4]), __uint_as_float(x[i][u + 5]));
+                            d = pk_max3(d, __uint_as_float(x[i][u + 6]), __uint_as_float(x[i][u + 7]));
+                        }
+                    return fmaxf(fmaxf(a, b), fmaxf(c, d)) * p.scale_log2;
+                };
+                // Any reference point m gives the same quotient; it follows the maximum lazily, only when that has grown by more than 2^8.
+                // P goes in times 2^7, so that fp16 holds weights down to 2^-31 of the heaviest key's.
+                const float top = highest();
+                const float m_new = top > m_run + 8.f ? top : m_run;
+                if (OWN_P && j > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);
+                if (!ok) break;
+                if (__any_sync(0xffffffffu, m_new != m_run)) {
+                    const float alpha = m_run == m_new ? 1.f : pk_ex2(m_run - m_new);
+                    l_run *= alpha;
+                    if (j > 0) {          // the last P V is done: these scores were issued after it, or it has been waited for
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int i = 0; i < EP / 16; ++i) {
+                            uint32_t o16[16];
+                            tmem_ld16(o_tmem + i * 16, o16);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) o16[u] = __float_as_uint(__uint_as_float(o16[u]) * alpha);
+                            tmem_st16(o_tmem + i * 16, o16);
+                        }
+                        tmem_wait_st();
+                    }
+                    m_run = m_new;
+                }
+                if (pingpong && (t == 1 || turns > 0) &&
+                    !wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), KST_WAIT_SOFTMAX)) { ok = false; break; }
+                const float m_sub = m_new == -INFINITY ? 0.f : 7.f - m_new;
+                const uint64_t a2 = pack2(m_sub, m_sub);
+                uint64_t sum0 = pack2(0.f, 0.f), sum1 = pack2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        float e0, e1;
+                        unpack2(fma2(pack2(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1])), k2, a2), e0, e1);
+                        e0 = pk_ex2(e0), e1 = pk_ex2(e1);
+                        if (u & 1) sum1 = add2(sum1, pack2(e0, e1));
+                        else sum0 = add2(sum0, pack2(e0, e1));
+                        const __half2 h = __floats2half2_rn(e0, e1);
+                        pk[u] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                    pk_tmem_st16(p_tmem + i * 16, pk);
+                    if (HALVES && i == 1) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_half[t]);
+                    }
+                }
+                if (pingpong) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&exp_turn[1 - t]);
+                    ++turns;
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+                float s0, s1;
+                unpack2(add2(sum0, sum1), s0, s1);
+                l_run += s0 + s1;
+            }
+            if (ok && it.nblk > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);
+            if (!ok) break;
+            tc_fence_after();
+            const float f = it.slot >= 0 || l_run == 0.f ? 1.f : 1.f / l_run;
+            const int64_t at = (int64_t)(it.q0 + l) * p.oN + (int64_t)(it.h * p.share + it.g0 + g) * p.oH;
+            const int prow = t * PK_ROWS + row;
+            const int bad = *reinterpret_cast<volatile int*>(&odd[s]);      // written before the last P V was issued
+#pragma unroll 1
+            for (int i = 0; i < EP / 16; ++i) {
+                uint32_t o16[16];
+                __syncwarp();
+                if (it.nblk > 0) {
+                    tmem_ld16(o_tmem + i * 16, o16);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) o16[u] = 0;
+                }
+                if (!live || i * 16 >= p.E) continue;
+                float v[2][8];
+#pragma unroll
+                for (int u = 0; u < 16; ++u) v[u >> 3][u & 7] = __uint_as_float(o16[u]) * f;
+                if (bad != 0x7fffffff) {        // what was taken out, for those who see it
+                    const int end = (it.j0 + it.nblk) * PK_KEYS - 1 < last ? (it.j0 + it.nblk) * PK_KEYS - 1 : last;
+#pragma unroll 1
+                    for (int key = bad * PK_KEYS; key <= end; ++key) {
+                        const __half* q = p.v + (int64_t)(it.k0 + key) * p.vN + it.h * p.vH + i * 16;
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            if (i * 16 + u >= p.E) break;
+                            const float y = __half2float(q[u]);
+                            if (!(fabsf(y) < INFINITY)) v[u >> 3][u & 7] += y;
+                        }
+                    }
+                }
+                if (it.slot >= 0) {
+                    float4* d = reinterpret_cast<float4*>(p.part + (int64_t)it.slot * (2 * PK_ROWS * EP)) + i * 4 * (2 * PK_ROWS) + prow;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) d[u * 2 * PK_ROWS] = make_float4(v[u >> 1][(u & 1) * 4], v[u >> 1][(u & 1) * 4 + 1], v[u >> 1][(u & 1) * 4 + 2], v[u >> 1][(u & 1) * 4 + 3]);
+                } else {
+                    pk_store8(p, at + i * 16, p.E - i * 16, v[0]);
+                    pk_store8(p, at + i * 16 + 8, p.E - i * 16 - 8, v[1]);
+                }
+            }
+            if (live && it.slot >= 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)it.slot * 2 * PK_ROWS + prow) * 2) = make_float2(m_run, l_run);
+            tc_fence_before();           // the next part's first P V writes O over
+        }
+    }
+    if (*abort_flag) {
+        for (int i = 0; i < 4; ++i) __nanosleep(1000000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// The parts of what was cut, sixteen elements of a row a thread, in the order of the keys.
+template <int EP>
+__global__ void __launch_bounds__(256)
+packed_join_kernel(const PackedParams p) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int i = blockIdx.x / (EP / 16), e = (int)(blockIdx.x % (EP / 16)) * 16, prow = threadIdx.x;
+    if (i >= p.counts[PC_CUT] || e >= p.E) return;
+    const int4 at = p.cut[i], x = p.entry[at.x];
+    PackedSeq s;
+    s.of(p, x.x);
+    const int h = at.y / p.groups, g0 = (at.y - h * p.groups) * p.G;
+    const int t = prow / PK_ROWS, row = prow - t * PK_ROWS, l0 = p.by_g.div(row), g = row - l0 * p.G, l = (x.y * 2 + t) * p.T + l0;
+    if (l0 >= p.T || l >= s.n || g0 + g >= p.share) return;
+    const int64_t slot = p.slot[at.x] + at.y * x.w;
+    auto stat = [&](int w) { return *reinterpret_cast<const float2*>(p.part_ml + ((slot + w) * 2 * PK_ROWS + prow) * 2); };
+    float M = -INFINITY, sum = 0.f, v[2][8] = {};
+    for (int w = 0; w < x.w; ++w) M = fmaxf(M, stat(w).x);
+    for (int w = 0; w < x.w; ++w) {
+        const float2 ml = stat(w);
+        const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
+        const float4* y = reinterpret_cast<const float4*>(p.part + (slot + w) * (2 * PK_ROWS * EP)) + e / 4 * (2 * PK_ROWS) + prow;
+        sum = fmaf(ml.y, f, sum);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float4 a = y[u * 2 * PK_ROWS];
+            float* d = &v[u >> 1][(u & 1) * 4];
+            d[0] = fmaf(a.x, f, d[0]), d[1] = fmaf(a.y, f, d[1]), d[2] = fmaf(a.z, f, d[2]), d[3] = fmaf(a.w, f, d[3]);
+        }
+    }
+    const float inv = sum == 0.f ? 1.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k >> 3][k & 7] *= inv;
+    const int64_t to = (int64_t)(s.q0 + l) * p.oN + (int64_t)(h * p.share + g0 + g) * p.oH + e;
+    pk_store8(p, to, p.E - e, v[0]);
+    pk_store8(p, to + 8, p.E - e - 8, v[1]);
+}
+
+// An operand whose rows a tensor map cannot express, brought to rows of E8 elements: eight elements a thread.
+__global__ void __launch_bounds__(256)
+packed_rows_kernel(const __half* x, int64_t xN, int64_t xH, __half* to, int E, int E8, int H, int64_t total) {
+    grid_dep_wait();
+    grid_dep_launch();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int per = E8 / 8, c = (int)(i % per);
+    const int64_t row = i / per, n = row / H;
+    const __half* q = x + n * xN + (row - n * H) * xH + c * 8;
+    __align__(16) __half v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c * 8 + k < E ? q[k] : __half(0.f);
+    *reinterpret_cast<uint4*>(to + row * E8 + c * 8) = *reinterpret_cast<const uint4*>(v);
+}
+
+struct PackedOperand {
+    const __half* ptr;
+    int64_t sN, sH;
+};
+
+template <int EP>
+static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, const PackedOperand& k, const PackedOperand& v, int64_t items, int64_t entries) {
+    using Cfg = PkCfg<EP>;
+    auto kern = attention_packed_kernel<EP>;
+    static std::atomic<uint64_t> asked{0};
+    B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
+    CUtensorMap tq, tk, tv;
+    auto map = [&](CUtensorMap* m, const PackedOperand& a, int64_t heads, int64_t rows, uint32_t box_h, uint32_t box_n) {
+        const uint64_t dims[3] = {(uint64_t)p.E, (uint64_t)heads, (uint64_t)rows};
+        const uint64_t strides[2] = {(uint64_t)a.sH * 2, (uint64_t)a.sN * 2};
+        const uint32_t box[3] = {64, box_h, box_n};
+        return make_tmap(ctx, m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    const int64_t Nk = p.Nk > 0 ? p.Nk : 1;           // without keys the maps are over q, and not read through
+    int rc = map(&tq, q, p.Hq, p.N, p.G, p.T);
+    if (!rc) rc = map(&tk, k, p.H, Nk, 1, PK_KEYS);
+    if (!rc) rc = map(&tv, v, p.H, Nk, 1, PK_KEYS);
+    if (rc) return rc;
+    const int64_t sms = ctx->prop.multiProcessorCount;
+    p.sms = (int)sms, p.most = (int)entries;
+    p.planned = items > sms || p.Nk > 16 * PK_KEYS;
+    const int64_t slots = sms, rows = slots * 2 * PK_ROWS;
+    if (p.planned) {
+        void* ws = nullptr;
+        const size_t list = (size_t)(entries + 1) * (2 * sizeof(int4) + 2 * sizeof(int)) + (p.B + 1) * sizeof(int) + slots * sizeof(int4) + 64 + 16 * 8;
+        rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float) + list, &ws);
+        if (rc) return rc;
+        uint8_t* at = static_cast<uint8_t*>(ws);
+        auto room = [&](size_t bytes) {
+            uint8_t* r = at;
+            at += (bytes + 15) / 16 * 16;
+            return (void*)r;
+        };
+        p.part = (float*)room(rows * EP * sizeof(float));
+        p.part_ml = (float*)room(rows * 2 * sizeof(float));
+        p.entry = (int4*)room((entries + 1) * sizeof(int4));
+        p.loose = (int4*)room((entries + 1) * sizeof(int4));
+        p.cut = (int4*)room(slots * sizeof(int4));
+        p.unit = (int*)room((entries + 1) * sizeof(int));
+        p.slot = (int*)room((entries + 1) * sizeof(int));
+        p.pairs = (int*)room((p.B + 1) * sizeof(int));
+        p.counts = (int*)room(64);
+        B200_CUDA(launch_dep(packed_plan_kernel, dim3(1), dim3(1024), 0, ctx->stream, 1, p));
+        ctx->launches++;
+    }
+    const int64_t grid = p.planned ? sms : items;
+    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(PK_THREADS), Cfg::SMEM, ctx->stream, 1, tq, tk, tv, p));
+    ctx->launches++;
+    if (p.planned) {
+        B200_CUDA(launch_dep(packed_join_kernel<EP>, dim3((unsigned)(sms / 2 * (EP / 16))), dim3(256), 0, ctx->stream, 1, p));
+        ctx->launches++;
+    }
+    return B200_OK;
+}
+
+} // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, int64_t Hq, int64_t H, int64_t B, const b200_strided4* q,
+                              const b200_strided4* k, const b200_strided4* v, const b200_strided4* out, int out_dtype, float scale,
+                              int causal, const int32_t* starts, const int32_t* kstarts) {
+    B200_REQUIRE(ctx && q && k && v && out, B200_EINVAL, "attention_packed: null argument");
+    B200_REQUIRE(E >= 0 && N >= 0 && Nk >= 0 && Hq >= 0 && H >= 0 && B >= 0, B200_EINVAL, "attention_packed: E=%lld N=%lld Nk=%lld Hq=%lld H=%lld B=%lld",
+                 (long long)E, (long long)N, (long long)Nk, (long long)Hq, (long long)H, (long long)B);
+    B200_REQUIRE(out_dtype == B200_F16 || out_dtype == B200_F32, B200_DECLINE_ELTYPE, "attention_packed: result type %d", out_dtype);
+    B200_REQUIRE(scale >= 0.f && scale < INFINITY, B200_EINVAL, "attention_packed: scale %g", scale);
+    B200_REQUIRE(H > 0 ? Hq % H == 0 : Hq == 0, B200_DECLINE_EXTENT, "attention_packed: %lld heads over %lld", (long long)Hq, (long long)H);
+    B200_REQUIRE(E <= 128, B200_DECLINE_TILING, "attention_packed: heads of %lld elements (at most 128)", (long long)E);
+    B200_REQUIRE(N < (1ll << 30) && Nk < (1ll << 30) && Hq < 65536 && B < (1ll << 24), B200_DECLINE_EXTENT,
+                 "attention_packed: N=%lld Nk=%lld Hq=%lld B=%lld", (long long)N, (long long)Nk, (long long)Hq, (long long)B);
+    for (const b200_strided4* a : {q, k, v, out})
+        B200_REQUIRE(E <= 1 || a->stride[0] == 1, B200_DECLINE_ALIGN, "attention_packed: E is not contiguous");
+    if (E == 0 || N == 0 || Hq == 0 || B == 0) return B200_OK;
+    B200_REQUIRE(q->ptr && out->ptr && starts && kstarts && (Nk == 0 || (k->ptr && v->ptr)), B200_EINVAL, "attention_packed: null array");
+    B200_CUDA(cudaSetDevice(ctx->device));
+    PackedParams p = {};
+    p.starts = starts, p.kstarts = kstarts;
+    p.N = (int)N, p.Nk = (int)Nk, p.B = (int)B, p.H = (int)H, p.Hq = (int)Hq, p.E = (int)E;
+    p.causal = causal, p.out_f32 = out_dtype == B200_F32;
+    p.out = const_cast<void*>(out->ptr);
+    p.oN = out->stride[1], p.oH = out->stride[2];
+    const int64_t size = p.out_f32 ? 4 : 2;
+    p.out_whole = ((uintptr_t)p.out | (uint64_t)(p.oN * size) | (uint64_t)(p.oH * size)) % 16 == 0;
+    p.scale_log2 = fmaxf((float)((double)scale * 1.4426950408889634), 0x1p-100f);   // above 0, so that a hidden score of -inf stays that
+    p.d_status = ctx->d_status;
+    // Heads of a tile: as many rows used as can be of 128 times those of all of a key head's tiles; of equals, the most heads.
+    p.share = (int)(Hq / H);
+    double best = 0;
+    for (int g = 1; g <= p.share && g <= PK_ROWS; ++g) {
+        const double used = (double)(PK_ROWS / g * g) * p.share / (double)(cdiv(p.share, g) * g);
+        if (used >= best) best = used, p.G = g;
+    }
+    p.T = PK_ROWS / p.G;
+    p.groups = (int)cdiv(p.share, p.G);
+    p.by_g = Divisor::of(p.G);
+    p.heads = (int)(p.H * p.groups);
+    const int64_t entries = N / (2 * p.T) + (B < N ? B : N), items = entries * p.heads;    // at most
+    B200_REQUIRE(items < (1ll << 30), B200_DECLINE_EXTENT, "attention_packed: %lld row tiles", (long long)items);
+    PackedOperand op[3];
+    const b200_strided4* in[3] = {q, k, v};
+    int64_t E8 = (E + 7) / 8 * 8;
+    for (int i = 0; i < 3; ++i) {
+        const int64_t rows = i ? Nk : N, heads = i ? H : Hq;
+        op[i] = {(const __half*)in[i]->ptr, in[i]->stride[1], in[i]->stride[2]};
+        if (heads == 1) op[i].sH = E8;         // a stride that nothing is read through
+        if (rows == 1) op[i].sN = E8;
+        if (rows == 0) {                       // no keys at all: the maps are over something that is there
+            op[i] = op[0];
+            continue;
+        }
+        if (((uintptr_t)op[i].ptr % 16 | (uint64_t)op[i].sN % 8 | (uint64_t)op[i].sH % 8) == 0 && op[i].sN > 0 && op[i].sH > 0) continue;
+        void* ws = nullptr;
+        int rc = ws_scratch(ctx, (size_t)(rows * heads * E8) * sizeof(__half), &ws);
+        if (rc) return rc;
+        const int64_t total = rows * heads * (E8 / 8);
+        B200_REQUIRE(cdiv(total, 256) < (1ll << 31), B200_DECLINE_EXTENT, "attention_packed: %lld rows to copy", (long long)rows);
+        B200_CUDA(launch_dep(packed_rows_kernel, dim3((unsigned)cdiv(total, 256)), dim3(256), 0, ctx->stream, 1, op[i].ptr, op[i].sN, op[i].sH, (__half*)ws,
+                             (int)E, (int)E8, (int)heads, total));
+        ctx->launches++;
+        op[i] = {(const __half*)ws, heads * E8, E8};
+    }
+    p.v = op[2].ptr, p.vN = op[2].sN, p.vH = op[2].sH;
+    return E <= 64 ? pk_launch<64>(ctx, p, op[0], op[1], op[2], items, entries) : pk_launch<128>(ctx, p, op[0], op[1], op[2], items, entries);
+}
+
+} // extern "C"

@@ -42,6 +42,8 @@ static int (*p_matmul4)(b200_ctx*, const b200_q4*, int64_t, const void*, int64_t
 
 static int (*p_normrotary)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, const b200_strided4*, const b200_strided4*, const void*, int, int64_t,
                            int64_t, float, const uint64_t*, int64_t, int, float, const int32_t*, int64_t, int64_t, const int32_t*, const int32_t*);
+static int (*p_packed)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, const b200_strided4*, const b200_strided4*,
+                       const b200_strided4*, const b200_strided4*, int, float, int, const int32_t*, const int32_t*);
 
 static int64_t attr_int(PyObject* o, PyObject* name, int* ok) {
     PyObject* v = PyObject_GetAttr(o, name);
@@ -439,11 +441,40 @@ static PyObject* h_binddecode(PyObject* self, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-// bindaround(norm and rotation): the entry points around a decoder's step, as addresses
+// packedsdpa(handle, out, q, k, v, starts, kstarts, scale, causal)
+static PyObject* h_packedsdpa(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    Arr x[4], starts;                  // out, q, k, v
+    b200_strided4 s[4];
+    const int32_t* kstarts;
+    b200_ctx* c;
+    int rc;
+    if (n != 9 || !(c = handle(a[0])) || !PyFloat_Check(a[7]) || !PyBool_Check(a[8])) Py_RETURN_NONE;
+    for (int i = 0; i < 4; ++i) {
+        if (!load(a[1 + i], &x[i]) || x[i].nd != 3 || (i > 0 && x[i].code != B200_F16)) Py_RETURN_NONE;
+        x[i].stride[3] = 0;
+        strided(&x[i], &s[i]);
+    }
+    for (int i = 0; i < 3; ++i)
+        if (x[0].shape[i] != x[1].shape[i] || x[2].shape[i] != x[3].shape[i]) Py_RETURN_NONE;
+    const int64_t E = x[1].shape[0], N = x[1].shape[1], Hq = x[1].shape[2], Nk = x[2].shape[1], H = x[2].shape[2];
+    if (x[2].shape[0] != E || (H ? Hq % H != 0 : Hq != 0)) Py_RETURN_NONE;
+    if (!load_any(a[5], &starts) || starts.code != CODE_I32 || starts.size < 1 || !dense(&starts)) Py_RETURN_NONE;
+    if (!counts(a[6], starts.size, &kstarts)) Py_RETURN_NONE;
+    if (a[6] == Py_None) {
+        if (Nk < N) Py_RETURN_NONE;
+        kstarts = (const int32_t*)starts.ptr;
+    }
+    ENTER(rc, p_packed(c, E, N, Nk, Hq, H, starts.size - 1, &s[1], &s[2], &s[3], &s[0], x[0].code, (float)PyFloat_AS_DOUBLE(a[7]), a[8] == Py_True,
+                       (const int32_t*)starts.ptr, kstarts));
+    return PyLong_FromLong(rc);
+}
+
+// bindaround(norm and rotation, packed attention): the entry points around a decoder's step, as addresses
 static PyObject* h_bindaround(PyObject* self, PyObject* args) {
-    unsigned long long a;
-    if (!PyArg_ParseTuple(args, "K", &a)) return NULL;
+    unsigned long long a, b;
+    if (!PyArg_ParseTuple(args, "KK", &a, &b)) return NULL;
     *(void**)&p_normrotary = (void*)(uintptr_t)a;
+    *(void**)&p_packed = (void*)(uintptr_t)b;
     Py_RETURN_NONE;
 }
 
@@ -467,6 +498,7 @@ static PyMethodDef methods[] = {{"bind", h_bind, METH_VARARGS, NULL},
                                 {"binddecode", h_binddecode, METH_VARARGS, NULL},
                                 {"rotary", (PyCFunction)(void (*)(void))h_rotary, METH_FASTCALL, NULL},
                                 {"bindaround", h_bindaround, METH_VARARGS, NULL},
+                                {"packedsdpa", (PyCFunction)(void (*)(void))h_packedsdpa, METH_FASTCALL, NULL},
                                 {"normrotary", (PyCFunction)(void (*)(void))h_normrotary, METH_FASTCALL, NULL},
                                 {"cacheappend", (PyCFunction)(void (*)(void))h_cacheappend, METH_FASTCALL, NULL},
                                 {"cacheread", (PyCFunction)(void (*)(void))h_cacheread, METH_FASTCALL, NULL},

@@ -80,6 +80,8 @@ struct b200_ctx {
 // Device status of the paged cache, reported by the next synchronisation: a page number outside the cache, a length or a count of
 // new tokens that does not fit the call.  Nothing is read or written there.
 enum : int { KST_CACHE_PAGE = 120, KST_CACHE_LENGTH = 121 };
+// Of packed sequences: first rows that are not in order, or past the array's; what they name is cut to what is there.
+enum : int { KST_PACKED_STARTS = 122 };
 
 constexpr int SK_FLAG_COUNT = 4096;
 constexpr int GEMV_COUNTER_COUNT = 1024;    // arrival counters of the split matrix-vector product, after the flags

@@ -1,0 +1,181 @@
+"""Attention of packed sequences against fp64 (tests/decode_ref.py), at the lengths, head layouts and masks where it can go wrong.
+
+Tolerances count roundings.  A weight is rounded to fp16 (2^-11 of itself; below 2^-14 of 2^-7 of the heaviest weight a step of 2^-24, so
+2^-32 of the heaviest a key), scores are fp32 sums of E products (E 2^-24 of the sum of their sizes, which moves a weight by as much), sums and
+exponentials fp32 (2^-21), the result half a step of its type."""
+import numpy as np
+import pytest
+
+import juliavision_b200 as jv
+from tests import decode_ref as ref
+from tests.test_gpu_decode import F16, F32, STEP, ints, near
+
+pytestmark = pytest.mark.gpu
+
+
+class Packed:
+    """Sequences side by side: news[b] rows over news[b] + past[b] keys (fewer keys than rows where past is negative), `spare` rows behind."""
+
+    def __init__(self, ctx, rng, E, Hq, H, news, past, spare=2, layout="joined", scale=1.0):
+        self.ctx, self.E, self.Hq, self.H = ctx, E, Hq, H
+        self.news, self.keys = np.asarray(news), np.asarray(news) + np.asarray(past)
+        self.starts, self.kstarts = (np.concatenate(([0], np.cumsum(n))) for n in (self.news, self.keys))
+        N, Nk = int(self.starts[-1]) + spare, int(self.kstarts[-1]) + spare
+        self.q, self.k, self.v = ((rng.standard_normal((n, h, E)) * scale).astype(F16) for n, h in ((N, Hq), (Nk, H), (Nk, H)))
+        self.layout = layout
+
+    def device(self):
+        ctx, E = self.ctx, self.E
+        if self.layout == "joined":         # keys and values side by side, token-major
+            kv = ctx.toback(np.stack((self.k, self.v), 1))
+            Nk = len(self.k)
+            dk, dv = (jv.DeviceArray(ctx, kv.ptr + i * self.H * E * 2, F16, (E, Nk, self.H), (1, 2 * self.H * E, E), owner=kv) for i in range(2))
+            return ctx.toback(self.q).permute((0, 2, 1)), dk, dv
+        if self.layout == "heads":          # head-major
+            return tuple(ctx.toback(np.ascontiguousarray(a.transpose(1, 0, 2))) for a in (self.q, self.k, self.v))
+        out = []                            # rows of an odd pitch, off 16-byte boundaries
+        for a in (self.q, self.k, self.v):
+            wide = np.zeros(a.shape[:2] + (E + 1,), F16)
+            wide[..., 1:] = a
+            d = ctx.toback(wide)
+            out.append(jv.DeviceArray(ctx, d.ptr + 2, F16, (E, a.shape[0], a.shape[1]), (1, (E + 1) * a.shape[1], E + 1), owner=d))
+        return tuple(out)
+
+    def run(self, dtype, causal, scale=None, same=False):
+        ctx = self.ctx
+        buf = ctx.allocate(dtype, self.E, self.Hq, len(self.q))
+        ctx.fill_bytes(buf, 0xFF)
+        out = buf.permute((0, 2, 1))
+        ctx.ws.reset()
+        jv.packedsdpa_(ctx, out, *self.device(), ints(ctx, self.starts), None if same else ints(ctx, self.kstarts), scale=scale, causal=causal)
+        ctx.synchronize()
+        return buf.to_host()
+
+    def check(self, got, dtype, causal, scale=None):
+        E = self.E
+        scale = 1.0 / np.sqrt(E) if scale is None else scale
+        for b, (n, m) in enumerate(zip(self.news, self.keys)):
+            q0, k0 = self.starts[b], self.kstarts[b]
+            q, k, v = self.q[q0:q0 + n].astype(np.float64), self.k[k0:k0 + m].astype(np.float64), self.v[k0:k0 + m].astype(np.float64)
+            hidden = (np.arange(m) > np.arange(n)[:, None] + (m - n)) if causal else np.zeros((n, m), bool)
+            with np.errstate(invalid="ignore"):
+                o, a, reach = ref.attention(q, k, v, hidden, scale)
+                most = np.max(np.abs(np.where(np.isfinite(v), v, 0)), initial=0)
+                mine = got[q0:q0 + n].astype(np.float64)
+                same = np.isinf(o) & (mine == o)
+                near(np.where(same, 0, mine), np.where(same, 0, o), np.nan_to_num(STEP[dtype][0] * np.abs(o) + STEP[dtype][1] + a * (2.0 ** -11 + 2.0 ** -21 + 4 * E * 2.0 ** -24 * reach),
+                                                      posinf=0) + m * 2.0 ** -32 * most)
+        assert np.isnan(got[self.starts[-1]:].astype(np.float64)).all()      # rows that belong to nobody
+
+
+CASES = [  # E, Hq, H, news, past
+    (64, 1, 1, [1], [0]), (64, 20, 20, [77], [0]), (128, 4, 1, [1, 0, 2, 127, 128, 129, 130], [0] * 7), (128, 8, 2, [5, 300, 0, 33, 257], [0, 700, 50, 128, 1]),
+    (80, 10, 2, [200, 63, 64], [0, 1000, 1]), (72, 7, 1, [100, 37], [0, 3]), (40, 6, 3, [256, 255, 1], [256, 1, 2000]), (128, 71, 1, [9, 40], [0, 0]),
+    (96, 5, 5, [1] * 33, [0, 1, 126, 127, 128, 129, 200, 300, 1, 2, 3] * 3), (8, 3, 3, [150], [0]), (33, 4, 2, [70, 5], [0, 9]), (128, 130, 1, [3, 1], [4, 60]),
+    (64, 12, 4, [100, 50, 0, 7], [-30, -50, 0, -6]), (128, 2, 1, [700], [0]), (1, 2, 1, [40], [0]), (128, 16, 16, [600, 1], [0, 4000])]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_packed(ctx, case, causal, dtype):
+    E, Hq, H, news, past = case
+    p = Packed(ctx, np.random.default_rng(1), E, Hq, H, news, past)
+    p.check(p.run(dtype, causal), dtype, causal)
+
+
+@pytest.mark.parametrize("layout", ["heads", "odd"])
+@pytest.mark.parametrize("E", [64, 80, 128, 20])
+def test_layouts(ctx, layout, E):
+    p = Packed(ctx, np.random.default_rng(2), E, 6, 2, [130, 1, 40], [0, 5, 100], layout=layout)
+    p.check(p.run(F16, True), F16, True)
+
+
+@pytest.mark.parametrize("E", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_and_long(ctx, E, causal):
+    """More pairs of tiles than SMs: the list of the work; and one long among many short, which is cut along its keys."""
+    rng = np.random.default_rng(3)
+    p = Packed(ctx, rng, E, 8, 4, rng.integers(0, 400, 60), np.zeros(60, int))
+    p.check(p.run(F16, causal), F16, causal)
+    p = Packed(ctx, rng, E, 4, 2, [3] + [1] * 20 + [50], [20000] + list(rng.integers(0, 100, 20)) + [5000])
+    p.check(p.run(F32, causal), F32, causal)
+
+
+def test_same_places_and_scales(ctx):
+    p = Packed(ctx, np.random.default_rng(4), 64, 4, 2, [90, 200], [0, 0])
+    for scale in (0.0, 1.0, 3.0):
+        p.check(p.run(F32, True, scale, same=True), F32, True, scale)
+
+
+@pytest.mark.parametrize("E", [64, 96])
+def test_far_apart_scores(ctx, E):
+    """Maxima that grow along the keys by more than the reference point lets pass."""
+    p = Packed(ctx, np.random.default_rng(5), E, 4, 2, [300, 40], [100, 500])
+    p.k *= np.linspace(0.1, 12, len(p.k))[:, None, None].astype(F16)
+    for causal in (True, False):
+        p.check(p.run(F32, causal), F32, causal)
+
+
+@pytest.mark.parametrize("E", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_hidden_keys_may_hold_anything(ctx, E, causal):
+    """Infinities and NaN in keys and values: rows that see them show it, no other row and no other sequence does."""
+    rng = np.random.default_rng(6)
+    p = Packed(ctx, rng, E, 4, 2, [140, 130, 5], [0, 200, 300])
+    for b, at in ((0, 139), (0, 70), (1, 329), (1, 300), (2, 303)):
+        p.v[p.kstarts[b] + at, b % 2, 3 + b] = (np.inf, -np.inf, np.nan)[(b + at) % 3]
+    p.v[p.kstarts[-1]:] = np.nan
+    p.k[p.kstarts[-1]:] = np.nan
+    p.k[p.kstarts[1] + 325, 1] = np.nan
+    p.v[p.kstarts[1] + 10, 0, 7] = np.inf        # of a block that all rows see
+    p.v[p.kstarts[0] + 70, 0, 5], p.v[p.kstarts[0] + 75, 0, 5] = np.inf, -np.inf
+    p.check(p.run(F32, causal), F32, causal)
+
+
+def test_parts_that_meet_hold_anything(ctx):
+    """The same where the keys are cut and joined."""
+    p = Packed(ctx, np.random.default_rng(7), 128, 2, 1, [20], [30000])
+    p.v[30010, 0, 9], p.v[30000, 0, 1], p.v[20, 0, 2] = np.nan, np.inf, -np.inf
+    p.check(p.run(F32, True), F32, True)
+
+
+def test_bad_starts_are_cut_and_reported(ctx):
+    for bad in ([0, 50, 20, 60], [0, 30, 60, 1000], [-4, 30, 60, 60], [0, 60, 0, 60]):
+        p = Packed(ctx, np.random.default_rng(8), 64, 2, 2, [20, 20, 20], [0, 0, 0], spare=0)
+        p.starts = p.kstarts = np.array(bad)
+        with pytest.raises(jv.B200Error) as e:
+            p.run(F16, True)
+        assert e.value.code == 4
+        ctx.synchronize()
+
+
+def test_recorded(ctx):
+    """One graph, lengths changed between replays; two graphs share the workspace."""
+    rng = np.random.default_rng(9)
+    p = Packed(ctx, rng, 128, 8, 2, [400, 700], [0, 3000], spare=0)
+    d, ds, dk = p.device(), ints(ctx, p.starts), ints(ctx, p.kstarts)
+    outs = [ctx.allocate(F16, 128, 8, len(p.q)) for _ in range(2)]
+    views = [o.permute((0, 2, 1)) for o in outs]
+    ctx.ws.reset()
+    jv.packedsdpa_(ctx, views[0], *d, ds, dk)
+    graphs = []
+    for o in views:
+        ctx.ws.reset()
+        graphs.append(ctx.capture(lambda o=o: jv.packedsdpa_(ctx, o, *d, ds, dk)))
+    for first in (400, 11, 1090):
+        starts, kstarts = np.array([0, first, 1100], np.int32), np.array([0, 2 * first, 4100], np.int32)
+        ctx.upload(ds, starts)
+        ctx.upload(dk, kstarts)
+        for o in outs:
+            ctx.fill_bytes(o, 0xFF)
+        for g in graphs:
+            g.replay()
+        ctx.synchronize()
+        got = [o.to_host() for o in outs]
+        ctx.ws.reset()
+        jv.packedsdpa_(ctx, views[0], *d, ds, dk)
+        ctx.synchronize()
+        assert all(np.array_equal(g, outs[0].to_host()) for g in got)
+        p.news, p.keys, p.starts, p.kstarts = np.diff(starts), np.diff(kstarts), starts, kstarts
+        p.check(got[0], F16, True)
