@@ -308,6 +308,25 @@ int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int
                          const b200_strided4* out, int out_dtype, float scale, int causal, const int32_t* lens,
                          const int32_t* news);
 
+/* -------------------------------------------------------------------- beam search */
+/*
+ * Of the K V continuations scores[k] + x[v,k] - log sum_u exp x[u,k] of each of B searches the N best, in order, ties to the lowest
+ * k V + v: best, parents and tokens (N,B).  logits (V,K,B), fp16 or fp32, V contiguous, beams ldk and searches ldb elements apart; scores (K,B).
+ * Logits are read in whole aligned 16-byte blocks.  A beam with ended[k,b] != 0 (ended NULL: none) has one continuation, token `pad` at its own score.
+ * A beam whose score is not finite, or whose logits have no finite log sum, offers its tokens at -inf, which come last, lowest first.
+ * Exponentials are fp32, their sums over shares fp32, over a row and the scores fp64.  K and N are at most 32, N at most K V.  Scratch comes
+ * from the context's workspace.
+ */
+int b200_beam_select(b200_ctx* ctx, int64_t V, int64_t K, int64_t B, int64_t N, const void* logits, int dtype, int64_t ldk, int64_t ldb,
+                     const float* scores, const int32_t* ended, int64_t pad, float* best, int32_t* parents, int32_t* tokens);
+/* Beam k of search b, sequence k + K b of n caches of the same sizes and strides (their own table, table_ld and width are not read), goes on from
+ * the tokens of beam parents[k,b].  own (width,K B): the pages that each beam writes, no page twice.  In the table, entries below the last full
+ * page become the parent's, the others the beam's own; the tokens and maxima of the page that is not full are copied from the
+ * parent's own page to the beam's.  lens (K,B): the beams of a search are equally long (the first one's counts; others are reported).
+ * A parent outside [0,K) leaves the beam where it was, a page outside the cache is not touched; the next b200_sync reports either. */
+int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int64_t K, int64_t B, int32_t* table, int64_t table_ld,
+                       const int32_t* own, int64_t own_ld, int64_t width, const int32_t* parents, const int32_t* lens);
+
 /* ------------------------------------------------------------------- 4-bit weights */
 /*
  * A weight (M,K) of 4-bit values with a scale, and perhaps a zero point, for each `group` (32, 64 or 128) inputs of an

@@ -7,6 +7,7 @@ is no fallback if the library is missing.
 """
 from ._lib import B200Error, SO_PATH, lib
 from .attention import packedsdpa_, sdpa, sdpa_, sdpaplan
+from .beam import beamselect_, cachereorder_
 from .kvcache import Cache8, cache8, cacheappend_, cacheread_, cachesdpa_
 from .context import Ctx, DeviceArray, DeviceCaps, Workspace, caps
 from .conv import convolution_, convolutiontranspose_, convsize, convtransposesize, onebyone, shufflecase
@@ -33,5 +34,5 @@ __all__ = [
     "maxpool2d_", "to_copy_", "MMGemvPlan", "foldoutcasts", "foldincasts", "foldbatchnorm", "foldrelu", "hoistcasts", "weightsource", "readsafetensors", "safetensorsnames",
     "Event", "StreamedPass", "Diagnostics", "TwoGemmPlan", "convolutiontranspose_", "convtransposesize", "shufflecase",
     "Cache8", "cache8", "cacheappend_", "cacheread_", "cachesdpa_", "Weight4", "matmul4_", "pack4", "quantise4", "RotaryPlan", "rotary_",
-    "rotaryfrequencies", "rotaryplan", "normrotary_", "packedsdpa_",
+    "rotaryfrequencies", "rotaryplan", "normrotary_", "packedsdpa_", "beamselect_", "cachereorder_",
 ]

@@ -113,6 +113,8 @@ SIGNATURES = {
     "b200_norm_rotary_f16": (_i32, [_vp, _i64, _i64, _i64, _i64, _s4, _s4, _vp, _i32, _i64, _i64, _f32, _vp, _i64, _i32, _f32, _vp, _i64, _i64,
                                     _vp, _vp]),
     "b200_attention_packed_f16": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _s4, _s4, _s4, _s4, _i32, _f32, _i32, _vp, _vp]),
+    "b200_beam_select": (_i32, [_vp, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "b200_cache_reorder": (_i32, [_vp, _c8, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     "b200_cache_append": (_i32, [_vp, _c8, _i64, _i64, _s4, _s4, _vp, _vp]),
     "b200_cache_read": (_i32, [_vp, _c8, _i32, _i64, _i64, _vp, _vp, _s4, _i32]),
     "b200_cache_attention": (_i32, [_vp, _c8, _i64, _i64, _i64, _s4, _s4, _i32, _f32, _i32, _vp, _vp]),
@@ -173,7 +175,7 @@ def host():
         m.bind(at(L.b200_gemm_f16), at(L.b200_gemv), at(L.b200_attention_f16_bias), at(L.b200_layernorm),
                at(L.b200_conv2d_grouped_f16))
         m.binddecode(at(L.b200_rotary_f16), at(L.b200_cache_append), at(L.b200_cache_read), at(L.b200_cache_attention), at(L.b200_matmul_q4))
-        m.bindaround(at(L.b200_norm_rotary_f16), at(L.b200_attention_packed_f16))
+        m.bindaround(at(L.b200_norm_rotary_f16), at(L.b200_attention_packed_f16), at(L.b200_beam_select), at(L.b200_cache_reorder))
         _host = m
     return _host
 

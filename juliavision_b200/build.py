@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(CSRC, "libb200dnn.so")
 SOURCES = ["ctx.cu", "layernorm.cu", "gemm.cu", "attention.cu", "glue.cu", "conv.cu", "conv_implicit.cu", "gemv.cu", "gemm_rows.cu", "gemm_rows_tc.cu", "attention_window.cu", "attention_few.cu", "selftest.cu",
-           "rotary.cu", "norm_rotary.cu", "cache8.cu", "cache8_attention.cu", "cache8_prompt.cu", "linear4.cu", "attention_packed.cu"]
+           "rotary.cu", "norm_rotary.cu", "cache8.cu", "cache8_attention.cu", "cache8_prompt.cu", "linear4.cu", "attention_packed.cu", "beam.cu", "cache8_reorder.cu"]
 HEADERS = ["internal.h", "ptx.cuh", "act.cuh", "gemm_rows.cuh", "cache8.cuh", "rotary.cuh", "shares.cuh", os.path.join("..", "..", "include", "b200dnn.h")]
 HOST_SRC = os.path.join(CSRC, "hostcalls.c")   # the entry points' host side, a CPython extension
 HOST_SO = os.path.join(CSRC, "hostcalls" + EXTENSION_SUFFIXES[0])   # for this interpreter: another builds its own

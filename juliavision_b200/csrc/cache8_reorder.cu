@@ -1,0 +1,156 @@
+// Beams of a search change places: beam s goes on from its parent's tokens.  Of those, whole pages change hands by their numbers, and stay
+// where they are: column s of the table becomes its parent's up to the last full page.  The page that is not full is copied, its tokens and its
+// maxima, from the one that the parent was writing to the one that s writes: a beam only ever writes pages of its own (`own`), one for every T
+// tokens, so that no page is written that another beam reads.
+//
+// Bandwidth-bound: the tokens of a part-filled page, read and written, for every beam whose parent is another.  A thread takes the same 16
+// bytes of all of a search's beams and reads them all before it writes any, so the beams may change places in any way without a second copy.
+#include "cache8.cuh"
+
+namespace b200 {
+
+constexpr int CR_CACHES = 128;       // of a launch
+constexpr int CR_BEAMS = 32;         // of a search
+
+struct ReorderParams {
+    uint8_t* data[2 * CR_CACHES];    // keys and values of a cache
+    float* most[2 * CR_CACHES];
+    CacheView c;                     // sizes and strides, the same for all; table unused
+    int32_t* table;
+    const int32_t *own, *parents, *lens;
+    int64_t table_ld, own_ld;
+    int K, blocks, tables;           // blocks of a side of a page; whether this launch brings the table up to date
+};
+
+// What every block looks up of its search; whatever the arrays hold, it is inside the cache.
+struct ReorderSearch {
+    int full, kept;                  // whole pages, tokens of the next
+    __device__ __forceinline__ ReorderSearch(const ReorderParams& p, int64_t search) {
+        const int n = p.c.tokens((int)(search * p.K), p.lens);
+        full = n >> p.c.logT;
+        kept = n - (full << p.c.logT);
+    }
+};
+__device__ __forceinline__ int cr_parent(const ReorderParams& p, int64_t search, int k) {
+    const int s = p.parents[search * p.K + k];
+    if (s >= 0 && s < p.K) return s;
+    atomicCAS(p.c.d_status, 0, KST_BEAM_PARENT);
+    return k;
+}
+
+template <int K>     // beams of a search at most
+__global__ void __launch_bounds__(256)
+cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
+    __shared__ int parent[CR_BEAMS];
+    __shared__ int64_t page[CR_BEAMS];           // that a beam writes, or -1
+    const int tid = threadIdx.x;
+    const int64_t search = blockIdx.y;
+    grid_dep_wait();
+    grid_dep_launch();
+    const ReorderSearch s(p, search);
+    if (tid < p.K) {
+        const int from = cr_parent(p, search, tid);
+        parent[tid] = from;
+        int64_t pg = -1;
+        if (s.kept > 0 && s.full < p.c.width) {
+            pg = p.own[(search * p.K + tid) * p.own_ld + s.full];
+            if (pg < 0 || pg >= p.c.P) {
+                p.c.report(KST_CACHE_PAGE);
+                pg = -1;
+            }
+        }
+        page[tid] = pg;
+        if (p.tables && blockIdx.x == 0 && p.lens[search * p.K + tid] != p.lens[search * p.K]) p.c.report(KST_CACHE_LENGTH);
+    }
+    __syncthreads();
+    if (blockIdx.x < (unsigned)p.tables) {       // the first block: the table
+        for (int i = tid; i < p.c.width; i += 256) {
+            int32_t* at = p.table + search * p.K * p.table_ld + i;
+            int32_t was[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) was[k] = k < p.K ? i < s.full ? at[parent[k] * p.table_ld] : p.own[(search * p.K + k) * p.own_ld + i] : 0;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k < p.K) at[k * p.table_ld] = was[k];
+        }
+        return;
+    }
+    if (s.kept == 0) return;
+    const int unit = blockIdx.x - p.tables, side = unit / p.blocks, block = unit - side * p.blocks;
+    const bool value = side & 1;
+    const int per = p.c.E / 16, row = s.kept * per;               // of a head
+    const int i = block * 256 + tid;
+    uint8_t* data = p.data[side];
+    if (i < row * p.c.H) {
+        const int h = i / row, t = (i - h * row) / per, e = i - h * row - t * per;
+        uint8_t* at = data + t * (value ? p.c.vT : p.c.kT) + h * (value ? p.c.vH : p.c.kH) + e * 16;
+        const int64_t pitch = value ? p.c.vP : p.c.kP;
+        uint4 v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) v[k] = *reinterpret_cast<const uint4*>(at + page[parent[k]] * pitch);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) *reinterpret_cast<uint4*>(at + page[k] * pitch) = v[k];
+    }
+    if (block == 0)
+        for (int h = tid; h < p.c.H; h += 256) {
+            float* at = p.most[side] + h;
+            float v[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) v[k] = at[page[parent[k]] * p.c.H];
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) at[page[k] * p.c.H] = v[k];
+        }
+}
+
+} // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int64_t K, int64_t B, int32_t* table, int64_t table_ld,
+                       const int32_t* own, int64_t own_ld, int64_t width, const int32_t* parents, const int32_t* lens) {
+    B200_REQUIRE(ctx && (caches || n == 0), B200_EINVAL, "cache_reorder: null argument");
+    B200_REQUIRE(n >= 0 && K >= 0 && B >= 0, B200_EINVAL, "cache_reorder: %lld caches, K=%lld B=%lld", (long long)n, (long long)K, (long long)B);
+    B200_REQUIRE(K <= CR_BEAMS && B < 65536, B200_DECLINE_EXTENT, "cache_reorder: %lld beams (at most %d), %lld searches", (long long)K, CR_BEAMS, (long long)B);
+    if (n == 0 || K == 0 || B == 0) return B200_OK;
+    B200_REQUIRE(table && own && parents && lens, B200_EINVAL, "cache_reorder: null array");
+    B200_REQUIRE(own_ld >= width, B200_DECLINE_EXTENT, "cache_reorder: leading dimension %lld of %lld pages", (long long)own_ld, (long long)width);
+    B200_CUDA(cudaSetDevice(ctx->device));
+    ReorderParams p = {};
+    for (int64_t at = 0; at < n; at += CR_CACHES) {
+        const int count = (int)(n - at < CR_CACHES ? n - at : CR_CACHES);
+        for (int i = 0; i < count; ++i) {
+            b200_cache8 c = caches[at + i];
+            c.table = table, c.table_ld = table_ld, c.width = width;
+            CacheView v;
+            int rc = cache_view(ctx, &c, "cache_reorder", &v);
+            if (rc) return rc;
+            if (at == 0 && i == 0) p.c = v;
+            B200_REQUIRE(v.E == p.c.E && v.T == p.c.T && v.H == p.c.H && v.P == p.c.P && v.kT == p.c.kT && v.kH == p.c.kH && v.kP == p.c.kP &&
+                             v.vT == p.c.vT && v.vH == p.c.vH && v.vP == p.c.vP,
+                         B200_DECLINE_EXTENT, "cache_reorder: cache %lld has other sizes or strides than the first", (long long)(at + i));
+            p.data[2 * i] = v.k, p.data[2 * i + 1] = v.v;
+            p.most[2 * i] = v.kmax, p.most[2 * i + 1] = v.vmax;
+        }
+        p.table = table, p.table_ld = table_ld, p.own = own, p.own_ld = own_ld;
+        p.parents = parents, p.lens = lens;
+        p.K = (int)K;
+        p.tables = at == 0;
+        p.blocks = (int)cdiv((int64_t)p.c.H * p.c.T * (p.c.E / 16), 256);
+        const int64_t grid = p.tables + 2 * count * (int64_t)p.blocks;
+        B200_REQUIRE(grid < (1ll << 31), B200_DECLINE_EXTENT, "cache_reorder: %d heads in %d caches", p.c.H, count);
+        const dim3 g((unsigned)grid, (unsigned)B), b(256);
+        auto run = [&](auto kern) { return launch_dep(kern, g, b, 0, ctx->stream, 1, p); };
+        B200_CUDA(K <= 4 ? run(cache_reorder_kernel<4>) : K <= 8 ? run(cache_reorder_kernel<8>) : K <= 16 ? run(cache_reorder_kernel<16>)
+                                                                                                        : run(cache_reorder_kernel<32>));
+        ctx->launches++;
+    }
+    return B200_OK;
+}
+
+} // extern "C"

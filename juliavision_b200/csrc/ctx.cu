@@ -291,6 +291,7 @@ int b200_sync(b200_ctx* c) {
         cudaStreamSynchronize(c->stream);
         if (st == KST_CACHE_PAGE) return fail(B200_EKERNEL, "a cache's table holds a page number outside the cache (device status %d)", st);
         if (st == KST_PACKED_STARTS) return fail(B200_EKERNEL, "packed sequences' first rows are out of order or past the array (device status %d)", st);
+        if (st == KST_BEAM_PARENT) return fail(B200_EKERNEL, "a beam's parent is not a beam of its search (device status %d)", st);
         if (st == KST_CACHE_LENGTH) return fail(B200_EKERNEL, "a sequence's length or count of new tokens does not fit the call (device status %d)", st);
         return fail(B200_EKERNEL, "a kernel gave up a bounded wait (device status %d)", st);
     }

@@ -44,6 +44,10 @@ static int (*p_normrotary)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, const 
                            int64_t, float, const uint64_t*, int64_t, int, float, const int32_t*, int64_t, int64_t, const int32_t*, const int32_t*);
 static int (*p_packed)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, const b200_strided4*, const b200_strided4*,
                        const b200_strided4*, const b200_strided4*, int, float, int, const int32_t*, const int32_t*);
+static int (*p_beamselect)(b200_ctx*, int64_t, int64_t, int64_t, int64_t, const void*, int, int64_t, int64_t, const float*, const int32_t*, int64_t,
+                           float*, int32_t*, int32_t*);
+static int (*p_reorder)(b200_ctx*, const b200_cache8*, int64_t, int64_t, int64_t, int32_t*, int64_t, const int32_t*, int64_t, int64_t, const int32_t*,
+                        const int32_t*);
 
 static int64_t attr_int(PyObject* o, PyObject* name, int* ok) {
     PyObject* v = PyObject_GetAttr(o, name);
@@ -469,12 +473,66 @@ static PyObject* h_packedsdpa(PyObject* self, PyObject* const* a, Py_ssize_t n) 
     return PyLong_FromLong(rc);
 }
 
-// bindaround(norm and rotation, packed attention): the entry points around a decoder's step, as addresses
+// A dense (rows, columns) array of one type, or (where it may be) None: 1 with *p set, else 0.
+static int matrix(PyObject* o, int code, int64_t rows, int64_t columns, int may, void* p) {
+    Arr a;
+    memset(p, 0, sizeof(void*));
+    if (o == Py_None) return may;
+    if (!load_any(o, &a) || a.code != code || a.nd != 2 || a.shape[0] != rows || a.shape[1] != columns || !dense(&a)) return 0;
+    *(void**)p = P(a);
+    return 1;
+}
+
+// beamselect(handle, best, parents, tokens, logits, scores, ended, pad)
+static PyObject* h_beamselect(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    Arr best, x, scores;
+    int32_t *parents, *tokens, *ended;
+    b200_ctx* c;
+    int rc, over;
+    if (n != 8 || !(c = handle(a[0])) || !PyLong_Check(a[7]) || !load(a[1], &best) || !load(a[4], &x) || !load(a[5], &scores)) Py_RETURN_NONE;
+    const int64_t pad = PyLong_AsLongLongAndOverflow(a[7], &over);
+    if (over || best.nd != 2 || best.code != B200_F32 || scores.nd != 2 || scores.code != B200_F32 || !dense(&best) || !dense(&scores)) Py_RETURN_NONE;
+    const int64_t K = scores.shape[0], B = scores.shape[1], N = best.shape[0], V = x.shape[0];
+    if (best.shape[1] != B || (V > 1 && x.stride[0] != 1)) Py_RETURN_NONE;
+    if (x.nd == 3 ? x.shape[1] != K || x.shape[2] != B : x.nd != 2 || x.shape[1] != K * B) Py_RETURN_NONE;
+    if (!matrix(a[2], CODE_I32, N, B, 0, &parents) || !matrix(a[3], CODE_I32, N, B, 0, &tokens) || !matrix(a[6], CODE_I32, K, B, 1, &ended)) Py_RETURN_NONE;
+    ENTER(rc, p_beamselect(c, V, K, B, N, P(x), x.code, x.stride[1], x.nd == 3 ? x.stride[2] : K * x.stride[1], (const float*)P(scores), ended, pad,
+                           (float*)P(best), parents, tokens));
+    return PyLong_FromLong(rc);
+}
+
+// cachereorder(handle, caches, table, own, parents, lens)
+static PyObject* h_cachereorder(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    enum { MOST = 128 };
+    b200_cache8 caches[MOST];
+    Arr t[2], parents;                 // the table, the beams' own
+    const int32_t* lens;
+    b200_ctx* c;
+    int rc;
+    if (n != 6 || !(c = handle(a[0])) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[1]) > MOST) Py_RETURN_NONE;
+    const Py_ssize_t count = PyList_GET_SIZE(a[1]);
+    if (!load_any(a[4], &parents) || parents.code != CODE_I32 || parents.nd != 2 || !dense(&parents)) Py_RETURN_NONE;
+    const int64_t K = parents.shape[0], B = parents.shape[1];
+    for (int i = 0; i < 2; ++i)
+        if (!load_any(a[2 + i], &t[i]) || t[i].code != CODE_I32 || t[i].nd != 2 || t[i].shape[1] != K * B || (t[i].shape[0] != 1 && t[i].stride[0] != 1))
+            Py_RETURN_NONE;
+    if (t[0].shape[0] != t[1].shape[0] || a[5] == Py_None || !counts(a[5], K * B, &lens)) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < count; ++i)
+        if (!kept(PyList_GET_ITEM(a[1], i), &caches[i], sizeof caches[i])) Py_RETURN_NONE;
+    int64_t ld[2];
+    for (int i = 0; i < 2; ++i) ld[i] = K * B > 1 ? t[i].stride[1] : (t[i].shape[0] > 1 ? t[i].shape[0] : 1);
+    ENTER(rc, p_reorder(c, caches, count, K, B, (int32_t*)P(t[0]), ld[0], (const int32_t*)P(t[1]), ld[1], t[0].shape[0], (const int32_t*)P(parents), lens));
+    return PyLong_FromLong(rc);
+}
+
+// bindaround(norm and rotation, packed attention, beams' choice, reordered caches): the entry points around a decoder's step, as addresses
 static PyObject* h_bindaround(PyObject* self, PyObject* args) {
-    unsigned long long a, b;
-    if (!PyArg_ParseTuple(args, "KK", &a, &b)) return NULL;
+    unsigned long long a, b, c, d;
+    if (!PyArg_ParseTuple(args, "KKKK", &a, &b, &c, &d)) return NULL;
     *(void**)&p_normrotary = (void*)(uintptr_t)a;
     *(void**)&p_packed = (void*)(uintptr_t)b;
+    *(void**)&p_beamselect = (void*)(uintptr_t)c;
+    *(void**)&p_reorder = (void*)(uintptr_t)d;
     Py_RETURN_NONE;
 }
 
@@ -499,6 +557,8 @@ static PyMethodDef methods[] = {{"bind", h_bind, METH_VARARGS, NULL},
                                 {"rotary", (PyCFunction)(void (*)(void))h_rotary, METH_FASTCALL, NULL},
                                 {"bindaround", h_bindaround, METH_VARARGS, NULL},
                                 {"packedsdpa", (PyCFunction)(void (*)(void))h_packedsdpa, METH_FASTCALL, NULL},
+                                {"beamselect", (PyCFunction)(void (*)(void))h_beamselect, METH_FASTCALL, NULL},
+                                {"cachereorder", (PyCFunction)(void (*)(void))h_cachereorder, METH_FASTCALL, NULL},
                                 {"normrotary", (PyCFunction)(void (*)(void))h_normrotary, METH_FASTCALL, NULL},
                                 {"cacheappend", (PyCFunction)(void (*)(void))h_cacheappend, METH_FASTCALL, NULL},
                                 {"cacheread", (PyCFunction)(void (*)(void))h_cacheread, METH_FASTCALL, NULL},

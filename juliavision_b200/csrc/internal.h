@@ -82,6 +82,8 @@ struct b200_ctx {
 enum : int { KST_CACHE_PAGE = 120, KST_CACHE_LENGTH = 121 };
 // Of packed sequences: first rows that are not in order, or past the array's; what they name is cut to what is there.
 enum : int { KST_PACKED_STARTS = 122 };
+// Of a beam search: a parent that is not one of the search's beams; the beam stays where it was.
+enum : int { KST_BEAM_PARENT = 123 };
 
 constexpr int SK_FLAG_COUNT = 4096;
 constexpr int GEMV_COUNTER_COUNT = 1024;    // arrival counters of the split matrix-vector product, after the flags
