@@ -463,7 +463,9 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 int first = 0x7fffffff;
                 for (int j = 0; ok && j < it.nblk; ++j, i += 2) {
                     const int st = (i + 1) % STAGES, key0 = (it.j0 + j) * PK_KEYS;
-                    ok = wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
+                    // K too, which it does not need: loads land in any order, and a stage seen last two fills ago looks full
+                    ok = wait(&full[i % STAGES], (uint32_t)((i / STAGES) & 1), KST_WAIT_FULL) &&
+                         wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
                     if (!ok) break;
                     if (key0 + PK_KEYS - 1 > see) {       // some row does not see some key: 0 times what is not finite is no zero
                         uint4* tile = reinterpret_cast<uint4*>(smem + Cfg::S_KV + st * Cfg::SIDE);

@@ -150,6 +150,22 @@ def test_bad_starts_are_cut_and_reported(ctx):
         ctx.synchronize()
 
 
+@pytest.mark.parametrize("E", [64, 128])
+def test_calls_one_after_the_other(ctx, E):
+    """The same bits from every call, however the loads of its tiles land: no answer depends on which block takes what, or when."""
+    rng = np.random.default_rng(10)
+    p = Packed(ctx, rng, E, 16, 4, rng.integers(1, 1500, 24), np.zeros(24, int))
+    d, ds = p.device(), ints(ctx, p.starts)
+    outs = [ctx.allocate(F16, E, 16, len(p.q)) for _ in range(6)]
+    for turn in range(5):
+        for o in outs:
+            ctx.ws.reset()
+            jv.packedsdpa_(ctx, o.permute((0, 2, 1)), *d, ds)
+        ctx.synchronize()
+        first = outs[0].to_host()[:p.starts[-1]]
+        assert all(np.array_equal(first, o.to_host()[:p.starts[-1]]) for o in outs[1:])
+
+
 def test_recorded(ctx):
     """One graph, lengths changed between replays; two graphs share the workspace."""
     rng = np.random.default_rng(9)
