@@ -28,9 +28,37 @@ constexpr int PK_THREADS = 384;
 constexpr int PK_ROWS = 128, PK_KEYS = 128;      // of a tile
 constexpr int PK_ATOM = 128 * 128;               // 128 rows x 64 fp16
 constexpr int PK_PARTS = 2;                      // parts of the work on their way from warp 8 to the others
-constexpr int PK_SOFTMAX_REGS = 232, PK_OTHER_REGS = 40;
+constexpr int PK_SOFTMAX_REGS = 224, PK_OTHER_REGS = 56;
 static_assert(256 * PK_SOFTMAX_REGS + 128 * PK_OTHER_REGS <= PK_THREADS * 168, "what the launch holds");
 constexpr int PK_BUCKETS = 1024;                 // lengths that the list tells apart
+
+// 2^x of two numbers in the units of the FMAs, without the exponential unit: x = n + f, 2^f by a polynomial of degree 4 (the one of least largest
+// relative error, 2.9e-6, among those that are 1 at 0), n added to the exponent.  Below -127 it is 2^-127.  A NaN is lost.
+__device__ __forceinline__ void pk_exp2(uint64_t x2, float& e0, float& e1) {
+    float x0, x1, p0, p1, t0, t1;
+    unpack2(x2, x0, x1);
+    const uint64_t x = pack2(fmaxf(x0, -127.f), fmaxf(x1, -127.f)), magic = pack2(12582912.f, 12582912.f);   // 1.5 * 2^23: the sum's last bit is 1
+    uint64_t t;
+    asm("add.rm.ftz.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
+    const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f)), f = fma2(n, pack2(-1.f, -1.f), x);
+    uint64_t y = fma2(f, pack2(0.013425155f, 0.013425155f), pack2(0.052245375f, 0.052245375f));
+    y = fma2(y, f, pack2(0.24127856f, 0.24127856f));
+    y = fma2(y, f, pack2(0.69304514f, 0.69304514f));
+    y = fma2(y, f, pack2(1.f, 1.f));
+    unpack2(y, p0, p1);
+    unpack2(t, t0, t1);
+    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+struct __align__(16) PackedEntry {
+    int q0, n, k0, m;                  // the sequence: first row, rows, first key, keys
+    int pair, blocks, parts, pad;
+};
+struct __align__(16) PackedCut {
+    int slot, parts, head, token;      // first slot, parts; unit of the row pair; first token of tile 0
+    int q0, n, pad[2];
+};
 
 struct PackedParams {
     const __half* v;                   // for what is not finite
@@ -46,17 +74,17 @@ struct PackedParams {
     int heads;                         // H * groups: units of a row pair
     int most;                          // row pairs that the list has room for: what sequences in order can have
     int planned;
-    // the list (null without one): entries' first units, [entries + 1]; entries (sequence, pair, blocks of keys, parts); first slots; counters
-    int *unit, *slot, *counts;
-    int4* entry;
-    int* pairs;                        // [B + 1] first pair of a sequence
-    int4* loose;                       // entries in the order of the sequences
-    int4* cut;                         // (entry, head) of what was cut
+    // The list (null without one), longest first: row pairs with their sequence's place and size, pair, blocks of keys and parts; where some are cut,
+    // also their first units and slots; counters; the cut ones a head at a time, as the launch that joins them wants them.
+    PackedEntry* entry;
+    int *unit, *slot;
+    int4* counts;                      // units, entries, cut heads, units taken beyond the first of each block
+    int* first;                        // [B] first pair of a sequence, where they are too many for shared memory
+    PackedCut* cut;
     float *part, *part_ml;             // [slots][E / 4][256 rows][4] and [slots][256][2]: reference point, sum
     int sms;
     int* d_status;
 };
-enum { PC_NEXT = 0, PC_UNITS = 1, PC_ENTRIES = 2, PC_CUT = 3 };
 
 __device__ __forceinline__ float pk_ex2(float x) {
     float y;
@@ -100,7 +128,11 @@ struct PackedSeq {
 };
 
 // ------------------------------------------------------------------------------------------ the list of the work
-__device__ __forceinline__ int pk_block_scan(int x, int* sums, int& total) {   // exclusive, 1024 threads
+// One block, which the launch behind it waits for: sequences in shared memory, few barriers, no lane waits for another's atomic (10 to 31 us with
+// sequences in global memory and sums by atomics, 3 to 5 so).
+constexpr int PL_THREADS = 1024, PL_SEQS = 1024;    // sequences kept in shared memory
+
+__device__ __forceinline__ int pl_scan(int x, int* sums, int& total) {   // exclusive; sums: 32 of its own
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int upto = x;
 #pragma unroll
@@ -111,103 +143,152 @@ __device__ __forceinline__ int pk_block_scan(int x, int* sums, int& total) {   /
     __syncthreads();
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < 32; ++i) {
-        if (i < warp) before += sums[i];
-        total += sums[i];
+    const int mine = sums[lane];
+    int all = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, all, d);
+        if (lane >= d) all += y;
     }
-    return before + upto - x;
+    total = __shfl_sync(0xffffffffu, all, 31);
+    return __shfl_sync(0xffffffffu, all - mine, warp) + upto - x;
+}
+// One more in bucket b for each lane that is `on`; the lane's place in it.
+__device__ __forceinline__ int pl_count(int* bucket, int b, bool on) {
+    const unsigned same = __match_any_sync(0xffffffffu, on ? b : -1);
+    const int lane = threadIdx.x & 31, leader = __ffs(same) - 1;
+    int at = 0;
+    if (on && lane == leader) at = atomicAdd(&bucket[b], __popc(same));
+    return __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1));
 }
 
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(PL_THREADS)
 packed_plan_kernel(const PackedParams p) {
-    __shared__ int sums[32], bucket[PK_BUCKETS];
-    __shared__ unsigned long long blocks;
+    __shared__ int sums[32], bucket[PK_BUCKETS], first_here[PL_SEQS];
+    __shared__ int4 seqs[PL_SEQS];
+    static_assert(PK_BUCKETS == PL_THREADS, "a bucket a thread");
     const int tid = threadIdx.x;
     grid_dep_wait();
     grid_dep_launch();
-    // pairs of each sequence
+    const bool here = p.B <= PL_SEQS;
+    int* first = here ? first_here : p.first;
     int entries = 0;
-    for (int base = 0; base < p.B; base += 1024) {
-        int n = 0, total;
+    for (int base = 0; base < p.B; base += PL_THREADS) {
+        PackedSeq s = {0, 0, 0, 0};
+        if (base + tid < p.B) s.of(p, base + tid);
+        int total;
+        const int at = pl_scan(s.pairs(p), sums, total);
         if (base + tid < p.B) {
-            PackedSeq s;
-            s.of(p, base + tid);
-            n = s.pairs(p);
+            first[base + tid] = entries + at;
+            if (here) seqs[tid] = make_int4(s.q0, s.n, s.k0, s.m);
         }
-        const int at = pk_block_scan(n, sums, total);
-        if (base + tid < p.B) p.pairs[base + tid] = entries + at;
         entries = entries + total < p.most ? entries + total : p.most;      // sequences that overlap, which has been reported
-    }
-    if (tid == 0) {
-        p.pairs[p.B] = entries;
-        blocks = 0;
     }
     bucket[tid] = 0;
     __syncthreads();
-    unsigned long long mine = 0;
-    for (int e = tid; e < entries; e += 1024) {
+    auto entry = [&](int e, PackedSeq& s, int& pair, int& blocks) {
         int lo = 0, hi = p.B;          // the last sequence whose first pair is at or before e
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (p.pairs[mid] <= e) lo = mid;
+            if (first[mid] <= e) lo = mid;
             else hi = mid;
         }
+        if (here) {
+            const int4 x = seqs[lo];
+            s = {x.x, x.y, x.z, x.w};
+        } else {
+            s.of(p, lo);
+        }
+        pair = e - first[lo];
+        blocks = s.blocks(p, pair);
+    };
+    // Blocks of keys of all pairs and heads; what an SM's share of them is.  The first 1024 pairs stay in registers.
+    PackedSeq s0 = {0, 0, 0, 0};
+    int pair0 = 0, blocks0 = 0;
+    long long mine = 0;
+    for (int e = tid; e < entries; e += PL_THREADS) {
         PackedSeq s;
-        s.of(p, lo);
-        const int pair = e - p.pairs[lo], n = s.blocks(p, pair);
-        p.loose[e] = make_int4(lo, pair, n, 1);
+        int pair, n;
+        entry(e, s, pair, n);
+        if (e == tid) s0 = s, pair0 = pair, blocks0 = n;
         mine += n > 0 ? n : 1;
     }
-    if (mine) atomicAdd(&blocks, mine);
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    __shared__ long long total_of[32];
+    if ((tid & 31) == 0) total_of[tid >> 5] = mine;
     __syncthreads();
-    const unsigned long long all = blocks * p.heads;
-    for (int e = tid; e < entries; e += 1024) {
-        int4 x = p.loose[e];
-        // as many parts as it has SMs' shares: the parts of all that is cut are no more than the SMs
-        const int s = all > 0 ? (int)((unsigned long long)x.z * p.sms / all) : 1;
-        x.w = s > 1 ? s < x.z ? s : x.z : 1;
-        p.loose[e] = x;
-        const int size = x.z / x.w;
-        atomicAdd(&bucket[size < PK_BUCKETS ? PK_BUCKETS - 1 - size : 0], 1);
+    long long all = total_of[tid & 31];
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
+    all *= p.heads;
+    // As many parts as a pair has SMs' shares: the parts of all that is cut are no more than the SMs.
+    auto parts_of = [&](int blocks) {
+        const int s = all > 0 ? (int)((long long)blocks * p.sms / all) : 1;
+        return s > 1 ? s < blocks ? s : blocks : 1;
+    };
+    auto bucket_of = [&](int blocks, int parts) {
+        const int size = blocks / parts;
+        return size < PK_BUCKETS ? PK_BUCKETS - 1 - size : 0;
+    };
+    const int rounds = (entries + PL_THREADS - 1) / PL_THREADS;
+    bool cut = false;
+    for (int r = 0; r < rounds; ++r) {
+        const int e = r * PL_THREADS + tid;
+        PackedSeq s = s0;
+        int pair = pair0, n = blocks0;
+        if (r > 0 && e < entries) entry(e, s, pair, n);
+        const int parts = parts_of(n);
+        cut |= e < entries && parts > 1;
+        pl_count(bucket, bucket_of(n, parts), e < entries);
     }
-    __syncthreads();
+    const bool cuts = __syncthreads_or(cut);
     {
         int total;
-        const int n = bucket[tid], at = pk_block_scan(n, sums, total);
-        __syncthreads();
+        const int n = bucket[tid], at = pl_scan(n, sums, total);
         bucket[tid] = at;
     }
     __syncthreads();
-    for (int e = tid; e < entries; e += 1024) {
-        const int4 x = p.loose[e];
-        const int size = x.z / x.w;
-        p.entry[atomicAdd(&bucket[size < PK_BUCKETS ? PK_BUCKETS - 1 - size : 0], 1)] = x;
+    for (int r = 0; r < rounds; ++r) {
+        const int e = r * PL_THREADS + tid;
+        PackedSeq s = s0;
+        int pair = pair0, n = blocks0;
+        if (r > 0 && e < entries) entry(e, s, pair, n);
+        const int parts = parts_of(n), at = pl_count(bucket, bucket_of(n, parts), e < entries);
+        if (e < entries) {
+            int4* to = reinterpret_cast<int4*>(p.entry + at);
+            to[0] = make_int4(s.q0, s.n, s.k0, s.m);
+            to[1] = make_int4(pair, n, parts, 0);
+        }
     }
-    __syncthreads();
-    int units = 0, slots = 0, cuts = 0;
-    for (int base = 0; base < entries; base += 1024) {
-        const int e = base + tid, parts = e < entries ? p.entry[e].w : 0;
-        int total;
-        int at = pk_block_scan(parts * p.heads, sums, total);
-        if (e < entries) p.unit[e] = units + at;
-        units += total;
-        at = pk_block_scan(parts > 1 ? parts * p.heads : 0, sums, total);
-        if (e < entries) p.slot[e] = slots + at;
-        slots += total;
-        at = pk_block_scan(parts > 1 ? p.heads : 0, sums, total);
-        if (parts > 1)
-            for (int h = 0; h < p.heads; ++h) p.cut[cuts + at + h] = make_int4(e, h, 0, 0);
-        cuts += total;
+    int units = entries * p.heads, many = 0;
+    if (cuts) {
+        __syncthreads();
+        units = 0;
+        int slots = 0;
+        for (int base = 0; base < entries; base += PL_THREADS) {
+            const int e = base + tid;
+            PackedEntry x = {};
+            if (e < entries) x = p.entry[e];
+            int total;
+            int at = pl_scan(x.parts * p.heads, sums, total);
+            if (e < entries) p.unit[e] = units + at;
+            units += total;
+            at = pl_scan(x.parts > 1 ? x.parts * p.heads : 0, sums, total);
+            if (e < entries) p.slot[e] = slots + at;
+            const int slot = slots + at;
+            slots += total;
+            at = pl_scan(x.parts > 1 ? p.heads : 0, sums, total);
+            if (x.parts > 1)
+                for (int h = 0; h < p.heads; ++h) {
+                    int4* to = reinterpret_cast<int4*>(p.cut + many + at + h);
+                    to[0] = make_int4(slot + h * x.parts, x.parts, h, x.pair * 2 * p.T);
+                    to[1] = make_int4(x.q0, x.n, 0, 0);
+                }
+            many += total;
+        }
     }
-    if (tid == 0) {
-        p.unit[entries] = units;
-        p.counts[PC_NEXT] = 0;
-        p.counts[PC_UNITS] = units;
-        p.counts[PC_ENTRIES] = entries;
-        p.counts[PC_CUT] = cuts;
-    }
+    if (tid == 0) *p.counts = make_int4(units, entries, many, 0);
 }
 
 // A block's work: some of the key blocks of two tiles.
@@ -217,13 +298,10 @@ struct PackedPart {
     int j0, nblk, slot, more;    // key blocks; slot < 0: the whole of the item
 };
 
-__device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, int b, int pair, int head, int part, int parts, int slot) {
-    PackedSeq s;
-    s.of(p, b);
+__device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, const PackedSeq& s, int pair, int blocks, int head, int part, int parts, int slot) {
     x.q0 = s.q0, x.n = s.n, x.k0 = s.k0, x.m = s.m;
     x.h = head / p.groups, x.g0 = (head - x.h * p.groups) * p.G;
     x.token = pair * 2 * p.T;
-    const int blocks = s.blocks(p, pair);
     x.j0 = (int)((long long)part * blocks / parts);
     x.nblk = (int)((long long)(part + 1) * blocks / parts) - x.j0;
     x.slot = parts > 1 ? slot + head * parts + part : -1;
@@ -233,18 +311,27 @@ __device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, in
 // Unit `unit` of the list, found by a whole warp.
 __device__ __forceinline__ bool pk_listed(const PackedParams& p, int unit, PackedPart& x) {
     const int lane = threadIdx.x & 31;
-    if (unit >= p.counts[PC_UNITS]) return false;
-    int lo = 0, hi = p.counts[PC_ENTRIES];          // the last entry whose first unit is at or before this one
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const bool before = at < hi && p.unit[at] <= unit;
-        const int k = 31 - __clz(__ballot_sync(0xffffffffu, before));
-        lo += k * step;
-        hi = lo + step < hi ? lo + step : hi;
+    // where nothing is cut it is its pair's `heads` units on; asked for along with the counters
+    int e = unit / p.heads < p.most ? unit / p.heads : p.most - 1, slot = 0;
+    const int4 counts = *p.counts;
+    PackedEntry it = p.entry[e];
+    int rel = unit - e * p.heads;
+    if (unit >= counts.x) return false;
+    if (counts.z > 0) {
+        int lo = 0, hi = counts.y;          // the last entry whose first unit is at or before this one
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+            const bool before = at < hi && p.unit[at] <= unit;
+            const int k = 31 - __clz(__ballot_sync(0xffffffffu, before));
+            lo += k * step;
+            hi = lo + step < hi ? lo + step : hi;
+        }
+        it = p.entry[lo];
+        rel = unit - p.unit[lo];
+        slot = p.slot[lo];
     }
-    const int4 e = p.entry[lo];
-    const int rel = unit - p.unit[lo], part = rel / p.heads;
-    pk_part(p, x, e.x, e.y, rel - part * p.heads, part, e.w, p.slot[lo]);
+    const int part = rel / p.heads;
+    pk_part(p, x, PackedSeq{it.q0, it.n, it.k0, it.m}, it.pair, it.blocks, rel - part * p.heads, part, it.parts, slot);
     return true;
 }
 // Pair `pair` of all sequences' in order, without a list.
@@ -252,12 +339,9 @@ __device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, Packe
     const int lane = threadIdx.x & 31, pair = unit / p.heads;
     int before = 0;
     for (int base = 0; base < p.B; base += 32) {
-        int n = 0;
-        if (base + lane < p.B) {
-            PackedSeq s;
-            s.of(p, base + lane);
-            n = s.pairs(p);
-        }
+        PackedSeq s = {0, 0, 0, 0};
+        if (base + lane < p.B) s.of(p, base + lane);
+        const int n = s.pairs(p);
         int upto = n;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -267,7 +351,9 @@ __device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, Packe
         const unsigned past = __ballot_sync(0xffffffffu, before + upto > pair);
         if (past) {
             const int k = __ffs(past) - 1;
-            pk_part(p, x, base + k, pair - before - __shfl_sync(0xffffffffu, upto - n, k), unit - pair * p.heads, 0, 1, 0);
+            const int at = pair - before - __shfl_sync(0xffffffffu, upto - n, k);
+            for (int* v : {&s.q0, &s.n, &s.k0, &s.m}) *v = __shfl_sync(0xffffffffu, *v, k);
+            pk_part(p, x, s, at, s.blocks(p, at), unit - pair * p.heads, 0, 1, 0);
             return true;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -279,8 +365,11 @@ template <int EP> struct PkCfg {
     static constexpr int ATOMS = EP / 64;
     static constexpr int SIDE = ATOMS * PK_ATOM;                 // an operand tile
     static constexpr bool OWN_P = EP == 64;                      // P beside S in tensor memory; else over S
-    static constexpr int STAGES = OWN_P ? 10 : 5;                // K(0), V(0), K(1), ...
-    static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_BARS = S_KV + STAGES * SIDE;
+    static constexpr int STAGES = OWN_P ? 8 : 4;                 // K(0), V(0), K(1), ...
+    static constexpr int POLY = OWN_P ? 8 : 4;                   // every POLYth pair of exponentials is a polynomial
+    static constexpr int FIRST = 3;                              // quarters of P that P V does not wait for the rest with, where P lies over S
+    static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_OUT = S_KV + STAGES * SIDE;   // operands, rows on their way out (4 KB a warp)
+    static constexpr int S_BARS = S_OUT + 8 * 4096;
     static constexpr int BARRIERS = 2 * 2 + 3 * STAGES + 2 * 6 + 2 * PK_PARTS;
     static constexpr int S_PART = S_BARS + (BARRIERS + 1) * 8;
     static constexpr int SMEM = S_PART + PK_PARTS * (int)sizeof(PackedPart) + 16;
@@ -288,6 +377,16 @@ template <int EP> struct PkCfg {
     static_assert(SMEM <= 232448, "shared memory over budget");
 };
 
+// Of 16 bytes of a row's results what is left of the row, number by number.
+__device__ __noinline__ void pk_store_some(char* d, int left, int log, const uint4 x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < left && i < 16 >> log) {
+            if (log == 2) reinterpret_cast<uint32_t*>(d)[i] = w[i & 3];
+            else reinterpret_cast<uint16_t*>(d)[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+        }
+}
 __device__ __forceinline__ void pk_store8(const PackedParams& p, int64_t at, int count, const float (&v)[8]) {   // eight results of a row, or fewer
     if (p.out_whole && count >= 8) {
         if (p.out_f32) {
@@ -424,7 +523,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 __syncwarp();
                 if (!some) break;
                 if (p.planned) {          // on its way while this part's operands are asked for
-                    if (lane == 0) unit = gridDim.x + atomicAdd(&p.counts[PC_NEXT], 1);
+                    if (lane == 0) unit = gridDim.x + atomicAdd(&p.counts->w, 1);
                     unit = __shfl_sync(0xffffffffu, unit, 0);
                 }
                 if (it.nblk == 0) continue;
@@ -468,27 +567,41 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                          wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
                     if (!ok) break;
                     if (key0 + PK_KEYS - 1 > see) {       // some row does not see some key: 0 times what is not finite is no zero
-                        uint4* tile = reinterpret_cast<uint4*>(smem + Cfg::S_KV + st * Cfg::SIDE);
-                        bool mine = false;
-#pragma unroll 4
-                        for (int c = lane; c < Cfg::SIDE / 16; c += 32) {
-                            uint4 x = tile[c];
-                            const uint32_t hit = ((x.x & 0x7fff7fffu) + 0x04000400u) | ((x.y & 0x7fff7fffu) + 0x04000400u) |
-                                                 ((x.z & 0x7fff7fffu) + 0x04000400u) | ((x.w & 0x7fff7fffu) + 0x04000400u);
-                            if (hit & 0x80008000u) {
-                                uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+                        // Keys from here on some row does not see.  A number times 0 is 0, anything else a NaN that stays one in a sum.
+                        const int from = see < key0 ? 0 : see + 1 - key0;
+                        uint8_t* tile = smem + Cfg::S_KV + st * Cfg::SIDE;
+                        const __half2 zero = __half2half2(__ushort_as_half(0));
+                        __half2 sum[4] = {zero, zero, zero, zero};
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    const uint32_t bad = ((w[k] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
-                                    w[k] &= ~((bad >> 15) * 0xffffu);
-                                }
-                                tile[c] = x;
-                                mine |= key0 + (c % (PK_ATOM / 16)) / 8 < it.m;      // a key of this sequence
+                        for (int a = 0; a < ATOMS; ++a) {
+                            const uint4* row = reinterpret_cast<const uint4*>(tile + a * PK_ATOM);
+#pragma unroll 8
+                            for (int c = from * 8 + lane; c < 128 * 8; c += 32) {
+                                const uint4 x = row[c];
+                                sum[0] = __hfma2(*reinterpret_cast<const __half2*>(&x.x), zero, sum[0]);
+                                sum[1] = __hfma2(*reinterpret_cast<const __half2*>(&x.y), zero, sum[1]);
+                                sum[2] = __hfma2(*reinterpret_cast<const __half2*>(&x.z), zero, sum[2]);
+                                sum[3] = __hfma2(*reinterpret_cast<const __half2*>(&x.w), zero, sum[3]);
                             }
                         }
-                        if (__any_sync(0xffffffffu, mine) && key0 < first) {
-                            first = key0;
-                            if (lane == 0) odd[s] = it.j0 + j;
+                        const __half2 any = __hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3]));
+                        if (__any_sync(0xffffffffu, __hisnan(__low2half(any)) || __hisnan(__high2half(any)))) {
+                            bool mine = false;
+#pragma unroll 1
+                            for (int i2 = from * 32 + lane; i2 < 128 * 32; i2 += 32)       // by words of two
+#pragma unroll
+                                for (int a = 0; a < ATOMS; ++a) {
+                                    uint32_t* w = reinterpret_cast<uint32_t*>(tile + a * PK_ATOM) + i2;
+                                    const uint32_t bad = ((*w & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+                                    if (bad) {
+                                        *w &= ~((bad >> 15) * 0xffffu);
+                                        mine |= key0 + i2 / 32 < it.m;      // a key of this sequence
+                                    }
+                                }
+                            if (__any_sync(0xffffffffu, mine) && key0 < first) {
+                                first = key0;
+                                if (lane == 0) odd[s] = it.j0 + j;
+                            }
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
@@ -558,14 +671,14 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                         ok = wait(&p_half[t], ph, KST_WAIT_SOFTMAX);
                         if (!ok) break;
                         tc_fence_after();
-                        if (elect_one()) issue_pv(j, st, 0, 4);
+                        if (elect_one()) issue_pv(j, st, 0, 2 * Cfg::FIRST);
                         __syncwarp();
                     }
                     ok = ok && wait(&p_full[t], ph, KST_WAIT_SOFTMAX);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        issue_pv(j, st, HALVES ? 4 : 0, 8);
+                        issue_pv(j, st, HALVES ? 2 * Cfg::FIRST : 0, 8);
                         umma_commit(&pv_done[t]);
                         umma_commit(&empty[st]);
                     }
@@ -657,33 +770,55 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     }
                     m_run = m_new;
                 }
-                if (pingpong && (t == 1 || turns > 0) &&
+                if (pingpong && (!OWN_P || j == 0) && (t == 1 || turns > 0) &&
                     !wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), KST_WAIT_SOFTMAX)) { ok = false; break; }
                 const float m_sub = m_new == -INFINITY ? 0.f : 7.f - m_new;
                 const uint64_t a2 = pack2(m_sub, m_sub);
                 uint64_t sum0 = pack2(0.f, 0.f), sum1 = pack2(0.f, 0.f);
+                if (!OWN_P) {      // all exponents first
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 32; u += 2) {
+                            float e0, e1;
+                            unpack2(fma2(pack2(__uint_as_float(x[i][u]), __uint_as_float(x[i][u + 1])), k2, a2), e0, e1);
+                            x[i][u] = __float_as_uint(e0), x[i][u + 1] = __float_as_uint(e1);
+                            asm volatile("" : "+r"(x[i][u]), "+r"(x[i][u + 1]));
+                        }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) {
                         float e0, e1;
-                        unpack2(fma2(pack2(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1])), k2, a2), e0, e1);
-                        e0 = pk_ex2(e0), e1 = pk_ex2(e1);
+                        uint64_t y = pack2(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1]));
+                        if (OWN_P) y = fma2(y, k2, a2);
+                        if (u % Cfg::POLY == Cfg::POLY - 1) {
+                            pk_exp2(y, e0, e1);
+                        } else {
+                            unpack2(y, e0, e1);
+                            e0 = pk_ex2(e0), e1 = pk_ex2(e1);
+                        }
+                        x[i][2 * u] = __float_as_uint(e0), x[i][2 * u + 1] = __float_as_uint(e1);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 16; ++u) {
+                        const float e0 = __uint_as_float(x[i][2 * u]), e1 = __uint_as_float(x[i][2 * u + 1]);
                         if (u & 1) sum1 = add2(sum1, pack2(e0, e1));
                         else sum0 = add2(sum0, pack2(e0, e1));
                         const __half2 h = __floats2half2_rn(e0, e1);
                         pk[u] = *reinterpret_cast<const uint32_t*>(&h);
                     }
                     pk_tmem_st16(p_tmem + i * 16, pk);
-                    if (HALVES && i == 1) {
+                    if (HALVES && i == Cfg::FIRST - 1) {
                         tmem_wait_st();
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&p_half[t]);
                     }
                 }
-                if (pingpong) {
+                if (pingpong && (!OWN_P || j == 0)) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&exp_turn[1 - t]);
                     ++turns;
@@ -696,51 +831,87 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 unpack2(add2(sum0, sum1), s0, s1);
                 l_run += s0 + s1;
             }
+            const float f = it.slot >= 0 || l_run == 0.f ? 1.f : 1.f / l_run;
+            // Whole results go out 128 bytes of a row at a time through shared memory of the warp's own, so that a store is of four rows' whole
+            // lines: this lane's are rows lane / 8, lane / 8 + 4, ...
+            const int64_t at = (int64_t)(it.q0 + l) * p.oN + (int64_t)(it.h * p.share + it.g0 + g) * p.oH;
+            const unsigned lives = __ballot_sync(0xffffffffu, live) >> (lane >> 3);
+            const int log = p.out_f32 ? 2 : 1, each = 16 >> log, wide = 128 >> log;       // columns of 16 bytes, of a round
+            char* row_out[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row_out[i] = (char*)p.out + (__shfl_sync(0xffffffffu, at, i * 4 + (lane >> 3)) << log);
+            const uint32_t stage = smem_u32(smem + Cfg::S_OUT + warp * 4096), mine = stage + lane * 128, swz = (uint32_t)(lane & 7) << 4;
+            const uint32_t theirs = stage + (lane >> 3) * 128, other = (uint32_t)(lane & 7) << 4 ^ (uint32_t)(lane >> 3) << 4;   // rows 4 apart: the swizzle's upper bit turns
             if (ok && it.nblk > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);
             if (!ok) break;
             tc_fence_after();
-            const float f = it.slot >= 0 || l_run == 0.f ? 1.f : 1.f / l_run;
-            const int64_t at = (int64_t)(it.q0 + l) * p.oN + (int64_t)(it.h * p.share + it.g0 + g) * p.oH;
-            const int prow = t * PK_ROWS + row;
             const int bad = *reinterpret_cast<volatile int*>(&odd[s]);      // written before the last P V was issued
 #pragma unroll 1
-            for (int i = 0; i < EP / 16; ++i) {
-                uint32_t o16[16];
+            for (int e = 0; e < p.E; e += 32) {
+                uint32_t o[32];
                 __syncwarp();
                 if (it.nblk > 0) {
-                    tmem_ld16(o_tmem + i * 16, o16);
+                    tmem_ld32(o_tmem + e, o);
                     tmem_wait_ld();
                 } else {
 #pragma unroll
-                    for (int u = 0; u < 16; ++u) o16[u] = 0;
+                    for (int u = 0; u < 32; ++u) o[u] = 0;
                 }
-                if (!live || i * 16 >= p.E) continue;
-                float v[2][8];
 #pragma unroll
-                for (int u = 0; u < 16; ++u) v[u >> 3][u & 7] = __uint_as_float(o16[u]) * f;
-                if (bad != 0x7fffffff) {        // what was taken out, for those who see it
+                for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
+                if (bad != 0x7fffffff && live) {        // what was taken out, for those who see it
                     const int end = (it.j0 + it.nblk) * PK_KEYS - 1 < last ? (it.j0 + it.nblk) * PK_KEYS - 1 : last;
 #pragma unroll 1
-                    for (int key = bad * PK_KEYS; key <= end; ++key) {
-                        const __half* q = p.v + (int64_t)(it.k0 + key) * p.vN + it.h * p.vH + i * 16;
+                    for (int key = max(bad * PK_KEYS, all_see(it.token) + 1); key <= end; ++key) {
+                        const __half* q = p.v + (int64_t)(it.k0 + key) * p.vN + it.h * p.vH + e;
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) {
-                            if (i * 16 + u >= p.E) break;
+                        for (int u = 0; u < 32; ++u) {
+                            if (e + u >= p.E) break;
                             const float y = __half2float(q[u]);
-                            if (!(fabsf(y) < INFINITY)) v[u >> 3][u & 7] += y;
+                            if (!(fabsf(y) < INFINITY)) o[u] = __float_as_uint(__uint_as_float(o[u]) + y);
                         }
                     }
                 }
+                __syncwarp();
                 if (it.slot >= 0) {
-                    float4* d = reinterpret_cast<float4*>(p.part + (int64_t)it.slot * (2 * PK_ROWS * EP)) + i * 4 * (2 * PK_ROWS) + prow;
+                    float4* d = reinterpret_cast<float4*>(p.part + (int64_t)it.slot * (2 * PK_ROWS * EP)) + e * (PK_ROWS / 2) + t * PK_ROWS + row;
+                    if (live)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) d[u * 2 * PK_ROWS] = make_float4(v[u >> 1][(u & 1) * 4], v[u >> 1][(u & 1) * 4 + 1], v[u >> 1][(u & 1) * 4 + 2], v[u >> 1][(u & 1) * 4 + 3]);
+                        for (int u = 0; u < 8; ++u)
+                            if (e + 4 * u < p.E) d[u * 2 * PK_ROWS] = make_float4(__uint_as_float(o[4 * u]), __uint_as_float(o[4 * u + 1]), __uint_as_float(o[4 * u + 2]), __uint_as_float(o[4 * u + 3]));
+                    continue;
+                }
+                if (p.out_f32) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) st_shared_v4(mine + ((uint32_t)(c << 4) ^ swz), o + 4 * c);
                 } else {
-                    pk_store8(p, at + i * 16, p.E - i * 16, v[0]);
-                    pk_store8(p, at + i * 16 + 8, p.E - i * 16 - 8, v[1]);
+                    const uint32_t half = (e & 32) << 1;          // which half of the row's 128 bytes
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const __half2 h = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * u]), __uint_as_float(o[8 * c + 2 * u + 1]));
+                            w[u] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        st_shared_v4(mine + ((half | (uint32_t)(c << 4)) ^ swz), w);
+                    }
+                    if ((e & 32) == 0 && e + 32 < p.E) continue;      // the other half first
+                }
+                __syncwarp();
+                const int first = e & ~(wide - 1), column = first + (lane & 7) * each;
+                const int left = p.E - column;                   // of the row, from this lane's 16 bytes on
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t w[4];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(theirs + i * 512 + (other ^ (uint32_t)(i & 1) << 6)) : "memory");
+                    if ((lives >> (4 * i) & 1) == 0 || left <= 0) continue;
+                    char* d = row_out[i] + (column << log);
+                    if (p.out_whole && left >= each) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+                    else pk_store_some(d, left, log, make_uint4(w[0], w[1], w[2], w[3]));
                 }
             }
-            if (live && it.slot >= 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)it.slot * 2 * PK_ROWS + prow) * 2) = make_float2(m_run, l_run);
+            if (live && it.slot >= 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)it.slot * 2 * PK_ROWS + t * PK_ROWS + row) * 2) = make_float2(m_run, l_run);
             tc_fence_before();           // the next part's first P V writes O over
         }
     }
@@ -762,18 +933,17 @@ packed_join_kernel(const PackedParams p) {
     grid_dep_wait();
     grid_dep_launch();
     const int i = blockIdx.x / (EP / 16), e = (int)(blockIdx.x % (EP / 16)) * 16, prow = threadIdx.x;
-    if (i >= p.counts[PC_CUT] || e >= p.E) return;
-    const int4 at = p.cut[i], x = p.entry[at.x];
-    PackedSeq s;
-    s.of(p, x.x);
-    const int h = at.y / p.groups, g0 = (at.y - h * p.groups) * p.G;
-    const int t = prow / PK_ROWS, row = prow - t * PK_ROWS, l0 = p.by_g.div(row), g = row - l0 * p.G, l = (x.y * 2 + t) * p.T + l0;
-    if (l0 >= p.T || l >= s.n || g0 + g >= p.share) return;
-    const int64_t slot = p.slot[at.x] + at.y * x.w;
+    const int4 counts = *p.counts;
+    const PackedCut x = p.cut[i];                 // there is room for as many as there are blocks of this launch
+    if (i >= counts.z || e >= p.E) return;
+    const int h = x.head / p.groups, g0 = (x.head - h * p.groups) * p.G;
+    const int t = prow / PK_ROWS, row = prow - t * PK_ROWS, l0 = p.by_g.div(row), g = row - l0 * p.G, l = x.token + t * p.T + l0;
+    if (l0 >= p.T || l >= x.n || g0 + g >= p.share) return;
+    const int64_t slot = x.slot;
     auto stat = [&](int w) { return *reinterpret_cast<const float2*>(p.part_ml + ((slot + w) * 2 * PK_ROWS + prow) * 2); };
     float M = -INFINITY, sum = 0.f, v[2][8] = {};
-    for (int w = 0; w < x.w; ++w) M = fmaxf(M, stat(w).x);
-    for (int w = 0; w < x.w; ++w) {
+    for (int w = 0; w < x.parts; ++w) M = fmaxf(M, stat(w).x);
+    for (int w = 0; w < x.parts; ++w) {
         const float2 ml = stat(w);
         const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
         const float4* y = reinterpret_cast<const float4*>(p.part + (slot + w) * (2 * PK_ROWS * EP)) + e / 4 * (2 * PK_ROWS) + prow;
@@ -788,7 +958,7 @@ packed_join_kernel(const PackedParams p) {
     const float inv = sum == 0.f ? 1.f : 1.f / sum;
 #pragma unroll
     for (int k = 0; k < 16; ++k) v[k >> 3][k & 7] *= inv;
-    const int64_t to = (int64_t)(s.q0 + l) * p.oN + (int64_t)(h * p.share + g0 + g) * p.oH + e;
+    const int64_t to = (int64_t)(x.q0 + l) * p.oN + (int64_t)(h * p.share + g0 + g) * p.oH + e;
     pk_store8(p, to, p.E - e, v[0]);
     pk_store8(p, to + 8, p.E - e - 8, v[1]);
 }
@@ -838,7 +1008,7 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     const int64_t slots = sms, rows = slots * 2 * PK_ROWS;
     if (p.planned) {
         void* ws = nullptr;
-        const size_t list = (size_t)(entries + 1) * (2 * sizeof(int4) + 2 * sizeof(int)) + (p.B + 1) * sizeof(int) + slots * sizeof(int4) + 64 + 16 * 8;
+        const size_t list = (size_t)entries * (sizeof(PackedEntry) + 2 * sizeof(int)) + p.B * sizeof(int) + slots * sizeof(PackedCut) + sizeof(int4) + 16 * 8;
         rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float) + list, &ws);
         if (rc) return rc;
         uint8_t* at = static_cast<uint8_t*>(ws);
@@ -849,14 +1019,13 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
         };
         p.part = (float*)room(rows * EP * sizeof(float));
         p.part_ml = (float*)room(rows * 2 * sizeof(float));
-        p.entry = (int4*)room((entries + 1) * sizeof(int4));
-        p.loose = (int4*)room((entries + 1) * sizeof(int4));
-        p.cut = (int4*)room(slots * sizeof(int4));
-        p.unit = (int*)room((entries + 1) * sizeof(int));
-        p.slot = (int*)room((entries + 1) * sizeof(int));
-        p.pairs = (int*)room((p.B + 1) * sizeof(int));
-        p.counts = (int*)room(64);
-        B200_CUDA(launch_dep(packed_plan_kernel, dim3(1), dim3(1024), 0, ctx->stream, 1, p));
+        p.entry = (PackedEntry*)room(entries * sizeof(PackedEntry));
+        p.cut = (PackedCut*)room(slots * sizeof(PackedCut));
+        p.counts = (int4*)room(sizeof(int4));
+        p.unit = (int*)room(entries * sizeof(int));
+        p.slot = (int*)room(entries * sizeof(int));
+        p.first = (int*)room(p.B * sizeof(int));
+        B200_CUDA(launch_dep(packed_plan_kernel, dim3(1), dim3(PL_THREADS), 0, ctx->stream, 1, p));
         ctx->launches++;
     }
     const int64_t grid = p.planned ? sms : items;
