@@ -13,6 +13,7 @@
 //   warp 8     finds the block's next part of the work (below), tells the others, and asks for Q, K and V
 //   warps 9, 10  issue one tile's products each:  Q K(0)', P(0) V(0), Q K(1)', ...
 //   warp 11    hands V on to them; where a row does not see a key of the block, it first takes out of the tile what is not finite
+//   warps 12-15  take both tiles' results out while the softmax is at the next part
 //
 // Lengths are on the device, so the work is listed there: the row pairs of all sequences, longest first, those that are longer than an
 // SM's share cut along their keys (packed_plan_kernel).  Blocks take the list's units in order as they become free; a second launch joins what
@@ -24,12 +25,12 @@
 
 namespace b200 {
 
-constexpr int PK_THREADS = 384;
+constexpr int PK_THREADS = 512;
 constexpr int PK_ROWS = 128, PK_KEYS = 128;      // of a tile
 constexpr int PK_ATOM = 128 * 128;               // 128 rows x 64 fp16
-constexpr int PK_PARTS = 2;                      // parts of the work on their way from warp 8 to the others
-constexpr int PK_SOFTMAX_REGS = 224, PK_OTHER_REGS = 56;
-static_assert(256 * PK_SOFTMAX_REGS + 128 * PK_OTHER_REGS <= PK_THREADS * 168, "what the launch holds");
+constexpr int PK_PARTS = 3;                      // parts of the work on their way from warp 8 to the others
+constexpr int PK_SOFTMAX_REGS = 184, PK_OTHER_REGS = 48, PK_OUT_REGS = 88;
+static_assert(256 * PK_SOFTMAX_REGS + 128 * PK_OTHER_REGS + 128 * PK_OUT_REGS <= PK_THREADS * 128, "what the launch holds");
 constexpr int PK_BUCKETS = 1024;                 // lengths that the list tells apart
 
 // 2^x of two numbers in the units of the FMAs, without the exponential unit: x = n + f, 2^f by a polynomial of degree 4 (the one of least largest
@@ -49,6 +50,17 @@ __device__ __forceinline__ void pk_exp2(uint64_t x2, float& e0, float& e1) {
     unpack2(t, t0, t1);
     e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
     e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// mbar_wait in as few instructions as it takes: what the roles of a block run through, all together, has to fit the nearer instruction caches.  A
+// try sleeps for 1.5 us at most, so that the tries end after some three seconds; why is left in shared memory, for the block's end.
+constexpr uint32_t PK_TRIES = 1u << 21;
+__device__ __forceinline__ bool pk_wait(uint64_t* bar, uint32_t parity, int code, volatile int* why) {
+#pragma unroll 1
+    for (uint32_t n = PK_TRIES; n != 0; --n)
+        if (mbar_try_wait(bar, parity)) return true;
+    *why = code;
+    return false;
 }
 
 struct __align__(16) PackedEntry {
@@ -298,27 +310,36 @@ struct PackedPart {
     int j0, nblk, slot, more;    // key blocks; slot < 0: the whole of the item
 };
 
-__device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, const PackedSeq& s, int pair, int blocks, int head, int part, int parts, int slot) {
-    x.q0 = s.q0, x.n = s.n, x.k0 = s.k0, x.m = s.m;
-    x.h = head / p.groups, x.g0 = (head - x.h * p.groups) * p.G;
-    x.token = pair * 2 * p.T;
-    x.j0 = (int)((long long)part * blocks / parts);
-    x.nblk = (int)((long long)(part + 1) * blocks / parts) - x.j0;
-    x.slot = parts > 1 ? slot + head * parts + part : -1;
-    x.more = 1;
+// A unit of the work: a part of the keys of a row pair, for one group of heads of a key head.
+struct PackedUnit {
+    PackedSeq s;
+    int pair, blocks, head, part, parts, slot;
+};
+__device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, const PackedUnit& u) {
+    x.q0 = u.s.q0, x.n = u.s.n, x.k0 = u.s.k0, x.m = u.s.m;
+    x.h = u.head / p.groups, x.g0 = (u.head - x.h * p.groups) * p.G;
+    x.token = u.pair * 2 * p.T;
+    x.j0 = 0, x.nblk = u.blocks, x.slot = -1;
+    if (u.parts > 1) {      // no more parts than SMs, fewer than 2^23 blocks
+        x.j0 = (int)((unsigned)(u.part * u.blocks) / (unsigned)u.parts);
+        x.nblk = (int)((unsigned)((u.part + 1) * u.blocks) / (unsigned)u.parts) - x.j0;
+        x.slot = u.slot + u.head * u.parts + u.part;
+    }
 }
 
 // Unit `unit` of the list, found by a whole warp.
-__device__ __forceinline__ bool pk_listed(const PackedParams& p, int unit, PackedPart& x) {
+__device__ __forceinline__ bool pk_listed(const PackedParams& p, int unit, PackedUnit& x) {
     const int lane = threadIdx.x & 31;
     // where nothing is cut it is its pair's `heads` units on; asked for along with the counters
-    int e = unit / p.heads < p.most ? unit / p.heads : p.most - 1, slot = 0;
+    int e = unit / p.heads, rel = unit - e * p.heads;
+    e = e < p.most ? e : p.most - 1;
     const int4 counts = *p.counts;
     PackedEntry it = p.entry[e];
-    int rel = unit - e * p.heads;
     if (unit >= counts.x) return false;
+    x.part = 0, x.slot = 0;
     if (counts.z > 0) {
         int lo = 0, hi = counts.y;          // the last entry whose first unit is at or before this one
+#pragma unroll 1
         while (hi - lo > 1) {
             const int step = (hi - lo + 31) / 32, at = lo + lane * step;
             const bool before = at < hi && p.unit[at] <= unit;
@@ -328,16 +349,19 @@ __device__ __forceinline__ bool pk_listed(const PackedParams& p, int unit, Packe
         }
         it = p.entry[lo];
         rel = unit - p.unit[lo];
-        slot = p.slot[lo];
+        x.part = rel / p.heads;
+        rel -= x.part * p.heads;
+        x.slot = p.slot[lo];
     }
-    const int part = rel / p.heads;
-    pk_part(p, x, PackedSeq{it.q0, it.n, it.k0, it.m}, it.pair, it.blocks, rel - part * p.heads, part, it.parts, slot);
+    x.s = {it.q0, it.n, it.k0, it.m};
+    x.pair = it.pair, x.blocks = it.blocks, x.parts = it.parts, x.head = rel;
     return true;
 }
-// Pair `pair` of all sequences' in order, without a list.
-__device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, PackedPart& x) {
+// Without a list: the row pairs of all sequences in their order.
+__device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, PackedUnit& x) {
     const int lane = threadIdx.x & 31, pair = unit / p.heads;
     int before = 0;
+#pragma unroll 1
     for (int base = 0; base < p.B; base += 32) {
         PackedSeq s = {0, 0, 0, 0};
         if (base + lane < p.B) s.of(p, base + lane);
@@ -351,9 +375,11 @@ __device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, Packe
         const unsigned past = __ballot_sync(0xffffffffu, before + upto > pair);
         if (past) {
             const int k = __ffs(past) - 1;
-            const int at = pair - before - __shfl_sync(0xffffffffu, upto - n, k);
+            x.pair = pair - before - __shfl_sync(0xffffffffu, upto - n, k);
             for (int* v : {&s.q0, &s.n, &s.k0, &s.m}) *v = __shfl_sync(0xffffffffu, *v, k);
-            pk_part(p, x, s, at, s.blocks(p, at), unit - pair * p.heads, 0, 1, 0);
+            x.s = s;
+            x.blocks = s.blocks(p, x.pair), x.head = unit - pair * p.heads;
+            x.part = 0, x.parts = 1, x.slot = 0;
             return true;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -366,27 +392,18 @@ template <int EP> struct PkCfg {
     static constexpr int SIDE = ATOMS * PK_ATOM;                 // an operand tile
     static constexpr bool OWN_P = EP == 64;                      // P beside S in tensor memory; else over S
     static constexpr int STAGES = OWN_P ? 8 : 4;                 // K(0), V(0), K(1), ...
-    static constexpr int POLY = OWN_P ? 8 : 4;                   // every POLYth pair of exponentials is a polynomial
+    static constexpr int POLY = 4;                               // every POLYth pair of exponentials is a polynomial
     static constexpr int FIRST = 3;                              // quarters of P that P V does not wait for the rest with, where P lies over S
-    static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_OUT = S_KV + STAGES * SIDE;   // operands, rows on their way out (4 KB a warp)
-    static constexpr int S_BARS = S_OUT + 8 * 4096;
-    static constexpr int BARRIERS = 2 * 2 + 3 * STAGES + 2 * 6 + 2 * PK_PARTS;
+    static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_OUT = S_KV + STAGES * SIDE;   // operands; 128 bytes of a tile's rows on their way out, twice
+    static constexpr int S_STAT = S_OUT + 2 * PK_ATOM;           // a row's reference point and sum
+    static constexpr int S_BARS = S_STAT + 2 * PK_ROWS * 8;
+    static constexpr int BARRIERS = 2 * 2 + 3 * STAGES + 2 * 8 + 2 * PK_PARTS;
     static constexpr int S_PART = S_BARS + (BARRIERS + 1) * 8;
-    static constexpr int SMEM = S_PART + PK_PARTS * (int)sizeof(PackedPart) + 16;
+    static constexpr int SMEM = S_PART + PK_PARTS * ((int)sizeof(PackedPart) + 4);
     static constexpr int O_COL = 2 * PK_KEYS, P_COL = O_COL + 2 * EP;
     static_assert(SMEM <= 232448, "shared memory over budget");
 };
 
-// Of 16 bytes of a row's results what is left of the row, number by number.
-__device__ __noinline__ void pk_store_some(char* d, int left, int log, const uint4 x) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < left && i < 16 >> log) {
-            if (log == 2) reinterpret_cast<uint32_t*>(d)[i] = w[i & 3];
-            else reinterpret_cast<uint16_t*>(d)[i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-        }
-}
 __device__ __forceinline__ void pk_store8(const PackedParams& p, int64_t at, int count, const float (&v)[8]) {   // eight results of a row, or fewer
     if (p.out_whole && count >= 8) {
         if (p.out_f32) {
@@ -413,7 +430,7 @@ __device__ __forceinline__ void pk_store8(const PackedParams& p, int64_t at, int
 template <int EP>
 __global__ void __launch_bounds__(PK_THREADS, 1)
 attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_constant__ CUtensorMap tmapK,
-                        const __grid_constant__ CUtensorMap tmapV, const PackedParams p) {
+                        const __grid_constant__ CUtensorMap tmapV, const __grid_constant__ CUtensorMap tmapO, const PackedParams p) {
     using Cfg = PkCfg<EP>;
     constexpr int STAGES = Cfg::STAGES, ATOMS = Cfg::ATOMS;
     constexpr bool OWN_P = Cfg::OWN_P, HALVES = !OWN_P;
@@ -434,16 +451,19 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
     uint64_t* p_full = p_half + 2;                 // [2] all of it
     uint64_t* pv_done = p_full + 2;                // [2] its last product
     uint64_t* exp_turn = pv_done + 2;              // [2] whose turn it is to run its exponentials
-    uint64_t* a_full = exp_turn + 2;               // [PK_PARTS] a part of the work
+    uint64_t* o_full = exp_turn + 2;               // [2] a part's row sums are there, and the last of its P
+    uint64_t* o_empty = o_full + 2;                // [2] they and O have been read
+    uint64_t* a_full = o_empty + 2;                // [PK_PARTS] a part of the work
     uint64_t* a_empty = a_full + PK_PARTS;         // every other warp
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(a_empty + PK_PARTS);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* why = reinterpret_cast<volatile int*>(tmem_slot + 1);       // 0, or the code of a wait that ran out
     PackedPart* part = reinterpret_cast<PackedPart*>(smem + Cfg::S_PART);
     int* odd = reinterpret_cast<int*>(part + PK_PARTS);   // [PK_PARTS] the first key block of a part from which something was taken out
-    static_assert(Cfg::BARRIERS == 4 + 3 * STAGES + 12 + 2 * PK_PARTS, "barriers counted by the layout");
+    static_assert(Cfg::BARRIERS == 4 + 3 * STAGES + 16 + 2 * PK_PARTS, "barriers counted by the layout");
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 1);
             mbar_init(&q_empty[t], 1);
@@ -453,17 +473,21 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
             mbar_init(&p_full[t], 4);
             mbar_init(&pv_done[t], 1);
             mbar_init(&exp_turn[t], 4);
+            mbar_init(&o_full[t], 4);
+            mbar_init(&o_empty[t], 4);
         }
+#pragma unroll 1
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&ready[s], 1);
             mbar_init(&empty[s], 2);
         }
+#pragma unroll 1
         for (int s = 0; s < PK_PARTS; ++s) {
             mbar_init(&a_full[s], 1);
             mbar_init(&a_empty[s], PK_THREADS / 32 - 1);
         }
-        *abort_flag = 0;
+        *why = 0;
         fence_barrier_init();
         prefetch_tmap(&tmapQ);
         prefetch_tmap(&tmapK);
@@ -482,7 +506,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
 
     // A warp leaves a wait that runs out as one: lanes that went on alone would wait for the others in the next vote, for good.
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) -> bool {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.d_status, code, abort_flag));
+        return __all_sync(0xffffffffu, pk_wait(bar, parity, code, why));
     };
     PackedPart it;
     int parts_seen = 0;
@@ -503,16 +527,191 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
     // The last key that every row of both tiles sees; blocks that end behind it are masked.
     auto all_see = [&](int token) { return p.causal && it.m - it.n + token < it.m - 1 ? it.m - it.n + token : it.m - 1; };
 
-    if (warp >= 8) {
+    float2* stats = reinterpret_cast<float2*>(smem + Cfg::S_STAT);
+    // A row of a tile: its token in the tile, its head.  Which rows are any sequence's, and the last key that each sees.
+    auto live_row = [&](int t, int l0, int g) { return l0 < p.T && it.token + t * p.T + l0 < it.n && it.g0 + g < p.share; };
+    auto last_key = [&](int t, int l0) { return p.causal ? min(it.m - it.n + it.token + t * p.T + l0, it.m - 1) : it.m - 1; };
+
+    if (warp >= 12) {
+        // ------------------------------------------------------ results
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OUT_REGS));
+        const int quad = warp & 3, row = quad * 32 + lane, l0 = p.by_g.div(row), g = row - l0 * p.G;
+        int busy0 = 0, busy1 = 0, parts0 = 0, parts1 = 0;        // blocks and parts of a tile before this one
+        constexpr int BAR = 1;                  // the four warps' own barrier
+        const uint32_t out = smem_u32(smem + Cfg::S_OUT), swz = (uint32_t)(row & 7) << 4;
+        // They leave together, wherever a wait runs out: one alone would leave the others at their barrier for good.
+        // what the loops ask for each time round, out of the constant bank
+        int E = p.E, log = p.out_f32 ? 2 : 1;
+        for (int* v : {&E, &log}) asm volatile("" : "+r"(*v));
+        bool ok = true;
+#pragma unroll 1
+        for (;;) {
+            const int s = take();
+            if (named_bar_or(BAR, 128, s < 0)) break;
+#pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                if (it.token + t * p.T >= it.n) continue;
+                const uint32_t o_tmem = tmem_base + (uint32_t(quad * 32) << 16) + Cfg::O_COL + t * EP;
+                const bool live = live_row(t, l0, g);
+                const int row0 = it.q0 + it.token + t * p.T, head0 = it.h * p.share + it.g0;
+                // Whole tiles go out 128 bytes of a row at a time through shared memory and a tensor map; a store for every 16 bytes cost the SM 6000
+                // clocks an item in instructions, two blocks of keys, and a bulk copy a row more.  Tiles with rows that are nobody's go out row by row.
+                const bool whole = p.out_whole && it.token + (t + 1) * p.T <= it.n && it.g0 + p.G <= p.share;
+                const int64_t at = (int64_t)(row0 + l0) * p.oN + (int64_t)(head0 + g) * p.oH;
+                const int turn = t ? parts1++ : parts0++, blocks = t ? (busy1 += it.nblk) : (busy0 += it.nblk);
+                ok = wait(&o_full[t], (uint32_t)(turn & 1), KST_WAIT_SOFTMAX);
+                if (ok && it.nblk > 0) ok = wait(&pv_done[t], (uint32_t)((blocks - 1) & 1), KST_WAIT_SOFTMAX);
+                if (named_bar_or(BAR, 128, !ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const int nblk = it.nblk, slot = it.slot;
+                const float2 stat = stats[t * PK_ROWS + row];
+                const float f = it.slot >= 0 || stat.y == 0.f ? 1.f : 1.f / stat.y;
+                const int bad = *reinterpret_cast<volatile int*>(&odd[s]);      // written before the last P V was issued
+                if (whole && log == 1 && slot < 0 && nblk > 0 && bad == 0x7fffffff) {        // the ordinary case, without a branch to wait for
+                    if (threadIdx.x == 12 * 32) tma_store_wait_read<0>();                    // what went out before has been read
+                    named_bar_sync(BAR, 128);
+#pragma unroll
+                    for (int e = 0; e < EP; e += 16) {
+                        uint32_t o[16], w[8];
+                        tmem_ld16(o_tmem + e, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            float a, b;
+                            unpack2(mul2(pack2(__uint_as_float(o[2 * u]), __uint_as_float(o[2 * u + 1])), pack2(f, f)), a, b);
+                            const __half2 h = __floats2half2_rn(a, b);
+                            w[u] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            st_shared_v4(out + (e >> 6) * PK_ATOM + row * 128 + ((uint32_t)((e & 48) * 2 | c << 4) ^ swz), w + 4 * c);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_empty[t]);
+                    fence_proxy_async_smem();
+                    named_bar_sync(BAR, 128);
+                    if (threadIdx.x == 12 * 32) {
+                        tma_store_3d(&tmapO, smem + Cfg::S_OUT, 0, head0, row0);
+                        if (E > 64) tma_store_3d(&tmapO, smem + Cfg::S_OUT + PK_ATOM, 64, head0, row0);
+                        tma_store_commit();
+                    }
+                    continue;
+                }
+#pragma unroll 1
+                for (int e = 0; e < E; e += 32) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    if (nblk > 0) {
+                        tmem_ld32(o_tmem + e, o);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) o[u] = 0;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 32; u += 2) {
+                        float a, b;
+                        unpack2(mul2(pack2(__uint_as_float(o[u]), __uint_as_float(o[u + 1])), pack2(f, f)), a, b);
+                        o[u] = __float_as_uint(a), o[u + 1] = __float_as_uint(b);
+                    }
+                    if (bad != 0x7fffffff) {        // what was taken out, for those who see it
+                        const int end = live ? min((it.j0 + it.nblk) * PK_KEYS - 1, last_key(t, l0)) : -1;
+#pragma unroll 1
+                        for (int key = max(bad * PK_KEYS, all_see(it.token) + 1); key <= end; ++key) {
+                            const __half* q = p.v + (int64_t)(it.k0 + key) * p.vN + it.h * p.vH + e;
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) {
+                                if (e + u >= E) break;
+                                const float y = __half2float(q[u]);
+                                if (!(fabsf(y) < INFINITY)) o[u] = __float_as_uint(__uint_as_float(o[u]) + y);
+                            }
+                        }
+                    }
+                    if (e + 32 >= E) {          // all of O is in registers or on its way
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&o_empty[t]);
+                    }
+                    if (slot >= 0) {
+                        float4* d = reinterpret_cast<float4*>(p.part + (int64_t)slot * (2 * PK_ROWS * EP)) + e * (PK_ROWS / 2) + t * PK_ROWS + row;
+                        if (live)
+#pragma unroll
+                            for (int u = 0; u < 8; ++u)
+                                if (e + 4 * u < E) d[u * 2 * PK_ROWS] = make_float4(__uint_as_float(o[4 * u]), __uint_as_float(o[4 * u + 1]), __uint_as_float(o[4 * u + 2]), __uint_as_float(o[4 * u + 3]));
+                        continue;
+                    }
+                    const int in = (e << log) & 255;          // byte of the two buffers' 256 of a row
+                    const uint32_t mine = out + (in >> 7) * PK_ATOM + row * 128, at8 = (uint32_t)(in & 127);
+                    if (in == 0) {                 // what went out before has been read
+                        if (threadIdx.x == 12 * 32) tma_store_wait_read<0>();
+                        named_bar_sync(BAR, 128);
+                    }
+                    if (log == 2) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) st_shared_v4(mine + ((uint32_t)(c << 4) ^ swz), o + 4 * c);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const __half2 h = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * u]), __uint_as_float(o[8 * c + 2 * u + 1]));
+                                w[u] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                            st_shared_v4(mine + ((at8 | (uint32_t)(c << 4)) ^ swz), w);
+                        }
+                    }
+                    if (in + (32 << log) < 256 && e + 32 < E) continue;      // until the buffers, or the row, are full
+                    const int from = (e << log & ~255) >> log;
+                    if (whole) {
+                        fence_proxy_async_smem();
+                        named_bar_sync(BAR, 128);
+                        if (threadIdx.x == 12 * 32) {
+                            tma_store_3d(&tmapO, smem + Cfg::S_OUT, from, head0, row0);
+                            if (in >= 128) tma_store_3d(&tmapO, smem + Cfg::S_OUT + PK_ATOM, from + (128 >> log), head0, row0);
+                            tma_store_commit();
+                        }
+                    } else {
+                        __syncwarp();
+                        const unsigned lives = __ballot_sync(0xffffffffu, live);
+#pragma unroll 1
+                        for (int i = lane >> 3; i < 64; i += 4) {             // four rows of a buffer at a time, 16 bytes a lane
+                            const int r = i & 31, column = from + ((i >> 5) * 128 + (lane & 7) * 16 >> log), left = E - column;
+                            char* d = (char*)p.out + ((__shfl_sync(0xffffffffu, at, r) + column) << log);
+                            const uint8_t* x = smem + Cfg::S_OUT + (i >> 5) * PK_ATOM + (quad * 32 + r) * 128 + (((lane ^ r) & 7) << 4);
+                            if ((lives >> r & 1) == 0) continue;
+                            if (p.out_whole && left >= 16 >> log) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(x);
+                            else
+#pragma unroll 1
+                                for (int k = 0; k < left && k < 16 >> log; ++k) {
+                                    if (log == 2) reinterpret_cast<uint32_t*>(d)[k] = reinterpret_cast<const uint32_t*>(x)[k];
+                                    else reinterpret_cast<uint16_t*>(d)[k] = reinterpret_cast<const uint16_t*>(x)[k];
+                                }
+                        }
+                    }
+                }
+                if (live && it.slot >= 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)it.slot * 2 * PK_ROWS + t * PK_ROWS + row) * 2) = stat;
+            }
+            if (!ok) break;
+            done_with(s);
+        }
+        if (threadIdx.x == 12 * 32) tma_store_wait_all<0>();
+    } else if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OTHER_REGS));
         if (warp == 8) {
             // -------------------------------------------------- the work, and its operands
-            int unit = blockIdx.x, i = 0, tiles[2] = {0, 0};       // sides asked for so far; parts of a tile
+            int unit = blockIdx.x, i = 0, tiles0 = 0, tiles1 = 0;       // sides asked for so far; parts of a tile
             bool ok = true;
+            PackedUnit u = {};
+            bool some = p.planned ? pk_listed(p, unit, u) : pk_direct(p, unit, u);
+#pragma unroll 1
             for (int n = 0; ok; ++n) {
-                it.more = 0;
-                const bool some = p.planned ? pk_listed(p, unit, it) : n == 0 && pk_direct(p, unit, it);
-                if (!some) it.more = 0;
+                if (some) pk_part(p, it, u);
+                it.more = some;
                 const int s = n % PK_PARTS;
                 if (!wait(&a_empty[s], (uint32_t)((n / PK_PARTS) & 1) ^ 1, KST_WAIT_EMPTY)) break;
                 if (lane == 0) {
@@ -522,15 +721,13 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 }
                 __syncwarp();
                 if (!some) break;
-                if (p.planned) {          // on its way while this part's operands are asked for
-                    if (lane == 0) unit = gridDim.x + atomicAdd(&p.counts->w, 1);
-                    unit = __shfl_sync(0xffffffffu, unit, 0);
-                }
-                if (it.nblk == 0) continue;
-                for (int t = 0; ok && t < 2; ++t) {
-                    if (it.token + t * p.T >= it.n) continue;
-                    ok = wait(&q_empty[t], (uint32_t)(tiles[t] & 1) ^ 1, KST_WAIT_EMPTY);
-                    ++tiles[t];
+                some = false;
+                if (p.planned && lane == 0) unit = gridDim.x + atomicAdd(&p.counts->w, 1);      // on its way under this part's first loads
+                const int sides = 2 * it.nblk;
+                auto load_q = [&](int t, int& tiles) {
+                    if (it.token + t * p.T >= it.n || sides == 0) return;
+                    ok = ok && wait(&q_empty[t], (uint32_t)(tiles & 1) ^ 1, KST_WAIT_EMPTY);
+                    ++tiles;
                     if (ok && elect_one()) {
                         mbar_arrive_expect_tx(&q_full[t], ATOMS * 128 * p.G * p.T);
 #pragma unroll
@@ -539,8 +736,17 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                                         it.q0 + it.token + t * p.T);
                     }
                     __syncwarp();
-                }
-                for (int j = 0; ok && j < 2 * it.nblk; ++j, ++i) {
+                };
+                load_q(0, tiles0);
+#pragma unroll 1
+                for (int j = 0; ok && (j < sides || j == 0); ++j) {
+                    // What comes next is looked up once this part's first sides are asked for, and they are brought nearer.
+                    if (p.planned && j == (sides > STAGES ? STAGES : sides >> 1)) {
+                        unit = __shfl_sync(0xffffffffu, unit, 0);
+                        some = pk_listed(p, unit, u);
+                    }
+                    if (j >= sides) break;
+                    if (j == 1) load_q(1, tiles1);          // tile 1 is the later one to be done with its last part
                     const int st = i % STAGES;
                     ok = wait(&empty[st], (uint32_t)((i / STAGES) & 1) ^ 1, KST_WAIT_EMPTY);
                     if (ok && elect_one()) {
@@ -551,15 +757,18 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                                         it.k0 + (it.j0 + (j >> 1)) * PK_KEYS);
                     }
                     __syncwarp();
+                    ++i;
                 }
             }
         } else if (warp == 11) {
             // -------------------------------------------------- values that may be multiplied
             int i = 0;
             bool ok = true;
+#pragma unroll 1
             for (int s; ok && (s = take()) >= 0; done_with(s)) {
                 const int see = all_see(it.token);
                 int first = 0x7fffffff;
+#pragma unroll 1
                 for (int j = 0; ok && j < it.nblk; ++j, i += 2) {
                     const int st = (i + 1) % STAGES, key0 = (it.j0 + j) * PK_KEYS;
                     // K too, which it does not need: loads land in any order, and a stage seen last two fills ago looks full
@@ -572,10 +781,10 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                         uint8_t* tile = smem + Cfg::S_KV + st * Cfg::SIDE;
                         const __half2 zero = __half2half2(__ushort_as_half(0));
                         __half2 sum[4] = {zero, zero, zero, zero};
-#pragma unroll
+#pragma unroll 1
                         for (int a = 0; a < ATOMS; ++a) {
                             const uint4* row = reinterpret_cast<const uint4*>(tile + a * PK_ATOM);
-#pragma unroll 8
+#pragma unroll 4
                             for (int c = from * 8 + lane; c < 128 * 8; c += 32) {
                                 const uint4 x = row[c];
                                 sum[0] = __hfma2(*reinterpret_cast<const __half2*>(&x.x), zero, sum[0]);
@@ -620,7 +829,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
             const uint32_t q_addr = smem_u32(smem + Cfg::S_Q + t * Cfg::SIDE), kv_addr = smem_u32(smem + Cfg::S_KV);
             const uint32_t s_tmem = tmem_base + t * PK_KEYS, o_tmem = tmem_base + Cfg::O_COL + t * EP;
             const uint32_t p_tmem = OWN_P ? tmem_base + Cfg::P_COL + t * 64 : s_tmem;
-            int i = 0, busy = 0, parts = 0;      // sides of the ring before this part; blocks of this tile; parts of this tile
+            int i = 0, busy = 0, parts = 0, lives = 0;      // sides of the ring before this part; blocks of this tile; parts of it with keys; all of its parts
             auto issue_qk = [&](int j) -> bool {
                 const int st = (i + 2 * j) % STAGES;
                 if (!wait(&full[st], (uint32_t)(((i + 2 * j) / STAGES) & 1), KST_WAIT_FULL)) return false;
@@ -647,8 +856,10 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 for (int k = k0; k < k1; ++k) umma_ts(o_tmem, p_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
             };
             bool ok = true;
+#pragma unroll 1
             for (int s; ok && (s = take()) >= 0; done_with(s)) {
                 if (it.token + t * p.T >= it.n) {      // no rows: what the other tile reads is released from here too
+#pragma unroll 1
                     for (int j = 0; ok && j < 2 * it.nblk; ++j) {
                         const int st = (i + j) % STAGES;
                         const int vb = (i + j) >> 1;
@@ -660,12 +871,15 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     i += 2 * it.nblk;
                     continue;
                 }
+                ++lives;
                 if (it.nblk == 0) continue;
                 ok = wait(&q_full[t], (uint32_t)(parts & 1), KST_WAIT_FULL) && issue_qk(0);
+#pragma unroll 1
                 for (int j = 0; ok && j < it.nblk; ++j) {
                     if (OWN_P && j + 1 < it.nblk && !issue_qk(j + 1)) { ok = false; break; }
                     const int st = (i + 2 * j + 1) % STAGES, vb = (i >> 1) + j;
                     const uint32_t ph = (uint32_t)((busy + j) & 1);
+                    if (j == 0 && !wait(&o_empty[t], (uint32_t)(lives & 1), KST_WAIT_TMEM_EMPTY)) { ok = false; break; }   // of the part before
                     ok = wait(&ready[vb % STAGES], (uint32_t)((vb / STAGES) & 1), KST_WAIT_FULL);
                     if (ok && HALVES) {
                         ok = wait(&p_half[t], ph, KST_WAIT_SOFTMAX);
@@ -695,18 +909,18 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
         const uint32_t lane_base = uint32_t(quad * 32) << 16;
         const uint32_t s_tmem = tmem_base + lane_base + t * PK_KEYS, o_tmem = tmem_base + lane_base + Cfg::O_COL + t * EP;
         const uint32_t p_tmem = OWN_P ? tmem_base + lane_base + Cfg::P_COL + t * 64 : s_tmem;
-        const int l0 = p.by_g.div(row), g = row - l0 * p.G;       // the row's token and head in its tile
-        int busy = 0, turns = 0;          // blocks of this tile, of both tiles, before this one
+        const int l0 = p.by_g.div(row);       // the row's token in its tile
+        int busy = 0, turns = 0, lives = 0;          // blocks of this tile, turns of both, parts of this tile before this one
         bool ok = true;
+#pragma unroll 1
         for (int s; ok && (s = take()) >= 0; done_with(s)) {
             if (it.token + t * p.T >= it.n) continue;
-            const int l = it.token + t * p.T + l0;                                   // its token in the sequence
-            const bool live = l0 < p.T && l < it.n && it.g0 + g < p.share;
-            const int last = p.causal && it.m - it.n + l < it.m - 1 ? it.m - it.n + l : it.m - 1;   // the last key this row sees
+            const int last = last_key(t, l0);
             const int see = all_see(it.token + t * p.T);
             float m_run = -INFINITY, l_run = 0.f;
             const bool pingpong = it.token + p.T < it.n;
             const uint64_t k2 = pack2(p.scale_log2, p.scale_log2);
+#pragma unroll 1
             for (int j = 0; ok && j < it.nblk; ++j, ++busy) {
                 const int key0 = (it.j0 + j) * PK_KEYS;
                 ok = wait(&s_full[t], (uint32_t)(busy & 1), KST_WAIT_TMEM_FULL);
@@ -729,9 +943,11 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     const int seen = last - key0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
+                        if (key0 + i * 32 + 31 > see) {
 #pragma unroll
-                        for (int u = 0; u < 32; ++u)
-                            if (i * 32 + u > seen) x[i][u] = 0xff800000u;
+                            for (int u = 0; u < 32; ++u)
+                                if (i * 32 + u > seen) x[i][u] = 0xff800000u;
+                        }
                 }
                 auto highest = [&]() -> float {
                     float a = -INFINITY, b = -INFINITY, c = -INFINITY, d = -INFINITY;
@@ -750,7 +966,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 // P goes in times 2^7, so that fp16 holds weights down to 2^-31 of the heaviest key's.
                 const float top = highest();
                 const float m_new = top > m_run + 8.f ? top : m_run;
-                if (OWN_P && j > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);
+                if (OWN_P && busy > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);     // P and O are free
                 if (!ok) break;
                 if (__any_sync(0xffffffffu, m_new != m_run)) {
                     const float alpha = m_run == m_new ? 1.f : pk_ex2(m_run - m_new);
@@ -770,7 +986,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     }
                     m_run = m_new;
                 }
-                if (pingpong && (!OWN_P || j == 0) && (t == 1 || turns > 0) &&
+                if (pingpong && j == 0 && (t == 1 || turns > 0) &&
                     !wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), KST_WAIT_SOFTMAX)) { ok = false; break; }
                 const float m_sub = m_new == -INFINITY ? 0.f : 7.f - m_new;
                 const uint64_t a2 = pack2(m_sub, m_sub);
@@ -818,7 +1034,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                         if (lane == 0) mbar_arrive(&p_half[t]);
                     }
                 }
-                if (pingpong && (!OWN_P || j == 0)) {
+                if (pingpong && j == 0) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&exp_turn[1 - t]);
                     ++turns;
@@ -831,95 +1047,20 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 unpack2(add2(sum0, sum1), s0, s1);
                 l_run += s0 + s1;
             }
-            const float f = it.slot >= 0 || l_run == 0.f ? 1.f : 1.f / l_run;
-            // Whole results go out 128 bytes of a row at a time through shared memory of the warp's own, so that a store is of four rows' whole
-            // lines: this lane's are rows lane / 8, lane / 8 + 4, ...
-            const int64_t at = (int64_t)(it.q0 + l) * p.oN + (int64_t)(it.h * p.share + it.g0 + g) * p.oH;
-            const unsigned lives = __ballot_sync(0xffffffffu, live) >> (lane >> 3);
-            const int log = p.out_f32 ? 2 : 1, each = 16 >> log, wide = 128 >> log;       // columns of 16 bytes, of a round
-            char* row_out[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) row_out[i] = (char*)p.out + (__shfl_sync(0xffffffffu, at, i * 4 + (lane >> 3)) << log);
-            const uint32_t stage = smem_u32(smem + Cfg::S_OUT + warp * 4096), mine = stage + lane * 128, swz = (uint32_t)(lane & 7) << 4;
-            const uint32_t theirs = stage + (lane >> 3) * 128, other = (uint32_t)(lane & 7) << 4 ^ (uint32_t)(lane >> 3) << 4;   // rows 4 apart: the swizzle's upper bit turns
-            if (ok && it.nblk > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);
+            if (ok) ok = wait(&o_empty[t], (uint32_t)(lives & 1) ^ 1, KST_WAIT_TMEM_EMPTY);      // the part before's have been read
             if (!ok) break;
-            tc_fence_after();
-            const int bad = *reinterpret_cast<volatile int*>(&odd[s]);      // written before the last P V was issued
-#pragma unroll 1
-            for (int e = 0; e < p.E; e += 32) {
-                uint32_t o[32];
-                __syncwarp();
-                if (it.nblk > 0) {
-                    tmem_ld32(o_tmem + e, o);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 32; ++u) o[u] = 0;
-                }
-#pragma unroll
-                for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * f);
-                if (bad != 0x7fffffff && live) {        // what was taken out, for those who see it
-                    const int end = (it.j0 + it.nblk) * PK_KEYS - 1 < last ? (it.j0 + it.nblk) * PK_KEYS - 1 : last;
-#pragma unroll 1
-                    for (int key = max(bad * PK_KEYS, all_see(it.token) + 1); key <= end; ++key) {
-                        const __half* q = p.v + (int64_t)(it.k0 + key) * p.vN + it.h * p.vH + e;
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) {
-                            if (e + u >= p.E) break;
-                            const float y = __half2float(q[u]);
-                            if (!(fabsf(y) < INFINITY)) o[u] = __float_as_uint(__uint_as_float(o[u]) + y);
-                        }
-                    }
-                }
-                __syncwarp();
-                if (it.slot >= 0) {
-                    float4* d = reinterpret_cast<float4*>(p.part + (int64_t)it.slot * (2 * PK_ROWS * EP)) + e * (PK_ROWS / 2) + t * PK_ROWS + row;
-                    if (live)
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            if (e + 4 * u < p.E) d[u * 2 * PK_ROWS] = make_float4(__uint_as_float(o[4 * u]), __uint_as_float(o[4 * u + 1]), __uint_as_float(o[4 * u + 2]), __uint_as_float(o[4 * u + 3]));
-                    continue;
-                }
-                if (p.out_f32) {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) st_shared_v4(mine + ((uint32_t)(c << 4) ^ swz), o + 4 * c);
-                } else {
-                    const uint32_t half = (e & 32) << 1;          // which half of the row's 128 bytes
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const __half2 h = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * u]), __uint_as_float(o[8 * c + 2 * u + 1]));
-                            w[u] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                        st_shared_v4(mine + ((half | (uint32_t)(c << 4)) ^ swz), w);
-                    }
-                    if ((e & 32) == 0 && e + 32 < p.E) continue;      // the other half first
-                }
-                __syncwarp();
-                const int first = e & ~(wide - 1), column = first + (lane & 7) * each;
-                const int left = p.E - column;                   // of the row, from this lane's 16 bytes on
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    uint32_t w[4];
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(theirs + i * 512 + (other ^ (uint32_t)(i & 1) << 6)) : "memory");
-                    if ((lives >> (4 * i) & 1) == 0 || left <= 0) continue;
-                    char* d = row_out[i] + (column << log);
-                    if (p.out_whole && left >= each) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-                    else pk_store_some(d, left, log, make_uint4(w[0], w[1], w[2], w[3]));
-                }
-            }
-            if (live && it.slot >= 0) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)it.slot * 2 * PK_ROWS + t * PK_ROWS + row) * 2) = make_float2(m_run, l_run);
-            tc_fence_before();           // the next part's first P V writes O over
+            stats[t * PK_ROWS + row] = make_float2(m_run, l_run);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_full[t]);
+            ++lives;
         }
     }
-    if (*abort_flag) {
+    if (*why) {
         for (int i = 0; i < 4; ++i) __nanosleep(1000000);
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *why) atomicCAS(p.d_status, 0, *why);
     if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
@@ -990,7 +1131,7 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     auto kern = attention_packed_kernel<EP>;
     static std::atomic<uint64_t> asked{0};
     B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tk, tv, to;
     auto map = [&](CUtensorMap* m, const PackedOperand& a, int64_t heads, int64_t rows, uint32_t box_h, uint32_t box_n) {
         const uint64_t dims[3] = {(uint64_t)p.E, (uint64_t)heads, (uint64_t)rows};
         const uint64_t strides[2] = {(uint64_t)a.sH * 2, (uint64_t)a.sN * 2};
@@ -1001,6 +1142,12 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     int rc = map(&tq, q, p.Hq, p.N, p.G, p.T);
     if (!rc) rc = map(&tk, k, p.H, Nk, 1, PK_KEYS);
     if (!rc) rc = map(&tv, v, p.H, Nk, 1, PK_KEYS);
+    to = tq;
+    if (!rc && p.out_whole) {
+        const uint64_t size = p.out_f32 ? 4 : 2, dims[3] = {(uint64_t)p.E, (uint64_t)p.Hq, (uint64_t)p.N}, strides[2] = {(uint64_t)p.oH * size, (uint64_t)p.oN * size};
+        const uint32_t box[3] = {(uint32_t)(128 / size), (uint32_t)p.G, (uint32_t)p.T};
+        rc = make_tmap(ctx, &to, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p.out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
     if (rc) return rc;
     const int64_t sms = ctx->prop.multiProcessorCount;
     p.sms = (int)sms, p.most = (int)entries;
@@ -1029,7 +1176,7 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
         ctx->launches++;
     }
     const int64_t grid = p.planned ? sms : items;
-    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(PK_THREADS), Cfg::SMEM, ctx->stream, 1, tq, tk, tv, p));
+    B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(PK_THREADS), Cfg::SMEM, ctx->stream, 1, tq, tk, tv, to, p));
     ctx->launches++;
     if (p.planned) {
         B200_CUDA(launch_dep(packed_join_kernel<EP>, dim3((unsigned)(sms / 2 * (EP / 16))), dim3(256), 0, ctx->stream, 1, p));
@@ -1067,8 +1214,10 @@ int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, i
     p.causal = causal, p.out_f32 = out_dtype == B200_F32;
     p.out = const_cast<void*>(out->ptr);
     p.oN = out->stride[1], p.oH = out->stride[2];
+    if (N == 1 && p.oN <= 0) p.oN = 8;         // strides that nothing is reached through
+    if (Hq == 1 && p.oH <= 0) p.oH = 8;
     const int64_t size = p.out_f32 ? 4 : 2;
-    p.out_whole = ((uintptr_t)p.out | (uint64_t)(p.oN * size) | (uint64_t)(p.oH * size)) % 16 == 0;
+    p.out_whole = ((uintptr_t)p.out | (uint64_t)(p.oN * size) | (uint64_t)(p.oH * size)) % 16 == 0 && p.oN > 0 && p.oH > 0;
     p.scale_log2 = fmaxf((float)((double)scale * 1.4426950408889634), 0x1p-100f);   // above 0, so that a hidden score of -inf stays that
     p.d_status = ctx->d_status;
     // Heads of a tile: as many rows used as can be of 128 times those of all of a key head's tiles; of equals, the most heads.
