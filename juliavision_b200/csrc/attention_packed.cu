@@ -33,25 +33,6 @@ constexpr int PK_SOFTMAX_REGS = 184, PK_OTHER_REGS = 48, PK_OUT_REGS = 88;
 static_assert(256 * PK_SOFTMAX_REGS + 128 * PK_OTHER_REGS + 128 * PK_OUT_REGS <= PK_THREADS * 128, "what the launch holds");
 constexpr int PK_BUCKETS = 1024;                 // lengths that the list tells apart
 
-// 2^x of two numbers in the units of the FMAs, without the exponential unit: x = n + f, 2^f by a polynomial of degree 4 (the one of least largest
-// relative error, 2.9e-6, among those that are 1 at 0), n added to the exponent.  Below -127 it is 2^-127.  A NaN is lost.
-__device__ __forceinline__ void pk_exp2(uint64_t x2, float& e0, float& e1) {
-    float x0, x1, p0, p1, t0, t1;
-    unpack2(x2, x0, x1);
-    const uint64_t x = pack2(fmaxf(x0, -127.f), fmaxf(x1, -127.f)), magic = pack2(12582912.f, 12582912.f);   // 1.5 * 2^23: the sum's last bit is 1
-    uint64_t t;
-    asm("add.rm.ftz.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
-    const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f)), f = fma2(n, pack2(-1.f, -1.f), x);
-    uint64_t y = fma2(f, pack2(0.013425155f, 0.013425155f), pack2(0.052245375f, 0.052245375f));
-    y = fma2(y, f, pack2(0.24127856f, 0.24127856f));
-    y = fma2(y, f, pack2(0.69304514f, 0.69304514f));
-    y = fma2(y, f, pack2(1.f, 1.f));
-    unpack2(y, p0, p1);
-    unpack2(t, t0, t1);
-    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 // mbar_wait in as few instructions as it takes: what the roles of a block run through, all together, has to fit the nearer instruction caches.  A
 // try sleeps for 1.5 us at most, so that the tries end after some three seconds; why is left in shared memory, for the block's end.
 constexpr uint32_t PK_TRIES = 1u << 21;
@@ -392,7 +373,6 @@ template <int EP> struct PkCfg {
     static constexpr int SIDE = ATOMS * PK_ATOM;                 // an operand tile
     static constexpr bool OWN_P = EP == 64;                      // P beside S in tensor memory; else over S
     static constexpr int STAGES = OWN_P ? 8 : 4;                 // K(0), V(0), K(1), ...
-    static constexpr int POLY = 4;                               // every POLYth pair of exponentials is a polynomial
     static constexpr int FIRST = 3;                              // quarters of P that P V does not wait for the rest with, where P lies over S
     static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_OUT = S_KV + STAGES * SIDE;   // operands; 128 bytes of a tile's rows on their way out, twice
     static constexpr int S_STAT = S_OUT + 2 * PK_ATOM;           // a row's reference point and sum
@@ -991,36 +971,14 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 const float m_sub = m_new == -INFINITY ? 0.f : 7.f - m_new;
                 const uint64_t a2 = pack2(m_sub, m_sub);
                 uint64_t sum0 = pack2(0.f, 0.f), sum1 = pack2(0.f, 0.f);
-                if (!OWN_P) {      // all exponents first
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int u = 0; u < 32; u += 2) {
-                            float e0, e1;
-                            unpack2(fma2(pack2(__uint_as_float(x[i][u]), __uint_as_float(x[i][u + 1])), k2, a2), e0, e1);
-                            x[i][u] = __float_as_uint(e0), x[i][u + 1] = __float_as_uint(e1);
-                            asm volatile("" : "+r"(x[i][u]), "+r"(x[i][u + 1]));
-                        }
-                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int u = 0; u < 16; ++u) {
                         float e0, e1;
-                        uint64_t y = pack2(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1]));
-                        if (OWN_P) y = fma2(y, k2, a2);
-                        if (u % Cfg::POLY == Cfg::POLY - 1) {
-                            pk_exp2(y, e0, e1);
-                        } else {
-                            unpack2(y, e0, e1);
-                            e0 = pk_ex2(e0), e1 = pk_ex2(e1);
-                        }
-                        x[i][2 * u] = __float_as_uint(e0), x[i][2 * u + 1] = __float_as_uint(e1);
-                    }
-#pragma unroll
-                    for (int u = 0; u < 16; ++u) {
-                        const float e0 = __uint_as_float(x[i][2 * u]), e1 = __uint_as_float(x[i][2 * u + 1]);
+                        unpack2(fma2(pack2(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1])), k2, a2), e0, e1);
+                        e0 = pk_ex2(e0), e1 = pk_ex2(e1);
                         if (u & 1) sum1 = add2(sum1, pack2(e0, e1));
                         else sum0 = add2(sum0, pack2(e0, e1));
                         const __half2 h = __floats2half2_rn(e0, e1);
