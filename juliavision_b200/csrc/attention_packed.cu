@@ -534,8 +534,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 const uint32_t o_tmem = tmem_base + (uint32_t(quad * 32) << 16) + Cfg::O_COL + t * EP;
                 const bool live = live_row(t, l0, g);
                 const int row0 = it.q0 + it.token + t * p.T, head0 = it.h * p.share + it.g0;
-                // Whole tiles go out 128 bytes of a row at a time through shared memory and a tensor map; a store for every 16 bytes cost the SM 6000
-                // clocks an item in instructions, two blocks of keys, and a bulk copy a row more.  Tiles with rows that are nobody's go out row by row.
+                // Whole tiles of fp16 go out through shared memory and a tensor map, others a row a lane.  A store for every 16 bytes of all tiles cost the
+                // SM 6000 clocks an item in instructions and waits for them, two blocks of keys; a bulk copy for every row more.
                 const bool whole = p.out_whole && it.token + (t + 1) * p.T <= it.n && it.g0 + p.G <= p.share;
                 const int64_t at = (int64_t)(row0 + l0) * p.oN + (int64_t)(head0 + g) * p.oH;
                 const int turn = t ? parts1++ : parts0++, blocks = t ? (busy1 += it.nblk) : (busy0 += it.nblk);
@@ -624,15 +624,18 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                                 if (e + 4 * u < E) d[u * 2 * PK_ROWS] = make_float4(__uint_as_float(o[4 * u]), __uint_as_float(o[4 * u + 1]), __uint_as_float(o[4 * u + 2]), __uint_as_float(o[4 * u + 3]));
                         continue;
                     }
-                    const int in = (e << log) & 255;          // byte of the two buffers' 256 of a row
-                    const uint32_t mine = out + (in >> 7) * PK_ATOM + row * 128, at8 = (uint32_t)(in & 127);
-                    if (in == 0) {                 // what went out before has been read
-                        if (threadIdx.x == 12 * 32) tma_store_wait_read<0>();
-                        named_bar_sync(BAR, 128);
-                    }
+                    // a row a lane
+                    if (!live) continue;
+                    char* to = (char*)p.out + (at + e << log);
+                    const bool vectors = p.out_whole && e + 32 <= E;
                     if (log == 2) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) st_shared_v4(mine + ((uint32_t)(c << 4) ^ swz), o + 4 * c);
+                        for (int c = 0; c < 8; ++c)
+                            if (vectors || (p.out_whole && e + 4 * c + 4 <= E)) reinterpret_cast<uint4*>(to)[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                            else
+#pragma unroll
+                                for (int u = 0; u < 4; ++u)
+                                    if (e + 4 * c + u < E) reinterpret_cast<uint32_t*>(to)[4 * c + u] = o[4 * c + u];
                     } else {
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
@@ -642,35 +645,11 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                                 const __half2 h = __floats2half2_rn(__uint_as_float(o[8 * c + 2 * u]), __uint_as_float(o[8 * c + 2 * u + 1]));
                                 w[u] = *reinterpret_cast<const uint32_t*>(&h);
                             }
-                            st_shared_v4(mine + ((at8 | (uint32_t)(c << 4)) ^ swz), w);
-                        }
-                    }
-                    if (in + (32 << log) < 256 && e + 32 < E) continue;      // until the buffers, or the row, are full
-                    const int from = (e << log & ~255) >> log;
-                    if (whole) {
-                        fence_proxy_async_smem();
-                        named_bar_sync(BAR, 128);
-                        if (threadIdx.x == 12 * 32) {
-                            tma_store_3d(&tmapO, smem + Cfg::S_OUT, from, head0, row0);
-                            if (in >= 128) tma_store_3d(&tmapO, smem + Cfg::S_OUT + PK_ATOM, from + (128 >> log), head0, row0);
-                            tma_store_commit();
-                        }
-                    } else {
-                        __syncwarp();
-                        const unsigned lives = __ballot_sync(0xffffffffu, live);
-#pragma unroll 1
-                        for (int i = lane >> 3; i < 64; i += 4) {             // four rows of a buffer at a time, 16 bytes a lane
-                            const int r = i & 31, column = from + ((i >> 5) * 128 + (lane & 7) * 16 >> log), left = E - column;
-                            char* d = (char*)p.out + ((__shfl_sync(0xffffffffu, at, r) + column) << log);
-                            const uint8_t* x = smem + Cfg::S_OUT + (i >> 5) * PK_ATOM + (quad * 32 + r) * 128 + (((lane ^ r) & 7) << 4);
-                            if ((lives >> r & 1) == 0) continue;
-                            if (p.out_whole && left >= 16 >> log) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(x);
+                            if (vectors || (p.out_whole && e + 8 * c + 8 <= E)) reinterpret_cast<uint4*>(to)[c] = make_uint4(w[0], w[1], w[2], w[3]);
                             else
-#pragma unroll 1
-                                for (int k = 0; k < left && k < 16 >> log; ++k) {
-                                    if (log == 2) reinterpret_cast<uint32_t*>(d)[k] = reinterpret_cast<const uint32_t*>(x)[k];
-                                    else reinterpret_cast<uint16_t*>(d)[k] = reinterpret_cast<const uint16_t*>(x)[k];
-                                }
+#pragma unroll
+                                for (int u = 0; u < 8; ++u)
+                                    if (e + 8 * c + u < E) reinterpret_cast<uint16_t*>(to)[8 * c + u] = (uint16_t)(w[u / 2] >> (u % 2 * 16));
                         }
                     }
                 }
@@ -1101,10 +1080,10 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     if (!rc) rc = map(&tk, k, p.H, Nk, 1, PK_KEYS);
     if (!rc) rc = map(&tv, v, p.H, Nk, 1, PK_KEYS);
     to = tq;
-    if (!rc && p.out_whole) {
-        const uint64_t size = p.out_f32 ? 4 : 2, dims[3] = {(uint64_t)p.E, (uint64_t)p.Hq, (uint64_t)p.N}, strides[2] = {(uint64_t)p.oH * size, (uint64_t)p.oN * size};
-        const uint32_t box[3] = {(uint32_t)(128 / size), (uint32_t)p.G, (uint32_t)p.T};
-        rc = make_tmap(ctx, &to, p.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p.out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc && p.out_whole && !p.out_f32) {
+        const uint64_t dims[3] = {(uint64_t)p.E, (uint64_t)p.Hq, (uint64_t)p.N}, strides[2] = {(uint64_t)p.oH * 2, (uint64_t)p.oN * 2};
+        const uint32_t box[3] = {64, (uint32_t)p.G, (uint32_t)p.T};
+        rc = make_tmap(ctx, &to, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p.out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     }
     if (rc) return rc;
     const int64_t sms = ctx->prop.multiProcessorCount;
