@@ -5,6 +5,10 @@
 //
 // Bandwidth-bound: the tokens of a part-filled page, read and written, for every beam whose parent is another.  A thread takes the same 16
 // bytes of all of a search's beams and reads them all before it writes any, so the beams may change places in any way without a second copy.
+// 16 searches of 4 beams in 16 caches of 8 heads of 128, 55 MB in all: 13.4 us (4.1 TB/s; the copy's rate would give 8.3), of 5 beams in 32
+// caches of 20 heads of 64, 11 MB: 5.7 us, of which a launch and three reads that wait for one another are more than half.  Blocks go round the
+// sides of the caches, as many as are filled, sixteen blocks an SM: a block for each 256 vectors a page might have looked everything up for
+// nothing or for one vector a thread (18.2 us), and with eight an SM, six of which are resident, fewer reads are under way (14.2 us).
 #include "cache8.cuh"
 
 namespace b200 {
@@ -19,7 +23,7 @@ struct ReorderParams {
     int32_t* table;
     const int32_t *own, *parents, *lens;
     int64_t table_ld, own_ld;
-    int K, blocks, tables;           // blocks of a side of a page; whether this launch brings the table up to date
+    int K, sides, tables;            // keys and values of all caches; whether this launch brings the table up to date
 };
 
 // What every block looks up of its search; whatever the arrays hold, it is inside the cache.
@@ -42,7 +46,7 @@ template <int K>     // beams of a search at most
 __global__ void __launch_bounds__(256)
 cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
     __shared__ int parent[CR_BEAMS];
-    __shared__ int64_t page[CR_BEAMS];           // that a beam writes, or -1
+    __shared__ int64_t page[CR_BEAMS], source[CR_BEAMS];          // that a beam writes, or -1; that it copies from, or -1
     const int tid = threadIdx.x;
     const int64_t search = blockIdx.y;
     grid_dep_wait();
@@ -63,6 +67,8 @@ cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
         if (p.tables && blockIdx.x == 0 && p.lens[search * p.K + tid] != p.lens[search * p.K]) p.c.report(KST_CACHE_LENGTH);
     }
     __syncthreads();
+    if (tid < p.K) source[tid] = parent[tid] != tid && page[tid] >= 0 ? page[parent[tid]] : -1;
+    __syncthreads();
     if (blockIdx.x < (unsigned)p.tables) {       // the first block: the table
         for (int i = tid; i < p.c.width; i += 256) {
             int32_t* at = p.table + search * p.K * p.table_ld + i;
@@ -76,34 +82,36 @@ cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
         return;
     }
     if (s.kept == 0) return;
-    const int unit = blockIdx.x - p.tables, side = unit / p.blocks, block = unit - side * p.blocks;
-    const bool value = side & 1;
     const int per = p.c.E / 16, row = s.kept * per;               // of a head
-    const int i = block * 256 + tid;
-    uint8_t* data = p.data[side];
-    if (i < row * p.c.H) {
-        const int h = i / row, t = (i - h * row) / per, e = i - h * row - t * per;
-        uint8_t* at = data + t * (value ? p.c.vT : p.c.kT) + h * (value ? p.c.vH : p.c.kH) + e * 16;
-        const int64_t pitch = value ? p.c.vP : p.c.kP;
-        uint4 v[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) v[k] = *reinterpret_cast<const uint4*>(at + page[parent[k]] * pitch);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-            if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) *reinterpret_cast<uint4*>(at + page[k] * pitch) = v[k];
-    }
-    if (block == 0)
-        for (int h = tid; h < p.c.H; h += 256) {
-            float* at = p.most[side] + h;
-            float v[K];
+    const int blocks = (row * p.c.H + 255) / 256;                 // of a side
+    const int stride = gridDim.x - p.tables;
+    for (int unit = blockIdx.x - p.tables; unit < p.sides * blocks; unit += stride) {
+        const int side = unit / blocks, block = unit - side * blocks, i = block * 256 + tid;
+        const bool value = side & 1;
+        if (i < row * p.c.H) {
+            const int h = i / row, t = (i - h * row) / per, e = i - h * row - t * per;
+            uint8_t* at = p.data[side] + t * (value ? p.c.vT : p.c.kT) + h * (value ? p.c.vH : p.c.kH) + e * 16;
+            const int64_t pitch = value ? p.c.vP : p.c.kP;
+            uint4 v[K];
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) v[k] = at[page[parent[k]] * p.c.H];
+                if (k < p.K && source[k] >= 0) v[k] = *reinterpret_cast<const uint4*>(at + source[k] * pitch);
 #pragma unroll
             for (int k = 0; k < K; ++k)
-                if (k < p.K && parent[k] != k && page[k] >= 0 && page[parent[k]] >= 0) at[page[k] * p.c.H] = v[k];
+                if (k < p.K && source[k] >= 0) *reinterpret_cast<uint4*>(at + page[k] * pitch) = v[k];
         }
+        if (block == 0)
+            for (int h = tid; h < p.c.H; h += 256) {
+                float* at = p.most[side] + h;
+                float v[K];
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k < p.K && source[k] >= 0) v[k] = at[source[k] * p.c.H];
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+                    if (k < p.K && source[k] >= 0) at[page[k] * p.c.H] = v[k];
+            }
+    }
 }
 
 } // namespace b200
@@ -141,9 +149,11 @@ int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int6
         p.parents = parents, p.lens = lens;
         p.K = (int)K;
         p.tables = at == 0;
-        p.blocks = (int)cdiv((int64_t)p.c.H * p.c.T * (p.c.E / 16), 256);
-        const int64_t grid = p.tables + 2 * count * (int64_t)p.blocks;
-        B200_REQUIRE(grid < (1ll << 31), B200_DECLINE_EXTENT, "cache_reorder: %d heads in %d caches", p.c.H, count);
+        p.sides = 2 * count;
+        const int64_t blocks = cdiv((int64_t)p.c.H * p.c.T * (p.c.E / 16), 256);
+        B200_REQUIRE(blocks < (1 << 23), B200_DECLINE_EXTENT, "cache_reorder: %d heads", p.c.H);
+        const int64_t share = cdiv(16 * (int64_t)ctx->prop.multiProcessorCount, B), units = p.sides * blocks;      // sixteen blocks an SM
+        const int64_t grid = p.tables + (units < share ? units : share);
         const dim3 g((unsigned)grid, (unsigned)B), b(256);
         auto run = [&](auto kern) { return launch_dep(kern, g, b, 0, ctx->stream, 1, p); };
         B200_CUDA(K <= 4 ? run(cache_reorder_kernel<4>) : K <= 8 ? run(cache_reorder_kernel<8>) : K <= 16 ? run(cache_reorder_kernel<16>)
