@@ -128,30 +128,36 @@ int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int6
     if (n == 0 || K == 0 || B == 0) return B200_OK;
     B200_REQUIRE(table && own && parents && lens, B200_EINVAL, "cache_reorder: null array");
     B200_REQUIRE(own_ld >= width, B200_DECLINE_EXTENT, "cache_reorder: leading dimension %lld of %lld pages", (long long)own_ld, (long long)width);
-    B200_CUDA(cudaSetDevice(ctx->device));
     ReorderParams p = {};
+    for (int64_t i = 0; i < n; ++i) {            // all of them, before the first launch
+        b200_cache8 c = caches[i];
+        c.table = table, c.table_ld = table_ld, c.width = width;
+        CacheView v;
+        int rc = cache_view(ctx, &c, "cache_reorder", &v);
+        if (rc) return rc;
+        if (i == 0) p.c = v;
+        B200_REQUIRE(v.E == p.c.E && v.T == p.c.T && v.H == p.c.H && v.P == p.c.P && v.kT == p.c.kT && v.kH == p.c.kH && v.kP == p.c.kP &&
+                         v.vT == p.c.vT && v.vH == p.c.vH && v.vP == p.c.vP,
+                     B200_DECLINE_EXTENT, "cache_reorder: cache %lld has other sizes or strides than the first", (long long)i);
+        bool twice = c.k == c.v;                 // moved twice at the same time
+        for (int64_t j = 0; j < i; ++j) twice |= caches[j].k == c.k || caches[j].v == c.v || caches[j].k == c.v || caches[j].v == c.k;
+        B200_REQUIRE(!twice, B200_EINVAL, "cache_reorder: the array of cache %lld is given twice", (long long)i);
+    }
+    const int64_t blocks = cdiv((int64_t)p.c.H * p.c.T * (p.c.E / 16), 256);
+    B200_REQUIRE(blocks < (1 << 23), B200_DECLINE_EXTENT, "cache_reorder: %d heads", p.c.H);
+    B200_CUDA(cudaSetDevice(ctx->device));
+    p.table = table, p.table_ld = table_ld, p.own = own, p.own_ld = own_ld;
+    p.parents = parents, p.lens = lens;
+    p.K = (int)K;
     for (int64_t at = 0; at < n; at += CR_CACHES) {
         const int count = (int)(n - at < CR_CACHES ? n - at : CR_CACHES);
         for (int i = 0; i < count; ++i) {
-            b200_cache8 c = caches[at + i];
-            c.table = table, c.table_ld = table_ld, c.width = width;
-            CacheView v;
-            int rc = cache_view(ctx, &c, "cache_reorder", &v);
-            if (rc) return rc;
-            if (at == 0 && i == 0) p.c = v;
-            B200_REQUIRE(v.E == p.c.E && v.T == p.c.T && v.H == p.c.H && v.P == p.c.P && v.kT == p.c.kT && v.kH == p.c.kH && v.kP == p.c.kP &&
-                             v.vT == p.c.vT && v.vH == p.c.vH && v.vP == p.c.vP,
-                         B200_DECLINE_EXTENT, "cache_reorder: cache %lld has other sizes or strides than the first", (long long)(at + i));
-            p.data[2 * i] = v.k, p.data[2 * i + 1] = v.v;
-            p.most[2 * i] = v.kmax, p.most[2 * i + 1] = v.vmax;
+            const b200_cache8& c = caches[at + i];
+            p.data[2 * i] = (uint8_t*)c.k, p.data[2 * i + 1] = (uint8_t*)c.v;
+            p.most[2 * i] = c.kmax, p.most[2 * i + 1] = c.vmax;
         }
-        p.table = table, p.table_ld = table_ld, p.own = own, p.own_ld = own_ld;
-        p.parents = parents, p.lens = lens;
-        p.K = (int)K;
         p.tables = at == 0;
         p.sides = 2 * count;
-        const int64_t blocks = cdiv((int64_t)p.c.H * p.c.T * (p.c.E / 16), 256);
-        B200_REQUIRE(blocks < (1 << 23), B200_DECLINE_EXTENT, "cache_reorder: %d heads", p.c.H);
         const int64_t share = cdiv(16 * (int64_t)ctx->prop.multiProcessorCount, B), units = p.sides * blocks;      // sixteen blocks an SM
         const int64_t grid = p.tables + (units < share ? units : share);
         const dim3 g((unsigned)grid, (unsigned)B), b(256);

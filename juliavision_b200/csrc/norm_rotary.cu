@@ -232,7 +232,8 @@ int b200_norm_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t
     p.out = (__half*)const_cast<void*>(out->ptr);
     p.xL = x->stride[1], p.xH = x->stride[2], p.xB = x->stride[3];
     p.oL = out->stride[1], p.oH = out->stride[2], p.oB = out->stride[3];
-    p.weight = weight, p.weight_ld = weight_ld, p.weight_f32 = weight_dtype == B200_F32, p.split = (int)split;
+    p.weight = weight, p.weight_ld = weight_ld, p.weight_f32 = weight_dtype == B200_F32;
+    p.split = (int)(split < 0 && weight_ld == 0 ? H : split);      // one column: loaded once a lane
     p.freq = (const unsigned long long*)freq;
     p.at = {positions, lens, news, pos_l, pos_b, (int)L};
     p.gain = gain, p.eps = eps;
