@@ -2,8 +2,12 @@
 // kstarts[b+1] - 1, query head i reads key head i / (Hq / H), and the last query row stands at the last key:
 //     out = softmax(scale Q K' + mask) V, row i of n seeing, when causal, the keys up to i + keys - n, else all of its sequence's.
 //
-// Tensor-bound for long sequences: 4 E flops a row and visible key on tcgen05, and as many clocks for the exponentials as for the
-// products at E = 128, twice as many at 64.
+// 4 E flops a row and visible key on tcgen05, and as many clocks of the exponential unit as of the products at E = 128, twice as many at 64.
+// What bounds it at E = 128 is the chain of a block of keys, which two tiles have between them to hide: 2900 clocks for two tiles and 128 keys, where
+// the products are 2048, of which a tile's softmax is 1300 for exponentials and sums, 240 to 430 for the maximum and 75 for the load of S, and its
+// product goes out only then; at E = 64 it is the exponentials.  Once the power limit holds, fewer clocks alone gain little (below, and at the
+// exponentials).  32 query heads on 8 key heads of 128, causal: 16384 rows 1995 us (1.10 PFLOP/s), 37 sequences of up to 2000 580 us (0.76; 507
+// before the limit holds); 20 heads of 64: 16 sequences of up to 1500 161 us, one of 77 rows 7.3.
 //
 // The query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads (G T <= 128), so that keys and
 // values are read once for all of them and a tile's rows lie close together under the causal mask.  A block takes two tiles and walks their keys
@@ -122,7 +126,7 @@ struct PackedSeq {
 
 // ------------------------------------------------------------------------------------------ the list of the work
 // One block, which the launch behind it waits for: sequences in shared memory, few barriers, no lane waits for another's atomic (10 to 31 us with
-// sequences in global memory and sums by atomics, 3 to 5 so).
+// sequences in global memory and sums by atomics, 6 to 8 so).
 constexpr int PL_THREADS = 1024, PL_SEQS = 1024;    // sequences kept in shared memory
 
 __device__ __forceinline__ int pl_scan(int x, int* sums, int& total) {   // exclusive; sums: 32 of its own
@@ -371,9 +375,11 @@ __device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, Packe
 template <int EP> struct PkCfg {
     static constexpr int ATOMS = EP / 64;
     static constexpr int SIDE = ATOMS * PK_ATOM;                 // an operand tile
-    static constexpr bool OWN_P = EP == 64;                      // P beside S in tensor memory; else over S
+    // P beside S in tensor memory where there is room for it, so that the next scores come while P V reads; else over S.
+    static constexpr bool OWN_P = EP == 64;
     static constexpr int STAGES = OWN_P ? 8 : 4;                 // K(0), V(0), K(1), ...
-    static constexpr int FIRST = 3;                              // quarters of P that P V does not wait for the rest with, where P lies over S
+    // Quarters of P that P V starts with, where P lies over S: three, 2922 clocks for two tiles and a block of keys; with two 3062.
+    static constexpr int FIRST = 3;
     static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_OUT = S_KV + STAGES * SIDE;   // operands; 128 bytes of a tile's rows on their way out, twice
     static constexpr int S_STAT = S_OUT + 2 * PK_ATOM;           // a row's reference point and sum
     static constexpr int S_BARS = S_STAT + 2 * PK_ROWS * 8;
@@ -427,7 +433,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
     uint64_t* empty = ready + STAGES;              // [STAGES] one arrival a tile
     uint64_t* s_full = empty + STAGES;             // [2] a tile's scores are there
     uint64_t* s_empty = s_full + 2;                // [2] and in registers
-    uint64_t* p_half = s_empty + 2;                // [2] half of its P
+    uint64_t* p_half = s_empty + 2;                // [2] the first FIRST quarters of its P
     uint64_t* p_full = p_half + 2;                 // [2] all of it
     uint64_t* pv_done = p_full + 2;                // [2] its last product
     uint64_t* exp_turn = pv_done + 2;              // [2] whose turn it is to run its exponentials
@@ -922,7 +928,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     return fmaxf(fmaxf(a, b), fmaxf(c, d)) * p.scale_log2;
                 };
                 // Any reference point m gives the same quotient; it follows the maximum lazily, only when that has grown by more than 2^8.
-                // P goes in times 2^7, so that fp16 holds weights down to 2^-31 of the heaviest key's.
+                // P goes in times 2^7, so that fp16 holds weights down to 2^-31 of the heaviest key's.  Each weight is rounded once to fp16, half a
+                // step 2^-11 of itself, as the product's operand; the sum that divides takes them as they were, in fp32.
                 const float top = highest();
                 const float m_new = top > m_run + 8.f ? top : m_run;
                 if (OWN_P && busy > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);     // P and O are free
@@ -945,6 +952,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     }
                     m_run = m_new;
                 }
+                // In a part's first block the tiles take turns at the exponentials, so that one's run under the other's products; from there on they
+                // fall into step by themselves (turns at every block: 599 us for 594 of 37 sequences of up to 2000, 2059 for 1994 of 16384 rows).
                 if (pingpong && j == 0 && (t == 1 || turns > 0) &&
                     !wait(&exp_turn[t], (uint32_t)((t == 1 ? turns : turns - 1) & 1), KST_WAIT_SOFTMAX)) { ok = false; break; }
                 const float m_sub = m_new == -INFINITY ? 0.f : 7.f - m_new;
@@ -957,6 +966,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     for (int u = 0; u < 16; ++u) {
                         float e0, e1;
                         unpack2(fma2(pack2(__uint_as_float(x[i][2 * u]), __uint_as_float(x[i][2 * u + 1])), k2, a2), e0, e1);
+                        // All by the exponential unit: a polynomial for every fourth pair takes 2 to 4 % fewer clocks and, under the power limit,
+                        // 594 us for 585 (E = 128) and 166 for 162 (E = 64).
                         e0 = pk_ex2(e0), e1 = pk_ex2(e1);
                         if (u & 1) sum1 = add2(sum1, pack2(e0, e1));
                         else sum0 = add2(sum0, pack2(e0, e1));

@@ -195,3 +195,78 @@ def test_recorded(ctx):
         assert all(np.array_equal(g, outs[0].to_host()) for g in got)
         p.news, p.keys, p.starts, p.kstarts = np.diff(starts), np.diff(kstarts), starts, kstarts
         p.check(got[0], F16, True)
+
+
+@pytest.mark.parametrize("E", [64, 128])
+def test_more_sequences_than_a_block_lists_at_once(ctx, E):
+    """Thousands of sequences, most of them short or empty: their places in memory of the device, pairs beyond those kept in registers."""
+    rng = np.random.default_rng(11)
+    news = rng.integers(0, 4, 2600)
+    news[[5, 1023, 1024, 2599]] = 300, 200, 129, 257
+    past = rng.integers(0, 20, 2600)
+    past[700] = 9000
+    p = Packed(ctx, rng, E, 2, 1, news, past)
+    p.check(p.run(F16, True), F16, True)
+    p = Packed(ctx, rng, E, 2, 1, [0] * 1500, [3] * 1500, spare=300)
+    p.check(p.run(F16, True), F16, True)
+    p = Packed(ctx, rng, E, 2, 2, [1] * 1500, rng.integers(0, 300, 1500))          # a token each, as a step of serving is
+    p.check(p.run(F32, True), F32, True)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("way", ["heads", "odd", "backwards"])
+def test_where_results_go(ctx, dtype, way):
+    """Head-major, off 16-byte boundaries with something between the rows, and from the last row to the first."""
+    E, Hq = 72, 6
+    p = Packed(ctx, np.random.default_rng(12), E, Hq, 3, [140, 3, 70, 260], [0, 9, 50, 1])
+    N, size = len(p.q), np.dtype(dtype).itemsize
+    pitch = E + 3 if way == "odd" else E
+    buf = ctx.allocate(dtype, pitch, Hq, N) if way != "heads" else ctx.allocate(dtype, pitch, N, Hq)
+    ctx.fill_bytes(buf, 0xFF)
+    at, strides = {"heads": (0, (1, E, N * E)), "odd": (1, (1, Hq * pitch, pitch)), "backwards": ((N - 1) * Hq * E, (1, -Hq * E, E))}[way]
+    out = jv.DeviceArray(ctx, buf.ptr + at * size, dtype, (E, N, Hq), strides, owner=buf)
+    ctx.ws.reset()
+    jv.packedsdpa_(ctx, out, *p.device(), ints(ctx, p.starts), ints(ctx, p.kstarts))
+    ctx.synchronize()
+    got = buf.to_host()
+    if way == "heads":
+        got = got.transpose(1, 0, 2)
+    if way == "odd":
+        between = np.delete(got.ravel()[:N * Hq * pitch].reshape(N * Hq, pitch), range(1, E + 1), 1)
+        assert np.isnan(between.astype(np.float64)).all()
+        got = got[..., 1:E + 1]
+    p.check(got[::-1] if way == "backwards" else got, dtype, True)
+
+
+def test_heads_that_share_memory(ctx):
+    """Keys and values broadcast over heads, queries over rows, rows from the last to the first: strides of 0 and below."""
+    rng = np.random.default_rng(13)
+    E, N, Hq, H = 64, 150, 4, 2
+    p = Packed(ctx, rng, E, Hq, H, [90, 60], [0, 0], spare=0)
+    p.k[:], p.v[:], p.q[:] = p.k[:, :1], p.v[:, :1], p.q[:1]
+    dk, dv, dq = ctx.toback(np.ascontiguousarray(p.k[:, 0])), ctx.toback(np.ascontiguousarray(p.v[::-1, 0])), ctx.toback(p.q[0])
+    k = jv.DeviceArray(ctx, dk.ptr, F16, (E, N, H), (1, E, 0), owner=dk)
+    v = jv.DeviceArray(ctx, dv.ptr + (N - 1) * E * 2, F16, (E, N, H), (1, -E, 0), owner=dv)
+    q = jv.DeviceArray(ctx, dq.ptr, F16, (E, N, Hq), (1, 0, E), owner=dq)
+    out = ctx.allocate(F32, E, Hq, N)
+    ctx.ws.reset()
+    jv.packedsdpa_(ctx, out.permute((0, 2, 1)), q, k, v, ints(ctx, p.starts))
+    ctx.synchronize()
+    p.check(out.to_host(), F32, True)
+
+
+def test_two_contexts_at_once(ctx):
+    """Calls of two contexts, each with its own stream and workspace, under way at the same time."""
+    other = jv.Ctx(0)
+    rng = np.random.default_rng(14)
+    made = [Packed(c, rng, E, 8, 2, rng.integers(1, 600, 12), [0] * 12) for c, E in ((ctx, 128), (other, 64))]
+    held = [(p.device(), ints(p.ctx, p.starts), p.ctx.allocate(F16, p.E, 8, len(p.q))) for p in made]
+    for p, (_, _, buf) in zip(made, held):
+        p.ctx.fill_bytes(buf, 0xFF)
+    for _ in range(8):
+        for p, (d, ds, buf) in zip(made, held):
+            p.ctx.ws.reset()
+            jv.packedsdpa_(p.ctx, buf.permute((0, 2, 1)), *d, ds)
+    for p, (_, _, buf) in zip(made, held):
+        p.ctx.synchronize()
+        p.check(buf.to_host(), F16, True)
