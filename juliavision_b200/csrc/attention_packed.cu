@@ -7,7 +7,8 @@
 // the products are 2048, of which a tile's softmax is 1300 for exponentials and sums, 240 to 430 for the maximum and 75 for the load of S, and its
 // product goes out only then; at E = 64 it is the exponentials.  Once the power limit holds, fewer clocks alone gain little (below, and at the
 // exponentials).  32 query heads on 8 key heads of 128, causal: 16384 rows 1995 us (1.10 PFLOP/s), 37 sequences of up to 2000 580 us (0.76; 507
-// before the limit holds); 20 heads of 64: 16 sequences of up to 1500 161 us, one of 77 rows 7.3.
+// before the limit holds); 20 heads of 64: 16 sequences of up to
+// 1500 161 us, 3 of 500 rows behind 30000 keys 264, one of 77 rows 7.3.
 //
 // The query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads (G T <= 128), so that keys and
 // values are read once for all of them and a tile's rows lie close together under the causal mask.  A block takes two tiles and walks their keys
@@ -19,9 +20,10 @@
 //   warp 11    hands V on to them; where a row does not see a key of the block, it first takes out of the tile what is not finite
 //   warps 12-15  take both tiles' results out while the softmax is at the next part
 //
-// Lengths are on the device, so the work is listed there: the row pairs of all sequences, longest first, those that are longer than an
-// SM's share cut along their keys (packed_plan_kernel).  Blocks take the list's units in order as they become free; a second launch joins what
-// was cut.  Calls whose pairs all run at once, over few keys, take them as they come and need neither.
+// Lengths are on the device, so the work is listed there: the row pairs of all sequences, longest first (packed_plan_kernel).  Blocks take the
+// list's units in order as they become free.  Where some pairs are a large part of what an SM has to do, such pairs' blocks of keys are dealt out
+// first, the same number in a row to each SM, which cuts pairs along their keys; a second launch joins what was cut.  Calls whose pairs all
+// run at once, over few keys, take them as they come and need neither.
 #include <cuda_fp16.h>
 
 #include "internal.h"
@@ -33,8 +35,9 @@ constexpr int PK_THREADS = 512;
 constexpr int PK_ROWS = 128, PK_KEYS = 128;      // of a tile
 constexpr int PK_ATOM = 128 * 128;               // 128 rows x 64 fp16
 constexpr int PK_PARTS = 3;                      // parts of the work on their way from warp 8 to the others
-constexpr int PK_SOFTMAX_REGS = 184, PK_OTHER_REGS = 48, PK_OUT_REGS = 88;
+constexpr int PK_SOFTMAX_REGS = 184, PK_OTHER_REGS = 56, PK_OUT_REGS = 88;
 static_assert(256 * PK_SOFTMAX_REGS + 128 * PK_OTHER_REGS + 128 * PK_OUT_REGS <= PK_THREADS * 128, "what the launch holds");
+constexpr int PK_IDLE = 10;                      // blocks of keys an SM may stand idle before pairs are cut
 constexpr int PK_BUCKETS = 1024;                 // lengths that the list tells apart
 
 // mbar_wait in as few instructions as it takes: what the roles of a block run through, all together, has to fit the nearer instruction caches.  A
@@ -50,10 +53,10 @@ __device__ __forceinline__ bool pk_wait(uint64_t* bar, uint32_t parity, int code
 
 struct __align__(16) PackedEntry {
     int q0, n, k0, m;                  // the sequence: first row, rows, first key, keys
-    int pair, blocks, parts, pad;
+    int pair, blocks, pad[2];
 };
 struct __align__(16) PackedCut {
-    int slot, parts, head, token;      // first slot, parts; unit of the row pair; first token of tile 0
+    int slot, parts, head, token;      // first slot (the others are the next even ones), parts; unit of the row pair; first token of tile 0
     int q0, n, pad[2];
 };
 
@@ -71,14 +74,15 @@ struct PackedParams {
     int heads;                         // H * groups: units of a row pair
     int most;                          // row pairs that the list has room for: what sequences in order can have
     int planned;
-    // The list (null without one), longest first: row pairs with their sequence's place and size, pair, blocks of keys and parts; where some are cut,
-    // also their first units and slots; counters; the cut ones a head at a time, as the launch that joins them wants them.
+    // The list (null without one): row pairs with their sequence's place and size, pair and blocks of keys, the long ones first; how many blocks the
+    // long ones before have, of all heads; counters; what is cut, a head at a time, as the launch that joins it wants it.
     PackedEntry* entry;
-    int *unit, *slot;
-    int4* counts;                      // units, entries, cut heads, units taken beyond the first of each block
+    int* before;
+    int4* counts;                      // units, long entries, cut heads, units taken beyond the first of each block;
+                                       // blocks dealt to an SM, the first of them, the long ones' blocks, units before what is dealt
     int* first;                        // [B] first pair of a sequence, where they are too many for shared memory
     PackedCut* cut;
-    float *part, *part_ml;             // [slots][E / 4][256 rows][4] and [slots][256][2]: reference point, sum
+    float *part, *part_ml;             // [2 an SM][E / 4][256 rows][4] and [2 an SM][256][2]: reference point, sum
     int sms;
     int* d_status;
 };
@@ -203,43 +207,60 @@ packed_plan_kernel(const PackedParams p) {
     PackedSeq s0 = {0, 0, 0, 0};
     int pair0 = 0, blocks0 = 0;
     long long mine = 0;
+    int longest = 0;
     for (int e = tid; e < entries; e += PL_THREADS) {
         PackedSeq s;
         int pair, n;
         entry(e, s, pair, n);
         if (e == tid) s0 = s, pair0 = pair, blocks0 = n;
         mine += n > 0 ? n : 1;
+        longest = n > longest ? n : longest;
     }
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    longest = __reduce_max_sync(0xffffffffu, longest);
     __shared__ long long total_of[32];
-    if ((tid & 31) == 0) total_of[tid >> 5] = mine;
+    __shared__ int longest_of[32];
+    if ((tid & 31) == 0) total_of[tid >> 5] = mine, longest_of[tid >> 5] = longest;
     __syncthreads();
     long long all = total_of[tid & 31];
+    longest = __reduce_max_sync(0xffffffffu, longest_of[tid & 31]);
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) all += __shfl_xor_sync(0xffffffffu, all, d);
     all *= p.heads;
-    // As many parts as a pair has SMs' shares: the parts of all that is cut are no more than the SMs.
-    auto parts_of = [&](int blocks) {
-        const int s = all > 0 ? (int)((long long)blocks * p.sms / all) : 1;
-        return s > 1 ? s < blocks ? s : blocks : 1;
-    };
-    auto bucket_of = [&](int blocks, int parts) {
-        const int size = blocks / parts;
-        return size < PK_BUCKETS ? PK_BUCKETS - 1 - size : 0;
+    // Long: more than an SM's share, or a quarter of it where all pairs are alike, whose last round leaves SMs idle (where they differ, longest first
+    // evens that out: 320 of 16 to 32 blocks, E = 128, 148 us; with the longer ones dealt out, which then share fewer of their keys in the L2 cache,
+    // 170).  They stand first, in the sequences' order, for some of them are cut, and which ones must not hang on the order of atomics.  The
+    // others follow, longest first; pairs of a bucket come in any order, which changes no result.
+    const bool alike = (long long)entries * p.heads * longest * 4 <= all * 5;
+    const long long least = alike ? all / 4 / p.sms : all / p.sms;
+    const bool longs = longest > least + (alike ? 0 : PK_IDLE) && all < 0x7fffffff - p.sms;
+    auto bucket_of = [&](int blocks) { return blocks < PK_BUCKETS ? PK_BUCKETS - 1 - blocks : 0; };
+    auto set_down = [&](int at, const PackedSeq& s, int pair, int n) {
+        int4* to = reinterpret_cast<int4*>(p.entry + at);
+        to[0] = make_int4(s.q0, s.n, s.k0, s.m);
+        to[1] = make_int4(pair, n, 0, 0);
     };
     const int rounds = (entries + PL_THREADS - 1) / PL_THREADS;
-    bool cut = false;
+    int many_long = 0, blocks_long = 0;
     for (int r = 0; r < rounds; ++r) {
         const int e = r * PL_THREADS + tid;
         PackedSeq s = s0;
         int pair = pair0, n = blocks0;
         if (r > 0 && e < entries) entry(e, s, pair, n);
-        const int parts = parts_of(n);
-        cut |= e < entries && parts > 1;
-        pl_count(bucket, bucket_of(n, parts), e < entries);
+        const bool is = longs && e < entries && n > least;
+        pl_count(bucket, bucket_of(n), e < entries && !is);
+        if (longs) {
+            int total;
+            int at = many_long + pl_scan(is, sums, total);
+            many_long += total;
+            if (is) set_down(at, s, pair, n);
+            const int before = blocks_long + pl_scan(is ? n * p.heads : 0, sums, total);
+            blocks_long += total;
+            if (is) p.before[at] = before;
+        }
     }
-    const bool cuts = __syncthreads_or(cut);
+    __syncthreads();
     {
         int total;
         const int n = bucket[tid], at = pl_scan(n, sums, total);
@@ -251,41 +272,57 @@ packed_plan_kernel(const PackedParams p) {
         PackedSeq s = s0;
         int pair = pair0, n = blocks0;
         if (r > 0 && e < entries) entry(e, s, pair, n);
-        const int parts = parts_of(n), at = pl_count(bucket, bucket_of(n, parts), e < entries);
-        if (e < entries) {
-            int4* to = reinterpret_cast<int4*>(p.entry + at);
-            to[0] = make_int4(s.q0, s.n, s.k0, s.m);
-            to[1] = make_int4(pair, n, parts, 0);
-        }
+        const bool is = longs && e < entries && n > least;
+        const int at = pl_count(bucket, bucket_of(n), e < entries && !is);
+        if (e < entries && !is) set_down(many_long + at, s, pair, n);
     }
-    int units = entries * p.heads, many = 0;
-    if (cuts) {
+    // Which long ones are dealt out: all of them, or, where they are alike, those that are left when each SM has had as many whole ones as go
+    // round; and none where the SMs that would stand idle then lose less than ten blocks of keys (20 heads of 64, 4096 rows, 27 blocks: 127 us
+    // for 146 whole; 100 rows over 3000 keys, 15 blocks: 23 for 32; 16 heads of 128, 4096 rows, 9 blocks: 158 for 149).
+    int whole = many_long * p.heads, each = 0, many = 0, from = blocks_long;
+    if (many_long > 0) {
+        const int items = whole, left = items % p.sms;
+        if (!alike) whole = 0;
+        else if (left > 0 && longest - (long long)longest * left / p.sms > PK_IDLE) whole = items - left;
         __syncthreads();
-        units = 0;
-        int slots = 0;
-        for (int base = 0; base < entries; base += PL_THREADS) {
-            const int e = base + tid;
-            PackedEntry x = {};
-            if (e < entries) x = p.entry[e];
-            int total;
-            int at = pl_scan(x.parts * p.heads, sums, total);
-            if (e < entries) p.unit[e] = units + at;
-            units += total;
-            at = pl_scan(x.parts > 1 ? x.parts * p.heads : 0, sums, total);
-            if (e < entries) p.slot[e] = slots + at;
-            const int slot = slots + at;
-            slots += total;
-            at = pl_scan(x.parts > 1 ? p.heads : 0, sums, total);
-            if (x.parts > 1)
-                for (int h = 0; h < p.heads; ++h) {
-                    int4* to = reinterpret_cast<int4*>(p.cut + many + at + h);
-                    to[0] = make_int4(slot + h * x.parts, x.parts, h, x.pair * 2 * p.T);
-                    to[1] = make_int4(x.q0, x.n, 0, 0);
+        if (whole < items) {
+            const int e = whole / p.heads;
+            from = p.before[e] + (whole - e * p.heads) * p.entry[e].blocks;
+            each = (blocks_long - from + p.sms - 1) / p.sms;
+        }
+        // SM c's first block of keys is from + c * each; where that is inside a pair, the pair is cut, and the first such SM lists it.
+        for (int base = 0; each > 0 && base < p.sms; base += PL_THREADS) {
+            const int c = base + tid;
+            PackedCut x = {};
+            if (c > 0 && c < p.sms && from + (long long)c * each < blocks_long) {
+                const int at = from + c * each;
+                int lo = 0, hi = many_long;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if (p.before[mid] <= at) lo = mid;
+                    else hi = mid;
                 }
+                const PackedEntry y = p.entry[lo];
+                const int rel = at - p.before[lo], size = y.blocks, head = rel / size, start = at - (rel - head * size);
+                if (start < at && start >= at - each) {
+                    x.parts = (start - from + size - 1) / each - (c - 1) + 1;
+                    x.slot = 2 * (c - 1) + (start > at - each), x.head = head, x.token = y.pair * 2 * p.T, x.q0 = y.q0, x.n = y.n;
+                }
+            }
+            int total;
+            const int at = pl_scan(x.parts > 0, sums, total);
+            if (x.parts > 0) {
+                int4* to = reinterpret_cast<int4*>(p.cut + many + at);
+                to[0] = make_int4(x.slot, x.parts, x.head, x.token);
+                to[1] = make_int4(x.q0, x.n, 0, 0);
+            }
             many += total;
         }
     }
-    if (tid == 0) *p.counts = make_int4(units, entries, many, 0);
+    if (tid == 0) {
+        p.counts[0] = make_int4(entries * p.heads, many_long, many, 0);
+        p.counts[1] = make_int4(each, from, blocks_long, whole);
+    }
 }
 
 // A block's work: some of the key blocks of two tiles.
@@ -295,51 +332,66 @@ struct PackedPart {
     int j0, nblk, slot, more;    // key blocks; slot < 0: the whole of the item
 };
 
-// A unit of the work: a part of the keys of a row pair, for one group of heads of a key head.
+// A unit of the work: a row pair, or a part of its keys, for one group of heads of a key head.
 struct PackedUnit {
     PackedSeq s;
-    int pair, blocks, head, part, parts, slot;
+    int pair, blocks, head, j0, slot;
+    int next;                    // of the blocks dealt out, the first behind this unit; -1 before, PK_DEALT behind them
 };
 __device__ __forceinline__ void pk_part(const PackedParams& p, PackedPart& x, const PackedUnit& u) {
     x.q0 = u.s.q0, x.n = u.s.n, x.k0 = u.s.k0, x.m = u.s.m;
     x.h = u.head / p.groups, x.g0 = (u.head - x.h * p.groups) * p.G;
     x.token = u.pair * 2 * p.T;
-    x.j0 = 0, x.nblk = u.blocks, x.slot = -1;
-    if (u.parts > 1) {      // no more parts than SMs, fewer than 2^23 blocks
-        x.j0 = (int)((unsigned)(u.part * u.blocks) / (unsigned)u.parts);
-        x.nblk = (int)((unsigned)((u.part + 1) * u.blocks) / (unsigned)u.parts) - x.j0;
-        x.slot = u.slot + u.head * u.parts + u.part;
-    }
+    x.j0 = u.j0, x.nblk = u.blocks, x.slot = u.slot;
 }
 
-// Unit `unit` of the list, found by a whole warp.
+// The next of what is dealt out to this block, and then unit `unit` of the list; found by a whole warp.
+constexpr int PK_DEALT = -2;     // PackedUnit::next behind what was dealt out
 __device__ __forceinline__ bool pk_listed(const PackedParams& p, int unit, PackedUnit& x) {
     const int lane = threadIdx.x & 31;
-    // where nothing is cut it is its pair's `heads` units on; asked for along with the counters
+    // where nothing is dealt out it is its pair's `heads` units on; asked for along with the counters
     int e = unit / p.heads, rel = unit - e * p.heads;
-    e = e < p.most ? e : p.most - 1;
-    const int4 counts = *p.counts;
-    PackedEntry it = p.entry[e];
-    if (unit >= counts.x) return false;
-    x.part = 0, x.slot = 0;
-    if (counts.z > 0) {
-        int lo = 0, hi = counts.y;          // the last entry whose first unit is at or before this one
+    PackedEntry it = p.entry[e < p.most ? e : p.most - 1];
+    const int4 counts = p.counts[0], dealt = p.counts[1];
+    x.j0 = 0, x.slot = -1;
+    if (dealt.x > 0 && x.next != PK_DEALT) {
+        const long long mine = dealt.y + (long long)blockIdx.x * dealt.x;
+        const int start = mine < dealt.z ? (int)mine : dealt.z, end = dealt.z - start < dealt.x ? dealt.z : start + dealt.x;
+        const int at = x.next < 0 ? start : x.next;
+        if (at < end) {
+            int lo = 0, hi = counts.y;          // the last entry that begins at or before this block of keys
 #pragma unroll 1
-        while (hi - lo > 1) {
-            const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-            const bool before = at < hi && p.unit[at] <= unit;
-            const int k = 31 - __clz(__ballot_sync(0xffffffffu, before));
-            lo += k * step;
-            hi = lo + step < hi ? lo + step : hi;
+            while (hi - lo > 1) {
+                const int step = (hi - lo + 31) / 32, to = lo + lane * step;
+                const bool before = to < hi && p.before[to] <= at;
+                const int k = 31 - __clz(__ballot_sync(0xffffffffu, before));
+                lo += k * step;
+                hi = lo + step < hi ? lo + step : hi;
+            }
+            it = p.entry[lo];
+            const int into = at - p.before[lo], size = it.blocks;
+            x.head = into / size;
+            x.j0 = into - x.head * size;
+            const int here = size - x.j0 < end - at ? size - x.j0 : end - at;
+            x.blocks = here;
+            x.next = at + here;
+            if (here < size) x.slot = 2 * blockIdx.x + (at > start);      // at most the first and the last of a block
+            x.s = {it.q0, it.n, it.k0, it.m};
+            x.pair = it.pair;
+            return true;
         }
-        it = p.entry[lo];
-        rel = unit - p.unit[lo];
-        x.part = rel / p.heads;
-        rel -= x.part * p.heads;
-        x.slot = p.slot[lo];
     }
+    x.next = PK_DEALT;
+    if (dealt.x > 0 && unit >= dealt.w) {       // behind what was dealt out
+        const int skipped = unit + counts.y * p.heads - dealt.w;
+        e = skipped / p.heads, rel = skipped - e * p.heads;
+        if (skipped < counts.x) it = p.entry[e];
+        unit = skipped;
+    }
+    if (unit >= counts.x) return false;
+    x.blocks = it.blocks;
     x.s = {it.q0, it.n, it.k0, it.m};
-    x.pair = it.pair, x.blocks = it.blocks, x.parts = it.parts, x.head = rel;
+    x.pair = it.pair, x.head = rel;
     return true;
 }
 // Without a list: the row pairs of all sequences in their order.
@@ -364,7 +416,7 @@ __device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, Packe
             for (int* v : {&s.q0, &s.n, &s.k0, &s.m}) *v = __shfl_sync(0xffffffffu, *v, k);
             x.s = s;
             x.blocks = s.blocks(p, x.pair), x.head = unit - pair * p.heads;
-            x.part = 0, x.parts = 1, x.slot = 0;
+            x.j0 = 0, x.slot = -1;
             return true;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -672,6 +724,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
             int unit = blockIdx.x, i = 0, tiles0 = 0, tiles1 = 0;       // sides asked for so far; parts of a tile
             bool ok = true;
             PackedUnit u = {};
+            u.next = -1;
             bool some = p.planned ? pk_listed(p, unit, u) : pk_direct(p, unit, u);
 #pragma unroll 1
             for (int n = 0; ok; ++n) {
@@ -687,7 +740,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 __syncwarp();
                 if (!some) break;
                 some = false;
-                if (p.planned && lane == 0) unit = gridDim.x + atomicAdd(&p.counts->w, 1);      // on its way under this part's first loads
+                if (p.planned && u.next == PK_DEALT && lane == 0) unit = gridDim.x + atomicAdd(&p.counts->w, 1);      // on its way under this part's first loads
                 const int sides = 2 * it.nblk;
                 auto load_q = [&](int t, int& tiles) {
                     if (it.token + t * p.T >= it.n || sides == 0) return;
@@ -1028,14 +1081,14 @@ packed_join_kernel(const PackedParams p) {
     const int h = x.head / p.groups, g0 = (x.head - h * p.groups) * p.G;
     const int t = prow / PK_ROWS, row = prow - t * PK_ROWS, l0 = p.by_g.div(row), g = row - l0 * p.G, l = x.token + t * p.T + l0;
     if (l0 >= p.T || l >= x.n || g0 + g >= p.share) return;
-    const int64_t slot = x.slot;
-    auto stat = [&](int w) { return *reinterpret_cast<const float2*>(p.part_ml + ((slot + w) * 2 * PK_ROWS + prow) * 2); };
+    auto slot = [&](int w) -> int64_t { return w == 0 ? x.slot : 2 * (x.slot / 2 + w); };
+    auto stat = [&](int w) { return *reinterpret_cast<const float2*>(p.part_ml + (slot(w) * 2 * PK_ROWS + prow) * 2); };
     float M = -INFINITY, sum = 0.f, v[2][8] = {};
     for (int w = 0; w < x.parts; ++w) M = fmaxf(M, stat(w).x);
     for (int w = 0; w < x.parts; ++w) {
         const float2 ml = stat(w);
         const float f = ml.x == M ? 1.f : exp2f(ml.x - M);
-        const float4* y = reinterpret_cast<const float4*>(p.part + (slot + w) * (2 * PK_ROWS * EP)) + e / 4 * (2 * PK_ROWS) + prow;
+        const float4* y = reinterpret_cast<const float4*>(p.part + slot(w) * (2 * PK_ROWS * EP)) + e / 4 * (2 * PK_ROWS) + prow;
         sum = fmaf(ml.y, f, sum);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -1099,11 +1152,13 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     if (rc) return rc;
     const int64_t sms = ctx->prop.multiProcessorCount;
     p.sms = (int)sms, p.most = (int)entries;
+    // The list and the second launch cost 2 to 6 us (20 heads of 64 over 77 keys 7.4 us without, 13.0 with), cut keys save more where there are many
+    // (16 heads of 128 on 8, 100 rows over 1800 keys 24.2 without, 26.2 with; over 3100 35.9 and 29.8).
     p.planned = items > sms || p.Nk > 16 * PK_KEYS;
-    const int64_t slots = sms, rows = slots * 2 * PK_ROWS;
+    const int64_t slots = 2 * sms, rows = slots * 2 * PK_ROWS;
     if (p.planned) {
         void* ws = nullptr;
-        const size_t list = (size_t)entries * (sizeof(PackedEntry) + 2 * sizeof(int)) + p.B * sizeof(int) + slots * sizeof(PackedCut) + sizeof(int4) + 16 * 8;
+        const size_t list = (size_t)entries * (sizeof(PackedEntry) + sizeof(int)) + p.B * sizeof(int) + sms * sizeof(PackedCut) + 2 * sizeof(int4) + 16 * 8;
         rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float) + list, &ws);
         if (rc) return rc;
         uint8_t* at = static_cast<uint8_t*>(ws);
@@ -1115,10 +1170,9 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
         p.part = (float*)room(rows * EP * sizeof(float));
         p.part_ml = (float*)room(rows * 2 * sizeof(float));
         p.entry = (PackedEntry*)room(entries * sizeof(PackedEntry));
-        p.cut = (PackedCut*)room(slots * sizeof(PackedCut));
-        p.counts = (int4*)room(sizeof(int4));
-        p.unit = (int*)room(entries * sizeof(int));
-        p.slot = (int*)room(entries * sizeof(int));
+        p.cut = (PackedCut*)room(sms * sizeof(PackedCut));
+        p.counts = (int4*)room(2 * sizeof(int4));
+        p.before = (int*)room(entries * sizeof(int));
         p.first = (int*)room(p.B * sizeof(int));
         B200_CUDA(launch_dep(packed_plan_kernel, dim3(1), dim3(PL_THREADS), 0, ctx->stream, 1, p));
         ctx->launches++;
@@ -1127,7 +1181,7 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     B200_CUDA(launch_dep(kern, dim3((unsigned)grid), dim3(PK_THREADS), Cfg::SMEM, ctx->stream, 1, tq, tk, tv, to, p));
     ctx->launches++;
     if (p.planned) {
-        B200_CUDA(launch_dep(packed_join_kernel<EP>, dim3((unsigned)(sms / 2 * (EP / 16))), dim3(256), 0, ctx->stream, 1, p));
+        B200_CUDA(launch_dep(packed_join_kernel<EP>, dim3((unsigned)(sms * (EP / 16))), dim3(256), 0, ctx->stream, 1, p));
         ctx->launches++;
     }
     return B200_OK;
