@@ -139,6 +139,7 @@ beam_scan_kernel(const BeamParams p) {
     const int stop = block0 + p.tiles * TILE < end ? block0 + p.tiles * TILE : end;
     unsigned long long list = 0;                     // no element's key is 0
     float m = -INFINITY, s = 0.f;
+    if (threadIdx.x == 0) count = 0;                 // read behind a barrier, of a block behind the row's end too
     const int full = (end - block0) / (32 * U), warps = full < BM_WARPS ? full : BM_WARPS;      // warps with an element in every lane
 #pragma unroll 1
     for (int tile = block0; tile < stop; tile += TILE) {
@@ -196,10 +197,7 @@ beam_scan_kernel(const BeamParams p) {
             }
             if (lane == 0) bounds[warp] = warp < warps ? nth : 0xffffffffu;
         }
-        if (tile == block0) {
-            if (threadIdx.x == 0) count = 0;
-            __syncthreads();
-        }
+        if (tile == block0) __syncthreads();
         const float bound = warps > 0 ? bm_number(__reduce_min_sync(0xffffffffu, bounds[lane & (BM_WARPS - 1)])) : -INFINITY;
         // the candidates
         uint32_t hits = 0;

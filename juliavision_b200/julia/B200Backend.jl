@@ -359,6 +359,37 @@ function cachesdpa!(ctx::Ctx{B200Backend}, out, q, cache::Cache8, table, lens; n
     out
 end
 
+s3(a) = (r = rootstrides(a); Strided4(Ptr{Cvoid}(r[1]), (Int64.(r[2])[1:3]..., Int64(0))))       # three axes
+# Sequences side by side: q, out (E, N, Hq), k, v (E, Nk, H), starts and kstarts one Int32 more than sequences.
+function packedsdpa!(ctx::Ctx{B200Backend}, out, q, k, v, starts; kstarts = starts, scale = 1 / sqrt(size(q, 1)), causal = true)
+    check(ccall((:b200_attention_packed_f16, LIB), Cint,
+                (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Ref{Strided4}, Ref{Strided4}, Cint, Cfloat, Cint,
+                 Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, size(q, 1), size(q, 2), size(k, 2), size(q, 3), size(k, 3), length(starts) - 1, s3(q), s3(k), s3(v), s3(out),
+                dtcode(eltype(out)), Float32(scale), causal, pointer(starts), pointer(kstarts)))
+    out
+end
+
+# The N best of K * V continuations: best, parents, tokens (N, B); logits (V, K, B), scores (K, B).
+function beamselect!(ctx::Ctx{B200Backend}, best, parents, tokens, logits, scores; ended = nothing, pad = 0)
+    V, K, B = size(logits)
+    check(ccall((:b200_beam_select, LIB), Cint,
+                (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Cint, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, V, K, B, size(best, 1), pointer(logits), dtcode(eltype(logits)), stride(logits, 2), stride(logits, 3),
+                pointer(scores), nullable(ended), pad, pointer(best), pointer(parents), pointer(tokens)))
+    best, parents, tokens
+end
+
+# Beam k of search b goes on from beam parents[k, b] (counted from 0) in all of `caches`; table, own (pages a sequence, K * B).
+function cachereorder!(ctx::Ctx{B200Backend}, caches::AbstractVector, table, own, parents, lens)
+    c = Cache8C[cachec(x, table) for x in caches]
+    check(ccall((:b200_cache_reorder, LIB), Cint,
+                (Ptr{Cvoid}, Ptr{Cache8C}, Int64, Int64, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}),
+                ctx.backend.handle, c, length(c), size(parents, 1), size(parents, 2), pointer(table), stride(table, 2), pointer(own),
+                stride(own, 2), size(table, 1), pointer(parents), pointer(lens)))
+    table
+end
+
 struct Q4                           # b200_q4; the arrays it points to are Weight4's
     data::Ptr{Cvoid}
     scales::Ptr{Cvoid}

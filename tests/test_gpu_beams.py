@@ -130,6 +130,18 @@ def test_strides_and_alignment(ctx, dtype, offset):
     agree(select(ctx, x, scores, 7, device=two), want)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_rows_that_end_where_a_block_does(ctx, dtype):
+    """Rows of an odd pitch start at all places of a vector; those that start on one leave a block without an element."""
+    rng = np.random.default_rng(8)
+    V = 1024 * (8 if dtype == F16 else 4)
+    x, scores = rng.standard_normal((2, 5, V + 1)).astype(dtype), -rng.random((2, 5)).astype(F32)
+    d = ctx.toback(x)
+    rows = jv.DeviceArray(ctx, d.ptr, dtype, (V, 5, 2), (1, V + 1, 5 * (V + 1)), owner=d)
+    for _ in range(3):
+        agree(select(ctx, x[..., :V], scores, 9, device=rows), choice(x[..., :V], scores, 9))
+
+
 def test_recorded_choice(ctx):
     rng = np.random.default_rng(4)
     x, scores = rng.standard_normal((3, 5, 30011)).astype(F16), -rng.random((3, 5)).astype(F32)
