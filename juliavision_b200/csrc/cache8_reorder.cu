@@ -5,16 +5,18 @@
 //
 // Bandwidth-bound: the tokens of a part-filled page, read and written, for every beam whose parent is another.  A thread takes the same 16
 // bytes of all of a search's beams and reads them all before it writes any, so the beams may change places in any way without a second copy.
-// 16 searches of 4 beams in 16 caches of 8 heads of 128, 55 MB in all: 13.4 us (4.1 TB/s; the copy's rate would give 8.3), of 5 beams in 32
-// caches of 20 heads of 64, 11 MB: 5.7 us, of which a launch and three reads that wait for one another are more than half.  Blocks go round the
-// sides of the caches, as many as are filled, sixteen blocks an SM: a block for each 256 vectors a page might have looked everything up for
-// nothing or for one vector a thread (18.2 us), and with eight an SM, six of which are resident, fewer reads are under way (14.2 us).
+// 16 searches of 4 beams in 16 caches of 8 heads of 128, 55 MB in all: 11.6 us (4.7 TB/s; the copy's rate would give 8.3), of 5 beams in 32
+// caches of 20 heads of 64, 11 MB: 5.3 us, of which a launch and three reads that wait for one another are more than half.  A block takes a head
+// of a cache's keys or values at a time, whatever is filled of the page, and goes on to another where there are more than 32 blocks an SM (16:
+// 12.3 us, 12: 13.6).  By 256 vectors over all heads, which costs three divisions a vector, it took 13.4 us, and with a block for each that a
+// full page would have 18.2.
 #include "cache8.cuh"
 
 namespace b200 {
 
 constexpr int CR_CACHES = 128;       // of a launch
 constexpr int CR_BEAMS = 32;         // of a search
+constexpr int CR_THREADS = 128;
 
 struct ReorderParams {
     uint8_t* data[2 * CR_CACHES];    // keys and values of a cache
@@ -23,6 +25,7 @@ struct ReorderParams {
     int32_t* table;
     const int32_t *own, *parents, *lens;
     int64_t table_ld, own_ld;
+    Divisor by_vectors;              // of a token and head
     int K, sides, tables;            // keys and values of all caches; whether this launch brings the table up to date
 };
 
@@ -43,7 +46,7 @@ __device__ __forceinline__ int cr_parent(const ReorderParams& p, int64_t search,
 }
 
 template <int K>     // beams of a search at most
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(CR_THREADS)
 cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
     __shared__ int parent[CR_BEAMS];
     __shared__ int64_t page[CR_BEAMS], source[CR_BEAMS];          // that a beam writes, or -1; that it copies from, or -1
@@ -70,7 +73,7 @@ cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
     if (tid < p.K) source[tid] = parent[tid] != tid && page[tid] >= 0 ? page[parent[tid]] : -1;
     __syncthreads();
     if (blockIdx.x < (unsigned)p.tables) {       // the first block: the table
-        for (int i = tid; i < p.c.width; i += 256) {
+        for (int i = tid; i < p.c.width; i += CR_THREADS) {
             int32_t* at = p.table + search * p.K * p.table_ld + i;
             int32_t was[K];
 #pragma unroll
@@ -82,16 +85,15 @@ cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
         return;
     }
     if (s.kept == 0) return;
-    const int per = p.c.E / 16, row = s.kept * per;               // of a head
-    const int blocks = (row * p.c.H + 255) / 256;                 // of a side
-    const int stride = gridDim.x - p.tables;
-    for (int unit = blockIdx.x - p.tables; unit < p.sides * blocks; unit += stride) {
-        const int side = unit / blocks, block = unit - side * blocks, i = block * 256 + tid;
+    const int row = s.kept * (p.c.E / 16), stride = gridDim.x - p.tables;        // vectors of a head
+    for (int unit = blockIdx.x - p.tables; unit < p.sides * p.c.H; unit += stride) {
+        const int side = unit / p.c.H, h = unit - side * p.c.H;
         const bool value = side & 1;
-        if (i < row * p.c.H) {
-            const int h = i / row, t = (i - h * row) / per, e = i - h * row - t * per;
-            uint8_t* at = p.data[side] + t * (value ? p.c.vT : p.c.kT) + h * (value ? p.c.vH : p.c.kH) + e * 16;
-            const int64_t pitch = value ? p.c.vP : p.c.kP;
+        uint8_t* head = p.data[side] + h * (value ? p.c.vH : p.c.kH);
+        const int64_t pitch = value ? p.c.vP : p.c.kP, token = value ? p.c.vT : p.c.kT;
+        for (int i = tid; i < row; i += CR_THREADS) {
+            const int t = p.by_vectors.div(i);
+            uint8_t* at = head + t * token + (i - t * (p.c.E / 16)) * 16;
             uint4 v[K];
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -100,17 +102,13 @@ cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
             for (int k = 0; k < K; ++k)
                 if (k < p.K && source[k] >= 0) *reinterpret_cast<uint4*>(at + page[k] * pitch) = v[k];
         }
-        if (block == 0)
-            for (int h = tid; h < p.c.H; h += 256) {
-                float* at = p.most[side] + h;
-                float v[K];
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k < p.K && source[k] >= 0) v[k] = at[source[k] * p.c.H];
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-                    if (k < p.K && source[k] >= 0) at[page[k] * p.c.H] = v[k];
-            }
+        if (tid < 32) {              // the maxima: a lane a beam
+            float* at = p.most[side] + h;
+            const bool on = tid < p.K && source[tid] >= 0;
+            const float v = on ? at[source[tid] * p.c.H] : 0.f;
+            __syncwarp();
+            if (on) at[page[tid] * p.c.H] = v;
+        }
     }
 }
 
@@ -143,8 +141,7 @@ int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int6
         for (int64_t j = 0; j < i; ++j) twice |= caches[j].k == c.k || caches[j].v == c.v || caches[j].k == c.v || caches[j].v == c.k;
         B200_REQUIRE(!twice, B200_EINVAL, "cache_reorder: the array of cache %lld is given twice", (long long)i);
     }
-    const int64_t blocks = cdiv((int64_t)p.c.H * p.c.T * (p.c.E / 16), 256);
-    B200_REQUIRE(blocks < (1 << 23), B200_DECLINE_EXTENT, "cache_reorder: %d heads", p.c.H);
+    p.by_vectors = Divisor::of(p.c.E / 16);
     B200_CUDA(cudaSetDevice(ctx->device));
     p.table = table, p.table_ld = table_ld, p.own = own, p.own_ld = own_ld;
     p.parents = parents, p.lens = lens;
@@ -158,9 +155,9 @@ int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int6
         }
         p.tables = at == 0;
         p.sides = 2 * count;
-        const int64_t share = cdiv(16 * (int64_t)ctx->prop.multiProcessorCount, B), units = p.sides * blocks;      // sixteen blocks an SM
+        const int64_t share = cdiv(32 * (int64_t)ctx->prop.multiProcessorCount, B), units = p.sides * (int64_t)p.c.H;      // 32 blocks an SM
         const int64_t grid = p.tables + (units < share ? units : share);
-        const dim3 g((unsigned)grid, (unsigned)B), b(256);
+        const dim3 g((unsigned)grid, (unsigned)B), b(CR_THREADS);
         auto run = [&](auto kern) { return launch_dep(kern, g, b, 0, ctx->stream, 1, p); };
         B200_CUDA(K <= 4 ? run(cache_reorder_kernel<4>) : K <= 8 ? run(cache_reorder_kernel<8>) : K <= 16 ? run(cache_reorder_kernel<16>)
                                                                                                         : run(cache_reorder_kernel<32>));
