@@ -5,10 +5,11 @@
 // Bandwidth-bound: two bytes read and two written an element.  A warp takes one token and some or all of its heads.  It computes the
 // token's cosines and sines once, a pair a lane, and hands them round through shared memory of its own; then a group of lanes takes a head,
 // 16 elements a lane, so that both halves of a pair lie in one lane and the sum of squares is a few shuffles.  Nothing waits for another
-// warp.  40 heads of 128 of 2 x 8192 tokens, 294 MB there and back: 58 us (5.05 TB/s; the copy's rate would give 45), 24 of 96 of 7 x 611, 31 MB:
-// 8.3, 40 of 64 of 8 tokens: 3.9, a launch.  What is under way at once bounds the large ones: cosines, sines and weights take 48 registers a
-// lane, which leaves 24 warps an SM.  One head of a group at a time takes 61.8 and 9.4 us, four 67 and 11.7; cosines and sines read from
-// shared memory for each head 55 and 8.8; fewer registers by force spill (61 to 69).
+// warp.  40 heads of 128 of 2 x 8192 tokens, 294 MB there and back: 55 us (5.35 TB/s; the copy's rate would give 45), 24 of 96 of 7 x 611, 31 MB:
+// 8.4, 40 of 64 of 8 tokens: 3.9, a launch.  What is under way at once bounds the large ones: 72 registers a lane leave 28 warps an SM.  With the
+// turns in registers too, read once a token and not once a head, there are 24 (58.5 us); arithmetic on one element at a time and not on
+// two, which takes more of them and more instructions, 55.2 and 8.8; one head of a group at a time 61.8 and 9.4, four 67 and 11.7; fewer
+// registers by force spill (61 to 69).
 #include <cuda_fp16.h>
 
 #include "internal.h"
@@ -57,29 +58,26 @@ __device__ __forceinline__ int nr_column(const NormRotaryParams& p, int h) { ret
 template <int G, int U>
 __global__ void __launch_bounds__(32 * NR_WARPS)
 norm_rotary_kernel(const NormRotaryParams p) {
-    __shared__ __align__(16) float2 turns[NR_WARPS][8 * G];
+    __shared__ __align__(16) float turns[NR_WARPS][16 * G];      // cosines and sines of two pairs together, those of a lane G apart
     const int lane = threadIdx.x & 31, g = lane / G, u = lane % G, half = p.rot / 2, units = p.rot / 16;
     grid_dep_wait();
     grid_dep_launch();
     NormRotaryWork w;
     if (!w.of(p)) return;       // the same for the warp
-    float2* mine = turns[threadIdx.x >> 5];
+    float* mine = turns[threadIdx.x >> 5];
     for (int i = lane; i < half; i += 32) {
         float s, c;
         rot_turn(w.position, p.freq[i], s, c);
-        mine[i] = make_float2(c * p.gain, s * p.gain);
+        float* to = mine + ((i % 8 / 2) * G + i / 8) * 4 + i % 2;
+        to[0] = c * p.gain, to[2] = s * p.gain;
     }
     __syncwarp();
     const bool on = u * 16 < p.E, turned = u < units;
     const int e0 = !turned || p.interleaved ? u * 16 : u * 8, e1 = turned && !p.interleaved ? e0 + half : e0 + 8;
-    float cs[8], sn[8], wt[16];
+    uint64_t wt[8];                          // of two elements
+    const uint64_t minus = pack2(-1.f, -1.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 t = turned ? mine[u * 8 + j] : make_float2(1.f, 0.f);
-        cs[j] = t.x, sn[j] = t.y;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) wt[j] = 1.f;
+    for (int j = 0; j < 8; ++j) wt[j] = pack2(1.f, 1.f);
     int have = -1;
     const __half* x = p.x + w.l * p.xL + w.b * p.xB;
     __half* o = p.out + w.l * p.oL + w.b * p.oB;
@@ -100,13 +98,16 @@ norm_rotary_kernel(const NormRotaryParams p) {
         for (int k = 0; k < U; ++k) {
             const int head = h + k * STEP;
             const uint32_t raw[8] = {a[k].x, a[k].y, a[k].z, a[k].w, b[k].x, b[k].y, b[k].z, b[k].w};
-            float v[16], sum = 0.f;
+            uint64_t v[8], squares = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float2 f = rot_unpack(raw[j]);
-                v[2 * j] = f.x, v[2 * j + 1] = f.y;
-                sum = fmaf(f.x, f.x, fmaf(f.y, f.y, sum));
+                v[j] = pack2(f.x, f.y);
+                squares = fma2(v[j], v[j], squares);
             }
+            float sum, odd;
+            unpack2(squares, sum, odd);
+            sum += odd;
 #pragma unroll
             for (int d = 1; d < G; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (!on || head >= w.h1) continue;
@@ -118,7 +119,7 @@ norm_rotary_kernel(const NormRotaryParams p) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float4 f = __ldg(reinterpret_cast<const float4*>(q + (j < 2 ? e0 : e1) + (j & 1) * 4));
-                        wt[4 * j] = f.x, wt[4 * j + 1] = f.y, wt[4 * j + 2] = f.z, wt[4 * j + 3] = f.w;
+                        wt[2 * j] = pack2(f.x, f.y), wt[2 * j + 1] = pack2(f.z, f.w);
                     }
                 } else {
                     const __half* q = (const __half*)p.weight + column * p.weight_ld;
@@ -129,27 +130,38 @@ norm_rotary_kernel(const NormRotaryParams p) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float2 t = rot_unpack(r[i]);
-                            wt[8 * j + 2 * i] = t.x, wt[8 * j + 2 * i + 1] = t.y;
+                            wt[4 * j + i] = pack2(t.x, t.y);
                         }
                     }
                 }
             }
             const float r = rsqrtf(fmaf(sum, each, p.eps));
+            const uint64_t rr = pack2(r, r);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = v[j] * r * wt[j];
+            for (int j = 0; j < 8; ++j) v[j] = mul2(mul2(v[j], rr), wt[j]);
             uint32_t to[8];
+            auto rounded = [](uint64_t y) {
+                float a, b;
+                unpack2(y, a, b);
+                return rot_pack(a, b);
+            };
+            auto turn = [&](int j) { return reinterpret_cast<const ulonglong2*>(mine)[j * G + u]; };
             if (!turned) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) to[j] = rot_pack(v[2 * j], v[2 * j + 1]);
+                for (int j = 0; j < 8; ++j) to[j] = rounded(v[j]);
             } else if (p.interleaved) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    to[j] = rot_pack(v[2 * j] * cs[j] - v[2 * j + 1] * sn[j], v[2 * j + 1] * cs[j] + v[2 * j] * sn[j]);
+                for (int j = 0; j < 8; ++j) {
+                    float a, b, c[2], s[2];
+                    unpack2(v[j], a, b), unpack2(turn(j / 2).x, c[0], c[1]), unpack2(turn(j / 2).y, s[0], s[1]);
+                    to[j] = rot_pack(a * c[j & 1] - b * s[j & 1], b * c[j & 1] + a * s[j & 1]);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    to[j] = rot_pack(v[2 * j] * cs[2 * j] - v[8 + 2 * j] * sn[2 * j], v[2 * j + 1] * cs[2 * j + 1] - v[9 + 2 * j] * sn[2 * j + 1]);
-                    to[4 + j] = rot_pack(v[8 + 2 * j] * cs[2 * j] + v[2 * j] * sn[2 * j], v[9 + 2 * j] * cs[2 * j + 1] + v[2 * j + 1] * sn[2 * j + 1]);
+                    const ulonglong2 y = turn(j);
+                    to[j] = rounded(fma2(v[j], y.x, mul2(mul2(v[4 + j], minus), y.y)));
+                    to[4 + j] = rounded(fma2(v[4 + j], y.x, mul2(v[j], y.y)));
                 }
             }
             __half* q = o + head * p.oH;
