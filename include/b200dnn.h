@@ -311,7 +311,7 @@ int b200_cache_attention(b200_ctx* ctx, const b200_cache8* cache, int64_t L, int
 /* -------------------------------------------------------------------- beam search */
 /*
  * Of the K V continuations scores[k] + x[v,k] - log sum_u exp x[u,k] of each of B searches the N best, in order, ties to the lowest
- * k V + v: best, parents and tokens (N,B).  logits (V,K,B), fp16 or fp32, V contiguous, beams ldk and searches ldb elements apart; scores (K,B).
+ * k V + v: best, parents and tokens (N,B), apart from what is read.  logits (V,K,B), fp16 or fp32, V contiguous, beams ldk and searches ldb elements apart; scores (K,B).
  * Logits are read in whole aligned 16-byte blocks.  A beam with ended[k,b] != 0 (ended NULL: none) has one continuation, token `pad` at its own score.
  * A beam whose score is not finite, or whose logits have no finite log sum, offers its tokens at -inf, which come last, lowest first.
  * Exponentials are fp32, their sums over shares fp32, over a row and the scores fp64.  K and N are at most 32, N at most K V.  Scratch comes
@@ -323,7 +323,8 @@ int b200_beam_select(b200_ctx* ctx, int64_t V, int64_t K, int64_t B, int64_t N, 
  * the tokens of beam parents[k,b].  own (width,K B): the pages that each beam writes, no page twice.  In the table, entries below the last full
  * page become the parent's, the others the beam's own; the tokens and maxima of the page that is not full are copied from the
  * parent's own page to the beam's.  lens (K,B): the beams of a search are equally long (the first one's counts; others are reported).
- * A parent outside [0,K) leaves the beam where it was, a page outside the cache is not touched; the next b200_sync reports either. */
+ * A parent outside [0,K) leaves the beam where it was, a page outside the cache is not touched; the next b200_sync reports either.
+ * No array of keys or values is given twice. */
 int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int64_t K, int64_t B, int32_t* table, int64_t table_ld,
                        const int32_t* own, int64_t own_ld, int64_t width, const int32_t* parents, const int32_t* lens);
 

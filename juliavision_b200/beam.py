@@ -2,7 +2,7 @@
 decoder).
 
 A step of a search of K beams: the model's logits, `beamselect_`, `cachereorder_` with the parents it gives, the next token.  Nothing is read
-back between, so a step can be recorded; the host follows parents and tokens afterwards.
+back between, so a step can be recorded; the host follows parents and tokens afterwards, or between replays where it marks beams as ended.
 """
 from __future__ import annotations
 
@@ -29,7 +29,7 @@ def beamselect_(ctx: Ctx, best: DeviceArray, parents: DeviceArray, tokens: Devic
     sums, beams and tokens as best (N, B) fp32, parents and tokens (N, B) int32.  logits (V, K, B) or (V, K * B), fp16 or fp32, V contiguous;
     scores (K, B) fp32.  A beam whose number in ended (K, B) int32 is not 0 has one continuation, the token `pad` at its own score.  A
     beam whose score is not finite, or whose logits have no finite log sum (a NaN, +inf, nothing but -inf), offers its tokens at -inf; they come last, lowest
-    first.  At most 32 beams and 32 results."""
+    first.  At most 32 beams and 32 results, which lie apart from what is read."""
     rc = _lib.host().beamselect(ctx.handle, best, parents, tokens, logits, scores, ended, pad)
     if rc is not None:
         check(rc)
@@ -56,7 +56,7 @@ def cachereorder_(ctx: Ctx, caches: Union[Cache8, Sequence[Cache8]], table: Devi
     a layer, of the same sizes and strides, which share `table` (pages a sequence, K * B), sequence k + K b being beam k of search b.
     own (pages a sequence, K * B) names the pages that each beam writes, no page twice; a table starts as a copy of it.  Whole pages change
     hands in `table`; the page that is not full is copied to the beam's own, and entries behind it become the beam's own again.  lens (K * B): a
-    search's beams are equally long.  A prompt is handed to all beams by parents of 0 after it has been written as beam 0's."""
+    search's beams are equally long.  No array is given twice.  A prompt is handed to all beams by parents of 0 after it has been written as beam 0's."""
     rc = _lib.host().cachereorder(ctx.handle, caches, table, own, parents, lens)
     if rc is not None:
         check(rc)

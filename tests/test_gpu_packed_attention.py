@@ -270,3 +270,19 @@ def test_two_contexts_at_once(ctx):
     for p, (_, _, buf) in zip(made, held):
         p.ctx.synchronize()
         p.check(buf.to_host(), F16, True)
+
+
+@pytest.mark.parametrize("E", [64, 128])
+@pytest.mark.parametrize("shape", ["left over", "few", "some long"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_dealt_out(ctx, E, shape, causal):
+    """Pairs that are alike and do not go round the SMs: whole ones first and the rest cut; fewer than SMs; long ones of unequal lengths among
+    short ones.  The same bits every time."""
+    rng = np.random.default_rng(15)
+    news, past, Hq, H = {"left over": ([8] * 160, [1500] * 160, 1, 1), "few": ([130] * 3, [2600] * 3, 4, 2),
+                         "some long": ([40, 3, 100, 256] + [20] * 60, [9000, 5000, 12000, 7000] + list(rng.integers(0, 200, 60)), 3, 3)}[shape]
+    p = Packed(ctx, rng, E, Hq, H, news, past)
+    first = p.run(F16, causal)
+    p.check(first, F16, causal)
+    for _ in range(3):
+        assert np.array_equal(first[:p.starts[-1]], p.run(F16, causal)[:p.starts[-1]])
