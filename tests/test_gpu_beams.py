@@ -247,3 +247,33 @@ def test_bad_entries_are_skipped_and_reported(ctx, wrong):
         assert np.array_equal(new[0], want) and np.array_equal(dtable.to_host(), [[0, 1], [2, 3], [2, 5]])
     if wrong in ("page", "length"):      # nothing to copy from, or to; or no page that is part full
         assert np.array_equal(new[0], old[0]) and np.array_equal(new[3], old[3])
+
+
+def test_offsets_past_32_bits(ctx):
+    """Searches that lie further than 2^32 bytes apart."""
+    rng = np.random.default_rng(9)
+    V, K, ldb = 1003, 3, (1 << 31) + 40
+    d = ctx.allocate(F16, ldb + K * V)
+    x, scores = rng.standard_normal((2, K, V)).astype(F16), -rng.random((2, K)).astype(F32)
+    for b in range(2):
+        ctx.upload(jv.DeviceArray(ctx, d.ptr + 2 * ldb * b, F16, (V, K), owner=d), x[b])
+    agree(select(ctx, x, scores, 5, device=jv.DeviceArray(ctx, d.ptr, F16, (V, K, 2), (1, V, ldb), owner=d)), choice(x, scores, 5))
+
+
+def test_reorder_past_32_bits(ctx):
+    E, T, H, P = 128, 128, 8, 40000                     # 5.2 GB of keys and of values
+    c = jv.Cache8(*(ctx.allocate(np.int8, E, T, H, P) for _ in range(2)), *(ctx.allocate(F32, H, P) for _ in range(2)))
+    rng = np.random.default_rng(10)
+    own = np.array([[39999], [3], [39000]])
+    page = lambda a, g: jv.DeviceArray(ctx, a.ptr + g * E * T * H, np.int8, (E, T, H), owner=a)  # noqa: E731
+    data = rng.integers(-127, 128, (3, 2, H, T, E)).astype(np.int8)
+    for s in range(3):
+        for i, a in enumerate((c.k, c.v)):
+            ctx.upload(page(a, own[s, 0]), data[s, i])
+    jv.cachereorder_(ctx, c, ints(ctx, own), ints(ctx, own), ints(ctx, [[1, 2, 0]]), ints(ctx, [77] * 3))
+    ctx.synchronize()
+    for s, source in enumerate((1, 2, 0)):
+        for i, a in enumerate((c.k, c.v)):
+            want = data[s, i].copy()
+            want[:, :77] = data[source, i][:, :77]
+            assert np.array_equal(page(a, own[s, 0]).to_host(), want)

@@ -135,3 +135,20 @@ def test_recorded(ctx):
         call()
         ctx.synchronize()
         assert np.array_equal(replayed, out.to_host())
+
+
+def test_offsets_past_32_bits(ctx):
+    """Sequences that lie further than 2^32 bytes apart."""
+    rng = np.random.default_rng(6)
+    E, L, H, apart = 64, 5, 3, (1 << 31) + 64
+    d = ctx.allocate(F16, apart + L * H * E)
+    x = rng.standard_normal((2, L, H, E)).astype(F16)
+    part = lambda b: jv.DeviceArray(ctx, d.ptr + 2 * apart * b, F16, (E, H, L), owner=d)  # noqa: E731
+    for b in range(2):
+        ctx.upload(part(b), x[b])
+    view = jv.DeviceArray(ctx, d.ptr, F16, (E, L, H, 2), (1, H * E, E, apart), owner=d)
+    jv.normrotary_(ctx, jv.rotaryplan(ctx, E), view, view, lens=ints(ctx, [L, 99]))
+    ctx.synchronize()
+    z = normed(x, np.ones((H, E)), 1e-6)
+    want = ref.rotary(z, np.array([[0], [94]]) + np.arange(L), jv.rotaryfrequencies(E)[0], 1.0, False)
+    near(np.stack([part(b).to_host() for b in range(2)]), want, tolerance(want, z, E, 1.0))

@@ -286,3 +286,25 @@ def test_keys_dealt_out(ctx, E, shape, causal):
     p.check(first, F16, causal)
     for _ in range(3):
         assert np.array_equal(first[:p.starts[-1]], p.run(F16, causal)[:p.starts[-1]])
+
+
+def test_offsets_past_32_bits(ctx):
+    """The last rows of arrays of more than 2^32 bytes, queries and results; keys and values of them through a stride."""
+    rng = np.random.default_rng(16)
+    E, Hq, n, m = 128, 32, 150, 200
+    N, Nk = (1 << 19) + 300, 70000
+    p = Packed(ctx, rng, E, Hq, 1, [n], [m - n], spare=0)
+    q, out = (ctx.allocate(F16, E, Hq, N) for _ in range(2))
+    k = ctx.allocate(F16, 256 * E, Nk)
+    last = lambda a, rows: jv.DeviceArray(ctx, a.ptr + 2 * Hq * E * (N - rows), F16, (E, Hq, rows), owner=a)  # noqa: E731
+    ctx.upload(last(q, n), p.q)
+    ctx.fill_bytes(last(out, n), 0xFF)
+    at = lambda i, row: jv.DeviceArray(ctx, k.ptr + 2 * E * (256 * row + i), F16, (E,), owner=k)  # noqa: E731
+    for row in range(m):
+        for i, a in ((0, p.k), (255, p.v)):
+            ctx.upload(at(i, Nk - m + row), np.ascontiguousarray(a[row, 0]))
+    dk, dv = (jv.DeviceArray(ctx, k.ptr + 2 * E * i, F16, (E, Nk, 1), (1, 256 * E, E), owner=k) for i in (0, 255))
+    ctx.ws.reset()
+    jv.packedsdpa_(ctx, out.permute((0, 2, 1)), q.permute((0, 2, 1)), dk, dv, ints(ctx, [N - n, N]), ints(ctx, [Nk - m, Nk]))
+    ctx.synchronize()
+    p.check(last(out, n).to_host(), F16, True)
