@@ -15,6 +15,7 @@
 // order, took 57 us.)  Rows with more candidates than there is room, ties of thousands or logits that rise all along, put the others into
 // a list of the warp's 32 largest, one a lane.  The second launch, a block a search, merges a row's parts, takes log sums and scores in fp64
 // and merges the rows'.
+#include <cfloat>
 #include <cuda_fp16.h>
 
 #include "internal.h"
@@ -198,7 +199,8 @@ beam_scan_kernel(const BeamParams p) {
             if (lane == 0) bounds[warp] = warp < warps ? nth : 0xffffffffu;
         }
         if (tile == block0) __syncthreads();
-        const float bound = warps > 0 ? bm_number(__reduce_min_sync(0xffffffffu, bounds[lane & (BM_WARPS - 1)])) : -INFINITY;
+        // -inf is no candidate, however few others a row has: the second launch knows which tokens come then
+        const float bound = fmaxf(warps > 0 ? bm_number(__reduce_min_sync(0xffffffffu, bounds[lane & (BM_WARPS - 1)])) : -INFINITY, -FLT_MAX);
         // the candidates
         uint32_t hits = 0;
 #pragma unroll
@@ -347,9 +349,21 @@ beam_pick_kernel(const BeamParams p) {
             if (lane == 0 && !over) value = score;
             if (over) token = (uint32_t)lane;
         } else if (!over && sum < INFINITY && sum > -INFINITY) {
-            some = list != 0;
+            const int found = __popc(__ballot_sync(0xffffffffu, list != 0 && lane < p.N));
             token = ~(uint32_t)list;
-            value = score + ((double)bm_number((uint32_t)(list >> 32)) - sum);
+            if (list != 0) value = score + ((double)bm_number((uint32_t)(list >> 32)) - sum);
+            if (found < p.N) {              // then those at -inf, lowest first: the lane - found th that is not listed
+                uint32_t t = (uint32_t)(lane - found);
+                for (int round = 0; round < found; ++round) {
+                    uint32_t below = 0;
+                    for (int i = 0; i < found; ++i) below += __shfl_sync(0xffffffffu, token, i) <= t;
+                    t = (uint32_t)(lane - found) + below;
+                }
+                if (lane >= found) token = t;
+                some = lane < found || (int64_t)t < p.V;
+            } else {
+                some = true;
+            }
         }
         if (some && lane < p.N) {
             const unsigned long long b = (unsigned long long)__double_as_longlong(value + 0.0);

@@ -109,6 +109,21 @@ def test_what_is_not_finite(ctx):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("V", [5, 40, 3000, 60000])
+def test_few_tokens_that_may_come(ctx, dtype, V):
+    """All but a few logits at -inf: those few, and then the lowest of the others at -inf, whichever of them are among the few."""
+    rng = np.random.default_rng(11)
+    N = min(20, V)
+    x, scores = np.full((6, 2, V), -np.inf, dtype), -rng.random((6, 2)).astype(F32)
+    for b, few in enumerate(([], [0], [V - 1, 1], list(range(N - 2)), [0, 2, 3, 4], list(range(max(V - 25, 0), V)))):
+        for k in range(2):
+            for t in few:
+                x[b, k, t] = rng.standard_normal()
+    scores[4, 1] = -np.inf
+    agree(select(ctx, x, scores, N), choice(x, scores, N))
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("offset", [0, 1, 3, 5])
 def test_strides_and_alignment(ctx, dtype, offset):
     """Rows that start anywhere, beams and searches apart; the two-axis form of a projection's result."""
