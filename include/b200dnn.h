@@ -240,8 +240,8 @@ int b200_attention_f16_route(int64_t E, int64_t Lq, int64_t Lk, int64_t H, int64
  * were.  A key that a row does not see has no part in it, whatever it holds.  q, k and v fp16, out fp16 or fp32; scale is 0 or more.
  * Scores, softmax and sums are fp32; the weights of the second product are rounded to fp16, up to 2^8 of the heaviest when it came and times 2^7.
  * starts and kstarts are device arrays of B + 1 numbers; where they are not in order or past the arrays they are cut, and the next b200_sync
- * reports it (B200_EKERNEL).  out overlaps no operand.  Scratch comes from the context's workspace (40 MB at most, and a copy of each
- * operand whose pointer or strides are not multiples of 16 bytes).
+ * reports it (B200_EKERNEL).  out overlaps no operand.  Scratch comes from the context's workspace (40 MB and 40 bytes a row at most, and a copy
+ * of each operand whose pointer or strides are not multiples of 16 bytes).
  */
 int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, int64_t Hq, int64_t H, int64_t B, const b200_strided4* q,
                               const b200_strided4* k, const b200_strided4* v, const b200_strided4* out, int out_dtype, float scale,

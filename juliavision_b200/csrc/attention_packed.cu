@@ -4,11 +4,11 @@
 //
 // 4 E flops a row and visible key on tcgen05, and as many clocks of the exponential unit as of the products at E = 128, twice as many at 64.
 // What bounds it at E = 128 is the chain of a block of keys, which two tiles have between them to hide: 2900 clocks for two tiles and 128 keys, where
-// the products are 2048, of which a tile's softmax is 1300 for exponentials and sums, 240 to 430 for the maximum and 75 for the load of S, and its
-// product goes out only then; at E = 64 it is the exponentials.  Once the power limit holds, fewer clocks alone gain little (below, and at the
-// exponentials).  32 query heads on 8 key heads of 128, causal: 16384 rows 1995 us (1.10 PFLOP/s), 37 sequences of up to 2000 580 us (0.76; 507
-// before the limit holds); 20 heads of 64: 16 sequences of up to
-// 1500 161 us, 3 of 500 rows behind 30000 keys 264, one of 77 rows 7.3.
+// the products are 2048. A tile's softmax is 1300 for exponentials and sums, 240 to 430 for the maximum and 75 for the load of S, and its
+// product goes out only then; at E = 64 it is the exponentials (2600 clocks, 2048 of them the unit's).  From one part of the work to the next a
+// block takes 1500 to 2500 clocks more.  Once the power limit holds, fewer clocks alone gain little (below, and at the exponentials).  32 query
+// heads on 8 key heads of 128, causal: 16384 rows 2010 us (1.09 PFLOP/s), 37 sequences of up to 2000 580 us (0.76; 507 before the limit holds); 20
+// heads of 64: 16 sequences of up to 1500 164 us, 3 of 500 rows behind 30000 keys 266, one of 77 rows 7.3.
 //
 // The query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads (G T <= 128), so that keys and
 // values are read once for all of them and a tile's rows lie close together under the causal mask.  A block takes two tiles and walks their keys
