@@ -120,10 +120,10 @@ extern "C" {
 
 int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int64_t K, int64_t B, int32_t* table, int64_t table_ld,
                        const int32_t* own, int64_t own_ld, int64_t width, const int32_t* parents, const int32_t* lens) {
-    B200_REQUIRE(ctx && (caches || n == 0), B200_EINVAL, "cache_reorder: null argument");
-    B200_REQUIRE(n >= 0 && K >= 0 && B >= 0, B200_EINVAL, "cache_reorder: %lld caches, K=%lld B=%lld", (long long)n, (long long)K, (long long)B);
+    B200_REQUIRE(ctx && (caches || n <= 0), B200_EINVAL, "cache_reorder: null argument");
+    B200_REQUIRE(n >= 1 && K >= 0 && B >= 0, B200_EINVAL, "cache_reorder: %lld caches, K=%lld B=%lld", (long long)n, (long long)K, (long long)B);
     B200_REQUIRE(K <= CR_BEAMS && B < 65536, B200_DECLINE_EXTENT, "cache_reorder: %lld beams (at most %d), %lld searches", (long long)K, CR_BEAMS, (long long)B);
-    if (n == 0 || K == 0 || B == 0) return B200_OK;
+    if (K == 0 || B == 0) return B200_OK;
     B200_REQUIRE(table && own && parents && lens, B200_EINVAL, "cache_reorder: null array");
     B200_REQUIRE(own_ld >= width, B200_DECLINE_EXTENT, "cache_reorder: leading dimension %lld of %lld pages", (long long)own_ld, (long long)width);
     ReorderParams p = {};

@@ -81,6 +81,7 @@ def test_cachereorder_refusals():
         return cache(E=E, P=P, k=arr(np.int8, (E, 16, 2, P), ptr=(2 * at) << 20), v=arr(np.int8, (E, 16, 2, P), ptr=(2 * at + 1) << 20))
     c, t, parents, lens = made(1), arr(I32, (3, 4)), arr(I32, (2, 2)), arr(I32, (4,))
     refused(16, jv.cachereorder_, c, t, t, arr(I32, (4,)), lens)
+    refused(1, jv.cachereorder_, [], t, t, parents, lens)                  # without a cache nothing says how long a page is
     refused(16, jv.cachereorder_, c, t, t, arr(np.int64, (2, 2)), lens)
     refused(16, jv.cachereorder_, c, arr(I32, (3, 5)), t, parents, lens)
     refused(16, jv.cachereorder_, c, t, arr(F32, (3, 4)), parents, lens)

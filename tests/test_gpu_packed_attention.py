@@ -213,6 +213,20 @@ def test_more_sequences_than_a_block_lists_at_once(ctx, E):
     p.check(p.run(F32, True), F32, True)
 
 
+@pytest.mark.parametrize("N", [1, 3, 30000])
+def test_no_keys_at_all(ctx, N):
+    """Zeros for the rows that are a sequence's, whatever the queries hold."""
+    q = ctx.toback(np.full((N, 3, 64), np.nan, F16))
+    kv = jv.DeviceArray(ctx, q.ptr, F16, (64, 0, 1), owner=q)
+    out = ctx.allocate(F16, 64, 3, N)
+    ctx.fill_bytes(out, 0xFF)
+    ctx.ws.reset()
+    jv.packedsdpa_(ctx, out.permute((0, 2, 1)), q.permute((0, 2, 1)), kv, kv, ints(ctx, [0, N // 2, N - N // 3]), ints(ctx, [0, 0, 0]))
+    ctx.synchronize()
+    got = out.to_host()
+    assert not got[:N - N // 3].any() and np.isnan(got[N - N // 3:]).all()
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("way", ["heads", "odd", "backwards"])
 def test_where_results_go(ctx, dtype, way):
