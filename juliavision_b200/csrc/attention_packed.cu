@@ -430,6 +430,7 @@ template <int EP> struct PkCfg {
     // P beside S in tensor memory where there is room for it, so that the next scores come while P V reads; else over S.
     static constexpr bool OWN_P = EP == 64;
     static constexpr int STAGES = OWN_P ? 8 : 4;                 // K(0), V(0), K(1), ...
+    static_assert(STAGES % 2 == 0, "V has stages of its own, every fill of which warp 11 waits for");
     // Quarters of P that P V starts with, where P lies over S: three, 2922 clocks for two tiles and a block of keys; with two 3062.
     static constexpr int FIRST = 3;
     static constexpr int S_Q = 0, S_KV = 2 * SIDE, S_OUT = S_KV + STAGES * SIDE;   // operands; 128 bytes of a tile's rows on their way out, twice
@@ -789,9 +790,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
 #pragma unroll 1
                 for (int j = 0; ok && j < it.nblk; ++j, i += 2) {
                     const int st = (i + 1) % STAGES, key0 = (it.j0 + j) * PK_KEYS;
-                    // K too, which it does not need: loads land in any order, and a stage seen last two fills ago looks full
-                    ok = wait(&full[i % STAGES], (uint32_t)((i / STAGES) & 1), KST_WAIT_FULL) &&
-                         wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
+                    // Not K's, which is filled again without this warp's say; V's stage only once this block has been handed on
+                    ok = wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
                     if (!ok) break;
                     if (key0 + PK_KEYS - 1 > see) {       // some row does not see some key: 0 times what is not finite is no zero
                         // Keys from here on some row does not see.  A number times 0 is 0, anything else a NaN that stays one in a sum.
