@@ -324,7 +324,7 @@ int b200_beam_select(b200_ctx* ctx, int64_t V, int64_t K, int64_t B, int64_t N, 
  * page become the parent's, the others the beam's own; the tokens and maxima of the page that is not full are copied from the
  * parent's own page to the beam's.  lens (K,B): the beams of a search are equally long (the first one's counts; others are reported).
  * A parent outside [0,K) leaves the beam where it was, a page outside the cache is not touched; the next b200_sync reports either.
- * No array of keys or values is given twice. */
+ * No array of keys or values is given twice; table and own share no memory. */
 int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int64_t K, int64_t B, int32_t* table, int64_t table_ld,
                        const int32_t* own, int64_t own_ld, int64_t width, const int32_t* parents, const int32_t* lens);
 

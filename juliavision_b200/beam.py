@@ -54,7 +54,7 @@ def cachereorder_(ctx: Ctx, caches: Union[Cache8, Sequence[Cache8]], table: Devi
                   lens: DeviceArray) -> DeviceArray:
     """Beam k of search b goes on from the tokens of beam parents[k, b] (parents (K, B) int32, as `beamselect_` gives them).  `caches`: one
     a layer, of the same sizes and strides, which share `table` (pages a sequence, K * B), sequence k + K b being beam k of search b.
-    own (pages a sequence, K * B) names the pages that each beam writes, no page twice; a table starts as a copy of it.  Whole pages change
+    own (pages a sequence, K * B) names the pages that each beam writes, no page twice; a table starts as a copy of it and shares no memory with it.  Whole pages change
     hands in `table`; the page that is not full is copied to the beam's own, and entries behind it become the beam's own again.  lens (K * B): a
     search's beams are equally long.  No array is given twice.  A prompt is handed to all beams by parents of 0 after it has been written as beam 0's."""
     rc = _lib.host().cachereorder(ctx.handle, caches, table, own, parents, lens)

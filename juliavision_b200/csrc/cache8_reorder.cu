@@ -112,6 +112,17 @@ cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
     }
 }
 
+// Whether two arrays of `columns` columns of `width` numbers have one in common.  With leading dimensions that differ, whether they lie in one another.
+static bool cr_meet(const int32_t* a, int64_t a_ld, const int32_t* b, int64_t b_ld, int64_t columns, int64_t width) {
+    const int64_t size = sizeof(int32_t), d = (int64_t)((uintptr_t)b - (uintptr_t)a), w = width * size;
+    const int64_t a_span = (columns - 1) * a_ld * size + w, b_span = (columns - 1) * b_ld * size + w;
+    if (d >= a_span || -d >= b_span) return false;
+    if (columns == 1 || a_ld != b_ld) return true;
+    const int64_t ld = a_ld * size, into = (d % ld + ld) % ld, apart = (d - into) / ld;       // b begins `into` bytes behind the start of a's column `apart`
+    const auto inside = [&](int64_t c) { return c < columns && -c < columns; };
+    return (into < w && inside(apart)) || (ld - into < w && inside(apart + 1));
+}
+
 } // namespace b200
 
 using namespace b200;
@@ -141,6 +152,8 @@ int b200_cache_reorder(b200_ctx* ctx, const b200_cache8* caches, int64_t n, int6
         for (int64_t j = 0; j < i; ++j) twice |= caches[j].k == c.k || caches[j].v == c.v || caches[j].k == c.v || caches[j].v == c.k;
         B200_REQUIRE(!twice, B200_EINVAL, "cache_reorder: the array of cache %lld is given twice", (long long)i);
     }
+    // A table over `own` would overwrite with the parents' pages what says which pages a beam writes; two beams could then write one.
+    B200_REQUIRE(!cr_meet(table, table_ld, own, own_ld, K * B, width), B200_EINVAL, "cache_reorder: table and own share memory");
     p.by_vectors = Divisor::of(p.c.E / 16);
     B200_CUDA(cudaSetDevice(ctx->device));
     p.table = table, p.table_ld = table_ld, p.own = own, p.own_ld = own_ld;
