@@ -238,7 +238,8 @@ int b200_attention_f16_route(int64_t E, int64_t Lq, int64_t Lk, int64_t H, int64
  * query head i reads key head i / (Hq / H).  A sequence's last row stands at its last key: row i of n rows and m keys sees, when
  * causal, the keys up to i + m - n, else all m.  A row that sees none comes out as zeros; rows that belong to no sequence are left as they
  * were.  A key that a row does not see has no part in it, whatever it holds.  q, k and v fp16, out fp16 or fp32; scale is 0 or more.
- * Scores, softmax and sums are fp32; the weights of the second product are rounded to fp16, up to 2^8 of the heaviest when it came and times 2^7.
+ * Scores, softmax and sums are fp32.  The weights of the second product, up to 2^8 of the heaviest when it came and times 2^7, are rounded to fp16 for
+ * fp16 results and go in as two fp16 numbers each for fp32 results, which takes up to half as long again.
  * starts and kstarts are device arrays of B + 1 numbers; where they are not in order or past the arrays they are cut, and the next b200_sync
  * reports it (B200_EKERNEL).  out overlaps no operand.  Scratch comes from the context's workspace (40 MB and 40 bytes a row at most, and a copy
  * of each operand whose pointer or strides are not multiples of 16 bytes).

@@ -109,7 +109,8 @@ def packedsdpa_(ctx: Ctx, out: DeviceArray, q: DeviceArray, k: DeviceArray, v: D
     query head i reads key head i // (Hq // H).  Sequence b is rows starts[b] .. starts[b + 1] - 1 of q and kstarts[b] .. kstarts[b + 1] - 1
     (those of `starts` without it) of k and v; both are int32 on the device, one number more than sequences.  Its last row stands at its last
     key: row i of n sees, when causal, the keys up to i + keys - n, else all of its sequence's.  A row that sees none comes out as zeros;
-    rows of `out` that belong to no sequence are left as they were.  `out` does not overlap q, k or v."""
+    rows of `out` that belong to no sequence are left as they were.  `out` does not overlap q, k or v.  The softmax's weights are rounded to fp16
+    for fp16 results; for fp32 results they keep 22 bits, which takes up to half as long again."""
     if scale is None and q.ndim == 3 and q.shape[0] > 0:
         scale = 1.0 / sqrt(q.shape[0])
     rc = _lib.host().packedsdpa(ctx.handle, out, q, k, v, starts, kstarts, scale, causal)

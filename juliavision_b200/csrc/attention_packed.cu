@@ -424,12 +424,13 @@ __device__ __forceinline__ bool pk_direct(const PackedParams& p, int unit, Packe
     return false;
 }
 
-template <int EP> struct PkCfg {
+template <int EP, bool TWO> struct PkCfg {                       // TWO: fp32 results, weights as two fp16 numbers
     static constexpr int ATOMS = EP / 64;
     static constexpr int SIDE = ATOMS * PK_ATOM;                 // an operand tile
-    // P beside S in tensor memory where there is room for it, so that the next scores come while P V reads; else over S.
-    static constexpr bool OWN_P = EP == 64;
-    static constexpr int STAGES = OWN_P ? 8 : 4;                 // K(0), V(0), K(1), ...
+    // P beside S in tensor memory where there is room for it, so that the next scores come while P V reads; else over S, whose 128 columns two
+    // halves of P fill.
+    static constexpr bool SMALL = EP == 64, OWN_P = SMALL && !TWO;
+    static constexpr int STAGES = SMALL ? 8 : 4;                 // K(0), V(0), K(1), ...
     static_assert(STAGES % 2 == 0, "V has stages of its own, every fill of which warp 11 waits for");
     // Quarters of P that P V starts with, where P lies over S: three, 2922 clocks for two tiles and a block of keys; with two 3062.
     static constexpr int FIRST = 3;
@@ -466,11 +467,11 @@ __device__ __forceinline__ void pk_store8(const PackedParams& p, int64_t at, int
         }
 }
 
-template <int EP>
+template <int EP, bool TWO>
 __global__ void __launch_bounds__(PK_THREADS, 1)
 attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_constant__ CUtensorMap tmapK,
                         const __grid_constant__ CUtensorMap tmapV, const __grid_constant__ CUtensorMap tmapO, const PackedParams p) {
-    using Cfg = PkCfg<EP>;
+    using Cfg = PkCfg<EP, TWO>;
     constexpr int STAGES = Cfg::STAGES, ATOMS = Cfg::ATOMS;
     constexpr bool OWN_P = Cfg::OWN_P, HALVES = !OWN_P;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -565,6 +566,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
     };
     // The last key that every row of both tiles sees; blocks that end behind it are masked.
     auto all_see = [&](int token) { return p.causal && it.m - it.n + token < it.m - 1 ? it.m - it.n + token : it.m - 1; };
+    // The last key whose value is multiplied whatever it holds.  A weight's lower half may be 0 or below, which makes a NaN of an infinity: none then.
+    auto as_it_is = [&]() { return TWO ? -1 : all_see(it.token); };
 
     float2* stats = reinterpret_cast<float2*>(smem + Cfg::S_STAT);
     // A row of a tile: its token in the tile, its head.  Which rows are any sequence's, and the last key that each sees.
@@ -580,8 +583,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
         const uint32_t out = smem_u32(smem + Cfg::S_OUT), swz = (uint32_t)(row & 7) << 4;
         // They leave together, wherever a wait runs out: one alone would leave the others at their barrier for good.
         // what the loops ask for each time round, out of the constant bank
-        int E = p.E, log = p.out_f32 ? 2 : 1;
-        for (int* v : {&E, &log}) asm volatile("" : "+r"(*v));
+        int E = p.E;
+        asm volatile("" : "+r"(E));
         bool ok = true;
 #pragma unroll 1
         for (;;) {
@@ -609,7 +612,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 const float2 stat = stats[t * PK_ROWS + row];
                 const float f = it.slot >= 0 || stat.y == 0.f ? 1.f : 1.f / stat.y;
                 const int bad = *reinterpret_cast<volatile int*>(&odd[s]);      // written before the last P V was issued
-                if (whole && log == 1 && slot < 0 && nblk > 0 && bad == 0x7fffffff) {        // the ordinary case, without a branch to wait for
+                if (!TWO && whole && slot < 0 && nblk > 0 && bad == 0x7fffffff) {        // the ordinary case, without a branch to wait for
                     if (threadIdx.x == 12 * 32) tma_store_wait_read<0>();                    // what went out before has been read
                     named_bar_sync(BAR, 128);
 #pragma unroll
@@ -660,7 +663,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     if (bad != 0x7fffffff) {        // what was taken out, for those who see it
                         const int end = live ? min((it.j0 + it.nblk) * PK_KEYS - 1, last_key(t, l0)) : -1;
 #pragma unroll 1
-                        for (int key = max(bad * PK_KEYS, all_see(it.token) + 1); key <= end; ++key) {
+                        for (int key = max(bad * PK_KEYS, as_it_is() + 1); key <= end; ++key) {
                             const __half* q = p.v + (int64_t)(it.k0 + key) * p.vN + it.h * p.vH + e;
 #pragma unroll
                             for (int u = 0; u < 32; ++u) {
@@ -685,9 +688,9 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     }
                     // a row a lane
                     if (!live) continue;
-                    char* to = (char*)p.out + (at + e << log);
+                    char* to = (char*)p.out + (at + e) * (TWO ? 4 : 2);
                     const bool vectors = p.out_whole && e + 32 <= E;
-                    if (log == 2) {
+                    if (TWO) {
 #pragma unroll
                         for (int c = 0; c < 8; ++c)
                             if (vectors || (p.out_whole && e + 4 * c + 4 <= E)) reinterpret_cast<uint4*>(to)[c] = make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
@@ -785,7 +788,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
             bool ok = true;
 #pragma unroll 1
             for (int s; ok && (s = take()) >= 0; done_with(s)) {
-                const int see = all_see(it.token);
+                const int see = as_it_is();
                 int first = 0x7fffffff;
 #pragma unroll 1
                 for (int j = 0; ok && j < it.nblk; ++j, i += 2) {
@@ -793,8 +796,8 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     // Not K's, which is filled again without this warp's say; V's stage only once this block has been handed on
                     ok = wait(&full[st], (uint32_t)(((i + 1) / STAGES) & 1), KST_WAIT_FULL);
                     if (!ok) break;
-                    if (key0 + PK_KEYS - 1 > see) {       // some row does not see some key: 0 times what is not finite is no zero
-                        // Keys from here on some row does not see.  A number times 0 is 0, anything else a NaN that stays one in a sum.
+                    if (key0 + PK_KEYS - 1 > see) {       // some row's weight may be 0, of which what is not finite makes a NaN
+                        // Keys from here on.  A number times 0 is 0, anything else a NaN that stays one in a sum.
                         const int from = see < key0 ? 0 : see + 1 - key0;
                         uint8_t* tile = smem + Cfg::S_KV + st * Cfg::SIDE;
                         const __half2 zero = __half2half2(__ushort_as_half(0));
@@ -871,7 +874,10 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
             auto issue_pv = [&](int j, int st, int k0, int k1) {
                 const uint32_t v_addr = kv_addr + st * Cfg::SIDE;
 #pragma unroll
-                for (int k = k0; k < k1; ++k) umma_ts(o_tmem, p_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
+                for (int k = k0; k < k1; ++k) {
+                    umma_ts(o_tmem, p_tmem + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, (j | k) != 0);
+                    if (TWO) umma_ts(o_tmem, p_tmem + 64 + k * 8, smem_desc_at(vdesc0, v_addr + k * 2048), idesc_o, true);
+                }
             };
             bool ok = true;
 #pragma unroll 1
@@ -981,8 +987,11 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     return fmaxf(fmaxf(a, b), fmaxf(c, d)) * p.scale_log2;
                 };
                 // Any reference point m gives the same quotient; it follows the maximum lazily, only when that has grown by more than 2^8.
-                // P goes in times 2^7, so that fp16 holds weights down to 2^-31 of the heaviest key's.  Each weight is rounded once to fp16, half a
-                // step 2^-11 of itself, as the product's operand; the sum that divides takes them as they were, in fp32.
+                // P goes in times 2^7, so that fp16 holds weights down to 2^-31 of the heaviest key's.  Where the result is rounded to fp16 anyhow, each
+                // weight is rounded once to fp16, half a step 2^-11 of itself, as the product's operand; where the caller asks for fp32 it goes in as
+                // two fp16 numbers, off by 2^-22, in twice the products (error against 64 bits 1.7e-4 -> 9e-6 and 2090 us -> 3130 for 16384 rows, 1.6e-4 ->
+                // 1e-6 and 775 -> 925 for 37 sequences of up to 2000, 2e-4 -> 3e-6 and 173 -> 240 for 16 of up to 1500).  The sum that divides takes
+                // the weights as they were, in fp32.
                 const float top = highest();
                 const float m_new = top > m_run + 8.f ? top : m_run;
                 if (OWN_P && busy > 0) ok = wait(&pv_done[t], (uint32_t)((busy - 1) & 1), KST_WAIT_SOFTMAX);     // P and O are free
@@ -1026,8 +1035,18 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                         else sum0 = add2(sum0, pack2(e0, e1));
                         const __half2 h = __floats2half2_rn(e0, e1);
                         pk[u] = *reinterpret_cast<const uint32_t*>(&h);
+                        if (TWO) x[i][2 * u] = __float_as_uint(e0), x[i][2 * u + 1] = __float_as_uint(e1);
                     }
                     pk_tmem_st16(p_tmem + i * 16, pk);
+                    if (TWO) {
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pk[u]));
+                            const __half2 h = __floats2half2_rn(__uint_as_float(x[i][2 * u]) - f.x, __uint_as_float(x[i][2 * u + 1]) - f.y);
+                            pk[u] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        pk_tmem_st16(p_tmem + 64 + i * 16, pk);
+                    }
                     if (HALVES && i == Cfg::FIRST - 1) {
                         tmem_wait_st();
                         tc_fence_before();
@@ -1126,10 +1145,10 @@ struct PackedOperand {
     int64_t sN, sH;
 };
 
-template <int EP>
+template <int EP, bool TWO>
 static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, const PackedOperand& k, const PackedOperand& v, int64_t items, int64_t entries) {
-    using Cfg = PkCfg<EP>;
-    auto kern = attention_packed_kernel<EP>;
+    using Cfg = PkCfg<EP, TWO>;
+    auto kern = attention_packed_kernel<EP, TWO>;
     static std::atomic<uint64_t> asked{0};
     B200_CUDA(allow_smem(ctx, kern, Cfg::SMEM, asked));
     CUtensorMap tq, tk, tv, to;
@@ -1259,7 +1278,9 @@ int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, i
         op[i] = {(const __half*)ws, heads * E8, E8};
     }
     p.v = op[2].ptr, p.vN = op[2].sN, p.vH = op[2].sH;
-    return E <= 64 ? pk_launch<64>(ctx, p, op[0], op[1], op[2], items, entries) : pk_launch<128>(ctx, p, op[0], op[1], op[2], items, entries);
+    auto launch = [&](auto run) { return run(ctx, p, op[0], op[1], op[2], items, entries); };
+    if (p.out_f32) return E <= 64 ? launch(pk_launch<64, true>) : launch(pk_launch<128, true>);
+    return E <= 64 ? launch(pk_launch<64, false>) : launch(pk_launch<128, false>);
 }
 
 } // extern "C"
