@@ -10,9 +10,10 @@
 // heads on 8 key heads of 128, causal: 16384 rows 2010 us (1.09 PFLOP/s), 37 sequences of up to 2000 580 us (0.76; 507 before the limit holds); 20
 // heads of 64: 16 sequences of up to 1500 164 us, 3 of 500 rows behind 30000 keys 266, one of 77 rows 7.3.
 //
-// The query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads (G T <= 128), so that keys and
-// values are read once for all of them and a tile's rows lie close together under the causal mask.  A block takes two tiles and walks their keys
-// in blocks of 128: S = Q K' and O += P V with S, P (fp16) and O in tensor memory, Q, K and V by TMA through the caller's strides.
+// Query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads, G being the largest power of two up to 128
+// that divides the number that share, so that keys and values are read once for G heads and a tile's rows lie close together under the causal
+// mask; of 3, 5 or 7 heads each reads them for itself.  A block takes two tiles and walks their keys in blocks of 128: S = Q K' and O += P V with
+// S, P (fp16) and O in tensor memory, Q, K and V by TMA through the caller's strides.
 //
 //   warps 0-3  softmax of tile 0, warps 4-7 of tile 1: one thread a row, its 128 scores in registers
 //   warp 8     finds the block's next part of the work (below), tells the others, and asks for Q, K and V
@@ -67,8 +68,8 @@ struct PackedParams {
     int64_t oN, oH;
     const int32_t *starts, *kstarts;
     int N, Nk, B, H, Hq, E;
-    int G, T, groups, share;           // heads and tokens of a tile; tiles' worth of heads of a key head; heads that share a key head
-    Divisor by_g;
+    int G, T, groups, share;           // heads and tokens of a tile, G T = 128; tiles' worth of heads of a key head; heads that share a key head
+    int log_g;
     int causal, out_f32, out_whole;
     float scale_log2;
     int heads;                         // H * groups: units of a row pair
@@ -571,13 +572,13 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
 
     float2* stats = reinterpret_cast<float2*>(smem + Cfg::S_STAT);
     // A row of a tile: its token in the tile, its head.  Which rows are any sequence's, and the last key that each sees.
-    auto live_row = [&](int t, int l0, int g) { return l0 < p.T && it.token + t * p.T + l0 < it.n && it.g0 + g < p.share; };
+    auto live_row = [&](int t, int l0) { return l0 < it.n - it.token - t * p.T; };
     auto last_key = [&](int t, int l0) { return p.causal ? min(it.m - it.n + it.token + t * p.T + l0, it.m - 1) : it.m - 1; };
 
     if (warp >= 12) {
         // ------------------------------------------------------ results
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PK_OUT_REGS));
-        const int quad = warp & 3, row = quad * 32 + lane, l0 = p.by_g.div(row), g = row - l0 * p.G;
+        const int quad = warp & 3, row = quad * 32 + lane, l0 = row >> p.log_g, g = row & (p.G - 1);
         int busy0 = 0, busy1 = 0, parts0 = 0, parts1 = 0;        // blocks and parts of a tile before this one
         constexpr int BAR = 1;                  // the four warps' own barrier
         const uint32_t out = smem_u32(smem + Cfg::S_OUT), swz = (uint32_t)(row & 7) << 4;
@@ -594,11 +595,11 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
             for (int t = 0; t < 2; ++t) {
                 if (it.token + t * p.T >= it.n) continue;
                 const uint32_t o_tmem = tmem_base + (uint32_t(quad * 32) << 16) + Cfg::O_COL + t * EP;
-                const bool live = live_row(t, l0, g);
+                const bool live = live_row(t, l0);
                 const int row0 = it.q0 + it.token + t * p.T, head0 = it.h * p.share + it.g0;
                 // Whole tiles of fp16 go out through shared memory and a tensor map, others a row a lane.  A store for every 16 bytes of all tiles cost the
                 // SM 6000 clocks an item in instructions and waits for them, two blocks of keys; a bulk copy for every row more.
-                const bool whole = p.out_whole && it.token + (t + 1) * p.T <= it.n && it.g0 + p.G <= p.share;
+                const bool whole = p.out_whole && it.token + (t + 1) * p.T <= it.n;
                 const int64_t at = (int64_t)(row0 + l0) * p.oN + (int64_t)(head0 + g) * p.oH;
                 const int turn = t ? parts1++ : parts0++, blocks = t ? (busy1 += it.nblk) : (busy0 += it.nblk);
                 ok = wait(&o_full[t], (uint32_t)(turn & 1), KST_WAIT_SOFTMAX);
@@ -751,7 +752,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                     ok = ok && wait(&q_empty[t], (uint32_t)(tiles & 1) ^ 1, KST_WAIT_EMPTY);
                     ++tiles;
                     if (ok && elect_one()) {
-                        mbar_arrive_expect_tx(&q_full[t], ATOMS * 128 * p.G * p.T);
+                        mbar_arrive_expect_tx(&q_full[t], Cfg::SIDE);
 #pragma unroll
                         for (int a = 0; a < ATOMS; ++a)
                             tma_load_3d(smem + Cfg::S_Q + t * Cfg::SIDE + a * PK_ATOM, &tmapQ, &q_full[t], a * 64, it.h * p.share + it.g0,
@@ -933,7 +934,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
         const uint32_t lane_base = uint32_t(quad * 32) << 16;
         const uint32_t s_tmem = tmem_base + lane_base + t * PK_KEYS, o_tmem = tmem_base + lane_base + Cfg::O_COL + t * EP;
         const uint32_t p_tmem = OWN_P ? tmem_base + lane_base + Cfg::P_COL + t * 64 : s_tmem;
-        const int l0 = p.by_g.div(row);       // the row's token in its tile
+        const int l0 = row >> p.log_g;        // the row's token in its tile
         int busy = 0, turns = 0, lives = 0;          // blocks of this tile, turns of both, parts of this tile before this one
         bool ok = true;
 #pragma unroll 1
@@ -1098,8 +1099,8 @@ packed_join_kernel(const PackedParams p) {
     const PackedCut x = p.cut[i];                 // there is room for as many as there are blocks of this launch
     if (i >= counts.z || e >= p.E) return;
     const int h = x.head / p.groups, g0 = (x.head - h * p.groups) * p.G;
-    const int t = prow / PK_ROWS, row = prow - t * PK_ROWS, l0 = p.by_g.div(row), g = row - l0 * p.G, l = x.token + t * p.T + l0;
-    if (l0 >= p.T || l >= x.n || g0 + g >= p.share) return;
+    const int t = prow / PK_ROWS, row = prow - t * PK_ROWS, l0 = row >> p.log_g, g = row & (p.G - 1), l = x.token + t * p.T + l0;
+    if (l >= x.n) return;
     auto slot = [&](int w) -> int64_t { return w == 0 ? x.slot : 2 * (x.slot / 2 + w); };
     auto stat = [&](int w) { return *reinterpret_cast<const float2*>(p.part_ml + (slot(w) * 2 * PK_ROWS + prow) * 2); };
     float M = -INFINITY, sum = 0.f, v[2][8] = {};
@@ -1139,6 +1140,16 @@ packed_rows_kernel(const __half* x, int64_t xN, int64_t xH, __half* to, int E, i
     for (int k = 0; k < 8; ++k) v[k] = c * 8 + k < E ? q[k] : __half(0.f);
     *reinterpret_cast<uint4*>(to + row * E8 + c * 8) = *reinterpret_cast<const uint4*>(v);
 }
+
+// Heads of a tile: the largest power of two that divides those of a key head, so that every row of a tile is some token's and head's, and every tile of a
+// key head has as many.  Of 3, 5 or 7 heads each is then a unit of its own and reads the keys again.
+constexpr int pk_heads(int share) {
+    int g = 1;
+    while (g < PK_ROWS && share % (2 * g) == 0) g *= 2;
+    return g;
+}
+static_assert(pk_heads(1) == 1 && pk_heads(5) == 1 && pk_heads(6) == 2 && pk_heads(12) == 4 && pk_heads(130) == 2 && pk_heads(384) == 128 && pk_heads(512) == 128,
+              "what stands above");
 
 struct PackedOperand {
     const __half* ptr;
@@ -1241,16 +1252,11 @@ int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, i
     p.out_whole = ((uintptr_t)p.out | (uint64_t)(p.oN * size) | (uint64_t)(p.oH * size)) % 16 == 0 && p.oN > 0 && p.oH > 0;
     p.scale_log2 = fmaxf((float)((double)scale * 1.4426950408889634), 0x1p-100f);   // above 0, so that a hidden score of -inf stays that
     p.d_status = ctx->d_status;
-    // Heads of a tile: as many rows used as can be of 128 times those of all of a key head's tiles; of equals, the most heads.
     p.share = (int)(Hq / H);
-    double best = 0;
-    for (int g = 1; g <= p.share && g <= PK_ROWS; ++g) {
-        const double used = (double)(PK_ROWS / g * g) * p.share / (double)(cdiv(p.share, g) * g);
-        if (used >= best) best = used, p.G = g;
-    }
+    p.G = pk_heads(p.share);
+    for (p.log_g = 0; 1 << p.log_g < p.G;) ++p.log_g;
     p.T = PK_ROWS / p.G;
-    p.groups = (int)cdiv(p.share, p.G);
-    p.by_g = Divisor::of(p.G);
+    p.groups = p.share / p.G;
     p.heads = (int)(p.H * p.groups);
     const int64_t entries = N / (2 * p.T) + (B < N ? B : N), items = entries * p.heads;    // at most
     B200_REQUIRE(items < (1ll << 30), B200_DECLINE_EXTENT, "attention_packed: %lld row tiles", (long long)items);
