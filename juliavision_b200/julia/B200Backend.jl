@@ -299,9 +299,23 @@ function rotary!(ctx::Ctx{B200Backend}, plan::RotaryPlan, out, x; lens, news = n
     out
 end
 
+# The library sees pointers and the sizes it is told: what they are taken from is compared first.
+demand(ok, what) = ok || throw(DimensionMismatch(what))
+dense(a) = strides(a) == Base.size_to_strides(1, size(a)...)
+isdense(a, T, dims...) = eltype(a) === T && size(a) == dims && dense(a)
+iscounts(a, n) = a === nothing || (eltype(a) === Int32 && length(a) == n && dense(a))
+along(a) = size(a, 1) <= 1 || stride(a, 1) == 1
+
 # weight (E,), (E, H), or with split (E, 2): heads up to `split` take its first column.
 function normrotary!(ctx::Ctx{B200Backend}, plan::RotaryPlan, out, x, weight = nothing; eps = 1f-6, split = nothing, lens, news = nothing)
+    demand(ndims(x) == 4 && eltype(x) === eltype(out) === Float16 && size(out) == size(x), "normrotary!: x and out are (E, L, H, B) of Float16")
     E, L, H, B = size(x)
+    demand(lens !== nothing && iscounts(lens, B) && iscounts(news, B), "normrotary!: lens and news are one Int32 a sequence")
+    demand(2 * length(plan.freq) >= plan.rot, "normrotary!: the plan has a frequency for each pair")
+    demand(split === nothing || (weight !== nothing && 0 <= split <= H), "normrotary!: split between the heads of a weight")
+    demand(weight === nothing || (eltype(weight) in (Float16, Float32) && ndims(weight) in (1, 2) && size(weight, 1) == E && along(weight) &&
+                                  (split === nothing ? size(weight, 2) in (1, H) : size(weight, 2) == 2)),
+           "normrotary!: weight is (E,), (E, H), or with split (E, 2)")
     check(ccall((:b200_norm_rotary_f16, LIB), Cint,
                 (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Ptr{Cvoid}, Cint, Int64, Int64, Cfloat,
                  Ptr{Cvoid}, Int64, Cint, Cfloat, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}),
@@ -362,6 +376,11 @@ end
 s3(a) = (r = rootstrides(a); Strided4(Ptr{Cvoid}(r[1]), (Int64.(r[2])[1:3]..., Int64(0))))       # three axes
 # Sequences side by side: q, out (E, N, Hq), k, v (E, Nk, H), starts and kstarts one Int32 more than sequences.
 function packedsdpa!(ctx::Ctx{B200Backend}, out, q, k, v, starts; kstarts = starts, scale = 1 / sqrt(size(q, 1)), causal = true)
+    demand(ndims(q) == ndims(k) == 3 && size(out) == size(q) && size(v) == size(k) && size(k, 1) == size(q, 1), "packedsdpa!: q and out are (E, N, Hq), k and v (E, Nk, H)")
+    demand(eltype(q) === eltype(k) === eltype(v) === Float16 && eltype(out) in (Float16, Float32), "packedsdpa!: q, k and v are Float16")
+    demand(length(starts) >= 1 && iscounts(starts, length(starts)) && kstarts !== nothing && iscounts(kstarts, length(starts)),
+           "packedsdpa!: starts and kstarts are one Int32 more than sequences")
+    demand(kstarts !== starts || size(k, 2) >= size(q, 2), "packedsdpa!: as many keys as rows where they lie at the same places")
     check(ccall((:b200_attention_packed_f16, LIB), Cint,
                 (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Int64, Int64, Ref{Strided4}, Ref{Strided4}, Ref{Strided4}, Ref{Strided4}, Cint, Cfloat, Cint,
                  Ptr{Cvoid}, Ptr{Cvoid}),
@@ -372,7 +391,11 @@ end
 
 # The N best of K * V continuations: best, parents, tokens (N, B); logits (V, K, B), scores (K, B).
 function beamselect!(ctx::Ctx{B200Backend}, best, parents, tokens, logits, scores; ended = nothing, pad = 0)
+    demand(ndims(logits) == 3 && eltype(logits) in (Float16, Float32) && along(logits), "beamselect!: logits are (V, K, B) of Float16 or Float32")
     V, K, B = size(logits)
+    demand(isdense(scores, Float32, K, B) && (ended === nothing || isdense(ended, Int32, K, B)), "beamselect!: scores and ended are dense (K, B)")
+    demand(isdense(best, Float32, size(best, 1), B) && isdense(parents, Int32, size(best)...) && isdense(tokens, Int32, size(best)...),
+           "beamselect!: best, parents and tokens are dense (N, B)")
     check(ccall((:b200_beam_select, LIB), Cint,
                 (Ptr{Cvoid}, Int64, Int64, Int64, Int64, Ptr{Cvoid}, Cint, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Ptr{Cvoid}, Ptr{Cvoid}),
                 ctx.backend.handle, V, K, B, size(best, 1), pointer(logits), dtcode(eltype(logits)), stride(logits, 2), stride(logits, 3),
@@ -382,6 +405,11 @@ end
 
 # Beam k of search b goes on from beam parents[k, b] (counted from 0) in all of `caches`; table, own (pages a sequence, K * B).
 function cachereorder!(ctx::Ctx{B200Backend}, caches::AbstractVector, table, own, parents, lens)
+    demand(ndims(parents) == 2 && isdense(parents, Int32, size(parents)...), "cachereorder!: parents are a dense (K, B) of Int32")
+    demand(ndims(table) == 2 && eltype(table) === eltype(own) === Int32 && size(own) == size(table) && size(table, 2) == length(parents) && along(table) && along(own),
+           "cachereorder!: table and own are (pages, K * B) of Int32")
+    demand(lens !== nothing && iscounts(lens, length(parents)), "cachereorder!: lens is one Int32 a beam")
+    demand(all(x -> size(x.v) == size(x.k) && size(x.kmax) == size(x.vmax) == size(x.k)[3:4], caches), "cachereorder!: caches are (E, T, H, P), their maxima (H, P)")
     c = Cache8C[cachec(x, table) for x in caches]
     check(ccall((:b200_cache_reorder, LIB), Cint,
                 (Ptr{Cvoid}, Ptr{Cache8C}, Int64, Int64, Int64, Ptr{Cvoid}, Int64, Ptr{Cvoid}, Int64, Int64, Ptr{Cvoid}, Ptr{Cvoid}),
