@@ -241,8 +241,8 @@ int b200_attention_f16_route(int64_t E, int64_t Lq, int64_t Lk, int64_t H, int64
  * Scores, softmax and sums are fp32.  The weights of the second product, up to 2^8 of the heaviest when it came and times 2^7, are rounded to fp16 for
  * fp16 results and go in as two fp16 numbers each for fp32 results, which takes up to half as long again.
  * starts and kstarts are device arrays of B + 1 numbers; where they are not in order or past the arrays they are cut, and the next b200_sync
- * reports it (B200_EKERNEL).  out overlaps no operand.  Scratch comes from the context's workspace (40 MB and 40 bytes a row at most, and a copy
- * of each operand whose pointer or strides are not multiples of 16 bytes).
+ * reports it (B200_EKERNEL).  out overlaps no operand.  Scratch comes from the context's workspace (40 MB, 54 bytes a row and 4 bytes a sequence
+ * at most, and a copy of each operand whose pointer or strides are not multiples of 16 bytes).
  */
 int b200_attention_packed_f16(b200_ctx* ctx, int64_t E, int64_t N, int64_t Nk, int64_t Hq, int64_t H, int64_t B, const b200_strided4* q,
                               const b200_strided4* k, const b200_strided4* v, const b200_strided4* out, int out_dtype, float scale,

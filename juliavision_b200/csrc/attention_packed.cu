@@ -1188,7 +1188,9 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
     const int64_t slots = 2 * sms, rows = slots * 2 * PK_ROWS;
     if (p.planned) {
         void* ws = nullptr;
-        const size_t list = (size_t)entries * (sizeof(PackedEntry) + sizeof(int)) + p.B * sizeof(int) + sms * sizeof(PackedCut) + 2 * sizeof(int4) + 16 * 8;
+        // 36 bytes an entry, of which there are one and a half a row at most (a token a tile, a row a sequence)
+        const int64_t firsts = p.B > PL_SEQS ? p.B : 0;
+        const size_t list = (size_t)entries * (sizeof(PackedEntry) + sizeof(int)) + firsts * sizeof(int) + sms * sizeof(PackedCut) + 2 * sizeof(int4) + 16 * 8;
         rc = ws_scratch(ctx, rows * (EP + 2) * sizeof(float) + list, &ws);
         if (rc) return rc;
         uint8_t* at = static_cast<uint8_t*>(ws);
@@ -1203,7 +1205,7 @@ static int pk_launch(b200_ctx* ctx, PackedParams& p, const PackedOperand& q, con
         p.cut = (PackedCut*)room(sms * sizeof(PackedCut));
         p.counts = (int4*)room(2 * sizeof(int4));
         p.before = (int*)room(entries * sizeof(int));
-        p.first = (int*)room(p.B * sizeof(int));
+        p.first = (int*)room(firsts * sizeof(int));
         B200_CUDA(launch_dep(packed_plan_kernel, dim3(1), dim3(PL_THREADS), 0, ctx->stream, 1, p));
         ctx->launches++;
     }
