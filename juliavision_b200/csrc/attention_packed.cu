@@ -7,8 +7,8 @@
 // the products are 2048. A tile's softmax is 1300 for exponentials and sums, 240 to 430 for the maximum and 75 for the load of S, and its
 // product goes out only then; at E = 64 it is the exponentials (2600 clocks, 2048 of them the unit's).  From one part of the work to the next a
 // block takes 1500 to 2500 clocks more.  Once the power limit holds, fewer clocks alone gain little (below, and at the exponentials).  32 query
-// heads on 8 key heads of 128, causal: 16384 rows 2010 us (1.09 PFLOP/s), 37 sequences of up to 2000 580 us (0.76; 507 before the limit holds); 20
-// heads of 64: 16 sequences of up to 1500 164 us, 3 of 500 rows behind 30000 keys 266, one of 77 rows 7.3.
+// heads on 8 key heads of 128, causal: 16384 rows 1980 us (1.11 PFLOP/s), 37 sequences of up to 2000 570 us (0.77); 20 heads
+// of 64: 16 sequences of up to 1500 162 us, one of 77 rows 7.2; 20 of 80 on 4, 3 sequences of 500 rows behind 30000 keys: 262.
 //
 // Query heads that share a key head are stacked with the tokens: a tile's 128 rows are T tokens of G heads, G being the largest power of two up to 128
 // that divides the number that share, so that keys and values are read once for G heads and a tile's rows lie close together under the causal
@@ -763,7 +763,7 @@ attention_packed_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_
                 load_q(0, tiles0);
 #pragma unroll 1
                 for (int j = 0; ok && (j < sides || j == 0); ++j) {
-                    // What comes next is looked up once this part's first sides are asked for, and they are brought nearer.
+                    // What comes next is looked up once this part's first sides are asked for.
                     if (p.planned && j == (sides > STAGES ? STAGES : sides >> 1)) {
                         unit = __shfl_sync(0xffffffffu, unit, 0);
                         some = pk_listed(p, unit, u);

@@ -5,11 +5,12 @@
 //
 // Bandwidth-bound: the tokens of a part-filled page, read and written, for every beam whose parent is another.  A thread takes the same 16
 // bytes of all of a search's beams and reads them all before it writes any, so the beams may change places in any way without a second copy.
-// 16 searches of 4 beams in 16 caches of 8 heads of 128, 55 MB in all, none of it in the L2 cache before: 14.0 us (3.9 TB/s; the copy's rate would
-// give 8.3), of 5 beams in 32 caches of 20 heads of 64, 11 MB: 6, of which a launch and three reads that wait for one another are more than half.
+// 16 searches of 4 beams in 16 caches of 8 heads of 128, 55 MB in all, none of it in the L2 cache before: 16.0 us (3.4 TB/s; the copy's rate would
+// give 8.3), of 5 beams in 32 caches of 20 heads of 64, 11 MB: 7.6 (6.0 with all of it there), of which a launch and three reads one after another
+// are more than half: lengths, parents (which do not hang on lengths; the check of these stands between) and pages.
 // A block takes a head of a cache's keys or values at a time, whatever is filled of the page, and goes on to another where there are more than 32
-// blocks an SM.  With what is moved in the L2 cache already: 11.6 us so, 12.3 with 16 blocks an SM and 13.6 with 12; by 256 vectors over all
-// heads, which costs three divisions a vector, 13.4; with a block for each 256 vectors of full pages 18.2.
+// blocks an SM: with 16 blocks 17.2 us, with 12 19.0; with what is moved in the L2 cache already 10.2, 10.9 and 12.5.  By 256 vectors over all
+// heads, which costs three divisions a vector, 15.3 where this took 14.0; with a block for each 256 vectors of full pages 18.2 where that took 13.4.
 #include "cache8.cuh"
 
 namespace b200 {
@@ -46,7 +47,7 @@ __device__ __forceinline__ int cr_parent(const ReorderParams& p, int64_t search,
 }
 
 template <int K>     // beams of a search at most
-__global__ void __launch_bounds__(CR_THREADS, K <= 4 ? 12 : 1)        // 40 registers for 52: 15.3 us -> 14.0
+__global__ void __launch_bounds__(CR_THREADS, K <= 4 ? 12 : 1)        // 40 registers for 52: 16.5 us -> 16.0
 cache_reorder_kernel(const __grid_constant__ ReorderParams p) {
     __shared__ int parent[CR_BEAMS];
     __shared__ int64_t page[CR_BEAMS], source[CR_BEAMS];          // that a beam writes, or -1; that it copies from, or -1

@@ -5,11 +5,11 @@
 // Bandwidth-bound: two bytes read and two written an element.  A warp takes one token and some or all of its heads.  It computes the
 // token's cosines and sines once, a pair a lane, and hands them round through shared memory of its own; then a group of lanes takes a head,
 // 16 elements a lane, so that both halves of a pair lie in one lane and the sum of squares is a few shuffles.  Nothing waits for another
-// warp.  40 heads of 128 of 2 x 8192 tokens, 294 MB there and back: 55 us (5.35 TB/s; the copy's rate would give 45), 24 of 96 of 7 x 611, 31 MB:
-// 8.4, 40 of 64 of 8 tokens: 3.9, a launch.  What is under way at once bounds the large ones: 72 registers a lane leave 28 warps an SM.  With the
-// turns in registers too, read once a token and not once a head, there are 24 (58.5 us); arithmetic on one element at a time and not on
-// two, which takes more of them and more instructions, 55.2 and 8.8; one head of a group at a time 61.8 and 9.4, four 67 and 11.7; fewer
-// registers by force spill (61 to 69).
+// warp.  With nothing of it in the L2 cache 40 heads of 128 of 2 x 8192 tokens, 294 MB there and back: 52 us (5.65 TB/s; the copy's rate would give 45),
+// 24 of 96 of 7 x 611, 31 MB: 11.3 (9.0 with all of it there), 40 of 64 of 8 tokens: 3.8, a launch.  What is under way at once bounds the large
+// ones: 72 registers a lane leave 28 warps an SM.  One head of a group at a time 59.6 and 12.1, four 59.6 and 14.7.  With the turns in registers
+// too, read once a token and not once a head, there are 24 warps (58.5 us for 55 in the same runs); arithmetic on one element at a time and
+// not on two takes more registers and instructions (55.2 for 55); fewer registers by force spill (61 to 69).
 #include <cuda_fp16.h>
 
 #include "internal.h"
@@ -259,7 +259,7 @@ int b200_norm_rotary_f16(b200_ctx* ctx, int64_t E, int64_t L, int64_t H, int64_t
     int G = 1;
     while (vec && G * 16 < E) G *= 2;
     // Heads of a warp: all of a token's, halved while there are fewer than 16 warps an SM and each still has a head for every group.  Each warp
-    // computes its token's turns: with up to 128 warps an SM 2 x 8192 tokens take 63 us for 58, 7 x 611 15.7 for 8.3.
+    // computes its token's turns: with up to 128 warps an SM 2 x 8192 tokens take 56.5 us for 52, 7 x 611 17.7 for 11.3.
     const int64_t tokens = L * B, sms = ctx->prop.multiProcessorCount, least = vec ? 32 / G : 1;
     int64_t heads = H;
     while (heads > least && tokens * cdiv(H, heads) < 16 * sms) heads = cdiv(heads, 2 * least) * least;
