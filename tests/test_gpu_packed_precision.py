@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+import juliavision_b200 as jv
 from tests import decode_ref as ref
-from tests.test_gpu_decode import F32, STEP, near
+from tests.test_gpu_decode import F32, STEP, ints, near
 from tests.test_gpu_packed_attention import Packed
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +62,31 @@ def test_values_that_are_not_finite(ctx, E, causal):
     p.check(p.run(F32, causal), F32, causal)
     p.k[:] = p.k[:1]              # equal weights: each a number of fp16
     p.check(p.run(F32, causal), F32, causal)
+
+
+@pytest.mark.parametrize("E", [64, 128])
+def test_calls_and_replays_one_after_the_other(ctx, E):
+    """The same bits from every call, however the loads of its tiles land, and from two graphs that share the workspace."""
+    rng = np.random.default_rng(34)
+    p = Packed(ctx, rng, E, 8, 2, rng.integers(1, 1500, 24), np.zeros(24, int))
+    d, ds = p.device(), ints(ctx, p.starts)
+    outs = [ctx.allocate(F32, E, 8, len(p.q)) for _ in range(4)]
+
+    def call(o):
+        ctx.ws.reset()
+        jv.packedsdpa_(ctx, o.permute((0, 2, 1)), *d, ds)
+    for o in outs:
+        call(o)
+    graphs = [ctx.capture(lambda o=o: call(o)) for o in outs[:2]]
+    ctx.synchronize()
+    first = outs[3].to_host()[:p.starts[-1]]
+    for turn in range(4):
+        for o in outs:
+            ctx.fill_bytes(o, 0xFF)
+        for g in graphs:
+            g.replay()
+        for o in outs[2:]:
+            call(o)
+        ctx.synchronize()
+        assert all(np.array_equal(first, o.to_host()[:p.starts[-1]]) for o in outs)
+    bound(p, outs[0].to_host(), True)
